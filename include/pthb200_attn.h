@@ -279,6 +279,126 @@ int32_t pthb200_write_args_bytes(void);
 /* Enqueue the writer on `stream`.  No allocation, no synchronisation. */
 int32_t pthb200_write_kv(const PthB200WriteArgs* args, void* stream);
 
+/* ---- 16-bit paged cache: tables, writer, attention -------------------------------
+ * Layers whose cache is not quantised (and encoders' states) live in the same pages, as
+ * 16-bit cells: k_cache / v_cache are [num_blocks, block_size, num_kv_heads, head_size] views of
+ * one 16-bit type (byte strides given, rows contiguous), addressed by the same block tables and
+ * slots as the int8 cache.  The reference has no counterpart of these calls: its op reads int8
+ * cells alone and takes the tables as given. */
+
+/* Block tables, slots and offsets of a step, from the requests' lengths.  Request r holds
+ * context_lens[r] tokens and gets query_lens[r] new ones; with BS = block_size
+ *   seq_lens[r] = context_lens[r] + query_lens[r];   query_start_loc[r] = sum of query_lens[0..r)
+ *   request r needs the pages ceil(context/BS) .. ceil(seq/BS): page j of them becomes
+ *   block_table[r][j] = the next id of free_blocks, in the order of requests and pages
+ *   token t, the i-th new one of r, has position p = context_lens[r] + i and
+ *   slot block_table[r][p / BS] * BS + p % BS
+ * Tokens at or past query_start_loc[num_reqs] (padding) get slot -1 and position 0; at most
+ * num_tokens tokens are written.  *pages_taken receives the number of pages that were needed: if
+ * it exceeds num_free, the pages past the list are entered as -1 and their tokens get slot -1, as
+ * do tokens past the end of their row of the table.  A negative length counts as 0.  The sums
+ * must stay below 2^31. */
+typedef struct PthB200TablesArgs {
+  int32_t abi_version;  /* PTH_ATTN_ABI_VERSION */
+  int32_t struct_bytes; /* sizeof(PthB200TablesArgs) of the caller */
+  const int32_t* context_lens; /* [num_reqs] */
+  const int32_t* query_lens;   /* [num_reqs] */
+  const int32_t* free_blocks;  /* [num_free] */
+  int32_t* block_table;        /* [num_reqs, num_pages], rows block_table_row_stride elements apart */
+  int64_t block_table_row_stride;
+  int32_t* seq_lens;        /* [num_reqs] */
+  int32_t* query_start_loc; /* [num_reqs + 1] */
+  int64_t* slot_mapping;    /* [num_tokens] */
+  int64_t* positions;       /* [num_tokens] or NULL */
+  int32_t* pages_taken;     /* [1] */
+  int32_t num_reqs;         /* at most 16384 */
+  int32_t num_tokens;
+  int32_t num_free;
+  int32_t num_pages;
+  int32_t block_size;
+} PthB200TablesArgs;
+int32_t pthb200_tables_args_bytes(void);
+int32_t pthb200_page_tables(const PthB200TablesArgs* args, void* stream);
+
+/* Writer: rounds the rows of new tokens to the cache's type and stores them at their slots.
+ * key / value: [num_tokens, num_kv_heads, head_size] of src_dtype (F32, F16 or BF16), rows
+ * contiguous.  A slot outside [0, num_blocks * block_size) skips the token. */
+typedef struct PthB200Kv16WriteArgs {
+  int32_t abi_version;  /* PTH_ATTN_ABI_VERSION */
+  int32_t struct_bytes; /* sizeof(PthB200Kv16WriteArgs) of the caller */
+  const void* key;
+  const void* value;
+  int32_t src_dtype;
+  int32_t cache_dtype; /* F16 or BF16 */
+  int64_t key_stride_token;
+  int64_t key_stride_head;
+  int64_t value_stride_token;
+  int64_t value_stride_head;
+  PthAttnStream k_cache; /* written through */
+  PthAttnStream v_cache;
+  const int64_t* slot_mapping; /* [num_tokens] */
+  int32_t num_blocks;
+  int32_t block_size;
+  int32_t num_kv_heads;
+  int32_t head_size; /* 64, 128 or 256 */
+  int32_t num_tokens;
+} PthB200Kv16WriteArgs;
+int32_t pthb200_kv16_write_args_bytes(void);
+int32_t pthb200_kv16_write(const PthB200Kv16WriteArgs* args, void* stream);
+
+/* Attention over the 16-bit cache.  q, out and the cache have one type (dtype); k_cache and
+ * v_cache have the same strides.  Every query token of request r sees the same keys
+ * [lo, seq_lens[r]), lo = window > 0 ? max(0, seq_lens[r] - window) : 0, all of them at a
+ * window of 0:
+ *   pthb200_kv16_decode  one token per request, the newest of its cache: token r is request r's
+ *                        (num_tokens == num_reqs, query_start_loc NULL);
+ *   pthb200_kv16_cross   the tokens query_start_loc[r] .. query_start_loc[r + 1) of request r over
+ *                        the states of its encoder (window must be 0).  max_query_len bounds them: tokens
+ *                        of a request past it are not computed.
+ * A request without keys gets out = 0 and a log-sum-exp of -inf.  lse (optional) is the natural
+ * logarithm, dense [num_tokens, num_q_heads].  Block ids of visible keys must lie in
+ * [0, num_blocks); memory of slots that no request sees is not read.
+ *
+ * workspace: pthb200_kv16_workspace_bytes of it, 256-byte aligned, zeroed ONCE before its first use; a
+ * call leaves it ready for the next one.  Calls that may overlap need workspaces of their own. */
+typedef struct PthB200Kv16Args {
+  int32_t abi_version;  /* PTH_ATTN_ABI_VERSION */
+  int32_t struct_bytes; /* sizeof(PthB200Kv16Args) of the caller */
+  const void* q;        /* [num_tokens, num_q_heads, head_size] */
+  int64_t q_stride_token;
+  int64_t q_stride_head;
+  void* out;
+  int64_t out_stride_token;
+  int64_t out_stride_head;
+  float* lse; /* [num_tokens, num_q_heads] or NULL */
+  PthAttnStream k_cache;
+  PthAttnStream v_cache;
+  const int32_t* block_table; /* [num_reqs, *] */
+  int64_t block_table_row_stride;
+  const int32_t* seq_lens;        /* [num_reqs] */
+  const int32_t* query_start_loc; /* [num_reqs + 1]; NULL for decode */
+  void* workspace;
+  int64_t workspace_bytes;
+  int32_t dtype; /* F16 or BF16 */
+  int32_t num_blocks;
+  int32_t block_size;
+  int32_t num_kv_heads;
+  int32_t num_q_heads; /* at most 64 per KV head */
+  int32_t head_size; /* 64, 128 or 256 */
+  int32_t num_reqs;
+  int32_t num_tokens;
+  int32_t max_query_len;
+  int32_t window;
+  float softmax_scale;
+} PthB200Kv16Args;
+int32_t pthb200_kv16_args_bytes(void);
+/* Workspace of any call of this head size on a device of num_sms SMs. */
+int64_t pthb200_kv16_workspace_bytes(int32_t head_size, int32_t num_sms);
+int32_t pthb200_kv16_decode(const PthB200Kv16Args* args, void* stream);
+int32_t pthb200_kv16_cross(const PthB200Kv16Args* args, void* stream);
+/* Validates as the calls above do, without launching (cross: query_start_loc is not NULL). */
+int32_t pthb200_kv16_check(const PthB200Kv16Args* args);
+
 /* Host-only helpers of the op layer (no device access).
  * pthb200_tile_tokens: query tokens per row tile for a launch planned with `wm`
  * (1, 2 or 4), group size G and host bound max_query_len; returns -1 if wm is

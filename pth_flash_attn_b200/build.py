@@ -20,7 +20,9 @@ LIB = HERE / "libpthb200_attn.so"
 OP_LIB = HERE / "_C.abi3.so"
 
 CUDA_SOURCES = ["launcher.cu", "scalar_kernel.cu", "combine_kernel.cu", "umma_kernel.cu", "umma_i8_kernel.cu",
-                "umma_rows_kernel.cu", "umma_rows256_kernel.cu", "umma_rows2_kernel.cu", "writer_kernel.cu", "copy_ceiling_kernel.cu"]
+                "umma_rows_kernel.cu", "umma_rows256_kernel.cu", "umma_rows2_kernel.cu", "writer_kernel.cu", "copy_ceiling_kernel.cu",
+                "kv16_api.cu", "page_tables_kernel.cu", "kv16_writer_kernel.cu", "kv16_simple_kernel.cu"]
+OP_SOURCES = ["torch_op.cpp", "torch_kv16.cpp"]
 NVCC_FLAGS = [
     "-std=c++17", "-O3", "-lineinfo", "-gencode", "arch=compute_100a,code=sm_100a",
     "-Xcompiler", "-fPIC", "-Xcompiler", "-fno-gnu-unique", "-rdc=false",
@@ -60,14 +62,14 @@ def build_op_library(force: bool = False) -> Path:
     import torch
     from torch.utils import cpp_extension
 
-    src = CSRC / "torch_op.cpp"
-    if not force and _newer(OP_LIB, [src, LIB]):
+    sources = [CSRC / s for s in OP_SOURCES]
+    if not force and _newer(OP_LIB, [*sources, LIB]):
         return OP_LIB
     includes = [f"-I{p}" for p in cpp_extension.include_paths()]
     cuda_inc = Path(os.environ.get("CUDA_HOME", "/usr/local/cuda")) / "include"
     torch_lib = Path(torch.__file__).parent / "lib"
     cmd = [
-        "g++", "-std=c++17", "-O2", "-fPIC", "-shared", "-fno-gnu-unique", str(src), "-o", str(OP_LIB),
+        "g++", "-std=c++17", "-O2", "-fPIC", "-shared", "-fno-gnu-unique", *map(str, sources), "-o", str(OP_LIB),
         *includes, f"-I{cuda_inc}", f"-L{HERE}", "-lpthb200_attn", "-Wl,-rpath,$ORIGIN",
         f"-L{torch_lib}", "-ltorch", "-ltorch_cpu", "-lc10", f"-Wl,-rpath,{torch_lib}",
     ]

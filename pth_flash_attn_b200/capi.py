@@ -126,6 +126,84 @@ class PthB200WriteArgs(ctypes.Structure):
     ]
 
 
+class PthB200TablesArgs(ctypes.Structure):
+    _fields_ = [
+        ("abi_version", ctypes.c_int32),
+        ("struct_bytes", ctypes.c_int32),
+        ("context_lens", ctypes.c_void_p),
+        ("query_lens", ctypes.c_void_p),
+        ("free_blocks", ctypes.c_void_p),
+        ("block_table", ctypes.c_void_p),
+        ("block_table_row_stride", ctypes.c_int64),
+        ("seq_lens", ctypes.c_void_p),
+        ("query_start_loc", ctypes.c_void_p),
+        ("slot_mapping", ctypes.c_void_p),
+        ("positions", ctypes.c_void_p),
+        ("pages_taken", ctypes.c_void_p),
+        ("num_reqs", ctypes.c_int32),
+        ("num_tokens", ctypes.c_int32),
+        ("num_free", ctypes.c_int32),
+        ("num_pages", ctypes.c_int32),
+        ("block_size", ctypes.c_int32),
+    ]
+
+
+class PthB200Kv16WriteArgs(ctypes.Structure):
+    _fields_ = [
+        ("abi_version", ctypes.c_int32),
+        ("struct_bytes", ctypes.c_int32),
+        ("key", ctypes.c_void_p),
+        ("value", ctypes.c_void_p),
+        ("src_dtype", ctypes.c_int32),
+        ("cache_dtype", ctypes.c_int32),
+        ("key_stride_token", ctypes.c_int64),
+        ("key_stride_head", ctypes.c_int64),
+        ("value_stride_token", ctypes.c_int64),
+        ("value_stride_head", ctypes.c_int64),
+        ("k_cache", PthAttnStream),
+        ("v_cache", PthAttnStream),
+        ("slot_mapping", ctypes.c_void_p),
+        ("num_blocks", ctypes.c_int32),
+        ("block_size", ctypes.c_int32),
+        ("num_kv_heads", ctypes.c_int32),
+        ("head_size", ctypes.c_int32),
+        ("num_tokens", ctypes.c_int32),
+    ]
+
+
+class PthB200Kv16Args(ctypes.Structure):
+    _fields_ = [
+        ("abi_version", ctypes.c_int32),
+        ("struct_bytes", ctypes.c_int32),
+        ("q", ctypes.c_void_p),
+        ("q_stride_token", ctypes.c_int64),
+        ("q_stride_head", ctypes.c_int64),
+        ("out", ctypes.c_void_p),
+        ("out_stride_token", ctypes.c_int64),
+        ("out_stride_head", ctypes.c_int64),
+        ("lse", ctypes.c_void_p),
+        ("k_cache", PthAttnStream),
+        ("v_cache", PthAttnStream),
+        ("block_table", ctypes.c_void_p),
+        ("block_table_row_stride", ctypes.c_int64),
+        ("seq_lens", ctypes.c_void_p),
+        ("query_start_loc", ctypes.c_void_p),
+        ("workspace", ctypes.c_void_p),
+        ("workspace_bytes", ctypes.c_int64),
+        ("dtype", ctypes.c_int32),
+        ("num_blocks", ctypes.c_int32),
+        ("block_size", ctypes.c_int32),
+        ("num_kv_heads", ctypes.c_int32),
+        ("num_q_heads", ctypes.c_int32),
+        ("head_size", ctypes.c_int32),
+        ("num_reqs", ctypes.c_int32),
+        ("num_tokens", ctypes.c_int32),
+        ("max_query_len", ctypes.c_int32),
+        ("window", ctypes.c_int32),
+        ("softmax_scale", ctypes.c_float),
+    ]
+
+
 class PthB200Options(ctypes.Structure):
     _fields_ = [
         ("abi_version", ctypes.c_int32),
@@ -154,6 +232,15 @@ EXPORTED_SYMBOLS = (
     "pthb200_copy_ceiling",
     "pthb200_write_args_bytes",
     "pthb200_write_kv",
+    "pthb200_tables_args_bytes",
+    "pthb200_page_tables",
+    "pthb200_kv16_write_args_bytes",
+    "pthb200_kv16_write",
+    "pthb200_kv16_args_bytes",
+    "pthb200_kv16_workspace_bytes",
+    "pthb200_kv16_decode",
+    "pthb200_kv16_cross",
+    "pthb200_kv16_check",
     "pthb200_tile_tokens",
     "pthb200_check_call",
     "pthb200_launch_count",
@@ -216,6 +303,17 @@ class B200Lib:
         lib.pthb200_write_args_bytes.argtypes = []
         lib.pthb200_write_kv.restype = ctypes.c_int32
         lib.pthb200_write_kv.argtypes = [ctypes.POINTER(PthB200WriteArgs), ctypes.c_void_p]
+        for name in ("pthb200_tables_args_bytes", "pthb200_kv16_write_args_bytes", "pthb200_kv16_args_bytes"):
+            getattr(lib, name).restype = ctypes.c_int32
+            getattr(lib, name).argtypes = []
+        lib.pthb200_kv16_workspace_bytes.restype = ctypes.c_int64
+        lib.pthb200_kv16_workspace_bytes.argtypes = [ctypes.c_int32] * 2
+        for name, args in (("pthb200_page_tables", PthB200TablesArgs), ("pthb200_kv16_write", PthB200Kv16WriteArgs),
+                           ("pthb200_kv16_decode", PthB200Kv16Args), ("pthb200_kv16_cross", PthB200Kv16Args)):
+            getattr(lib, name).restype = ctypes.c_int32
+            getattr(lib, name).argtypes = [ctypes.POINTER(args), ctypes.c_void_p]
+        lib.pthb200_kv16_check.restype = ctypes.c_int32
+        lib.pthb200_kv16_check.argtypes = [ctypes.POINTER(PthB200Kv16Args)]
         for fn in (lib.pthb200_test_schedule, lib.pthb200_test_range_schedule):
             fn.restype = ctypes.c_int32
             fn.argtypes = [ctypes.c_void_p] * 2 + [ctypes.c_int32] * 10 + [ctypes.c_void_p, ctypes.c_int32]
@@ -239,6 +337,11 @@ class B200Lib:
             raise RuntimeError(f"{path}: PthAttnCombineArgs size differs from the ctypes mirror")
         if lib.pthb200_write_args_bytes() != ctypes.sizeof(PthB200WriteArgs):
             raise RuntimeError(f"{path}: PthB200WriteArgs size differs from the ctypes mirror")
+        for args, size in ((PthB200TablesArgs, lib.pthb200_tables_args_bytes()),
+                           (PthB200Kv16WriteArgs, lib.pthb200_kv16_write_args_bytes()),
+                           (PthB200Kv16Args, lib.pthb200_kv16_args_bytes())):
+            if size != ctypes.sizeof(args):
+                raise RuntimeError(f"{path}: {args.__name__} size differs from the ctypes mirror")
         if lib.pthb200_options_bytes() != ctypes.sizeof(PthB200Options):
             raise RuntimeError(f"{path}: PthB200Options size differs from the ctypes mirror")
 
@@ -273,6 +376,29 @@ class B200Lib:
     def write_kv(self, args: "PthB200WriteArgs", *, stream: int = 0) -> int:
         """Quantise and store the K / V rows of new tokens (the cache writer)."""
         return int(self.lib.pthb200_write_kv(ctypes.byref(args), stream or None))
+
+    def page_tables(self, args: PthB200TablesArgs, *, stream: int = 0) -> int:
+        """Block table, slots, positions and offsets of a step from its requests' lengths."""
+        return int(self.lib.pthb200_page_tables(ctypes.byref(args), stream or None))
+
+    def kv16_write(self, args: PthB200Kv16WriteArgs, *, stream: int = 0) -> int:
+        """Store the K / V rows of new tokens in the 16-bit cache."""
+        return int(self.lib.pthb200_kv16_write(ctypes.byref(args), stream or None))
+
+    def kv16_decode(self, args: PthB200Kv16Args, *, stream: int = 0) -> int:
+        """Attention of one token per request over the 16-bit cache."""
+        return int(self.lib.pthb200_kv16_decode(ctypes.byref(args), stream or None))
+
+    def kv16_cross(self, args: PthB200Kv16Args, *, stream: int = 0) -> int:
+        """Attention of every request's tokens over its encoder's states in the 16-bit cache."""
+        return int(self.lib.pthb200_kv16_cross(ctypes.byref(args), stream or None))
+
+    def kv16_check(self, args: PthB200Kv16Args) -> int:
+        """The checks of the two calls above, without a launch."""
+        return int(self.lib.pthb200_kv16_check(ctypes.byref(args)))
+
+    def kv16_workspace_bytes(self, head_size: int, num_sms: int) -> int:
+        return int(self.lib.pthb200_kv16_workspace_bytes(head_size, num_sms))
 
     def tile_tokens(self, wm: int, group: int, max_query_len: int) -> int:
         return int(self.lib.pthb200_tile_tokens(wm, group, max_query_len))
@@ -360,6 +486,14 @@ def new_write_args() -> PthB200WriteArgs:
     a = PthB200WriteArgs()
     a.abi_version = ABI_VERSION
     a.struct_bytes = ctypes.sizeof(PthB200WriteArgs)
+    return a
+
+
+def new_args(kind):
+    """A zeroed argument block of one of the structures above, with its version and size."""
+    a = kind()
+    a.abi_version = ABI_VERSION
+    a.struct_bytes = ctypes.sizeof(kind)
     return a
 
 

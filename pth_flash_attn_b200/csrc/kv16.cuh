@@ -1,0 +1,56 @@
+// Parameters shared by the kernels of the 16-bit paged cache (include/pthb200_attn.h: pthb200_page_tables,
+// pthb200_kv16_*), and their host-side launchers.
+#pragma once
+
+#include <string>
+
+#include "params.cuh"
+
+namespace pthb200 {
+
+struct Kv16Params {
+  const uint8_t* q;
+  int64_t q_stride_token, q_stride_head;
+  uint8_t* out;
+  int64_t out_stride_token, out_stride_head;
+  float* lse;  // [num_tokens, num_q_heads] or nullptr
+  const uint8_t* k;
+  const uint8_t* v;
+  int64_t stride_block, stride_slot, stride_head;  // of both
+  const int32_t* block_table;
+  int64_t block_table_row_stride;
+  const int32_t* seq_lens;
+  const int32_t* query_start_loc;  // nullptr: token r is request r's only one
+  uint8_t* workspace;
+  int32_t dtype;
+  int32_t block_size, block_shift;  // block_shift: log2(block_size), -1 if it is not a power of two
+  int32_t num_kv_heads, num_q_heads, group, head_size;
+  int32_t num_reqs, num_tokens, max_query_len, window;
+  float scale_log2;  // softmax_scale * log2(e)
+};
+
+// The query tokens of a request (none past the caller's bound or the end of the token arrays), and its visible keys.
+__device__ __forceinline__ int kv16_tokens(const Kv16Params& p, int r, int* first) {
+  if (p.query_start_loc == nullptr) {
+    *first = r;
+    return 1;
+  }
+  *first = __ldg(p.query_start_loc + r);
+  const int end = min(__ldg(p.query_start_loc + r + 1), p.num_tokens);
+  return max(0, min(end - *first, p.max_query_len));
+}
+__device__ __forceinline__ void kv16_visible(const Kv16Params& p, int r, int* lo, int* hi) {
+  *hi = max(0, __ldg(p.seq_lens + r));
+  *lo = p.window > 0 ? max(0, *hi - p.window) : 0;
+}
+
+// launcher.cu: the calling thread's error text.
+int32_t clear_error();
+int32_t set_error(int32_t code, const std::string& msg);
+
+int64_t kv16_workspace_bytes(int head_size, int num_sms);
+cudaError_t launch_kv16_attention(const Kv16Params& p, cudaStream_t stream);
+cudaError_t launch_kv16_writer(const PthB200Kv16WriteArgs& a, cudaStream_t stream);
+cudaError_t launch_page_tables(const PthB200TablesArgs& a, cudaStream_t stream);
+
+}  // namespace pthb200

@@ -26,6 +26,16 @@ int32_t fail(int32_t code, const std::string& msg) {
     if (!(cond)) return fail(PTH_ATTN_EINVAL, (msg)); \
   } while (0)
 
+}  // namespace
+
+int32_t clear_error() {
+  g_last_error.clear();
+  return PTH_ATTN_OK;
+}
+int32_t set_error(int32_t code, const std::string& msg) { return fail(code, msg); }
+
+namespace {
+
 bool aligned(const void* ptr, int64_t a) { return reinterpret_cast<uintptr_t>(ptr) % (uintptr_t)a == 0; }
 
 bool is_head_size(int32_t d) { return d == 64 || d == 128 || d == 256; }

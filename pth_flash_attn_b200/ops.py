@@ -11,6 +11,9 @@ metadata checks of the C++ op in the same order with the same messages, so a bad
 call fails at trace time with the reason it would fail with at run time.  Checks
 that need addresses or a device stay in C++.
 
+The ops of the 16-bit paged cache (:mod:`.kv16`) come from the same library and are
+reached from here too.
+
 This module makes no ``torch.cuda`` call.
 """
 
@@ -20,6 +23,9 @@ import math
 from pathlib import Path
 
 import torch
+
+from . import kv16
+from .kv16 import kv16_cross_attention, kv16_decode_attention, kv16_write, page_tables  # noqa: F401
 
 OP_NAMESPACE = "pth_flash_attn"
 OP_NAME = "pth_flash_attn_fwd"
@@ -216,6 +222,7 @@ def _load_library() -> bool:
     torch.ops.load_library(str(LIBRARY_PATH))
     torch.library.register_fake(OP_QUALNAME)(pth_flash_attn_fwd_fake)
     torch.library.register_fake(LSE_OP_QUALNAME)(pth_flash_attn_fwd_lse_fake)
+    kv16.register()
     return True
 
 
