@@ -5,6 +5,7 @@
 #include <string>
 
 #include "params.cuh"
+#include "tcgen05.cuh"
 
 namespace pthb200 {
 
@@ -42,6 +43,29 @@ __device__ __forceinline__ int kv16_tokens(const Kv16Params& p, int r, int* firs
 __device__ __forceinline__ void kv16_visible(const Kv16Params& p, int r, int* lo, int* hi) {
   *hi = max(0, __ldg(p.seq_lens + r));
   *lo = p.window > 0 ? max(0, *hi - p.window) : 0;
+}
+
+// ---- shared memory images and waits of the tensor-core kernels ----
+
+// Shared-memory operand descriptor, rows of 128 bytes in the 128-byte swizzle (chunk c of 16 bytes of row r lies at
+// chunk c ^ (r & 7)): groups of 8 rows are 1,024 bytes.  K-major: sbo = next 8 rows.  MN-major (the row is a K index and
+// holds 64 elements of M / N): sbo = next 8 rows, lbo = next 64 elements.
+__device__ __forceinline__ uint64_t swizzled_desc(uint32_t saddr, uint32_t lbo_bytes, uint32_t sbo_bytes) {
+  return tc::smem_desc(saddr, lbo_bytes, sbo_bytes) | (uint64_t)2 << 61;
+}
+// Asynchronous copy of 16 bytes, or of none: then the destination is zeroed.
+__device__ __forceinline__ void copy16(uint32_t dst, const uint8_t* src, bool live) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(live ? 16 : 0) : "memory");
+}
+// One arrival on the barrier when this thread's copies so far have landed (it counts like any other arrival).
+__device__ __forceinline__ void copies_arrive(uint64_t* bar) {
+  asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(tc::smem_u32(bar)) : "memory");
+}
+__device__ __forceinline__ void copies_wait_all() { asm volatile("cp.async.wait_all;" ::: "memory"); }
+__device__ __forceinline__ float kv16_exp2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
 }
 
 // launcher.cu: the calling thread's error text.

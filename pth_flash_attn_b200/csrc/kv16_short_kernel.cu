@@ -1,0 +1,771 @@
+// Attention over the 16-bit paged cache for requests of few query rows (a row is a query token and head): one-token decode,
+// cross attention of a few tokens.
+//
+// Orientation: the 128 keys of a tile sit on the MMA's M dimension, the rows of a KV head on N, so tensor work goes
+// into keys and not into padding:
+//   S^T[key, row] = sum_d K[key, d] Q[row, d]         A = K as it lies in the cache (K-major), B = Q
+//   O^T[d, row]  += sum_key V[key, d] P[key, row]     A = V as it lies in the cache (MN-major), B = P
+// Both operands A are the cache's own bytes: no element of K or V passes through a register.
+//
+// Softmax in one pass: ref is a running bound of a row's scores (log2 units), P = 2^(s - ref), l = sum P.  ref is a row's
+// maximum less kGain when it is set, and moves (with l and O rescaled) only when a score outgrows it by kSlack, so that most
+// tiles need no maximum at all, only a vote of the 128 threads.  P goes into the MMA as the sum of two 16-bit
+// numbers (hi + lo: 2 x 8 or 2 x 11 bits), side by side on N: at the instruction's minimum of 16 columns that costs
+// eight rows nothing, and the outputs' error is their own rounding (with one: 1.4 times it).  kGain keeps fp16's lo above its smallest
+// numbers; 2^(kGain + kSlack) is below its largest.
+//
+// What bounds it: the cache's bytes, 4 D per key and KV head at 4 D G flops.  The tile's parts (128 keys x 128 dims of K, of
+// V) are units of one ring of shared memory, K of the next tile ahead of V of this one, which is the order in which they are
+// used; four warps fill it with 16-byte copies that go to their swizzled place, zero where a key is not visible (so what lies
+// there in memory, NaN included, is never read).  Two CTAs per SM keep 192 KB in flight.  Copies of pages instead (tiled
+// TMA, boxes of 16 slots x 64 dims, 64 requests x 8,192 keys x 8 heads x 128 dims) moved 6.83 TB/s, with boxes of 4 KB 7.06, 16-byte
+// copies 7.17, which also take pages of any size and place.
+//
+// Schedule: the KV tiles of all (request, row tile) form one sequence, which is cut into equal runs, one for every group of Hkv
+// CTAs; CTA h of a group reads head h, so the heads of a page are read at the same time.  A request that a cut divides
+// leaves partial (O, ref, l) of its pieces in the workspace, and the CTA that arrives last merges them in the pieces' order:
+// one launch, and the same bits whoever is last.
+#include "kv16.cuh"
+#include "page_copy.cuh"
+#include "pdl.cuh"
+
+namespace pthb200 {
+
+__device__ unsigned int g_kv16_status = 0;
+
+namespace {
+
+constexpr int kTile = 128;             // keys
+constexpr int kSoftmaxThreads = 128;   // warps 0-3: thread t is key t of a tile, then dim t of the output
+constexpr int kLoadWarp = 4;           // warps 4-7
+constexpr int kMmaWarp = 8;
+constexpr int kThreads = 288;
+constexpr int kCounterBytes = 4096;    // arrival counters at the start of the workspace, one per CTA
+constexpr float kGain = 7.f, kSlack = 8.f;
+constexpr int kRunMin = 1;             // KV tiles a run holds at least
+
+template <int HD, int RP>
+struct Geo {
+  static constexpr int dims = HD < 128 ? HD : 128;   // of a unit
+  static constexpr int parts = HD / dims;            // units of a tile's K, and of its V
+  static constexpr int unit = kTile * dims * 2;
+  static constexpr int cols = RP < 16 ? 16 : RP;     // N of QK (its rows past RP repeat the first)
+  static constexpr int qimage = RP * HD * 2;
+  static constexpr int pimage = 2 * RP * kTile * 2;
+  static constexpr int fixed = 2 * qimage + pimage + 4 * RP * 4 * 2 + 512;
+  // Two CTAs per SM where three units fit, else one.
+  static constexpr int units2 = (115712 - fixed - 1024) / unit;
+  static constexpr int ctas = units2 >= 3 && RP <= 16 ? 2 : 1;
+  static constexpr int most = 98304 * (3 - ctas) / unit;
+  static constexpr int fit = ctas == 2 ? units2 : (232448 - fixed - 1024) / unit;
+  static constexpr int units = fit < most ? fit : most;
+  static_assert(units >= 3, "K and V of a tile, and the next K");
+  static constexpr int s_col = 0, o_col = 2 * cols;  // TMEM columns: S twice, O of every part (hi, lo)
+  static constexpr int tmem_need = 2 * cols + parts * 2 * RP;
+  static constexpr int tmem = tmem_need <= 64 ? 64 : tmem_need <= 128 ? 128 : 256;
+  static_assert(tmem_need <= 256, "two CTAs share the SM's columns");
+  // shared memory, behind the first 1,024-byte boundary
+  static constexpr int q = units * unit;
+  static constexpr int p = q + 2 * qimage;
+  static constexpr int wmax = p + pimage;            // float [4 warps][RP]
+  static constexpr int wsum = wmax + 4 * RP * 4;     // float [4 warps][RP]
+  static constexpr int bars = wsum + 4 * RP * 4;
+  static constexpr int n_bars = 2 * units + 2 + 2 + 1 + 1;
+  static constexpr int misc = bars + n_bars * 8;     // ints: abort flag, TMEM address, first request, last arrival; 64-bit scan
+  static constexpr int total = misc + 160 + 1024;
+  static_assert(n_bars * 8 + 160 <= 512, "fixed part");
+};
+
+struct Bars {  // offsets behind [units] full, [units] empty
+  static constexpr int q_empty = 0, s_ready = 2, p_ready = 4, pv_done = 5;
+};
+
+// One piece of a request's row tile: keys [key0, key0 + 128 tiles) of those visible, [lo, hi).
+struct Piece {
+  int r, row0, rows;          // rows row0 .. row0 + rows of the request's q_len x G
+  int first_token;
+  int key0, tiles, lo, hi;
+  bool begins, ends;
+  long long start;            // of the row tile in the sequence
+  int row_tiles_keys;         // KV tiles of the whole row tile
+};
+
+template <int RP>
+struct Walk {
+  long long at, end, start;   // position in the sequence, end of the run, start of request r
+  int r;
+};
+
+struct ReqShape {
+  int tokens, first, lo, hi, tiles, row_tiles;
+};
+template <int RP>
+__device__ __forceinline__ ReqShape req_shape(const Kv16Params& p, int r) {
+  ReqShape s;
+  kv16_visible(p, r, &s.lo, &s.hi);
+  s.tokens = kv16_tokens(p, r, &s.first);
+  const int rows = s.tokens * p.group;
+  s.row_tiles = (rows + RP - 1) / RP;
+  s.tiles = s.hi > s.lo && rows > 0 ? (s.hi + kTile - 1) / kTile - s.lo / kTile : 0;
+  return s;
+}
+template <int RP>
+__device__ __forceinline__ bool next_piece(const Kv16Params& p, Walk<RP>& w, Piece* out) {
+  if (w.at >= w.end) return false;
+  ReqShape s = req_shape<RP>(p, w.r);
+  long long n = (long long)s.tiles * s.row_tiles;
+  while (w.at >= w.start + n) {
+    w.start += n;
+    ++w.r;
+    s = req_shape<RP>(p, w.r);
+    n = (long long)s.tiles * s.row_tiles;
+  }
+  const long long off = w.at - w.start;
+  const int rt = s.row_tiles == 1 ? 0 : (int)(off / s.tiles);
+  const int tile = (int)(off - (long long)rt * s.tiles);
+  out->r = w.r;
+  out->row0 = rt * RP;
+  out->rows = min(RP, s.tokens * p.group - rt * RP);
+  out->first_token = s.first;
+  out->lo = s.lo;
+  out->hi = s.hi;
+  out->key0 = (s.lo / kTile + tile) * kTile;
+  out->tiles = (int)min((long long)(s.tiles - tile), w.end - w.at);
+  out->begins = tile == 0;
+  out->ends = tile + out->tiles == s.tiles;
+  out->start = w.start + (long long)rt * s.tiles;
+  out->row_tiles_keys = s.tiles;
+  w.at += out->tiles;
+  return true;
+}
+// Token and query head of a row of a request.
+__device__ __forceinline__ void row_of(const Kv16Params& p, int first_token, int kvh, int row, int* token, int* head) {
+  const int t = p.query_start_loc == nullptr ? 0 : (int)((uint32_t)row / (uint32_t)p.group);
+  *token = first_token + t;
+  *head = kvh * p.group + row - t * p.group;
+}
+
+__device__ __forceinline__ float redux_max(float x) {
+  float y;
+  asm volatile("redux.sync.max.f32 %0, %1, 0xffffffff;" : "=f"(y) : "f"(x));
+  return y;
+}
+// Barrier of the softmax warps that tells whether any of them has seen `x`.
+__device__ __forceinline__ bool softmax_any(bool x) {
+  uint32_t r;
+  asm volatile(
+      "{\n\t"
+      ".reg .pred p, q;\n\t"
+      "setp.ne.u32 p, %1, 0;\n\t"
+      "barrier.cta.red.or.pred q, 1, 128, p;\n\t"
+      "selp.u32 %0, 1, 0, q;\n\t"
+      "}\n"
+      : "=r"(r)
+      : "r"((uint32_t)x)
+      : "memory");
+  return r != 0;
+}
+__device__ __forceinline__ void softmax_sync() { named_barrier(1, kSoftmaxThreads); }
+
+template <int N>
+__device__ __forceinline__ void tmem_load(uint32_t addr, uint32_t* r) {
+  if constexpr (N == 8) {
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7])
+                 : "r"(addr)
+                 : "memory");
+  } else {
+#pragma unroll
+    for (int i = 0; i < N; i += 16) tc::tmem_ld16(addr + i, r + i);
+  }
+}
+template <int N>
+__device__ __forceinline__ void tmem_store(uint32_t addr, const uint32_t* r) {
+  static_assert(N % 16 == 0, "columns");
+#pragma unroll
+  for (int i = 0; i < N; i += 16) tc::tmem_st16(addr + i, r + i);
+}
+
+// Two numbers as 16-bit parts: hi is their rounding, lo the rounding of what is left.
+template <bool kHalf>
+__device__ __forceinline__ void split2(float a, float b, uint32_t* hi, uint32_t* lo) {
+  if constexpr (kHalf) {
+    const __half2 h = __floats2half2_rn(a, b);
+    const float2 f = __half22float2(h);
+    const __half2 l = __floats2half2_rn(a - f.x, b - f.y);
+    *hi = *reinterpret_cast<const uint32_t*>(&h);
+    *lo = *reinterpret_cast<const uint32_t*>(&l);
+  } else {
+    const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
+    const uint32_t w = *reinterpret_cast<const uint32_t*>(&h);
+    const __nv_bfloat162 l = __floats2bfloat162_rn(a - __uint_as_float(w << 16), b - __uint_as_float(w & 0xffff0000u));
+    *hi = w;
+    *lo = *reinterpret_cast<const uint32_t*>(&l);
+  }
+}
+
+template <int HD, int RP>
+__device__ __forceinline__ float* partial_slot(const Kv16Params& p, int cta, bool begins) {
+  float* base = reinterpret_cast<float*>(p.workspace + kCounterBytes);
+  return base + (int64_t)(2 * cta + (begins ? 1 : 0)) * (RP * (HD + 2));  // [RP][HD] O, [RP] ref, [RP] l
+}
+
+// Merges the pieces of a row tile, left by the CTAs of groups g0 .. g0 + pieces - 1, and writes its rows.
+template <int HD, int RP>
+__device__ __forceinline__ void merge_pieces(const Kv16Params& p, const Piece& it, int kvh, int g0, int pieces, int heads, int hslot) {
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  constexpr int kVec = HD >= 128 ? HD / 128 : 1;
+  for (int n = warp; n < it.rows; n += 4) {
+    auto slot = [&](int k) { return partial_slot<HD, RP>(p, (g0 + k) * heads + hslot, k == 0); };
+    float top = -INFINITY;
+    for (int k = lane; k < pieces; k += 32) top = fmaxf(top, __ldcg(slot(k) + RP * HD + n));
+    top = redux_max(top);
+    const float use = top == -INFINITY ? 0.f : top;
+    float l = 0.f;
+    for (int k = lane; k < pieces; k += 32) {
+      const float* s = slot(k) + RP * HD + n;
+      l = fmaf(kv16_exp2(__ldcg(s) - use), __ldcg(s + RP), l);
+    }
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) l += __shfl_xor_sync(0xffffffffu, l, o);
+    float acc[kVec][4];
+#pragma unroll
+    for (int v = 0; v < kVec; ++v) acc[v][0] = acc[v][1] = acc[v][2] = acc[v][3] = 0.f;
+    const int d0 = (HD == 64 ? lane & 15 : lane) * 4;
+    constexpr int kBatch = 8;
+    for (int k0 = 0; k0 < pieces; k0 += kBatch) {
+      float4 o[kBatch][kVec];
+      float w[kBatch];
+#pragma unroll
+      for (int b = 0; b < kBatch; ++b) {
+        const float* s = slot(min(k0 + b, pieces - 1));
+        w[b] = __ldcg(s + RP * HD + n);
+#pragma unroll
+        for (int v = 0; v < kVec; ++v) o[b][v] = __ldcg(reinterpret_cast<const float4*>(s + n * HD + v * 128 + d0));
+      }
+#pragma unroll
+      for (int b = 0; b < kBatch; ++b) {
+        const float f = k0 + b < pieces ? kv16_exp2(w[b] - use) : 0.f;
+#pragma unroll
+        for (int v = 0; v < kVec; ++v) {
+          if (k0 + b >= pieces) continue;
+          acc[v][0] = fmaf(f, o[b][v].x, acc[v][0]);
+          acc[v][1] = fmaf(f, o[b][v].y, acc[v][1]);
+          acc[v][2] = fmaf(f, o[b][v].z, acc[v][2]);
+          acc[v][3] = fmaf(f, o[b][v].w, acc[v][3]);
+        }
+      }
+    }
+    const float inv = l == 0.f ? 0.f : 1.f / l;
+    int token, head;
+    row_of(p, it.first_token, kvh, it.row0 + n, &token, &head);
+    uint8_t* out = p.out + (int64_t)token * p.out_stride_token + (int64_t)head * p.out_stride_head;
+#pragma unroll
+    for (int v = 0; v < kVec; ++v) {
+      uint2 w;
+      if (p.dtype == PTH_ATTN_F16) {
+        const __half2 a = __floats2half2_rn(acc[v][0] * inv, acc[v][1] * inv), b = __floats2half2_rn(acc[v][2] * inv, acc[v][3] * inv);
+        w = make_uint2(*reinterpret_cast<const uint32_t*>(&a), *reinterpret_cast<const uint32_t*>(&b));
+      } else {
+        const __nv_bfloat162 a = __floats2bfloat162_rn(acc[v][0] * inv, acc[v][1] * inv), b = __floats2bfloat162_rn(acc[v][2] * inv, acc[v][3] * inv);
+        w = make_uint2(*reinterpret_cast<const uint32_t*>(&a), *reinterpret_cast<const uint32_t*>(&b));
+      }
+      if (HD >= 128 || lane < 16) *reinterpret_cast<uint2*>(out + (v * 128 + d0) * 2) = w;
+    }
+    if (lane == 0 && p.lse != nullptr) p.lse[(int64_t)token * p.num_q_heads + head] = l == 0.f ? -INFINITY : (use + log2f(l)) * kLn2;
+  }
+}
+
+template <int HD, int RP, bool kHalf>
+__global__ void __launch_bounds__(kThreads, (Geo<HD, RP>::ctas)) kv16_short_kernel(const __grid_constant__ Kv16Params p) {
+  using G = Geo<HD, RP>;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* const smem = smem_raw + ((1024u - (tc::smem_u32(smem_raw) & 1023u)) & 1023u);
+  uint64_t* const full = reinterpret_cast<uint64_t*>(smem + G::bars);
+  uint64_t* const empty = full + G::units;
+  uint64_t* const bars = empty + G::units;
+  volatile int* const abort_flag = reinterpret_cast<volatile int*>(smem + G::misc);
+  uint32_t* const tslot = reinterpret_cast<uint32_t*>(smem + G::misc + 4);
+  int* const first_req = reinterpret_cast<int*>(smem + G::misc + 8);
+  int* const arrival = reinterpret_cast<int*>(smem + G::misc + 12);
+  long long* const first_start = reinterpret_cast<long long*>(smem + G::misc + 16);
+  long long* const warp_tiles = reinterpret_cast<long long*>(smem + G::misc + 24);  // [9 warps]
+  static_assert((G::misc + 16) % 8 == 0, "64-bit words");
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+
+  if (warp == kMmaWarp) {
+    if (lane == 0) {
+      for (int i = 0; i < G::units; ++i) {
+        tc::mbar_init(&full[i], 128);
+        tc::mbar_init(&empty[i], 1);
+      }
+      for (int i = 0; i < 2; ++i) {
+        tc::mbar_init(&bars[Bars::q_empty + i], 1);
+        tc::mbar_init(&bars[Bars::s_ready + i], 1);
+      }
+      tc::mbar_init(&bars[Bars::p_ready], kSoftmaxThreads);
+      tc::mbar_init(&bars[Bars::pv_done], 1);
+      *abort_flag = 0;
+      tc::mbar_init_fence();
+    }
+    __syncwarp();
+    tc::tmem_alloc(tslot, G::tmem);
+    tc::tmem_relinquish();
+  }
+  pdl_wait();
+
+  // ---- the run of this CTA: every CTA sums the requests' tiles up ----
+  const int heads = min(p.num_kv_heads, (int)gridDim.x);   // KV heads that a group reads at the same time
+  const int hslot = (int)blockIdx.x % heads, group = (int)blockIdx.x / heads;
+  const int per = (p.num_reqs + kThreads - 1) / kThreads, r0 = min(p.num_reqs, tid * per), r1 = min(p.num_reqs, r0 + per);
+  long long mine = 0;
+  for (int r = r0; r < r1; ++r) {
+    const ReqShape s = req_shape<RP>(p, r);
+    mine += (long long)s.tiles * s.row_tiles;
+  }
+  long long upto = mine;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const long long x = __shfl_up_sync(0xffffffffu, upto, o);
+    if (lane >= o) upto += x;
+  }
+  if (lane == 31) warp_tiles[warp] = upto;
+  tc::fence_before_sync();
+  __syncthreads();
+  tc::fence_after_sync();
+  long long work = 0, before = upto - mine;
+  for (int w = 0; w < kThreads / 32; ++w) {
+    if (w < warp) before += warp_tiles[w];
+    work += warp_tiles[w];
+  }
+  const long long most = work / kRunMin > 0 ? work / kRunMin : 1;
+  const int groups = (int)min((long long)((int)gridDim.x / heads), most);
+  const long long run_begin = group < groups ? work * group / groups : 0, run_end = group < groups ? work * (group + 1) / groups : 0;
+  if (run_begin < run_end && before <= run_begin && run_begin < before + mine) {
+    long long start = before;
+    int r = r0;
+    for (;; ++r) {
+      const ReqShape s = req_shape<RP>(p, r);
+      const long long n = (long long)s.tiles * s.row_tiles;
+      if (run_begin < start + n) break;
+      start += n;
+    }
+    *first_req = r;
+    *first_start = start;
+  }
+  // requests without a visible key: zero, -inf
+  for (int r = (int)blockIdx.x; r < p.num_reqs; r += (int)gridDim.x) {
+    const ReqShape s = req_shape<RP>(p, r);
+    if (s.tiles > 0 || s.tokens == 0) continue;
+    for (int64_t i = tid; i < (int64_t)s.tokens * p.num_q_heads * (HD / 8); i += kThreads) {
+      const int64_t row = i / (HD / 8);
+      const int token = s.first + (int)(row / p.num_q_heads), head = (int)(row % p.num_q_heads), c = (int)(i % (HD / 8));
+      *reinterpret_cast<uint4*>(p.out + (int64_t)token * p.out_stride_token + (int64_t)head * p.out_stride_head + c * 16) = make_uint4(0u, 0u, 0u, 0u);
+      if (c == 0 && p.lse != nullptr) p.lse[(int64_t)token * p.num_q_heads + head] = -INFINITY;
+    }
+  }
+  __syncthreads();
+  const uint32_t tmem_base = *tslot;
+  const bool works = run_begin < run_end;
+  Walk<RP> start;
+  start.at = run_begin;
+  start.end = run_end;
+  start.start = works ? *first_start : 0;
+  start.r = works ? *first_req : 0;
+  bool ok = true;
+
+  if (warp >= kLoadWarp && warp < kMmaWarp) {
+    // =========================== copies ==========================================
+    // A warp owns 32 keys of every tile: lane l knows where key l of them lies, and the lanes copy rows of
+    // 16-byte chunks, 2 (128 dims) or 4 rows at a time.
+    constexpr int kChunks = G::dims / 8, kRows = 32 / kChunks;
+    const int base_key = (warp - kLoadWarp) * 32, chunk = lane % kChunks, sub = lane / kChunks;
+    const uint32_t ring = tc::smem_u32(smem);
+    uint32_t unit = 0, item = 0;
+    auto load_unit = [&](const uint8_t* src, long long off, bool q_too, const Piece& it, int kvh) {
+      const uint32_t s = unit % G::units;
+      if (unit >= G::units) ok &= wait_or_abort(&empty[s], ((unit / G::units) - 1) & 1, abort_flag);
+      if (q_too) {
+        // the rows of Q: chunk c of row n at c (RP 16) + n 16
+        if (item >= 2) ok &= wait_or_abort(&bars[Bars::q_empty + (item & 1)], ((item >> 1) - 1) & 1, abort_flag);
+        const uint32_t dst = tc::smem_u32(smem + G::q) + (item & 1) * G::qimage;
+        for (int i = tid - kLoadWarp * 32; i < RP * (HD / 8); i += 128) {
+          const int n = i / (HD / 8), c = i % (HD / 8);
+          int token, head;
+          row_of(p, it.first_token, kvh, it.row0 + min(n, it.rows - 1), &token, &head);
+          copy16(dst + c * (RP * 16) + n * 16, p.q + (int64_t)token * p.q_stride_token + (int64_t)head * p.q_stride_head + c * 16, n < it.rows);
+        }
+        ++item;
+      }
+      const uint32_t dst = ring + s * G::unit + (chunk >> 3) * (kTile * 128);
+#pragma unroll
+      for (int i = 0; i < 32 / kRows; ++i) {
+        const int row = i * kRows + sub;
+        const long long o = __shfl_sync(0xffffffffu, off, row);
+        copy16(dst + (base_key + row) * 128 + (((chunk & 7) ^ (row & 7)) << 4), o >= 0 ? src + o + chunk * 16 : src, o >= 0);
+      }
+      copies_arrive(&full[s]);
+      ++unit;
+    };
+    for (int kvh = hslot; kvh < p.num_kv_heads && works; kvh += heads) {
+      const uint8_t* kb = p.k + (int64_t)kvh * p.stride_head;
+      const uint8_t* vb = p.v + (int64_t)kvh * p.stride_head;
+      Walk<RP> w = start;
+      Piece it;
+      int left = 0;       // tiles of `it` behind the one whose block id is on its way
+      int key0 = 0;       // first key of that tile
+      // the block id and slot of this lane's key of the next tile, -1 where it sees none; false at the run's end
+      int blk = -1, slot = 0;
+      bool fresh = false, have;
+      auto fetch = [&]() -> bool {
+        if (left == 0) {
+          if (!next_piece<RP>(p, w, &it)) return false;
+          left = it.tiles;
+          key0 = it.key0;
+          fresh = true;
+        } else {
+          key0 += kTile;
+          fresh = false;
+        }
+        --left;
+        const int pos = key0 + base_key + lane;
+        blk = -1;
+        if (pos >= it.lo && pos < it.hi) {
+          int page;
+          if (p.block_shift >= 0) {
+            page = pos >> p.block_shift;
+            slot = pos & (p.block_size - 1);
+          } else {
+            page = (int)((uint32_t)pos / (uint32_t)p.block_size);
+            slot = pos - page * p.block_size;
+          }
+          blk = __ldg(p.block_table + (int64_t)it.r * p.block_table_row_stride + page);
+        }
+        return true;
+      };
+      auto place_of = [&]() -> long long { return blk >= 0 ? (long long)blk * p.stride_block + (long long)slot * p.stride_slot : -1ll; };
+      have = fetch();
+      long long off = 0, off_v = 0;
+      bool have_v = false;
+      while (have || have_v) {
+        Piece cur = it;
+        const bool first = fresh, now = have;
+        if (now) {
+          off = place_of();
+          have = fetch();   // (its load is in flight while this tile's copies are issued)
+#pragma unroll
+          for (int part = 0; part < G::parts; ++part) load_unit(kb + part * 256, off, first && part == 0, cur, kvh);
+        }
+        if (have_v) {
+#pragma unroll
+          for (int part = 0; part < G::parts; ++part) load_unit(vb + part * 256, off_v, false, cur, kvh);
+        }
+        off_v = off;
+        have_v = now;
+      }
+    }
+    copies_wait_all();
+  } else if (warp == kMmaWarp) {
+    // =========================== MMAs ============================================
+    // QK of a tile is issued ahead of PV of the one before, in the order in which the units arrive.
+    constexpr uint32_t fmt = kHalf ? tc::kFmtF16 : tc::kFmtBF16;
+    constexpr uint32_t qk_desc = tc::instr_desc(128, G::cols, fmt, fmt, 0, 0);
+    constexpr uint32_t pv_desc = tc::instr_desc(128, 2 * RP, fmt, fmt, 1, 1);
+    const uint32_t ring = tc::smem_u32(smem), q_s = tc::smem_u32(smem + G::q), p_s = tc::smem_u32(smem + G::p);
+    uint32_t unit = 0, tile = 0, item = 0;
+    auto arrived = [&]() -> uint32_t {
+      const uint32_t s = unit % G::units;
+      ok &= wait_or_abort(&full[s], (unit / G::units) & 1, abort_flag);
+      tc::fence_async_smem();   // (the copies wrote through the generic proxy)
+      ++unit;
+      return s;
+    };
+    auto qk = [&](bool last_of_item) {
+#pragma unroll
+      for (int part = 0; part < G::parts; ++part) {
+        const uint32_t s = arrived();
+        if (elect_one()) {
+          tc::fence_after_sync();
+#pragma unroll
+          for (int kk = 0; kk < G::dims / 16; ++kk) {
+            const uint64_t a = swizzled_desc(ring + s * G::unit + (kk >> 2) * (kTile * 128) + (kk & 3) * 32, 16, 1024);
+            const uint64_t b = tc::smem_desc(q_s + (item & 1) * G::qimage + (part * (G::dims / 8) + kk * 2) * (RP * 16), RP * 16, RP == 8 ? 0 : 128);
+            tc::mma_ss(tmem_base + G::s_col + (tile & 1) * G::cols, a, b, qk_desc, part > 0 || kk > 0);
+          }
+          tc::mma_commit(&empty[s]);
+          if (part == G::parts - 1) {
+            tc::mma_commit(&bars[Bars::s_ready + (tile & 1)]);
+            if (last_of_item) tc::mma_commit(&bars[Bars::q_empty + (item & 1)]);
+          }
+        }
+        __syncwarp();
+      }
+      ++tile;
+      if (last_of_item) ++item;
+    };
+    uint32_t pv_tile = 0;
+    auto pv = [&](bool first_of_item) {
+      ok &= wait_or_abort(&bars[Bars::p_ready], pv_tile & 1, abort_flag);
+#pragma unroll
+      for (int part = 0; part < G::parts; ++part) {
+        const uint32_t s = arrived();
+        if (elect_one()) {
+          tc::fence_after_sync();
+#pragma unroll
+          for (int kk = 0; kk < kTile / 16; ++kk) {
+            // (64 dims: the instruction's other 64 rows are the same bytes again, which nothing reads)
+            const uint64_t a = swizzled_desc(ring + s * G::unit + kk * 2048, HD == 64 ? 0 : kTile * 128, 1024);
+            const uint64_t b = tc::smem_desc(p_s + kk * 256, 128, kTile * 16);
+            tc::mma_ss(tmem_base + G::o_col + part * 2 * RP, a, b, pv_desc, !first_of_item || kk > 0);
+          }
+          tc::mma_commit(&empty[s]);
+          if (part == G::parts - 1) tc::mma_commit(&bars[Bars::pv_done]);
+        }
+        __syncwarp();
+      }
+      ++pv_tile;
+    };
+    for (int kvh = hslot; kvh < p.num_kv_heads && works; kvh += heads) {
+      Walk<RP> w = start;
+      Piece it;
+      bool pending = false, pending_first = false;
+      while (next_piece<RP>(p, w, &it)) {
+        for (int t = 0; t < it.tiles; ++t) {
+          qk(t == it.tiles - 1);
+          if (pending) pv(pending_first);
+          pending = true;
+          pending_first = t == 0;
+        }
+      }
+      if (pending) pv(pending_first);
+    }
+  } else if (warp < kLoadWarp) {
+    // =========================== softmax =========================================
+    const uint32_t lane_addr = (uint32_t)(warp * 32) << 16;
+    float* const wmax = reinterpret_cast<float*>(smem + G::wmax);
+    float* const wsum = reinterpret_cast<float*>(smem + G::wsum);
+    uint8_t* const p_img = smem + G::p + tid * 16;
+    uint32_t tile = 0;
+    for (int kvh = hslot; kvh < p.num_kv_heads && works; kvh += heads) {
+      Walk<RP> w = start;
+      Piece it;
+      while (next_piece<RP>(p, w, &it)) {
+        float ref[RP], l[RP];
+#pragma unroll
+        for (int n = 0; n < RP; ++n) {
+          ref[n] = -INFINITY;
+          l[n] = 0.f;
+        }
+        for (int t = 0; t < it.tiles; ++t, ++tile) {
+          ok &= wait_or_abort(&bars[Bars::s_ready + (tile & 1)], (tile >> 1) & 1, abort_flag);
+          tc::fence_after_sync();
+          uint32_t sr[RP];
+          tmem_load<RP>(tmem_base + G::s_col + (tile & 1) * G::cols + lane_addr, sr);
+          tc::tmem_ld_wait<RP>(sr);
+          const int pos = it.key0 + t * kTile + tid;
+          if (pos < it.lo || pos >= it.hi) {
+#pragma unroll
+            for (int n = 0; n < RP; ++n) sr[n] = 0xff800000u;  // -inf
+          }
+          float x[RP];
+          bool outgrown = false;
+#pragma unroll
+          for (int n = 0; n < RP; ++n) {
+            x[n] = fmaf(__uint_as_float(sr[n]), p.scale_log2, -ref[n]);
+            outgrown |= n < it.rows && !(x[n] <= kGain + kSlack);   // (also where ref is not set yet)
+          }
+          if (softmax_any(outgrown)) {
+#pragma unroll
+            for (int n = 0; n < RP; ++n) {
+              const float m = redux_max(__uint_as_float(sr[n]));
+              if (lane == 0) wmax[warp * RP + n] = m * p.scale_log2;
+            }
+            softmax_sync();
+            float alpha[RP];
+            bool moved = false;
+#pragma unroll
+            for (int n = 0; n < RP; ++n) {
+              const float m = fmaxf(fmaxf(wmax[n], wmax[RP + n]), fmaxf(wmax[2 * RP + n], wmax[3 * RP + n])) - kGain;
+              const float to = fmaxf(ref[n], m);
+              alpha[n] = to == -INFINITY ? 1.f : kv16_exp2(ref[n] - to);
+              moved |= alpha[n] != 1.f;
+              ref[n] = to;
+              l[n] *= alpha[n];
+              x[n] = fmaf(__uint_as_float(sr[n]), p.scale_log2, to == -INFINITY ? 0.f : -to);
+            }
+            if (t > 0 && moved) {   // (the same in all threads)
+              ok &= wait_or_abort(&bars[Bars::pv_done], (tile - 1) & 1, abort_flag);
+              tc::fence_after_sync();
+#pragma unroll
+              for (int part = 0; part < G::parts; ++part) {
+                uint32_t o[2 * RP];
+                const uint32_t addr = tmem_base + G::o_col + part * 2 * RP + lane_addr;
+                tmem_load<2 * RP>(addr, o);
+                tc::tmem_ld_wait<2 * RP>(o);
+#pragma unroll
+                for (int n = 0; n < RP; ++n) {
+                  o[n] = __float_as_uint(__uint_as_float(o[n]) * alpha[n]);
+                  o[RP + n] = __float_as_uint(__uint_as_float(o[RP + n]) * alpha[n]);
+                }
+                tmem_store<2 * RP>(addr, o);
+              }
+              tc::tmem_st_wait();
+            }
+            softmax_sync();  // (the maxima have been read)
+          }
+          uint32_t hi[RP / 2], lo[RP / 2];
+#pragma unroll
+          for (int n = 0; n < RP; n += 2) {
+            const float a = kv16_exp2(x[n]), b = kv16_exp2(x[n + 1]);
+            l[n] += a;
+            l[n + 1] += b;
+            split2<kHalf>(a, b, &hi[n / 2], &lo[n / 2]);
+          }
+          if (tile > 0) ok &= wait_or_abort(&bars[Bars::pv_done], (tile - 1) & 1, abort_flag);  // (P of the last tile has been read)
+#pragma unroll
+          for (int j = 0; j < RP / 8; ++j) {
+            *reinterpret_cast<uint4*>(p_img + j * (kTile * 16)) = make_uint4(hi[4 * j], hi[4 * j + 1], hi[4 * j + 2], hi[4 * j + 3]);
+            *reinterpret_cast<uint4*>(p_img + (RP / 8 + j) * (kTile * 16)) = make_uint4(lo[4 * j], lo[4 * j + 1], lo[4 * j + 2], lo[4 * j + 3]);
+          }
+          tc::fence_async_smem();
+          tc::fence_before_sync();
+          mbar_arrive(&bars[Bars::p_ready]);
+        }
+        // ---- the piece's rows ----
+#pragma unroll
+        for (int n = 0; n < RP; ++n) {
+#pragma unroll
+          for (int o = 16; o > 0; o >>= 1) l[n] += __shfl_xor_sync(0xffffffffu, l[n], o);
+        }
+        if (lane == 0) {
+#pragma unroll
+          for (int n = 0; n < RP; ++n) wsum[warp * RP + n] = l[n];
+        }
+        softmax_sync();
+#pragma unroll
+        for (int n = 0; n < RP; ++n) l[n] = (wsum[n] + wsum[RP + n]) + (wsum[2 * RP + n] + wsum[3 * RP + n]);
+        ok &= wait_or_abort(&bars[Bars::pv_done], (tile - 1) & 1, abort_flag);
+        tc::fence_after_sync();
+        const bool whole = it.begins && it.ends;
+        float* const slot = partial_slot<HD, RP>(p, (int)blockIdx.x, it.begins);
+#pragma unroll
+        for (int part = 0; part < G::parts; ++part) {
+          uint32_t o[2 * RP];
+          tmem_load<2 * RP>(tmem_base + G::o_col + part * 2 * RP + lane_addr, o);
+          tc::tmem_ld_wait<2 * RP>(o);
+          const int d = part * 128 + tid;
+          if (d < HD) {
+#pragma unroll
+            for (int n = 0; n < RP; ++n) {
+              if (n < it.rows) {
+                const float v = __uint_as_float(o[n]) + __uint_as_float(o[RP + n]);
+                if (whole) {
+                  int token, head;
+                  row_of(p, it.first_token, kvh, it.row0 + n, &token, &head);
+                  store_out_elem(p.out + (int64_t)token * p.out_stride_token + (int64_t)head * p.out_stride_head, d, kHalf ? PTH_ATTN_F16 : PTH_ATTN_BF16,
+                                 l[n] == 0.f ? 0.f : v / l[n]);
+                } else {
+                  slot[n * HD + d] = v;
+                }
+              }
+            }
+          }
+        }
+        tc::fence_before_sync();
+        if (tid == 0) {
+#pragma unroll
+          for (int n = 0; n < RP; ++n) {
+            if (n < it.rows) {
+              if (whole) {
+                int token, head;
+                row_of(p, it.first_token, kvh, it.row0 + n, &token, &head);
+                if (p.lse != nullptr)
+                  p.lse[(int64_t)token * p.num_q_heads + head] = l[n] == 0.f ? -INFINITY : ((ref[n] == -INFINITY ? 0.f : ref[n]) + log2f(l[n])) * kLn2;
+              } else {
+                slot[RP * HD + n] = ref[n];
+                slot[RP * HD + RP + n] = l[n];
+              }
+            }
+          }
+        }
+        if (!whole) {
+          const int g0 = (int)(((it.start + 1) * groups - 1) / work), g1 = (int)(((it.start + it.row_tiles_keys) * groups - 1) / work);
+          __threadfence();
+          softmax_sync();
+          int* const counter = reinterpret_cast<int*>(p.workspace) + g0 * heads + hslot;
+          if (tid == 0) *arrival = atomicAdd(counter, 1);
+          softmax_sync();
+          if (*arrival == g1 - g0) {
+            __threadfence();
+            if (tid == 0) *counter = 0;   // (for the next call)
+            merge_pieces<HD, RP>(p, it, kvh, g0, g1 - g0 + 1, heads, hslot);
+          }
+        }
+        softmax_sync();  // (the sums and the arrival have been read)
+      }
+    }
+  }
+  tc::fence_before_sync();
+  __syncthreads();
+  if (warp == kMmaWarp) tc::tmem_dealloc(tmem_base, G::tmem);
+  if (tid == 0 && *abort_flag) atomicOr(&g_kv16_status, 8u);
+  (void)ok;
+}
+
+template <int HD, int RP, bool kHalf>
+cudaError_t launch_one(const Kv16Params& p, cudaStream_t stream) {
+  using G = Geo<HD, RP>;
+  static_assert(G::total <= 232448, "shared memory of one CTA");
+  static_assert(G::ctas == 1 || G::total <= 115712, "shared memory of two CTAs");
+  static bool configured[64] = {};
+  int dev = 0;
+  cudaError_t err = cudaGetDevice(&dev);
+  if (err != cudaSuccess) return err;
+  if (dev < 0 || dev >= 64 || !configured[dev]) {
+    err = cudaFuncSetAttribute(kv16_short_kernel<HD, RP, kHalf>, cudaFuncAttributeMaxDynamicSharedMemorySize, G::total);
+    if (err != cudaSuccess) return err;
+    if (dev >= 0 && dev < 64) configured[dev] = true;
+  }
+  const int sms = sm_count();
+  if (sms <= 0) return cudaErrorInvalidDevice;
+  return pdl_launch(kv16_short_kernel<HD, RP, kHalf>, dim3((unsigned)(sms * G::ctas)), dim3(kThreads), G::total, stream, p);
+}
+template <int HD, int RP>
+cudaError_t launch_type(const Kv16Params& p, cudaStream_t stream) {
+  return p.dtype == PTH_ATTN_F16 ? launch_one<HD, RP, true>(p, stream) : launch_one<HD, RP, false>(p, stream);
+}
+template <int HD>
+cudaError_t launch_rows(const Kv16Params& p, cudaStream_t stream) {
+  const int64_t rows = (int64_t)p.max_query_len * p.group;
+  if (rows <= 8) return launch_type<HD, 8>(p, stream);
+  if (rows <= 16) return launch_type<HD, 16>(p, stream);
+  return launch_type<HD, 32>(p, stream);
+}
+
+}  // namespace
+
+// Counters, and two partial row tiles per CTA: twice the SMs' number of CTAs with 16 rows, or as many with 32.
+int64_t kv16_workspace_bytes(int head_size, int num_sms) {
+  return kCounterBytes + (int64_t)num_sms * 2 * 2 * 16 * (head_size + 2) * 4;
+}
+
+cudaError_t launch_kv16_attention(const Kv16Params& p, cudaStream_t stream) {
+  switch (p.head_size) {
+    case 64:
+      return launch_rows<64>(p, stream);
+    case 128:
+      return launch_rows<128>(p, stream);
+    default:
+      return launch_rows<256>(p, stream);
+  }
+}
+
+// Reads and clears this kernel's status word (device must be idle).
+cudaError_t read_kv16_status(unsigned int* v) {
+  unsigned int zero = 0;
+  cudaError_t err = cudaMemcpyFromSymbol(v, g_kv16_status, sizeof(*v));
+  if (err != cudaSuccess) return err;
+  return cudaMemcpyToSymbol(g_kv16_status, &zero, sizeof(zero));
+}
+
+}  // namespace pthb200
