@@ -21,7 +21,7 @@ OP_LIB = HERE / "_C.abi3.so"
 
 CUDA_SOURCES = ["launcher.cu", "scalar_kernel.cu", "combine_kernel.cu", "umma_kernel.cu", "umma_i8_kernel.cu",
                 "umma_rows_kernel.cu", "umma_rows256_kernel.cu", "umma_rows2_kernel.cu", "writer_kernel.cu", "copy_ceiling_kernel.cu",
-                "kv16_api.cu", "page_tables_kernel.cu", "kv16_writer_kernel.cu", "kv16_short_kernel.cu"]
+                "kv16_api.cu", "page_tables_kernel.cu", "kv16_writer_kernel.cu", "kv16_short_kernel.cu", "kv16_tall_kernel.cu"]
 OP_SOURCES = ["torch_op.cpp", "torch_kv16.cpp"]
 NVCC_FLAGS = [
     "-std=c++17", "-O3", "-lineinfo", "-gencode", "arch=compute_100a,code=sm_100a",

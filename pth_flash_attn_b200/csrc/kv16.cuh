@@ -72,8 +72,11 @@ __device__ __forceinline__ float kv16_exp2(float x) {
 int32_t clear_error();
 int32_t set_error(int32_t code, const std::string& msg);
 
-int64_t kv16_workspace_bytes(int head_size, int num_sms);
-cudaError_t launch_kv16_attention(const Kv16Params& p, cudaStream_t stream);
+// kv16_short_kernel.cu, kv16_tall_kernel.cu
+int64_t kv16_short_workspace_bytes(int head_size, int num_sms);
+int64_t kv16_tall_workspace_bytes(int head_size, int num_sms);
+cudaError_t launch_kv16_short(const Kv16Params& p, cudaStream_t stream);
+cudaError_t launch_kv16_tall(const Kv16Params& p, cudaStream_t stream);
 cudaError_t launch_kv16_writer(const PthB200Kv16WriteArgs& a, cudaStream_t stream);
 cudaError_t launch_page_tables(const PthB200TablesArgs& a, cudaStream_t stream);
 

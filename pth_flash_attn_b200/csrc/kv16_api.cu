@@ -1,5 +1,6 @@
 // C entries of the 16-bit paged cache (include/pthb200_attn.h): argument checks, each naming its field, and the
 // launches.  Nothing here allocates, reads device memory or synchronises.
+#include <algorithm>
 #include <cmath>
 
 #include "kv16.cuh"
@@ -112,6 +113,13 @@ int32_t build(const PthB200Kv16Args* a, bool cross, Kv16Params* p) {
   return PTH_ATTN_OK;
 }
 
+// Query rows per KV head from which a launch goes to the kernel with the rows on the MMA's M dimension.
+constexpr int64_t kTallRows = 33;
+
+int64_t workspace_bytes(int head_size, int num_sms) {
+  return std::max(kv16_short_workspace_bytes(head_size, num_sms), kv16_tall_workspace_bytes(head_size, num_sms));
+}
+
 int32_t attention(const PthB200Kv16Args* a, bool cross, void* stream) {
   clear_error();
   Kv16Params p;
@@ -120,9 +128,10 @@ int32_t attention(const PthB200Kv16Args* a, bool cross, void* stream) {
   int dev = 0, sms = 0;
   if (cudaGetDevice(&dev) != cudaSuccess || cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess)
     return set_error(PTH_ATTN_ECUDA, "cannot query the current device");
-  const int64_t need = kv16_workspace_bytes(a->head_size, sms);
+  const int64_t need = workspace_bytes(a->head_size, sms);
   KV16_REQUIRE(a->workspace_bytes >= need, "workspace has " + std::to_string(a->workspace_bytes) + " bytes, " + std::to_string(need) + " are needed");
-  return launched(launch_kv16_attention(p, static_cast<cudaStream_t>(stream)), "attention");
+  const bool tall = (int64_t)p.max_query_len * p.group >= kTallRows && p.max_query_len > 1;
+  return launched((tall ? launch_kv16_tall : launch_kv16_short)(p, static_cast<cudaStream_t>(stream)), "attention");
 }
 
 }  // namespace
@@ -134,7 +143,7 @@ int32_t pthb200_tables_args_bytes(void) { return (int32_t)sizeof(PthB200TablesAr
 int32_t pthb200_kv16_write_args_bytes(void) { return (int32_t)sizeof(PthB200Kv16WriteArgs); }
 int32_t pthb200_kv16_args_bytes(void) { return (int32_t)sizeof(PthB200Kv16Args); }
 int64_t pthb200_kv16_workspace_bytes(int32_t head_size, int32_t num_sms) {
-  return pthb200::is_head_size(head_size) && num_sms >= 1 ? pthb200::kv16_workspace_bytes(head_size, num_sms) : -1;
+  return pthb200::is_head_size(head_size) && num_sms >= 1 ? pthb200::workspace_bytes(head_size, num_sms) : -1;
 }
 
 int32_t pthb200_page_tables(const PthB200TablesArgs* a, void* stream) {

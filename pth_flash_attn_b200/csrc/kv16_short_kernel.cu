@@ -25,7 +25,7 @@
 // CTAs; CTA h of a group reads head h, so the heads of a page are read at the same time.  A request that a cut divides
 // leaves partial (O, ref, l) of its pieces in the workspace, and the CTA that arrives last merges them in the pieces' order:
 // one launch, and the same bits whoever is last.
-#include "kv16.cuh"
+#include "kv16_sched.cuh"
 #include "page_copy.cuh"
 #include "pdl.cuh"
 
@@ -35,14 +35,11 @@ __device__ unsigned int g_kv16_status = 0;
 
 namespace {
 
-constexpr int kTile = 128;             // keys
 constexpr int kSoftmaxThreads = 128;   // warps 0-3: thread t is key t of a tile, then dim t of the output
 constexpr int kLoadWarp = 4;           // warps 4-7
 constexpr int kMmaWarp = 8;
 constexpr int kThreads = 288;
-constexpr int kCounterBytes = 4096;    // arrival counters at the start of the workspace, one per CTA
 constexpr float kGain = 7.f, kSlack = 8.f;
-constexpr int kRunMin = 1;             // KV tiles a run holds at least
 
 template <int HD, int RP>
 struct Geo {
@@ -71,7 +68,7 @@ struct Geo {
   static constexpr int wsum = wmax + 4 * RP * 4;     // float [4 warps][RP]
   static constexpr int bars = wsum + 4 * RP * 4;
   static constexpr int n_bars = 2 * units + 2 + 2 + 1 + 1;
-  static constexpr int misc = bars + n_bars * 8;     // ints: abort flag, TMEM address, first request, last arrival; 64-bit scan
+  static constexpr int misc = bars + n_bars * 8;     // ints: abort flag, TMEM address, arrival; scratch of find_run
   static constexpr int total = misc + 160 + 1024;
   static_assert(n_bars * 8 + 160 <= 512, "fixed part");
 };
@@ -80,76 +77,6 @@ struct Bars {  // offsets behind [units] full, [units] empty
   static constexpr int q_empty = 0, s_ready = 2, p_ready = 4, pv_done = 5;
 };
 
-// One piece of a request's row tile: keys [key0, key0 + 128 tiles) of those visible, [lo, hi).
-struct Piece {
-  int r, row0, rows;          // rows row0 .. row0 + rows of the request's q_len x G
-  int first_token;
-  int key0, tiles, lo, hi;
-  bool begins, ends;
-  long long start;            // of the row tile in the sequence
-  int row_tiles_keys;         // KV tiles of the whole row tile
-};
-
-template <int RP>
-struct Walk {
-  long long at, end, start;   // position in the sequence, end of the run, start of request r
-  int r;
-};
-
-struct ReqShape {
-  int tokens, first, lo, hi, tiles, row_tiles;
-};
-template <int RP>
-__device__ __forceinline__ ReqShape req_shape(const Kv16Params& p, int r) {
-  ReqShape s;
-  kv16_visible(p, r, &s.lo, &s.hi);
-  s.tokens = kv16_tokens(p, r, &s.first);
-  const int rows = s.tokens * p.group;
-  s.row_tiles = (rows + RP - 1) / RP;
-  s.tiles = s.hi > s.lo && rows > 0 ? (s.hi + kTile - 1) / kTile - s.lo / kTile : 0;
-  return s;
-}
-template <int RP>
-__device__ __forceinline__ bool next_piece(const Kv16Params& p, Walk<RP>& w, Piece* out) {
-  if (w.at >= w.end) return false;
-  ReqShape s = req_shape<RP>(p, w.r);
-  long long n = (long long)s.tiles * s.row_tiles;
-  while (w.at >= w.start + n) {
-    w.start += n;
-    ++w.r;
-    s = req_shape<RP>(p, w.r);
-    n = (long long)s.tiles * s.row_tiles;
-  }
-  const long long off = w.at - w.start;
-  const int rt = s.row_tiles == 1 ? 0 : (int)(off / s.tiles);
-  const int tile = (int)(off - (long long)rt * s.tiles);
-  out->r = w.r;
-  out->row0 = rt * RP;
-  out->rows = min(RP, s.tokens * p.group - rt * RP);
-  out->first_token = s.first;
-  out->lo = s.lo;
-  out->hi = s.hi;
-  out->key0 = (s.lo / kTile + tile) * kTile;
-  out->tiles = (int)min((long long)(s.tiles - tile), w.end - w.at);
-  out->begins = tile == 0;
-  out->ends = tile + out->tiles == s.tiles;
-  out->start = w.start + (long long)rt * s.tiles;
-  out->row_tiles_keys = s.tiles;
-  w.at += out->tiles;
-  return true;
-}
-// Token and query head of a row of a request.
-__device__ __forceinline__ void row_of(const Kv16Params& p, int first_token, int kvh, int row, int* token, int* head) {
-  const int t = p.query_start_loc == nullptr ? 0 : (int)((uint32_t)row / (uint32_t)p.group);
-  *token = first_token + t;
-  *head = kvh * p.group + row - t * p.group;
-}
-
-__device__ __forceinline__ float redux_max(float x) {
-  float y;
-  asm volatile("redux.sync.max.f32 %0, %1, 0xffffffff;" : "=f"(y) : "f"(x));
-  return y;
-}
 // Barrier of the softmax warps that tells whether any of them has seen `x`.
 __device__ __forceinline__ bool softmax_any(bool x) {
   uint32_t r;
@@ -286,11 +213,7 @@ __global__ void __launch_bounds__(kThreads, (Geo<HD, RP>::ctas)) kv16_short_kern
   uint64_t* const bars = empty + G::units;
   volatile int* const abort_flag = reinterpret_cast<volatile int*>(smem + G::misc);
   uint32_t* const tslot = reinterpret_cast<uint32_t*>(smem + G::misc + 4);
-  int* const first_req = reinterpret_cast<int*>(smem + G::misc + 8);
-  int* const arrival = reinterpret_cast<int*>(smem + G::misc + 12);
-  long long* const first_start = reinterpret_cast<long long*>(smem + G::misc + 16);
-  long long* const warp_tiles = reinterpret_cast<long long*>(smem + G::misc + 24);  // [9 warps]
-  static_assert((G::misc + 16) % 8 == 0, "64-bit words");
+  int* const arrival = reinterpret_cast<int*>(smem + G::misc + 8);
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
 
   if (warp == kMmaWarp) {
@@ -314,151 +237,69 @@ __global__ void __launch_bounds__(kThreads, (Geo<HD, RP>::ctas)) kv16_short_kern
   }
   pdl_wait();
 
-  // ---- the run of this CTA: every CTA sums the requests' tiles up ----
-  const int heads = min(p.num_kv_heads, (int)gridDim.x);   // KV heads that a group reads at the same time
-  const int hslot = (int)blockIdx.x % heads, group = (int)blockIdx.x / heads;
-  const int per = (p.num_reqs + kThreads - 1) / kThreads, r0 = min(p.num_reqs, tid * per), r1 = min(p.num_reqs, r0 + per);
-  long long mine = 0;
-  for (int r = r0; r < r1; ++r) {
-    const ReqShape s = req_shape<RP>(p, r);
-    mine += (long long)s.tiles * s.row_tiles;
-  }
-  long long upto = mine;
-#pragma unroll
-  for (int o = 1; o < 32; o <<= 1) {
-    const long long x = __shfl_up_sync(0xffffffffu, upto, o);
-    if (lane >= o) upto += x;
-  }
-  if (lane == 31) warp_tiles[warp] = upto;
+  const Run<RP> run = find_run<RP, kThreads>(p, reinterpret_cast<long long*>(smem + G::misc + 16));
+  zero_requests<HD, RP, kThreads>(p);
   tc::fence_before_sync();
   __syncthreads();
   tc::fence_after_sync();
-  long long work = 0, before = upto - mine;
-  for (int w = 0; w < kThreads / 32; ++w) {
-    if (w < warp) before += warp_tiles[w];
-    work += warp_tiles[w];
-  }
-  const long long most = work / kRunMin > 0 ? work / kRunMin : 1;
-  const int groups = (int)min((long long)((int)gridDim.x / heads), most);
-  const long long run_begin = group < groups ? work * group / groups : 0, run_end = group < groups ? work * (group + 1) / groups : 0;
-  if (run_begin < run_end && before <= run_begin && run_begin < before + mine) {
-    long long start = before;
-    int r = r0;
-    for (;; ++r) {
-      const ReqShape s = req_shape<RP>(p, r);
-      const long long n = (long long)s.tiles * s.row_tiles;
-      if (run_begin < start + n) break;
-      start += n;
-    }
-    *first_req = r;
-    *first_start = start;
-  }
-  // requests without a visible key: zero, -inf
-  for (int r = (int)blockIdx.x; r < p.num_reqs; r += (int)gridDim.x) {
-    const ReqShape s = req_shape<RP>(p, r);
-    if (s.tiles > 0 || s.tokens == 0) continue;
-    for (int64_t i = tid; i < (int64_t)s.tokens * p.num_q_heads * (HD / 8); i += kThreads) {
-      const int64_t row = i / (HD / 8);
-      const int token = s.first + (int)(row / p.num_q_heads), head = (int)(row % p.num_q_heads), c = (int)(i % (HD / 8));
-      *reinterpret_cast<uint4*>(p.out + (int64_t)token * p.out_stride_token + (int64_t)head * p.out_stride_head + c * 16) = make_uint4(0u, 0u, 0u, 0u);
-      if (c == 0 && p.lse != nullptr) p.lse[(int64_t)token * p.num_q_heads + head] = -INFINITY;
-    }
-  }
-  __syncthreads();
   const uint32_t tmem_base = *tslot;
-  const bool works = run_begin < run_end;
-  Walk<RP> start;
-  start.at = run_begin;
-  start.end = run_end;
-  start.start = works ? *first_start : 0;
-  start.r = works ? *first_req : 0;
+  const int heads = run.heads, hslot = run.hslot;
+  const bool works = run.start.at < run.start.end;
+  const Walk<RP> start = run.start;
   bool ok = true;
 
   if (warp >= kLoadWarp && warp < kMmaWarp) {
     // =========================== copies ==========================================
-    // A warp owns 32 keys of every tile: lane l knows where key l of them lies, and the lanes copy rows of
-    // 16-byte chunks, 2 (128 dims) or 4 rows at a time.
-    constexpr int kChunks = G::dims / 8, kRows = 32 / kChunks;
-    const int base_key = (warp - kLoadWarp) * 32, chunk = lane % kChunks, sub = lane / kChunks;
+    // A warp owns 32 keys of every tile: lane l knows where key l of them lies.
+    const int base_key = (warp - kLoadWarp) * 32;
     const uint32_t ring = tc::smem_u32(smem);
     uint32_t unit = 0, item = 0;
-    auto load_unit = [&](const uint8_t* src, long long off, bool q_too, const Piece& it, int kvh) {
+    auto next_unit = [&]() -> uint32_t {
       const uint32_t s = unit % G::units;
       if (unit >= G::units) ok &= wait_or_abort(&empty[s], ((unit / G::units) - 1) & 1, abort_flag);
-      if (q_too) {
-        // the rows of Q: chunk c of row n at c (RP 16) + n 16
-        if (item >= 2) ok &= wait_or_abort(&bars[Bars::q_empty + (item & 1)], ((item >> 1) - 1) & 1, abort_flag);
-        const uint32_t dst = tc::smem_u32(smem + G::q) + (item & 1) * G::qimage;
-        for (int i = tid - kLoadWarp * 32; i < RP * (HD / 8); i += 128) {
-          const int n = i / (HD / 8), c = i % (HD / 8);
-          int token, head;
-          row_of(p, it.first_token, kvh, it.row0 + min(n, it.rows - 1), &token, &head);
-          copy16(dst + c * (RP * 16) + n * 16, p.q + (int64_t)token * p.q_stride_token + (int64_t)head * p.q_stride_head + c * 16, n < it.rows);
-        }
-        ++item;
-      }
-      const uint32_t dst = ring + s * G::unit + (chunk >> 3) * (kTile * 128);
-#pragma unroll
-      for (int i = 0; i < 32 / kRows; ++i) {
-        const int row = i * kRows + sub;
-        const long long o = __shfl_sync(0xffffffffu, off, row);
-        copy16(dst + (base_key + row) * 128 + (((chunk & 7) ^ (row & 7)) << 4), o >= 0 ? src + o + chunk * 16 : src, o >= 0);
-      }
-      copies_arrive(&full[s]);
       ++unit;
+      return s;
     };
     for (int kvh = hslot; kvh < p.num_kv_heads && works; kvh += heads) {
       const uint8_t* kb = p.k + (int64_t)kvh * p.stride_head;
       const uint8_t* vb = p.v + (int64_t)kvh * p.stride_head;
-      Walk<RP> w = start;
-      Piece it;
-      int left = 0;       // tiles of `it` behind the one whose block id is on its way
-      int key0 = 0;       // first key of that tile
-      // the block id and slot of this lane's key of the next tile, -1 where it sees none; false at the run's end
-      int blk = -1, slot = 0;
-      bool fresh = false, have;
-      auto fetch = [&]() -> bool {
-        if (left == 0) {
-          if (!next_piece<RP>(p, w, &it)) return false;
-          left = it.tiles;
-          key0 = it.key0;
-          fresh = true;
-        } else {
-          key0 += kTile;
-          fresh = false;
-        }
-        --left;
-        const int pos = key0 + base_key + lane;
-        blk = -1;
-        if (pos >= it.lo && pos < it.hi) {
-          int page;
-          if (p.block_shift >= 0) {
-            page = pos >> p.block_shift;
-            slot = pos & (p.block_size - 1);
-          } else {
-            page = (int)((uint32_t)pos / (uint32_t)p.block_size);
-            slot = pos - page * p.block_size;
-          }
-          blk = __ldg(p.block_table + (int64_t)it.r * p.block_table_row_stride + page);
-        }
-        return true;
-      };
-      auto place_of = [&]() -> long long { return blk >= 0 ? (long long)blk * p.stride_block + (long long)slot * p.stride_slot : -1ll; };
-      have = fetch();
-      long long off = 0, off_v = 0;
-      bool have_v = false;
+      KeyLookup<RP> keys(p, start, base_key + lane);
+      bool have = keys.fetch(), have_v = false;
+      long long off_v = 0;
       while (have || have_v) {
-        Piece cur = it;
-        const bool first = fresh, now = have;
+        const bool now = have;
+        long long off = 0;
         if (now) {
-          off = place_of();
-          have = fetch();   // (its load is in flight while this tile's copies are issued)
+          off = keys.offset();
+          const bool first = keys.fresh;
+          const int first_token = keys.it.first_token, row0 = keys.it.row0, rows = keys.it.rows;
+          have = keys.fetch();
 #pragma unroll
-          for (int part = 0; part < G::parts; ++part) load_unit(kb + part * 256, off, first && part == 0, cur, kvh);
+          for (int part = 0; part < G::parts; ++part) {
+            const uint32_t s = next_unit();
+            if (part == 0 && first) {
+              // the rows of Q come with the piece's first unit: chunk c of row n at c (RP 16) + n 16
+              if (item >= 2) ok &= wait_or_abort(&bars[Bars::q_empty + (item & 1)], ((item >> 1) - 1) & 1, abort_flag);
+              const uint32_t dst = tc::smem_u32(smem + G::q) + (item & 1) * G::qimage;
+              for (int i = tid - kLoadWarp * 32; i < RP * (HD / 8); i += 128) {
+                const int n = i / (HD / 8), c = i % (HD / 8);
+                int token, head;
+                row_of(p, first_token, kvh, row0 + min(n, rows - 1), &token, &head);
+                copy16(dst + c * (RP * 16) + n * 16, p.q + (int64_t)token * p.q_stride_token + (int64_t)head * p.q_stride_head + c * 16, n < rows);
+              }
+              ++item;
+            }
+            copy_keys<G::dims>(ring + s * G::unit, base_key, kb + part * 256, off);
+            copies_arrive(&full[s]);
+          }
         }
         if (have_v) {
 #pragma unroll
-          for (int part = 0; part < G::parts; ++part) load_unit(vb + part * 256, off_v, false, cur, kvh);
+          for (int part = 0; part < G::parts; ++part) {
+            const uint32_t s = next_unit();
+            copy_keys<G::dims>(ring + s * G::unit, base_key, vb + part * 256, off_v);
+            copies_arrive(&full[s]);
+          }
         }
         off_v = off;
         have_v = now;
@@ -689,7 +530,7 @@ __global__ void __launch_bounds__(kThreads, (Geo<HD, RP>::ctas)) kv16_short_kern
           }
         }
         if (!whole) {
-          const int g0 = (int)(((it.start + 1) * groups - 1) / work), g1 = (int)(((it.start + it.row_tiles_keys) * groups - 1) / work);
+          const int g0 = run.owner(it.start), g1 = run.owner(it.start + it.row_tiles_keys - 1);
           __threadfence();
           softmax_sync();
           int* const counter = reinterpret_cast<int*>(p.workspace) + g0 * heads + hslot;
@@ -745,11 +586,11 @@ cudaError_t launch_rows(const Kv16Params& p, cudaStream_t stream) {
 }  // namespace
 
 // Counters, and two partial row tiles per CTA: twice the SMs' number of CTAs with 16 rows, or as many with 32.
-int64_t kv16_workspace_bytes(int head_size, int num_sms) {
+int64_t kv16_short_workspace_bytes(int head_size, int num_sms) {
   return kCounterBytes + (int64_t)num_sms * 2 * 2 * 16 * (head_size + 2) * 4;
 }
 
-cudaError_t launch_kv16_attention(const Kv16Params& p, cudaStream_t stream) {
+cudaError_t launch_kv16_short(const Kv16Params& p, cudaStream_t stream) {
   switch (p.head_size) {
     case 64:
       return launch_rows<64>(p, stream);

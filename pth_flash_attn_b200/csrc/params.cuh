@@ -233,6 +233,7 @@ cudaError_t read_rows_status(unsigned int* v);
 cudaError_t read_rows256_status(unsigned int* v);
 cudaError_t read_rows2_status(unsigned int* v);
 cudaError_t read_kv16_status(unsigned int* v);
+cudaError_t read_kv16_tall_status(unsigned int* v);
 cudaError_t launch_umma_rows2_attention(const KernelParams& p, cudaStream_t stream);
 cudaError_t launch_umma_rows256_attention(const KernelParams& p, cudaStream_t stream);
 cudaError_t launch_combine_kernel(const CombineParams& p, cudaStream_t stream);

@@ -345,6 +345,8 @@ def test_no_requests_and_no_tokens():
 
 def test_refusals_on_the_device():
     b = Batch([40, 50], [1, 1], 8, 2, 128, BF16)
+    with pytest.raises(RuntimeError, match="kv16_decode_attention: workspace has 100 bytes"):
+        ops.kv16_decode_attention(b.out, b.lse, b.q, b.k, b.v, b.bt, b.lens, 1.0, b.ws[:100])
     with pytest.raises(RuntimeError, match="workspace must be on the same device as q"):
         ops.kv16_decode_attention(b.out, b.lse, b.q, b.k, b.v, b.bt, b.lens, 1.0, b.ws.cpu())
     k = torch.zeros((4, 16, 2, 132), dtype=BF16, device="cuda")[..., 4:]
