@@ -27,6 +27,8 @@ struct Kv16Params {
   int32_t block_size, block_shift;  // block_shift: log2(block_size), -1 if it is not a power of two
   int32_t num_kv_heads, num_q_heads, group, head_size;
   int32_t num_reqs, num_tokens, max_query_len, window;
+  int32_t num_blocks;
+  int32_t box_slots;  // slots of a TMA box (tall kernel; 0: none)
   float scale_log2;  // softmax_scale * log2(e)
 };
 
@@ -52,6 +54,36 @@ __device__ __forceinline__ void kv16_visible(const Kv16Params& p, int r, int* lo
 // holds 64 elements of M / N): sbo = next 8 rows, lbo = next 64 elements.
 __device__ __forceinline__ uint64_t swizzled_desc(uint32_t saddr, uint32_t lbo_bytes, uint32_t sbo_bytes) {
   return tc::smem_desc(saddr, lbo_bytes, sbo_bytes) | (uint64_t)2 << 61;
+}
+// Bounded wait for a phase of an mbarrier; once any wait of the CTA has given up, all do.  A try sleeps for a microsecond at
+// most, so the bound is between some 50 ms and 4 s.
+__device__ __forceinline__ bool kv16_wait(uint64_t* bar, uint32_t parity, volatile int* abort_flag) {
+#pragma unroll 1
+  for (uint32_t i = 0; i < (1u << 22); ++i) {
+    if (tc::mbar_try_wait_hint(bar, parity, 1000u)) return true;
+    if (*abort_flag) return false;
+  }
+  *abort_flag = 1;
+  return false;
+}
+// The same wait without sleep at first, where the next step of a chain hangs on it: a sleeping thread wakes late.
+__device__ __forceinline__ bool kv16_spin(uint64_t* bar, uint32_t parity, volatile int* abort_flag) {
+  const uint32_t bar_s = tc::smem_u32(bar);
+#pragma unroll 1
+  for (uint32_t i = 0; i < 4096; ++i) {
+    uint32_t done;
+    asm volatile(
+        "{\n\t"
+        ".reg .pred p;\n\t"
+        "mbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+        "selp.u32 %0, 1, 0, p;\n\t"
+        "}\n"
+        : "=r"(done)
+        : "r"(bar_s), "r"(parity)
+        : "memory");
+    if (done) return true;
+  }
+  return kv16_wait(bar, parity, abort_flag);
 }
 // Asynchronous copy of 16 bytes, or of none: then the destination is zeroed.
 __device__ __forceinline__ void copy16(uint32_t dst, const uint8_t* src, bool live) {

@@ -1,11 +1,10 @@
-// Schedule of the attention kernels of the 16-bit paged cache.
+// What the attention kernels of the 16-bit paged cache share: the pieces they work in, and how keys get to shared memory.
 //
 // A request's query rows (a row is a query token and head of one KV head, token-major) are cut into row tiles of RP; a row tile
-// reads all KV tiles (128 keys) that the request sees.  The tiles of all (request, row tile) form one sequence, which
-// is cut into equal runs, one for every group of Hkv CTAs; CTA h of a group reads KV head h, so that the heads of a page
-// are read at the same time.  A row tile that a cut divides is computed in pieces by the CTAs of neighbouring groups;
-// they leave partial results in the workspace, a slot of the CTA for the piece that begins a row tile and one for the piece
-// that goes on with one, and count their arrivals on the counter of the CTA that holds the first piece.
+// reads all KV tiles (128 keys) that the request sees.  A row tile that the schedule divides is computed in pieces, runs of
+// its KV tiles, by several CTAs; they leave partial results in the workspace, each CTA in a slot for the piece that begins a
+// row tile or in one for a piece that goes on with one, and count their arrivals on a counter of the CTA that holds the
+// first piece.  The last to arrive merges them, in the pieces' order.
 #pragma once
 
 #include "kv16.cuh"
@@ -15,22 +14,16 @@ namespace {
 
 constexpr int kTile = 128;             // keys
 constexpr int kCounterBytes = 4096;    // arrival counters at the start of the workspace, one per CTA
-constexpr int kRunMin = 1;             // KV tiles a run holds at least
 
-// One piece of a request's row tile: keys [key0, key0 + 128 tiles) of those visible, [lo, hi).
+// One piece of a row tile: keys [key0, key0 + 128 tiles) of those visible, [lo, hi).
 struct Piece {
-  int r, row0, rows;          // rows row0 .. row0 + rows of the request's q_len x G
+  int r, kvh;
+  int row0, rows;             // rows row0 .. row0 + rows of the request's q_len x G
   int first_token;
   int key0, tiles, lo, hi;
   bool begins, ends;
   long long start;            // of the row tile in the sequence
-  int row_tiles_keys;         // KV tiles of the whole row tile
-};
-
-template <int RP>
-struct Walk {
-  long long at, end, start;   // position in the sequence, end of the run, start of request r
-  int r;
+  int row_tile_tiles;         // KV tiles of the whole row tile
 };
 
 struct ReqShape {
@@ -46,34 +39,22 @@ __device__ __forceinline__ ReqShape req_shape(const Kv16Params& p, int r) {
   s.tiles = s.hi > s.lo && rows > 0 ? (s.hi + kTile - 1) / kTile - s.lo / kTile : 0;
   return s;
 }
+// Fills a piece with KV tiles tile .. tile + count of row tile rt.
 template <int RP>
-__device__ __forceinline__ bool next_piece(const Kv16Params& p, Walk<RP>& w, Piece* out) {
-  if (w.at >= w.end) return false;
-  ReqShape s = req_shape<RP>(p, w.r);
-  long long n = (long long)s.tiles * s.row_tiles;
-  while (w.at >= w.start + n) {
-    w.start += n;
-    ++w.r;
-    s = req_shape<RP>(p, w.r);
-    n = (long long)s.tiles * s.row_tiles;
-  }
-  const long long off = w.at - w.start;
-  const int rt = s.row_tiles == 1 ? 0 : (int)(off / s.tiles);
-  const int tile = (int)(off - (long long)rt * s.tiles);
-  out->r = w.r;
+__device__ __forceinline__ void make_piece(const Kv16Params& p, const ReqShape& s, int r, int kvh, int rt, int tile, int count, long long start, Piece* out) {
+  out->r = r;
+  out->kvh = kvh;
   out->row0 = rt * RP;
   out->rows = min(RP, s.tokens * p.group - rt * RP);
   out->first_token = s.first;
   out->lo = s.lo;
   out->hi = s.hi;
   out->key0 = (s.lo / kTile + tile) * kTile;
-  out->tiles = (int)min((long long)(s.tiles - tile), w.end - w.at);
+  out->tiles = count;
   out->begins = tile == 0;
-  out->ends = tile + out->tiles == s.tiles;
-  out->start = w.start + (long long)rt * s.tiles;
-  out->row_tiles_keys = s.tiles;
-  w.at += out->tiles;
-  return true;
+  out->ends = tile + count == s.tiles;
+  out->start = start;
+  out->row_tile_tiles = s.tiles;
 }
 // Token and query head of a row of a request.
 __device__ __forceinline__ void row_of(const Kv16Params& p, int first_token, int kvh, int row, int* token, int* head) {
@@ -88,31 +69,11 @@ __device__ __forceinline__ float redux_max(float x) {
   return y;
 }
 
-// The run of a CTA, and what the pieces' owners are found with: tile x of the sequence belongs to group
-// ((x + 1) groups - 1) / work.
-template <int RP>
-struct Run {
-  Walk<RP> start;       // at == end: the CTA has none
-  long long work;       // tiles of the sequence
-  int groups, heads, hslot;
-  __device__ __forceinline__ int owner(long long x) const { return (int)(((x + 1) * groups - 1) / work); }
-};
-// Every CTA sums the tiles of all requests up for itself.  scratch: 64-bit words, warps + 2.  Ends with a CTA barrier in front
-// of which the first piece's request is written.
-template <int RP, int kThreads>
-__device__ __forceinline__ Run<RP> find_run(const Kv16Params& p, long long* scratch) {
-  constexpr int kWarps = kThreads / 32;
-  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-  Run<RP> run;
-  run.heads = min(p.num_kv_heads, (int)gridDim.x);   // KV heads that a group reads at the same time
-  run.hslot = (int)blockIdx.x % run.heads;
-  const int group = (int)blockIdx.x / run.heads;
-  const int per = (p.num_reqs + kThreads - 1) / kThreads, r0 = min(p.num_reqs, tid * per), r1 = min(p.num_reqs, r0 + per);
-  long long mine = 0;
-  for (int r = r0; r < r1; ++r) {
-    const ReqShape s = req_shape<RP>(p, r);
-    mine += (long long)s.tiles * s.row_tiles;
-  }
+// Sum of `mine` over the threads in front of this one, and over all of them.  scratch: a 64-bit word per warp, free again
+// behind the caller's next barrier.
+template <int kThreads>
+__device__ __forceinline__ long long scan_threads(long long mine, long long* scratch, long long* total) {
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   long long upto = mine;
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
@@ -122,32 +83,12 @@ __device__ __forceinline__ Run<RP> find_run(const Kv16Params& p, long long* scra
   if (lane == 31) scratch[warp] = upto;
   __syncthreads();
   long long before = upto - mine;
-  run.work = 0;
-  for (int w = 0; w < kWarps; ++w) {
+  *total = 0;
+  for (int w = 0; w < kThreads / 32; ++w) {
     if (w < warp) before += scratch[w];
-    run.work += scratch[w];
+    *total += scratch[w];
   }
-  const long long most = run.work / kRunMin > 0 ? run.work / kRunMin : 1;
-  run.groups = (int)min((long long)((int)gridDim.x / run.heads), most);
-  run.start.at = group < run.groups ? run.work * group / run.groups : 0;
-  run.start.end = group < run.groups ? run.work * (group + 1) / run.groups : 0;
-  if (run.start.at < run.start.end && before <= run.start.at && run.start.at < before + mine) {
-    long long start = before;
-    int r = r0;
-    for (;; ++r) {
-      const ReqShape s = req_shape<RP>(p, r);
-      const long long n = (long long)s.tiles * s.row_tiles;
-      if (run.start.at < start + n) break;
-      start += n;
-    }
-    scratch[kWarps] = r;
-    scratch[kWarps + 1] = start;
-  }
-  __syncthreads();
-  const bool works = run.start.at < run.start.end;
-  run.start.r = works ? (int)scratch[kWarps] : 0;
-  run.start.start = works ? scratch[kWarps + 1] : 0;
-  return run;
+  return before;
 }
 
 // Rows of requests without a visible key: zero, -inf.
@@ -165,20 +106,20 @@ __device__ __forceinline__ void zero_requests(const Kv16Params& p) {
   }
 }
 
-// Tiles of a run, one after the other, for the lane of a copying warp that looks key `key` of every tile up in the block
-// table.  The entry of the next tile is on its way while the copies of this one are issued.
-template <int RP>
+// The KV tiles of a CTA's pieces, one after the other, for the lane of a copying warp that looks key `key` of every tile up in
+// the block table.  The entry of the next tile is on its way while the copies of this one are issued.
+template <class Walk>
 struct KeyLookup {
   const Kv16Params& p;
-  Walk<RP> w;
+  Walk w;
   Piece it;            // of the tile looked up last
   int key, left = 0, key0 = 0, blk = -1, slot = 0;
   bool fresh = false;  // the tile is its piece's first
-  __device__ __forceinline__ KeyLookup(const Kv16Params& params, const Walk<RP>& walk, int lane_key) : p(params), w(walk), key(lane_key) {}
+  __device__ __forceinline__ KeyLookup(const Kv16Params& params, const Walk& walk, int lane_key) : p(params), w(walk), key(lane_key) {}
   __device__ __forceinline__ bool fetch() {
     fresh = left == 0;
     if (fresh) {
-      if (!next_piece<RP>(p, w, &it)) return false;
+      if (!w.next(p, &it)) return false;
       left = it.tiles;
       key0 = it.key0;
     } else {

@@ -22,9 +22,8 @@
 // copies 7.17, which also take pages of any size and place.
 //
 // Schedule: the KV tiles of all (request, row tile) form one sequence, which is cut into equal runs, one for every group of Hkv
-// CTAs; CTA h of a group reads head h, so the heads of a page are read at the same time.  A request that a cut divides
-// leaves partial (O, ref, l) of its pieces in the workspace, and the CTA that arrives last merges them in the pieces' order:
-// one launch, and the same bits whoever is last.
+// CTAs; CTA h of a group reads head h, so that the heads of a page are read at the same time.  The pieces of a row tile that
+// a cut divides are merged by the CTA that arrives last: one launch, and the same bits whoever is last.
 #include "kv16_sched.cuh"
 #include "page_copy.cuh"
 #include "pdl.cuh"
@@ -39,6 +38,7 @@ constexpr int kSoftmaxThreads = 128;   // warps 0-3: thread t is key t of a tile
 constexpr int kLoadWarp = 4;           // warps 4-7
 constexpr int kMmaWarp = 8;
 constexpr int kThreads = 288;
+constexpr int kRunMin = 1;             // KV tiles a run holds at least
 constexpr float kGain = 7.f, kSlack = 8.f;
 
 template <int HD, int RP>
@@ -76,6 +76,88 @@ struct Geo {
 struct Bars {  // offsets behind [units] full, [units] empty
   static constexpr int q_empty = 0, s_ready = 2, p_ready = 4, pv_done = 5;
 };
+
+// The run of a CTA: a walk over its pieces.
+template <int RP>
+struct ShortWalk {
+  long long at, end, start;   // position in the sequence, end of the run, start of request r
+  int r, kvh;
+  long long begin, first_start;   // where the run begins, for further KV heads
+  int first_r, heads;
+  __device__ __forceinline__ bool next(const Kv16Params& p, Piece* out) {
+    if (at >= end) {
+      kvh += heads;
+      if (begin >= end || kvh >= p.num_kv_heads) return false;
+      at = begin;
+      start = first_start;
+      r = first_r;
+    }
+    ReqShape s = req_shape<RP>(p, r);
+    long long n = (long long)s.tiles * s.row_tiles;
+    while (at >= start + n) {
+      start += n;
+      ++r;
+      s = req_shape<RP>(p, r);
+      n = (long long)s.tiles * s.row_tiles;
+    }
+    const long long off = at - start;
+    const int rt = s.row_tiles == 1 ? 0 : (int)(off / s.tiles), tile = (int)(off - (long long)rt * s.tiles);
+    const int count = (int)min((long long)(s.tiles - tile), end - at);
+    make_piece<RP>(p, s, r, kvh, rt, tile, count, start + (long long)rt * s.tiles, out);
+    at += count;
+    return true;
+  }
+};
+// What the pieces' owners are found with: tile x of the sequence belongs to group ((x + 1) groups - 1) / work.
+template <int RP>
+struct ShortRun {
+  ShortWalk<RP> walk;
+  long long work;       // tiles of the sequence
+  int groups, heads, hslot;
+  __device__ __forceinline__ int owner(long long x) const { return (int)(((x + 1) * groups - 1) / work); }
+};
+// Every CTA sums the tiles of all requests up for itself.  scratch: 64-bit words, warps + 2.  Ends with a CTA barrier.
+template <int RP, int kThreads>
+__device__ __forceinline__ ShortRun<RP> find_run(const Kv16Params& p, long long* scratch) {
+  constexpr int kWarps = kThreads / 32;
+  const int tid = threadIdx.x;
+  ShortRun<RP> run;
+  run.heads = min(p.num_kv_heads, (int)gridDim.x);   // KV heads that a group reads at the same time
+  run.hslot = (int)blockIdx.x % run.heads;
+  const int group = (int)blockIdx.x / run.heads;
+  const int per = (p.num_reqs + kThreads - 1) / kThreads, r0 = min(p.num_reqs, tid * per), r1 = min(p.num_reqs, r0 + per);
+  long long mine = 0;
+  for (int r = r0; r < r1; ++r) {
+    const ReqShape s = req_shape<RP>(p, r);
+    mine += (long long)s.tiles * s.row_tiles;
+  }
+  const long long before = scan_threads<kThreads>(mine, scratch, &run.work);
+  const long long most = run.work / kRunMin > 0 ? run.work / kRunMin : 1;
+  run.groups = (int)min((long long)((int)gridDim.x / run.heads), most);
+  ShortWalk<RP>& w = run.walk;
+  w.begin = group < run.groups ? run.work * group / run.groups : 0;
+  w.end = group < run.groups ? run.work * (group + 1) / run.groups : 0;
+  if (w.begin < w.end && before <= w.begin && w.begin < before + mine) {
+    long long start = before;
+    int r = r0;
+    for (;; ++r) {
+      const ReqShape s = req_shape<RP>(p, r);
+      const long long n = (long long)s.tiles * s.row_tiles;
+      if (w.begin < start + n) break;
+      start += n;
+    }
+    scratch[kWarps] = r;
+    scratch[kWarps + 1] = start;
+  }
+  __syncthreads();
+  const bool works = w.begin < w.end;
+  w.at = w.begin;
+  w.first_r = w.r = works ? (int)scratch[kWarps] : 0;
+  w.first_start = w.start = works ? scratch[kWarps + 1] : 0;
+  w.kvh = run.hslot;
+  w.heads = run.heads;
+  return run;
+}
 
 // Barrier of the softmax warps that tells whether any of them has seen `x`.
 __device__ __forceinline__ bool softmax_any(bool x) {
@@ -237,15 +319,13 @@ __global__ void __launch_bounds__(kThreads, (Geo<HD, RP>::ctas)) kv16_short_kern
   }
   pdl_wait();
 
-  const Run<RP> run = find_run<RP, kThreads>(p, reinterpret_cast<long long*>(smem + G::misc + 16));
+  const ShortRun<RP> run = find_run<RP, kThreads>(p, reinterpret_cast<long long*>(smem + G::misc + 16));
   zero_requests<HD, RP, kThreads>(p);
   tc::fence_before_sync();
   __syncthreads();
   tc::fence_after_sync();
   const uint32_t tmem_base = *tslot;
   const int heads = run.heads, hslot = run.hslot;
-  const bool works = run.start.at < run.start.end;
-  const Walk<RP> start = run.start;
   bool ok = true;
 
   if (warp >= kLoadWarp && warp < kMmaWarp) {
@@ -256,21 +336,23 @@ __global__ void __launch_bounds__(kThreads, (Geo<HD, RP>::ctas)) kv16_short_kern
     uint32_t unit = 0, item = 0;
     auto next_unit = [&]() -> uint32_t {
       const uint32_t s = unit % G::units;
-      if (unit >= G::units) ok &= wait_or_abort(&empty[s], ((unit / G::units) - 1) & 1, abort_flag);
+      if (unit >= G::units) ok &= kv16_wait(&empty[s], ((unit / G::units) - 1) & 1, abort_flag);
       ++unit;
       return s;
     };
-    for (int kvh = hslot; kvh < p.num_kv_heads && works; kvh += heads) {
-      const uint8_t* kb = p.k + (int64_t)kvh * p.stride_head;
-      const uint8_t* vb = p.v + (int64_t)kvh * p.stride_head;
-      KeyLookup<RP> keys(p, start, base_key + lane);
+    {
+      KeyLookup<ShortWalk<RP>> keys(p, run.walk, base_key + lane);
       bool have = keys.fetch(), have_v = false;
       long long off_v = 0;
+      int64_t head_v = 0;
       while (have || have_v) {
         const bool now = have;
         long long off = 0;
+        int64_t head_k = 0;
         if (now) {
           off = keys.offset();
+          const int kvh = keys.it.kvh;
+          head_k = (int64_t)kvh * p.stride_head;
           const bool first = keys.fresh;
           const int first_token = keys.it.first_token, row0 = keys.it.row0, rows = keys.it.rows;
           have = keys.fetch();
@@ -279,7 +361,7 @@ __global__ void __launch_bounds__(kThreads, (Geo<HD, RP>::ctas)) kv16_short_kern
             const uint32_t s = next_unit();
             if (part == 0 && first) {
               // the rows of Q come with the piece's first unit: chunk c of row n at c (RP 16) + n 16
-              if (item >= 2) ok &= wait_or_abort(&bars[Bars::q_empty + (item & 1)], ((item >> 1) - 1) & 1, abort_flag);
+              if (item >= 2) ok &= kv16_wait(&bars[Bars::q_empty + (item & 1)], ((item >> 1) - 1) & 1, abort_flag);
               const uint32_t dst = tc::smem_u32(smem + G::q) + (item & 1) * G::qimage;
               for (int i = tid - kLoadWarp * 32; i < RP * (HD / 8); i += 128) {
                 const int n = i / (HD / 8), c = i % (HD / 8);
@@ -289,7 +371,7 @@ __global__ void __launch_bounds__(kThreads, (Geo<HD, RP>::ctas)) kv16_short_kern
               }
               ++item;
             }
-            copy_keys<G::dims>(ring + s * G::unit, base_key, kb + part * 256, off);
+            copy_keys<G::dims>(ring + s * G::unit, base_key, p.k + head_k + part * 256, off);
             copies_arrive(&full[s]);
           }
         }
@@ -297,11 +379,12 @@ __global__ void __launch_bounds__(kThreads, (Geo<HD, RP>::ctas)) kv16_short_kern
 #pragma unroll
           for (int part = 0; part < G::parts; ++part) {
             const uint32_t s = next_unit();
-            copy_keys<G::dims>(ring + s * G::unit, base_key, vb + part * 256, off_v);
+            copy_keys<G::dims>(ring + s * G::unit, base_key, p.v + head_v + part * 256, off_v);
             copies_arrive(&full[s]);
           }
         }
         off_v = off;
+        head_v = head_k;
         have_v = now;
       }
     }
@@ -316,7 +399,7 @@ __global__ void __launch_bounds__(kThreads, (Geo<HD, RP>::ctas)) kv16_short_kern
     uint32_t unit = 0, tile = 0, item = 0;
     auto arrived = [&]() -> uint32_t {
       const uint32_t s = unit % G::units;
-      ok &= wait_or_abort(&full[s], (unit / G::units) & 1, abort_flag);
+      ok &= kv16_wait(&full[s], (unit / G::units) & 1, abort_flag);
       tc::fence_async_smem();   // (the copies wrote through the generic proxy)
       ++unit;
       return s;
@@ -346,7 +429,7 @@ __global__ void __launch_bounds__(kThreads, (Geo<HD, RP>::ctas)) kv16_short_kern
     };
     uint32_t pv_tile = 0;
     auto pv = [&](bool first_of_item) {
-      ok &= wait_or_abort(&bars[Bars::p_ready], pv_tile & 1, abort_flag);
+      ok &= kv16_wait(&bars[Bars::p_ready], pv_tile & 1, abort_flag);
 #pragma unroll
       for (int part = 0; part < G::parts; ++part) {
         const uint32_t s = arrived();
@@ -366,20 +449,18 @@ __global__ void __launch_bounds__(kThreads, (Geo<HD, RP>::ctas)) kv16_short_kern
       }
       ++pv_tile;
     };
-    for (int kvh = hslot; kvh < p.num_kv_heads && works; kvh += heads) {
-      Walk<RP> w = start;
-      Piece it;
-      bool pending = false, pending_first = false;
-      while (next_piece<RP>(p, w, &it)) {
-        for (int t = 0; t < it.tiles; ++t) {
-          qk(t == it.tiles - 1);
-          if (pending) pv(pending_first);
-          pending = true;
-          pending_first = t == 0;
-        }
+    ShortWalk<RP> w = run.walk;
+    Piece it;
+    bool pending = false, pending_first = false;
+    while (w.next(p, &it)) {
+      for (int t = 0; t < it.tiles; ++t) {
+        qk(t == it.tiles - 1);
+        if (pending) pv(pending_first);
+        pending = true;
+        pending_first = t == 0;
       }
-      if (pending) pv(pending_first);
     }
+    if (pending) pv(pending_first);
   } else if (warp < kLoadWarp) {
     // =========================== softmax =========================================
     const uint32_t lane_addr = (uint32_t)(warp * 32) << 16;
@@ -387,10 +468,11 @@ __global__ void __launch_bounds__(kThreads, (Geo<HD, RP>::ctas)) kv16_short_kern
     float* const wsum = reinterpret_cast<float*>(smem + G::wsum);
     uint8_t* const p_img = smem + G::p + tid * 16;
     uint32_t tile = 0;
-    for (int kvh = hslot; kvh < p.num_kv_heads && works; kvh += heads) {
-      Walk<RP> w = start;
+    {
+      ShortWalk<RP> w = run.walk;
       Piece it;
-      while (next_piece<RP>(p, w, &it)) {
+      while (w.next(p, &it)) {
+        const int kvh = it.kvh;
         float ref[RP], l[RP];
 #pragma unroll
         for (int n = 0; n < RP; ++n) {
@@ -398,7 +480,7 @@ __global__ void __launch_bounds__(kThreads, (Geo<HD, RP>::ctas)) kv16_short_kern
           l[n] = 0.f;
         }
         for (int t = 0; t < it.tiles; ++t, ++tile) {
-          ok &= wait_or_abort(&bars[Bars::s_ready + (tile & 1)], (tile >> 1) & 1, abort_flag);
+          ok &= kv16_wait(&bars[Bars::s_ready + (tile & 1)], (tile >> 1) & 1, abort_flag);
           tc::fence_after_sync();
           uint32_t sr[RP];
           tmem_load<RP>(tmem_base + G::s_col + (tile & 1) * G::cols + lane_addr, sr);
@@ -435,7 +517,7 @@ __global__ void __launch_bounds__(kThreads, (Geo<HD, RP>::ctas)) kv16_short_kern
               x[n] = fmaf(__uint_as_float(sr[n]), p.scale_log2, to == -INFINITY ? 0.f : -to);
             }
             if (t > 0 && moved) {   // (the same in all threads)
-              ok &= wait_or_abort(&bars[Bars::pv_done], (tile - 1) & 1, abort_flag);
+              ok &= kv16_wait(&bars[Bars::pv_done], (tile - 1) & 1, abort_flag);
               tc::fence_after_sync();
 #pragma unroll
               for (int part = 0; part < G::parts; ++part) {
@@ -462,7 +544,7 @@ __global__ void __launch_bounds__(kThreads, (Geo<HD, RP>::ctas)) kv16_short_kern
             l[n + 1] += b;
             split2<kHalf>(a, b, &hi[n / 2], &lo[n / 2]);
           }
-          if (tile > 0) ok &= wait_or_abort(&bars[Bars::pv_done], (tile - 1) & 1, abort_flag);  // (P of the last tile has been read)
+          if (tile > 0) ok &= kv16_wait(&bars[Bars::pv_done], (tile - 1) & 1, abort_flag);  // (P of the last tile has been read)
 #pragma unroll
           for (int j = 0; j < RP / 8; ++j) {
             *reinterpret_cast<uint4*>(p_img + j * (kTile * 16)) = make_uint4(hi[4 * j], hi[4 * j + 1], hi[4 * j + 2], hi[4 * j + 3]);
@@ -485,7 +567,7 @@ __global__ void __launch_bounds__(kThreads, (Geo<HD, RP>::ctas)) kv16_short_kern
         softmax_sync();
 #pragma unroll
         for (int n = 0; n < RP; ++n) l[n] = (wsum[n] + wsum[RP + n]) + (wsum[2 * RP + n] + wsum[3 * RP + n]);
-        ok &= wait_or_abort(&bars[Bars::pv_done], (tile - 1) & 1, abort_flag);
+        ok &= kv16_wait(&bars[Bars::pv_done], (tile - 1) & 1, abort_flag);
         tc::fence_after_sync();
         const bool whole = it.begins && it.ends;
         float* const slot = partial_slot<HD, RP>(p, (int)blockIdx.x, it.begins);
@@ -530,7 +612,7 @@ __global__ void __launch_bounds__(kThreads, (Geo<HD, RP>::ctas)) kv16_short_kern
           }
         }
         if (!whole) {
-          const int g0 = run.owner(it.start), g1 = run.owner(it.start + it.row_tiles_keys - 1);
+          const int g0 = run.owner(it.start), g1 = run.owner(it.start + it.row_tile_tiles - 1);
           __threadfence();
           softmax_sync();
           int* const counter = reinterpret_cast<int*>(p.workspace) + g0 * heads + hslot;

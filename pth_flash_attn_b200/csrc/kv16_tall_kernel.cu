@@ -7,16 +7,33 @@
 // works on one row tile while the other's softmax runs; at 256 dims, where O alone takes half of TMEM, 128 rows with
 // two S buffers, which do the same for two tiles of keys.
 //
-// Softmax: ref is a running bound of the row's scores (log2 units) that moves, with l and O rescaled, only when the largest
-// score of a tile outgrows it by kSlack; P = 2^(s - ref) is rounded to the cache's type for the MMA (the error of the output
-// is sqrt(2) times that of its own rounding), its sum l is not.  P lands in two halves of 64 keys, each of
-// which the MMA takes as soon as it is complete.
+// Softmax in one pass: ref is a running bound of a row's scores (log2 units), P = 2^(s - ref), l = sum P.  It is set kGain below the
+// maximum of a row's first 64 keys.  Later ones need no maximum: the sum of 64 P, which the row sum takes anyway, says
+// whether one of them has outgrown ref too far (kMostSum); then ref moves to their maximum, O and l are rescaled and the
+// 64 are computed again.  P is rounded to the cache's type for the MMA (the error of the output is sqrt(2) times that
+// of its own rounding), its sum is not.  The steps are of 64 keys (128 at 256 dims) with two S buffers,
+// so that a step's QK and the last one's PV run beside its softmax.
 //
-// One warp issues the MMAs.  The two row tiles are two programs (QK of tile i, PV of tile i in halves, ...) that it polls in
-// turn: whichever has its operands goes next, so neither waits for the other, and nothing relies on the order in which MMAs on
+// What bounds it: the special function unit, which takes 8 cycles for a warp's 32 exponentials, 2,048 for the two row tiles' scores
+// of 128 keys (with the conversions beside them 2,460, measured on their own), and the MMAs, about 2,700 with QK in steps of
+// 64 keys (both operands from shared memory, which that takes 1.5 times as often).  4 x 2,048 tokens over 8,192 states, 32 heads
+// of 8, 128 dims, bf16: 977 us, 1,126 TFLOP/s.  (Steps of 128 keys with one S buffer, a row tile waiting for its MMAs: 1,241; an
+// eighth of the exponentials as a polynomial on the FMA pipe 981, a quarter 1,045; the row tiles' exponentials in turn no faster.)
+//
+// A warp per row tile issues its MMAs, so neither row tile waits for the other, and nothing relies on the order in which MMAs on
 // different accumulators run.
 //
-// Copies, schedule and merging of pieces: kv16_sched.cuh, as for the short kernel; a CTA per SM.
+// Copies: tiles that are visible as a whole come as boxes (tiled TMA, 64 dims of up to 32 slots of a page) where pages are a
+// multiple of 8 slots, others as 16-byte copies, which zero what is not visible.  (All by 16-byte copies: 1,300 cycles a
+// unit of 32 KB, more than the MMAs take.)
+//
+// Schedule: items (row tile, KV head, request), in the order request, head, row tile, so that neighbouring items read the same keys.
+// While the keys of a launch fit in the L2 cache, the sequence of all their KV tiles is cut into equal runs, one per CTA.
+// Otherwise all but the last one or two items per CTA go out in waves, CTA c taking items c, c + CTAs, ...: the CTAs then work
+// on the same few heads of one request at a time.  (Equal runs had them all over 268 MB of keys: 4 x 2,048 tokens over
+// 8,192 states drew 5.5 TB/s from memory and took 1,552 us.)  The tiles of the rest make up for unequal waves.
+#include <mutex>
+
 #include "kv16_sched.cuh"
 #include "page_copy.cuh"
 #include "pdl.cuh"
@@ -28,14 +45,20 @@ __device__ unsigned int g_kv16_tall_status = 0;
 
 namespace {
 
-constexpr float kGain = 7.f, kSlack = 8.f;
+constexpr float kGain = 7.f;
+constexpr float kMostSum = 32768.f;    // of 64 P: none of them leaves fp16's range
 constexpr int kLoadWarps = 4;
+constexpr int kTallReqs = 8192;        // requests of a launch (the API refuses more)
+constexpr int kTallCtas = 160;
+constexpr long long kL2Keys = 48 << 20;   // bytes of keys and values that a launch may spread its CTAs over
 
 template <int HD>
 struct Tall {
   static constexpr int rts = HD == 256 ? 1 : 2;      // row tiles of 128 rows
   static constexpr int rows = 128 * rts;
-  static constexpr int bufs = HD == 256 ? 2 : 1;     // S buffers of a row tile
+  static constexpr int keys = HD == 256 ? 128 : 64;  // of a step, one of the two S buffers of a row tile
+  static constexpr int steps = kTile / keys;         // of a KV tile
+  static constexpr int halves = keys / 64;           // of a step: P is handed over 64 keys at a time
   static constexpr int dims = HD < 128 ? HD : 128;   // of a unit
   static constexpr int parts = HD / dims;
   static constexpr int unit = kTile * dims * 2;
@@ -43,43 +66,30 @@ struct Tall {
   static constexpr int units = HD == 64 ? 8 : 5;
   static constexpr int softmax_warps = 4 * rts;
   static constexpr int load_warp = softmax_warps, mma_warp = load_warp + kLoadWarps;
-  static constexpr int threads = (mma_warp + 1) * 32;
-  // Registers: 13 warps start with 128 each (9 with 168), which setmaxnreg moves from the copies to the softmax.
+  static constexpr int threads = (mma_warp + rts) * 32;   // (an MMA warp per row tile)
+  // Registers: 14 warps start with 128 each (9 with 168), which setmaxnreg moves from the copies to the softmax.
   static constexpr int start_regs = HD == 256 ? 168 : 128, copy_regs = HD == 256 ? 72 : 56, softmax_regs = HD == 256 ? 232 : 160;
-  static_assert(softmax_warps * softmax_regs + kLoadWarps * copy_regs + start_regs <= (threads / 32) * start_regs, "a split that the launch holds");
-  static constexpr int s_col = 0, o_col = 256;       // S(rt, b) at 128 (rt + b), O(rt) at 256 + rt HD
+  static_assert(softmax_warps * softmax_regs + kLoadWarps * copy_regs + rts * start_regs <= (threads / 32) * start_regs, "a split that the launch holds");
+  static constexpr int s_col = 0, o_col = 256;       // S(rt, b) at (2 rt + b) keys, O(rt) at 256 + rt HD
   // shared memory, behind the first 1,024-byte boundary
   static constexpr int q = units * unit;
   static constexpr int bars = q + rts * qtile;
-  static constexpr int n_bars = 2 * units + 2 * rts + 4 * 2 + 2;
+  static constexpr int n_bars = 2 * units + 2 * rts + 20;
   static constexpr int misc = bars + n_bars * 8;
-  static constexpr int total = misc + 256 + 1024;
+  static constexpr int bounds = misc + 256;          // TallPlan's
+  static constexpr int total = bounds + (kTallCtas + 1) * 8 + 1024;
+  static_assert(kTallReqs * 16 + 16 <= units * unit + rts * qtile, "the plan's arrays lie where keys and queries come later");
   static_assert(total <= 232448, "shared memory of one CTA");
 };
 template <int HD>
 struct TallBars {  // behind [units] full, [units] empty
   static constexpr int q_full = 0, q_empty = Tall<HD>::rts;
-  static constexpr int s_ready = 2 * Tall<HD>::rts;  // [2] S buffer (rt + b)
-  static constexpr int p_ready = s_ready + 2;        // [2][2 halves]
-  static constexpr int pv_done = p_ready + 4;        // [2]
+  static constexpr int s_ready = 2 * Tall<HD>::rts;  // [4] S buffer 2 rt + b
+  static constexpr int p_ready = s_ready + 4;        // [4][2 halves]
+  static constexpr int pv_half = p_ready + 8;        // [4] PV of the first of two halves
+  static constexpr int pv_done = pv_half + 4;        // [4]
 };
 
-__device__ __forceinline__ bool test_wait(uint64_t* bar, uint32_t parity) {
-  uint32_t ok;
-  asm volatile(
-      "{\n\t"
-      ".reg .pred p;\n\t"
-      "mbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
-      "selp.u32 %0, 1, 0, p;\n\t"
-      "}\n"
-      : "=r"(ok)
-      : "r"(tc::smem_u32(bar)), "r"(parity)
-      : "memory");
-  return ok != 0;
-}
-__device__ __forceinline__ void mma_ts(uint32_t d_tmem, uint32_t a_tmem, uint64_t b_desc, uint32_t idesc, bool accumulate) {
-  mma_ts_words(d_tmem, a_tmem, (uint32_t)b_desc, (uint32_t)(b_desc >> 32), idesc, accumulate);
-}
 template <bool kHalf>
 __device__ __forceinline__ uint32_t pack16(float a, float b) {
   if constexpr (kHalf) {
@@ -91,14 +101,227 @@ __device__ __forceinline__ uint32_t pack16(float a, float b) {
   }
 }
 
+// Tiled TMA load of one box of a rank-4 tensor map into shared memory.
+__device__ __forceinline__ void tma_load_4d(uint32_t dst, const CUtensorMap* map, int x, int y, int z, int w, uint64_t* bar) {
+  asm volatile(
+      "cp.async.bulk.tensor.4d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5}], [%6];" ::"r"(dst),
+      "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(z), "r"(w), "r"(tc::smem_u32(bar))
+      : "memory");
+}
+
 template <int HD>
 __device__ __forceinline__ float* tall_slot(const Kv16Params& p, int cta, bool begins) {
   // [HD][rows] O, [rows] ref, [rows] l
   return reinterpret_cast<float*>(p.workspace + kCounterBytes) + (int64_t)(2 * cta + (begins ? 1 : 0)) * (Tall<HD>::rows * (HD + 2));
 }
 
+// P of 64 scores as pairs of 16-bit numbers, 2^(score scale + minus_ref); returns the sum of the unrounded ones.
+template <bool kHalf>
+__device__ __forceinline__ float exponentials(const uint32_t (&r)[64], float scale, float minus_ref, uint32_t (&pk)[32]) {
+  const f32x2 scale2 = pair(scale, scale), ref2 = pair(minus_ref, minus_ref);
+  f32x2 sum[2] = {0ull, 0ull};
+#pragma unroll
+  for (int n = 0; n < 32; ++n) {
+    float x, y;
+    unpair(fma2(pair(__uint_as_float(r[2 * n]), __uint_as_float(r[2 * n + 1])), scale2, ref2), x, y);
+    x = ex2f(x);
+    y = ex2f(y);
+    sum[n & 1] = add2(sum[n & 1], pair(x, y));
+    pk[n] = pack16<kHalf>(x, y);
+  }
+  return sum_pairs(sum);
+}
+
+// Steps of a piece: its keys from key0 on, as far as they are visible.
+template <int kKeys>
+__device__ __forceinline__ int piece_steps(const Piece& it) {
+  return (min(it.tiles * kTile, it.hi - it.key0) + kKeys - 1) / kKeys;
+}
+
+// Walk over the pieces of a CTA: its items of the waves, then its run of the tail.
+template <int RP>
+struct TallWalk {
+  int wave, waves, ctas, item;    // item: of the current wave
+  int r, first_item;              // request of the item, items in front of it
+  long long at, end;              // the run, in tiles of the whole sequence
+  int tail_r;
+  long long tail_start;           // of request tail_r in the sequence
+  __device__ __forceinline__ bool next(const Kv16Params& p, Piece* out) {
+    if (wave < waves) {
+      ReqShape s = req_shape<RP>(p, r);
+      int n = s.tiles > 0 ? s.row_tiles * p.num_kv_heads : 0;
+      while (item >= first_item + n) {
+        first_item += n;
+        ++r;
+        s = req_shape<RP>(p, r);
+        n = s.tiles > 0 ? s.row_tiles * p.num_kv_heads : 0;
+      }
+      const int off = item - first_item, kvh = (int)((uint32_t)off / (uint32_t)s.row_tiles);
+      make_piece<RP>(p, s, r, kvh, off - kvh * s.row_tiles, 0, s.tiles, 0, out);
+      ++wave;
+      item += ctas;
+      return true;
+    }
+    if (at >= end) return false;
+    ReqShape s = req_shape<RP>(p, tail_r);
+    long long n = (long long)s.tiles * s.row_tiles * p.num_kv_heads;
+    while (at >= tail_start + n) {
+      tail_start += n;
+      ++tail_r;
+      s = req_shape<RP>(p, tail_r);
+      n = (long long)s.tiles * s.row_tiles * p.num_kv_heads;
+    }
+    const long long off = at - tail_start;
+    const int it = (int)(off / s.tiles), tile = (int)(off - (long long)it * s.tiles);
+    const int kvh = (int)((uint32_t)it / (uint32_t)s.row_tiles);
+    const int count = (int)min((long long)(s.tiles - tile), end - at);
+    make_piece<RP>(p, s, tail_r, kvh, it - kvh * s.row_tiles, tile, count, tail_start + (long long)it * s.tiles, out);
+    at += count;
+    return true;
+  }
+};
+
+// Who has which items (see the head of this file).  Every CTA works it out for itself.  Requests: tile_first[r] KV tiles and
+// item_first[r] items lie in front of r, whose items have tiles[r] KV tiles.  arrays: room for them; bounds [CTAs + 1]: where
+// the runs begin, behind tile `base` of the sequence.
+template <int HD, int RP, int kThreads>
+__device__ __forceinline__ TallWalk<RP> make_plan(const Kv16Params& p, uint8_t* arrays, long long* bounds, long long* scratch, long long* base) {
+  const int R = p.num_reqs, C = (int)gridDim.x, tid = threadIdx.x, lane = tid & 31;
+  long long* const tile_first = reinterpret_cast<long long*>(arrays);
+  int* const item_first = reinterpret_cast<int*>(tile_first + R + 1);
+  int* const tiles = item_first + R + 1;
+  const int per = (R + kThreads - 1) / kThreads, r0 = min(R, tid * per), r1 = min(R, r0 + per);
+  long long my_items = 0, my_tiles = 0, my_keys = 0;
+  for (int r = r0; r < r1; ++r) {
+    const ReqShape s = req_shape<RP>(p, r);
+    const int n = s.tiles > 0 ? s.row_tiles * p.num_kv_heads : 0;
+    tiles[r] = s.tiles;
+    my_items += n;
+    my_tiles += (long long)n * s.tiles;
+    my_keys += s.tiles;
+  }
+  long long items, total, keys;
+  long long ib = scan_threads<kThreads>(my_items, scratch, &items);
+  __syncthreads();
+  long long tb = scan_threads<kThreads>(my_tiles, scratch, &total);
+  __syncthreads();
+  scan_threads<kThreads>(my_keys, scratch, &keys);
+  for (int r = r0; r < r1; ++r) {
+    const ReqShape s = req_shape<RP>(p, r);
+    const int n = s.tiles > 0 ? s.row_tiles * p.num_kv_heads : 0;
+    item_first[r] = (int)ib;
+    tile_first[r] = tb;
+    ib += n;
+    tb += (long long)n * s.tiles;
+  }
+  if (tid == 0) {
+    item_first[R] = (int)items;
+    tile_first[R] = total;
+  }
+  __syncthreads();
+  // request of an item, or of a tile of the sequence: the last that begins at or in front of it
+  auto of_item = [&](long long x) {
+    int lo = 0, hi = R - 1;
+    while (lo < hi) {
+      const int mid = (lo + hi + 1) >> 1;
+      if (item_first[mid] <= x) lo = mid; else hi = mid - 1;
+    }
+    return lo;
+  };
+  auto of_tile = [&](long long x) {
+    int lo = 0, hi = R - 1;
+    while (lo < hi) {
+      const int mid = (lo + hi + 1) >> 1;
+      if (tile_first[mid] <= x) lo = mid; else hi = mid - 1;
+    }
+    return lo;
+  };
+  const long long bytes = keys * p.num_kv_heads * ((long long)kTile * HD * 4);
+  const int waves = bytes > kL2Keys && items >= 2 * C ? (int)(items / C) - 1 : 0;
+  long long first_tail = 0;   // tile of the sequence
+  if (waves > 0) {
+    const long long f = (long long)waves * C;
+    const int r = of_item(f);
+    first_tail = tile_first[r] + (f - item_first[r]) * tiles[r];
+  }
+  const long long tail = total - first_tail;
+  if (waves == 0) {
+    const long long runs = min((long long)C, max(tail, 1ll));   // (none of them empty)
+    for (int c = tid; c <= C; c += kThreads) bounds[c] = c < runs ? tail * c / runs : tail;
+  } else {
+    // CTA c has load(c) tiles of the waves; the tail fills all up to a level: the smallest that holds it
+    for (int c = tid; c < C; c += kThreads) {
+      long long load = 0;
+      for (int w = 0; w < waves; ++w) load += tiles[of_item(c + (long long)w * C)];
+      bounds[c] = load;
+    }
+    __syncthreads();
+    if (tid < 32) {
+      long long load[kTallCtas / 32], most = 0;
+#pragma unroll
+      for (int i = 0; i < kTallCtas / 32; ++i) {
+        load[i] = lane + 32 * i < C ? bounds[lane + 32 * i] : (1ll << 60);
+        if (load[i] < (1ll << 60)) most = max(most, load[i]);
+      }
+#pragma unroll
+      for (int o = 16; o > 0; o >>= 1) most = max(most, __shfl_xor_sync(0xffffffffu, most, o));
+      long long lo = total / C, hi = most + tail / C + 1;   // (at lo there may be too little room, at hi there is enough)
+      while (lo < hi) {
+        const long long mid = (lo + hi) >> 1;
+        long long room = 0;
+#pragma unroll
+        for (int i = 0; i < kTallCtas / 32; ++i) room += max(0ll, mid - load[i]);
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) room += __shfl_xor_sync(0xffffffffu, room, o);
+        if (room >= tail) hi = mid; else lo = mid + 1;
+      }
+      // (CTAs in order: lane + 32 i, a row of lanes at a time)
+      long long upto = 0;
+#pragma unroll
+      for (int i = 0; i < kTallCtas / 32; ++i) {
+        const long long mine = max(0ll, lo - load[i]);
+        long long inc = mine;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+          const long long x = __shfl_up_sync(0xffffffffu, inc, o);
+          if (lane >= o) inc += x;
+        }
+        if (lane + 32 * i < C) bounds[lane + 32 * i] = min(tail, upto + inc - mine);
+        upto += __shfl_sync(0xffffffffu, inc, 31);
+      }
+      if (lane == 0) bounds[C] = tail;
+    }
+  }
+  __syncthreads();
+  TallWalk<RP> w;
+  w.wave = 0;
+  w.waves = waves;
+  w.ctas = C;
+  w.item = (int)blockIdx.x;
+  w.r = of_item(w.item);
+  w.first_item = R > 0 ? item_first[w.r] : 0;
+  w.at = first_tail + bounds[blockIdx.x];
+  w.end = first_tail + bounds[blockIdx.x + 1];
+  w.tail_r = of_tile(w.at);
+  w.tail_start = tile_first[w.tail_r];
+  *base = first_tail;
+  tc::fence_async_smem();   // (boxes are written where the arrays are, through the other proxy)
+  __syncthreads();
+  return w;
+}
+// CTA that has tile x of the sequence in its run.
+__device__ __forceinline__ int tall_owner(const long long* bounds, int ctas, long long x) {
+  int lo = 0, hi = ctas - 1;
+  while (lo < hi) {
+    const int mid = (lo + hi + 1) >> 1;
+    if (bounds[mid] <= x) lo = mid; else hi = mid - 1;
+  }
+  return lo;
+}
+
 template <int HD, bool kHalf>
-__global__ void __launch_bounds__(Tall<HD>::threads, 1) kv16_tall_kernel(const __grid_constant__ Kv16Params p) {
+__global__ void __launch_bounds__(Tall<HD>::threads, 1) kv16_tall_kernel(const __grid_constant__ Kv16Params p, const __grid_constant__ CUtensorMap k_map,
+                                                                        const __grid_constant__ CUtensorMap v_map) {
   using G = Tall<HD>;
   using B = TallBars<HD>;
   constexpr int RP = G::rows;
@@ -122,10 +345,11 @@ __global__ void __launch_bounds__(Tall<HD>::threads, 1) kv16_tall_kernel(const _
         tc::mbar_init(&bars[B::q_full + i], 32 * kLoadWarps);
         tc::mbar_init(&bars[B::q_empty + i], 1);
       }
-      for (int i = 0; i < 2; ++i) {
+      for (int i = 0; i < 4; ++i) {
         tc::mbar_init(&bars[B::s_ready + i], 1);
         tc::mbar_init(&bars[B::p_ready + 2 * i], 128);
         tc::mbar_init(&bars[B::p_ready + 2 * i + 1], 128);
+        tc::mbar_init(&bars[B::pv_half + i], 1);
         tc::mbar_init(&bars[B::pv_done + i], 1);
       }
       *abort_flag = 0;
@@ -136,14 +360,14 @@ __global__ void __launch_bounds__(Tall<HD>::threads, 1) kv16_tall_kernel(const _
     tc::tmem_relinquish();
   }
   pdl_wait();
-  const Run<RP> run = find_run<RP, G::threads>(p, reinterpret_cast<long long*>(smem + G::misc + 16));
+  long long* const bounds = reinterpret_cast<long long*>(smem + G::bounds);
+  long long base;
+  const TallWalk<RP> walk = make_plan<HD, RP, G::threads>(p, smem, bounds, reinterpret_cast<long long*>(smem + G::misc + 16), &base);
   zero_requests<HD, RP, G::threads>(p);
   tc::fence_before_sync();
   __syncthreads();
   tc::fence_after_sync();
   const uint32_t tmem_base = *tslot;
-  const int heads = run.heads, hslot = run.hslot;
-  const bool works = run.start.at < run.start.end;
   bool ok = true;
 
   if (warp >= G::load_warp && warp < G::mma_warp) {
@@ -155,31 +379,49 @@ __global__ void __launch_bounds__(Tall<HD>::threads, 1) kv16_tall_kernel(const _
     uint32_t q_count[G::rts];
 #pragma unroll
     for (int i = 0; i < G::rts; ++i) q_count[i] = 0;
-    auto load_unit = [&](const uint8_t* src, long long off) {
+    // A unit: boxes of box_slots slots x 64 dims where pages allow it and the tile is visible as a whole, else 16-byte
+    // copies, which leave out what is not visible.
+    const int boxes = p.box_slots > 0 ? 32 / p.box_slots : 0;   // of this warp's keys
+    const int box_lane = boxes > 0 ? (lane % boxes) * p.box_slots : 0;
+    const bool boxing = lane < boxes * (G::dims / 64);
+    auto load_unit = [&](const CUtensorMap& map, const uint8_t* src, int part, int kvh, bool as_boxes, long long off, int blk, int slot) {
       const uint32_t s = unit % G::units;
-      if (unit >= G::units) ok &= wait_or_abort(&empty[s], ((unit / G::units) - 1) & 1, abort_flag);
-      copy_keys<G::dims>(ring + s * G::unit, base_key, src, off);
-      copies_arrive(&full[s]);
+      if (unit >= G::units) ok &= kv16_wait(&empty[s], ((unit / G::units) - 1) & 1, abort_flag);
+      if (as_boxes) {
+        if (boxing) {
+          const int slab = lane / boxes;
+          mbar_arrive_expect_tx(&full[s], p.box_slots * 128);
+          tma_load_4d(ring + s * G::unit + slab * (kTile * 128) + (base_key + box_lane) * 128, &map, part * 128 + slab * 64, kvh, slot, blk, &full[s]);
+        } else {
+          mbar_arrive(&full[s]);
+        }
+        __syncwarp();
+      } else {
+        copy_keys<G::dims>(ring + s * G::unit, base_key, src + part * 256, off);
+        copies_arrive(&full[s]);
+      }
       ++unit;
     };
-    for (int kvh = hslot; kvh < p.num_kv_heads && works; kvh += heads) {
-      const uint8_t* kb = p.k + (int64_t)kvh * p.stride_head;
-      const uint8_t* vb = p.v + (int64_t)kvh * p.stride_head;
-      KeyLookup<RP> keys(p, run.start, base_key + lane);
+    {
+      KeyLookup<TallWalk<RP>> keys(p, walk, base_key + lane);
       bool have = keys.fetch();
       while (have) {
+        const int kvh = keys.it.kvh;
+        const uint8_t* kb = p.k + (int64_t)kvh * p.stride_head;
+        const uint8_t* vb = p.v + (int64_t)kvh * p.stride_head;
         const long long off = keys.offset();
-        const bool first = keys.fresh;
+        const bool first = keys.fresh, as_boxes = boxes > 0 && keys.key0 >= keys.it.lo && keys.key0 + kTile <= keys.it.hi;
         const int first_token = keys.it.first_token, row0 = keys.it.row0, rows = keys.it.rows;
+        const int blk = __shfl_sync(0xffffffffu, keys.blk, box_lane), slot = __shfl_sync(0xffffffffu, keys.slot, box_lane);
         have = keys.fetch();
 #pragma unroll
-        for (int part = 0; part < G::parts; ++part) load_unit(kb + part * 256, off);
+        for (int part = 0; part < G::parts; ++part) load_unit(k_map, kb, part, kvh, as_boxes, off, blk, slot);
         if (first) {
           // the piece's queries, behind its first keys: a row tile's as soon as QK has read the last one's
 #pragma unroll
           for (int rt = 0; rt < G::rts; ++rt) {
             if (rows <= rt * 128) continue;
-            if (q_count[rt] > 0) ok &= wait_or_abort(&bars[B::q_empty + rt], (q_count[rt] - 1) & 1, abort_flag);
+            if (q_count[rt] > 0) ok &= kv16_wait(&bars[B::q_empty + rt], (q_count[rt] - 1) & 1, abort_flag);
             ++q_count[rt];
             // a lane looks a row up, the warp copies it
             const int mine = rt * 128 + base_key + lane;
@@ -193,158 +435,103 @@ __global__ void __launch_bounds__(Tall<HD>::threads, 1) kv16_tall_kernel(const _
           }
         }
 #pragma unroll
-        for (int part = 0; part < G::parts; ++part) load_unit(vb + part * 256, off);
+        for (int part = 0; part < G::parts; ++part) load_unit(v_map, vb, part, kvh, as_boxes, off, blk, slot);
       }
     }
     copies_wait_all();
-  } else if (warp == G::mma_warp) {
+  } else if (warp >= G::mma_warp) {
     // =========================== MMAs ============================================
+    const int rt = warp - G::mma_warp;
     constexpr uint32_t fmt = kHalf ? tc::kFmtF16 : tc::kFmtBF16;
-    constexpr uint32_t qk_desc = tc::instr_desc(128, 128, fmt, fmt, 0, 0);
+    constexpr uint32_t qk_desc = tc::instr_desc(128, G::keys, fmt, fmt, 0, 0);
     constexpr uint32_t pv_desc = tc::instr_desc(128, G::dims, fmt, fmt, 0, 1);
-    const uint32_t ring = tc::smem_u32(smem), q_s = tc::smem_u32(smem + G::q);
-    // A row tile's program over the pieces of this CTA's run.
-    struct Program {
-      Walk<RP> w;
-      Piece it;
-      int kvh, qk, pv, half, tiles;   // next QK and PV of the piece
-      bool done, live;
-      uint32_t tile0;                 // of the piece in the order of all tiles of the CTA (units of the ring)
-      uint32_t s_qk, s_pv;            // live tiles so far: use of the S buffers
-      uint32_t q_used;
+    // (descriptors as two words, of which a step along an operand changes the lower one)
+    const uint64_t q_desc = swizzled_desc(tc::smem_u32(smem + G::q) + rt * G::qtile, 16, 1024);
+    const uint64_t k_desc = swizzled_desc(tc::smem_u32(smem), 16, 1024);
+    const uint64_t v_desc = swizzled_desc(tc::smem_u32(smem), kTile * 128, 1024);
+    const uint32_t o_tmem = tmem_base + G::o_col + rt * HD, s_tmem = tmem_base + G::s_col + 2 * rt * G::keys;
+    uint32_t unit = 0;                       // of the piece's next tile, in the order of all units of the CTA
+    uint32_t s_qk = 0, s_pv = 0, pieces = 0; // steps so far, pieces with live rows
+    auto arrived = [&](uint32_t u) -> uint32_t {
+      const uint32_t s = u % G::units;
+      ok &= kv16_wait(&full[s], (u / G::units) & 1, abort_flag);
+      return s;
     };
-    Program prog[G::rts];
-#pragma unroll
-    for (int rt = 0; rt < G::rts; ++rt) {
-      prog[rt].w = run.start;
-      prog[rt].kvh = hslot;
-      prog[rt].qk = prog[rt].pv = prog[rt].half = prog[rt].tiles = 0;
-      prog[rt].done = !works;
-      prog[rt].live = false;
-      prog[rt].tile0 = prog[rt].s_qk = prog[rt].s_pv = prog[rt].q_used = 0;
-    }
-    auto landed = [&](uint32_t u) { return test_wait(&full[u % G::units], (u / G::units) & 1); };
-    // (a row tile without rows frees the units as if it had read them)
-    auto pass = [&](uint32_t u) {
-      if (elect_one()) {
-        for (int part = 0; part < G::parts; ++part) mbar_arrive(&empty[(u + part) % G::units]);
-      }
-      __syncwarp();
-    };
-    auto try_qk = [&](Program& g, int rt) -> bool {
-      const uint32_t u = (g.tile0 + g.qk) * 2 * G::parts;
-      const uint32_t b = rt + g.s_qk % G::bufs, use = g.s_qk / G::bufs;
-      if (g.live && g.qk == 0 && !test_wait(&bars[B::q_full + rt], g.q_used & 1)) return false;
-      if (g.live && use > 0 && !test_wait(&bars[B::pv_done + b], (use - 1) & 1)) return false;
+    // step `sub` of the KV tile whose units begin at u; frees them where it is the tile's last
+    auto qk = [&](uint32_t u, int sub, bool tile_ends, bool first, bool last) {
+      const uint32_t b = s_qk & 1, use = s_qk >> 1;
+      if (first) ok &= kv16_wait(&bars[B::q_full + rt], (pieces - 1) & 1, abort_flag);
+      if (use > 0) ok &= kv16_wait(&bars[B::pv_done + 2 * rt + b], (use - 1) & 1, abort_flag);   // (P of that use has been read)
 #pragma unroll
       for (int part = 0; part < G::parts; ++part) {
-        if (!landed(u + part)) return false;
-      }
-      if (!g.live) {
-        pass(u);
-        ++g.qk;
-        return true;
-      }
-      tc::fence_async_smem();   // (the copies wrote through the generic proxy)
-      if (elect_one()) {
-        tc::fence_after_sync();
-#pragma unroll
-        for (int part = 0; part < G::parts; ++part) {
-          const uint32_t s = (u + part) % G::units;
+        const uint32_t s = arrived(u + part);
+        tc::fence_async_smem();   // (copies wrote through the generic proxy)
+        if (elect_one()) {
+          tc::fence_after_sync();
+          const uint32_t klo = (uint32_t)k_desc + s * (G::unit >> 4) + sub * ((G::keys * 128) >> 4), qlo = (uint32_t)q_desc + part * ((2 * kTile * 128) >> 4);
 #pragma unroll
           for (int kk = 0; kk < G::dims / 16; ++kk) {
-            const uint32_t at = (kk >> 2) * (kTile * 128) + (kk & 3) * 32;
-            tc::mma_ss(tmem_base + G::s_col + b * 128, swizzled_desc(q_s + rt * G::qtile + part * (2 * kTile * 128) + at, 16, 1024),
-                       swizzled_desc(ring + s * G::unit + at, 16, 1024), qk_desc, part > 0 || kk > 0);
+            constexpr uint32_t slab = (kTile * 128) >> 4;
+            const uint32_t at = (kk >> 2) * slab + (kk & 3) * 2;
+            if (part == 0 && kk == 0) mma_ss_words<false>(s_tmem + b * G::keys, qlo + at, (uint32_t)(q_desc >> 32), klo + at, (uint32_t)(k_desc >> 32), qk_desc);
+            else mma_ss_words<true>(s_tmem + b * G::keys, qlo + at, (uint32_t)(q_desc >> 32), klo + at, (uint32_t)(k_desc >> 32), qk_desc);
           }
-          tc::mma_commit(&empty[s]);
+          if (tile_ends) tc::mma_commit(&empty[s]);
+          if (part == G::parts - 1) {
+            tc::mma_commit(&bars[B::s_ready + 2 * rt + b]);
+            if (last) tc::mma_commit(&bars[B::q_empty + rt]);
+          }
         }
-        tc::mma_commit(&bars[B::s_ready + b]);
-        if (g.qk == g.tiles - 1) tc::mma_commit(&bars[B::q_empty + rt]);
+        __syncwarp();
       }
-      __syncwarp();
-      if (g.qk == 0) ++g.q_used;
-      ++g.qk;
-      ++g.s_qk;
-      return true;
+      ++s_qk;
     };
-    auto try_pv = [&](Program& g, int rt) -> bool {
-      const uint32_t u = (g.tile0 + g.pv) * 2 * G::parts + G::parts;
-      const uint32_t b = rt + g.s_pv % G::bufs, use = g.s_pv / G::bufs;
-      if (g.live && !test_wait(&bars[B::p_ready + 2 * b + g.half], use & 1)) return false;
+    auto pv = [&](uint32_t u, int sub, bool tile_ends, bool first) {
+      const uint32_t b = s_pv & 1, use = s_pv >> 1;
 #pragma unroll
-      for (int part = 0; part < G::parts; ++part) {
-        if (!landed(u + part)) return false;
-      }
-      if (!g.live) {
-        pass(u);
-        ++g.pv;
-        return true;
-      }
+      for (int part = 0; part < G::parts; ++part) arrived(u + part);
       tc::fence_async_smem();
-      if (elect_one()) {
-        tc::fence_after_sync();
 #pragma unroll
-        for (int part = 0; part < G::parts; ++part) {
-          const uint32_t s = (u + part) % G::units;
+      for (int half = 0; half < G::halves; ++half) {
+        ok &= kv16_wait(&bars[B::p_ready + 2 * (2 * rt + b) + half], use & 1, abort_flag);
+        if (elect_one()) {
+          tc::fence_after_sync();
 #pragma unroll
-          for (int kk = 0; kk < 4; ++kk)
-            mma_ts(tmem_base + G::o_col + rt * HD + part * 128, tmem_base + G::s_col + b * 128 + g.half * 32 + kk * 8,
-                   swizzled_desc(ring + s * G::unit + (g.half * 4 + kk) * 2048, kTile * 128, 1024), pv_desc, g.pv > 0 || g.half > 0 || kk > 0);
-          if (g.half == 1) tc::mma_commit(&empty[s]);
-        }
-        if (g.half == 1) tc::mma_commit(&bars[B::pv_done + b]);
-      }
-      __syncwarp();
-      g.half ^= 1;
-      if (g.half == 0) {
-        ++g.pv;
-        ++g.s_pv;
-      }
-      return true;
-    };
-    auto step = [&](Program& g, int rt) -> bool {
-      if (g.pv == g.tiles) {   // next piece
-        g.tile0 += (uint32_t)g.tiles;
-        while (!next_piece<RP>(p, g.w, &g.it)) {
-          g.kvh += heads;
-          if (g.kvh >= p.num_kv_heads) {
-            g.done = true;
-            return true;
+          for (int part = 0; part < G::parts; ++part) {
+            const uint32_t s = (u + part) % G::units;
+            const uint32_t vlo = (uint32_t)v_desc + s * (G::unit >> 4) + (sub * G::keys + half * 64) * (128 >> 4);
+#pragma unroll
+            for (int kk = 0; kk < 4; ++kk)
+              mma_ts_words(o_tmem + part * 128, s_tmem + b * G::keys + half * 32 + kk * 8, vlo + kk * (2048 >> 4), (uint32_t)(v_desc >> 32), pv_desc,
+                           !first || half > 0 || kk > 0);
+            if (tile_ends && half == G::halves - 1) tc::mma_commit(&empty[s]);
           }
-          g.w = run.start;
+          tc::mma_commit(&bars[(half == G::halves - 1 ? B::pv_done : B::pv_half) + 2 * rt + b]);
         }
-        g.tiles = g.it.tiles;
-        g.qk = g.pv = g.half = 0;
-        g.live = g.it.rows > rt * 128;
-        return true;
+        __syncwarp();
       }
-      if (g.qk < g.tiles && g.qk < g.pv + G::bufs && try_qk(g, rt)) return true;
-      return g.pv < g.qk && try_pv(g, rt);
+      ++s_pv;
     };
-    long long deadline = clock64() + (1ll << 32);
-    uint32_t idle = 0;
-    for (;;) {
-      bool all_done = true, moved = false;
-#pragma unroll
-      for (int rt = 0; rt < G::rts; ++rt) {
-        if (prog[rt].done) continue;
-        all_done = false;
-        moved |= step(prog[rt], rt);
-      }
-      if (all_done) break;
-      if (moved) {
-        idle = 0;
-      } else if ((++idle & 1023u) == 0) {
-        if (idle == 1024u) deadline = clock64() + (1ll << 32);
-        if (*abort_flag || clock64() > deadline) {
-          *abort_flag = 1;
-          ok = false;
-          break;
+    TallWalk<RP> w = walk;
+    Piece it;
+    while (w.next(p, &it)) {
+      if (it.rows <= rt * 128) {   // no rows: free the units as if they had been read
+        for (int u = 0; u < 2 * G::parts * it.tiles; ++u) {
+          const uint32_t s = arrived(unit + u);
+          if (elect_one()) mbar_arrive(&empty[s]);
+          __syncwarp();
+        }
+      } else {
+        ++pieces;
+        const int n = piece_steps<G::keys>(it);
+        // QK of a step ahead of PV of the one before: the softmax finds the next S when it is done with one
+        for (int j = 0; j <= n; ++j) {
+          if (j < n) qk(unit + j / G::steps * 2 * G::parts, j % G::steps, j % G::steps == G::steps - 1 || j == n - 1, j == 0, j == n - 1);
+          if (j > 0) pv(unit + (j - 1) / G::steps * 2 * G::parts + G::parts, (j - 1) % G::steps, (j - 1) % G::steps == G::steps - 1 || j == n, j == 1);
         }
       }
+      unit += 2 * G::parts * it.tiles;
     }
-    __syncwarp();
   } else {
     // =========================== softmax =========================================
     asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(G::softmax_regs));
@@ -354,90 +541,88 @@ __global__ void __launch_bounds__(Tall<HD>::threads, 1) kv16_tall_kernel(const _
     const int row = tid;   // of the CTA's rows
     uint32_t count = 0;    // live tiles so far
     auto rt_sync = [&] { named_barrier(1 + rt, 128); };
-    for (int kvh = hslot; kvh < p.num_kv_heads && works; kvh += heads) {
-      Walk<RP> w = run.start;
+    {
+      TallWalk<RP> w = walk;
       Piece it;
-      while (next_piece<RP>(p, w, &it)) {
+      while (w.next(p, &it)) {
         if (it.rows <= rt * 128) continue;
+        const int kvh = it.kvh;
         const bool padding = (row & ~31) >= it.rows;   // (of the whole warp)
         float ref = -INFINITY, l = 0.f;
-        for (int t = 0; t < it.tiles; ++t, ++count) {
-          const uint32_t b = rt + count % G::bufs, use = count / G::bufs;
-          const uint32_t s_tmem = tmem_base + G::s_col + b * 128 + lane_addr;
-          ok &= wait_or_abort(&bars[B::s_ready + b], use & 1, abort_flag);
+        const int n_steps = piece_steps<G::keys>(it);
+        for (int t = 0; t < n_steps; ++t, ++count) {
+          const uint32_t b = 2 * rt + (count & 1), use = count >> 1;
+          const uint32_t s_tmem = tmem_base + G::s_col + b * G::keys + lane_addr;
+          ok &= kv16_wait(&bars[B::s_ready + b], use & 1, abort_flag);
           if (padding) {   // (the order of the waits is kept, nothing is computed)
-            mbar_arrive(&bars[B::p_ready + 2 * b]);
-            mbar_arrive(&bars[B::p_ready + 2 * b + 1]);
+#pragma unroll
+            for (int half = 0; half < G::halves; ++half) mbar_arrive(&bars[B::p_ready + 2 * b + half]);
             continue;
           }
           tc::fence_after_sync();
-          uint32_t r[128];
-#pragma unroll
-          for (int c = 0; c < 4; ++c) tc::tmem_ld32(s_tmem + c * 32, r + c * 32);
-          tc::tmem_ld_wait<128>(r);
-          const int key0 = it.key0 + t * kTile;
-          if (key0 < it.lo || key0 + kTile > it.hi) {
-#pragma unroll
-            for (int n = 0; n < 128; ++n)
-              if (key0 + n < it.lo || key0 + n >= it.hi) r[n] = 0xff800000u;  // -inf
-          }
-          float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-#pragma unroll
-          for (int n = 0; n < 128; n += 8) {
-#pragma unroll
-            for (int e = 0; e < 4; ++e) mx[e] = max3(mx[e], __uint_as_float(r[n + 2 * e]), __uint_as_float(r[n + 2 * e + 1]));
-          }
-          const float top = max3(fmaxf(mx[0], mx[1]), mx[2], mx[3]) * p.scale_log2 - kGain;
-          const bool need = !(top <= ref + kSlack);   // (also where ref is not set yet)
-          if (__any_sync(0xffffffffu, need)) {
-            const float to = need ? fmaxf(ref, top) : ref;
-            const float alpha = to == -INFINITY ? 1.f : ex2f(ref - to);
-            ref = to;
-            l *= alpha;
-            if (t > 0) {
-              const uint32_t b1 = rt + (count - 1) % G::bufs, use1 = (count - 1) / G::bufs;
-              ok &= wait_or_abort(&bars[B::pv_done + b1], use1 & 1, abort_flag);
-              tc::fence_after_sync();
+          const int key0 = it.key0 + t * G::keys;
+          const bool edge = key0 < it.lo || key0 + G::keys > it.hi;
+          // (one copy of the code for both halves: the instruction cache is small)
 #pragma unroll 1
-              for (int c = 0; c < HD / 16; ++c) {
-                uint32_t o[16];
-                tc::tmem_ld16(o_tmem + c * 16, o);
-                tc::tmem_ld_wait<16>(o);
+          for (int half = 0; half < G::halves; ++half) {
+            uint32_t r[64];
+            tc::tmem_ld32(s_tmem + half * 64, r);
+            tc::tmem_ld32(s_tmem + half * 64 + 32, r + 32);
+            tc::tmem_ld_wait<64>(r);
+            if (edge) {
+              const int pos0 = key0 + half * 64;
 #pragma unroll
-                for (int n = 0; n < 16; ++n) o[n] = __float_as_uint(__uint_as_float(o[n]) * alpha);
-                tc::tmem_st16(o_tmem + c * 16, o);
+              for (int n = 0; n < 64; ++n)
+                if (pos0 + n < it.lo || pos0 + n >= it.hi) r[n] = 0xff800000u;  // -inf
+            }
+            auto maximum = [&] {
+              float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+              for (int n = 0; n < 64; n += 8) {
+#pragma unroll
+                for (int e = 0; e < 4; ++e) mx[e] = max3(mx[e], __uint_as_float(r[n + 2 * e]), __uint_as_float(r[n + 2 * e + 1]));
               }
-              tc::tmem_st_wait();
-            }
-          }
-          const float use_ref = ref == -INFINITY ? 0.f : -ref;
-          const f32x2 scale2 = pair(p.scale_log2, p.scale_log2), ref2 = pair(use_ref, use_ref);
-          f32x2 sum[2] = {0ull, 0ull};
+              return max3(fmaxf(mx[0], mx[1]), mx[2], mx[3]) * p.scale_log2 - kGain;
+            };
+            if (t == 0 && half == 0) ref = maximum();
+            uint32_t pk[32];
+            float total = exponentials<kHalf>(r, p.scale_log2, ref == -INFINITY ? 0.f : -ref, pk);
+            const bool outgrown = !(total <= kMostSum) || ref == -INFINITY;
+            if (__any_sync(0xffffffffu, outgrown)) {
+              const float to = outgrown ? fmaxf(ref, maximum()) : ref;
+              const float alpha = to == -INFINITY ? 1.f : ex2f(ref - to);
+              ref = to;
+              l *= alpha;
+              if (t > 0 || half > 0) {   // (PV of what P holds already is complete first)
+                if (half > 0) {
+                  ok &= kv16_wait(&bars[B::pv_half + b], use & 1, abort_flag);
+                } else {
+                  ok &= kv16_wait(&bars[B::pv_done + (b ^ 1)], ((count - 1) >> 1) & 1, abort_flag);
+                }
+                tc::fence_after_sync();
+#pragma unroll 1
+                for (int d = 0; d < HD / 16; ++d) {
+                  uint32_t o[16];
+                  tc::tmem_ld16(o_tmem + d * 16, o);
+                  tc::tmem_ld_wait<16>(o);
 #pragma unroll
-          for (int c = 0; c < 4; ++c) {
-            uint32_t pk[16];
-#pragma unroll
-            for (int n = 0; n < 16; ++n) {
-              float x, y;
-              unpair(fma2(pair(__uint_as_float(r[c * 32 + 2 * n]), __uint_as_float(r[c * 32 + 2 * n + 1])), scale2, ref2), x, y);
-              x = ex2f(x);
-              y = ex2f(y);
-              sum[n & 1] = add2(sum[n & 1], pair(x, y));
-              pk[n] = pack16<kHalf>(x, y);
+                  for (int n = 0; n < 16; ++n) o[n] = __float_as_uint(__uint_as_float(o[n]) * alpha);
+                  tc::tmem_st16(o_tmem + d * 16, o);
+                }
+                tc::tmem_st_wait();
+              }
+              total = exponentials<kHalf>(r, p.scale_log2, ref == -INFINITY ? 0.f : -ref, pk);
             }
-            tc::tmem_st16(s_tmem + c * 16, pk);
-            if (c & 1) {
-              tc::tmem_st_wait();
-              tc::fence_before_sync();
-              mbar_arrive(&bars[B::p_ready + 2 * b + (c >> 1)]);
-            }
+            l += total;
+            tc::tmem_st32(s_tmem + half * 32, pk);
+            tc::tmem_st_wait();
+            tc::fence_before_sync();
+            mbar_arrive(&bars[B::p_ready + 2 * b + half]);
           }
-          l += sum_pairs(sum);
         }
         // ---- the piece's rows ----
         {
-          const uint32_t b1 = rt + (count - 1) % G::bufs, use1 = (count - 1) / G::bufs;
-          ok &= wait_or_abort(&bars[B::pv_done + b1], use1 & 1, abort_flag);
+          ok &= kv16_wait(&bars[B::pv_done + 2 * rt + ((count - 1) & 1)], ((count - 1) >> 1) & 1, abort_flag);
           tc::fence_after_sync();
         }
         const bool whole = it.begins && it.ends, live = row < it.rows;
@@ -480,22 +665,26 @@ __global__ void __launch_bounds__(Tall<HD>::threads, 1) kv16_tall_kernel(const _
         tc::fence_before_sync();
         if (!whole) {
           // (a row tile's pieces are merged by the row tile's own threads: a counter each)
-          const int g0 = run.owner(it.start), g1 = run.owner(it.start + it.row_tiles_keys - 1);
+          const int c0 = tall_owner(bounds, (int)gridDim.x, it.start - base), c1 = tall_owner(bounds, (int)gridDim.x, it.start + it.row_tile_tiles - 1 - base);
           __threadfence();
           rt_sync();
-          int* const counter = reinterpret_cast<int*>(p.workspace) + 2 * (g0 * heads + hslot) + rt;
+          int* const counter = reinterpret_cast<int*>(p.workspace) + 2 * c0 + rt;
           if ((tid & 127) == 0) arrival[rt] = atomicAdd(counter, 1);
           rt_sync();
-          if (arrival[rt] == g1 - g0) {
+          // (a CTA with much of the waves may have none of the tail)
+          int pieces = 0;
+          for (int c = c0; c <= c1; ++c) pieces += bounds[c] < bounds[c + 1] ? 1 : 0;
+          if (arrival[rt] == pieces - 1) {
             __threadfence();
             if ((tid & 127) == 0) *counter = 0;   // (for the next call)
-            const int pieces = g1 - g0 + 1;
-            auto slot = [&](int k) { return tall_slot<HD>(p, (g0 + k) * heads + hslot, k == 0) + row; };
+            auto slot = [&](int c) { return tall_slot<HD>(p, c, c == c0) + row; };
             float top = -INFINITY, sum = 0.f;
-            for (int k = 0; k < pieces; ++k) top = fmaxf(top, __ldcg(slot(k) + HD * RP));
+            for (int c = c0; c <= c1; ++c)
+              if (bounds[c] < bounds[c + 1]) top = fmaxf(top, __ldcg(slot(c) + HD * RP));
             const float use = top == -INFINITY ? 0.f : top;
-            for (int k = 0; k < pieces; ++k) {
-              const float* s = slot(k) + HD * RP;
+            for (int c = c0; c <= c1; ++c) {
+              if (bounds[c] == bounds[c + 1]) continue;
+              const float* s = slot(c) + HD * RP;
               sum = fmaf(ex2f(__ldcg(s) - use), __ldcg(s + RP), sum);
             }
             const float inv = sum == 0.f ? 0.f : 1.f / sum;
@@ -506,8 +695,9 @@ __global__ void __launch_bounds__(Tall<HD>::threads, 1) kv16_tall_kernel(const _
 #pragma unroll
                 for (int n = 0; n < 32; ++n) o[n] = 0.f;
 #pragma unroll 1
-                for (int k = 0; k < pieces; ++k) {
-                  const float* s = slot(k);
+                for (int cta = c0; cta <= c1; ++cta) {
+                  if (bounds[cta] == bounds[cta + 1]) continue;
+                  const float* s = slot(cta);
                   const float f = ex2f(__ldcg(s + HD * RP) - use);
                   float v[32];
 #pragma unroll
@@ -534,6 +724,44 @@ __global__ void __launch_bounds__(Tall<HD>::threads, 1) kv16_tall_kernel(const _
   (void)ok;
 }
 
+// Tensor map over one of the caches, [dims][heads][slots][blocks], a box being 64 dims of box_slots slots of one head, in the
+// 128-byte swizzle.  Encoding one is a driver call of microseconds and depends on the view alone, of which an engine has a
+// few for its whole life: they are kept (once the table is full, further ones are encoded by every call).  False: the driver
+// refuses the view.
+bool page_box_map(const Kv16Params& p, const uint8_t* base, CUtensorMap* map) {
+  struct Entry {
+    const uint8_t* base;
+    int64_t stride_block, stride_slot, stride_head;
+    int32_t num_blocks, block_size, num_kv_heads, head_size, dtype, box_slots;
+    bool fine;
+    CUtensorMap map;
+  };
+  constexpr int kEntries = 128;
+  static Entry entries[kEntries];
+  static int used = 0;
+  static std::mutex mu;
+  std::lock_guard<std::mutex> lock(mu);
+  for (int i = 0; i < used; ++i) {
+    const Entry& e = entries[i];
+    if (e.base == base && e.stride_block == p.stride_block && e.stride_slot == p.stride_slot && e.stride_head == p.stride_head &&
+        e.num_blocks == p.num_blocks && e.block_size == p.block_size && e.num_kv_heads == p.num_kv_heads && e.head_size == p.head_size &&
+        e.dtype == p.dtype && e.box_slots == p.box_slots) {
+      *map = e.map;
+      return e.fine;
+    }
+  }
+  const EncodeTiledFn fn = encode_tiled_fn();
+  const cuuint64_t dims[4] = {(cuuint64_t)p.head_size, (cuuint64_t)p.num_kv_heads, (cuuint64_t)p.block_size, (cuuint64_t)p.num_blocks};
+  const cuuint64_t strides[3] = {(cuuint64_t)p.stride_head, (cuuint64_t)p.stride_slot, (cuuint64_t)p.stride_block};
+  const cuuint32_t box[4] = {64, 1, (cuuint32_t)p.box_slots, 1}, elem[4] = {1, 1, 1, 1};
+  const bool fine = fn != nullptr && fn(map, p.dtype == PTH_ATTN_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4,
+                                        const_cast<uint8_t*>(base), dims, strides, box, elem, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                                        CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+  if (used < kEntries)
+    entries[used++] = Entry{base, p.stride_block, p.stride_slot, p.stride_head, p.num_blocks, p.block_size, p.num_kv_heads, p.head_size, p.dtype, p.box_slots, fine, *map};
+  return fine;
+}
+
 template <int HD, bool kHalf>
 cudaError_t launch_one(const Kv16Params& p, cudaStream_t stream) {
   using G = Tall<HD>;
@@ -547,8 +775,15 @@ cudaError_t launch_one(const Kv16Params& p, cudaStream_t stream) {
     if (dev >= 0 && dev < 64) configured[dev] = true;
   }
   const int sms = sm_count();
-  if (sms <= 0) return cudaErrorInvalidDevice;
-  return pdl_launch(kv16_tall_kernel<HD, kHalf>, dim3((unsigned)sms), dim3(G::threads), G::total, stream, p);
+  if (sms <= 0 || sms > kTallCtas) return cudaErrorInvalidDevice;
+  // Boxes take pages of a multiple of 8 slots: the swizzle repeats every 8 rows.
+  Kv16Params q = p;
+  q.box_slots = 0;
+  for (int slots = 32; slots >= 8 && q.box_slots == 0; slots >>= 1)
+    if (p.block_size % slots == 0) q.box_slots = slots;
+  CUtensorMap k_map{}, v_map{};
+  if (q.box_slots > 0 && !(page_box_map(q, p.k, &k_map) && page_box_map(q, p.v, &v_map))) q.box_slots = 0;
+  return pdl_launch(kv16_tall_kernel<HD, kHalf>, dim3((unsigned)sms), dim3(G::threads), G::total, stream, q, k_map, v_map);
 }
 template <int HD>
 cudaError_t launch_type(const Kv16Params& p, cudaStream_t stream) {
