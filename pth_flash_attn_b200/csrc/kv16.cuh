@@ -29,6 +29,7 @@ struct Kv16Params {
   int32_t num_reqs, num_tokens, max_query_len, window;
   int32_t num_blocks;
   int32_t box_slots;  // slots of a TMA box (tall kernel; 0: none)
+  int32_t out_wide;   // rows of out lie on 32-byte boundaries (tall kernel)
   float scale_log2;  // softmax_scale * log2(e)
 };
 
@@ -65,25 +66,6 @@ __device__ __forceinline__ bool kv16_wait(uint64_t* bar, uint32_t parity, volati
   }
   *abort_flag = 1;
   return false;
-}
-// The same wait without sleep at first, where the next step of a chain hangs on it: a sleeping thread wakes late.
-__device__ __forceinline__ bool kv16_spin(uint64_t* bar, uint32_t parity, volatile int* abort_flag) {
-  const uint32_t bar_s = tc::smem_u32(bar);
-#pragma unroll 1
-  for (uint32_t i = 0; i < 4096; ++i) {
-    uint32_t done;
-    asm volatile(
-        "{\n\t"
-        ".reg .pred p;\n\t"
-        "mbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
-        "selp.u32 %0, 1, 0, p;\n\t"
-        "}\n"
-        : "=r"(done)
-        : "r"(bar_s), "r"(parity)
-        : "memory");
-    if (done) return true;
-  }
-  return kv16_wait(bar, parity, abort_flag);
 }
 // Asynchronous copy of 16 bytes, or of none: then the destination is zeroed.
 __device__ __forceinline__ void copy16(uint32_t dst, const uint8_t* src, bool live) {

@@ -54,7 +54,6 @@ int32_t build(const PthB200Kv16Args* a, bool cross, Kv16Params* p) {
                "num_q_heads must be a positive multiple of num_kv_heads");
   KV16_REQUIRE(a->num_q_heads / a->num_kv_heads <= 64, "num_q_heads / num_kv_heads must be <= 64");
   KV16_REQUIRE(a->num_reqs >= 0 && a->num_tokens >= 0, "num_reqs and num_tokens must be >= 0");
-  KV16_REQUIRE(a->num_reqs <= 8192, "num_reqs must be <= 8192");
   KV16_REQUIRE(a->block_size >= 1 && a->num_blocks >= 1, "block_size and num_blocks must be >= 1");
   KV16_REQUIRE(std::isfinite(a->softmax_scale) && a->softmax_scale > 0.f, "softmax_scale must be finite and > 0");
   KV16_REQUIRE(a->window >= 0, "window must be >= 0");

@@ -15,15 +15,54 @@ namespace {
 constexpr int kTile = 128;             // keys
 constexpr int kCounterBytes = 4096;    // arrival counters at the start of the workspace, one per CTA
 
-// One piece of a row tile: keys [key0, key0 + 128 tiles) of those visible, [lo, hi).
+// One piece of a row tile: the keys [lo, hi) from key0 on, in `tiles` KV tiles.
 struct Piece {
   int r, kvh;
   int row0, rows;             // rows row0 .. row0 + rows of the request's q_len x G
   int first_token;
   int key0, tiles, lo, hi;
-  bool begins, ends;
-  long long start;            // of the row tile in the sequence
-  int row_tile_tiles;         // KV tiles of the whole row tile
+  int begins, ends;           // the row tile's first piece, its last
+  int first_cta, last_cta;    // that have its pieces (in the counting of the kernel's schedule)
+  int sparse;                 // CTAs between them may have none
+  int unused[2];
+};
+static_assert(sizeof(Piece) == 64, "queue entry");
+
+// The pieces of a CTA go from the warp that works them out to the others through a queue in shared memory, so the others
+// neither carry the schedule's state nor wait for the lengths it reads.  An entry without tiles ends it.
+constexpr int kQueue = 4;
+struct PieceQueue {
+  Piece* entry;      // [kQueue]
+  uint64_t* full;    // [kQueue]: one arrival
+  uint64_t* empty;   // [kQueue]: one per reading warp
+  uint32_t i = 0;
+  __device__ __forceinline__ PieceQueue(Piece* entries, uint64_t* bars) : entry(entries), full(bars), empty(bars + kQueue) {}
+  __device__ __forceinline__ void init(int readers) {
+    for (int k = 0; k < kQueue; ++k) {
+      tc::mbar_init(&full[k], 1);
+      tc::mbar_init(&empty[k], readers);
+    }
+  }
+  __device__ __forceinline__ bool put(const Piece& x, volatile int* abort_flag) {
+    const uint32_t k = i % kQueue;
+    const bool ok = i < kQueue || kv16_wait(&empty[k], ((i / kQueue) - 1) & 1, abort_flag);
+    if ((threadIdx.x & 31) == 0) {
+      entry[k] = x;
+      asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(tc::smem_u32(&full[k])) : "memory");
+    }
+    __syncwarp();
+    ++i;
+    return ok;
+  }
+  __device__ __forceinline__ bool get(Piece* x, volatile int* abort_flag) {
+    const uint32_t k = i % kQueue;
+    if (!kv16_wait(&full[k], (i / kQueue) & 1, abort_flag)) return false;
+    *x = entry[k];
+    __syncwarp();
+    if ((threadIdx.x & 31) == 0) asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(tc::smem_u32(&empty[k])) : "memory");
+    ++i;
+    return x->tiles > 0;
+  }
 };
 
 struct ReqShape {
@@ -39,22 +78,22 @@ __device__ __forceinline__ ReqShape req_shape(const Kv16Params& p, int r) {
   s.tiles = s.hi > s.lo && rows > 0 ? (s.hi + kTile - 1) / kTile - s.lo / kTile : 0;
   return s;
 }
-// Fills a piece with KV tiles tile .. tile + count of row tile rt.
-template <int RP>
-__device__ __forceinline__ void make_piece(const Kv16Params& p, const ReqShape& s, int r, int kvh, int rt, int tile, int count, long long start, Piece* out) {
-  out->r = r;
-  out->kvh = kvh;
-  out->row0 = rt * RP;
-  out->rows = min(RP, s.tokens * p.group - rt * RP);
-  out->first_token = s.first;
-  out->lo = s.lo;
-  out->hi = s.hi;
-  out->key0 = (s.lo / kTile + tile) * kTile;
-  out->tiles = count;
-  out->begins = tile == 0;
-  out->ends = tile + count == s.tiles;
-  out->start = start;
-  out->row_tile_tiles = s.tiles;
+// Counts an arrival behind everything that this CTA's threads have written in front of a barrier that this thread has passed,
+// and ahead of what they read behind the next one: the partial results of all who arrived before.
+__device__ __forceinline__ int arrive_at(int* counter) {
+  int before;
+  asm volatile("atom.add.acq_rel.gpu.global.s32 %0, [%1], 1;" : "=r"(before) : "l"(counter) : "memory");
+  return before;
+}
+template <bool kHalf>
+__device__ __forceinline__ uint32_t pack16(float a, float b) {
+  if constexpr (kHalf) {
+    const __half2 h = __floats2half2_rn(a, b);
+    return *reinterpret_cast<const uint32_t*>(&h);
+  } else {
+    const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
+    return *reinterpret_cast<const uint32_t*>(&h);
+  }
 }
 // Token and query head of a row of a request.
 __device__ __forceinline__ void row_of(const Kv16Params& p, int first_token, int kvh, int row, int* token, int* head) {
@@ -97,6 +136,7 @@ __device__ __forceinline__ void zero_requests(const Kv16Params& p) {
   for (int r = (int)blockIdx.x; r < p.num_reqs; r += (int)gridDim.x) {
     const ReqShape s = req_shape<RP>(p, r);
     if (s.tiles > 0 || s.tokens == 0) continue;
+#pragma unroll 1
     for (int64_t i = threadIdx.x; i < (int64_t)s.tokens * p.num_q_heads * (HD / 8); i += kThreads) {
       const int64_t row = i / (HD / 8);
       const int token = s.first + (int)(row / p.num_q_heads), head = (int)(row % p.num_q_heads), c = (int)(i % (HD / 8));
@@ -108,18 +148,19 @@ __device__ __forceinline__ void zero_requests(const Kv16Params& p) {
 
 // The KV tiles of a CTA's pieces, one after the other, for the lane of a copying warp that looks key `key` of every tile up in
 // the block table.  The entry of the next tile is on its way while the copies of this one are issued.
-template <class Walk>
 struct KeyLookup {
   const Kv16Params& p;
-  Walk w;
+  PieceQueue queue;
+  volatile int* abort_flag;
   Piece it;            // of the tile looked up last
   int key, left = 0, key0 = 0, blk = -1, slot = 0;
   bool fresh = false;  // the tile is its piece's first
-  __device__ __forceinline__ KeyLookup(const Kv16Params& params, const Walk& walk, int lane_key) : p(params), w(walk), key(lane_key) {}
+  __device__ __forceinline__ KeyLookup(const Kv16Params& params, const PieceQueue& q, volatile int* abort, int lane_key)
+      : p(params), queue(q), abort_flag(abort), key(lane_key) {}
   __device__ __forceinline__ bool fetch() {
     fresh = left == 0;
     if (fresh) {
-      if (!w.next(p, &it)) return false;
+      if (!queue.get(&it, abort_flag)) return false;
       left = it.tiles;
       key0 = it.key0;
     } else {

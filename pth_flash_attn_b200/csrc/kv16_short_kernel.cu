@@ -21,9 +21,9 @@
 // TMA, boxes of 16 slots x 64 dims, 64 requests x 8,192 keys x 8 heads x 128 dims) moved 6.83 TB/s, with boxes of 4 KB 7.06, 16-byte
 // copies 7.17, which also take pages of any size and place.
 //
-// Schedule: the KV tiles of all (request, row tile) form one sequence, which is cut into equal runs, one for every group of Hkv
-// CTAs; CTA h of a group reads head h, so that the heads of a page are read at the same time.  The pieces of a row tile that
-// a cut divides are merged by the CTA that arrives last: one launch, and the same bits whoever is last.
+// Schedule: the keys of all (request, row tile) form one sequence, which is cut into equal runs, one for every group of Hkv CTAs;
+// CTA h of a group reads head h, so that the heads of a page are read at the same time.  The pieces of a row tile that a cut
+// divides are merged by the CTA that arrives last: one launch, and the same bits whoever is last.
 #include "kv16_sched.cuh"
 #include "page_copy.cuh"
 #include "pdl.cuh"
@@ -36,9 +36,11 @@ namespace {
 
 constexpr int kSoftmaxThreads = 128;   // warps 0-3: thread t is key t of a tile, then dim t of the output
 constexpr int kLoadWarp = 4;           // warps 4-7
-constexpr int kMmaWarp = 8;
-constexpr int kThreads = 288;
-constexpr int kRunMin = 1;             // KV tiles a run holds at least
+constexpr int kMmaWarp = 8, kScheduleWarp = 9;
+constexpr int kThreads = 320;
+// The sequence is counted in grains of 32 keys; a row tile counts kPieceGrains more, what its queries and its end take.
+constexpr int kGrain = 32, kPieceGrains = 4;
+constexpr int kRunMin = 4;             // length of a run at least
 constexpr float kGain = 7.f, kSlack = 8.f;
 
 template <int HD, int RP>
@@ -49,7 +51,7 @@ struct Geo {
   static constexpr int cols = RP < 16 ? 16 : RP;     // N of QK (its rows past RP repeat the first)
   static constexpr int qimage = RP * HD * 2;
   static constexpr int pimage = 2 * RP * kTile * 2;
-  static constexpr int fixed = 2 * qimage + pimage + 4 * RP * 4 * 2 + 512;
+  static constexpr int fixed = 2 * qimage + pimage + 4 * RP * 4 * 2 + 768;
   // Two CTAs per SM where three units fit, else one.
   static constexpr int units2 = (115712 - fixed - 1024) / unit;
   static constexpr int ctas = units2 >= 3 && RP <= 16 ? 2 : 1;
@@ -57,6 +59,11 @@ struct Geo {
   static constexpr int fit = ctas == 2 ? units2 : (232448 - fixed - 1024) / unit;
   static constexpr int units = fit < most ? fit : most;
   static_assert(units >= 3, "K and V of a tile, and the next K");
+  // Registers that the copies hand to the softmax from what a thread starts with (168 with one CTA per SM, 96 with two); with 8
+  // rows nothing spills as it is.
+  static constexpr bool moves = RP == 32 || (RP == 16 && ctas == 2);
+  static constexpr int softmax_regs = RP == 32 ? 232 : 128, copy_regs = RP == 32 ? 72 : 64, start_regs = RP == 32 ? 168 : 96;
+  static_assert(!moves || 4 * softmax_regs + 4 * copy_regs <= 8 * start_regs, "a split that the launch holds");
   static constexpr int s_col = 0, o_col = 2 * cols;  // TMEM columns: S twice, O of every part (hi, lo)
   static constexpr int tmem_need = 2 * cols + parts * 2 * RP;
   static constexpr int tmem = tmem_need <= 64 ? 64 : tmem_need <= 128 ? 128 : 256;
@@ -66,17 +73,23 @@ struct Geo {
   static constexpr int p = q + 2 * qimage;
   static constexpr int wmax = p + pimage;            // float [4 warps][RP]
   static constexpr int wsum = wmax + 4 * RP * 4;     // float [4 warps][RP]
-  static constexpr int bars = wsum + 4 * RP * 4;
-  static constexpr int n_bars = 2 * units + 2 + 2 + 1 + 1;
+  static constexpr int pieces = wsum + 4 * RP * 4;   // PieceQueue's entries
+  static constexpr int bars = pieces + kQueue * 64;
+  static constexpr int n_bars = 2 * units + 2 + 2 + 1 + 1 + 2 * kQueue;
   static constexpr int misc = bars + n_bars * 8;     // ints: abort flag, TMEM address, arrival; scratch of find_run
   static constexpr int total = misc + 160 + 1024;
-  static_assert(n_bars * 8 + 160 <= 512, "fixed part");
+  static_assert(kQueue * 64 + n_bars * 8 + 160 <= 768, "fixed part");
 };
 
 struct Bars {  // offsets behind [units] full, [units] empty
-  static constexpr int q_empty = 0, s_ready = 2, p_ready = 4, pv_done = 5;
+  static constexpr int q_empty = 0, s_ready = 2, p_ready = 4, pv_done = 5, queue = 6;
 };
 
+// Length of a row tile in the sequence: its keys in grains, and what a piece costs besides.
+template <int RP>
+__device__ __forceinline__ int row_tile_length(const ReqShape& s) {
+  return s.tiles > 0 ? (s.hi - s.lo / kGrain * kGrain + kGrain - 1) / kGrain + kPieceGrains : 0;
+}
 // The run of a CTA: a walk over its pieces.
 template <int RP>
 struct ShortWalk {
@@ -84,79 +97,115 @@ struct ShortWalk {
   int r, kvh;
   long long begin, first_start;   // where the run begins, for further KV heads
   int first_r, heads;
+  long long work;             // length of the sequence
+  int groups;                 // that it is cut among
+  // Group that has position x of the sequence.
+  __device__ __forceinline__ int owner(long long x) const { return (int)(((x + 1) * groups - 1) / work); }
   __device__ __forceinline__ bool next(const Kv16Params& p, Piece* out) {
-    if (at >= end) {
-      kvh += heads;
-      if (begin >= end || kvh >= p.num_kv_heads) return false;
-      at = begin;
-      start = first_start;
-      r = first_r;
+    for (;;) {
+      if (at >= end) {
+        kvh += heads;
+        if (begin >= end || kvh >= p.num_kv_heads) return false;
+        at = begin;
+        start = first_start;
+        r = first_r;
+      }
+      ReqShape s = req_shape<RP>(p, r);
+      int n = row_tile_length<RP>(s);
+      while (at >= start + (long long)n * s.row_tiles) {
+        start += (long long)n * s.row_tiles;
+        ++r;
+        s = req_shape<RP>(p, r);
+        n = row_tile_length<RP>(s);
+      }
+      const long long off = at - start;
+      const int rt = s.row_tiles == 1 ? 0 : (int)(off / n), a = (int)(off - (long long)rt * n);
+      const int b = (int)min((long long)n, a + (end - at));
+      at += b - a;
+      if (b <= kPieceGrains) continue;   // (no keys yet)
+      const int base = s.lo / kGrain * kGrain;
+      out->r = r;
+      out->kvh = kvh;
+      out->row0 = rt * RP;
+      out->rows = min(RP, s.tokens * p.group - rt * RP);
+      out->first_token = s.first;
+      out->key0 = base + max(0, a - kPieceGrains) * kGrain;
+      out->lo = max(s.lo, out->key0);
+      out->hi = min(s.hi, base + (b - kPieceGrains) * kGrain);
+      out->tiles = (out->hi - out->key0 + kTile - 1) / kTile;
+      out->begins = a <= kPieceGrains;
+      out->ends = b == n;
+      out->first_cta = owner(start + (long long)rt * n + kPieceGrains);
+      out->last_cta = owner(start + (long long)rt * n + n - 1);
+      return true;
     }
-    ReqShape s = req_shape<RP>(p, r);
-    long long n = (long long)s.tiles * s.row_tiles;
-    while (at >= start + n) {
-      start += n;
-      ++r;
-      s = req_shape<RP>(p, r);
-      n = (long long)s.tiles * s.row_tiles;
-    }
-    const long long off = at - start;
-    const int rt = s.row_tiles == 1 ? 0 : (int)(off / s.tiles), tile = (int)(off - (long long)rt * s.tiles);
-    const int count = (int)min((long long)(s.tiles - tile), end - at);
-    make_piece<RP>(p, s, r, kvh, rt, tile, count, start + (long long)rt * s.tiles, out);
-    at += count;
-    return true;
   }
 };
-// What the pieces' owners are found with: tile x of the sequence belongs to group ((x + 1) groups - 1) / work.
+// Cuts the sequence, of which [before, before + mine) are requests from r0 on.  Returns whether this CTA's run begins among
+// them, and where.
 template <int RP>
-struct ShortRun {
-  ShortWalk<RP> walk;
-  long long work;       // tiles of the sequence
-  int groups, heads, hslot;
-  __device__ __forceinline__ int owner(long long x) const { return (int)(((x + 1) * groups - 1) / work); }
-};
-// Every CTA sums the tiles of all requests up for itself.  scratch: 64-bit words, warps + 2.  Ends with a CTA barrier.
-template <int RP, int kThreads>
-__device__ __forceinline__ ShortRun<RP> find_run(const Kv16Params& p, long long* scratch) {
+__device__ __forceinline__ bool begin_run(const Kv16Params& p, ShortWalk<RP>& w, int group, int r0, long long before, long long mine, int* r, long long* start) {
+  w.groups = (int)min((long long)((int)gridDim.x / w.heads), max(w.work / kRunMin, 1ll));
+  w.begin = group < w.groups ? w.work * group / w.groups : 0;
+  w.end = group < w.groups ? w.work * (group + 1) / w.groups : 0;
+  if (w.begin >= w.end || w.begin < before || w.begin >= before + mine) return false;
+  *start = before;
+#pragma unroll 1
+  for (*r = r0;; ++*r) {
+    const ReqShape s = req_shape<RP>(p, *r);
+    const long long n = (long long)row_tile_length<RP>(s) * s.row_tiles;
+    if (w.begin < *start + n) return true;
+    *start += n;
+  }
+}
+// Every CTA sums the requests' lengths up for itself: up to kWarpReqs requests its scheduling warp alone (scratch is nullptr),
+// else all its threads.  scratch: 64-bit words, warps + 2.
+constexpr int kWarpReqs = 256;
+template <int RP>
+__device__ __forceinline__ ShortWalk<RP> find_run(const Kv16Params& p, long long* scratch) {
   constexpr int kWarps = kThreads / 32;
-  const int tid = threadIdx.x;
-  ShortRun<RP> run;
-  run.heads = min(p.num_kv_heads, (int)gridDim.x);   // KV heads that a group reads at the same time
-  run.hslot = (int)blockIdx.x % run.heads;
-  const int group = (int)blockIdx.x / run.heads;
-  const int per = (p.num_reqs + kThreads - 1) / kThreads, r0 = min(p.num_reqs, tid * per), r1 = min(p.num_reqs, r0 + per);
+  const int tid = threadIdx.x, lane = tid & 31;
+  ShortWalk<RP> w;
+  w.heads = min(p.num_kv_heads, (int)gridDim.x);   // KV heads that a group reads at the same time
+  w.kvh = (int)blockIdx.x % w.heads;
+  const int group = (int)blockIdx.x / w.heads;
+  const int ranks = scratch == nullptr ? 32 : kThreads, rank = scratch == nullptr ? lane : tid;
+  const int per = (p.num_reqs + ranks - 1) / ranks, r0 = min(p.num_reqs, rank * per), r1 = min(p.num_reqs, r0 + per);
   long long mine = 0;
+#pragma unroll 1
   for (int r = r0; r < r1; ++r) {
     const ReqShape s = req_shape<RP>(p, r);
-    mine += (long long)s.tiles * s.row_tiles;
+    mine += (long long)row_tile_length<RP>(s) * s.row_tiles;
   }
-  const long long before = scan_threads<kThreads>(mine, scratch, &run.work);
-  const long long most = run.work / kRunMin > 0 ? run.work / kRunMin : 1;
-  run.groups = (int)min((long long)((int)gridDim.x / run.heads), most);
-  ShortWalk<RP>& w = run.walk;
-  w.begin = group < run.groups ? run.work * group / run.groups : 0;
-  w.end = group < run.groups ? run.work * (group + 1) / run.groups : 0;
-  if (w.begin < w.end && before <= w.begin && w.begin < before + mine) {
-    long long start = before;
-    int r = r0;
-    for (;; ++r) {
-      const ReqShape s = req_shape<RP>(p, r);
-      const long long n = (long long)s.tiles * s.row_tiles;
-      if (w.begin < start + n) break;
-      start += n;
+  long long before, first_start = 0;
+  int first_r = 0;
+  if (scratch == nullptr) {
+    long long upto = mine;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const long long x = __shfl_up_sync(0xffffffffu, upto, o);
+      if (lane >= o) upto += x;
     }
-    scratch[kWarps] = r;
-    scratch[kWarps + 1] = start;
+    w.work = __shfl_sync(0xffffffffu, upto, 31);
+    before = upto - mine;
+    const uint32_t here = __ballot_sync(0xffffffffu, begin_run<RP>(p, w, group, r0, before, mine, &first_r, &first_start));
+    const int from = here != 0u ? __ffs(here) - 1 : 0;
+    first_r = __shfl_sync(0xffffffffu, first_r, from);
+    first_start = __shfl_sync(0xffffffffu, first_start, from);
+  } else {
+    before = scan_threads<kThreads>(mine, scratch, &w.work);
+    if (begin_run<RP>(p, w, group, r0, before, mine, &first_r, &first_start)) {
+      scratch[kWarps] = first_r;
+      scratch[kWarps + 1] = first_start;
+    }
+    __syncthreads();
+    first_r = (int)scratch[kWarps];
+    first_start = scratch[kWarps + 1];
   }
-  __syncthreads();
-  const bool works = w.begin < w.end;
   w.at = w.begin;
-  w.first_r = w.r = works ? (int)scratch[kWarps] : 0;
-  w.first_start = w.start = works ? scratch[kWarps + 1] : 0;
-  w.kvh = run.hslot;
-  w.heads = run.heads;
-  return run;
+  w.first_r = w.r = first_r;
+  w.first_start = w.start = first_start;
+  return w;
 }
 
 // Barrier of the softmax warps that tells whether any of them has seen `x`.
@@ -219,45 +268,50 @@ __device__ __forceinline__ float* partial_slot(const Kv16Params& p, int cta, boo
   return base + (int64_t)(2 * cta + (begins ? 1 : 0)) * (RP * (HD + 2));  // [RP][HD] O, [RP] ref, [RP] l
 }
 
-// Merges the pieces of a row tile, left by the CTAs of groups g0 .. g0 + pieces - 1, and writes its rows.
-template <int HD, int RP>
+// Merges the pieces of a row tile, left by the CTAs of groups g0 .. g0 + pieces - 1, and writes its rows: a warp per row, a lane per
+// four columns.  The statistics and columns of eight pieces (four at 256 dims) are loaded together; the running sums are rescaled when a later piece has the
+// larger ref.
+template <int HD, int RP, bool kHalf>
 __device__ __forceinline__ void merge_pieces(const Kv16Params& p, const Piece& it, int kvh, int g0, int pieces, int heads, int hslot) {
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  constexpr int kVec = HD >= 128 ? HD / 128 : 1;
+  constexpr int kVec = HD >= 128 ? HD / 128 : 1, kBatch = 8 / kVec;
+  const int d0 = (HD == 64 ? lane & 15 : lane) * 4;
+#pragma unroll 1
   for (int n = warp; n < it.rows; n += 4) {
-    auto slot = [&](int k) { return partial_slot<HD, RP>(p, (g0 + k) * heads + hslot, k == 0); };
-    float top = -INFINITY;
-    for (int k = lane; k < pieces; k += 32) top = fmaxf(top, __ldcg(slot(k) + RP * HD + n));
-    top = redux_max(top);
-    const float use = top == -INFINITY ? 0.f : top;
-    float l = 0.f;
-    for (int k = lane; k < pieces; k += 32) {
-      const float* s = slot(k) + RP * HD + n;
-      l = fmaf(kv16_exp2(__ldcg(s) - use), __ldcg(s + RP), l);
-    }
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) l += __shfl_xor_sync(0xffffffffu, l, o);
-    float acc[kVec][4];
+    float top = -INFINITY, l = 0.f, acc[kVec][4];
 #pragma unroll
     for (int v = 0; v < kVec; ++v) acc[v][0] = acc[v][1] = acc[v][2] = acc[v][3] = 0.f;
-    const int d0 = (HD == 64 ? lane & 15 : lane) * 4;
-    constexpr int kBatch = 8;
+#pragma unroll 1
     for (int k0 = 0; k0 < pieces; k0 += kBatch) {
       float4 o[kBatch][kVec];
-      float w[kBatch];
+      float ref[kBatch], sum[kBatch];
 #pragma unroll
       for (int b = 0; b < kBatch; ++b) {
-        const float* s = slot(min(k0 + b, pieces - 1));
-        w[b] = __ldcg(s + RP * HD + n);
+        const int k = min(k0 + b, pieces - 1);
+        const float* s = partial_slot<HD, RP>(p, (g0 + k) * heads + hslot, k == 0);
+        ref[b] = __ldcg(s + RP * HD + n);
+        sum[b] = __ldcg(s + RP * HD + RP + n);
 #pragma unroll
         for (int v = 0; v < kVec; ++v) o[b][v] = __ldcg(reinterpret_cast<const float4*>(s + n * HD + v * 128 + d0));
       }
+      float to = top;
+#pragma unroll
+      for (int b = 0; b < kBatch; ++b) to = fmaxf(to, ref[b]);
+      const float use = to == -INFINITY ? 0.f : to, alpha = kv16_exp2(top - use);
+      top = to;
+      l *= alpha;
+#pragma unroll
+      for (int v = 0; v < kVec; ++v) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) acc[v][e] *= alpha;
+      }
 #pragma unroll
       for (int b = 0; b < kBatch; ++b) {
-        const float f = k0 + b < pieces ? kv16_exp2(w[b] - use) : 0.f;
+        if (k0 + b >= pieces) break;
+        const float f = kv16_exp2(ref[b] - use);
+        l = fmaf(f, sum[b], l);
 #pragma unroll
         for (int v = 0; v < kVec; ++v) {
-          if (k0 + b >= pieces) continue;
           acc[v][0] = fmaf(f, o[b][v].x, acc[v][0]);
           acc[v][1] = fmaf(f, o[b][v].y, acc[v][1]);
           acc[v][2] = fmaf(f, o[b][v].z, acc[v][2]);
@@ -271,17 +325,11 @@ __device__ __forceinline__ void merge_pieces(const Kv16Params& p, const Piece& i
     uint8_t* out = p.out + (int64_t)token * p.out_stride_token + (int64_t)head * p.out_stride_head;
 #pragma unroll
     for (int v = 0; v < kVec; ++v) {
-      uint2 w;
-      if (p.dtype == PTH_ATTN_F16) {
-        const __half2 a = __floats2half2_rn(acc[v][0] * inv, acc[v][1] * inv), b = __floats2half2_rn(acc[v][2] * inv, acc[v][3] * inv);
-        w = make_uint2(*reinterpret_cast<const uint32_t*>(&a), *reinterpret_cast<const uint32_t*>(&b));
-      } else {
-        const __nv_bfloat162 a = __floats2bfloat162_rn(acc[v][0] * inv, acc[v][1] * inv), b = __floats2bfloat162_rn(acc[v][2] * inv, acc[v][3] * inv);
-        w = make_uint2(*reinterpret_cast<const uint32_t*>(&a), *reinterpret_cast<const uint32_t*>(&b));
-      }
+      const uint2 w = make_uint2(pack16<kHalf>(acc[v][0] * inv, acc[v][1] * inv), pack16<kHalf>(acc[v][2] * inv, acc[v][3] * inv));
       if (HD >= 128 || lane < 16) *reinterpret_cast<uint2*>(out + (v * 128 + d0) * 2) = w;
     }
-    if (lane == 0 && p.lse != nullptr) p.lse[(int64_t)token * p.num_q_heads + head] = l == 0.f ? -INFINITY : (use + log2f(l)) * kLn2;
+    if (lane == 0 && p.lse != nullptr)
+      p.lse[(int64_t)token * p.num_q_heads + head] = l == 0.f ? -INFINITY : ((top == -INFINITY ? 0.f : top) + log2f(l)) * kLn2;
   }
 }
 
@@ -310,6 +358,7 @@ __global__ void __launch_bounds__(kThreads, (Geo<HD, RP>::ctas)) kv16_short_kern
       }
       tc::mbar_init(&bars[Bars::p_ready], kSoftmaxThreads);
       tc::mbar_init(&bars[Bars::pv_done], 1);
+      PieceQueue(nullptr, &bars[Bars::queue]).init(kThreads / 32 - 1);
       *abort_flag = 0;
       tc::mbar_init_fence();
     }
@@ -319,18 +368,26 @@ __global__ void __launch_bounds__(kThreads, (Geo<HD, RP>::ctas)) kv16_short_kern
   }
   pdl_wait();
 
-  const ShortRun<RP> run = find_run<RP, kThreads>(p, reinterpret_cast<long long*>(smem + G::misc + 16));
-  zero_requests<HD, RP, kThreads>(p);
+  ShortWalk<RP> walk;
+  if (p.num_reqs > kWarpReqs) walk = find_run<RP>(p, reinterpret_cast<long long*>(smem + G::misc + 16));
   tc::fence_before_sync();
   __syncthreads();
   tc::fence_after_sync();
   const uint32_t tmem_base = *tslot;
-  const int heads = run.heads, hslot = run.hslot;
+  PieceQueue queue(reinterpret_cast<Piece*>(smem + G::pieces), &bars[Bars::queue]);
   bool ok = true;
 
-  if (warp >= kLoadWarp && warp < kMmaWarp) {
+  if (warp == kScheduleWarp) {
+    // =========================== schedule ========================================
+    if (p.num_reqs <= kWarpReqs) walk = find_run<RP>(p, nullptr);
+    Piece it;
+    while (walk.next(p, &it)) ok &= queue.put(it, abort_flag);
+    it.tiles = 0;
+    ok &= queue.put(it, abort_flag);
+  } else if (warp >= kLoadWarp && warp < kMmaWarp) {
     // =========================== copies ==========================================
     // A warp owns 32 keys of every tile: lane l knows where key l of them lies.
+    if constexpr (G::moves) asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(G::copy_regs));
     const int base_key = (warp - kLoadWarp) * 32;
     const uint32_t ring = tc::smem_u32(smem);
     uint32_t unit = 0, item = 0;
@@ -341,7 +398,7 @@ __global__ void __launch_bounds__(kThreads, (Geo<HD, RP>::ctas)) kv16_short_kern
       return s;
     };
     {
-      KeyLookup<ShortWalk<RP>> keys(p, run.walk, base_key + lane);
+      KeyLookup keys(p, queue, abort_flag, base_key + lane);
       bool have = keys.fetch(), have_v = false;
       long long off_v = 0;
       int64_t head_v = 0;
@@ -449,10 +506,9 @@ __global__ void __launch_bounds__(kThreads, (Geo<HD, RP>::ctas)) kv16_short_kern
       }
       ++pv_tile;
     };
-    ShortWalk<RP> w = run.walk;
     Piece it;
     bool pending = false, pending_first = false;
-    while (w.next(p, &it)) {
+    while (queue.get(&it, abort_flag)) {
       for (int t = 0; t < it.tiles; ++t) {
         qk(t == it.tiles - 1);
         if (pending) pv(pending_first);
@@ -463,15 +519,17 @@ __global__ void __launch_bounds__(kThreads, (Geo<HD, RP>::ctas)) kv16_short_kern
     if (pending) pv(pending_first);
   } else if (warp < kLoadWarp) {
     // =========================== softmax =========================================
+    if constexpr (G::moves) asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(G::softmax_regs));
     const uint32_t lane_addr = (uint32_t)(warp * 32) << 16;
     float* const wmax = reinterpret_cast<float*>(smem + G::wmax);
     float* const wsum = reinterpret_cast<float*>(smem + G::wsum);
     uint8_t* const p_img = smem + G::p + tid * 16;
     uint32_t tile = 0;
+    zero_requests<HD, RP, kSoftmaxThreads>(p);
     {
-      ShortWalk<RP> w = run.walk;
+      const int heads = min(p.num_kv_heads, (int)gridDim.x), hslot = (int)blockIdx.x % heads;
       Piece it;
-      while (w.next(p, &it)) {
+      while (queue.get(&it, abort_flag)) {
         const int kvh = it.kvh;
         float ref[RP], l[RP];
 #pragma unroll
@@ -557,8 +615,10 @@ __global__ void __launch_bounds__(kThreads, (Geo<HD, RP>::ctas)) kv16_short_kern
         // ---- the piece's rows ----
 #pragma unroll
         for (int n = 0; n < RP; ++n) {
+          if (n < it.rows) {
 #pragma unroll
-          for (int o = 16; o > 0; o >>= 1) l[n] += __shfl_xor_sync(0xffffffffu, l[n], o);
+            for (int o = 16; o > 0; o >>= 1) l[n] += __shfl_xor_sync(0xffffffffu, l[n], o);
+          }
         }
         if (lane == 0) {
 #pragma unroll
@@ -586,7 +646,7 @@ __global__ void __launch_bounds__(kThreads, (Geo<HD, RP>::ctas)) kv16_short_kern
                   int token, head;
                   row_of(p, it.first_token, kvh, it.row0 + n, &token, &head);
                   store_out_elem(p.out + (int64_t)token * p.out_stride_token + (int64_t)head * p.out_stride_head, d, kHalf ? PTH_ATTN_F16 : PTH_ATTN_BF16,
-                                 l[n] == 0.f ? 0.f : v / l[n]);
+                                 l[n] == 0.f ? 0.f : __fdividef(v, l[n]));
                 } else {
                   slot[n * HD + d] = v;
                 }
@@ -612,16 +672,16 @@ __global__ void __launch_bounds__(kThreads, (Geo<HD, RP>::ctas)) kv16_short_kern
           }
         }
         if (!whole) {
-          const int g0 = run.owner(it.start), g1 = run.owner(it.start + it.row_tile_tiles - 1);
-          __threadfence();
+          const int g0 = it.first_cta, g1 = it.last_cta;   // (groups)
           softmax_sync();
           int* const counter = reinterpret_cast<int*>(p.workspace) + g0 * heads + hslot;
-          if (tid == 0) *arrival = atomicAdd(counter, 1);
+          if (tid == 0) {
+            *arrival = arrive_at(counter);
+            if (*arrival == g1 - g0) *counter = 0;   // (for the next call)
+          }
           softmax_sync();
           if (*arrival == g1 - g0) {
-            __threadfence();
-            if (tid == 0) *counter = 0;   // (for the next call)
-            merge_pieces<HD, RP>(p, it, kvh, g0, g1 - g0 + 1, heads, hslot);
+            merge_pieces<HD, RP, kHalf>(p, it, kvh, g0, g1 - g0 + 1, heads, hslot);
           }
         }
         softmax_sync();  // (the sums and the arrival have been read)

@@ -3,9 +3,9 @@
 // Orientation: query rows on the MMA's M dimension, a thread per row in the softmax:
 //   S[row, key] = sum_d Q[row, d] K[key, d]       A = Q, B = K as it lies in the cache (K-major), accumulator in TMEM
 //   O[row, d]  += sum_key P[row, key] V[key, d]   A = P in TMEM over S, B = V as it lies in the cache (MN-major)
-// A CTA owns 256 rows (two MMA row tiles of 128) at 64 and 128 dims, so that every K and V tile serves twice and the tensor core
-// works on one row tile while the other's softmax runs; at 256 dims, where O alone takes half of TMEM, 128 rows with
-// two S buffers, which do the same for two tiles of keys.
+// An SM holds two row tiles of 128 rows, so that the tensor core and one's softmax have work while the other's waits: of one CTA at
+// 128 dims, where every K and V tile then serves twice, of two CTAs at 64 dims, whose items may be different ones (a request's
+// last rows seldom fill both).  At 256 dims O alone takes half of TMEM: one row tile.
 //
 // Softmax in one pass: ref is a running bound of a row's scores (log2 units), P = 2^(s - ref), l = sum P.  It is set kGain below the
 // maximum of a row's first 64 keys.  Later ones need no maximum: the sum of 64 P, which the row sum takes anyway, says
@@ -48,13 +48,14 @@ namespace {
 constexpr float kGain = 7.f;
 constexpr float kMostSum = 32768.f;    // of 64 P: none of them leaves fp16's range
 constexpr int kLoadWarps = 4;
-constexpr int kTallReqs = 8192;        // requests of a launch (the API refuses more)
-constexpr int kTallCtas = 160;
+constexpr int kPlanReqs = 4096;        // requests up to which a launch may go out in waves
+constexpr int kTallSms = 160;
 constexpr long long kL2Keys = 48 << 20;   // bytes of keys and values that a launch may spread its CTAs over
 
 template <int HD>
 struct Tall {
-  static constexpr int rts = HD == 256 ? 1 : 2;      // row tiles of 128 rows
+  static constexpr int rts = HD == 128 ? 2 : 1;      // row tiles of 128 rows
+  static constexpr int ctas = HD == 64 ? 2 : 1;      // per SM
   static constexpr int rows = 128 * rts;
   static constexpr int keys = HD == 256 ? 128 : 64;  // of a step, one of the two S buffers of a row tile
   static constexpr int steps = kTile / keys;         // of a KV tile
@@ -63,23 +64,28 @@ struct Tall {
   static constexpr int parts = HD / dims;
   static constexpr int unit = kTile * dims * 2;
   static constexpr int qtile = 128 * HD * 2;         // Q of a row tile: slabs of 64 dims, 128 rows of 128 bytes each
-  static constexpr int units = HD == 64 ? 8 : 5;
+  static constexpr int units = 5;
   static constexpr int softmax_warps = 4 * rts;
-  static constexpr int load_warp = softmax_warps, mma_warp = load_warp + kLoadWarps;
-  static constexpr int threads = (mma_warp + rts) * 32;   // (an MMA warp per row tile)
-  // Registers: 14 warps start with 128 each (9 with 168), which setmaxnreg moves from the copies to the softmax.
-  static constexpr int start_regs = HD == 256 ? 168 : 128, copy_regs = HD == 256 ? 72 : 56, softmax_regs = HD == 256 ? 232 : 160;
-  static_assert(softmax_warps * softmax_regs + kLoadWarps * copy_regs + rts * start_regs <= (threads / 32) * start_regs, "a split that the launch holds");
-  static constexpr int s_col = 0, o_col = 256;       // S(rt, b) at (2 rt + b) keys, O(rt) at 256 + rt HD
+  static constexpr int load_warp = softmax_warps, mma_warp = load_warp + kLoadWarps, schedule_warp = mma_warp + rts;   // (an MMA warp per row tile)
+  static constexpr int threads = (schedule_warp + 1) * 32;
+  // Registers that a thread starts with, which setmaxnreg moves from the copies to the softmax.
+  static constexpr int start_regs = HD == 256 ? 168 : HD == 128 ? 128 : 96;
+  static constexpr int copy_regs = HD == 256 ? 72 : 56, softmax_regs = HD == 256 ? 232 : HD == 128 ? 160 : 136;
+  static_assert(softmax_warps * softmax_regs + kLoadWarps * copy_regs <= (softmax_warps + kLoadWarps) * start_regs, "a split that the launch holds");
+  static constexpr int s_col = 0, o_col = 2 * rts * keys;   // TMEM columns: S(rt, b) at (2 rt + b) keys, O(rt) at o_col + rt HD
+  static constexpr int tmem = HD == 64 ? 256 : 512;
+  static_assert(o_col + rts * HD <= tmem, "accumulators");
   // shared memory, behind the first 1,024-byte boundary
+  static constexpr int most_ctas = kTallSms * ctas;
   static constexpr int q = units * unit;
   static constexpr int bars = q + rts * qtile;
-  static constexpr int n_bars = 2 * units + 2 * rts + 20;
-  static constexpr int misc = bars + n_bars * 8;
-  static constexpr int bounds = misc + 256;          // TallPlan's
-  static constexpr int total = bounds + (kTallCtas + 1) * 8 + 1024;
-  static_assert(kTallReqs * 16 + 16 <= units * unit + rts * qtile, "the plan's arrays lie where keys and queries come later");
-  static_assert(total <= 232448, "shared memory of one CTA");
+  static constexpr int n_bars = 2 * units + 2 * rts + 20 + 2 * kQueue;
+  static constexpr int pieces = bars + n_bars * 8;   // PieceQueue's entries
+  static constexpr int misc = pieces + kQueue * 64;
+  static constexpr int bounds = misc + 32;           // the plan's, and its scratch in front
+  static constexpr int total = bounds + (most_ctas + 1) * 8 + 1024;
+  static_assert(kPlanReqs * 16 + 16 <= units * unit + rts * qtile, "the plan's arrays lie where keys and queries come later");
+  static_assert(total <= (ctas == 2 ? 115712 : 232448), "shared memory");
 };
 template <int HD>
 struct TallBars {  // behind [units] full, [units] empty
@@ -88,18 +94,8 @@ struct TallBars {  // behind [units] full, [units] empty
   static constexpr int p_ready = s_ready + 4;        // [4][2 halves]
   static constexpr int pv_half = p_ready + 8;        // [4] PV of the first of two halves
   static constexpr int pv_done = pv_half + 4;        // [4]
+  static constexpr int queue = pv_done + 4;
 };
-
-template <bool kHalf>
-__device__ __forceinline__ uint32_t pack16(float a, float b) {
-  if constexpr (kHalf) {
-    const __half2 h = __floats2half2_rn(a, b);
-    return *reinterpret_cast<const uint32_t*>(&h);
-  } else {
-    const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
-    return *reinterpret_cast<const uint32_t*>(&h);
-  }
-}
 
 // Tiled TMA load of one box of a rank-4 tensor map into shared memory.
 __device__ __forceinline__ void tma_load_4d(uint32_t dst, const CUtensorMap* map, int x, int y, int z, int w, uint64_t* bar) {
@@ -138,17 +134,35 @@ __device__ __forceinline__ int piece_steps(const Piece& it) {
   return (min(it.tiles * kTile, it.hi - it.key0) + kKeys - 1) / kKeys;
 }
 
-// Walk over the pieces of a CTA: its items of the waves, then its run of the tail.
+// Walk over the pieces of a CTA: its items of the waves, then its run of the rest.
 template <int RP>
 struct TallWalk {
   int wave, waves, ctas, item;    // item: of the current wave
   int r, first_item;              // request of the item, items in front of it
-  long long at, end;              // the run, in tiles of the whole sequence
+  long long at, end;              // the run, in KV tiles of the whole sequence
   int tail_r;
   long long tail_start;           // of request tail_r in the sequence
+  long long base, work;           // where the runs' tiles begin in the sequence, and how many there are
+  int runs;                       // without waves: that they are cut into, equally
+  const long long* bounds;        // with waves: where the CTAs' runs begin, behind `base`
+  // CTA that has tile x of the sequence in its run.
+  __device__ __forceinline__ int owner(long long x) const {
+    x -= base;
+    if (waves == 0) return (int)(((x + 1) * runs - 1) / work);
+    int lo = 0, hi = ctas - 1;
+    while (lo < hi) {
+      const int mid = (lo + hi + 1) >> 1;
+      if (bounds[mid] <= x) lo = mid; else hi = mid - 1;
+    }
+    return lo;
+  }
   __device__ __forceinline__ bool next(const Kv16Params& p, Piece* out) {
-    if (wave < waves) {
-      ReqShape s = req_shape<RP>(p, r);
+    const bool whole = wave < waves;
+    if (!whole && at >= end) return false;
+    ReqShape s;
+    int it, tile, count;   // item of the request, tiles of it
+    if (whole) {
+      s = req_shape<RP>(p, r);
       int n = s.tiles > 0 ? s.row_tiles * p.num_kv_heads : 0;
       while (item >= first_item + n) {
         first_item += n;
@@ -156,171 +170,207 @@ struct TallWalk {
         s = req_shape<RP>(p, r);
         n = s.tiles > 0 ? s.row_tiles * p.num_kv_heads : 0;
       }
-      const int off = item - first_item, kvh = (int)((uint32_t)off / (uint32_t)s.row_tiles);
-      make_piece<RP>(p, s, r, kvh, off - kvh * s.row_tiles, 0, s.tiles, 0, out);
+      it = item - first_item;
+      tile = 0;
+      count = s.tiles;
+      out->r = r;
+      out->first_cta = out->last_cta = 0;
       ++wave;
       item += ctas;
-      return true;
-    }
-    if (at >= end) return false;
-    ReqShape s = req_shape<RP>(p, tail_r);
-    long long n = (long long)s.tiles * s.row_tiles * p.num_kv_heads;
-    while (at >= tail_start + n) {
-      tail_start += n;
-      ++tail_r;
+    } else {
       s = req_shape<RP>(p, tail_r);
-      n = (long long)s.tiles * s.row_tiles * p.num_kv_heads;
+      long long n = (long long)s.tiles * s.row_tiles * p.num_kv_heads;
+      while (at >= tail_start + n) {
+        tail_start += n;
+        ++tail_r;
+        s = req_shape<RP>(p, tail_r);
+        n = (long long)s.tiles * s.row_tiles * p.num_kv_heads;
+      }
+      const long long off = at - tail_start;
+      it = (int)(off / s.tiles);
+      tile = (int)(off - (long long)it * s.tiles);
+      count = (int)min((long long)(s.tiles - tile), end - at);
+      out->r = tail_r;
+      out->first_cta = owner(at - tile);
+      out->last_cta = owner(at - tile + s.tiles - 1);
+      at += count;
     }
-    const long long off = at - tail_start;
-    const int it = (int)(off / s.tiles), tile = (int)(off - (long long)it * s.tiles);
-    const int kvh = (int)((uint32_t)it / (uint32_t)s.row_tiles);
-    const int count = (int)min((long long)(s.tiles - tile), end - at);
-    make_piece<RP>(p, s, tail_r, kvh, it - kvh * s.row_tiles, tile, count, tail_start + (long long)it * s.tiles, out);
-    at += count;
+    const int kvh = (int)((uint32_t)it / (uint32_t)s.row_tiles), rt = it - kvh * s.row_tiles;
+    out->kvh = kvh;
+    out->row0 = rt * RP;
+    out->rows = min(RP, s.tokens * p.group - rt * RP);
+    out->first_token = s.first;
+    out->key0 = (s.lo / kTile + tile) * kTile;
+    out->tiles = count;
+    out->lo = s.lo;
+    out->hi = s.hi;
+    out->begins = tile == 0;
+    out->ends = tile + count == s.tiles;
+    out->sparse = waves > 0;
     return true;
   }
 };
 
-// Who has which items (see the head of this file).  Every CTA works it out for itself.  Requests: tile_first[r] KV tiles and
-// item_first[r] items lie in front of r, whose items have tiles[r] KV tiles.  arrays: room for them; bounds [CTAs + 1]: where
-// the runs begin, behind tile `base` of the sequence.
-template <int HD, int RP, int kThreads>
-__device__ __forceinline__ TallWalk<RP> make_plan(const Kv16Params& p, uint8_t* arrays, long long* bounds, long long* scratch, long long* base) {
-  const int R = p.num_reqs, C = (int)gridDim.x, tid = threadIdx.x, lane = tid & 31;
-  long long* const tile_first = reinterpret_cast<long long*>(arrays);
-  int* const item_first = reinterpret_cast<int*>(tile_first + R + 1);
-  int* const tiles = item_first + R + 1;
+// Who has which items (see the head of this file), worked out by all threads of every CTA.  arrays: room for 16 bytes a request;
+// bounds [CTAs + 1].  The result is good in every thread.
+template <int HD, int RP, int kThreads, int kMostCtas>
+__device__ __forceinline__ TallWalk<RP> make_plan(const Kv16Params& p, uint8_t* arrays, long long* bounds) {
+  constexpr int kWarps = kThreads / 32;
+  static_assert(3 * kWarps <= kMostCtas, "scratch");
+  long long* const scratch = bounds;
+  const int R = p.num_reqs, C = (int)gridDim.x, tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int per = (R + kThreads - 1) / kThreads, r0 = min(R, tid * per), r1 = min(R, r0 + per);
-  long long my_items = 0, my_tiles = 0, my_keys = 0;
+  // items (0), KV tiles of all items (1), KV tiles of the requests' keys (2): in front of this thread's requests, and in all
+  long long mine[3] = {0, 0, 0}, before[3], total[3] = {0, 0, 0};
+#pragma unroll 1
+  for (int r = r0; r < r1; ++r) {
+    const ReqShape s = req_shape<RP>(p, r);
+    const int n = s.tiles > 0 ? s.row_tiles * p.num_kv_heads : 0;
+    mine[0] += n;
+    mine[1] += (long long)n * s.tiles;
+    mine[2] += s.tiles;
+  }
+#pragma unroll
+  for (int k = 0; k < 3; ++k) {
+    long long upto = mine[k];
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const long long x = __shfl_up_sync(0xffffffffu, upto, o);
+      if (lane >= o) upto += x;
+    }
+    if (lane == 31) scratch[3 * warp + k] = upto;
+    before[k] = upto - mine[k];
+  }
+  __syncthreads();
+#pragma unroll 1
+  for (int w = 0; w < kWarps; ++w) {
+#pragma unroll
+    for (int k = 0; k < 3; ++k) {
+      const long long x = scratch[3 * w + k];
+      if (w < warp) before[k] += x;
+      total[k] += x;
+    }
+  }
+  TallWalk<RP> w;
+  w.wave = 0;
+  w.ctas = C;
+  w.item = (int)blockIdx.x;
+  w.r = w.first_item = 0;
+  w.base = 0;
+  w.bounds = bounds;
+  const bool waves = total[2] * p.num_kv_heads * ((long long)kTile * HD * 4) > kL2Keys && total[0] >= 2 * C && R <= kPlanReqs;
+  w.waves = waves ? (int)(total[0] / C) - 1 : 0;
+  if (!waves) {
+    w.work = total[1];
+    w.runs = (int)min((long long)C, max(w.work, 1ll));   // (none of them empty)
+    w.at = (int)blockIdx.x < w.runs ? w.work * blockIdx.x / w.runs : w.work;
+    w.end = (int)blockIdx.x < w.runs ? w.work * (blockIdx.x + 1) / w.runs : w.work;
+    __syncthreads();   // (the sums have been read)
+    if (w.at < w.end && before[1] <= w.at && w.at < before[1] + mine[1]) {
+      long long start = before[1];
+      int r = r0;
+#pragma unroll 1
+      for (;; ++r) {
+        const ReqShape s = req_shape<RP>(p, r);
+        const long long n = (long long)s.tiles * s.row_tiles * p.num_kv_heads;
+        if (w.at < start + n) break;
+        start += n;
+      }
+      scratch[0] = r;
+      scratch[1] = start;
+    }
+    __syncthreads();
+    w.tail_r = (int)scratch[0];
+    w.tail_start = scratch[1];
+    return w;
+  }
+  // tile_first[r] KV tiles and item_first[r] items lie in front of request r, whose items have tiles[r] KV tiles
+  long long* const tile_first = reinterpret_cast<long long*>(arrays);
+  int* const item_first = reinterpret_cast<int*>(tile_first + R);
+  int* const tiles = item_first + R;
+#pragma unroll 1
   for (int r = r0; r < r1; ++r) {
     const ReqShape s = req_shape<RP>(p, r);
     const int n = s.tiles > 0 ? s.row_tiles * p.num_kv_heads : 0;
     tiles[r] = s.tiles;
-    my_items += n;
-    my_tiles += (long long)n * s.tiles;
-    my_keys += s.tiles;
-  }
-  long long items, total, keys;
-  long long ib = scan_threads<kThreads>(my_items, scratch, &items);
-  __syncthreads();
-  long long tb = scan_threads<kThreads>(my_tiles, scratch, &total);
-  __syncthreads();
-  scan_threads<kThreads>(my_keys, scratch, &keys);
-  for (int r = r0; r < r1; ++r) {
-    const ReqShape s = req_shape<RP>(p, r);
-    const int n = s.tiles > 0 ? s.row_tiles * p.num_kv_heads : 0;
-    item_first[r] = (int)ib;
-    tile_first[r] = tb;
-    ib += n;
-    tb += (long long)n * s.tiles;
-  }
-  if (tid == 0) {
-    item_first[R] = (int)items;
-    tile_first[R] = total;
+    item_first[r] = (int)before[0];
+    tile_first[r] = before[1];
+    before[0] += n;
+    before[1] += (long long)n * s.tiles;
   }
   __syncthreads();
   // request of an item, or of a tile of the sequence: the last that begins at or in front of it
-  auto of_item = [&](long long x) {
+  auto last_of = [&](const auto* first, long long x) {
     int lo = 0, hi = R - 1;
+#pragma unroll 1
     while (lo < hi) {
       const int mid = (lo + hi + 1) >> 1;
-      if (item_first[mid] <= x) lo = mid; else hi = mid - 1;
+      if (first[mid] <= x) lo = mid; else hi = mid - 1;
     }
     return lo;
   };
-  auto of_tile = [&](long long x) {
-    int lo = 0, hi = R - 1;
-    while (lo < hi) {
-      const int mid = (lo + hi + 1) >> 1;
-      if (tile_first[mid] <= x) lo = mid; else hi = mid - 1;
-    }
-    return lo;
-  };
-  const long long bytes = keys * p.num_kv_heads * ((long long)kTile * HD * 4);
-  const int waves = bytes > kL2Keys && items >= 2 * C ? (int)(items / C) - 1 : 0;
-  long long first_tail = 0;   // tile of the sequence
-  if (waves > 0) {
-    const long long f = (long long)waves * C;
-    const int r = of_item(f);
-    first_tail = tile_first[r] + (f - item_first[r]) * tiles[r];
-  }
-  const long long tail = total - first_tail;
-  if (waves == 0) {
-    const long long runs = min((long long)C, max(tail, 1ll));   // (none of them empty)
-    for (int c = tid; c <= C; c += kThreads) bounds[c] = c < runs ? tail * c / runs : tail;
-  } else {
-    // CTA c has load(c) tiles of the waves; the tail fills all up to a level: the smallest that holds it
-    for (int c = tid; c < C; c += kThreads) {
-      long long load = 0;
-      for (int w = 0; w < waves; ++w) load += tiles[of_item(c + (long long)w * C)];
-      bounds[c] = load;
-    }
-    __syncthreads();
-    if (tid < 32) {
-      long long load[kTallCtas / 32], most = 0;
-#pragma unroll
-      for (int i = 0; i < kTallCtas / 32; ++i) {
-        load[i] = lane + 32 * i < C ? bounds[lane + 32 * i] : (1ll << 60);
-        if (load[i] < (1ll << 60)) most = max(most, load[i]);
-      }
-#pragma unroll
-      for (int o = 16; o > 0; o >>= 1) most = max(most, __shfl_xor_sync(0xffffffffu, most, o));
-      long long lo = total / C, hi = most + tail / C + 1;   // (at lo there may be too little room, at hi there is enough)
-      while (lo < hi) {
-        const long long mid = (lo + hi) >> 1;
-        long long room = 0;
-#pragma unroll
-        for (int i = 0; i < kTallCtas / 32; ++i) room += max(0ll, mid - load[i]);
-#pragma unroll
-        for (int o = 16; o > 0; o >>= 1) room += __shfl_xor_sync(0xffffffffu, room, o);
-        if (room >= tail) hi = mid; else lo = mid + 1;
-      }
-      // (CTAs in order: lane + 32 i, a row of lanes at a time)
-      long long upto = 0;
-#pragma unroll
-      for (int i = 0; i < kTallCtas / 32; ++i) {
-        const long long mine = max(0ll, lo - load[i]);
-        long long inc = mine;
-#pragma unroll
-        for (int o = 1; o < 32; o <<= 1) {
-          const long long x = __shfl_up_sync(0xffffffffu, inc, o);
-          if (lane >= o) inc += x;
-        }
-        if (lane + 32 * i < C) bounds[lane + 32 * i] = min(tail, upto + inc - mine);
-        upto += __shfl_sync(0xffffffffu, inc, 31);
-      }
-      if (lane == 0) bounds[C] = tail;
-    }
+  const long long f = (long long)w.waves * C;
+  const int fr = last_of(item_first, f);
+  w.base = tile_first[fr] + (f - item_first[fr]) * tiles[fr];
+  w.work = total[1] - w.base;
+  w.runs = 0;
+  // CTA c has load(c) tiles of the waves; the rest fills all up to a level: the smallest that holds it
+#pragma unroll 1
+  for (int c = tid; c < C; c += kThreads) {
+    long long load = 0;
+#pragma unroll 1
+    for (int k = 0; k < w.waves; ++k) load += tiles[last_of(item_first, c + (long long)k * C)];
+    bounds[c] = load;
   }
   __syncthreads();
-  TallWalk<RP> w;
-  w.wave = 0;
-  w.waves = waves;
-  w.ctas = C;
-  w.item = (int)blockIdx.x;
-  w.r = of_item(w.item);
-  w.first_item = R > 0 ? item_first[w.r] : 0;
-  w.at = first_tail + bounds[blockIdx.x];
-  w.end = first_tail + bounds[blockIdx.x + 1];
-  w.tail_r = of_tile(w.at);
+  if (tid < 32) {
+    constexpr int kRows = kMostCtas / 32;   // (CTAs lane + 32 i)
+    long long most = 0;
+#pragma unroll 1
+    for (int c = lane; c < C; c += 32) most = max(most, bounds[c]);
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) most = max(most, __shfl_xor_sync(0xffffffffu, most, o));
+    long long lo = total[1] / C, hi = most + w.work / C + 1;   // (at lo there may be too little room, at hi there is enough)
+#pragma unroll 1
+    while (lo < hi) {
+      const long long mid = (lo + hi) >> 1;
+      long long room = 0;
+#pragma unroll 1
+      for (int c = lane; c < C; c += 32) room += max(0ll, mid - bounds[c]);
+#pragma unroll
+      for (int o = 16; o > 0; o >>= 1) room += __shfl_xor_sync(0xffffffffu, room, o);
+      if (room >= w.work) hi = mid; else lo = mid + 1;
+    }
+    long long upto = 0;
+#pragma unroll 1
+    for (int i = 0; i < kRows; ++i) {
+      const int c = lane + 32 * i;
+      const long long share = c < C ? max(0ll, lo - bounds[c]) : 0;
+      long long inc = share;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const long long x = __shfl_up_sync(0xffffffffu, inc, o);
+        if (lane >= o) inc += x;
+      }
+      if (c < C) bounds[c] = min(w.work, upto + inc - share);
+      upto += __shfl_sync(0xffffffffu, inc, 31);
+    }
+    if (lane == 0) bounds[C] = w.work;
+  }
+  __syncthreads();
+  w.r = last_of(item_first, w.item);
+  w.first_item = item_first[w.r];
+  w.at = w.base + bounds[blockIdx.x];
+  w.end = w.base + bounds[blockIdx.x + 1];
+  w.tail_r = last_of(tile_first, w.at);
   w.tail_start = tile_first[w.tail_r];
-  *base = first_tail;
   tc::fence_async_smem();   // (boxes are written where the arrays are, through the other proxy)
   __syncthreads();
   return w;
 }
-// CTA that has tile x of the sequence in its run.
-__device__ __forceinline__ int tall_owner(const long long* bounds, int ctas, long long x) {
-  int lo = 0, hi = ctas - 1;
-  while (lo < hi) {
-    const int mid = (lo + hi + 1) >> 1;
-    if (bounds[mid] <= x) lo = mid; else hi = mid - 1;
-  }
-  return lo;
-}
 
 template <int HD, bool kHalf>
-__global__ void __launch_bounds__(Tall<HD>::threads, 1) kv16_tall_kernel(const __grid_constant__ Kv16Params p, const __grid_constant__ CUtensorMap k_map,
+__global__ void __launch_bounds__(Tall<HD>::threads, Tall<HD>::ctas) kv16_tall_kernel(const __grid_constant__ Kv16Params p, const __grid_constant__ CUtensorMap k_map,
                                                                         const __grid_constant__ CUtensorMap v_map) {
   using G = Tall<HD>;
   using B = TallBars<HD>;
@@ -352,25 +402,32 @@ __global__ void __launch_bounds__(Tall<HD>::threads, 1) kv16_tall_kernel(const _
         tc::mbar_init(&bars[B::pv_half + i], 1);
         tc::mbar_init(&bars[B::pv_done + i], 1);
       }
+      PieceQueue(nullptr, &bars[B::queue]).init(G::threads / 32 - 1);
       *abort_flag = 0;
       tc::mbar_init_fence();
     }
     __syncwarp();
-    tc::tmem_alloc(tslot, 512);
+    tc::tmem_alloc(tslot, G::tmem);
     tc::tmem_relinquish();
   }
   pdl_wait();
   long long* const bounds = reinterpret_cast<long long*>(smem + G::bounds);
-  long long base;
-  const TallWalk<RP> walk = make_plan<HD, RP, G::threads>(p, smem, bounds, reinterpret_cast<long long*>(smem + G::misc + 16), &base);
-  zero_requests<HD, RP, G::threads>(p);
+  const TallWalk<RP> plan = make_plan<HD, RP, G::threads, G::most_ctas>(p, smem, bounds);
   tc::fence_before_sync();
   __syncthreads();
   tc::fence_after_sync();
   const uint32_t tmem_base = *tslot;
+  PieceQueue queue(reinterpret_cast<Piece*>(smem + G::pieces), &bars[B::queue]);
   bool ok = true;
 
-  if (warp >= G::load_warp && warp < G::mma_warp) {
+  if (warp == G::schedule_warp) {
+    // =========================== schedule ========================================
+    TallWalk<RP> w = plan;
+    Piece it;
+    while (w.next(p, &it)) ok &= queue.put(it, abort_flag);
+    it.tiles = 0;
+    ok &= queue.put(it, abort_flag);
+  } else if (warp >= G::load_warp && warp < G::mma_warp) {
     // =========================== copies ==========================================
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(G::copy_regs));
     const int base_key = (warp - G::load_warp) * 32;
@@ -403,7 +460,7 @@ __global__ void __launch_bounds__(Tall<HD>::threads, 1) kv16_tall_kernel(const _
       ++unit;
     };
     {
-      KeyLookup<TallWalk<RP>> keys(p, walk, base_key + lane);
+      KeyLookup keys(p, queue, abort_flag, base_key + lane);
       bool have = keys.fetch();
       while (have) {
         const int kvh = keys.it.kvh;
@@ -512,9 +569,8 @@ __global__ void __launch_bounds__(Tall<HD>::threads, 1) kv16_tall_kernel(const _
       }
       ++s_pv;
     };
-    TallWalk<RP> w = walk;
     Piece it;
-    while (w.next(p, &it)) {
+    while (queue.get(&it, abort_flag)) {
       if (it.rows <= rt * 128) {   // no rows: free the units as if they had been read
         for (int u = 0; u < 2 * G::parts * it.tiles; ++u) {
           const uint32_t s = arrived(unit + u);
@@ -541,10 +597,10 @@ __global__ void __launch_bounds__(Tall<HD>::threads, 1) kv16_tall_kernel(const _
     const int row = tid;   // of the CTA's rows
     uint32_t count = 0;    // live tiles so far
     auto rt_sync = [&] { named_barrier(1 + rt, 128); };
+    zero_requests<HD, RP, 128 * G::rts>(p);
     {
-      TallWalk<RP> w = walk;
       Piece it;
-      while (w.next(p, &it)) {
+      while (queue.get(&it, abort_flag)) {
         if (it.rows <= rt * 128) continue;
         const int kvh = it.kvh;
         const bool padding = (row & ~31) >= it.rows;   // (of the whole warp)
@@ -631,6 +687,17 @@ __global__ void __launch_bounds__(Tall<HD>::threads, 1) kv16_tall_kernel(const _
         uint8_t* const out = p.out + (int64_t)token * p.out_stride_token + (int64_t)head * p.out_stride_head;
         float* const lse = p.lse != nullptr ? p.lse + (int64_t)token * p.num_q_heads + head : nullptr;
         auto write32 = [&](const float* o, int d0) {   // 32 columns of the row
+          if (p.out_wide) {
+#pragma unroll
+            for (int c = 0; c < 2; ++c)
+              asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(out + (d0 + c * 16) * 2),
+                           "r"(pack16<kHalf>(o[c * 16], o[c * 16 + 1])), "r"(pack16<kHalf>(o[c * 16 + 2], o[c * 16 + 3])),
+                           "r"(pack16<kHalf>(o[c * 16 + 4], o[c * 16 + 5])), "r"(pack16<kHalf>(o[c * 16 + 6], o[c * 16 + 7])),
+                           "r"(pack16<kHalf>(o[c * 16 + 8], o[c * 16 + 9])), "r"(pack16<kHalf>(o[c * 16 + 10], o[c * 16 + 11])),
+                           "r"(pack16<kHalf>(o[c * 16 + 12], o[c * 16 + 13])), "r"(pack16<kHalf>(o[c * 16 + 14], o[c * 16 + 15]))
+                           : "memory");
+            return;
+          }
 #pragma unroll
           for (int c = 0; c < 4; ++c)
             *reinterpret_cast<uint4*>(out + (d0 + c * 8) * 2) =
@@ -665,52 +732,49 @@ __global__ void __launch_bounds__(Tall<HD>::threads, 1) kv16_tall_kernel(const _
         tc::fence_before_sync();
         if (!whole) {
           // (a row tile's pieces are merged by the row tile's own threads: a counter each)
-          const int c0 = tall_owner(bounds, (int)gridDim.x, it.start - base), c1 = tall_owner(bounds, (int)gridDim.x, it.start + it.row_tile_tiles - 1 - base);
-          __threadfence();
+          const int c0 = it.first_cta, c1 = it.last_cta;
+          auto none = [&](int c) { return it.sparse != 0 && bounds[c] == bounds[c + 1]; };   // (a CTA with much of the waves may have none of the rest)
           rt_sync();
-          int* const counter = reinterpret_cast<int*>(p.workspace) + 2 * c0 + rt;
-          if ((tid & 127) == 0) arrival[rt] = atomicAdd(counter, 1);
+          int* const counter = reinterpret_cast<int*>(p.workspace) + G::rts * c0 + rt;
+          if ((tid & 127) == 0) {
+            int pieces = 0;
+            for (int c = c0; c <= c1; ++c) pieces += none(c) ? 0 : 1;
+            arrival[rt] = arrive_at(counter) == pieces - 1;
+            if (arrival[rt]) *counter = 0;   // (for the next call)
+          }
           rt_sync();
-          // (a CTA with much of the waves may have none of the tail)
-          int pieces = 0;
-          for (int c = c0; c <= c1; ++c) pieces += bounds[c] < bounds[c + 1] ? 1 : 0;
-          if (arrival[rt] == pieces - 1) {
-            __threadfence();
-            if ((tid & 127) == 0) *counter = 0;   // (for the next call)
+          if (arrival[rt] && !padding) {
             auto slot = [&](int c) { return tall_slot<HD>(p, c, c == c0) + row; };
             float top = -INFINITY, sum = 0.f;
-            for (int c = c0; c <= c1; ++c)
-              if (bounds[c] < bounds[c + 1]) top = fmaxf(top, __ldcg(slot(c) + HD * RP));
-            const float use = top == -INFINITY ? 0.f : top;
+#pragma unroll 1
             for (int c = c0; c <= c1; ++c) {
-              if (bounds[c] == bounds[c + 1]) continue;
+              if (none(c)) continue;
               const float* s = slot(c) + HD * RP;
-              sum = fmaf(ex2f(__ldcg(s) - use), __ldcg(s + RP), sum);
+              const float r = __ldcg(s), l1 = __ldcg(s + RP), to = fmaxf(top, r), use = to == -INFINITY ? 0.f : to;
+              sum = fmaf(sum, ex2f(top - use), ex2f(r - use) * l1);
+              top = to;
             }
-            const float inv = sum == 0.f ? 0.f : 1.f / sum;
-            if (!padding) {
+            const float use = top == -INFINITY ? 0.f : top, inv = sum == 0.f ? 0.f : 1.f / sum;
 #pragma unroll 1
-              for (int c = 0; c < HD / 32; ++c) {
-                float o[32];
+            for (int c = 0; c < HD / 32; ++c) {
+              float o[32];
 #pragma unroll
-                for (int n = 0; n < 32; ++n) o[n] = 0.f;
+              for (int n = 0; n < 32; ++n) o[n] = 0.f;
 #pragma unroll 1
-                for (int cta = c0; cta <= c1; ++cta) {
-                  if (bounds[cta] == bounds[cta + 1]) continue;
-                  const float* s = slot(cta);
-                  const float f = ex2f(__ldcg(s + HD * RP) - use);
-                  float v[32];
+              for (int cta = c0; cta <= c1; ++cta) {
+                if (none(cta)) continue;
+                const float* s = slot(cta);
+                const float weight = __ldcg(s + HD * RP);
+                float v[32];
 #pragma unroll
-                  for (int n = 0; n < 32; ++n) v[n] = __ldcg(s + (c * 32 + n) * RP);
+                for (int n = 0; n < 32; ++n) v[n] = __ldcg(s + (c * 32 + n) * RP);
+                const float f = ex2f(weight - use) * inv;
 #pragma unroll
-                  for (int n = 0; n < 32; ++n) o[n] = fmaf(f, v[n], o[n]);
-                }
-#pragma unroll
-                for (int n = 0; n < 32; ++n) o[n] *= inv;
-                if (live) write32(o, c * 32);
+                for (int n = 0; n < 32; ++n) o[n] = fmaf(f, v[n], o[n]);
               }
-              if (live && lse != nullptr) *lse = sum == 0.f ? -INFINITY : (use + log2f(sum)) * kLn2;
+              if (live) write32(o, c * 32);
             }
+            if (live && lse != nullptr) *lse = sum == 0.f ? -INFINITY : (use + log2f(sum)) * kLn2;
           }
           rt_sync();   // (the arrival has been read)
         }
@@ -719,7 +783,7 @@ __global__ void __launch_bounds__(Tall<HD>::threads, 1) kv16_tall_kernel(const _
   }
   tc::fence_before_sync();
   __syncthreads();
-  if (warp == G::mma_warp) tc::tmem_dealloc(tmem_base, 512);
+  if (warp == G::mma_warp) tc::tmem_dealloc(tmem_base, G::tmem);
   if (tid == 0 && *abort_flag) atomicOr(&g_kv16_tall_status, 16u);
   (void)ok;
 }
@@ -775,15 +839,16 @@ cudaError_t launch_one(const Kv16Params& p, cudaStream_t stream) {
     if (dev >= 0 && dev < 64) configured[dev] = true;
   }
   const int sms = sm_count();
-  if (sms <= 0 || sms > kTallCtas) return cudaErrorInvalidDevice;
+  if (sms <= 0 || sms > kTallSms) return cudaErrorInvalidDevice;
   // Boxes take pages of a multiple of 8 slots: the swizzle repeats every 8 rows.
   Kv16Params q = p;
   q.box_slots = 0;
+  q.out_wide = reinterpret_cast<uintptr_t>(p.out) % 32 == 0 && p.out_stride_token % 32 == 0 && p.out_stride_head % 32 == 0;
   for (int slots = 32; slots >= 8 && q.box_slots == 0; slots >>= 1)
     if (p.block_size % slots == 0) q.box_slots = slots;
   CUtensorMap k_map{}, v_map{};
   if (q.box_slots > 0 && !(page_box_map(q, p.k, &k_map) && page_box_map(q, p.v, &v_map))) q.box_slots = 0;
-  return pdl_launch(kv16_tall_kernel<HD, kHalf>, dim3((unsigned)sms), dim3(G::threads), G::total, stream, q, k_map, v_map);
+  return pdl_launch(kv16_tall_kernel<HD, kHalf>, dim3((unsigned)(sms * G::ctas)), dim3(G::threads), G::total, stream, q, k_map, v_map);
 }
 template <int HD>
 cudaError_t launch_type(const Kv16Params& p, cudaStream_t stream) {
@@ -794,7 +859,7 @@ cudaError_t launch_type(const Kv16Params& p, cudaStream_t stream) {
 
 // Counters, and two partial row tiles per CTA.
 int64_t kv16_tall_workspace_bytes(int head_size, int num_sms) {
-  const int64_t rows = head_size == 256 ? 128 : 256;
+  const int64_t rows = head_size == 256 ? 128 : 256;   // of an SM's CTAs together
   return kCounterBytes + (int64_t)num_sms * 2 * rows * (head_size + 2) * 4;
 }
 
