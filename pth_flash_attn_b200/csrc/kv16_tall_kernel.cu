@@ -70,7 +70,7 @@ struct Tall {
   static constexpr int threads = (schedule_warp + 1) * 32;
   // Registers that a thread starts with, which setmaxnreg moves from the copies to the softmax.
   static constexpr int start_regs = HD == 256 ? 168 : HD == 128 ? 128 : 96;
-  static constexpr int copy_regs = HD == 256 ? 72 : 56, softmax_regs = HD == 256 ? 232 : HD == 128 ? 160 : 136;
+  static constexpr int copy_regs = HD == 256 ? 96 : 64, softmax_regs = HD == 256 ? 232 : HD == 128 ? 160 : 128;
   static_assert(softmax_warps * softmax_regs + kLoadWarps * copy_regs <= (softmax_warps + kLoadWarps) * start_regs, "a split that the launch holds");
   static constexpr int s_col = 0, o_col = 2 * rts * keys;   // TMEM columns: S(rt, b) at (2 rt + b) keys, O(rt) at o_col + rt HD
   static constexpr int tmem = HD == 64 ? 256 : 512;
@@ -686,23 +686,19 @@ __global__ void __launch_bounds__(Tall<HD>::threads, Tall<HD>::ctas) kv16_tall_k
         row_of(p, it.first_token, kvh, it.row0 + min(row, it.rows - 1), &token, &head);
         uint8_t* const out = p.out + (int64_t)token * p.out_stride_token + (int64_t)head * p.out_stride_head;
         float* const lse = p.lse != nullptr ? p.lse + (int64_t)token * p.num_q_heads + head : nullptr;
-        auto write32 = [&](const float* o, int d0) {   // 32 columns of the row
+        auto write16 = [&](const float* o, int d0) {   // 16 columns of the row
+          uint32_t w[8];
+#pragma unroll
+          for (int n = 0; n < 8; ++n) w[n] = pack16<kHalf>(o[2 * n], o[2 * n + 1]);
+          uint8_t* const to = out + d0 * 2;
           if (p.out_wide) {
-#pragma unroll
-            for (int c = 0; c < 2; ++c)
-              asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(out + (d0 + c * 16) * 2),
-                           "r"(pack16<kHalf>(o[c * 16], o[c * 16 + 1])), "r"(pack16<kHalf>(o[c * 16 + 2], o[c * 16 + 3])),
-                           "r"(pack16<kHalf>(o[c * 16 + 4], o[c * 16 + 5])), "r"(pack16<kHalf>(o[c * 16 + 6], o[c * 16 + 7])),
-                           "r"(pack16<kHalf>(o[c * 16 + 8], o[c * 16 + 9])), "r"(pack16<kHalf>(o[c * 16 + 10], o[c * 16 + 11])),
-                           "r"(pack16<kHalf>(o[c * 16 + 12], o[c * 16 + 13])), "r"(pack16<kHalf>(o[c * 16 + 14], o[c * 16 + 15]))
-                           : "memory");
-            return;
+            asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(to), "r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3]), "r"(w[4]),
+                         "r"(w[5]), "r"(w[6]), "r"(w[7])
+                         : "memory");
+          } else {
+            *reinterpret_cast<uint4*>(to) = make_uint4(w[0], w[1], w[2], w[3]);
+            *reinterpret_cast<uint4*>(to + 16) = make_uint4(w[4], w[5], w[6], w[7]);
           }
-#pragma unroll
-          for (int c = 0; c < 4; ++c)
-            *reinterpret_cast<uint4*>(out + (d0 + c * 8) * 2) =
-                make_uint4(pack16<kHalf>(o[c * 8], o[c * 8 + 1]), pack16<kHalf>(o[c * 8 + 2], o[c * 8 + 3]),
-                           pack16<kHalf>(o[c * 8 + 4], o[c * 8 + 5]), pack16<kHalf>(o[c * 8 + 6], o[c * 8 + 7]));
         };
         if (!padding) {
           const float inv = l == 0.f ? 0.f : 1.f / l;
@@ -716,7 +712,10 @@ __global__ void __launch_bounds__(Tall<HD>::threads, Tall<HD>::ctas) kv16_tall_k
               float o[32];
 #pragma unroll
               for (int n = 0; n < 32; ++n) o[n] = __uint_as_float(r[n]) * inv;
-              if (live) write32(o, c * 32);
+              if (live) {
+                write16(o, c * 32);
+                write16(o + 16, c * 32 + 16);
+              }
             } else {
 #pragma unroll
               for (int n = 0; n < 32; ++n) slot[(c * 32 + n) * RP] = __uint_as_float(r[n]);
@@ -746,33 +745,44 @@ __global__ void __launch_bounds__(Tall<HD>::threads, Tall<HD>::ctas) kv16_tall_k
           if (arrival[rt] && !padding) {
             auto slot = [&](int c) { return tall_slot<HD>(p, c, c == c0) + row; };
             float top = -INFINITY, sum = 0.f;
+            // (the loads of two pieces are in flight together; one that there is not counts nothing)
 #pragma unroll 1
-            for (int c = c0; c <= c1; ++c) {
-              if (none(c)) continue;
-              const float* s = slot(c) + HD * RP;
-              const float r = __ldcg(s), l1 = __ldcg(s + RP), to = fmaxf(top, r), use = to == -INFINITY ? 0.f : to;
-              sum = fmaf(sum, ex2f(top - use), ex2f(r - use) * l1);
+            for (int c = c0; c <= c1; c += 2) {
+              const bool a = !none(c), b = c < c1 && !none(c + 1);
+              const float* s = slot(a ? c : c0) + HD * RP;
+              const float* t = slot(b ? c + 1 : c0) + HD * RP;
+              const float ra = a ? __ldcg(s) : -INFINITY, la = __ldcg(s + RP), rb = b ? __ldcg(t) : -INFINITY, lb = __ldcg(t + RP);
+              const float to = max3(top, ra, rb), use = to == -INFINITY ? 0.f : to;
+              sum = fmaf(sum, ex2f(top - use), a ? ex2f(ra - use) * la : 0.f);
+              sum += b ? ex2f(rb - use) * lb : 0.f;
               top = to;
             }
             const float use = top == -INFINITY ? 0.f : top, inv = sum == 0.f ? 0.f : 1.f / sum;
 #pragma unroll 1
-            for (int c = 0; c < HD / 32; ++c) {
-              float o[32];
+            for (int c = 0; c < HD / 16; ++c) {
+              float o[16];
 #pragma unroll
-              for (int n = 0; n < 32; ++n) o[n] = 0.f;
+              for (int n = 0; n < 16; ++n) o[n] = 0.f;
 #pragma unroll 1
-              for (int cta = c0; cta <= c1; ++cta) {
-                if (none(cta)) continue;
-                const float* s = slot(cta);
-                const float weight = __ldcg(s + HD * RP);
-                float v[32];
+              for (int cta = c0; cta <= c1; cta += 2) {
+                const bool a = !none(cta), b = cta < c1 && !none(cta + 1);
+                const float* s = slot(a ? cta : c0);
+                const float* t = slot(b ? cta + 1 : c0);
+                const float wa = __ldcg(s + HD * RP), wb = __ldcg(t + HD * RP);
+                float v[16], u[16];
 #pragma unroll
-                for (int n = 0; n < 32; ++n) v[n] = __ldcg(s + (c * 32 + n) * RP);
-                const float f = ex2f(weight - use) * inv;
+                for (int n = 0; n < 16; ++n) {
+                  v[n] = __ldcg(s + (c * 16 + n) * RP);
+                  u[n] = __ldcg(t + (c * 16 + n) * RP);
+                }
+                const float fa = a ? ex2f(wa - use) * inv : 0.f, fb = b ? ex2f(wb - use) * inv : 0.f;
 #pragma unroll
-                for (int n = 0; n < 32; ++n) o[n] = fmaf(f, v[n], o[n]);
+                for (int n = 0; n < 16; ++n) {
+                  if (a) o[n] = fmaf(fa, v[n], o[n]);
+                  if (b) o[n] = fmaf(fb, u[n], o[n]);
+                }
               }
-              if (live) write32(o, c * 32);
+              if (live) write16(o, c * 16);
             }
             if (live && lse != nullptr) *lse = sum == 0.f ? -INFINITY : (use + log2f(sum)) * kLn2;
           }

@@ -11,7 +11,7 @@ namespace pthb200 {
 namespace {
 
 constexpr int kWriteThreads = 256;
-constexpr int kWriteBatch = 4;
+constexpr int kWriteBatch = 2;
 
 struct WriteParams {
   const uint8_t* src[2];

@@ -17,7 +17,7 @@ namespace {
 
 constexpr int kTableThreads = 256;
 constexpr int kTableWarps = kTableThreads / 32;
-constexpr int kTokensPerCta = 1024;   // entries a CTA takes at a time
+constexpr int kMostCtas = 592;        // four per SM
 
 __device__ __forceinline__ int pages_of(int64_t tokens, int block_size) {
   if (tokens <= 0) return 0;
@@ -36,11 +36,12 @@ __device__ __forceinline__ int owner(const int32_t* first, int n, int i) {
 }
 
 __global__ void __launch_bounds__(kTableThreads) page_tables_kernel(const __grid_constant__ PthB200TablesArgs a) {
-  extern __shared__ int32_t sums[];  // start [num_reqs + 1], first [num_reqs + 1]
+  extern __shared__ int32_t sums[];  // start [num_reqs + 1], first [num_reqs + 1], context [num_reqs]
   __shared__ int32_t warp_q[kTableWarps], warp_n[kTableWarps];
   const int R = a.num_reqs, tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   int32_t* const start = sums;
   int32_t* const first = sums + R + 1;
+  int32_t* const context = first + R + 1;
   pdl_wait();
   const int per = (R + kTableThreads - 1) / kTableThreads, r0 = min(R, tid * per), r1 = min(R, r0 + per);
   int q_sum = 0, n_sum = 0;
@@ -48,6 +49,7 @@ __global__ void __launch_bounds__(kTableThreads) page_tables_kernel(const __grid
     const int c = max(0, __ldg(a.context_lens + r)), q = max(0, __ldg(a.query_lens + r));
     start[r] = q_sum;
     first[r] = n_sum;
+    context[r] = c;
     q_sum += q;
     n_sum += pages_of((int64_t)c + q, a.block_size) - pages_of(c, a.block_size);
   }
@@ -84,12 +86,12 @@ __global__ void __launch_bounds__(kTableThreads) page_tables_kernel(const __grid
   const int stride = gridDim.x * kTableThreads, at = blockIdx.x * kTableThreads + tid;
   for (int r = at; r <= R; r += stride) {
     a.query_start_loc[r] = start[r];
-    if (r < R) a.seq_lens[r] = max(0, __ldg(a.context_lens + r)) + max(0, __ldg(a.query_lens + r));
+    if (r < R) a.seq_lens[r] = context[r] + (start[r + 1] - start[r]);
   }
   if (at == 0) *a.pages_taken = pages;
   for (int i = at; i < pages; i += stride) {
     const int r = owner(first, R, i);
-    const int64_t col = (int64_t)pages_of(max(0, __ldg(a.context_lens + r)), a.block_size) + (i - first[r]);
+    const int64_t col = (int64_t)pages_of(context[r], a.block_size) + (i - first[r]);
     if (col < a.num_pages) a.block_table[(int64_t)r * a.block_table_row_stride + col] = i < a.num_free ? __ldg(a.free_blocks + i) : -1;
   }
   for (int t = at; t < a.num_tokens; t += stride) {
@@ -97,7 +99,7 @@ __global__ void __launch_bounds__(kTableThreads) page_tables_kernel(const __grid
     int pos = 0;
     if (t < total) {
       const int r = owner(start, R, t);
-      const int c = max(0, __ldg(a.context_lens + r));
+      const int c = context[r];
       pos = c + (t - start[r]);
       const int col = (int)((uint32_t)pos / (uint32_t)a.block_size), old = pages_of(c, a.block_size);
       if (col < a.num_pages) {
@@ -119,18 +121,19 @@ __global__ void __launch_bounds__(kTableThreads) page_tables_kernel(const __grid
 }  // namespace
 
 cudaError_t launch_page_tables(const PthB200TablesArgs& a, cudaStream_t stream) {
-  const int smem = 2 * (a.num_reqs + 1) * 4;  // 131 KB at the most requests
+  const int smem = (3 * a.num_reqs + 2) * 4;  // 197 KB at the most requests
   static bool configured[64] = {};
   int dev = 0;
   cudaError_t err = cudaGetDevice(&dev);
   if (err != cudaSuccess) return err;
   if (dev < 0 || dev >= 64 || !configured[dev]) {
-    err = cudaFuncSetAttribute(page_tables_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 2 * 16385 * 4);
+    err = cudaFuncSetAttribute(page_tables_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (3 * 16384 + 2) * 4);
     if (err != cudaSuccess) return err;
     if (dev >= 0 && dev < 64) configured[dev] = true;
   }
-  const int ctas = (a.num_tokens + kTokensPerCta - 1) / kTokensPerCta;
-  return pdl_launch(page_tables_kernel, dim3((unsigned)(ctas < 1 ? 1 : ctas > 592 ? 592 : ctas)), dim3(kTableThreads), smem, stream, a);
+  // a thread per token as far as the SMs hold them at once: what a token waits for are two loads, one after the other
+  const int ctas = (a.num_tokens + kTableThreads - 1) / kTableThreads;
+  return pdl_launch(page_tables_kernel, dim3((unsigned)(ctas < 1 ? 1 : ctas > kMostCtas ? kMostCtas : ctas)), dim3(kTableThreads), smem, stream, a);
 }
 
 }  // namespace pthb200

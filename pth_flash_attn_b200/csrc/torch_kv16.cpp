@@ -55,8 +55,8 @@ struct Check {
                     t.stride(t.dim() - 1));
   }
   void device(const Tensor& t, const Tensor& as, const char* name, const char* of) const {
-    STD_TORCH_CHECK(t.is_cuda() == as.is_cuda() && t.get_device_index() == as.get_device_index(), op, name,
-                    " must be on the same device as ", of);
+    // (a CPU tensor's index is -1)
+    STD_TORCH_CHECK(t.get_device_index() == as.get_device_index(), op, name, " must be on the same device as ", of);
   }
   void vector(const Tensor& t, ScalarType type, const char* name) const {
     rank(t, 1, name);
