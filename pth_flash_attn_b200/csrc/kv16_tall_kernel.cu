@@ -507,25 +507,45 @@ __global__ void __launch_bounds__(Tall<HD>::threads, Tall<HD>::ctas) kv16_tall_k
     const uint64_t k_desc = swizzled_desc(tc::smem_u32(smem), 16, 1024);
     const uint64_t v_desc = swizzled_desc(tc::smem_u32(smem), kTile * 128, 1024);
     const uint32_t o_tmem = tmem_base + G::o_col + rt * HD, s_tmem = tmem_base + G::s_col + 2 * rt * G::keys;
-    uint32_t unit = 0;                       // of the piece's next tile, in the order of all units of the CTA
-    uint32_t s_qk = 0, s_pv = 0, pieces = 0; // steps so far, pieces with live rows
-    auto arrived = [&](uint32_t u) -> uint32_t {
-      const uint32_t s = u % G::units;
-      ok &= kv16_wait(&full[s], (u / G::units) & 1, abort_flag);
-      return s;
-    };
-    // step `sub` of the KV tile whose units begin at u; frees them where it is the tile's last
-    auto qk = [&](uint32_t u, int sub, bool tile_ends, bool first, bool last) {
-      const uint32_t b = s_qk & 1, use = s_qk >> 1;
-      if (first) ok &= kv16_wait(&bars[B::q_full + rt], (pieces - 1) & 1, abort_flag);
-      if (use > 0) ok &= kv16_wait(&bars[B::pv_done + 2 * rt + b], (use - 1) & 1, abort_flag);   // (P of that use has been read)
+    // (this warp's own instructions bound the kernel before its MMAs do: it keeps ring slots and phases instead of dividing,
+    // and asks and fences only where there is something to wait for)
+    uint32_t k_slot[G::parts], k_phase[G::parts], v_slot[G::parts], v_phase[G::parts];   // of the next tile's units
+#pragma unroll
+    for (int part = 0; part < G::parts; ++part) {
+      k_slot[part] = part;
+      v_slot[part] = G::parts + part;
+      k_phase[part] = v_phase[part] = 0;
+    }
+    static_assert(2 * G::parts <= G::units, "a tile's units lap the ring at most once");
+    auto next_tile = [&](uint32_t (&slot)[G::parts], uint32_t (&phase)[G::parts]) {
 #pragma unroll
       for (int part = 0; part < G::parts; ++part) {
-        const uint32_t s = arrived(u + part);
-        tc::fence_async_smem();   // (copies wrote through the generic proxy)
-        if (elect_one()) {
-          tc::fence_after_sync();
-          const uint32_t klo = (uint32_t)k_desc + s * (G::unit >> 4) + sub * ((G::keys * 128) >> 4), qlo = (uint32_t)q_desc + part * ((2 * kTile * 128) >> 4);
+        slot[part] += 2 * G::parts;
+        if (slot[part] >= G::units) {
+          slot[part] -= G::units;
+          phase[part] ^= 1;
+        }
+      }
+    };
+    auto landed = [&](const uint32_t (&slot)[G::parts], const uint32_t (&phase)[G::parts], bool copied) {
+#pragma unroll
+      for (int part = 0; part < G::parts; ++part) ok &= kv16_wait(&full[slot[part]], phase[part], abort_flag);
+      if (copied) tc::fence_async_smem();   // (16-byte copies wrote through the generic proxy)
+    };
+    uint32_t s_qk = 0, s_pv = 0, pieces = 0; // steps so far, pieces with live rows
+    auto qk = [&](int sub, bool copied, bool tile_ends, bool first, bool last) {
+      const uint32_t b = s_qk & 1;
+      if (first) {
+        ok &= kv16_wait(&bars[B::q_full + rt], (pieces - 1) & 1, abort_flag);
+        tc::fence_async_smem();
+      }
+      if (sub == 0) landed(k_slot, k_phase, copied);
+      if (s_qk > 1) ok &= kv16_wait(&bars[B::pv_done + 2 * rt + b], ((s_qk >> 1) - 1) & 1, abort_flag);   // (P of the step before last has been read)
+      if (elect_one()) {
+        tc::fence_after_sync();
+#pragma unroll
+        for (int part = 0; part < G::parts; ++part) {
+          const uint32_t klo = (uint32_t)k_desc + k_slot[part] * (G::unit >> 4) + sub * ((G::keys * 128) >> 4), qlo = (uint32_t)q_desc + part * ((2 * kTile * 128) >> 4);
 #pragma unroll
           for (int kk = 0; kk < G::dims / 16; ++kk) {
             constexpr uint32_t slab = (kTile * 128) >> 4;
@@ -533,60 +553,71 @@ __global__ void __launch_bounds__(Tall<HD>::threads, Tall<HD>::ctas) kv16_tall_k
             if (part == 0 && kk == 0) mma_ss_words<false>(s_tmem + b * G::keys, qlo + at, (uint32_t)(q_desc >> 32), klo + at, (uint32_t)(k_desc >> 32), qk_desc);
             else mma_ss_words<true>(s_tmem + b * G::keys, qlo + at, (uint32_t)(q_desc >> 32), klo + at, (uint32_t)(k_desc >> 32), qk_desc);
           }
-          if (tile_ends) tc::mma_commit(&empty[s]);
-          if (part == G::parts - 1) {
-            tc::mma_commit(&bars[B::s_ready + 2 * rt + b]);
-            if (last) tc::mma_commit(&bars[B::q_empty + rt]);
-          }
+          if (tile_ends) tc::mma_commit(&empty[k_slot[part]]);
         }
-        __syncwarp();
+        tc::mma_commit(&bars[B::s_ready + 2 * rt + b]);
+        if (last) tc::mma_commit(&bars[B::q_empty + rt]);
       }
+      __syncwarp();
+      if (tile_ends) next_tile(k_slot, k_phase);
       ++s_qk;
     };
-    auto pv = [&](uint32_t u, int sub, bool tile_ends, bool first) {
-      const uint32_t b = s_pv & 1, use = s_pv >> 1;
-#pragma unroll
-      for (int part = 0; part < G::parts; ++part) arrived(u + part);
-      tc::fence_async_smem();
+    auto pv = [&](int sub, bool copied, bool tile_ends, bool first) {
+      const uint32_t b = s_pv & 1;
+      if (sub == 0) landed(v_slot, v_phase, copied);
 #pragma unroll
       for (int half = 0; half < G::halves; ++half) {
-        ok &= kv16_wait(&bars[B::p_ready + 2 * (2 * rt + b) + half], use & 1, abort_flag);
+        ok &= kv16_wait(&bars[B::p_ready + 2 * (2 * rt + b) + half], (s_pv >> 1) & 1, abort_flag);
         if (elect_one()) {
           tc::fence_after_sync();
 #pragma unroll
           for (int part = 0; part < G::parts; ++part) {
-            const uint32_t s = (u + part) % G::units;
-            const uint32_t vlo = (uint32_t)v_desc + s * (G::unit >> 4) + (sub * G::keys + half * 64) * (128 >> 4);
+            const uint32_t vlo = (uint32_t)v_desc + v_slot[part] * (G::unit >> 4) + (sub * G::keys + half * 64) * (128 >> 4);
 #pragma unroll
             for (int kk = 0; kk < 4; ++kk)
               mma_ts_words(o_tmem + part * 128, s_tmem + b * G::keys + half * 32 + kk * 8, vlo + kk * (2048 >> 4), (uint32_t)(v_desc >> 32), pv_desc,
                            !first || half > 0 || kk > 0);
-            if (tile_ends && half == G::halves - 1) tc::mma_commit(&empty[s]);
+            if (tile_ends && half == G::halves - 1) tc::mma_commit(&empty[v_slot[part]]);
           }
           tc::mma_commit(&bars[(half == G::halves - 1 ? B::pv_done : B::pv_half) + 2 * rt + b]);
         }
         __syncwarp();
       }
+      if (tile_ends) next_tile(v_slot, v_phase);
       ++s_pv;
     };
     Piece it;
     while (queue.get(&it, abort_flag)) {
       if (it.rows <= rt * 128) {   // no rows: free the units as if they had been read
-        for (int u = 0; u < 2 * G::parts * it.tiles; ++u) {
-          const uint32_t s = arrived(unit + u);
-          if (elect_one()) mbar_arrive(&empty[s]);
+#pragma unroll 1
+        for (int i = 0; i < it.tiles; ++i) {
+          landed(k_slot, k_phase, false);
+          landed(v_slot, v_phase, false);
+          if (elect_one()) {
+#pragma unroll
+            for (int part = 0; part < G::parts; ++part) {
+              mbar_arrive(&empty[k_slot[part]]);
+              mbar_arrive(&empty[v_slot[part]]);
+            }
+          }
           __syncwarp();
+          next_tile(k_slot, k_phase);
+          next_tile(v_slot, v_phase);
         }
-      } else {
-        ++pieces;
-        const int n = piece_steps<G::keys>(it);
-        // QK of a step ahead of PV of the one before: the softmax finds the next S when it is done with one
-        for (int j = 0; j <= n; ++j) {
-          if (j < n) qk(unit + j / G::steps * 2 * G::parts, j % G::steps, j % G::steps == G::steps - 1 || j == n - 1, j == 0, j == n - 1);
-          if (j > 0) pv(unit + (j - 1) / G::steps * 2 * G::parts + G::parts, (j - 1) % G::steps, (j - 1) % G::steps == G::steps - 1 || j == n, j == 1);
-        }
+        continue;
       }
-      unit += 2 * G::parts * it.tiles;
+      ++pieces;
+      const int n = piece_steps<G::keys>(it);
+      auto tile_copied = [&](int j) {   // (as the copying warps decide it)
+        const int key0 = it.key0 + j / G::steps * kTile;
+        return p.box_slots == 0 || key0 < it.lo || key0 + kTile > it.hi;
+      };
+      // QK of a step ahead of PV of the one before: the softmax finds the next S when it is done with one
+#pragma unroll 1
+      for (int j = 0; j <= n; ++j) {
+        if (j < n) qk(j % G::steps, tile_copied(j), j % G::steps == G::steps - 1 || j == n - 1, j == 0, j == n - 1);
+        if (j > 0) pv((j - 1) % G::steps, tile_copied(j - 1), (j - 1) % G::steps == G::steps - 1 || j == n, j == 1);
+      }
     }
   } else {
     // =========================== softmax =========================================
