@@ -356,11 +356,13 @@ int32_t pthb200_kv16_write(const PthB200Kv16WriteArgs* args, void* stream);
  *                        the states of its encoder (window must be 0).  max_query_len bounds them: tokens
  *                        of a request past it are not computed.
  * A request without keys gets out = 0 and a log-sum-exp of -inf.  lse (optional) is the natural
- * logarithm, dense [num_tokens, num_q_heads].  Block ids of visible keys must lie in
- * [0, num_blocks); memory of slots that no request sees is not read.
+ * logarithm, dense [num_tokens, num_q_heads].  Keys past the row of the block table do not exist, and a
+ * block id outside [0, num_blocks) stands for keys and values of zero; what lies in slots that no request
+ * sees has no influence.
  *
  * workspace: pthb200_kv16_workspace_bytes of it, 256-byte aligned, zeroed ONCE before its first use; a
- * call leaves it ready for the next one.  Calls that may overlap need workspaces of their own. */
+ * call leaves it ready for the next one.  Calls that may overlap need workspaces of their own.  (Zero it again
+ * after pthb200_device_status has reported a wait that gave up.) */
 typedef struct PthB200Kv16Args {
   int32_t abi_version;  /* PTH_ATTN_ABI_VERSION */
   int32_t struct_bytes; /* sizeof(PthB200Kv16Args) of the caller */
@@ -387,6 +389,7 @@ typedef struct PthB200Kv16Args {
   int32_t head_size; /* 64, 128 or 256 */
   int32_t num_reqs;
   int32_t num_tokens;
+  int32_t num_pages; /* columns of block_table */
   int32_t max_query_len;
   int32_t window;
   float softmax_scale;

@@ -198,6 +198,7 @@ class PthB200Kv16Args(ctypes.Structure):
         ("head_size", ctypes.c_int32),
         ("num_reqs", ctypes.c_int32),
         ("num_tokens", ctypes.c_int32),
+        ("num_pages", ctypes.c_int32),
         ("max_query_len", ctypes.c_int32),
         ("window", ctypes.c_int32),
         ("softmax_scale", ctypes.c_float),

@@ -28,6 +28,7 @@ struct Kv16Params {
   int32_t num_kv_heads, num_q_heads, group, head_size;
   int32_t num_reqs, num_tokens, max_query_len, window;
   int32_t num_blocks;
+  int32_t most_keys;  // that a row of the block table has room for
   int32_t box_slots;  // slots of a TMA box (tall kernel; 0: none)
   int32_t out_wide;   // rows of out lie on 32-byte boundaries (tall kernel)
   float scale_log2;  // softmax_scale * log2(e)
@@ -39,12 +40,12 @@ __device__ __forceinline__ int kv16_tokens(const Kv16Params& p, int r, int* firs
     *first = r;
     return 1;
   }
-  *first = __ldg(p.query_start_loc + r);
+  *first = max(0, __ldg(p.query_start_loc + r));
   const int end = min(__ldg(p.query_start_loc + r + 1), p.num_tokens);
   return max(0, min(end - *first, p.max_query_len));
 }
 __device__ __forceinline__ void kv16_visible(const Kv16Params& p, int r, int* lo, int* hi) {
-  *hi = max(0, __ldg(p.seq_lens + r));
+  *hi = max(0, min(__ldg(p.seq_lens + r), p.most_keys));
   *lo = p.window > 0 ? max(0, *hi - p.window) : 0;
 }
 

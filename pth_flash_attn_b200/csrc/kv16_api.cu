@@ -1,6 +1,7 @@
 // C entries of the 16-bit paged cache (include/pthb200_attn.h): argument checks, each naming its field, and the
 // launches.  Nothing here allocates, reads device memory or synchronises.
 #include <algorithm>
+#include <climits>
 #include <cmath>
 
 #include "kv16.cuh"
@@ -74,8 +75,9 @@ int32_t build(const PthB200Kv16Args* a, bool cross, Kv16Params* p) {
   KV16_REQUIRE(a->k_cache.stride_block == a->v_cache.stride_block && a->k_cache.stride_slot == a->v_cache.stride_slot &&
                    a->k_cache.stride_head == a->v_cache.stride_head,
                "k_cache and v_cache must have the same strides");
-  KV16_REQUIRE(a->block_table != nullptr && a->seq_lens != nullptr, "block_table and seq_lens must not be NULL");
-  KV16_REQUIRE(a->block_table_row_stride >= 0, "block_table_row_stride must be >= 0");
+  KV16_REQUIRE(a->num_pages == 0 || a->block_table != nullptr, "block_table is NULL");
+  KV16_REQUIRE(a->seq_lens != nullptr, "seq_lens is NULL");
+  KV16_REQUIRE(a->block_table_row_stride >= 0 && a->num_pages >= 0, "block_table_row_stride and num_pages must be >= 0");
   KV16_REQUIRE(a->workspace != nullptr && aligned(a->workspace, 256), "workspace must not be NULL and 256-byte aligned");
 
   *p = Kv16Params{};
@@ -106,6 +108,7 @@ int32_t build(const PthB200Kv16Args* a, bool cross, Kv16Params* p) {
   p->group = a->num_q_heads / a->num_kv_heads;
   p->head_size = a->head_size;
   p->num_blocks = a->num_blocks;
+  p->most_keys = (int32_t)std::min<int64_t>((int64_t)a->num_pages * a->block_size, INT32_MAX);
   p->num_reqs = a->num_reqs;
   p->num_tokens = a->num_tokens;
   p->max_query_len = cross ? a->max_query_len : 1;

@@ -179,10 +179,11 @@ struct KeyLookup {
         slot = pos - page * p.block_size;
       }
       blk = __ldg(p.block_table + (int64_t)it.r * p.block_table_row_stride + page);
+      if ((uint32_t)blk >= (uint32_t)p.num_blocks) blk = -1;
     }
     return true;
   }
-  // Byte offset of the key's row inside a KV head's stream; -1: the request does not see the key.
+  // Byte offset of the key's row inside a KV head's stream; -1: there is none to read.
   __device__ __forceinline__ long long offset() const { return blk >= 0 ? (long long)blk * p.stride_block + (long long)slot * p.stride_slot : -1ll; }
 };
 

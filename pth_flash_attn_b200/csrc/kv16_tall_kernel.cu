@@ -32,8 +32,6 @@
 // Otherwise all but the last one or two items per CTA go out in waves, CTA c taking items c, c + CTAs, ...: the CTAs then work
 // on the same few heads of one request at a time.  (Equal runs had them all over 268 MB of keys: 4 x 2,048 tokens over
 // 8,192 states drew 5.5 TB/s from memory and took 1,552 us.)  The tiles of the rest make up for unequal waves.
-#include <mutex>
-
 #include "kv16_sched.cuh"
 #include "page_copy.cuh"
 #include "pdl.cuh"
@@ -830,41 +828,15 @@ __global__ void __launch_bounds__(Tall<HD>::threads, Tall<HD>::ctas) kv16_tall_k
 }
 
 // Tensor map over one of the caches, [dims][heads][slots][blocks], a box being 64 dims of box_slots slots of one head, in the
-// 128-byte swizzle.  Encoding one is a driver call of microseconds and depends on the view alone, of which an engine has a
-// few for its whole life: they are kept (once the table is full, further ones are encoded by every call).  False: the driver
-// refuses the view.
+// 128-byte swizzle.  False: the driver refuses the view.  (Encoded for every call: a microsecond of the host.)
 bool page_box_map(const Kv16Params& p, const uint8_t* base, CUtensorMap* map) {
-  struct Entry {
-    const uint8_t* base;
-    int64_t stride_block, stride_slot, stride_head;
-    int32_t num_blocks, block_size, num_kv_heads, head_size, dtype, box_slots;
-    bool fine;
-    CUtensorMap map;
-  };
-  constexpr int kEntries = 128;
-  static Entry entries[kEntries];
-  static int used = 0;
-  static std::mutex mu;
-  std::lock_guard<std::mutex> lock(mu);
-  for (int i = 0; i < used; ++i) {
-    const Entry& e = entries[i];
-    if (e.base == base && e.stride_block == p.stride_block && e.stride_slot == p.stride_slot && e.stride_head == p.stride_head &&
-        e.num_blocks == p.num_blocks && e.block_size == p.block_size && e.num_kv_heads == p.num_kv_heads && e.head_size == p.head_size &&
-        e.dtype == p.dtype && e.box_slots == p.box_slots) {
-      *map = e.map;
-      return e.fine;
-    }
-  }
   const EncodeTiledFn fn = encode_tiled_fn();
   const cuuint64_t dims[4] = {(cuuint64_t)p.head_size, (cuuint64_t)p.num_kv_heads, (cuuint64_t)p.block_size, (cuuint64_t)p.num_blocks};
   const cuuint64_t strides[3] = {(cuuint64_t)p.stride_head, (cuuint64_t)p.stride_slot, (cuuint64_t)p.stride_block};
   const cuuint32_t box[4] = {64, 1, (cuuint32_t)p.box_slots, 1}, elem[4] = {1, 1, 1, 1};
-  const bool fine = fn != nullptr && fn(map, p.dtype == PTH_ATTN_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4,
-                                        const_cast<uint8_t*>(base), dims, strides, box, elem, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
-                                        CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
-  if (used < kEntries)
-    entries[used++] = Entry{base, p.stride_block, p.stride_slot, p.stride_head, p.num_blocks, p.block_size, p.num_kv_heads, p.head_size, p.dtype, p.box_slots, fine, *map};
-  return fine;
+  return fn != nullptr && fn(map, p.dtype == PTH_ATTN_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4,
+                             const_cast<uint8_t*>(base), dims, strides, box, elem, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                             CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
 template <int HD, bool kHalf>

@@ -92,7 +92,7 @@ __global__ void __launch_bounds__(kTableThreads) page_tables_kernel(const __grid
   for (int i = at; i < pages; i += stride) {
     const int r = owner(first, R, i);
     const int64_t col = (int64_t)pages_of(context[r], a.block_size) + (i - first[r]);
-    if (col < a.num_pages) a.block_table[(int64_t)r * a.block_table_row_stride + col] = i < a.num_free ? __ldg(a.free_blocks + i) : -1;
+    if (col >= 0 && col < a.num_pages) a.block_table[(int64_t)r * a.block_table_row_stride + col] = i < a.num_free ? __ldg(a.free_blocks + i) : -1;
   }
   for (int t = at; t < a.num_tokens; t += stride) {
     int64_t slot = -1;
@@ -102,13 +102,13 @@ __global__ void __launch_bounds__(kTableThreads) page_tables_kernel(const __grid
       const int c = context[r];
       pos = c + (t - start[r]);
       const int col = (int)((uint32_t)pos / (uint32_t)a.block_size), old = pages_of(c, a.block_size);
-      if (col < a.num_pages) {
+      if ((uint32_t)col < (uint32_t)a.num_pages) {
         int block;
         if (col < old) {
           block = __ldg(a.block_table + (int64_t)r * a.block_table_row_stride + col);
         } else {
           const int i = first[r] + (col - old);
-          block = i < a.num_free ? __ldg(a.free_blocks + i) : -1;
+          block = (uint32_t)i < (uint32_t)a.num_free ? __ldg(a.free_blocks + i) : -1;
         }
         if (block >= 0) slot = (int64_t)block * a.block_size + (pos - col * a.block_size);
       }

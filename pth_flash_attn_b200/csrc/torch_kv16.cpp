@@ -248,6 +248,7 @@ PthB200Kv16Args attention_args(const Check& c, Tensor& out, Tensor& lse, const T
   c.count(T, "T");
   c.count(Hq, "Hq");
   c.count(R, "num_reqs");
+  c.count(block_table.size(1), "block_table.size(1)");
   c.device(out, q, "out", "q");
   c.device(lse, q, "lse", "q");
   c.device(k_cache, q, "k_cache", "q");
@@ -278,6 +279,7 @@ PthB200Kv16Args attention_args(const Check& c, Tensor& out, Tensor& lse, const T
   a.head_size = static_cast<int32_t>(D);
   a.num_reqs = static_cast<int32_t>(R);
   a.num_tokens = static_cast<int32_t>(T);
+  a.num_pages = static_cast<int32_t>(block_table.size(1));
   a.softmax_scale = static_cast<float>(softmax_scale);
   return a;
 }

@@ -355,3 +355,46 @@ def test_refusals_on_the_device():
     v = torch.zeros((*b.k.shape[:3], 136), dtype=BF16, device="cuda")[..., :128]
     with pytest.raises(RuntimeError, match="must have the same strides"):
         ops.kv16_cross_attention(b.out, b.lse, b.q, b.k, v, b.bt, b.lens, b.qsl, 1, 1.0, b.ws)
+
+
+OUTSIDE = [-1, -(1 << 31), 1 << 30, "one past the last"]
+
+
+@pytest.mark.parametrize("page", [5, 16, 64])
+@pytest.mark.parametrize("D", [64, 128, 256])
+@pytest.mark.parametrize("q_lens", [[1, 1, 1, 1], [1, 9, 2, 0], [300, 70, 129, 5]])
+def test_block_ids_outside_the_cache_are_keys_of_zeros(q_lens, D, page):
+    """Pages that a table does not hold (a free list that ran dry enters -1): no memory behind the cache is read."""
+    b = Batch([1000, 300, 129, 40], q_lens, 8, 2, D, BF16, page=page, seed=19)
+    zeros = next(i for i in range(b.k.shape[0]) if not bool((b.table == i).any()))
+    b.k[zeros], b.v[zeros] = 0, 0
+    bad = b.table.clone()
+    for r, n in enumerate(b.kv_lens):
+        last = -(-n // page) - 1
+        for at, block in ((0, OUTSIDE[r % 4]), (last // 2, OUTSIDE[(r + 1) % 4]), (last, OUTSIDE[(r + 2) % 4])):
+            bad[r, at] = b.k.shape[0] if isinstance(block, str) else block
+            b.table[r, at] = zeros
+    b.bt = bad.cuda()
+    if max(q_lens) == 1:
+        b.decode().check()
+    b.cross().check()
+
+
+@pytest.mark.parametrize("D", [64, 128, 256])
+@pytest.mark.parametrize("q_lens", [[1, 1, 1, 1], [300, 70, 129, 5]])
+def test_keys_past_the_row_of_the_table_do_not_exist(q_lens, D):
+    """A length that the block table has no room for ends where the table does."""
+    b = Batch([1000, 300, 960, 40], q_lens, 8, 2, D, BF16, seed=20)
+    b.bt = b.bt[:, :60]
+    b.kv_lens[0] = 960
+    b.lens[2] = (1 << 31) - 1
+    if max(q_lens) == 1:
+        b.decode().check()
+    b.cross().check()
+
+
+def test_tables_without_columns():
+    b = Batch([40, 300], [1, 1], 8, 2, 128, BF16, seed=21)
+    b.bt, b.kv_lens = b.bt[:, :0], [0, 0]
+    b.decode().check()
+    b.cross().check()

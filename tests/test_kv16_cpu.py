@@ -137,6 +137,7 @@ def _kv16_args(cross):
     a.workspace, a.workspace_bytes = _BASE, 1 << 10
     a.dtype, a.num_blocks, a.block_size, a.num_kv_heads, a.num_q_heads, a.head_size = capi.BF16, 4, 16, 2, 8, 64
     a.num_reqs = a.num_tokens = 3
+    a.num_pages = 2
     a.max_query_len, a.softmax_scale = 1, 0.5
     if cross:
         a.query_start_loc = _BASE + 768
@@ -149,7 +150,8 @@ def _kv16_args(cross):
     ("head_size", 96, "head_size must be"), ("num_q_heads", 7, "num_q_heads must be a positive multiple"), ("num_q_heads", 130, "must be <= 64"),
     ("block_size", 0, "block_size"), ("num_blocks", 0, "num_blocks"), ("softmax_scale", float("inf"), "softmax_scale"), ("window", -1, "window"),
     ("q", None, "q is NULL"), ("q", _BASE + 8, "q must be 16-byte aligned"), ("out_stride_head", 8, "out byte strides"), ("lse", _BASE + 2, "lse must be"),
-    ("block_table", None, "block_table"), ("workspace", _BASE + 16, "workspace"), ("num_tokens", -1, "num_tokens")])
+    ("block_table", None, "block_table"), ("workspace", _BASE + 16, "workspace"), ("num_tokens", -1, "num_tokens"),
+    ("num_pages", -1, "num_pages must be >= 0")])
 def test_c_abi_refusals(field, value, message, cross):
     lib = capi.load_library()
     a = _kv16_args(cross)
