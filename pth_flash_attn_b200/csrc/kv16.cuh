@@ -58,8 +58,10 @@ __device__ __forceinline__ uint64_t swizzled_desc(uint32_t saddr, uint32_t lbo_b
   return tc::smem_desc(saddr, lbo_bytes, sbo_bytes) | (uint64_t)2 << 61;
 }
 // Bounded wait for a phase of an mbarrier; once any wait of the CTA has given up, all do.  A try sleeps for a microsecond at
-// most, so the bound is between some 50 ms and 4 s.
+// most, so the bound is between some 50 ms and 4 s.  (A test goes first: a try that may sleep takes 200 cycles where the phase is
+// complete already, a test 100, and a softmax step has little else to wait for.)
 __device__ __forceinline__ bool kv16_wait(uint64_t* bar, uint32_t parity, volatile int* abort_flag) {
+  if (tc::mbar_test_wait(bar, parity)) return true;
 #pragma unroll 1
   for (uint32_t i = 0; i < (1u << 22); ++i) {
     if (tc::mbar_try_wait_hint(bar, parity, 1000u)) return true;

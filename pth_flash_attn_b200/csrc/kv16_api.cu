@@ -108,7 +108,7 @@ int32_t build(const PthB200Kv16Args* a, bool cross, Kv16Params* p) {
   p->group = a->num_q_heads / a->num_kv_heads;
   p->head_size = a->head_size;
   p->num_blocks = a->num_blocks;
-  p->most_keys = (int32_t)std::min<int64_t>((int64_t)a->num_pages * a->block_size, INT32_MAX);
+  p->most_keys = (int32_t)std::min<int64_t>((int64_t)a->num_pages * a->block_size, INT32_MAX - 1024);
   p->num_reqs = a->num_reqs;
   p->num_tokens = a->num_tokens;
   p->max_query_len = cross ? a->max_query_len : 1;
@@ -117,8 +117,15 @@ int32_t build(const PthB200Kv16Args* a, bool cross, Kv16Params* p) {
   return PTH_ATTN_OK;
 }
 
-// Query rows per KV head from which a launch goes to the kernel with the rows on the MMA's M dimension.
-constexpr int64_t kTallRows = 33;
+// Rows (query tokens x G) from which a launch of more than one token goes to the kernel with the rows on the MMA's M
+// dimension.  Keys on M against rows on M, us:
+//   rows  D 128, G 4: 8 x 500  8 x 4,000  64 x 500  64 x 4,000 keys   D 64, G 1: 64 x 500  64 x 4,000   D 256, G 4: 64 x 4,000
+//     16         27 / 33      48 / 57      67 / 58     203 / 244             69 / 58     209 / 245             352 / 491
+//     32         37 / 33      57 / 56     131 / 59     317 / 244            198 / 59     408 / 246             545 / 493
+//     64         56 / 33      89 / 58     219 / 59     588 / 244            346 / 64     800 / 253           1,111 / 494
+// Single tokens of wide groups stay with the keys on M, which divides few requests better: 8 x 4,000 keys, 32 heads of 1 KV head
+// 55 / 68, 1 x 131,072, 64 of 2 183 / 243; 64 x 4,000, 64 of 2 88 / 83, and 64 x 8,000, 48 of 2 131 / 127.
+constexpr int64_t kTallRows = 17;
 
 int64_t workspace_bytes(int head_size, int num_sms) {
   return std::max(kv16_short_workspace_bytes(head_size, num_sms), kv16_tall_workspace_bytes(head_size, num_sms));

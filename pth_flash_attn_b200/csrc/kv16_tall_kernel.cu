@@ -539,7 +539,7 @@ __global__ void __launch_bounds__(Tall<HD>::threads, Tall<HD>::ctas) kv16_tall_k
       }
       if (sub == 0) landed(k_slot, k_phase, copied);
       if (s_qk > 1) ok &= kv16_wait(&bars[B::pv_done + 2 * rt + b], ((s_qk >> 1) - 1) & 1, abort_flag);   // (P of the step before last has been read)
-      if (elect_one()) {
+      {
         tc::fence_after_sync();
 #pragma unroll
         for (int part = 0; part < G::parts; ++part) {
@@ -556,7 +556,6 @@ __global__ void __launch_bounds__(Tall<HD>::threads, Tall<HD>::ctas) kv16_tall_k
         tc::mma_commit(&bars[B::s_ready + 2 * rt + b]);
         if (last) tc::mma_commit(&bars[B::q_empty + rt]);
       }
-      __syncwarp();
       if (tile_ends) next_tile(k_slot, k_phase);
       ++s_qk;
     };
@@ -566,7 +565,7 @@ __global__ void __launch_bounds__(Tall<HD>::threads, Tall<HD>::ctas) kv16_tall_k
 #pragma unroll
       for (int half = 0; half < G::halves; ++half) {
         ok &= kv16_wait(&bars[B::p_ready + 2 * (2 * rt + b) + half], (s_pv >> 1) & 1, abort_flag);
-        if (elect_one()) {
+        {
           tc::fence_after_sync();
 #pragma unroll
           for (int part = 0; part < G::parts; ++part) {
@@ -579,26 +578,24 @@ __global__ void __launch_bounds__(Tall<HD>::threads, Tall<HD>::ctas) kv16_tall_k
           }
           tc::mma_commit(&bars[(half == G::halves - 1 ? B::pv_done : B::pv_half) + 2 * rt + b]);
         }
-        __syncwarp();
       }
       if (tile_ends) next_tile(v_slot, v_phase);
       ++s_pv;
     };
     Piece it;
+    const bool leader = elect_one();   // (one lane takes all steps of a piece: the others would only have to be waited for)
     while (queue.get(&it, abort_flag)) {
+      if (!leader) continue;
       if (it.rows <= rt * 128) {   // no rows: free the units as if they had been read
 #pragma unroll 1
         for (int i = 0; i < it.tiles; ++i) {
           landed(k_slot, k_phase, false);
           landed(v_slot, v_phase, false);
-          if (elect_one()) {
 #pragma unroll
-            for (int part = 0; part < G::parts; ++part) {
-              mbar_arrive(&empty[k_slot[part]]);
-              mbar_arrive(&empty[v_slot[part]]);
-            }
+          for (int part = 0; part < G::parts; ++part) {
+            mbar_arrive(&empty[k_slot[part]]);
+            mbar_arrive(&empty[v_slot[part]]);
           }
-          __syncwarp();
           next_tile(k_slot, k_phase);
           next_tile(v_slot, v_phase);
         }
