@@ -28,7 +28,8 @@
 // unit of 32 KB, more than the MMAs take.)
 //
 // Schedule: items (row tile, KV head, request), in the order request, head, row tile, so that neighbouring items read the same keys.
-// While the keys of a launch fit in the L2 cache, the sequence of all their KV tiles is cut into equal runs, one per CTA.
+// While the keys of a launch fit in the L2 cache, the sequence of all their KV tiles is cut into equal runs, one per CTA (an item
+// counts kItemTiles more, which stand in front of its tiles).
 // Otherwise all but the last one or two items per CTA go out in waves, CTA c taking items c, c + CTAs, ...: the CTAs then work
 // on the same few heads of one request at a time.  (Equal runs had them all over 268 MB of keys: 4 x 2,048 tokens over
 // 8,192 states drew 5.5 TB/s from memory and took 1,552 us.)  The tiles of the rest make up for unequal waves.
@@ -46,6 +47,10 @@ namespace {
 constexpr float kGain = 7.f;
 constexpr float kMostSum = 32768.f;    // of 64 P: none of them leaves fp16's range
 constexpr int kLoadWarps = 4;
+// KV tiles that an item counts besides its own: its queries, its first maximum and its rows' way out.  With 0, 1, 2, 3, us:
+//   16 x 4-448 tokens over 64-1,500 states, 16 heads of 16, 64 dims: 64, 51, 53, 53;  32 of 8, 128 dims: 127, 88, 81, 83;
+//   32 of 8, 256 dims: 193, 172, 171, 181;  100 x 1-100 over 64-1,000, 32 of 8, 128 dims: 161, 144, 154, 154.
+constexpr int kItemTiles = 2;
 constexpr int kPlanReqs = 4096;        // requests up to which a launch may go out in waves
 constexpr int kTallSms = 160;
 constexpr long long kL2Keys = 48 << 20;   // bytes of keys and values that a launch may spread its CTAs over
@@ -132,18 +137,21 @@ __device__ __forceinline__ int piece_steps(const Piece& it) {
   return (min(it.tiles * kTile, it.hi - it.key0) + kKeys - 1) / kKeys;
 }
 
+// Length of an item in the sequence that is cut into runs: its KV tiles, and what its queries and its end take besides.
+__device__ __forceinline__ int item_length(const ReqShape& s) { return s.tiles > 0 ? s.tiles + kItemTiles : 0; }
+
 // Walk over the pieces of a CTA: its items of the waves, then its run of the rest.
 template <int RP>
 struct TallWalk {
   int wave, waves, ctas, item;    // item: of the current wave
   int r, first_item;              // request of the item, items in front of it
-  long long at, end;              // the run, in KV tiles of the whole sequence
+  long long at, end;              // the run, in the whole sequence
   int tail_r;
   long long tail_start;           // of request tail_r in the sequence
-  long long base, work;           // where the runs' tiles begin in the sequence, and how many there are
+  long long base, work;           // where the runs begin in the sequence, and how long they are together
   int runs;                       // without waves: that they are cut into, equally
   const long long* bounds;        // with waves: where the CTAs' runs begin, behind `base`
-  // CTA that has tile x of the sequence in its run.
+  // CTA that has position x of the sequence in its run.
   __device__ __forceinline__ int owner(long long x) const {
     x -= base;
     if (waves == 0) return (int)(((x + 1) * runs - 1) / work);
@@ -155,11 +163,9 @@ struct TallWalk {
     return lo;
   }
   __device__ __forceinline__ bool next(const Kv16Params& p, Piece* out) {
-    const bool whole = wave < waves;
-    if (!whole && at >= end) return false;
     ReqShape s;
     int it, tile, count;   // item of the request, tiles of it
-    if (whole) {
+    if (wave < waves) {
       s = req_shape<RP>(p, r);
       int n = s.tiles > 0 ? s.row_tiles * p.num_kv_heads : 0;
       while (item >= first_item + n) {
@@ -176,22 +182,26 @@ struct TallWalk {
       ++wave;
       item += ctas;
     } else {
-      s = req_shape<RP>(p, tail_r);
-      long long n = (long long)s.tiles * s.row_tiles * p.num_kv_heads;
-      while (at >= tail_start + n) {
-        tail_start += n;
-        ++tail_r;
+      do {
+        if (at >= end) return false;
         s = req_shape<RP>(p, tail_r);
-        n = (long long)s.tiles * s.row_tiles * p.num_kv_heads;
-      }
-      const long long off = at - tail_start;
-      it = (int)(off / s.tiles);
-      tile = (int)(off - (long long)it * s.tiles);
-      count = (int)min((long long)(s.tiles - tile), end - at);
+        int n = item_length(s);
+        while (at >= tail_start + (long long)n * s.row_tiles * p.num_kv_heads) {
+          tail_start += (long long)n * s.row_tiles * p.num_kv_heads;
+          ++tail_r;
+          s = req_shape<RP>(p, tail_r);
+          n = item_length(s);
+        }
+        const long long off = at - tail_start;
+        it = (int)(off / n);
+        const int a = (int)(off - (long long)it * n), b = (int)min((long long)n, a + (end - at));   // of the item's length
+        tile = max(0, a - kItemTiles);
+        count = b - kItemTiles - tile;
+        out->first_cta = owner(at - a + kItemTiles);
+        out->last_cta = owner(at - a + n - 1);
+        at += b - a;
+      } while (count <= 0);   // (no keys yet)
       out->r = tail_r;
-      out->first_cta = owner(at - tile);
-      out->last_cta = owner(at - tile + s.tiles - 1);
-      at += count;
     }
     const int kvh = (int)((uint32_t)it / (uint32_t)s.row_tiles), rt = it - kvh * s.row_tiles;
     out->kvh = kvh;
@@ -218,14 +228,14 @@ __device__ __forceinline__ TallWalk<RP> make_plan(const Kv16Params& p, uint8_t* 
   long long* const scratch = bounds;
   const int R = p.num_reqs, C = (int)gridDim.x, tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int per = (R + kThreads - 1) / kThreads, r0 = min(R, tid * per), r1 = min(R, r0 + per);
-  // items (0), KV tiles of all items (1), KV tiles of the requests' keys (2): in front of this thread's requests, and in all
+  // items (0), their lengths (1), KV tiles of the requests' keys (2): in front of this thread's requests, and in all
   long long mine[3] = {0, 0, 0}, before[3], total[3] = {0, 0, 0};
 #pragma unroll 1
   for (int r = r0; r < r1; ++r) {
     const ReqShape s = req_shape<RP>(p, r);
     const int n = s.tiles > 0 ? s.row_tiles * p.num_kv_heads : 0;
     mine[0] += n;
-    mine[1] += (long long)n * s.tiles;
+    mine[1] += (long long)n * item_length(s);
     mine[2] += s.tiles;
   }
 #pragma unroll
@@ -270,7 +280,7 @@ __device__ __forceinline__ TallWalk<RP> make_plan(const Kv16Params& p, uint8_t* 
 #pragma unroll 1
       for (;; ++r) {
         const ReqShape s = req_shape<RP>(p, r);
-        const long long n = (long long)s.tiles * s.row_tiles * p.num_kv_heads;
+        const long long n = (long long)item_length(s) * s.row_tiles * p.num_kv_heads;
         if (w.at < start + n) break;
         start += n;
       }
@@ -282,22 +292,22 @@ __device__ __forceinline__ TallWalk<RP> make_plan(const Kv16Params& p, uint8_t* 
     w.tail_start = scratch[1];
     return w;
   }
-  // tile_first[r] KV tiles and item_first[r] items lie in front of request r, whose items have tiles[r] KV tiles
-  long long* const tile_first = reinterpret_cast<long long*>(arrays);
-  int* const item_first = reinterpret_cast<int*>(tile_first + R);
-  int* const tiles = item_first + R;
+  // length_first[r] of the sequence and item_first[r] items lie in front of request r, whose items are length[r] long
+  long long* const length_first = reinterpret_cast<long long*>(arrays);
+  int* const item_first = reinterpret_cast<int*>(length_first + R);
+  int* const length = item_first + R;
 #pragma unroll 1
   for (int r = r0; r < r1; ++r) {
     const ReqShape s = req_shape<RP>(p, r);
     const int n = s.tiles > 0 ? s.row_tiles * p.num_kv_heads : 0;
-    tiles[r] = s.tiles;
+    length[r] = item_length(s);
     item_first[r] = (int)before[0];
-    tile_first[r] = before[1];
+    length_first[r] = before[1];
     before[0] += n;
-    before[1] += (long long)n * s.tiles;
+    before[1] += (long long)n * length[r];
   }
   __syncthreads();
-  // request of an item, or of a tile of the sequence: the last that begins at or in front of it
+  // request of an item, or of a position of the sequence: the last that begins at or in front of it
   auto last_of = [&](const auto* first, long long x) {
     int lo = 0, hi = R - 1;
 #pragma unroll 1
@@ -309,15 +319,15 @@ __device__ __forceinline__ TallWalk<RP> make_plan(const Kv16Params& p, uint8_t* 
   };
   const long long f = (long long)w.waves * C;
   const int fr = last_of(item_first, f);
-  w.base = tile_first[fr] + (f - item_first[fr]) * tiles[fr];
+  w.base = length_first[fr] + (f - item_first[fr]) * length[fr];
   w.work = total[1] - w.base;
   w.runs = 0;
-  // CTA c has load(c) tiles of the waves; the rest fills all up to a level: the smallest that holds it
+  // CTA c has a load of the waves; the rest fills all up to a level: the smallest that holds it
 #pragma unroll 1
   for (int c = tid; c < C; c += kThreads) {
     long long load = 0;
 #pragma unroll 1
-    for (int k = 0; k < w.waves; ++k) load += tiles[last_of(item_first, c + (long long)k * C)];
+    for (int k = 0; k < w.waves; ++k) load += length[last_of(item_first, c + (long long)k * C)];
     bounds[c] = load;
   }
   __syncthreads();
@@ -360,8 +370,8 @@ __device__ __forceinline__ TallWalk<RP> make_plan(const Kv16Params& p, uint8_t* 
   w.first_item = item_first[w.r];
   w.at = w.base + bounds[blockIdx.x];
   w.end = w.base + bounds[blockIdx.x + 1];
-  w.tail_r = last_of(tile_first, w.at);
-  w.tail_start = tile_first[w.tail_r];
+  w.tail_r = last_of(length_first, w.at);
+  w.tail_start = length_first[w.tail_r];
   tc::fence_async_smem();   // (boxes are written where the arrays are, through the other proxy)
   __syncthreads();
   return w;
