@@ -21,6 +21,11 @@
 // TMA, boxes of 16 slots x 64 dims, 64 requests x 8,192 keys x 8 heads x 128 dims) moved 6.83 TB/s, with boxes of 4 KB 7.06, 16-byte
 // copies 7.17, which also take pages of any size and place.
 //
+// Measured, bf16, one call behind another: 64 requests x 8,192 keys, 32 heads of 8, 128 dims 320 us, 6.7 TB/s; 61 x 4,096-12,288, 12 of
+// 2, 256 dims 163 us, 6.5 TB/s; one request of 131,072 keys 95 us, 5.6 TB/s, of which the last arriver's merge of 37 pieces and
+// the start are 13; 8 requests of up to 4,095 keys 22.7 us for 79 MB, some 5 in front of the first tile (the launch, the
+// lengths, the block table, the first keys: one after the other) and 6 behind the last (the merge).
+//
 // Schedule: the keys of all (request, row tile) form one sequence, which is cut into equal runs, one for every group of Hkv CTAs;
 // CTA h of a group reads head h, so that the heads of a page are read at the same time.  The pieces of a row tile that a cut
 // divides are merged by the CTA that arrives last: one launch, and the same bits whoever is last.
@@ -38,9 +43,13 @@ constexpr int kSoftmaxThreads = 128;   // warps 0-3: thread t is key t of a tile
 constexpr int kLoadWarp = 4;           // warps 4-7
 constexpr int kMmaWarp = 8, kScheduleWarp = 9;
 constexpr int kThreads = 320;
-// The sequence is counted in grains of 32 keys; a row tile counts kPieceGrains more, what its queries and its end take.
+// The sequence is counted in grains of 32 keys; a row tile counts kPieceGrains more, what its queries and its end take.  (With 0, 4
+// and 8, us: 200 requests of up to 500 keys 65.5, 61.4, 61.5; 300 of up to 300 at 256 dims 47.1, 41.0, 38.9; 8 of up to 4,095 32.8,
+// 30.7, 30.7; 2,000 of 100 260, 258, 256.  Grains of 128 keys: 4 requests of 500 18.4 instead of 16.4.)
 constexpr int kGrain = 32, kPieceGrains = 4;
-constexpr int kRunMin = 4;             // length of a run at least
+// Length of a run at least, so that few keys are not spread over pieces that cost more to merge: with 1, 4 and 16, us, one request
+// of 2,000 keys 24.6, 18.5, 18.4, four of 500 16.4, 16.4, 18.4.
+constexpr int kRunMin = 4;
 constexpr float kGain = 7.f, kSlack = 8.f;
 
 template <int HD, int RP>
@@ -52,7 +61,8 @@ struct Geo {
   static constexpr int qimage = RP * HD * 2;
   static constexpr int pimage = 2 * RP * kTile * 2;
   static constexpr int fixed = 2 * qimage + pimage + 4 * RP * 4 * 2 + 768;
-  // Two CTAs per SM where three units fit, else one.
+  // Two CTAs per SM where three units fit, else one: one's softmax and merge beside the other's copies.  (One against two, us: 64 requests
+  // x 8,192 keys 348 / 329, 64 x 2,000 109 / 104, 64 x 64-1,500 at 64 dims 70 / 57.)
   static constexpr int units2 = (115712 - fixed - 1024) / unit;
   static constexpr int ctas = units2 >= 3 && RP <= 16 ? 2 : 1;
   static constexpr int most = 98304 * (3 - ctas) / unit;

@@ -14,25 +14,35 @@
 // of its own rounding), its sum is not.  The steps are of 64 keys (128 at 256 dims) with two S buffers,
 // so that a step's QK and the last one's PV run beside its softmax.
 //
-// What bounds it: the special function unit, which takes 8 cycles for a warp's 32 exponentials, 2,048 for the two row tiles' scores
-// of 128 keys (with the conversions beside them 2,460, measured on their own), and the MMAs, about 2,700 with QK in steps of
-// 64 keys (both operands from shared memory, which that takes 1.5 times as often).  4 x 2,048 tokens over 8,192 states, 32 heads
-// of 8, 128 dims, bf16: 977 us, 1,126 TFLOP/s.  (Steps of 128 keys with one S buffer, a row tile waiting for its MMAs: 1,241; an
-// eighth of the exponentials as a polynomial on the FMA pipe 981, a quarter 1,045; the row tiles' exponentials in turn no faster.)
+// What bounds it: a row tile's chain of a step.  Cycles per step of 64 keys at 128 dims, both row tiles at work: 1,380 for the
+// exponentials of both (8 of the special function unit for a warp's 32, the conversions beside them), 80 for S to come from TMEM, 160
+// for P to go there, some 300 for the two barriers: 2,000 in all, beside 1,350 of MMAs (eight of QK over 64 keys take 400 instead
+// of 256: both operands come from shared memory).  Without the exponentials a launch takes 15 % less, with an eighth of QK's MMAs and a
+// quarter of PV's 8 %.
+// Measured, bf16, alone: 4 x 2,048 tokens over 8,192 states, 32 heads of 8, 128 dims 944 us, 1,165 TFLOP/s (1,095 us, 1,004 TFLOP/s one
+// behind another, at the board's power limit); 8 x 1,000 over 4,000 at 256 dims 1,487 us, 705; 64 x 16 over 4,000, one row tile
+// of two, 207 us, 5.2 TB/s; 16 x 4-448 over 64-1,500, 16 heads of 16, 64 dims 47 us, of which the start is 3, an item's first maximum
+// and rows' way out 3 each, the last merge 4.
+// Taken back: steps of 128 keys with one S buffer, a row tile waiting for its MMAs, 1,241; an eighth of the exponentials as a
+// polynomial on the FMA pipe 981 against 977, a quarter 1,045; the row tiles' exponentials in turn, or half a step apart (983 against
+// 960); P rounded with integer instructions 1,007 against 958; MMAs predicated lane by lane in a warp that stays together 958 against 946.
 //
 // A warp per row tile issues its MMAs, so neither row tile waits for the other, and nothing relies on the order in which MMAs on
 // different accumulators run.
 //
 // Copies: tiles that are visible as a whole come as boxes (tiled TMA, 64 dims of up to 32 slots of a page) where pages are a
 // multiple of 8 slots, others as 16-byte copies, which zero what is not visible.  (All by 16-byte copies: 1,300 cycles a
-// unit of 32 KB, more than the MMAs take.)
+// unit of 32 KB.  Copies against boxes, us: 4 x 2,048 tokens over 8,192 states 1,049 / 961, 32 x 200 over 8,000 1,035 / 949, 8 x 1,000 over
+// 4,000 at 256 dims 2,026 / 1,677, 64 x 256 over 2,000 at 64 dims 303 / 298.)
 //
 // Schedule: items (row tile, KV head, request), in the order request, head, row tile, so that neighbouring items read the same keys.
 // While the keys of a launch fit in the L2 cache, the sequence of all their KV tiles is cut into equal runs, one per CTA (an item
 // counts kItemTiles more, which stand in front of its tiles).
 // Otherwise all but the last one or two items per CTA go out in waves, CTA c taking items c, c + CTAs, ...: the CTAs then work
-// on the same few heads of one request at a time.  (Equal runs had them all over 268 MB of keys: 4 x 2,048 tokens over
-// 8,192 states drew 5.5 TB/s from memory and took 1,552 us.)  The tiles of the rest make up for unequal waves.
+// on the same few heads of one request at a time.  The tiles of the rest make up for unequal waves.  Equal runs against waves, us:
+// above the bound 4 x 2,048 tokens over 8,192 states 981 / 944, 16 x 10-512 over 64-8,000 314 / 303, 64 x 64 over 64-4,000 at 64 dims
+// 166 / 146, 8 x 1,000 over 4,000 at 256 dims 1,641 / 1,487 (100 x 1-100 over 64-1,000 134 / 152); below it 8 x 1,200 over 1,000 at 64
+// dims 111 / 115, 16 x 4-448 over 64-1,500 at 128 dims 81 / 83 (30 x 400 over 200 122 / 118).
 #include "kv16_sched.cuh"
 #include "page_copy.cuh"
 #include "pdl.cuh"
