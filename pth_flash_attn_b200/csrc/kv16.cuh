@@ -85,6 +85,9 @@ __device__ __forceinline__ float kv16_exp2(float x) {
   return y;
 }
 
+// A sum under a weight.  Weights are above zero: one that has run out of exponents leaves an infinite sum as it is.
+__device__ __forceinline__ float weighed(float sum, float w) { return w == 0.f && isinf(sum) ? sum : sum * w; }
+
 // launcher.cu: the calling thread's error text.
 int32_t clear_error();
 int32_t set_error(int32_t code, const std::string& msg);

@@ -230,22 +230,29 @@ __device__ __forceinline__ void tmem_load(uint32_t addr, uint32_t* r) {
 }
 template <int N>
 __device__ __forceinline__ void tmem_store(uint32_t addr, const uint32_t* r) {
-  static_assert(N % 16 == 0, "columns");
+  if constexpr (N == 8) {
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"r"(addr), "r"(r[0]), "r"(r[1]), "r"(r[2]),
+                 "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7])
+                 : "memory");
+  } else {
 #pragma unroll
-  for (int i = 0; i < N; i += 16) tc::tmem_st16(addr + i, r + i);
+    for (int i = 0; i < N; i += 16) tc::tmem_st16(addr + i, r + i);
+  }
 }
 
-// Two numbers as 16-bit parts: hi is their rounding, lo the rounding of what is left.
+// Two numbers as 16-bit parts: hi is their rounding, but the type's smallest normal number at least, lo the rounding of what is
+// left.  So hi is above zero for every key, and an infinite value makes its part of the output infinite: that part says so,
+// whatever the sign of lo is (a hi of zero, or hi and lo together, would make it NaN).  Keys that are not visible have values of zero.
 template <bool kHalf>
 __device__ __forceinline__ void split2(float a, float b, uint32_t* hi, uint32_t* lo) {
   if constexpr (kHalf) {
-    const __half2 h = __floats2half2_rn(a, b);
+    const __half2 h = __hmax2_nan(__floats2half2_rn(a, b), __floats2half2_rn(0x1p-14f, 0x1p-14f));
     const float2 f = __half22float2(h);
     const __half2 l = __floats2half2_rn(a - f.x, b - f.y);
     *hi = *reinterpret_cast<const uint32_t*>(&h);
     *lo = *reinterpret_cast<const uint32_t*>(&l);
   } else {
-    const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
+    const __nv_bfloat162 h = __hmax2_nan(__floats2bfloat162_rn(a, b), __floats2bfloat162_rn(0x1p-126f, 0x1p-126f));
     const uint32_t w = *reinterpret_cast<const uint32_t*>(&h);
     const __nv_bfloat162 l = __floats2bfloat162_rn(a - __uint_as_float(w << 16), b - __uint_as_float(w & 0xffff0000u));
     *hi = w;
@@ -291,22 +298,40 @@ __device__ __forceinline__ void merge_pieces(const Kv16Params& p, const Piece& i
       const float use = to == -INFINITY ? 0.f : to, alpha = kv16_exp2(top - use);
       top = to;
       l *= alpha;
+      if (alpha == 0.f) {   // (the same in all lanes) out of exponents
 #pragma unroll
-      for (int v = 0; v < kVec; ++v) {
+        for (int v = 0; v < kVec; ++v) {
 #pragma unroll
-        for (int e = 0; e < 4; ++e) acc[v][e] *= alpha;
+          for (int e = 0; e < 4; ++e) acc[v][e] = weighed(acc[v][e], alpha);
+        }
+      } else {
+#pragma unroll
+        for (int v = 0; v < kVec; ++v) {
+#pragma unroll
+          for (int e = 0; e < 4; ++e) acc[v][e] *= alpha;
+        }
       }
 #pragma unroll
       for (int b = 0; b < kBatch; ++b) {
         if (k0 + b >= pieces) break;
         const float f = kv16_exp2(ref[b] - use);
         l = fmaf(f, sum[b], l);
+        if (f == 0.f) {   // (the same in all lanes)
 #pragma unroll
-        for (int v = 0; v < kVec; ++v) {
-          acc[v][0] = fmaf(f, o[b][v].x, acc[v][0]);
-          acc[v][1] = fmaf(f, o[b][v].y, acc[v][1]);
-          acc[v][2] = fmaf(f, o[b][v].z, acc[v][2]);
-          acc[v][3] = fmaf(f, o[b][v].w, acc[v][3]);
+          for (int v = 0; v < kVec; ++v) {
+            acc[v][0] += weighed(o[b][v].x, 0.f);
+            acc[v][1] += weighed(o[b][v].y, 0.f);
+            acc[v][2] += weighed(o[b][v].z, 0.f);
+            acc[v][3] += weighed(o[b][v].w, 0.f);
+          }
+        } else {
+#pragma unroll
+          for (int v = 0; v < kVec; ++v) {
+            acc[v][0] = fmaf(f, o[b][v].x, acc[v][0]);
+            acc[v][1] = fmaf(f, o[b][v].y, acc[v][1]);
+            acc[v][2] = fmaf(f, o[b][v].z, acc[v][2]);
+            acc[v][3] = fmaf(f, o[b][v].w, acc[v][3]);
+          }
         }
       }
     }
@@ -566,17 +591,14 @@ __global__ void __launch_bounds__(kThreads, (Geo<HD, RP>::ctas)) kv16_short_kern
               ok &= kv16_wait(&bars[Bars::pv_done], (tile - 1) & 1, abort_flag);
               tc::fence_after_sync();
 #pragma unroll
-              for (int part = 0; part < G::parts; ++part) {
-                uint32_t o[2 * RP];
-                const uint32_t addr = tmem_base + G::o_col + part * 2 * RP + lane_addr;
-                tmem_load<2 * RP>(addr, o);
-                tc::tmem_ld_wait<2 * RP>(o);
+              for (int half = 0; half < 2 * G::parts; ++half) {   // hi and lo of every part
+                uint32_t o[RP];
+                const uint32_t addr = tmem_base + G::o_col + half * RP + lane_addr;
+                tmem_load<RP>(addr, o);
+                tc::tmem_ld_wait<RP>(o);
 #pragma unroll
-                for (int n = 0; n < RP; ++n) {
-                  o[n] = __float_as_uint(__uint_as_float(o[n]) * alpha[n]);
-                  o[RP + n] = __float_as_uint(__uint_as_float(o[RP + n]) * alpha[n]);
-                }
-                tmem_store<2 * RP>(addr, o);
+                for (int n = 0; n < RP; ++n) o[n] = __float_as_uint(weighed(__uint_as_float(o[n]), alpha[n]));
+                tmem_store<RP>(addr, o);
               }
               tc::tmem_st_wait();
             }
@@ -629,7 +651,7 @@ __global__ void __launch_bounds__(kThreads, (Geo<HD, RP>::ctas)) kv16_short_kern
 #pragma unroll
             for (int n = 0; n < RP; ++n) {
               if (n < it.rows) {
-                const float v = __uint_as_float(o[n]) + __uint_as_float(o[RP + n]);
+                const float hi = __uint_as_float(o[n]), v = isinf(hi) ? hi : hi + __uint_as_float(o[RP + n]);
                 if (whole) {
                   int token, head;
                   row_of(p, it.first_token, kvh, it.row0 + n, &token, &head);

@@ -11,7 +11,8 @@
 // maximum of a row's first 64 keys.  Later ones need no maximum: the sum of 64 P, which the row sum takes anyway, says
 // whether one of them has outgrown ref too far (kMostSum); then ref moves to their maximum, O and l are rescaled and the
 // 64 are computed again.  P is rounded to the cache's type for the MMA (the error of the output is sqrt(2) times that
-// of its own rounding), its sum is not.  The steps are of 64 keys (128 at 256 dims) with two S buffers,
+// of its own rounding), its sum is not.  (A probability below 2^-31 of the row's largest may be zero in fp16: an infinite value
+// under it gives NaN.)  The steps are of 64 keys (128 at 256 dims) with two S buffers,
 // so that a step's QK and the last one's PV run beside its softmax.
 //
 // What bounds it: a row tile's chain of a step.  Cycles per step of 64 keys at 128 dims, both row tiles at work: 1,380 for the
@@ -708,7 +709,7 @@ __global__ void __launch_bounds__(Tall<HD>::threads, Tall<HD>::ctas) kv16_tall_k
                   tc::tmem_ld16(o_tmem + d * 16, o);
                   tc::tmem_ld_wait<16>(o);
 #pragma unroll
-                  for (int n = 0; n < 16; ++n) o[n] = __float_as_uint(__uint_as_float(o[n]) * alpha);
+                  for (int n = 0; n < 16; ++n) o[n] = __float_as_uint(weighed(__uint_as_float(o[n]), alpha));
                   tc::tmem_st16(o_tmem + d * 16, o);
                 }
                 tc::tmem_st_wait();
@@ -822,6 +823,14 @@ __global__ void __launch_bounds__(Tall<HD>::threads, Tall<HD>::ctas) kv16_tall_k
                   u[n] = __ldcg(t + (c * 16 + n) * RP);
                 }
                 const float fa = a ? ex2f(wa - use) * inv : 0.f, fb = b ? ex2f(wb - use) * inv : 0.f;
+                if (__any_sync(0xffffffffu, (a && fa == 0.f) || (b && fb == 0.f))) {   // a piece far below the others: its infinities count
+#pragma unroll
+                  for (int n = 0; n < 16; ++n) {
+                    if (a) o[n] += weighed(v[n], fa);
+                    if (b) o[n] += weighed(u[n], fb);
+                  }
+                  continue;
+                }
 #pragma unroll
                 for (int n = 0; n < 16; ++n) {
                   if (a) o[n] = fmaf(fa, v[n], o[n]);
