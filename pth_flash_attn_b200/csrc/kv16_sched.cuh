@@ -15,6 +15,13 @@ namespace {
 constexpr int kTile = 128;             // keys
 constexpr int kCounterBytes = 4096;    // arrival counters at the start of the workspace, one per CTA
 
+// 2^kGain is P of a row's largest score when its reference is set; scores that come later take P further up, by 2^8 at most.  fp16:
+// P, and the second half of a P in two halves, stay within its numbers, 2^-24 .. 65,504.  bf16 has the exponents of the 32-bit
+// sums: P is at most 2^-16, so that P times values of any size, summed over 65,536 keys, stays below 2^128 as the result does.
+// (On the other side a product below 2^-126 may be lost: 2^-102 of the output.)
+template <bool kHalf>
+constexpr float kGain = kHalf ? 7.f : -24.f;
+
 // One piece of a row tile: the keys [lo, hi) from key0 on, in `tiles` KV tiles.
 struct Piece {
   int r, kvh;

@@ -11,8 +11,7 @@
 // maximum less kGain when it is set, and moves (with l and O rescaled) only when a score outgrows it by kSlack, so that most
 // tiles need no maximum at all, only a vote of the 128 threads.  P goes into the MMA as the sum of two 16-bit
 // numbers (hi + lo: 2 x 8 or 2 x 11 bits), side by side on N: at the instruction's minimum of 16 columns that costs
-// eight rows nothing, and the outputs' error is their own rounding (with one: 1.4 times it).  kGain keeps fp16's lo above its smallest
-// numbers; 2^(kGain + kSlack) is below its largest.
+// eight rows nothing, and the outputs' error is their own rounding (with one: 1.4 times it).
 //
 // What bounds it: the cache's bytes, 4 D per key and KV head at 4 D G flops.  The tile's parts (128 keys x 128 dims of K, of
 // V) are units of one ring of shared memory, K of the next tile ahead of V of this one, which is the order in which they are
@@ -50,7 +49,7 @@ constexpr int kGrain = 32, kPieceGrains = 4;
 // Length of a run at least, so that few keys are not spread over pieces that cost more to merge: with 1, 4 and 16, us, one request
 // of 2,000 keys 24.6, 18.5, 18.4, four of 500 16.4, 16.4, 18.4.
 constexpr int kRunMin = 4;
-constexpr float kGain = 7.f, kSlack = 8.f;
+constexpr float kSlack = 8.f;
 
 template <int HD, int RP>
 struct Geo {
@@ -566,7 +565,7 @@ __global__ void __launch_bounds__(kThreads, (Geo<HD, RP>::ctas)) kv16_short_kern
 #pragma unroll
           for (int n = 0; n < RP; ++n) {
             x[n] = fmaf(__uint_as_float(sr[n]), p.scale_log2, -ref[n]);
-            outgrown |= n < it.rows && !(x[n] <= kGain + kSlack);   // (also where ref is not set yet)
+            outgrown |= n < it.rows && !(x[n] <= kGain<kHalf> + kSlack);   // (also where ref is not set yet)
           }
           if (softmax_any(outgrown)) {
 #pragma unroll
@@ -579,7 +578,7 @@ __global__ void __launch_bounds__(kThreads, (Geo<HD, RP>::ctas)) kv16_short_kern
             bool moved = false;
 #pragma unroll
             for (int n = 0; n < RP; ++n) {
-              const float m = fmaxf(fmaxf(wmax[n], wmax[RP + n]), fmaxf(wmax[2 * RP + n], wmax[3 * RP + n])) - kGain;
+              const float m = fmaxf(fmaxf(wmax[n], wmax[RP + n]), fmaxf(wmax[2 * RP + n], wmax[3 * RP + n])) - kGain<kHalf>;
               const float to = fmaxf(ref[n], m);
               alpha[n] = to == -INFINITY ? 1.f : kv16_exp2(ref[n] - to);
               moved |= alpha[n] != 1.f;

@@ -11,8 +11,8 @@
 // maximum of a row's first 64 keys.  Later ones need no maximum: the sum of 64 P, which the row sum takes anyway, says
 // whether one of them has outgrown ref too far (kMostSum); then ref moves to their maximum, O and l are rescaled and the
 // 64 are computed again.  P is rounded to the cache's type for the MMA (the error of the output is sqrt(2) times that
-// of its own rounding), its sum is not.  (A probability below 2^-31 of the row's largest may be zero in fp16: an infinite value
-// under it gives NaN.)  The steps are of 64 keys (128 at 256 dims) with two S buffers,
+// of its own rounding), its sum is not.  (A probability below 2^-31 of the row's largest, 2^-102 in bf16, may be
+// zero: an infinite value under it gives NaN.)  The steps are of 64 keys (128 at 256 dims) with two S buffers,
 // so that a step's QK and the last one's PV run beside its softmax.
 //
 // What bounds it: a row tile's chain of a step.  Cycles per step of 64 keys at 128 dims, both row tiles at work: 1,380 for the
@@ -55,8 +55,8 @@ __device__ unsigned int g_kv16_tall_status = 0;
 
 namespace {
 
-constexpr float kGain = 7.f;
-constexpr float kMostSum = 32768.f;    // of 64 P: none of them leaves fp16's range
+template <bool kHalf>
+constexpr float kMostSum = kHalf ? 0x1p15f : 0x1p-16f;   // of 64 P
 constexpr int kLoadWarps = 4;
 // KV tiles that an item counts besides its own: its queries, its first maximum and its rows' way out.  With 0, 1, 2, 3, us:
 //   16 x 4-448 tokens over 64-1,500 states, 16 heads of 16, 64 dims: 64, 51, 53, 53;  32 of 8, 128 dims: 127, 88, 81, 83;
@@ -685,12 +685,12 @@ __global__ void __launch_bounds__(Tall<HD>::threads, Tall<HD>::ctas) kv16_tall_k
 #pragma unroll
                 for (int e = 0; e < 4; ++e) mx[e] = max3(mx[e], __uint_as_float(r[n + 2 * e]), __uint_as_float(r[n + 2 * e + 1]));
               }
-              return max3(fmaxf(mx[0], mx[1]), mx[2], mx[3]) * p.scale_log2 - kGain;
+              return max3(fmaxf(mx[0], mx[1]), mx[2], mx[3]) * p.scale_log2 - kGain<kHalf>;
             };
             if (t == 0 && half == 0) ref = maximum();
             uint32_t pk[32];
             float total = exponentials<kHalf>(r, p.scale_log2, ref == -INFINITY ? 0.f : -ref, pk);
-            const bool outgrown = !(total <= kMostSum) || ref == -INFINITY;
+            const bool outgrown = !(total <= kMostSum<kHalf>) || ref == -INFINITY;
             if (__any_sync(0xffffffffu, outgrown)) {
               const float to = outgrown ? fmaxf(ref, maximum()) : ref;
               const float alpha = to == -INFINITY ? 1.f : ex2f(ref - to);

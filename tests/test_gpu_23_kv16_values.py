@@ -1,4 +1,5 @@
-"""GPU tests of attention over the 16-bit cache at values from the ends of its types: infinities among the visible values."""
+"""GPU tests of attention over the 16-bit cache at values from the ends of its types: infinities among the visible values, values
+near the largest of bf16, and far below one."""
 import math
 
 import pytest
@@ -115,3 +116,43 @@ def test_a_value_that_fp16_cannot_hold():
     ops.kv16_write(key, value, b.k, b.v, slots)
     _check_with_infinities(b.decode())
     assert bool((b.out[..., 5] == math.inf).all()) and bool((b.out[..., 6] == -math.inf).all())
+
+
+def _scale_values(b, size, seed=0):
+    """Values of +-size / 2 .. size: of one sign in even columns, of both in odd ones."""
+    gen = torch.Generator(device="cuda").manual_seed(seed)
+    x = (torch.rand(b.v.shape, generator=gen, device="cuda", dtype=torch.float64) / 2 + 0.5) * size
+    sign = torch.where(torch.rand(b.v.shape, generator=gen, device="cuda") < 0.5, -1.0, 1.0)
+    sign[..., ::2] = 1
+    b.v.copy_(torch.where(torch.isnan(b.v), math.nan, x * sign))
+    return b
+
+
+# (bf16 ends at 3.39e38, as 32 bits do: neither sums of weighted values nor their merges may pass it where the result does not)
+SIZES = [3.3e38, 1e37, 1e30, 1e-25]
+
+
+@pytest.mark.parametrize("size", SIZES)
+@pytest.mark.parametrize("Hq,Hkv,D", [(8, 2, 64), (8, 2, 128), (6, 1, 256), (32, 2, 128), (32, 1, 64), (32, 1, 256)])
+def test_decode_values_of_any_size(Hq, Hkv, D, size):
+    kv_lens = [1, 2, 0, 129, 700, 5000, 40000]
+    _scale_values(Batch(kv_lens, [1] * len(kv_lens), Hq, Hkv, D, BF16, seed=D), size).decode().check()
+
+
+@pytest.mark.parametrize("size", SIZES)
+@pytest.mark.parametrize("D", [64, 128, 256])
+@pytest.mark.parametrize("q_lens", [[1] * 6, [3] * 6, [70, 1, 300, 128, 5, 200]])
+def test_cross_values_of_any_size(q_lens, D, size):
+    _scale_values(Batch([1, 2, 129, 700, 5000, 30000], q_lens, 8, 2, D, BF16, seed=D), size).cross().check()
+
+
+# Weights that grow behind the first keys, by less than what moves a row's reference and by more.
+@pytest.mark.parametrize("levels", [(0.0,), (0.0,) + (5.4,) * 20, (0.0, 5.4, 5.6, 11.2), (0.0, 20.0, 40.0, 60.0)])
+@pytest.mark.parametrize("D", [64, 128, 256])
+@pytest.mark.parametrize("q_lens", [[1, 1], [70, 1]])
+def test_largest_values_under_growing_weights(q_lens, D, levels):
+    b = _scale_values(Batch([5000, 40], q_lens, 8, 2, D, BF16, seed=3), 3.3e38)
+    _stairs(b, 0, levels)
+    if max(q_lens) == 1:
+        b.decode().check(what=str(levels))
+    b.cross().check(what=str(levels))
