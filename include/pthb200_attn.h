@@ -399,6 +399,11 @@ int32_t pthb200_kv16_args_bytes(void);
 int64_t pthb200_kv16_workspace_bytes(int32_t head_size, int32_t num_sms);
 int32_t pthb200_kv16_decode(const PthB200Kv16Args* args, void* stream);
 int32_t pthb200_kv16_cross(const PthB200Kv16Args* args, void* stream);
+/* Test only: the call of that form (cross: query_start_loc is not NULL), in which a warp of CTA 0 stops short, so that
+ * the CTA's waits run out (a few seconds at most), it leaves and pthb200_device_status says so: role 1 the scheduling warp after
+ * `after` pieces, 2 a copying warp after as many units of keys or values, 3 an MMA warp after as many steps.  128 dims, bf16, at
+ * most 8 rows or more than 16.  The results are void; zero the workspace behind it. */
+int32_t pthb200_test_kv16_held(const PthB200Kv16Args* args, int32_t role, int32_t after, void* stream);
 /* Validates as the calls above do, without launching (cross: query_start_loc is not NULL). */
 int32_t pthb200_kv16_check(const PthB200Kv16Args* args);
 

@@ -242,6 +242,7 @@ EXPORTED_SYMBOLS = (
     "pthb200_kv16_decode",
     "pthb200_kv16_cross",
     "pthb200_kv16_check",
+    "pthb200_test_kv16_held",
     "pthb200_tile_tokens",
     "pthb200_check_call",
     "pthb200_launch_count",
@@ -313,6 +314,8 @@ class B200Lib:
                            ("pthb200_kv16_decode", PthB200Kv16Args), ("pthb200_kv16_cross", PthB200Kv16Args)):
             getattr(lib, name).restype = ctypes.c_int32
             getattr(lib, name).argtypes = [ctypes.POINTER(args), ctypes.c_void_p]
+        lib.pthb200_test_kv16_held.restype = ctypes.c_int32
+        lib.pthb200_test_kv16_held.argtypes = [ctypes.POINTER(PthB200Kv16Args), ctypes.c_int32, ctypes.c_int32, ctypes.c_void_p]
         lib.pthb200_kv16_check.restype = ctypes.c_int32
         lib.pthb200_kv16_check.argtypes = [ctypes.POINTER(PthB200Kv16Args)]
         for fn in (lib.pthb200_test_schedule, lib.pthb200_test_range_schedule):
@@ -397,6 +400,10 @@ class B200Lib:
     def kv16_check(self, args: PthB200Kv16Args) -> int:
         """The checks of the two calls above, without a launch."""
         return int(self.lib.pthb200_kv16_check(ctypes.byref(args)))
+
+    def test_kv16_held(self, args: PthB200Kv16Args, role: int, after: int, *, stream: int = 0) -> int:
+        """A call in which a warp of CTA 0 stops short (the bounded waits' test)."""
+        return int(self.lib.pthb200_test_kv16_held(ctypes.byref(args), role, after, stream or None))
 
     def kv16_workspace_bytes(self, head_size: int, num_sms: int) -> int:
         return int(self.lib.pthb200_kv16_workspace_bytes(head_size, num_sms))

@@ -32,7 +32,15 @@ struct Kv16Params {
   int32_t box_slots;  // slots of a TMA box (tall kernel; 0: none)
   int32_t out_wide;   // rows of out lie on 32-byte boundaries (tall kernel)
   float scale_log2;  // softmax_scale * log2(e)
+  int32_t held_role, held_after;  // read by the test's instances alone
 };
+// The test's instances of the attention kernels leave out what one warp of CTA 0 does from some point on, so that the CTA's waits
+// run out.
+enum Kv16Held { kHeldNone = 0, kHeldSchedule = 1, kHeldCopies = 2, kHeldMma = 3 };
+template <bool kHeld>
+__device__ __forceinline__ bool kv16_held(const Kv16Params& p, Kv16Held role, uint32_t done) {
+  return kHeld && blockIdx.x == 0 && p.held_role == role && done >= (uint32_t)p.held_after;
+}
 
 // The query tokens of a request (none past the caller's bound or the end of the token arrays), and its visible keys.
 __device__ __forceinline__ int kv16_tokens(const Kv16Params& p, int r, int* first) {
@@ -57,18 +65,25 @@ __device__ __forceinline__ void kv16_visible(const Kv16Params& p, int r, int* lo
 __device__ __forceinline__ uint64_t swizzled_desc(uint32_t saddr, uint32_t lbo_bytes, uint32_t sbo_bytes) {
   return tc::smem_desc(saddr, lbo_bytes, sbo_bytes) | (uint64_t)2 << 61;
 }
-// Bounded wait for a phase of an mbarrier; once any wait of the CTA has given up, all do.  A try sleeps for a microsecond at
-// most, so the bound is between some 50 ms and 4 s.  (A test goes first: a try that may sleep takes 200 cycles where the phase is
-// complete already, a test 100, and a softmax step has little else to wait for.)
+// Bounded wait for a phase of an mbarrier; once any wait of the CTA has given up, all do.  A try sleeps for one microsecond, or for
+// four where all warps of a CTA wait, so the bound is 0.3 to 1.1 s.  (A test goes first: a try that may sleep takes 200 cycles where
+// the phase is complete already, a test 100, and a softmax step has little else to wait for.)
+constexpr uint32_t kWaitTries = 1u << 18;
 __device__ __forceinline__ bool kv16_wait(uint64_t* bar, uint32_t parity, volatile int* abort_flag) {
   if (tc::mbar_test_wait(bar, parity)) return true;
 #pragma unroll 1
-  for (uint32_t i = 0; i < (1u << 22); ++i) {
+  for (uint32_t i = 0; i < kWaitTries; ++i) {
     if (tc::mbar_try_wait_hint(bar, parity, 1000u)) return true;
     if (*abort_flag) return false;
   }
   *abort_flag = 1;
   return false;
+}
+// Wait for what is in flight when a CTA leaves behind a wait that gave up: for 20 to 70 ms at most, whatever the flag says.
+__device__ __forceinline__ void kv16_drain(uint64_t* bar, uint32_t parity) {
+#pragma unroll 1
+  for (uint32_t i = 0; i < (1u << 14) && !tc::mbar_try_wait_hint(bar, parity, 1000u); ++i) {
+  }
 }
 // Asynchronous copy of 16 bytes, or of none: then the destination is zeroed.
 __device__ __forceinline__ void copy16(uint32_t dst, const uint8_t* src, bool live) {
@@ -97,6 +112,8 @@ int64_t kv16_short_workspace_bytes(int head_size, int num_sms);
 int64_t kv16_tall_workspace_bytes(int head_size, int num_sms);
 cudaError_t launch_kv16_short(const Kv16Params& p, cudaStream_t stream);
 cudaError_t launch_kv16_tall(const Kv16Params& p, cudaStream_t stream);
+cudaError_t launch_kv16_short_held(const Kv16Params& p, cudaStream_t stream);   // 128 dims, bf16, at most 8 rows
+cudaError_t launch_kv16_tall_held(const Kv16Params& p, cudaStream_t stream);    // 128 dims, bf16
 cudaError_t launch_kv16_writer(const PthB200Kv16WriteArgs& a, cudaStream_t stream);
 cudaError_t launch_page_tables(const PthB200TablesArgs& a, cudaStream_t stream);
 

@@ -131,7 +131,7 @@ int64_t workspace_bytes(int head_size, int num_sms) {
   return std::max(kv16_short_workspace_bytes(head_size, num_sms), kv16_tall_workspace_bytes(head_size, num_sms));
 }
 
-int32_t attention(const PthB200Kv16Args* a, bool cross, void* stream) {
+int32_t attention(const PthB200Kv16Args* a, bool cross, void* stream, Kv16Held held = kHeldNone, int32_t held_after = 0) {
   clear_error();
   Kv16Params p;
   if (int32_t rc = build(a, cross, &p)) return rc;
@@ -142,6 +142,13 @@ int32_t attention(const PthB200Kv16Args* a, bool cross, void* stream) {
   const int64_t need = workspace_bytes(a->head_size, sms);
   KV16_REQUIRE(a->workspace_bytes >= need, "workspace has " + std::to_string(a->workspace_bytes) + " bytes, " + std::to_string(need) + " are needed");
   const bool tall = (int64_t)p.max_query_len * p.group >= kTallRows && p.max_query_len > 1;
+  if (held != kHeldNone) {
+    KV16_REQUIRE(a->head_size == 128 && a->dtype == PTH_ATTN_BF16 && (tall || (int64_t)p.max_query_len * p.group <= 8),
+                 "the test's instances take 128 dims, bf16, and at most 8 rows or more than 16");
+    p.held_role = held;
+    p.held_after = held_after;
+    return launched((tall ? launch_kv16_tall_held : launch_kv16_short_held)(p, static_cast<cudaStream_t>(stream)), "attention");
+  }
   return launched((tall ? launch_kv16_tall : launch_kv16_short)(p, static_cast<cudaStream_t>(stream)), "attention");
 }
 
@@ -201,5 +208,12 @@ int32_t pthb200_kv16_check(const PthB200Kv16Args* a) {
 }
 int32_t pthb200_kv16_decode(const PthB200Kv16Args* a, void* stream) { return pthb200::attention(a, false, stream); }
 int32_t pthb200_kv16_cross(const PthB200Kv16Args* a, void* stream) { return pthb200::attention(a, true, stream); }
+int32_t pthb200_test_kv16_held(const PthB200Kv16Args* a, int32_t role, int32_t after, void* stream) {
+  using namespace pthb200;
+  clear_error();
+  KV16_REQUIRE(a != nullptr, "args is NULL");
+  KV16_REQUIRE(role >= kHeldSchedule && role <= kHeldMma && after >= 0, "role must be in [1, 3], after >= 0");
+  return attention(a, a->query_start_loc != nullptr, stream, static_cast<Kv16Held>(role), after);
+}
 
 }  // extern "C"

@@ -7,6 +7,8 @@
 // first piece.  The last to arrive merges them, in the pieces' order.
 #pragma once
 
+#include <climits>
+
 #include "kv16.cuh"
 
 namespace pthb200 {
@@ -37,14 +39,21 @@ static_assert(sizeof(Piece) == 64, "queue entry");
 
 // The pieces of a CTA go from the warp that works them out to the others through a queue in shared memory, so the others
 // neither carry the schedule's state nor wait for the lengths it reads.  An entry without tiles ends it.
+//
+// All warps take the same pieces, also when a wait of the CTA gives up: lanes shuffle and warps share named barriers, so one that
+// left while another found its piece would be waited for without end.  Therefore the scheduling warp alone ends the queue: where
+// its own wait gives up, or another has, it names the first piece that it has not entered, and an entry is not overwritten
+// before all have read it.  Its waits are bounded, and with them those for an entry.
 constexpr int kQueue = 4;
 struct PieceQueue {
   Piece* entry;      // [kQueue]
   uint64_t* full;    // [kQueue]: one arrival
   uint64_t* empty;   // [kQueue]: one per reading warp
+  volatile int* stop;   // pieces that there are, once that is decided before the end
   uint32_t i = 0;
-  __device__ __forceinline__ PieceQueue(Piece* entries, uint64_t* bars) : entry(entries), full(bars), empty(bars + kQueue) {}
+  __device__ __forceinline__ PieceQueue(Piece* entries, uint64_t* bars, int* stop_at) : entry(entries), full(bars), empty(bars + kQueue), stop(stop_at) {}
   __device__ __forceinline__ void init(int readers) {
+    *stop = INT_MAX;
     for (int k = 0; k < kQueue; ++k) {
       tc::mbar_init(&full[k], 1);
       tc::mbar_init(&empty[k], readers);
@@ -52,18 +61,27 @@ struct PieceQueue {
   }
   __device__ __forceinline__ bool put(const Piece& x, volatile int* abort_flag) {
     const uint32_t k = i % kQueue;
-    const bool ok = i < kQueue || kv16_wait(&empty[k], ((i / kQueue) - 1) & 1, abort_flag);
+    if (!__all_sync(0xffffffffu, *abort_flag == 0 && (i < kQueue || kv16_wait(&empty[k], ((i / kQueue) - 1) & 1, abort_flag)))) {
+      if ((threadIdx.x & 31) == 0) *stop = (int)i;
+      return false;
+    }
     if ((threadIdx.x & 31) == 0) {
       entry[k] = x;
       asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(tc::smem_u32(&full[k])) : "memory");
     }
     __syncwarp();
     ++i;
-    return ok;
+    return true;
   }
   __device__ __forceinline__ bool get(Piece* x, volatile int* abort_flag) {
     const uint32_t k = i % kQueue;
-    if (!kv16_wait(&full[k], (i / kQueue) & 1, abort_flag)) return false;
+    if (!tc::mbar_test_wait(&full[k], (i / kQueue) & 1)) {
+#pragma unroll 1
+      for (uint32_t n = 0; !tc::mbar_try_wait_hint(&full[k], (i / kQueue) & 1, 1000u); ++n) {
+        if (*stop <= (int)i || n == 16 * kWaitTries) return false;
+        if (n == kWaitTries) *abort_flag = 1;
+      }
+    }
     *x = entry[k];
     __syncwarp();
     if ((threadIdx.x & 31) == 0) asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(tc::smem_u32(&empty[k])) : "memory");
@@ -71,6 +89,18 @@ struct PieceQueue {
     return x->tiles > 0;
   }
 };
+
+// The scheduling warp: the pieces of `walk`, and the end.  never: a barrier that nothing arrives on.
+template <bool kHeld, class Walk>
+__device__ __forceinline__ void put_pieces(const Kv16Params& p, Walk& walk, PieceQueue& queue, uint64_t* never, volatile int* abort_flag) {
+  Piece it;
+  while (walk.next(p, &it)) {
+    if (kv16_held<kHeld>(p, kHeldSchedule, queue.i)) kv16_wait(never, 0, abort_flag);
+    if (!queue.put(it, abort_flag)) return;
+  }
+  it.tiles = 0;
+  queue.put(it, abort_flag);
+}
 
 struct ReqShape {
   int tokens, first, lo, hi, tiles, row_tiles;

@@ -84,14 +84,14 @@ struct Geo {
   static constexpr int wsum = wmax + 4 * RP * 4;     // float [4 warps][RP]
   static constexpr int pieces = wsum + 4 * RP * 4;   // PieceQueue's entries
   static constexpr int bars = pieces + kQueue * 64;
-  static constexpr int n_bars = 2 * units + 2 + 2 + 1 + 1 + 2 * kQueue;
-  static constexpr int misc = bars + n_bars * 8;     // ints: abort flag, TMEM address, arrival; scratch of find_run
+  static constexpr int n_bars = 2 * units + 2 + 2 + 1 + 1 + 2 * kQueue + 1;
+  static constexpr int misc = bars + n_bars * 8;     // ints: abort flag, TMEM address, arrival, stop; scratch of find_run
   static constexpr int total = misc + 160 + 1024;
   static_assert(kQueue * 64 + n_bars * 8 + 160 <= 768, "fixed part");
 };
 
 struct Bars {  // offsets behind [units] full, [units] empty
-  static constexpr int q_empty = 0, s_ready = 2, p_ready = 4, pv_done = 5, queue = 6;
+  static constexpr int q_empty = 0, s_ready = 2, p_ready = 4, pv_done = 5, queue = 6, drained = queue + 2 * kQueue;
 };
 
 // Length of a row tile in the sequence: its keys in grains, and what a piece costs besides.
@@ -348,7 +348,7 @@ __device__ __forceinline__ void merge_pieces(const Kv16Params& p, const Piece& i
   }
 }
 
-template <int HD, int RP, bool kHalf>
+template <int HD, int RP, bool kHalf, bool kHeld>
 __global__ void __launch_bounds__(kThreads, (Geo<HD, RP>::ctas)) kv16_short_kernel(const __grid_constant__ Kv16Params p) {
   using G = Geo<HD, RP>;
   extern __shared__ uint8_t smem_raw[];
@@ -359,6 +359,7 @@ __global__ void __launch_bounds__(kThreads, (Geo<HD, RP>::ctas)) kv16_short_kern
   volatile int* const abort_flag = reinterpret_cast<volatile int*>(smem + G::misc);
   uint32_t* const tslot = reinterpret_cast<uint32_t*>(smem + G::misc + 4);
   int* const arrival = reinterpret_cast<int*>(smem + G::misc + 8);
+  int* const stop = arrival + 1;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
 
   if (warp == kMmaWarp) {
@@ -373,7 +374,8 @@ __global__ void __launch_bounds__(kThreads, (Geo<HD, RP>::ctas)) kv16_short_kern
       }
       tc::mbar_init(&bars[Bars::p_ready], kSoftmaxThreads);
       tc::mbar_init(&bars[Bars::pv_done], 1);
-      PieceQueue(nullptr, &bars[Bars::queue]).init(kThreads / 32 - 1);
+      tc::mbar_init(&bars[Bars::drained], 1);
+      PieceQueue(nullptr, &bars[Bars::queue], stop).init(kThreads / 32 - 1);
       *abort_flag = 0;
       tc::mbar_init_fence();
     }
@@ -387,15 +389,12 @@ __global__ void __launch_bounds__(kThreads, (Geo<HD, RP>::ctas)) kv16_short_kern
   __syncthreads();
   tc::fence_after_sync();
   const uint32_t tmem_base = *tslot;
-  PieceQueue queue(reinterpret_cast<Piece*>(smem + G::pieces), &bars[Bars::queue]);
+  PieceQueue queue(reinterpret_cast<Piece*>(smem + G::pieces), &bars[Bars::queue], stop);
   bool ok = true;
 
   if (warp == kScheduleWarp) {
     // =========================== schedule ========================================
-    Piece it;
-    while (walk.next(p, &it)) ok &= queue.put(it, abort_flag);
-    it.tiles = 0;
-    ok &= queue.put(it, abort_flag);
+    put_pieces<kHeld>(p, walk, queue, &bars[Bars::drained], abort_flag);
   } else if (warp >= kLoadWarp && warp < kMmaWarp) {
     // =========================== copies ==========================================
     // A warp owns 32 keys of every tile: lane l knows where key l of them lies.
@@ -415,6 +414,7 @@ __global__ void __launch_bounds__(kThreads, (Geo<HD, RP>::ctas)) kv16_short_kern
       long long off_v = 0;
       int64_t head_v = 0;
       while (have || have_v) {
+        if (warp == kLoadWarp && kv16_held<kHeld>(p, kHeldCopies, unit)) break;
         const bool now = have;
         long long off = 0;
         int64_t head_k = 0;
@@ -522,6 +522,7 @@ __global__ void __launch_bounds__(kThreads, (Geo<HD, RP>::ctas)) kv16_short_kern
     bool pending = false, pending_first = false;
     while (queue.get(&it, abort_flag)) {
       for (int t = 0; t < it.tiles; ++t) {
+        if (kv16_held<kHeld>(p, kHeldMma, tile)) break;
         qk(t == it.tiles - 1);
         if (pending) pv(pending_first);
         pending = true;
@@ -699,12 +700,21 @@ __global__ void __launch_bounds__(kThreads, (Geo<HD, RP>::ctas)) kv16_short_kern
   }
   tc::fence_before_sync();
   __syncthreads();
-  if (warp == kMmaWarp) tc::tmem_dealloc(tmem_base, G::tmem);
-  if (tid == 0 && *abort_flag) atomicOr(&g_kv16_status, 8u);
+  if (warp == kMmaWarp) {
+    if (*abort_flag) {   // (copies have landed, MMAs may be in flight)
+      if (elect_one()) {
+        tc::mma_commit(&bars[Bars::drained]);
+        kv16_drain(&bars[Bars::drained], 0);
+        atomicOr(&g_kv16_status, 8u);
+      }
+      __syncwarp();
+    }
+    tc::tmem_dealloc(tmem_base, G::tmem);
+  }
   (void)ok;
 }
 
-template <int HD, int RP, bool kHalf>
+template <int HD, int RP, bool kHalf, bool kHeld = false>
 cudaError_t launch_one(const Kv16Params& p, cudaStream_t stream) {
   using G = Geo<HD, RP>;
   static_assert(G::total <= 232448, "shared memory of one CTA");
@@ -714,13 +724,13 @@ cudaError_t launch_one(const Kv16Params& p, cudaStream_t stream) {
   cudaError_t err = cudaGetDevice(&dev);
   if (err != cudaSuccess) return err;
   if (dev < 0 || dev >= 64 || !configured[dev]) {
-    err = cudaFuncSetAttribute(kv16_short_kernel<HD, RP, kHalf>, cudaFuncAttributeMaxDynamicSharedMemorySize, G::total);
+    err = cudaFuncSetAttribute(kv16_short_kernel<HD, RP, kHalf, kHeld>, cudaFuncAttributeMaxDynamicSharedMemorySize, G::total);
     if (err != cudaSuccess) return err;
     if (dev >= 0 && dev < 64) configured[dev] = true;
   }
   const int sms = sm_count();
   if (sms <= 0) return cudaErrorInvalidDevice;
-  return pdl_launch(kv16_short_kernel<HD, RP, kHalf>, dim3((unsigned)(sms * G::ctas)), dim3(kThreads), G::total, stream, p);
+  return pdl_launch(kv16_short_kernel<HD, RP, kHalf, kHeld>, dim3((unsigned)(sms * G::ctas)), dim3(kThreads), G::total, stream, p);
 }
 template <int HD, int RP>
 cudaError_t launch_type(const Kv16Params& p, cudaStream_t stream) {
@@ -751,6 +761,8 @@ cudaError_t launch_kv16_short(const Kv16Params& p, cudaStream_t stream) {
       return launch_rows<256>(p, stream);
   }
 }
+
+cudaError_t launch_kv16_short_held(const Kv16Params& p, cudaStream_t stream) { return launch_one<128, 8, false, true>(p, stream); }
 
 // Reads and clears this kernel's status word (device must be idle).
 cudaError_t read_kv16_status(unsigned int* v) {

@@ -93,7 +93,7 @@ struct Tall {
   static constexpr int most_ctas = kTallSms * ctas;
   static constexpr int q = units * unit;
   static constexpr int bars = q + rts * qtile;
-  static constexpr int n_bars = 2 * units + 2 * rts + 20 + 2 * kQueue;
+  static constexpr int n_bars = 2 * units + 2 * rts + 20 + 2 * kQueue + rts;
   static constexpr int pieces = bars + n_bars * 8;   // PieceQueue's entries
   static constexpr int misc = pieces + kQueue * 64;
   static constexpr int bounds = misc + 32;           // the plan's, and its scratch in front
@@ -109,6 +109,7 @@ struct TallBars {  // behind [units] full, [units] empty
   static constexpr int pv_half = p_ready + 8;        // [4] PV of the first of two halves
   static constexpr int pv_done = pv_half + 4;        // [4]
   static constexpr int queue = pv_done + 4;
+  static constexpr int drained = queue + 2 * kQueue; // [rts]
 };
 
 // Tiled TMA load of one box of a rank-4 tensor map into shared memory.
@@ -388,7 +389,7 @@ __device__ __forceinline__ TallWalk<RP> make_plan(const Kv16Params& p, uint8_t* 
   return w;
 }
 
-template <int HD, bool kHalf>
+template <int HD, bool kHalf, bool kHeld>
 __global__ void __launch_bounds__(Tall<HD>::threads, Tall<HD>::ctas) kv16_tall_kernel(const __grid_constant__ Kv16Params p, const __grid_constant__ CUtensorMap k_map,
                                                                         const __grid_constant__ CUtensorMap v_map) {
   using G = Tall<HD>;
@@ -401,7 +402,8 @@ __global__ void __launch_bounds__(Tall<HD>::threads, Tall<HD>::ctas) kv16_tall_k
   uint64_t* const bars = empty + G::units;
   volatile int* const abort_flag = reinterpret_cast<volatile int*>(smem + G::misc);
   uint32_t* const tslot = reinterpret_cast<uint32_t*>(smem + G::misc + 4);
-  int* const arrival = reinterpret_cast<int*>(smem + G::misc + 8);
+  int* const arrival = reinterpret_cast<int*>(smem + G::misc + 8);   // [2]
+  int* const stop = arrival + 2;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
 
   if (warp == G::mma_warp) {
@@ -413,6 +415,7 @@ __global__ void __launch_bounds__(Tall<HD>::threads, Tall<HD>::ctas) kv16_tall_k
       for (int i = 0; i < G::rts; ++i) {
         tc::mbar_init(&bars[B::q_full + i], 32 * kLoadWarps);
         tc::mbar_init(&bars[B::q_empty + i], 1);
+        tc::mbar_init(&bars[B::drained + i], 1);
       }
       for (int i = 0; i < 4; ++i) {
         tc::mbar_init(&bars[B::s_ready + i], 1);
@@ -421,7 +424,7 @@ __global__ void __launch_bounds__(Tall<HD>::threads, Tall<HD>::ctas) kv16_tall_k
         tc::mbar_init(&bars[B::pv_half + i], 1);
         tc::mbar_init(&bars[B::pv_done + i], 1);
       }
-      PieceQueue(nullptr, &bars[B::queue]).init(G::threads / 32 - 1);
+      PieceQueue(nullptr, &bars[B::queue], stop).init(G::threads / 32 - 1);
       *abort_flag = 0;
       tc::mbar_init_fence();
     }
@@ -436,16 +439,14 @@ __global__ void __launch_bounds__(Tall<HD>::threads, Tall<HD>::ctas) kv16_tall_k
   __syncthreads();
   tc::fence_after_sync();
   const uint32_t tmem_base = *tslot;
-  PieceQueue queue(reinterpret_cast<Piece*>(smem + G::pieces), &bars[B::queue]);
+  PieceQueue queue(reinterpret_cast<Piece*>(smem + G::pieces), &bars[B::queue], stop);
   bool ok = true;
+  int issued = 0;   // units that this thread has had a part in (copying warps)
 
   if (warp == G::schedule_warp) {
     // =========================== schedule ========================================
     TallWalk<RP> w = plan;
-    Piece it;
-    while (w.next(p, &it)) ok &= queue.put(it, abort_flag);
-    it.tiles = 0;
-    ok &= queue.put(it, abort_flag);
+    put_pieces<kHeld>(p, w, queue, &bars[B::drained], abort_flag);
   } else if (warp >= G::load_warp && warp < G::mma_warp) {
     // =========================== copies ==========================================
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(G::copy_regs));
@@ -460,11 +461,16 @@ __global__ void __launch_bounds__(Tall<HD>::threads, Tall<HD>::ctas) kv16_tall_k
     const int boxes = p.box_slots > 0 ? 32 / p.box_slots : 0;   // of this warp's keys
     const int box_lane = boxes > 0 ? (lane % boxes) * p.box_slots : 0;
     const bool boxing = lane < boxes * (G::dims / 64);
+    // (Behind a wait that gave up nothing more is copied: a unit that is not free may be waiting for its boxes.)
     auto load_unit = [&](const CUtensorMap& map, const uint8_t* src, int part, int kvh, bool as_boxes, long long off, int blk, int slot) {
       const uint32_t s = unit % G::units;
-      if (unit >= G::units) ok &= kv16_wait(&empty[s], ((unit / G::units) - 1) & 1, abort_flag);
+      if (unit >= G::units && !kv16_wait(&empty[s], ((unit / G::units) - 1) & 1, abort_flag)) {
+        if (ok) issued = (int)unit;
+        ok = false;
+      }
       if (as_boxes) {
-        if (boxing) {
+        if (!ok) {
+        } else if (boxing) {
           const int slab = lane / boxes;
           mbar_arrive_expect_tx(&full[s], p.box_slots * 128);
           tma_load_4d(ring + s * G::unit + slab * (kTile * 128) + (base_key + box_lane) * 128, &map, part * 128 + slab * 64, kvh, slot, blk, &full[s]);
@@ -474,7 +480,7 @@ __global__ void __launch_bounds__(Tall<HD>::threads, Tall<HD>::ctas) kv16_tall_k
         __syncwarp();
       } else {
         copy_keys<G::dims>(ring + s * G::unit, base_key, src + part * 256, off);
-        copies_arrive(&full[s]);
+        if (ok) copies_arrive(&full[s]);
       }
       ++unit;
     };
@@ -482,6 +488,7 @@ __global__ void __launch_bounds__(Tall<HD>::threads, Tall<HD>::ctas) kv16_tall_k
       KeyLookup keys(p, queue, abort_flag, base_key + lane);
       bool have = keys.fetch();
       while (have) {
+        if (warp == G::load_warp && kv16_held<kHeld>(p, kHeldCopies, unit)) break;
         const int kvh = keys.it.kvh;
         const uint8_t* kb = p.k + (int64_t)kvh * p.stride_head;
         const uint8_t* vb = p.v + (int64_t)kvh * p.stride_head;
@@ -497,7 +504,7 @@ __global__ void __launch_bounds__(Tall<HD>::threads, Tall<HD>::ctas) kv16_tall_k
 #pragma unroll
           for (int rt = 0; rt < G::rts; ++rt) {
             if (rows <= rt * 128) continue;
-            if (q_count[rt] > 0) ok &= kv16_wait(&bars[B::q_empty + rt], (q_count[rt] - 1) & 1, abort_flag);
+            if (q_count[rt] > 0) kv16_wait(&bars[B::q_empty + rt], (q_count[rt] - 1) & 1, abort_flag);
             ++q_count[rt];
             // a lane looks a row up, the warp copies it
             const int mine = rt * 128 + base_key + lane;
@@ -515,6 +522,7 @@ __global__ void __launch_bounds__(Tall<HD>::threads, Tall<HD>::ctas) kv16_tall_k
       }
     }
     copies_wait_all();
+    if (ok) issued = (int)unit;
   } else if (warp >= G::mma_warp) {
     // =========================== MMAs ============================================
     const int rt = warp - G::mma_warp;
@@ -572,7 +580,7 @@ __global__ void __launch_bounds__(Tall<HD>::threads, Tall<HD>::ctas) kv16_tall_k
             if (part == 0 && kk == 0) mma_ss_words<false>(s_tmem + b * G::keys, qlo + at, (uint32_t)(q_desc >> 32), klo + at, (uint32_t)(k_desc >> 32), qk_desc);
             else mma_ss_words<true>(s_tmem + b * G::keys, qlo + at, (uint32_t)(q_desc >> 32), klo + at, (uint32_t)(k_desc >> 32), qk_desc);
           }
-          if (tile_ends) tc::mma_commit(&empty[k_slot[part]]);
+          if (tile_ends && ok) tc::mma_commit(&empty[k_slot[part]]);   // (a unit that has not landed is not given back)
         }
         tc::mma_commit(&bars[B::s_ready + 2 * rt + b]);
         if (last) tc::mma_commit(&bars[B::q_empty + rt]);
@@ -595,7 +603,7 @@ __global__ void __launch_bounds__(Tall<HD>::threads, Tall<HD>::ctas) kv16_tall_k
             for (int kk = 0; kk < 4; ++kk)
               mma_ts_words(o_tmem + part * 128, s_tmem + b * G::keys + half * 32 + kk * 8, vlo + kk * (2048 >> 4), (uint32_t)(v_desc >> 32), pv_desc,
                            !first || half > 0 || kk > 0);
-            if (tile_ends && half == G::halves - 1) tc::mma_commit(&empty[v_slot[part]]);
+            if (tile_ends && half == G::halves - 1 && ok) tc::mma_commit(&empty[v_slot[part]]);
           }
           tc::mma_commit(&bars[(half == G::halves - 1 ? B::pv_done : B::pv_half) + 2 * rt + b]);
         }
@@ -606,12 +614,13 @@ __global__ void __launch_bounds__(Tall<HD>::threads, Tall<HD>::ctas) kv16_tall_k
     Piece it;
     const bool leader = elect_one();   // (one lane takes all steps of a piece: the others would only have to be waited for)
     while (queue.get(&it, abort_flag)) {
-      if (!leader) continue;
+      if (!leader || !ok) continue;
       if (it.rows <= rt * 128) {   // no rows: free the units as if they had been read
 #pragma unroll 1
         for (int i = 0; i < it.tiles; ++i) {
           landed(k_slot, k_phase, false);
           landed(v_slot, v_phase, false);
+          if (!ok) break;
 #pragma unroll
           for (int part = 0; part < G::parts; ++part) {
             mbar_arrive(&empty[k_slot[part]]);
@@ -631,6 +640,8 @@ __global__ void __launch_bounds__(Tall<HD>::threads, Tall<HD>::ctas) kv16_tall_k
       // QK of a step ahead of PV of the one before: the softmax finds the next S when it is done with one
 #pragma unroll 1
       for (int j = 0; j <= n; ++j) {
+        if (kv16_held<kHeld>(p, kHeldMma, s_qk)) ok = false;
+        if (!ok) break;
         if (j < n) qk(j % G::steps, tile_copied(j), j % G::steps == G::steps - 1 || j == n - 1, j == 0, j == n - 1);
         if (j > 0) pv((j - 1) % G::steps, tile_copied(j - 1), (j - 1) % G::steps == G::steps - 1 || j == n, j == 1);
       }
@@ -848,9 +859,27 @@ __global__ void __launch_bounds__(Tall<HD>::threads, Tall<HD>::ctas) kv16_tall_k
   }
   tc::fence_before_sync();
   __syncthreads();
+  if (*abort_flag) {   // (the same in all threads) what is in flight comes to its end first: MMAs, and boxes
+    if (warp >= G::mma_warp && warp < G::schedule_warp && elect_one()) {
+      uint64_t* const drained = &bars[B::drained + warp - G::mma_warp];
+      tc::mma_commit(drained);
+      kv16_drain(drained, 0);
+    }
+    // (the copying threads stopped at units of their own: who has stopped short of another arrives without a copy, so that
+    // the units' last phases end with what has been asked for)
+    int* const most = arrival;
+    if (tid == 0) *most = 0;
+    __syncthreads();
+    atomicMax(most, issued);
+    __syncthreads();
+    if (warp >= G::load_warp && warp < G::mma_warp) {
+      for (; issued < *most; ++issued) mbar_arrive(&full[issued % G::units]);
+      for (int u = max(0, issued - G::units); u < issued; ++u) kv16_drain(&full[u % G::units], (u / G::units) & 1);
+    }
+    if (tid == 0) atomicOr(&g_kv16_tall_status, 16u);
+    __syncthreads();
+  }
   if (warp == G::mma_warp) tc::tmem_dealloc(tmem_base, G::tmem);
-  if (tid == 0 && *abort_flag) atomicOr(&g_kv16_tall_status, 16u);
-  (void)ok;
 }
 
 // Tensor map over one of the caches, [dims][heads][slots][blocks], a box being 64 dims of box_slots slots of one head, in the
@@ -865,7 +894,7 @@ bool page_box_map(const Kv16Params& p, const uint8_t* base, CUtensorMap* map) {
                              CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
-template <int HD, bool kHalf>
+template <int HD, bool kHalf, bool kHeld = false>
 cudaError_t launch_one(const Kv16Params& p, cudaStream_t stream) {
   using G = Tall<HD>;
   static bool configured[64] = {};
@@ -873,7 +902,7 @@ cudaError_t launch_one(const Kv16Params& p, cudaStream_t stream) {
   cudaError_t err = cudaGetDevice(&dev);
   if (err != cudaSuccess) return err;
   if (dev < 0 || dev >= 64 || !configured[dev]) {
-    err = cudaFuncSetAttribute(kv16_tall_kernel<HD, kHalf>, cudaFuncAttributeMaxDynamicSharedMemorySize, G::total);
+    err = cudaFuncSetAttribute(kv16_tall_kernel<HD, kHalf, kHeld>, cudaFuncAttributeMaxDynamicSharedMemorySize, G::total);
     if (err != cudaSuccess) return err;
     if (dev >= 0 && dev < 64) configured[dev] = true;
   }
@@ -887,7 +916,7 @@ cudaError_t launch_one(const Kv16Params& p, cudaStream_t stream) {
     if (p.block_size % slots == 0) q.box_slots = slots;
   CUtensorMap k_map{}, v_map{};
   if (q.box_slots > 0 && !(page_box_map(q, p.k, &k_map) && page_box_map(q, p.v, &v_map))) q.box_slots = 0;
-  return pdl_launch(kv16_tall_kernel<HD, kHalf>, dim3((unsigned)(sms * G::ctas)), dim3(G::threads), G::total, stream, q, k_map, v_map);
+  return pdl_launch(kv16_tall_kernel<HD, kHalf, kHeld>, dim3((unsigned)(sms * G::ctas)), dim3(G::threads), G::total, stream, q, k_map, v_map);
 }
 template <int HD>
 cudaError_t launch_type(const Kv16Params& p, cudaStream_t stream) {
@@ -912,6 +941,8 @@ cudaError_t launch_kv16_tall(const Kv16Params& p, cudaStream_t stream) {
       return launch_type<256>(p, stream);
   }
 }
+
+cudaError_t launch_kv16_tall_held(const Kv16Params& p, cudaStream_t stream) { return launch_one<128, false, true>(p, stream); }
 
 // Reads and clears this kernel's status word (device must be idle).
 cudaError_t read_kv16_tall_status(unsigned int* v) {
