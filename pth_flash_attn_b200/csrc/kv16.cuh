@@ -49,7 +49,7 @@ __device__ __forceinline__ int kv16_tokens(const Kv16Params& p, int r, int* firs
     return 1;
   }
   *first = max(0, __ldg(p.query_start_loc + r));
-  const int end = min(__ldg(p.query_start_loc + r + 1), p.num_tokens);
+  const int end = min(max(0, __ldg(p.query_start_loc + r + 1)), p.num_tokens);   // (so that the difference stays in 32 bits)
   return max(0, min(end - *first, p.max_query_len));
 }
 __device__ __forceinline__ void kv16_visible(const Kv16Params& p, int r, int* lo, int* hi) {
