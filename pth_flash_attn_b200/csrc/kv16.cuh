@@ -66,13 +66,15 @@ __device__ __forceinline__ uint64_t swizzled_desc(uint32_t saddr, uint32_t lbo_b
   return tc::smem_desc(saddr, lbo_bytes, sbo_bytes) | (uint64_t)2 << 61;
 }
 // Bounded wait for a phase of an mbarrier; once any wait of the CTA has given up, all do.  A try sleeps for one microsecond, or for
-// four where all warps of a CTA wait, so the bound is 0.3 to 1.1 s.  (A test goes first: a try that may sleep takes 200 cycles where
+// four where all warps of a CTA wait, so the bound is 0.3 to 1.1 s, or as many times that as the caller says, who may wait for other
+// warps' whole pieces (20 million keys in one piece take 0.3 s).  (A test goes first: a try that may sleep takes 200 cycles where
 // the phase is complete already, a test 100, and a softmax step has little else to wait for.)
 constexpr uint32_t kWaitTries = 1u << 18;
+template <uint32_t kTimes = 1>
 __device__ __forceinline__ bool kv16_wait(uint64_t* bar, uint32_t parity, volatile int* abort_flag) {
   if (tc::mbar_test_wait(bar, parity)) return true;
 #pragma unroll 1
-  for (uint32_t i = 0; i < kWaitTries; ++i) {
+  for (uint32_t i = 0; i < kTimes * kWaitTries; ++i) {
     if (tc::mbar_try_wait_hint(bar, parity, 1000u)) return true;
     if (*abort_flag) return false;
   }

@@ -45,6 +45,7 @@ static_assert(sizeof(Piece) == 64, "queue entry");
 // its own wait gives up, or another has, it names the first piece that it has not entered, and an entry is not overwritten
 // before all have read it.  Its waits are bounded, and with them those for an entry.
 constexpr int kQueue = 4;
+constexpr uint32_t kPieceTimes = 16;   // (of the bound on other waits)
 struct PieceQueue {
   Piece* entry;      // [kQueue]
   uint64_t* full;    // [kQueue]: one arrival
@@ -61,7 +62,7 @@ struct PieceQueue {
   }
   __device__ __forceinline__ bool put(const Piece& x, volatile int* abort_flag) {
     const uint32_t k = i % kQueue;
-    if (!__all_sync(0xffffffffu, *abort_flag == 0 && (i < kQueue || kv16_wait(&empty[k], ((i / kQueue) - 1) & 1, abort_flag)))) {
+    if (!__all_sync(0xffffffffu, *abort_flag == 0 && (i < kQueue || kv16_wait<kPieceTimes>(&empty[k], ((i / kQueue) - 1) & 1, abort_flag)))) {
       if ((threadIdx.x & 31) == 0) *stop = (int)i;
       return false;
     }
@@ -78,8 +79,8 @@ struct PieceQueue {
     if (!tc::mbar_test_wait(&full[k], (i / kQueue) & 1)) {
 #pragma unroll 1
       for (uint32_t n = 0; !tc::mbar_try_wait_hint(&full[k], (i / kQueue) & 1, 1000u); ++n) {
-        if (*stop <= (int)i || n == 16 * kWaitTries) return false;
-        if (n == kWaitTries) *abort_flag = 1;
+        if (*stop <= (int)i || n == 2 * kPieceTimes * kWaitTries) return false;
+        if (n == kPieceTimes * kWaitTries) *abort_flag = 1;
       }
     }
     *x = entry[k];
