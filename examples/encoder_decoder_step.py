@@ -47,7 +47,8 @@ class PagedCache:
                         self.positions[:n], self.taken, PAGE)
         ops.kv16_write(key, value, self.k, self.v, self.slots[:n])
         self.lens.copy_(self.seq_lens)
-        # (the pages that were taken leave the front of the list; its length stays what the captured call has)
+        # (the pages that were taken leave the front of the list; its length stays what the captured call has, and the pool has
+        # pages for every request's longest, so none of them comes round to the front again)
         at = (torch.arange(len(self.free), device=key.device) + self.taken) % len(self.free)
         self.free.copy_(self.free[at])
 

@@ -360,6 +360,13 @@ int32_t pthb200_kv16_write(const PthB200Kv16WriteArgs* args, void* stream);
  * block id outside [0, num_blocks) stands for keys and values of zero; what lies in slots that no request
  * sees has no influence.
  *
+ * Scores, their statistics and all sums have 32 bits (scaled scores up to 10^7, past which 32-bit scores are off by 1
+ * themselves).  Values may be of any size, infinities included: as in the formula, one infinite value makes its part of
+ * the output infinite, two of both signs make it NaN.  Calls whose requests have up to 16 rows (max_query_len x heads per KV
+ * head; any number of heads with one token) keep probabilities in two 16-bit parts, so that the output's error is its own
+ * rounding.  Others round them to dtype (1.4 times that error), and a probability below 2^-31 (F16) or 2^-102 (BF16) of its row's
+ * largest may be zero: an infinite value under it makes NaN.
+ *
  * workspace: pthb200_kv16_workspace_bytes of it, 256-byte aligned, zeroed ONCE before its first use; a
  * call leaves it ready for the next one.  Calls that may overlap need workspaces of their own.  (Zero it again
  * after pthb200_device_status has reported a wait that gave up.) */

@@ -20,10 +20,10 @@
 // TMA, boxes of 16 slots x 64 dims, 64 requests x 8,192 keys x 8 heads x 128 dims) moved 6.83 TB/s, with boxes of 4 KB 7.06, 16-byte
 // copies 7.17, which also take pages of any size and place.
 //
-// Measured, bf16, one call behind another: 64 requests x 8,192 keys, 32 heads of 8, 128 dims 320 us, 6.7 TB/s; 61 x 4,096-12,288, 12 of
-// 2, 256 dims 163 us, 6.5 TB/s; one request of 131,072 keys 95 us, 5.6 TB/s, of which the last arriver's merge of 37 pieces and
-// the start are 13; 8 requests of up to 4,095 keys 22.7 us for 79 MB, some 5 in front of the first tile (the launch, the
-// lengths, the block table, the first keys: one after the other) and 6 behind the last (the merge).
+// Measured, bf16, one call behind another: 64 requests x 8,192 keys, 32 heads of 8, 128 dims 321 us, 6.7 TB/s; 61 x 4,096-12,288, 12 of
+// 2, 256 dims 161 us, 6.5 TB/s; one request of 131,072 keys 91 us, 5.9 TB/s, of which the last arriver's merge of 37 pieces and
+// the start are 9; 8 requests of up to 4,095 keys 22.1 us for 79 MB, some 5 in front of the first tile (the launch, the
+// lengths, the block table, the first keys: one after the other) and 5 behind the last (the merge).
 //
 // Schedule: the keys of all (request, row tile) form one sequence, which is cut into equal runs, one for every group of Hkv CTAs;
 // CTA h of a group reads head h, so that the heads of a page are read at the same time.  The pieces of a row tile that a cut

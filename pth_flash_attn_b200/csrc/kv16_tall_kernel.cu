@@ -20,10 +20,11 @@
 // for P to go there, some 300 for the two barriers: 2,000 in all, beside 1,350 of MMAs (eight of QK over 64 keys take 400 instead
 // of 256: both operands come from shared memory).  Without the exponentials a launch takes 15 % less, with an eighth of QK's MMAs and a
 // quarter of PV's 8 %.
-// Measured, bf16, alone: 4 x 2,048 tokens over 8,192 states, 32 heads of 8, 128 dims 944 us, 1,165 TFLOP/s (1,095 us, 1,004 TFLOP/s one
-// behind another, at the board's power limit); 8 x 1,000 over 4,000 at 256 dims 1,487 us, 705; 64 x 16 over 4,000, one row tile
-// of two, 207 us, 5.2 TB/s; 16 x 4-448 over 64-1,500, 16 heads of 16, 64 dims 47 us, of which the start is 3, an item's first maximum
-// and rows' way out 3 each, the last merge 4.
+// Measured, bf16, behind a flush of L2: 4 x 2,048 tokens over 8,192 states, 32 heads of 8, 128 dims 950 us, 1,157 TFLOP/s (1,084 us, 1,014
+// TFLOP/s, in calls behind one another for seconds, at the board's power limit), in fp16 975 us; at 256 dims 2,840 us, 774, and 8 x
+// 1,000 over 4,000 1,477 us, 710; 16 heads of 16, 64 dims 510 us, 539.  64 x 16 over 4,000 at 128 dims, one row tile of two, 207 us,
+// 5.2 TB/s; 16 x 4-448 over 64-1,500, 16 heads of 16, 64 dims 47 us, of which the start is 3, an item's first maximum and rows' way
+// out 3 each, the last merge 4.
 // Taken back: steps of 128 keys with one S buffer, a row tile waiting for its MMAs, 1,241; an eighth of the exponentials as a
 // polynomial on the FMA pipe 981 against 977, a quarter 1,045; the row tiles' exponentials in turn, or half a step apart (983 against
 // 960); P rounded with integer instructions 1,007 against 958; MMAs predicated lane by lane in a warp that stays together 958 against 946.

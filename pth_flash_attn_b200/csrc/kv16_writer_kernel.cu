@@ -3,11 +3,13 @@
 // T Hkv D (source + 2) x 2.
 //
 // A thread moves 16 bytes of the cache, eight elements of a row, at a time and has the loads of kWriteBatch such
-// pieces in flight before it stores the first.  (With 1, 2 and 4, us: 4 x 2,048 tokens of 8 heads, 128 dims 21.5, 19.3, 19.4,
-// 4 times as many 64.5, 53.2, 53.2, 64 tokens 7.0, 7.1, 9.0: with 4 registers spill.)
+// pieces in flight before it stores the first.  (With 1, 2 and 4, bf16 to bf16 behind a flush of L2, us: 4 x 2,048 tokens of 8 heads,
+// 128 dims 21.5, 19.3, 19.4, 4 times as many 64.5, 53.2, 53.2, 64 tokens 7.0, 7.1, 9.0: with 4 registers spill.)
 //
-// Measured: 4 x 2,048 tokens, bf16, 13.5 us, 5.0 TB/s of the 67 MB that they are (of 6.56 measured by copies; the launch is
-// the rest); 64 tokens 5.9 us, the host's time for a call.
+// Measured behind a flush of L2, the same heads, 4 x 2,048 tokens and 4 times as many: bf16 sources 18.4 and 53.2 us (the latter 5.0
+// TB/s of what is read and written; copies move 6.56), fp32 24.5 and 69.6 (5.8 TB/s), fp16 to bf16, element by element, 22.5 and
+// 63.5.  One call behind another 4 x 2,048 tokens take 10.8, 15.4 and 13.3: L2 holds what the last one wrote.  64 tokens take
+// 2.0 to 2.5 us on the device and 5.7 for the host's call.
 #include "kv16.cuh"
 #include "pdl.cuh"
 

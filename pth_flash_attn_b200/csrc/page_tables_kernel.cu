@@ -5,13 +5,14 @@
 //
 // Every CTA sums the lengths of all requests up for itself (a thread takes a run of requests, then one scan over the
 // CTA) and keeps the two running sums in shared memory, so nothing is passed between CTAs and no second launch is
-// needed: 16 KB of lengths at the most requests a step sees, out of the L2 cache.  Tokens and new pages are then
+// needed: 8 bytes of lengths a request, 128 KB at the 16,384 that a call takes, out of the L2 cache.  Tokens and new pages are then
 // two flat lists that the CTAs deal out evenly however the lengths are spread; the request of an entry is found by
 // bisection.  A token's page is taken from the free list itself where it is new, so no CTA reads what
 // another writes.
 //
-// What bounds it is latency: the kernel runs 4.8 us for 64 requests of one token each, 6.6 for 4 x 2,048 tokens and 8.1 for 128
-// prompts of up to 2,500 tokens (3 MB written), and a call takes the host 6.2 us, so calls behind one another take 8.0 us each.
+// What bounds it is latency: alone and cold the kernel runs 4.8 us for 64 requests of one token each, 6.6 for 4 x 2,048 tokens and 8.1
+// for 128 prompts of up to 2,500 tokens (3 MB written); launches that wait in the stream behind one another take 2.5, 2.8 and
+// 4.2.  A call takes the host 6.2 us, so eager calls behind one another take 8.0 us each.
 #include "kv16.cuh"
 #include "pdl.cuh"
 

@@ -273,7 +273,9 @@ def kv16_cross_attention(out, lse, q, k_cache, v_cache, block_table, context_len
     ``context_lens[r]`` states of its encoder, which lie in pages of the cache.
 
     ``q``, ``out`` ``[T, Hq, D]``; ``max_query_len`` bounds the tokens of a request (1 for a decoding step); ``lse`` and
-    ``workspace`` as in :func:`kv16_decode_attention`.
+    ``workspace`` as in :func:`kv16_decode_attention`.  Where a request has more than one token and ``max_query_len`` times
+    ``Hq / Hkv`` is 17 or more, probabilities are rounded to the cache's type (1.4 times the error of the output's own rounding);
+    below, and in :func:`kv16_decode_attention`, they are kept in two such parts.
     """
     _op("kv16_cross_attention")(out, lse, q, k_cache, v_cache, block_table, context_lens, query_start_loc, max_query_len,
                                 softmax_scale, workspace)
