@@ -414,6 +414,175 @@ int32_t pthb200_test_kv16_held(const PthB200Kv16Args* args, int32_t role, int32_
 /* Validates as the calls above do, without launching (cross: query_start_loc is not NULL). */
 int32_t pthb200_kv16_check(const PthB200Kv16Args* args);
 
+/* ---- 8-bit paged cache with a scale per block of tokens and head; rotary positions -------
+ * k_cache / v_cache are [num_blocks, block_size, num_kv_heads, head_size] views of e4m3 numbers c (NaN as 0x7f or 0xff, no
+ * infinities), k_scale / v_scale fp32 [num_blocks, block_size / scale_tokens, num_kv_heads] (stride_block, stride_slot, which is
+ * that between blocks of tokens, and stride_head in bytes): an element is c * scale.  scale_tokens, the slots that share a
+ * scale, is a multiple of 16 that divides block_size.  Rows of c lie on 16-byte boundaries.  Block tables are those of the other
+ * caches.  The reference has no counterpart of these calls. */
+
+/* Writer: the keys and values of new tokens.  The i-th of the tokens query_start_loc[r] .. query_start_loc[r + 1) of request r
+ * has position p = seq_lens[r] - (number of them) + i, slot p % block_size of block block_table[r][p / block_size].  Of a block of
+ * tokens (the scale_tokens positions of a scale) that a call writes to, and a KV head:
+ *   need = the smallest power of two, 2^-126 to 2^120, with max |x| <= 448 need over the finite x that are written
+ *   its first position is written   scale' = need; what it held is void
+ *   else                            scale' = max(scale, need), and if that is larger, c' = round(c scale / scale') for the positions
+ *                                   in front of the written ones (a scale that is no positive finite number counts as zero)
+ *   new cells                       c = round(x / scale'), to nearest even; infinities and what is past 448 become +-448, NaN stays
+ * Positions behind the written ones are left as they are.  Tokens past max_query_len of a request, at negative positions, past the
+ * row of the table or in blocks outside [0, num_blocks) are skipped.  A block that two requests of a call write to gets
+ * either's values, or some of both. */
+typedef struct PthB200Kv8WriteArgs {
+  int32_t abi_version;  /* PTH_ATTN_ABI_VERSION */
+  int32_t struct_bytes; /* sizeof(PthB200Kv8WriteArgs) of the caller */
+  const void* key;      /* [num_tokens, num_kv_heads, head_size] of src_dtype, rows contiguous */
+  const void* value;
+  int64_t key_stride_token;
+  int64_t key_stride_head;
+  int64_t value_stride_token;
+  int64_t value_stride_head;
+  PthAttnStream k_cache; /* written through, like all four */
+  PthAttnStream v_cache;
+  PthAttnStream k_scale;
+  PthAttnStream v_scale;
+  const int32_t* block_table; /* [num_reqs, num_pages] */
+  int64_t block_table_row_stride;
+  const int32_t* seq_lens;        /* [num_reqs], the new tokens included */
+  const int32_t* query_start_loc; /* [num_reqs + 1] */
+  int32_t src_dtype; /* F32, F16 or BF16 */
+  int32_t num_blocks;
+  int32_t block_size;
+  int32_t scale_tokens;
+  int32_t num_kv_heads;
+  int32_t head_size; /* 64, 128 or 256 */
+  int32_t num_reqs;
+  int32_t num_tokens;
+  int32_t num_pages;
+  int32_t max_query_len;
+} PthB200Kv8WriteArgs;
+int32_t pthb200_kv8_write_args_bytes(void);
+int32_t pthb200_kv8_write(const PthB200Kv8WriteArgs* args, void* stream);
+
+/* Reader: row row_start_loc[r] + i of key / value becomes position first[r] + i of request r, c * scale rounded to dst_dtype; zero
+ * where there is no such cell.  Rows past max_rows of a request, and those that belong to none, are left as they are. */
+typedef struct PthB200Kv8ReadArgs {
+  int32_t abi_version;  /* PTH_ATTN_ABI_VERSION */
+  int32_t struct_bytes; /* sizeof(PthB200Kv8ReadArgs) of the caller */
+  void* key;            /* [num_rows, num_kv_heads, head_size] of dst_dtype, rows on 16-byte boundaries */
+  void* value;
+  int64_t key_stride_token;
+  int64_t key_stride_head;
+  int64_t value_stride_token;
+  int64_t value_stride_head;
+  PthAttnStream k_cache;
+  PthAttnStream v_cache;
+  PthAttnStream k_scale;
+  PthAttnStream v_scale;
+  const int32_t* block_table; /* [num_reqs, num_pages] */
+  int64_t block_table_row_stride;
+  const int32_t* first;         /* [num_reqs] */
+  const int32_t* row_start_loc; /* [num_reqs + 1] */
+  int32_t dst_dtype; /* F32, F16 or BF16 */
+  int32_t num_blocks;
+  int32_t block_size;
+  int32_t scale_tokens;
+  int32_t num_kv_heads;
+  int32_t head_size; /* 64, 128 or 256 */
+  int32_t num_reqs;
+  int32_t num_rows;
+  int32_t num_pages;
+  int32_t max_rows;
+} PthB200Kv8ReadArgs;
+int32_t pthb200_kv8_read_args_bytes(void);
+int32_t pthb200_kv8_read(const PthB200Kv8ReadArgs* args, void* stream);
+
+/* Attention over the 8-bit cache.  Token i of request r has position p = seq_lens[r] - q_len + i and sees the keys
+ * [max(0, p - window + 1), p] (from 0 on with a window of 0); without `causal` up to seq_lens[r] - 1.
+ *   pthb200_kv8_decode  one token per request, the newest of its cache (num_tokens == num_reqs, query_start_loc NULL, causal 1);
+ *   pthb200_kv8_attend  the tokens query_start_loc[r] .. query_start_loc[r + 1) of request r; tokens past max_query_len of it are
+ *                       not computed.
+ * A token that sees no key gets out = 0 and a log-sum-exp of -inf.  lse (optional) is the natural logarithm, dense
+ * [num_tokens, num_q_heads].  Keys past the row of the block table do not exist, and a block outside [0, num_blocks) stands for
+ * keys and values of zero.  Scales are positive finite numbers.  Statistics and sums have 32 bits; out is rounded once.
+ *
+ * workspace: pthb200_kv8_workspace_bytes of it, 256-byte aligned, zeroed ONCE before its first use; a call leaves it ready for the
+ * next one.  Calls that may overlap need workspaces of their own.  (Zero it again after pthb200_device_status has reported a
+ * wait that gave up.) */
+typedef struct PthB200Kv8Args {
+  int32_t abi_version;  /* PTH_ATTN_ABI_VERSION */
+  int32_t struct_bytes; /* sizeof(PthB200Kv8Args) of the caller */
+  const void* q;        /* [num_tokens, num_q_heads, head_size] */
+  int64_t q_stride_token;
+  int64_t q_stride_head;
+  void* out;
+  int64_t out_stride_token;
+  int64_t out_stride_head;
+  float* lse; /* [num_tokens, num_q_heads] or NULL */
+  PthAttnStream k_cache; /* k_cache and v_cache have the same strides, and so have the scales */
+  PthAttnStream v_cache;
+  PthAttnStream k_scale;
+  PthAttnStream v_scale;
+  const int32_t* block_table; /* [num_reqs, num_pages] */
+  int64_t block_table_row_stride;
+  const int32_t* seq_lens;        /* [num_reqs] */
+  const int32_t* query_start_loc; /* [num_reqs + 1]; NULL for decode */
+  void* workspace;
+  int64_t workspace_bytes;
+  int32_t dtype; /* of q and out: F16 or BF16 */
+  int32_t num_blocks;
+  int32_t block_size;
+  int32_t scale_tokens;
+  int32_t num_kv_heads;
+  int32_t num_q_heads; /* at most 64 per KV head */
+  int32_t head_size; /* 64, 128 or 256 */
+  int32_t num_reqs;
+  int32_t num_tokens;
+  int32_t num_pages;
+  int32_t max_query_len;
+  int32_t window;
+  int32_t causal;
+  float softmax_scale;
+} PthB200Kv8Args;
+int32_t pthb200_kv8_args_bytes(void);
+/* Workspace of any call of this head size on a device of num_sms SMs. */
+int64_t pthb200_kv8_workspace_bytes(int32_t head_size, int32_t num_sms);
+int32_t pthb200_kv8_decode(const PthB200Kv8Args* args, void* stream);
+int32_t pthb200_kv8_attend(const PthB200Kv8Args* args, void* stream);
+/* Validates as the calls above do, without launching (decode: query_start_loc is NULL). */
+int32_t pthb200_kv8_check(const PthB200Kv8Args* args);
+
+/* Rotary positions: of every head of token t, the first 2 num_frequencies dimensions turn, pair i by the angle
+ * a = positions[t] * frequencies[i] (in 64 bits):  (x, y) -> scale * (x cos a - y sin a, x sin a + y cos a).
+ * Pairs are (i, i + num_frequencies), or (2 i, 2 i + 1) if interleaved.  inverse: by -a, which is also the gradient.  Other
+ * dimensions are copied.  q_out / k_out may be q / k themselves, with the same strides, else they must not overlap them; a head count
+ * of 0 leaves a tensor out. */
+typedef struct PthB200RotaryArgs {
+  int32_t abi_version;  /* PTH_ATTN_ABI_VERSION */
+  int32_t struct_bytes; /* sizeof(PthB200RotaryArgs) of the caller */
+  const void* q;        /* [num_tokens, num_q_heads, head_size] of dtype, rows contiguous */
+  const void* k;        /* [num_tokens, num_k_heads, head_size] */
+  void* q_out;
+  void* k_out;
+  int64_t q_stride_token, q_stride_head;
+  int64_t k_stride_token, k_stride_head;
+  int64_t q_out_stride_token, q_out_stride_head;
+  int64_t k_out_stride_token, k_out_stride_head;
+  const int64_t* positions; /* [num_tokens] */
+  const void* frequencies;  /* [num_frequencies], radians per position */
+  int32_t frequencies_64;   /* double, else float */
+  int32_t dtype;            /* F32, F16 or BF16 */
+  int32_t num_tokens;
+  int32_t num_q_heads;
+  int32_t num_k_heads;
+  int32_t head_size;       /* up to 1024 */
+  int32_t num_frequencies; /* 1 .. head_size / 2 */
+  int32_t interleaved;
+  int32_t inverse;
+  float scale;
+} PthB200RotaryArgs;
+int32_t pthb200_rotary_args_bytes(void);
+int32_t pthb200_rotary(const PthB200RotaryArgs* args, void* stream);
+
 /* Host-only helpers of the op layer (no device access).
  * pthb200_tile_tokens: query tokens per row tile for a launch planned with `wm`
  * (1, 2 or 4), group size G and host bound max_query_len; returns -1 if wm is

@@ -21,8 +21,9 @@ OP_LIB = HERE / "_C.abi3.so"
 
 CUDA_SOURCES = ["launcher.cu", "scalar_kernel.cu", "combine_kernel.cu", "umma_kernel.cu", "umma_i8_kernel.cu",
                 "umma_rows_kernel.cu", "umma_rows256_kernel.cu", "umma_rows2_kernel.cu", "writer_kernel.cu", "copy_ceiling_kernel.cu",
-                "kv16_api.cu", "page_tables_kernel.cu", "kv16_writer_kernel.cu", "kv16_short_kernel.cu", "kv16_tall_kernel.cu"]
-OP_SOURCES = ["torch_op.cpp", "torch_kv16.cpp"]
+                "kv16_api.cu", "page_tables_kernel.cu", "kv16_writer_kernel.cu", "kv16_short_kernel.cu", "kv16_tall_kernel.cu",
+                "kv8_api.cu", "kv8_writer_kernel.cu", "kv8_reader_kernel.cu", "kv8_short_kernel.cu", "rotary_kernel.cu"]
+OP_SOURCES = ["torch_op.cpp", "torch_kv16.cpp", "torch_kv8.cpp"]
 NVCC_FLAGS = [
     "-std=c++17", "-O3", "-lineinfo", "-gencode", "arch=compute_100a,code=sm_100a",
     "-Xcompiler", "-fPIC", "-Xcompiler", "-fno-gnu-unique", "-rdc=false",
@@ -63,7 +64,7 @@ def build_op_library(force: bool = False) -> Path:
     from torch.utils import cpp_extension
 
     sources = [CSRC / s for s in OP_SOURCES]
-    if not force and _newer(OP_LIB, [*sources, LIB]):
+    if not force and _newer(OP_LIB, [*sources, *CSRC.glob("*.h"), LIB]):
         return OP_LIB
     includes = [f"-I{p}" for p in cpp_extension.include_paths()]
     cuda_inc = Path(os.environ.get("CUDA_HOME", "/usr/local/cuda")) / "include"

@@ -205,6 +205,137 @@ class PthB200Kv16Args(ctypes.Structure):
     ]
 
 
+class PthB200Kv8WriteArgs(ctypes.Structure):
+    _fields_ = [
+        ("abi_version", ctypes.c_int32),
+        ("struct_bytes", ctypes.c_int32),
+        ("key", ctypes.c_void_p),
+        ("value", ctypes.c_void_p),
+        ("key_stride_token", ctypes.c_int64),
+        ("key_stride_head", ctypes.c_int64),
+        ("value_stride_token", ctypes.c_int64),
+        ("value_stride_head", ctypes.c_int64),
+        ("k_cache", PthAttnStream),
+        ("v_cache", PthAttnStream),
+        ("k_scale", PthAttnStream),
+        ("v_scale", PthAttnStream),
+        ("block_table", ctypes.c_void_p),
+        ("block_table_row_stride", ctypes.c_int64),
+        ("seq_lens", ctypes.c_void_p),
+        ("query_start_loc", ctypes.c_void_p),
+        ("src_dtype", ctypes.c_int32),
+        ("num_blocks", ctypes.c_int32),
+        ("block_size", ctypes.c_int32),
+        ("scale_tokens", ctypes.c_int32),
+        ("num_kv_heads", ctypes.c_int32),
+        ("head_size", ctypes.c_int32),
+        ("num_reqs", ctypes.c_int32),
+        ("num_tokens", ctypes.c_int32),
+        ("num_pages", ctypes.c_int32),
+        ("max_query_len", ctypes.c_int32),
+    ]
+
+
+class PthB200Kv8ReadArgs(ctypes.Structure):
+    _fields_ = [
+        ("abi_version", ctypes.c_int32),
+        ("struct_bytes", ctypes.c_int32),
+        ("key", ctypes.c_void_p),
+        ("value", ctypes.c_void_p),
+        ("key_stride_token", ctypes.c_int64),
+        ("key_stride_head", ctypes.c_int64),
+        ("value_stride_token", ctypes.c_int64),
+        ("value_stride_head", ctypes.c_int64),
+        ("k_cache", PthAttnStream),
+        ("v_cache", PthAttnStream),
+        ("k_scale", PthAttnStream),
+        ("v_scale", PthAttnStream),
+        ("block_table", ctypes.c_void_p),
+        ("block_table_row_stride", ctypes.c_int64),
+        ("first", ctypes.c_void_p),
+        ("row_start_loc", ctypes.c_void_p),
+        ("dst_dtype", ctypes.c_int32),
+        ("num_blocks", ctypes.c_int32),
+        ("block_size", ctypes.c_int32),
+        ("scale_tokens", ctypes.c_int32),
+        ("num_kv_heads", ctypes.c_int32),
+        ("head_size", ctypes.c_int32),
+        ("num_reqs", ctypes.c_int32),
+        ("num_rows", ctypes.c_int32),
+        ("num_pages", ctypes.c_int32),
+        ("max_rows", ctypes.c_int32),
+    ]
+
+
+class PthB200Kv8Args(ctypes.Structure):
+    _fields_ = [
+        ("abi_version", ctypes.c_int32),
+        ("struct_bytes", ctypes.c_int32),
+        ("q", ctypes.c_void_p),
+        ("q_stride_token", ctypes.c_int64),
+        ("q_stride_head", ctypes.c_int64),
+        ("out", ctypes.c_void_p),
+        ("out_stride_token", ctypes.c_int64),
+        ("out_stride_head", ctypes.c_int64),
+        ("lse", ctypes.c_void_p),
+        ("k_cache", PthAttnStream),
+        ("v_cache", PthAttnStream),
+        ("k_scale", PthAttnStream),
+        ("v_scale", PthAttnStream),
+        ("block_table", ctypes.c_void_p),
+        ("block_table_row_stride", ctypes.c_int64),
+        ("seq_lens", ctypes.c_void_p),
+        ("query_start_loc", ctypes.c_void_p),
+        ("workspace", ctypes.c_void_p),
+        ("workspace_bytes", ctypes.c_int64),
+        ("dtype", ctypes.c_int32),
+        ("num_blocks", ctypes.c_int32),
+        ("block_size", ctypes.c_int32),
+        ("scale_tokens", ctypes.c_int32),
+        ("num_kv_heads", ctypes.c_int32),
+        ("num_q_heads", ctypes.c_int32),
+        ("head_size", ctypes.c_int32),
+        ("num_reqs", ctypes.c_int32),
+        ("num_tokens", ctypes.c_int32),
+        ("num_pages", ctypes.c_int32),
+        ("max_query_len", ctypes.c_int32),
+        ("window", ctypes.c_int32),
+        ("causal", ctypes.c_int32),
+        ("softmax_scale", ctypes.c_float),
+    ]
+
+
+class PthB200RotaryArgs(ctypes.Structure):
+    _fields_ = [
+        ("abi_version", ctypes.c_int32),
+        ("struct_bytes", ctypes.c_int32),
+        ("q", ctypes.c_void_p),
+        ("k", ctypes.c_void_p),
+        ("q_out", ctypes.c_void_p),
+        ("k_out", ctypes.c_void_p),
+        ("q_stride_token", ctypes.c_int64),
+        ("q_stride_head", ctypes.c_int64),
+        ("k_stride_token", ctypes.c_int64),
+        ("k_stride_head", ctypes.c_int64),
+        ("q_out_stride_token", ctypes.c_int64),
+        ("q_out_stride_head", ctypes.c_int64),
+        ("k_out_stride_token", ctypes.c_int64),
+        ("k_out_stride_head", ctypes.c_int64),
+        ("positions", ctypes.c_void_p),
+        ("frequencies", ctypes.c_void_p),
+        ("frequencies_64", ctypes.c_int32),
+        ("dtype", ctypes.c_int32),
+        ("num_tokens", ctypes.c_int32),
+        ("num_q_heads", ctypes.c_int32),
+        ("num_k_heads", ctypes.c_int32),
+        ("head_size", ctypes.c_int32),
+        ("num_frequencies", ctypes.c_int32),
+        ("interleaved", ctypes.c_int32),
+        ("inverse", ctypes.c_int32),
+        ("scale", ctypes.c_float),
+    ]
+
+
 class PthB200Options(ctypes.Structure):
     _fields_ = [
         ("abi_version", ctypes.c_int32),
@@ -243,6 +374,17 @@ EXPORTED_SYMBOLS = (
     "pthb200_kv16_cross",
     "pthb200_kv16_check",
     "pthb200_test_kv16_held",
+    "pthb200_kv8_write_args_bytes",
+    "pthb200_kv8_write",
+    "pthb200_kv8_read_args_bytes",
+    "pthb200_kv8_read",
+    "pthb200_kv8_args_bytes",
+    "pthb200_kv8_workspace_bytes",
+    "pthb200_kv8_decode",
+    "pthb200_kv8_attend",
+    "pthb200_kv8_check",
+    "pthb200_rotary_args_bytes",
+    "pthb200_rotary",
     "pthb200_tile_tokens",
     "pthb200_check_call",
     "pthb200_launch_count",
@@ -305,19 +447,26 @@ class B200Lib:
         lib.pthb200_write_args_bytes.argtypes = []
         lib.pthb200_write_kv.restype = ctypes.c_int32
         lib.pthb200_write_kv.argtypes = [ctypes.POINTER(PthB200WriteArgs), ctypes.c_void_p]
-        for name in ("pthb200_tables_args_bytes", "pthb200_kv16_write_args_bytes", "pthb200_kv16_args_bytes"):
+        for name in ("pthb200_tables_args_bytes", "pthb200_kv16_write_args_bytes", "pthb200_kv16_args_bytes",
+                     "pthb200_kv8_write_args_bytes", "pthb200_kv8_read_args_bytes", "pthb200_kv8_args_bytes", "pthb200_rotary_args_bytes"):
             getattr(lib, name).restype = ctypes.c_int32
             getattr(lib, name).argtypes = []
-        lib.pthb200_kv16_workspace_bytes.restype = ctypes.c_int64
-        lib.pthb200_kv16_workspace_bytes.argtypes = [ctypes.c_int32] * 2
+        for fn in (lib.pthb200_kv16_workspace_bytes, lib.pthb200_kv8_workspace_bytes):
+            fn.restype = ctypes.c_int64
+            fn.argtypes = [ctypes.c_int32] * 2
         for name, args in (("pthb200_page_tables", PthB200TablesArgs), ("pthb200_kv16_write", PthB200Kv16WriteArgs),
-                           ("pthb200_kv16_decode", PthB200Kv16Args), ("pthb200_kv16_cross", PthB200Kv16Args)):
+                           ("pthb200_kv16_decode", PthB200Kv16Args), ("pthb200_kv16_cross", PthB200Kv16Args),
+                           ("pthb200_kv8_write", PthB200Kv8WriteArgs), ("pthb200_kv8_read", PthB200Kv8ReadArgs),
+                           ("pthb200_kv8_decode", PthB200Kv8Args), ("pthb200_kv8_attend", PthB200Kv8Args),
+                           ("pthb200_rotary", PthB200RotaryArgs)):
             getattr(lib, name).restype = ctypes.c_int32
             getattr(lib, name).argtypes = [ctypes.POINTER(args), ctypes.c_void_p]
         lib.pthb200_test_kv16_held.restype = ctypes.c_int32
         lib.pthb200_test_kv16_held.argtypes = [ctypes.POINTER(PthB200Kv16Args), ctypes.c_int32, ctypes.c_int32, ctypes.c_void_p]
         lib.pthb200_kv16_check.restype = ctypes.c_int32
         lib.pthb200_kv16_check.argtypes = [ctypes.POINTER(PthB200Kv16Args)]
+        lib.pthb200_kv8_check.restype = ctypes.c_int32
+        lib.pthb200_kv8_check.argtypes = [ctypes.POINTER(PthB200Kv8Args)]
         for fn in (lib.pthb200_test_schedule, lib.pthb200_test_range_schedule):
             fn.restype = ctypes.c_int32
             fn.argtypes = [ctypes.c_void_p] * 2 + [ctypes.c_int32] * 10 + [ctypes.c_void_p, ctypes.c_int32]
@@ -343,7 +492,11 @@ class B200Lib:
             raise RuntimeError(f"{path}: PthB200WriteArgs size differs from the ctypes mirror")
         for args, size in ((PthB200TablesArgs, lib.pthb200_tables_args_bytes()),
                            (PthB200Kv16WriteArgs, lib.pthb200_kv16_write_args_bytes()),
-                           (PthB200Kv16Args, lib.pthb200_kv16_args_bytes())):
+                           (PthB200Kv16Args, lib.pthb200_kv16_args_bytes()),
+                           (PthB200Kv8WriteArgs, lib.pthb200_kv8_write_args_bytes()),
+                           (PthB200Kv8ReadArgs, lib.pthb200_kv8_read_args_bytes()),
+                           (PthB200Kv8Args, lib.pthb200_kv8_args_bytes()),
+                           (PthB200RotaryArgs, lib.pthb200_rotary_args_bytes())):
             if size != ctypes.sizeof(args):
                 raise RuntimeError(f"{path}: {args.__name__} size differs from the ctypes mirror")
         if lib.pthb200_options_bytes() != ctypes.sizeof(PthB200Options):
@@ -407,6 +560,33 @@ class B200Lib:
 
     def kv16_workspace_bytes(self, head_size: int, num_sms: int) -> int:
         return int(self.lib.pthb200_kv16_workspace_bytes(head_size, num_sms))
+
+    def kv8_write(self, args: PthB200Kv8WriteArgs, *, stream: int = 0) -> int:
+        """Store the K / V rows of new tokens in the 8-bit cache."""
+        return int(self.lib.pthb200_kv8_write(ctypes.byref(args), stream or None))
+
+    def kv8_read(self, args: PthB200Kv8ReadArgs, *, stream: int = 0) -> int:
+        """Runs of positions of the 8-bit cache back into 16- or 32-bit rows."""
+        return int(self.lib.pthb200_kv8_read(ctypes.byref(args), stream or None))
+
+    def kv8_decode(self, args: PthB200Kv8Args, *, stream: int = 0) -> int:
+        """Attention of one token per request over the 8-bit cache."""
+        return int(self.lib.pthb200_kv8_decode(ctypes.byref(args), stream or None))
+
+    def kv8_attend(self, args: PthB200Kv8Args, *, stream: int = 0) -> int:
+        """Attention of every request's new tokens over the 8-bit cache."""
+        return int(self.lib.pthb200_kv8_attend(ctypes.byref(args), stream or None))
+
+    def kv8_check(self, args: PthB200Kv8Args) -> int:
+        """The checks of the two calls above, without a launch."""
+        return int(self.lib.pthb200_kv8_check(ctypes.byref(args)))
+
+    def kv8_workspace_bytes(self, head_size: int, num_sms: int) -> int:
+        return int(self.lib.pthb200_kv8_workspace_bytes(head_size, num_sms))
+
+    def rotary(self, args: PthB200RotaryArgs, *, stream: int = 0) -> int:
+        """Queries and keys turned by their positions."""
+        return int(self.lib.pthb200_rotary(ctypes.byref(args), stream or None))
 
     def tile_tokens(self, wm: int, group: int, max_query_len: int) -> int:
         return int(self.lib.pthb200_tile_tokens(wm, group, max_query_len))

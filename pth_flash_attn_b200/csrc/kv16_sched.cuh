@@ -33,7 +33,8 @@ struct Piece {
   int begins, ends;           // the row tile's first piece, its last
   int first_cta, last_cta;    // that have its pieces (in the counting of the kernel's schedule)
   int sparse;                 // CTAs between them may have none
-  int unused[2];
+  int pos0;                   // position of the request's first query token (8-bit cache)
+  int unused;
 };
 static_assert(sizeof(Piece) == 64, "queue entry");
 
@@ -116,6 +117,8 @@ __device__ __forceinline__ ReqShape req_shape(const Kv16Params& p, int r) {
   s.tiles = s.hi > s.lo && rows > 0 ? (s.hi + kTile - 1) / kTile - s.lo / kTile : 0;
   return s;
 }
+// What a walk says of a piece besides: nothing here.
+__device__ __forceinline__ void place_piece(Piece*, const ReqShape&) {}
 // Counts an arrival behind everything that this CTA's threads have written in front of a barrier that this thread has passed,
 // and ahead of what they read behind the next one: the partial results of all who arrived before.
 __device__ __forceinline__ int arrive_at(int* counter) {
@@ -169,10 +172,10 @@ __device__ __forceinline__ long long scan_threads(long long mine, long long* scr
 }
 
 // Rows of requests without a visible key: zero, -inf.
-template <int HD, int RP, int kThreads>
-__device__ __forceinline__ void zero_requests(const Kv16Params& p) {
+template <int HD, int RP, int kThreads, class Params>
+__device__ __forceinline__ void zero_requests(const Params& p) {
   for (int r = (int)blockIdx.x; r < p.num_reqs; r += (int)gridDim.x) {
-    const ReqShape s = req_shape<RP>(p, r);
+    const auto s = req_shape<RP>(p, r);
     if (s.tiles > 0 || s.tokens == 0) continue;
 #pragma unroll 1
     for (int64_t i = threadIdx.x; i < (int64_t)s.tokens * p.num_q_heads * (HD / 8); i += kThreads) {

@@ -1,0 +1,666 @@
+// Attention over the 8-bit paged cache for requests of few query rows (a row is a query token and head): one-token decode,
+// verification of a few tokens.
+//
+// Orientation: the 128 keys of a tile sit on the MMA's M dimension, the rows of a KV head on N:
+//   S^T[key, row] = sum_d c_K[key, d] Q[row, d]         A = c_K as it lies in the cache (K-major), B = digits of Q
+//   O^T[d, row]  += sum_key c_V[key, d] Y[key, row]     A = c_V as it lies in the cache (MN-major), B = digits of Y
+// with Y = P scale_V / U.  Both operands A are the cache's own bytes (kind::f8f6f4): no cell passes through a register.
+//
+// Digits.  An MMA of this kind takes 8-bit numbers on both sides, so a factor of B goes in as a sum of e4m3 numbers, side by
+// side on N, each with an accumulator of its own: x = u (d0 + d1 / 16 + d2 / 256), every digit the rounding of what is left.  Digits have
+// four bits, and subnormal ones a step of 2^-9, so n digits keep 4 n bits of numbers down to 2^-14 of the largest, and are off by
+// 2^-(14 + 4 n) of it below.  bf16 queries take two (they are exact), fp16 queries three, Y three: its 2^-12 is an eighth of the
+// rounding of a bf16 output, and a key of 2^-25 of its row's largest weight still counts, over 131,072 keys.  At eight rows and
+// 16 or 32 columns they cost the tensor core nothing that shows.
+//   u is a power of two per row for Q (its largest into [128, 256)).  For Y it is U, the largest scale_V so far in the piece, to the
+// next power of two: the accumulators are rescaled where a tile brings a larger one.  scale_K multiplies a key's scores.
+//
+// Softmax in one pass: ref is a running bound of a row's scores (log2 units), P = 2^(s - ref), l = sum P.  ref is a row's
+// maximum less kGain when it is set, and moves (with l and O rescaled) only when a score outgrows it by kSlack: P is at most 2^8.
+//
+// What bounds it: the cache's bytes, 2 D per key and KV head.  The tile's parts (128 keys x 128 dims of K, of V) are units of one
+// ring of shared memory, K of the next tile ahead of V of this one; four warps fill it with 16-byte copies, zero where a key is not
+// visible (so what lies there in memory, NaN included, is never read).  Scales come with them, one per 16 keys.  The warp that works
+// out the pieces makes the digits of their queries.
+//
+// Schedule and merge: kv16_short.cuh.
+#include "kv8.cuh"
+
+#include "kv16_short.cuh"
+#include "pdl.cuh"
+
+namespace pthb200 {
+
+__device__ unsigned int g_kv8_short_status = 0;
+
+namespace {
+
+constexpr int kLoadWarp = 4;           // warps 4-7
+constexpr int kMmaWarp = 8, kScheduleWarp = 9;
+constexpr int kThreads = 320;
+constexpr float kGainY = 6.f, kSlackY = 2.f;
+constexpr int kRun = 16;               // keys that surely share a scale
+constexpr int kScaleTiles = 16;        // tiles whose scales are kept: more than the ring holds units of either kind, and two
+constexpr int kDigitsY = 3;
+
+// Column block c of 16 dims: 128 keys x 16 bytes.  (16 bytes more than they take: a warp's copies go to all banks.)
+constexpr int kColumn = kTile * 16 + 16;
+
+template <int HD, int RP, bool kHalf>
+struct Geo8 {
+  static constexpr int dims = HD < 128 ? HD : 128;   // of a unit
+  static constexpr int parts = HD / dims;            // units of a tile's K, and of its V
+  static constexpr int unit = dims / 16 * kColumn;
+  static constexpr int q_digits = kHalf ? 3 : 2;
+  static constexpr int cols = (q_digits * RP + 15) / 16 * 16;     // N of QK
+  static constexpr int pcols = (kDigitsY * RP + 15) / 16 * 16;    // N of PV
+  static constexpr int qimage = cols * HD;           // column block c of 16 dims at c (cols 16), column n at n 16
+  static constexpr int pimage = pcols * kTile;       // block of 16 columns at 2,048 each, key t at t 16
+  static constexpr int fixed = 2 * qimage + pimage + 3 * 4 * RP * 4 + 2 * RP * 4 + kScaleTiles * 64 + 1024;
+  static constexpr int units2 = (115712 - fixed - 128) / unit;
+  static constexpr int ctas = units2 >= 3 && RP <= 16 ? 2 : 1;
+  static constexpr int most = 2 * (kScaleTiles - 3);   // (see kScaleTiles)
+  static constexpr int fit = ctas == 2 ? units2 : (232448 - fixed - 128) / unit;
+  static constexpr int units = fit < most ? fit : most;
+  static_assert(units >= 3, "K and V of a tile, and the next K");
+  // Registers that the copies hand to the softmax from what a thread starts with (168 with one CTA per SM, 96 with two).
+  static constexpr int softmax_regs = ctas == 1 ? 232 : 128, copy_regs = ctas == 1 ? 72 : 64, start_regs = ctas == 1 ? 168 : 96;
+  static_assert(4 * softmax_regs + 4 * copy_regs <= 8 * start_regs, "a split that the launch holds");
+  static constexpr int s_col = 0, o_col = 2 * cols;  // TMEM columns: S twice, O of every part
+  static constexpr int tmem_need = 2 * cols + parts * pcols;
+  static constexpr int tmem = tmem_need <= 64 ? 64 : tmem_need <= 128 ? 128 : tmem_need <= 256 ? 256 : 512;
+  static_assert(tmem_need <= 512 && tmem * ctas <= 512, "the SM's columns");
+  // shared memory
+  static constexpr int q = units * unit;
+  static constexpr int p = q + 2 * qimage;
+  static constexpr int wmax = p + pimage;            // float [4 warps][RP]
+  static constexpr int wsum = wmax + 4 * RP * 4;     // float [4 warps][RP]
+  static constexpr int at = wsum + 4 * RP * 4;       // int [RP]: positions of the piece's rows
+  static constexpr int qfactor = at + 4 * RP * 4;    // float [2][RP]: a row's u x softmax scale x log2(e)
+  static constexpr int scales = qfactor + 2 * RP * 4;   // [kScaleTiles][2][8]: of the keys, of the values
+  static constexpr int pieces = scales + kScaleTiles * 64;   // PieceQueue's entries
+  static constexpr int bars = pieces + kQueue * 64;
+  static constexpr int n_bars = 2 * units + 2 + 2 + 2 + 1 + 1 + 2 * kQueue + 1;
+  static constexpr int misc = bars + n_bars * 8;     // ints: abort flag, TMEM address, arrival, stop; scratch of find_run
+  static constexpr int end = misc + 160, last64 = HD == 64 ? units * unit + 4 * kColumn : 0;   // (PV reads 64 rows past a unit of 64 dims)
+  static constexpr int total = (end > last64 ? end : last64) + 128;
+  static_assert(kQueue * 64 + n_bars * 8 + 160 <= 1024, "fixed part");
+};
+
+struct Bars8 {  // offsets behind [units] full, [units] empty
+  static constexpr int q_full = 0, q_empty = 2, s_ready = 4, p_ready = 6, pv_done = 7, queue = 8, drained = queue + 2 * kQueue;
+};
+
+// Two numbers' digits, the first in the low byte: d0 = round(x), d1 = round(16 (x - d0)), d2 = round(256 (x - d0 - d1 / 16)).
+template <int kDigits>
+__device__ __forceinline__ void digits2(float a, float b, uint32_t (&d)[kDigits]) {
+#pragma unroll
+  for (int i = 0; i < kDigits; ++i) {
+    d[i] = e4m3x2(a, b);
+    if (i + 1 < kDigits) {
+      const float2 f = float2_of_e4m3x2(d[i]);
+      a = (a - f.x) * 16.f;
+      b = (b - f.y) * 16.f;
+    }
+  }
+}
+
+// The 32 keys of a warp, from `base_key` of a tile on: rows of `kDims` bytes from off (the lane's key's) into a unit's column blocks.
+template <int kDims>
+__device__ __forceinline__ void copy_keys8(uint32_t unit, int base_key, const uint8_t* src, long long off) {
+  constexpr int kChunks = kDims / 16, kRows = 32 / kChunks;
+  const int lane = threadIdx.x & 31, chunk = lane % kChunks, sub = lane / kChunks;
+  const uint32_t dst = unit + chunk * kColumn + base_key * 16;
+#pragma unroll
+  for (int i = 0; i < 32 / kRows; ++i) {
+    const int row = i * kRows + sub;
+    const long long o = __shfl_sync(0xffffffffu, off, row);
+    copy16(dst + row * 16, o >= 0 ? src + o + chunk * 16 : src, o >= 0);
+  }
+}
+// Asynchronous copy of four bytes, or of none: then the destination is zeroed.
+__device__ __forceinline__ void copy4(uint32_t dst, const void* src, bool live) {
+  asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(dst), "l"(src), "r"(live ? 4 : 0) : "memory");
+}
+
+// The scales of a warp's two runs of 16 keys: of the first key of each that is visible (they share them).
+__device__ __forceinline__ void copy_scales(const Kv8Params& p, uint32_t to, int base_key, int kvh, int blk, int slot) {
+  const int lane = threadIdx.x & 31;
+  const uint32_t live = __ballot_sync(0xffffffffu, blk >= 0) >> (lane & 16) & 0xffffu;
+  const int from = (lane & 16) + (live != 0 ? __ffs(live) - 1 : 0);
+  const int b = __shfl_sync(0xffffffffu, blk, from), s = __shfl_sync(0xffffffffu, slot, from);
+  if ((lane & 15) < 2) {   // lane 0 the keys', lane 1 the values'
+    const int64_t at = (int64_t)b * p.scale_stride_block + (int64_t)((uint32_t)s / (uint32_t)p.scale_tokens) * p.scale_stride_group + (int64_t)kvh * p.scale_stride_head;
+    const float* const base = (lane & 15) == 0 ? p.k_scale : p.v_scale;
+    copy4(to + (lane & 15) * 32 + (base_key / kRun + (lane >> 4)) * 4, live != 0 ? base + at : base, live != 0);
+  }
+}
+
+// The digits of a piece's queries: one warp, a row by as many lanes as it has pieces of 8 dims, kBatch pieces of a lane in flight.
+template <int HD, int RP, bool kHalf>
+__device__ __forceinline__ void stage_queries(const Kv8Params& p, const Piece& it, uint8_t* image, float* factor) {
+  using G = Geo8<HD, RP, kHalf>;
+  constexpr int kLanes = HD / 8, kAtOnce = 32 / kLanes, kSteps = RP / kAtOnce, kBatch = kSteps < 4 ? kSteps : 4;
+  const int lane = threadIdx.x & 31, chunk = lane % kLanes, sub = lane / kLanes;
+#pragma unroll 1
+  for (int s0 = 0; s0 < kSteps; s0 += kBatch) {
+    uint4 w[kBatch];
+#pragma unroll
+    for (int b = 0; b < kBatch; ++b) {
+      const int n = (s0 + b) * kAtOnce + sub;
+      w[b] = make_uint4(0u, 0u, 0u, 0u);
+      if (n < it.rows) {
+        int token, head;
+        row_of(p, it.first_token, it.kvh, it.row0 + n, &token, &head);
+        w[b] = __ldg(reinterpret_cast<const uint4*>(p.q + (int64_t)token * p.q_stride_token + (int64_t)head * p.q_stride_head) + chunk);
+      }
+    }
+#pragma unroll
+    for (int b = 0; b < kBatch; ++b) {
+      const int n = (s0 + b) * kAtOnce + sub;
+      const uint32_t words[4] = {w[b].x, w[b].y, w[b].z, w[b].w};
+      float x[8];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        if constexpr (kHalf) {
+          const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&words[i]));
+          x[2 * i] = f.x;
+          x[2 * i + 1] = f.y;
+        } else {
+          x[2 * i] = __uint_as_float(words[i] << 16);
+          x[2 * i + 1] = __uint_as_float(words[i] & 0xffff0000u);
+        }
+      }
+      float top = 0.f;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) top = fmaxf(top, fabsf(x[i]));
+#pragma unroll
+      for (int o = kLanes / 2; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+      // u = 2^e: the row's largest into [128, 256); of a row with an infinity or NaN any u will do, of an empty one too
+      const int e = min(120, max(-119, (int)(__float_as_uint(top) >> 23) - 127 - 7));
+      const float up = power_of_two(-e);
+      uint32_t d[4][G::q_digits];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) digits2<G::q_digits>(x[2 * i] * up, x[2 * i + 1] * up, d[i]);
+      uint8_t* const to = image + (chunk >> 1) * (G::cols * 16) + n * 16 + (chunk & 1) * 8;
+#pragma unroll
+      for (int g = 0; g < G::q_digits; ++g)
+        *reinterpret_cast<uint2*>(to + g * (RP * 16)) = make_uint2(d[0][g] | d[1][g] << 16, d[2][g] | d[3][g] << 16);
+      if (chunk == 0) factor[n] = isinf(top) || isnan(top) ? NAN : power_of_two(e) * p.scale_log2;
+    }
+  }
+}
+
+template <int HD, int RP, bool kHalf>
+__global__ void __launch_bounds__(kThreads, (Geo8<HD, RP, kHalf>::ctas)) kv8_short_kernel(const __grid_constant__ Kv8Params p) {
+  using G = Geo8<HD, RP, kHalf>;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* const smem = smem_raw + ((128u - (tc::smem_u32(smem_raw) & 127u)) & 127u);
+  uint64_t* const full = reinterpret_cast<uint64_t*>(smem + G::bars);
+  uint64_t* const empty = full + G::units;
+  uint64_t* const bars = empty + G::units;
+  volatile int* const abort_flag = reinterpret_cast<volatile int*>(smem + G::misc);
+  uint32_t* const tslot = reinterpret_cast<uint32_t*>(smem + G::misc + 4);
+  int* const arrival = reinterpret_cast<int*>(smem + G::misc + 8);
+  int* const stop = arrival + 1;
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+
+  if (warp == kMmaWarp) {
+    if (lane == 0) {
+      for (int i = 0; i < G::units; ++i) {
+        tc::mbar_init(&full[i], 128);
+        tc::mbar_init(&empty[i], 1);
+      }
+      for (int i = 0; i < 2; ++i) {
+        tc::mbar_init(&bars[Bars8::q_full + i], 1);
+        tc::mbar_init(&bars[Bars8::q_empty + i], 2);   // the last QK has read the digits, the softmax the factors
+        tc::mbar_init(&bars[Bars8::s_ready + i], 2);   // the MMAs are complete; this warp has seen the tile's scales land
+      }
+      tc::mbar_init(&bars[Bars8::p_ready], kSoftmaxThreads);
+      tc::mbar_init(&bars[Bars8::pv_done], 1);
+      tc::mbar_init(&bars[Bars8::drained], 1);
+      PieceQueue(nullptr, &bars[Bars8::queue], stop).init(kThreads / 32 - 1);
+      *abort_flag = 0;
+      tc::mbar_init_fence();
+    }
+    __syncwarp();
+    tc::tmem_alloc(tslot, G::tmem);
+    tc::tmem_relinquish();
+  }
+  pdl_wait();
+  ShortWalk<RP, Kv8Params> walk = find_run<RP, kThreads>(p, reinterpret_cast<long long*>(smem + G::misc + 16));
+  tc::fence_before_sync();
+  __syncthreads();
+  tc::fence_after_sync();
+  const uint32_t tmem_base = *tslot;
+  PieceQueue queue(reinterpret_cast<Piece*>(smem + G::pieces), &bars[Bars8::queue], stop);
+  float* const qfactor = reinterpret_cast<float*>(smem + G::qfactor);
+  bool ok = true;
+
+  if (warp == kScheduleWarp) {
+    // =========================== schedule and queries ============================
+    Piece it;
+    uint32_t item = 0;
+    bool going = true;
+    while (going && walk.next(p, &it)) {
+      going = queue.put(it, abort_flag);
+      if (!going) break;
+      // (behind a wait that gave up the digits may still be read: nothing is written, and the next put ends the queue)
+      if (__all_sync(0xffffffffu, item < 2 || kv16_wait<kPieceTimes>(&bars[Bars8::q_empty + (item & 1)], ((item >> 1) - 1) & 1, abort_flag))) {
+        stage_queries<HD, RP, kHalf>(p, it, smem + G::q + (item & 1) * G::qimage, qfactor + (item & 1) * RP);
+        tc::fence_async_smem();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&bars[Bars8::q_full + (item & 1)]);
+      }
+      ++item;
+    }
+    if (going) {
+      it.tiles = 0;
+      queue.put(it, abort_flag);
+    }
+  } else if (warp >= kLoadWarp && warp < kMmaWarp) {
+    // =========================== copies ==========================================
+    // A warp owns 32 keys of every tile: lane l knows where key l of them lies.
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(G::copy_regs));
+    const int base_key = (warp - kLoadWarp) * 32;
+    const uint32_t ring = tc::smem_u32(smem), scales = tc::smem_u32(smem + G::scales);
+    uint32_t unit = 0, tile = 0;
+    auto next_unit = [&]() -> uint32_t {
+      const uint32_t s = unit % G::units;
+      if (unit >= G::units) ok &= kv16_wait(&empty[s], ((unit / G::units) - 1) & 1, abort_flag);
+      ++unit;
+      return s;
+    };
+    {
+      KeyLookup keys(p, queue, abort_flag, base_key + lane);
+      bool have = keys.fetch(), have_v = false;
+      long long off_v = 0;
+      int64_t head_v = 0;
+      while (have || have_v) {
+        const bool now = have;
+        long long off = 0;
+        int64_t head_k = 0;
+        if (now) {
+          off = keys.offset();
+          const int kvh = keys.it.kvh, blk = keys.blk, slot = keys.slot;
+          head_k = (int64_t)kvh * p.stride_head;
+          have = keys.fetch();
+#pragma unroll
+          for (int part = 0; part < G::parts; ++part) {
+            const uint32_t s = next_unit();
+            if (part == 0) copy_scales(p, scales + (tile++ % kScaleTiles) * 64, base_key, kvh, blk, slot);
+            copy_keys8<G::dims>(ring + s * G::unit, base_key, p.k + head_k + part * 128, off);
+            copies_arrive(&full[s]);
+          }
+        }
+        if (have_v) {
+#pragma unroll
+          for (int part = 0; part < G::parts; ++part) {
+            const uint32_t s = next_unit();
+            copy_keys8<G::dims>(ring + s * G::unit, base_key, p.v + head_v + part * 128, off_v);
+            copies_arrive(&full[s]);
+          }
+        }
+        off_v = off;
+        head_v = head_k;
+        have_v = now;
+      }
+    }
+    copies_wait_all();
+  } else if (warp == kMmaWarp) {
+    // =========================== MMAs ============================================
+    // QK of a tile is issued ahead of PV of the one before, in the order in which the units arrive.
+    constexpr uint32_t qk_desc = instr_desc_e4m3(128, G::cols, 0, 0);
+    constexpr uint32_t pv_desc = instr_desc_e4m3(128, G::pcols, 1, 1);
+    const uint32_t ring = tc::smem_u32(smem), q_s = tc::smem_u32(smem + G::q), p_s = tc::smem_u32(smem + G::p);
+    uint32_t unit = 0, tile = 0, item = 0;
+    auto arrived = [&]() -> uint32_t {
+      const uint32_t s = unit % G::units;
+      ok &= kv16_wait(&full[s], (unit / G::units) & 1, abort_flag);
+      tc::fence_async_smem();   // (the copies wrote through the generic proxy)
+      ++unit;
+      return s;
+    };
+    auto qk = [&](bool first_of_item, bool last_of_item) {
+      if (first_of_item) ok &= kv16_wait(&bars[Bars8::q_full + (item & 1)], (item >> 1) & 1, abort_flag);
+#pragma unroll
+      for (int part = 0; part < G::parts; ++part) {
+        const uint32_t s = arrived();
+        if (elect_one()) {
+          tc::fence_after_sync();
+#pragma unroll
+          for (int kk = 0; kk < G::dims / 32; ++kk) {
+            const uint64_t a = tc::smem_desc(ring + s * G::unit + kk * 2 * kColumn, kColumn, 128);
+            const uint64_t b = tc::smem_desc(q_s + (item & 1) * G::qimage + (part * (G::dims / 16) + kk * 2) * (G::cols * 16), G::cols * 16, 128);
+            mma_e4m3(tmem_base + G::s_col + (tile & 1) * G::cols, a, b, qk_desc, part > 0 || kk > 0);
+          }
+          tc::mma_commit(&empty[s]);
+          if (part == G::parts - 1) {
+            tc::mma_commit(&bars[Bars8::s_ready + (tile & 1)]);
+            mbar_arrive(&bars[Bars8::s_ready + (tile & 1)]);
+            if (last_of_item) tc::mma_commit(&bars[Bars8::q_empty + (item & 1)]);
+          }
+        }
+        __syncwarp();
+      }
+      ++tile;
+      if (last_of_item) ++item;
+    };
+    uint32_t pv_tile = 0;
+    auto pv = [&](bool first_of_item) {
+      ok &= kv16_wait(&bars[Bars8::p_ready], pv_tile & 1, abort_flag);
+#pragma unroll
+      for (int part = 0; part < G::parts; ++part) {
+        const uint32_t s = arrived();
+        if (elect_one()) {
+          tc::fence_after_sync();
+#pragma unroll
+          for (int kk = 0; kk < kTile / 32; ++kk) {
+            // (64 dims: the instruction's other 64 rows are what follows the unit, which nothing reads)
+            const uint64_t a = tc::smem_desc(ring + s * G::unit + kk * 512, 128, kColumn);
+            const uint64_t b = tc::smem_desc(p_s + kk * 512, 128, kTile * 16);
+            mma_e4m3(tmem_base + G::o_col + part * G::pcols, a, b, pv_desc, !first_of_item || kk > 0);
+          }
+          tc::mma_commit(&empty[s]);
+          if (part == G::parts - 1) tc::mma_commit(&bars[Bars8::pv_done]);
+        }
+        __syncwarp();
+      }
+      ++pv_tile;
+    };
+    Piece it;
+    bool pending = false, pending_first = false;
+    while (queue.get(&it, abort_flag)) {
+      for (int t = 0; t < it.tiles; ++t) {
+        qk(t == 0, t == it.tiles - 1);
+        if (pending) pv(pending_first);
+        pending = true;
+        pending_first = t == 0;
+      }
+    }
+    if (pending) pv(pending_first);
+  } else if (warp < kLoadWarp) {
+    // =========================== softmax =========================================
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(G::softmax_regs));
+    const uint32_t lane_addr = (uint32_t)(warp * 32) << 16;
+    float* const wmax = reinterpret_cast<float*>(smem + G::wmax);
+    float* const wsum = reinterpret_cast<float*>(smem + G::wsum);
+    int* const row_at = reinterpret_cast<int*>(smem + G::at);
+    uint8_t* const p_img = smem + G::p + tid * 16;
+    uint32_t tile = 0, item = 0;
+    zero_requests<HD, RP, kSoftmaxThreads>(p);
+    {
+      const int heads = min(p.num_kv_heads, (int)gridDim.x), hslot = (int)blockIdx.x % heads;
+      Piece it;
+      while (queue.get(&it, abort_flag)) {
+        const int kvh = it.kvh;
+        ok &= kv16_wait(&bars[Bars8::q_full + (item & 1)], (item >> 1) & 1, abort_flag);
+        const float* const factor = qfactor + (item & 1) * RP;
+        // rows of several tokens: keys that some of them see and others do not, [.., mask_lo) and [mask_hi, ..)
+        int mask_lo = 0, mask_hi = INT_MAX;
+        if (p.query_start_loc != nullptr) {
+          if (p.causal) mask_hi = it.pos0 + it.row0 / p.group + 1;
+          mask_lo = kv8_low(p, it.pos0 + (it.row0 + it.rows - 1) / p.group);
+          if (tid < RP) row_at[tid] = it.pos0 + (it.row0 + min(tid, it.rows - 1)) / p.group;
+          softmax_sync();
+        }
+        float ref[RP], l[RP];
+        int unit_e = -126;   // U = 2^unit_e
+#pragma unroll
+        for (int n = 0; n < RP; ++n) {
+          ref[n] = -INFINITY;
+          l[n] = 0.f;
+        }
+        for (int t = 0; t < it.tiles; ++t, ++tile) {
+          ok &= kv16_wait(&bars[Bars8::s_ready + (tile & 1)], (tile >> 1) & 1, abort_flag);
+          tc::fence_after_sync();
+          uint32_t sr[G::cols];
+          tmem_load<G::cols>(tmem_base + G::s_col + (tile & 1) * G::cols + lane_addr, sr);
+          tc::tmem_ld_wait<G::cols>(sr);
+          const float* const scale = reinterpret_cast<const float*>(smem + G::scales + (tile % kScaleTiles) * 64);
+          const float k_scale = scale[tid / kRun], v_scale = scale[8 + tid / kRun];
+          float most = 0.f;
+#pragma unroll
+          for (int i = 0; i < 8; ++i) most = fmaxf(most, fabsf(scale[8 + i]));
+          const int pos = it.key0 + t * kTile + tid;
+          float s[RP];
+#pragma unroll
+          for (int n = 0; n < RP; ++n) {
+            float x = fmaf(__uint_as_float(sr[RP + n]), 0.0625f, __uint_as_float(sr[n]));
+            if constexpr (G::q_digits == 3) x = fmaf(__uint_as_float(sr[2 * RP + n]), 0.00390625f, x);
+            s[n] = x * k_scale * factor[n];
+          }
+          const int key0 = it.key0 + t * kTile;
+          if (pos < it.lo || pos >= it.hi) {
+#pragma unroll
+            for (int n = 0; n < RP; ++n) s[n] = -INFINITY;
+          } else if (key0 < mask_lo || key0 + kTile > mask_hi) {
+#pragma unroll
+            for (int n = 0; n < RP; ++n) {
+              const int own = row_at[n];
+              if ((p.causal && pos > own) || pos < kv8_low(p, own)) s[n] = -INFINITY;
+            }
+          }
+          float x[RP];
+          bool outgrown = false;
+#pragma unroll
+          for (int n = 0; n < RP; ++n) {
+            x[n] = s[n] - ref[n];
+            outgrown |= n < it.rows && !(x[n] <= kGainY + kSlackY);   // (also where ref is not set yet)
+          }
+          const int e = min(126, max(-126, (int)((__float_as_uint(most) + 0x7fffffu) >> 23) - 127));   // 2^e >= most
+          const bool larger = e > unit_e;   // (the same in all threads)
+          if (softmax_any(outgrown || larger)) {
+#pragma unroll
+            for (int n = 0; n < RP; ++n) {
+              const float m = redux_max(s[n]);
+              if (lane == 0) wmax[warp * RP + n] = m;
+            }
+            softmax_sync();
+            const int unit_to = max(unit_e, e);
+            const float shrink = kv16_exp2((float)(unit_e - unit_to));
+            unit_e = unit_to;
+            float alpha[RP];
+            bool moved = shrink != 1.f;
+#pragma unroll
+            for (int n = 0; n < RP; ++n) {
+              const float m = fmaxf(fmaxf(wmax[n], wmax[RP + n]), fmaxf(wmax[2 * RP + n], wmax[3 * RP + n])) - kGainY;
+              const float to = fmaxf(ref[n], m);
+              alpha[n] = to == -INFINITY ? 1.f : kv16_exp2(ref[n] - to);
+              moved |= alpha[n] != 1.f;
+              ref[n] = to;
+              l[n] *= alpha[n];
+              x[n] = s[n] - (to == -INFINITY ? 0.f : to);
+            }
+            if (t > 0 && moved) {   // (the same in all threads)
+              ok &= kv16_wait(&bars[Bars8::pv_done], (tile - 1) & 1, abort_flag);
+              tc::fence_after_sync();
+#pragma unroll
+              for (int d = 0; d < kDigitsY * G::parts; ++d) {
+                uint32_t o[RP];
+                const uint32_t addr = tmem_base + G::o_col + (d / kDigitsY) * G::pcols + (d % kDigitsY) * RP + lane_addr;
+                tmem_load<RP>(addr, o);
+                tc::tmem_ld_wait<RP>(o);
+#pragma unroll
+                for (int n = 0; n < RP; ++n) o[n] = __float_as_uint(__uint_as_float(o[n]) * (alpha[n] * shrink));
+                tmem_store<RP>(addr, o);
+              }
+              tc::tmem_st_wait();
+            }
+            softmax_sync();  // (the maxima have been read)
+          }
+          const float y_scale = v_scale * power_of_two(-unit_e);
+          uint32_t y[RP / 2][kDigitsY];   // digits of two rows each
+#pragma unroll
+          for (int n = 0; n < RP; n += 2) {
+            const float a = kv16_exp2(x[n]), b = kv16_exp2(x[n + 1]);
+            l[n] += a;
+            l[n + 1] += b;
+            digits2<kDigitsY>(a * y_scale, b * y_scale, y[n / 2]);
+          }
+          if (tile > 0) ok &= kv16_wait(&bars[Bars8::pv_done], (tile - 1) & 1, abort_flag);  // (P of the last tile has been read)
+          // column d RP + n: digit d of row n; 16 columns are 16 bytes of the key's
+#pragma unroll
+          for (int j = 0; j < G::pcols / 16; ++j) {
+            uint32_t w[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              const int c = j * 16 + i * 4, d = c / RP, n = c % RP;
+              w[i] = d < kDigitsY ? y[n / 2][d < kDigitsY ? d : 0] | y[n / 2 + 1][d < kDigitsY ? d : 0] << 16 : 0u;
+            }
+            *reinterpret_cast<uint4*>(p_img + j * (kTile * 16)) = make_uint4(w[0], w[1], w[2], w[3]);
+          }
+          tc::fence_async_smem();
+          tc::fence_before_sync();
+          mbar_arrive(&bars[Bars8::p_ready]);
+        }
+        // ---- the piece's rows ----
+#pragma unroll
+        for (int n = 0; n < RP; ++n) {
+          if (n < it.rows) {
+#pragma unroll
+            for (int o = 16; o > 0; o >>= 1) l[n] += __shfl_xor_sync(0xffffffffu, l[n], o);
+          }
+        }
+        if (lane == 0) {
+#pragma unroll
+          for (int n = 0; n < RP; ++n) wsum[warp * RP + n] = l[n];
+        }
+        softmax_sync();
+        if (tid == 0) mbar_arrive(&bars[Bars8::q_empty + (item & 1)]);   // (all have read the factors)
+        ++item;
+#pragma unroll
+        for (int n = 0; n < RP; ++n) l[n] = (wsum[n] + wsum[RP + n]) + (wsum[2 * RP + n] + wsum[3 * RP + n]);
+        ok &= kv16_wait(&bars[Bars8::pv_done], (tile - 1) & 1, abort_flag);
+        tc::fence_after_sync();
+        const bool whole = it.begins && it.ends;
+        float* const slot = partial_slot<HD, RP>(p, (int)blockIdx.x, it.begins);
+        const float unit_value = power_of_two(unit_e);
+#pragma unroll
+        for (int part = 0; part < G::parts; ++part) {
+          uint32_t o[G::pcols];
+          tmem_load<G::pcols>(tmem_base + G::o_col + part * G::pcols + lane_addr, o);
+          tc::tmem_ld_wait<G::pcols>(o);
+          const int d = part * 128 + tid;
+          if (d < HD) {
+#pragma unroll
+            for (int n = 0; n < RP; ++n) {
+              if (n < it.rows) {
+                const float v = fmaf(fmaf(__uint_as_float(o[2 * RP + n]), 0.0625f, __uint_as_float(o[RP + n])), 0.0625f, __uint_as_float(o[n])) * unit_value;
+                if (whole) {
+                  int token, head;
+                  row_of(p, it.first_token, kvh, it.row0 + n, &token, &head);
+                  store_out_elem(p.out + (int64_t)token * p.out_stride_token + (int64_t)head * p.out_stride_head, d, kHalf ? PTH_ATTN_F16 : PTH_ATTN_BF16,
+                                 l[n] == 0.f ? 0.f : __fdividef(v, l[n]));
+                } else {
+                  slot[n * HD + d] = v;
+                }
+              }
+            }
+          }
+        }
+        tc::fence_before_sync();
+        if (tid == 0) {
+#pragma unroll
+          for (int n = 0; n < RP; ++n) {
+            if (n < it.rows) {
+              if (whole) {
+                int token, head;
+                row_of(p, it.first_token, kvh, it.row0 + n, &token, &head);
+                if (p.lse != nullptr)
+                  p.lse[(int64_t)token * p.num_q_heads + head] = l[n] == 0.f ? -INFINITY : ((ref[n] == -INFINITY ? 0.f : ref[n]) + log2f(l[n])) * kLn2;
+              } else {
+                slot[RP * HD + n] = ref[n];
+                slot[RP * HD + RP + n] = l[n];
+              }
+            }
+          }
+        }
+        if (!whole) {
+          const int g0 = it.first_cta, g1 = it.last_cta;   // (groups)
+          softmax_sync();
+          int* const counter = reinterpret_cast<int*>(p.workspace) + g0 * heads + hslot;
+          if (tid == 0) {
+            *arrival = arrive_at(counter);
+            if (*arrival == g1 - g0) *counter = 0;   // (for the next call)
+          }
+          softmax_sync();
+          if (*arrival == g1 - g0) merge_pieces<HD, RP, kHalf>(p, it, kvh, g0, g1 - g0 + 1, heads, hslot);
+        }
+        softmax_sync();  // (the sums and the arrival have been read)
+      }
+    }
+  }
+  tc::fence_before_sync();
+  __syncthreads();
+  if (warp == kMmaWarp) {
+    if (*abort_flag) {   // (copies have landed, MMAs may be in flight)
+      if (elect_one()) {
+        tc::mma_commit(&bars[Bars8::drained]);
+        kv16_drain(&bars[Bars8::drained], 0);
+        atomicOr(&g_kv8_short_status, 32u);
+      }
+      __syncwarp();
+    }
+    tc::tmem_dealloc(tmem_base, G::tmem);
+  }
+  (void)ok;
+}
+
+template <int HD, int RP, bool kHalf>
+cudaError_t launch_one(const Kv8Params& p, cudaStream_t stream) {
+  using G = Geo8<HD, RP, kHalf>;
+  static_assert(G::total <= 232448, "shared memory of one CTA");
+  static_assert(G::ctas == 1 || G::total <= 115712, "shared memory of two CTAs");
+  static bool configured[64] = {};
+  int dev = 0;
+  cudaError_t err = cudaGetDevice(&dev);
+  if (err != cudaSuccess) return err;
+  if (dev < 0 || dev >= 64 || !configured[dev]) {
+    err = cudaFuncSetAttribute(kv8_short_kernel<HD, RP, kHalf>, cudaFuncAttributeMaxDynamicSharedMemorySize, G::total);
+    if (err != cudaSuccess) return err;
+    if (dev >= 0 && dev < 64) configured[dev] = true;
+  }
+  const int sms = sm_count();
+  if (sms <= 0) return cudaErrorInvalidDevice;
+  return pdl_launch(kv8_short_kernel<HD, RP, kHalf>, dim3((unsigned)(sms * G::ctas)), dim3(kThreads), G::total, stream, p);
+}
+template <int HD, int RP>
+cudaError_t launch_type(const Kv8Params& p, cudaStream_t stream) {
+  return p.dtype == PTH_ATTN_F16 ? launch_one<HD, RP, true>(p, stream) : launch_one<HD, RP, false>(p, stream);
+}
+template <int HD>
+cudaError_t launch_rows(const Kv8Params& p, cudaStream_t stream) {
+  const int64_t rows = (int64_t)p.max_query_len * p.group;
+  if (rows <= 8) return launch_type<HD, 8>(p, stream);
+  if (rows <= 16) return launch_type<HD, 16>(p, stream);
+  return launch_type<HD, 32>(p, stream);
+}
+
+}  // namespace
+
+// Counters, and two partial row tiles per CTA: twice the SMs' number of CTAs with 16 rows, or as many with 32.
+int64_t kv8_short_workspace_bytes(int head_size, int num_sms) {
+  return kCounterBytes + (int64_t)num_sms * 2 * 2 * 16 * (head_size + 2) * 4;
+}
+
+cudaError_t launch_kv8_short(const Kv8Params& p, cudaStream_t stream) {
+  switch (p.head_size) {
+    case 64:
+      return launch_rows<64>(p, stream);
+    case 128:
+      return launch_rows<128>(p, stream);
+    default:
+      return launch_rows<256>(p, stream);
+  }
+}
+
+// Reads and clears this kernel's status word (device must be idle).
+cudaError_t read_kv8_short_status(unsigned int* v) {
+  unsigned int zero = 0;
+  cudaError_t err = cudaMemcpyFromSymbol(v, g_kv8_short_status, sizeof(*v));
+  if (err != cudaSuccess) return err;
+  return cudaMemcpyToSymbol(g_kv8_short_status, &zero, sizeof(zero));
+}
+
+}  // namespace pthb200

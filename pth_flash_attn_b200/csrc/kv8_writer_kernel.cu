@@ -1,0 +1,289 @@
+// Writer of the 8-bit paged cache: new tokens' K and V rows as e4m3 numbers, with a power of two as the scale of a block of tokens.
+//
+// A unit of work is a block of tokens of a request that the call writes to, a KV head, K or V.  Its new rows' largest finite value
+// gives the scale that they need; a block that goes on keeps its own unless it is too small, and then the cells in front of the
+// new ones are rounded again.  A power of two costs e4m3 nothing (its relative error is the same at any size) and makes both the
+// quotients and the re-rounding exact up to the one rounding.
+//
+// Blocks up to 32 tokens are a warp's work: its rows of 16 bytes a lane stay in registers between the maximum and the rounding.
+// Larger ones are a CTA's, which reads the rows again (from L2) for the rounding.  Bytes bound it: T Hkv D (source + 1) x 2.
+//
+// Units find their block without a list: request r's blocks are numbered from start_r / g + 2 r on, which leaves room for the two
+// more blocks than q / g that its tokens may touch (r itself where a request has one token at most).  Numbers that no block has
+// end at once.
+#include "kv8.cuh"
+
+#include "pdl.cuh"
+
+namespace pthb200 {
+namespace {
+
+constexpr int kWarps = 8;
+constexpr int kRowsKept = 4;   // pieces of 16 source bytes (32 in fp32) that a lane keeps
+
+struct Write8Params {
+  const uint8_t* src[2];
+  int64_t src_stride_token[2], src_stride_head[2];
+  uint8_t* cache[2];
+  int64_t stride_block[2], stride_slot[2], stride_head[2];
+  float* scale[2];
+  int64_t scale_stride_block[2], scale_stride_group[2], scale_stride_head[2];   // in elements
+  const int32_t* block_table;
+  int64_t block_table_row_stride;
+  const int32_t* seq_lens;
+  const int32_t* query_start_loc;
+  int32_t num_blocks, block_size, scale_tokens, num_kv_heads, num_reqs, num_tokens, num_pages, max_query_len, src_dtype;
+};
+
+// Eight elements of a source row in 32 bits.  kWide: rows lie on 16-byte boundaries.
+template <int kDtype, bool kWide>
+__device__ __forceinline__ void load8(const uint8_t* row, int e0, float (&x)[8]) {
+  if constexpr (kDtype == PTH_ATTN_F32) {
+    if constexpr (kWide) {
+      const float4 a = __ldg(reinterpret_cast<const float4*>(row) + e0 / 4), b = __ldg(reinterpret_cast<const float4*>(row) + e0 / 4 + 1);
+      x[0] = a.x, x[1] = a.y, x[2] = a.z, x[3] = a.w, x[4] = b.x, x[5] = b.y, x[6] = b.z, x[7] = b.w;
+    } else {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) x[i] = __ldg(reinterpret_cast<const float*>(row) + e0 + i);
+    }
+  } else {
+    uint32_t w[4];
+    if constexpr (kWide) {
+      const uint4 v = __ldg(reinterpret_cast<const uint4*>(row) + e0 / 8);
+      w[0] = v.x, w[1] = v.y, w[2] = v.z, w[3] = v.w;
+    } else {
+      const uint16_t* const h = reinterpret_cast<const uint16_t*>(row) + e0;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) w[i] = (uint32_t)__ldg(h + 2 * i) | (uint32_t)__ldg(h + 2 * i + 1) << 16;
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      if constexpr (kDtype == PTH_ATTN_F16) {
+        const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w[i]));
+        x[2 * i] = f.x;
+        x[2 * i + 1] = f.y;
+      } else {
+        x[2 * i] = __uint_as_float(w[i] << 16);
+        x[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
+      }
+    }
+  }
+}
+__device__ __forceinline__ float finite_max(const float (&x)[8]) {
+  float m = 0.f;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const float a = fabsf(x[i]);
+    m = a < INFINITY ? fmaxf(m, a) : m;
+  }
+  return m;
+}
+// The smallest power of two, 2^-126 to 2^120, with most <= 448 times it.
+__device__ __forceinline__ float needed_scale(float most) {
+  const uint32_t bits = __float_as_uint(most);
+  // 448 = 1.75 x 2^8: the exponent less 8, one more where the significand is above 1.75
+  const int e = (int)(bits >> 23) - 127 - 8 + ((bits & 0x7fffffu) > 0x600000u ? 1 : 0);
+  return power_of_two(min(120, max(-126, e)));
+}
+// Eight numbers as cells, x / scale: exactly scaled where the scale is a power of two.
+__device__ __forceinline__ uint2 cells8(const float (&x)[8], float scale) {
+  float y[8];
+  if ((__float_as_uint(scale) & 0x7fffffu) == 0) {
+    const float up = power_of_two(127 - (int)(__float_as_uint(scale) >> 23));
+#pragma unroll
+    for (int i = 0; i < 8; ++i) y[i] = x[i] * up;
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) y[i] = __fdiv_rn(x[i], scale);
+  }
+  return make_uint2(e4m3x2(y[0], y[1]) | e4m3x2(y[2], y[3]) << 16, e4m3x2(y[4], y[5]) | e4m3x2(y[6], y[7]) << 16);
+}
+__device__ __forceinline__ uint32_t rescaled(uint32_t w, float ratio) {
+  const float2 a = float2_of_e4m3x2(w & 0xffffu), b = float2_of_e4m3x2(w >> 16);
+  return e4m3x2(a.x * ratio, a.y * ratio) | e4m3x2(b.x * ratio, b.y * ratio) << 16;
+}
+
+// A block of tokens that the call writes to.
+struct Block {
+  int row0, rows;      // first new row of the source, their number
+  int begin;           // first new position in the block of tokens
+  int block, group;    // of the cache
+};
+
+// Block number x of the launch, found by a warp (the same in all lanes); false: there is none.
+__device__ __forceinline__ bool find_block(const Write8Params& p, int x, Block* out) {
+  const int g = p.scale_tokens, lane = threadIdx.x & 31;
+  auto base = [&](int r) -> long long {
+    return p.max_query_len == 1 ? r : (long long)(min(max(0, __ldg(p.query_start_loc + r)), p.num_tokens) / g) + 2ll * r;
+  };
+  int r = x;
+  if (p.max_query_len > 1) {   // the last request whose numbers begin at or in front of x, 32 at a time
+    int lo = 0, hi = p.num_reqs;
+#pragma unroll 1
+    while (hi - lo > 1) {
+      const int step = (hi - lo + 31) / 32, at = lo + lane * step;
+      const uint32_t before = __ballot_sync(0xffffffffu, at < hi && base(at) <= x);
+      if (before == 0) return false;   // (start offsets that go backwards)
+      const int last = 31 - __clz(before);
+      hi = min(hi, lo + (last + 1) * step);
+      lo += last * step;
+    }
+    r = lo;
+  }
+  if (r >= p.num_reqs) return false;
+  const int first = max(0, __ldg(p.query_start_loc + r)), end = min(max(0, __ldg(p.query_start_loc + r + 1)), p.num_tokens);
+  const int all = max(0, end - first), tokens = min(all, p.max_query_len), pos0 = max(0, __ldg(p.seq_lens + r)) - all;
+  const int skip = max(0, -pos0);   // tokens at negative positions
+  if (tokens <= skip) return false;
+  const long long nth = x - base(r);
+  const long long start = ((long long)(pos0 + skip) / g + nth) * g;
+  const long long from = max(start, (long long)pos0 + skip), to = min(start + g, (long long)pos0 + tokens);
+  if (nth < 0 || to <= from) return false;
+  const long long page = from / p.block_size;
+  if (page >= p.num_pages) return false;
+  out->block = __ldg(p.block_table + (int64_t)r * p.block_table_row_stride + page);
+  if ((uint32_t)out->block >= (uint32_t)p.num_blocks) return false;
+  out->group = (int)(start - page * p.block_size) / g;
+  out->begin = (int)(from - start);
+  out->rows = (int)(to - from);
+  out->row0 = first + (int)(from - pos0);
+  return true;
+}
+
+template <int HD, int kDtype, bool kWide, bool kCta>
+__global__ void __launch_bounds__(kWarps * 32) kv8_writer_kernel(const __grid_constant__ Write8Params p) {
+  constexpr int kLanes = HD / 8, kAtOnce = 32 / kLanes;      // lanes of a row, rows of a warp at a time
+  __shared__ float most_of[kWarps];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int chunk = lane % kLanes, sub = lane / kLanes;
+  // units: (block number, head, K or V), the last fastest
+  const int per = 2 * p.num_kv_heads;
+  const int64_t unit = kCta ? (int64_t)blockIdx.x : (int64_t)blockIdx.x * kWarps + warp;
+  const int x = (int)(unit / per), rest = (int)(unit - (int64_t)x * per), head = rest >> 1, v = rest & 1;
+  pdl_wait();
+  Block b;
+  if (!find_block(p, x, &b)) return;
+  const uint8_t* const src = p.src[v] + (int64_t)b.row0 * p.src_stride_token[v] + (int64_t)head * p.src_stride_head[v];
+  const int64_t stride = p.src_stride_token[v];
+  uint8_t* const cells = p.cache[v] + (int64_t)b.block * p.stride_block[v] + (int64_t)(b.group * p.scale_tokens) * p.stride_slot[v] + (int64_t)head * p.stride_head[v] + chunk * 8;
+  float* const scale_at = p.scale[v] + (int64_t)b.block * p.scale_stride_block[v] + (int64_t)b.group * p.scale_stride_group[v] + (int64_t)head * p.scale_stride_head[v];
+  float was = b.begin > 0 ? *scale_at : 0.f;
+  if (!(was > 0.f && was < INFINITY)) was = 0.f;
+  constexpr int kStep = (kCta ? kWarps : 1) * kAtOnce;       // rows of a round
+  const int mine = (kCta ? warp * kAtOnce : 0) + sub;
+  float most = 0.f, kept[kRowsKept][8];
+#pragma unroll 1
+  for (int n0 = 0; n0 < b.rows; n0 += kRowsKept * kStep) {
+#pragma unroll
+    for (int i = 0; i < kRowsKept; ++i) {
+      const int n = n0 + i * kStep + mine;
+#pragma unroll
+      for (int k = 0; k < 8; ++k) kept[i][k] = 0.f;
+      if (n < b.rows) load8<kDtype, kWide>(src + n * stride, chunk * 8, kept[i]);
+    }
+#pragma unroll
+    for (int i = 0; i < kRowsKept; ++i) most = fmaxf(most, finite_max(kept[i]));
+  }
+  most = redux_max(most);
+  if constexpr (kCta) {
+    if (lane == 0) most_of[warp] = most;
+    __syncthreads();
+#pragma unroll
+    for (int w = 0; w < kWarps; ++w) most = fmaxf(most, most_of[w]);
+  }
+  const float scale = fmaxf(was, needed_scale(most));
+  // the cells in front of the new ones
+  if (b.begin > 0 && scale > was) {
+    const float ratio = was / scale;
+#pragma unroll 1
+    for (int n = mine; n < b.begin; n += kStep) {
+      uint2* const at = reinterpret_cast<uint2*>(cells + (int64_t)n * p.stride_slot[v]);
+      const uint2 w = *at;
+      *at = make_uint2(rescaled(w.x, ratio), rescaled(w.y, ratio));
+    }
+  }
+  const bool once = b.rows <= kRowsKept * kStep;   // (the rows are in registers still)
+#pragma unroll 1
+  for (int n0 = 0; n0 < b.rows; n0 += kRowsKept * kStep) {
+#pragma unroll
+    for (int i = 0; i < kRowsKept; ++i) {
+      const int n = n0 + i * kStep + mine;
+      if (!once && n < b.rows) load8<kDtype, kWide>(src + n * stride, chunk * 8, kept[i]);
+    }
+#pragma unroll
+    for (int i = 0; i < kRowsKept; ++i) {
+      const int n = n0 + i * kStep + mine;
+      if (n < b.rows) *reinterpret_cast<uint2*>(cells + (int64_t)(b.begin + n) * p.stride_slot[v]) = cells8(kept[i], scale);
+    }
+  }
+  if constexpr (kCta) __syncthreads();   // (all have read the old scale)
+  if (lane == 0 && (!kCta || warp == 0) && scale != was) *scale_at = scale;
+}
+
+template <int HD, int kDtype>
+cudaError_t launch_for(const Write8Params& p, bool wide, cudaStream_t stream) {
+  const int64_t numbers = p.max_query_len == 1 ? p.num_reqs : (int64_t)(p.num_tokens / p.scale_tokens) + 2ll * p.num_reqs;
+  const int64_t units = numbers * 2 * p.num_kv_heads;
+  // a warp reads a block of 32 rows in two to eight rounds
+  const bool cta = p.scale_tokens > 32 && p.max_query_len > 1;
+  const int64_t ctas = cta ? units : (units + kWarps - 1) / kWarps;
+  if (ctas > 0x7fffffff) return cudaErrorInvalidConfiguration;
+  const dim3 grid((unsigned)ctas), block(kWarps * 32);
+  if (cta) return pdl_launch(wide ? kv8_writer_kernel<HD, kDtype, true, true> : kv8_writer_kernel<HD, kDtype, false, true>, grid, block, 0, stream, p);
+  return pdl_launch(wide ? kv8_writer_kernel<HD, kDtype, true, false> : kv8_writer_kernel<HD, kDtype, false, false>, grid, block, 0, stream, p);
+}
+template <int HD>
+cudaError_t launch_type(const Write8Params& p, bool wide, cudaStream_t stream) {
+  if (p.src_dtype == PTH_ATTN_F32) return launch_for<HD, PTH_ATTN_F32>(p, wide, stream);
+  if (p.src_dtype == PTH_ATTN_F16) return launch_for<HD, PTH_ATTN_F16>(p, wide, stream);
+  return launch_for<HD, PTH_ATTN_BF16>(p, wide, stream);
+}
+
+}  // namespace
+
+cudaError_t launch_kv8_writer(const PthB200Kv8WriteArgs& a, cudaStream_t stream) {
+  Write8Params p{};
+  const PthAttnStream* cache[2] = {&a.k_cache, &a.v_cache};
+  const PthAttnStream* scale[2] = {&a.k_scale, &a.v_scale};
+  p.src[0] = static_cast<const uint8_t*>(a.key);
+  p.src[1] = static_cast<const uint8_t*>(a.value);
+  p.src_stride_token[0] = a.key_stride_token;
+  p.src_stride_token[1] = a.value_stride_token;
+  p.src_stride_head[0] = a.key_stride_head;
+  p.src_stride_head[1] = a.value_stride_head;
+  bool wide = true;
+  for (int i = 0; i < 2; ++i) {
+    p.cache[i] = static_cast<uint8_t*>(const_cast<void*>(cache[i]->data));
+    p.stride_block[i] = cache[i]->stride_block;
+    p.stride_slot[i] = cache[i]->stride_slot;
+    p.stride_head[i] = cache[i]->stride_head;
+    p.scale[i] = static_cast<float*>(const_cast<void*>(scale[i]->data));
+    p.scale_stride_block[i] = scale[i]->stride_block / 4;
+    p.scale_stride_group[i] = scale[i]->stride_slot / 4;
+    p.scale_stride_head[i] = scale[i]->stride_head / 4;
+    wide = wide && reinterpret_cast<uintptr_t>(p.src[i]) % 16 == 0 && p.src_stride_token[i] % 16 == 0 && p.src_stride_head[i] % 16 == 0;
+  }
+  p.block_table = a.block_table;
+  p.block_table_row_stride = a.block_table_row_stride;
+  p.seq_lens = a.seq_lens;
+  p.query_start_loc = a.query_start_loc;
+  p.num_blocks = a.num_blocks;
+  p.block_size = a.block_size;
+  p.scale_tokens = a.scale_tokens;
+  p.num_kv_heads = a.num_kv_heads;
+  p.num_reqs = a.num_reqs;
+  p.num_tokens = a.num_tokens;
+  p.num_pages = a.num_pages;
+  p.max_query_len = a.max_query_len;
+  p.src_dtype = a.src_dtype;
+  switch (a.head_size) {
+    case 64:
+      return launch_type<64>(p, wide, stream);
+    case 128:
+      return launch_type<128>(p, wide, stream);
+    default:
+      return launch_type<256>(p, wide, stream);
+  }
+}
+
+}  // namespace pthb200

@@ -11,8 +11,8 @@ metadata checks of the C++ op in the same order with the same messages, so a bad
 call fails at trace time with the reason it would fail with at run time.  Checks
 that need addresses or a device stay in C++.
 
-The ops of the 16-bit paged cache (:mod:`.kv16`) come from the same library and are
-reached from here too.
+The ops of the 16-bit and of the 8-bit paged cache (:mod:`.kv16`, :mod:`.kv8`, with rotary positions) come from the
+same library and are reached from here too.
 
 This module makes no ``torch.cuda`` call.
 """
@@ -24,8 +24,10 @@ from pathlib import Path
 
 import torch
 
-from . import kv16
+from . import kv16, kv8
 from .kv16 import kv16_cross_attention, kv16_decode_attention, kv16_write, page_tables  # noqa: F401
+from .kv8 import (kv8_attention, kv8_decode_attention, kv8_read, kv8_write, rotary,  # noqa: F401
+                  rotary_frequencies)
 
 OP_NAMESPACE = "pth_flash_attn"
 OP_NAME = "pth_flash_attn_fwd"
@@ -223,6 +225,7 @@ def _load_library() -> bool:
     torch.library.register_fake(OP_QUALNAME)(pth_flash_attn_fwd_fake)
     torch.library.register_fake(LSE_OP_QUALNAME)(pth_flash_attn_fwd_lse_fake)
     kv16.register()
+    kv8.register()
     return True
 
 
