@@ -93,8 +93,8 @@ struct PieceQueue {
 };
 
 // The scheduling warp: the pieces of `walk`, and the end.  never: a barrier that nothing arrives on.
-template <bool kHeld, class Walk>
-__device__ __forceinline__ void put_pieces(const Kv16Params& p, Walk& walk, PieceQueue& queue, uint64_t* never, volatile int* abort_flag) {
+template <bool kHeld, class Params, class Walk>
+__device__ __forceinline__ void put_pieces(const Params& p, Walk& walk, PieceQueue& queue, uint64_t* never, volatile int* abort_flag) {
   Piece it;
   while (walk.next(p, &it)) {
     if (kv16_held<kHeld>(p, kHeldSchedule, queue.i)) kv16_wait(never, 0, abort_flag);

@@ -39,6 +39,11 @@ __device__ __forceinline__ float2 float2_of_e4m3x2(uint32_t w) {
   const uint32_t h = f16x2_of_e4m3x2(w);
   return __half22float2(*reinterpret_cast<const __half2*>(&h));
 }
+// Exponent of the smallest power of two with x <= 448 times it (448 = 1.75 x 2^8; x normal or zero).
+__device__ __forceinline__ int e4m3_exponent(float x) {
+  const uint32_t bits = __float_as_uint(x);
+  return (int)(bits >> 23) - 127 - 8 + ((bits & 0x7fffffu) > 0x600000u ? 1 : 0);
+}
 // 2^e, e in [-126, 127].
 __device__ __forceinline__ float power_of_two(int e) { return __uint_as_float((uint32_t)(e + 127) << 23); }
 
@@ -97,6 +102,9 @@ __device__ __forceinline__ void place_piece(Piece* out, const ReqShape8& s) { ou
 // kv8_short_kernel.cu
 int64_t kv8_short_workspace_bytes(int head_size, int num_sms);
 cudaError_t launch_kv8_short(const Kv8Params& p, cudaStream_t stream);
+// kv8_tall_kernel.cu.  *taken: whether the cache's view can be read by TMA boxes; if not, nothing has been launched.
+int64_t kv8_tall_workspace_bytes(int head_size, int num_sms);
+cudaError_t launch_kv8_tall(const Kv8Params& p, cudaStream_t stream, bool* taken);
 // kv8_writer_kernel.cu, kv8_reader_kernel.cu, rotary_kernel.cu
 cudaError_t launch_kv8_writer(const PthB200Kv8WriteArgs& a, cudaStream_t stream);
 cudaError_t launch_kv8_reader(const PthB200Kv8ReadArgs& a, cudaStream_t stream);

@@ -142,7 +142,12 @@ int32_t build(const PthB200Kv8Args* a, bool decode, Kv8Params* p) {
   return PTH_ATTN_OK;
 }
 
-int64_t workspace_bytes(int head_size, int num_sms) { return kv8_short_workspace_bytes(head_size, num_sms); }
+// Rows (query tokens x G) from which a launch of more than one token goes to the kernel with the rows on the MMA's M dimension.
+constexpr int64_t kTallRows = 33;
+
+int64_t workspace_bytes(int head_size, int num_sms) {
+  return std::max(kv8_short_workspace_bytes(head_size, num_sms), kv8_tall_workspace_bytes(head_size, num_sms));
+}
 
 int32_t attention(const PthB200Kv8Args* a, bool decode, void* stream) {
   clear_error();
@@ -154,6 +159,11 @@ int32_t attention(const PthB200Kv8Args* a, bool decode, void* stream) {
     return set_error(PTH_ATTN_ECUDA, "cannot query the current device");
   const int64_t need = workspace_bytes(a->head_size, sms);
   KV8_REQUIRE(a->workspace_bytes >= need, "workspace has " + std::to_string(a->workspace_bytes) + " bytes, " + std::to_string(need) + " are needed");
+  if ((int64_t)p.max_query_len * p.group >= kTallRows && p.max_query_len > 1) {
+    bool taken = false;
+    const int32_t rc = launched(launch_kv8_tall(p, static_cast<cudaStream_t>(stream), &taken), "attention");
+    if (rc != PTH_ATTN_OK || taken) return rc;
+  }
   return launched(launch_kv8_short(p, static_cast<cudaStream_t>(stream)), "attention");
 }
 

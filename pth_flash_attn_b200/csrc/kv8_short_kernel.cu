@@ -63,7 +63,7 @@ struct Geo8 {
   static constexpr int fit = ctas == 2 ? units2 : (232448 - fixed - 128) / unit;
   static constexpr int units = fit < most ? fit : most;
   static_assert(units >= 3, "K and V of a tile, and the next K");
-  // Registers that the copies hand to the softmax from what a thread starts with (168 with one CTA per SM, 96 with two).
+  // Registers that the copies hand to the softmax from what a thread starts with (launch_one asks; 168 with one CTA per SM, 96 with two).
   static constexpr int softmax_regs = ctas == 1 ? 232 : 128, copy_regs = ctas == 1 ? 72 : 64, start_regs = ctas == 1 ? 168 : 96;
   static_assert(4 * softmax_regs + 4 * copy_regs <= 8 * start_regs, "a split that the launch holds");
   static constexpr int s_col = 0, o_col = 2 * cols;  // TMEM columns: S twice, O of every part
@@ -617,7 +617,10 @@ cudaError_t launch_one(const Kv8Params& p, cudaStream_t stream) {
   cudaError_t err = cudaGetDevice(&dev);
   if (err != cudaSuccess) return err;
   if (dev < 0 || dev >= 64 || !configured[dev]) {
-    err = cudaFuncSetAttribute(kv8_short_kernel<HD, RP, kHalf>, cudaFuncAttributeMaxDynamicSharedMemorySize, G::total);
+    cudaFuncAttributes attr;
+    err = cudaFuncGetAttributes(&attr, kv8_short_kernel<HD, RP, kHalf>);
+    if (err == cudaSuccess && attr.numRegs < G::start_regs) err = cudaErrorInvalidConfiguration;   // (setmaxnreg would wait without end)
+    if (err == cudaSuccess) err = cudaFuncSetAttribute(kv8_short_kernel<HD, RP, kHalf>, cudaFuncAttributeMaxDynamicSharedMemorySize, G::total);
     if (err != cudaSuccess) return err;
     if (dev >= 0 && dev < 64) configured[dev] = true;
   }

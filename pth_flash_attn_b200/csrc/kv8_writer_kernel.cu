@@ -79,12 +79,7 @@ __device__ __forceinline__ float finite_max(const float (&x)[8]) {
   return m;
 }
 // The smallest power of two, 2^-126 to 2^120, with most <= 448 times it.
-__device__ __forceinline__ float needed_scale(float most) {
-  const uint32_t bits = __float_as_uint(most);
-  // 448 = 1.75 x 2^8: the exponent less 8, one more where the significand is above 1.75
-  const int e = (int)(bits >> 23) - 127 - 8 + ((bits & 0x7fffffu) > 0x600000u ? 1 : 0);
-  return power_of_two(min(120, max(-126, e)));
-}
+__device__ __forceinline__ float needed_scale(float most) { return power_of_two(min(120, max(-126, e4m3_exponent(most)))); }
 // Eight numbers as cells, x / scale: exactly scaled where the scale is a power of two.
 __device__ __forceinline__ uint2 cells8(const float (&x)[8], float scale) {
   float y[8];
