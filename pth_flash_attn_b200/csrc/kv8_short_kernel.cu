@@ -43,24 +43,33 @@ constexpr int kRun = 16;               // keys that surely share a scale
 constexpr int kScaleTiles = 16;        // tiles whose scales are kept: more than the ring holds units of either kind, and two
 constexpr int kDigitsY = 3;
 
-// Column block c of 16 dims: 128 keys x 16 bytes.  (16 bytes more than they take: a warp's copies go to all banks.)
-constexpr int kColumn = kTile * 16 + 16;
+// A unit is 128 rows, of a key each, of up to 128 bytes, in the swizzle of its rows' length (128 or 64 bytes): a row's 16-byte pieces stay
+// together.  (In column blocks of 16 dims, a row's pieces 2,064 bytes apart and on banks of their own, 64
+// requests x 8,192 keys of 8 heads took 307 us instead of 175: copies of 16 bytes to eight lines of shared memory move half as fast.)
+template <int kDims>
+__device__ __forceinline__ uint32_t swizzled_chunk(int row, int chunk) {   // where piece `chunk` of a row lies
+  return kDims == 128 ? (uint32_t)(chunk ^ (row & 7)) : (uint32_t)(chunk ^ ((row >> 1) & 3));
+}
+template <int kDims>
+__device__ __forceinline__ uint64_t unit_desc(uint32_t saddr, uint32_t lbo) {   // either major: the next 8 rows follow
+  return tc::smem_desc(saddr, lbo, 8 * kDims) | (uint64_t)(kDims == 128 ? 2 : 4) << 61;
+}
 
 template <int HD, int RP, bool kHalf>
 struct Geo8 {
   static constexpr int dims = HD < 128 ? HD : 128;   // of a unit
   static constexpr int parts = HD / dims;            // units of a tile's K, and of its V
-  static constexpr int unit = dims / 16 * kColumn;
+  static constexpr int unit = kTile * dims;
   static constexpr int q_digits = kHalf ? 3 : 2;
   static constexpr int cols = (q_digits * RP + 15) / 16 * 16;     // N of QK
   static constexpr int pcols = (kDigitsY * RP + 15) / 16 * 16;    // N of PV
   static constexpr int qimage = cols * HD;           // column block c of 16 dims at c (cols 16), column n at n 16
   static constexpr int pimage = pcols * kTile;       // block of 16 columns at 2,048 each, key t at t 16
   static constexpr int fixed = 2 * qimage + pimage + 3 * 4 * RP * 4 + 2 * RP * 4 + kScaleTiles * 64 + 1024;
-  static constexpr int units2 = (115712 - fixed - 128) / unit;
+  static constexpr int units2 = (115712 - fixed - 1024) / unit;
   static constexpr int ctas = units2 >= 3 && RP <= 16 ? 2 : 1;
   static constexpr int most = 2 * (kScaleTiles - 3);   // (see kScaleTiles)
-  static constexpr int fit = ctas == 2 ? units2 : (232448 - fixed - 128) / unit;
+  static constexpr int fit = ctas == 2 ? units2 : (232448 - fixed - 1024) / unit;
   static constexpr int units = fit < most ? fit : most;
   static_assert(units >= 3, "K and V of a tile, and the next K");
   // Registers that the copies hand to the softmax from what a thread starts with (launch_one asks; 168 with one CTA per SM, 96 with two).
@@ -70,7 +79,7 @@ struct Geo8 {
   static constexpr int tmem_need = 2 * cols + parts * pcols;
   static constexpr int tmem = tmem_need <= 64 ? 64 : tmem_need <= 128 ? 128 : tmem_need <= 256 ? 256 : 512;
   static_assert(tmem_need <= 512 && tmem * ctas <= 512, "the SM's columns");
-  // shared memory
+  // shared memory, behind the first 1,024-byte boundary
   static constexpr int q = units * unit;
   static constexpr int p = q + 2 * qimage;
   static constexpr int wmax = p + pimage;            // float [4 warps][RP]
@@ -82,8 +91,7 @@ struct Geo8 {
   static constexpr int bars = pieces + kQueue * 64;
   static constexpr int n_bars = 2 * units + 2 + 2 + 2 + 1 + 1 + 2 * kQueue + 1;
   static constexpr int misc = bars + n_bars * 8;     // ints: abort flag, TMEM address, arrival, stop; scratch of find_run
-  static constexpr int end = misc + 160, last64 = HD == 64 ? units * unit + 4 * kColumn : 0;   // (PV reads 64 rows past a unit of 64 dims)
-  static constexpr int total = (end > last64 ? end : last64) + 128;
+  static constexpr int total = misc + 160 + 1024;
   static_assert(kQueue * 64 + n_bars * 8 + 160 <= 1024, "fixed part");
 };
 
@@ -105,17 +113,17 @@ __device__ __forceinline__ void digits2(float a, float b, uint32_t (&d)[kDigits]
   }
 }
 
-// The 32 keys of a warp, from `base_key` of a tile on: rows of `kDims` bytes from off (the lane's key's) into a unit's column blocks.
+// The 32 keys of a warp, from `base_key` of a tile on: rows of `kDims` bytes from off (the lane's key's) into a unit.
 template <int kDims>
 __device__ __forceinline__ void copy_keys8(uint32_t unit, int base_key, const uint8_t* src, long long off) {
   constexpr int kChunks = kDims / 16, kRows = 32 / kChunks;
   const int lane = threadIdx.x & 31, chunk = lane % kChunks, sub = lane / kChunks;
-  const uint32_t dst = unit + chunk * kColumn + base_key * 16;
+  const uint32_t dst = unit + base_key * kDims;
 #pragma unroll
   for (int i = 0; i < 32 / kRows; ++i) {
     const int row = i * kRows + sub;
     const long long o = __shfl_sync(0xffffffffu, off, row);
-    copy16(dst + row * 16, o >= 0 ? src + o + chunk * 16 : src, o >= 0);
+    copy16(dst + row * kDims + (swizzled_chunk<kDims>(row, chunk) << 4), o >= 0 ? src + o + chunk * 16 : src, o >= 0);
   }
 }
 // Asynchronous copy of four bytes, or of none: then the destination is zeroed.
@@ -195,7 +203,7 @@ template <int HD, int RP, bool kHalf>
 __global__ void __launch_bounds__(kThreads, (Geo8<HD, RP, kHalf>::ctas)) kv8_short_kernel(const __grid_constant__ Kv8Params p) {
   using G = Geo8<HD, RP, kHalf>;
   extern __shared__ uint8_t smem_raw[];
-  uint8_t* const smem = smem_raw + ((128u - (tc::smem_u32(smem_raw) & 127u)) & 127u);
+  uint8_t* const smem = smem_raw + ((1024u - (tc::smem_u32(smem_raw) & 1023u)) & 1023u);
   uint64_t* const full = reinterpret_cast<uint64_t*>(smem + G::bars);
   uint64_t* const empty = full + G::units;
   uint64_t* const bars = empty + G::units;
@@ -330,7 +338,7 @@ __global__ void __launch_bounds__(kThreads, (Geo8<HD, RP, kHalf>::ctas)) kv8_sho
           tc::fence_after_sync();
 #pragma unroll
           for (int kk = 0; kk < G::dims / 32; ++kk) {
-            const uint64_t a = tc::smem_desc(ring + s * G::unit + kk * 2 * kColumn, kColumn, 128);
+            const uint64_t a = unit_desc<G::dims>(ring + s * G::unit + kk * 32, 16);
             const uint64_t b = tc::smem_desc(q_s + (item & 1) * G::qimage + (part * (G::dims / 16) + kk * 2) * (G::cols * 16), G::cols * 16, 128);
             mma_e4m3(tmem_base + G::s_col + (tile & 1) * G::cols, a, b, qk_desc, part > 0 || kk > 0);
           }
@@ -356,8 +364,8 @@ __global__ void __launch_bounds__(kThreads, (Geo8<HD, RP, kHalf>::ctas)) kv8_sho
           tc::fence_after_sync();
 #pragma unroll
           for (int kk = 0; kk < kTile / 32; ++kk) {
-            // (64 dims: the instruction's other 64 rows are what follows the unit, which nothing reads)
-            const uint64_t a = tc::smem_desc(ring + s * G::unit + kk * 512, 128, kColumn);
+            // (64 dims: the instruction's other 64 rows are the same bytes again, which nothing reads)
+            const uint64_t a = unit_desc<G::dims>(ring + s * G::unit + kk * 32 * G::dims, 0);
             const uint64_t b = tc::smem_desc(p_s + kk * 512, 128, kTile * 16);
             mma_e4m3(tmem_base + G::o_col + part * G::pcols, a, b, pv_desc, !first_of_item || kk > 0);
           }
