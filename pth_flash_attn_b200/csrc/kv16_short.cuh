@@ -176,13 +176,13 @@ __device__ __forceinline__ float* partial_slot(const Kv16Params& p, int cta, boo
 // Merges the pieces of a row tile, left by the CTAs of groups g0 .. g0 + pieces - 1, and writes its rows: a warp per row, a lane per
 // four columns.  The statistics and columns of eight pieces (four at 256 dims) are loaded together; the running sums are rescaled when a later piece has the
 // larger ref.
-template <int HD, int RP, bool kHalf>
+template <int HD, int RP, bool kHalf, int kWarps = 4>
 __device__ __forceinline__ void merge_pieces(const Kv16Params& p, const Piece& it, int kvh, int g0, int pieces, int heads, int hslot) {
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   constexpr int kVec = HD >= 128 ? HD / 128 : 1, kBatch = 8 / kVec;
   const int d0 = (HD == 64 ? lane & 15 : lane) * 4;
 #pragma unroll 1
-  for (int n = warp; n < it.rows; n += 4) {
+  for (int n = warp; n < it.rows; n += kWarps) {
     float top = -INFINITY, l = 0.f, acc[kVec][4];
 #pragma unroll
     for (int v = 0; v < kVec; ++v) acc[v][0] = acc[v][1] = acc[v][2] = acc[v][3] = 0.f;

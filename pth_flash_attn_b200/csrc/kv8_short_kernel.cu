@@ -9,9 +9,9 @@
 // Digits.  An MMA of this kind takes 8-bit numbers on both sides, so a factor of B goes in as a sum of e4m3 numbers, side by
 // side on N, each with an accumulator of its own: x = u (d0 + d1 / 16 + d2 / 256), every digit the rounding of what is left.  Digits have
 // four bits, and subnormal ones a step of 2^-9, so n digits keep 4 n bits of numbers down to 2^-14 of the largest, and are off by
-// 2^-(14 + 4 n) of it below.  bf16 queries take two (they are exact), fp16 queries three, Y three: its 2^-12 is an eighth of the
-// rounding of a bf16 output, and a key of 2^-25 of its row's largest weight still counts, over 131,072 keys.  At eight rows and
-// 16 or 32 columns they cost the tensor core nothing that shows.
+// 2^-(14 + 4 n) of it below.  bf16 queries take two (they are exact), fp16 queries three.  Y is rounded to fp16, which three digits
+// hold: 2^-11 of a weight is an eighth of the rounding of a bf16 output, and a key of 2^-24 of its row's largest weight still
+// counts, over 131,072 keys.  At eight rows and 16 or 32 columns they cost the tensor core nothing that shows.
 //   u is a power of two per row for Q (its largest into [128, 256)).  For Y it is U, the largest scale_V so far in the piece, to the
 // next power of two: the accumulators are rescaled where a tile brings a larger one.  scale_K multiplies a key's scores.
 //
@@ -35,10 +35,8 @@ __device__ unsigned int g_kv8_short_status = 0;
 
 namespace {
 
-constexpr int kLoadWarp = 4;           // warps 4-7
-constexpr int kMmaWarp = 8, kScheduleWarp = 9;
-constexpr int kThreads = 320;
 constexpr float kGainY = 6.f, kSlackY = 2.f;
+constexpr float kUnset = -1e30f;       // ref of a row that has seen no key: below every score, finite so that a hidden one gives P = 0
 constexpr int kRun = 16;               // keys that surely share a scale
 constexpr int kScaleTiles = 16;        // tiles whose scales are kept: more than the ring holds units of either kind, and two
 constexpr int kDigitsY = 3;
@@ -61,20 +59,25 @@ struct Geo8 {
   static constexpr int parts = HD / dims;            // units of a tile's K, and of its V
   static constexpr int unit = kTile * dims;
   static constexpr int q_digits = kHalf ? 3 : 2;
+  // Softmax warpgroups, which share the rows out among themselves; thread t of each is key t of a tile, then dim t of the output.
+  static constexpr int groups = RP == 8 ? 1 : 2;
+  static constexpr int rows = RP / groups;           // of a group
+  static constexpr int load_warp = 4 * groups, mma_warp = load_warp + 4, schedule_warp = mma_warp + 1, threads = (schedule_warp + 1) * 32;
   static constexpr int cols = (q_digits * RP + 15) / 16 * 16;     // N of QK
   static constexpr int pcols = (kDigitsY * RP + 15) / 16 * 16;    // N of PV
   static constexpr int qimage = cols * HD;           // column block c of 16 dims at c (cols 16), column n at n 16
   static constexpr int pimage = pcols * kTile;       // block of 16 columns at 2,048 each, key t at t 16
-  static constexpr int fixed = 2 * qimage + pimage + 3 * 4 * RP * 4 + 2 * RP * 4 + kScaleTiles * 64 + 1024;
+  static constexpr int fixed = 2 * qimage + pimage + 9 * RP * 4 + 2 * RP * 4 + kScaleTiles * 64 + 1024;
   static constexpr int units2 = (115712 - fixed - 1024) / unit;
   static constexpr int ctas = units2 >= 3 && RP <= 16 ? 2 : 1;
   static constexpr int most = 2 * (kScaleTiles - 3);   // (see kScaleTiles)
   static constexpr int fit = ctas == 2 ? units2 : (232448 - fixed - 1024) / unit;
   static constexpr int units = fit < most ? fit : most;
   static_assert(units >= 3, "K and V of a tile, and the next K");
-  // Registers that the copies hand to the softmax from what a thread starts with (launch_one asks; 168 with one CTA per SM, 96 with two).
-  static constexpr int softmax_regs = ctas == 1 ? 232 : 128, copy_regs = ctas == 1 ? 72 : 64, start_regs = ctas == 1 ? 168 : 96;
-  static_assert(4 * softmax_regs + 4 * copy_regs <= 8 * start_regs, "a split that the launch holds");
+  // Registers that the copies hand to the softmax from what a thread starts with (launch_one asks).
+  static constexpr int start_regs = RP == 8 ? 96 : ctas == 2 ? 72 : 128;
+  static constexpr int copy_regs = RP != 8 && ctas == 2 ? 40 : 64, softmax_regs = RP == 8 ? 112 : ctas == 2 ? 88 : 160;
+  static_assert(4 * groups * softmax_regs + 4 * copy_regs <= (4 * groups + 4) * start_regs, "a split that the launch holds");
   static constexpr int s_col = 0, o_col = 2 * cols;  // TMEM columns: S twice, O of every part
   static constexpr int tmem_need = 2 * cols + parts * pcols;
   static constexpr int tmem = tmem_need <= 64 ? 64 : tmem_need <= 128 ? 128 : tmem_need <= 256 ? 256 : 512;
@@ -82,10 +85,10 @@ struct Geo8 {
   // shared memory, behind the first 1,024-byte boundary
   static constexpr int q = units * unit;
   static constexpr int p = q + 2 * qimage;
-  static constexpr int wmax = p + pimage;            // float [4 warps][RP]
-  static constexpr int wsum = wmax + 4 * RP * 4;     // float [4 warps][RP]
+  static constexpr int wmax = p + pimage;            // float [groups][4 warps][rows]
+  static constexpr int wsum = wmax + 4 * RP * 4;     // float [groups][4 warps][rows]
   static constexpr int at = wsum + 4 * RP * 4;       // int [RP]: positions of the piece's rows
-  static constexpr int qfactor = at + 4 * RP * 4;    // float [2][RP]: a row's u x softmax scale x log2(e)
+  static constexpr int qfactor = at + RP * 4;    // float [2][RP]: a row's u x softmax scale x log2(e)
   static constexpr int scales = qfactor + 2 * RP * 4;   // [kScaleTiles][2][8]: of the keys, of the values
   static constexpr int pieces = scales + kScaleTiles * 64;   // PieceQueue's entries
   static constexpr int bars = pieces + kQueue * 64;
@@ -99,6 +102,22 @@ struct Bars8 {  // offsets behind [units] full, [units] empty
   static constexpr int q_full = 0, q_empty = 2, s_ready = 4, p_ready = 6, pv_done = 7, queue = 8, drained = queue + 2 * kQueue;
 };
 
+// Barrier of a softmax warpgroup that tells whether any of its threads has seen `x`.
+__device__ __forceinline__ bool group_any(int wg, bool x) {
+  uint32_t r;
+  asm volatile(
+      "{\n\t"
+      ".reg .pred p, q;\n\t"
+      "setp.ne.u32 p, %1, 0;\n\t"
+      "barrier.cta.red.or.pred q, %2, 128, p;\n\t"
+      "selp.u32 %0, 1, 0, q;\n\t"
+      "}\n"
+      : "=r"(r)
+      : "r"((uint32_t)x), "r"(1 + wg)
+      : "memory");
+  return r != 0;
+}
+
 // Two numbers' digits, the first in the low byte: d0 = round(x), d1 = round(16 (x - d0)), d2 = round(256 (x - d0 - d1 / 16)).
 template <int kDigits>
 __device__ __forceinline__ void digits2(float a, float b, uint32_t (&d)[kDigits]) {
@@ -109,6 +128,22 @@ __device__ __forceinline__ void digits2(float a, float b, uint32_t (&d)[kDigits]
       const float2 f = float2_of_e4m3x2(d[i]);
       a = (a - f.x) * 16.f;
       b = (b - f.y) * 16.f;
+    }
+  }
+}
+
+// Two weights' digits, the first in the low byte: of their rounding to fp16, whose 11 bits three digits hold.
+__device__ __forceinline__ void weight_digits2(float a, float b, uint32_t (&d)[kDigitsY]) {
+  __half2 h = __floats2half2_rn(a, b);
+#pragma unroll
+  for (int i = 0; i < kDigitsY; ++i) {
+    uint16_t r;
+    asm("cvt.rn.satfinite.e4m3x2.f16x2 %0, %1;" : "=h"(r) : "r"(*reinterpret_cast<const uint32_t*>(&h)));
+    d[i] = r;
+    if (i + 1 < kDigitsY) {
+      const uint32_t f = f16x2_of_e4m3x2(r);
+      const __half2 sixteen = __float2half2_rn(16.f);
+      h = __hfma2(*reinterpret_cast<const __half2*>(&f), __float2half2_rn(-16.f), __hmul2(h, sixteen));   // (exact)
     }
   }
 }
@@ -194,13 +229,13 @@ __device__ __forceinline__ void stage_queries(const Kv8Params& p, const Piece& i
 #pragma unroll
       for (int g = 0; g < G::q_digits; ++g)
         *reinterpret_cast<uint2*>(to + g * (RP * 16)) = make_uint2(d[0][g] | d[1][g] << 16, d[2][g] | d[3][g] << 16);
-      if (chunk == 0) factor[n] = isinf(top) || isnan(top) ? NAN : power_of_two(e) * p.scale_log2;
+      if (chunk == 0) factor[n] = isinf(top) ? NAN : fmaxf(power_of_two(e) * p.scale_log2, 1e-37f);   // (never zero: hidden scores are -inf)
     }
   }
 }
 
 template <int HD, int RP, bool kHalf>
-__global__ void __launch_bounds__(kThreads, (Geo8<HD, RP, kHalf>::ctas)) kv8_short_kernel(const __grid_constant__ Kv8Params p) {
+__global__ void __launch_bounds__((Geo8<HD, RP, kHalf>::threads), (Geo8<HD, RP, kHalf>::ctas)) kv8_short_kernel(const __grid_constant__ Kv8Params p) {
   using G = Geo8<HD, RP, kHalf>;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* const smem = smem_raw + ((1024u - (tc::smem_u32(smem_raw) & 1023u)) & 1023u);
@@ -213,7 +248,7 @@ __global__ void __launch_bounds__(kThreads, (Geo8<HD, RP, kHalf>::ctas)) kv8_sho
   int* const stop = arrival + 1;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
 
-  if (warp == kMmaWarp) {
+  if (warp == G::mma_warp) {
     if (lane == 0) {
       for (int i = 0; i < G::units; ++i) {
         tc::mbar_init(&full[i], 128);
@@ -221,13 +256,13 @@ __global__ void __launch_bounds__(kThreads, (Geo8<HD, RP, kHalf>::ctas)) kv8_sho
       }
       for (int i = 0; i < 2; ++i) {
         tc::mbar_init(&bars[Bars8::q_full + i], 1);
-        tc::mbar_init(&bars[Bars8::q_empty + i], 2);   // the last QK has read the digits, the softmax the factors
+        tc::mbar_init(&bars[Bars8::q_empty + i], 1 + G::groups);   // the last QK has read the digits, the softmax the factors
         tc::mbar_init(&bars[Bars8::s_ready + i], 2);   // the MMAs are complete; this warp has seen the tile's scales land
       }
-      tc::mbar_init(&bars[Bars8::p_ready], kSoftmaxThreads);
+      tc::mbar_init(&bars[Bars8::p_ready], kSoftmaxThreads * G::groups);
       tc::mbar_init(&bars[Bars8::pv_done], 1);
       tc::mbar_init(&bars[Bars8::drained], 1);
-      PieceQueue(nullptr, &bars[Bars8::queue], stop).init(kThreads / 32 - 1);
+      PieceQueue(nullptr, &bars[Bars8::queue], stop).init(G::threads / 32 - 1);
       *abort_flag = 0;
       tc::mbar_init_fence();
     }
@@ -236,7 +271,7 @@ __global__ void __launch_bounds__(kThreads, (Geo8<HD, RP, kHalf>::ctas)) kv8_sho
     tc::tmem_relinquish();
   }
   pdl_wait();
-  ShortWalk<RP, Kv8Params> walk = find_run<RP, kThreads>(p, reinterpret_cast<long long*>(smem + G::misc + 16));
+  ShortWalk<RP, Kv8Params> walk = find_run<RP, G::threads>(p, reinterpret_cast<long long*>(smem + G::misc + 16));
   tc::fence_before_sync();
   __syncthreads();
   tc::fence_after_sync();
@@ -245,7 +280,7 @@ __global__ void __launch_bounds__(kThreads, (Geo8<HD, RP, kHalf>::ctas)) kv8_sho
   float* const qfactor = reinterpret_cast<float*>(smem + G::qfactor);
   bool ok = true;
 
-  if (warp == kScheduleWarp) {
+  if (warp == G::schedule_warp) {
     // =========================== schedule and queries ============================
     Piece it;
     uint32_t item = 0;
@@ -266,11 +301,11 @@ __global__ void __launch_bounds__(kThreads, (Geo8<HD, RP, kHalf>::ctas)) kv8_sho
       it.tiles = 0;
       queue.put(it, abort_flag);
     }
-  } else if (warp >= kLoadWarp && warp < kMmaWarp) {
+  } else if (warp >= G::load_warp && warp < G::mma_warp) {
     // =========================== copies ==========================================
     // A warp owns 32 keys of every tile: lane l knows where key l of them lies.
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(G::copy_regs));
-    const int base_key = (warp - kLoadWarp) * 32;
+    const int base_key = (warp - G::load_warp) * 32;
     const uint32_t ring = tc::smem_u32(smem), scales = tc::smem_u32(smem + G::scales);
     uint32_t unit = 0, tile = 0;
     auto next_unit = [&]() -> uint32_t {
@@ -315,7 +350,7 @@ __global__ void __launch_bounds__(kThreads, (Geo8<HD, RP, kHalf>::ctas)) kv8_sho
       }
     }
     copies_wait_all();
-  } else if (warp == kMmaWarp) {
+  } else if (warp == G::mma_warp) {
     // =========================== MMAs ============================================
     // QK of a tile is issued ahead of PV of the one before, in the order in which the units arrive.
     constexpr uint32_t qk_desc = instr_desc_e4m3(128, G::cols, 0, 0);
@@ -387,136 +422,141 @@ __global__ void __launch_bounds__(kThreads, (Geo8<HD, RP, kHalf>::ctas)) kv8_sho
       }
     }
     if (pending) pv(pending_first);
-  } else if (warp < kLoadWarp) {
+  } else {
     // =========================== softmax =========================================
     asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(G::softmax_regs));
-    const uint32_t lane_addr = (uint32_t)(warp * 32) << 16;
-    float* const wmax = reinterpret_cast<float*>(smem + G::wmax);
-    float* const wsum = reinterpret_cast<float*>(smem + G::wsum);
-    int* const row_at = reinterpret_cast<int*>(smem + G::at);
-    uint8_t* const p_img = smem + G::p + tid * 16;
+    constexpr int RW = G::rows;
+    const int wg = warp >> 2, key = tid & 127, row_base = wg * RW;
+    const uint32_t lane_addr = (uint32_t)((warp & 3) * 32) << 16;
+    float* const wmax = reinterpret_cast<float*>(smem + G::wmax) + 4 * row_base;
+    float* const wsum = reinterpret_cast<float*>(smem + G::wsum) + 4 * row_base;
+    int* const row_at = reinterpret_cast<int*>(smem + G::at) + row_base;
+    uint8_t* const p_img = smem + G::p + key * 16;
+    auto group_sync = [&] { named_barrier(1 + wg, kSoftmaxThreads); };
+    auto all_sync = [&] { named_barrier(1 + G::groups, kSoftmaxThreads * G::groups); };
     uint32_t tile = 0, item = 0;
-    zero_requests<HD, RP, kSoftmaxThreads>(p);
+    zero_requests<HD, RP, kSoftmaxThreads * G::groups>(p);
     {
       const int heads = min(p.num_kv_heads, (int)gridDim.x), hslot = (int)blockIdx.x % heads;
       Piece it;
       while (queue.get(&it, abort_flag)) {
-        const int kvh = it.kvh;
+        const int kvh = it.kvh, rows = it.rows - row_base;   // of the group: RW or fewer, or none
         ok &= kv16_wait(&bars[Bars8::q_full + (item & 1)], (item >> 1) & 1, abort_flag);
-        const float* const factor = qfactor + (item & 1) * RP;
+        const float* const factor = qfactor + (item & 1) * RP + row_base;
         // rows of several tokens: keys that some of them see and others do not, [.., mask_lo) and [mask_hi, ..)
         int mask_lo = 0, mask_hi = INT_MAX;
         if (p.query_start_loc != nullptr) {
           if (p.causal) mask_hi = it.pos0 + it.row0 / p.group + 1;
           mask_lo = kv8_low(p, it.pos0 + (it.row0 + it.rows - 1) / p.group);
-          if (tid < RP) row_at[tid] = it.pos0 + (it.row0 + min(tid, it.rows - 1)) / p.group;
-          softmax_sync();
+          if (key < RW) row_at[key] = it.pos0 + (it.row0 + min(row_base + key, it.rows - 1)) / p.group;
+          group_sync();
         }
-        float ref[RP], l[RP];
+        float ref[RW], l[RW];
         int unit_e = -126;   // U = 2^unit_e
 #pragma unroll
-        for (int n = 0; n < RP; ++n) {
-          ref[n] = -INFINITY;
+        for (int n = 0; n < RW; ++n) {
+          ref[n] = kUnset;
           l[n] = 0.f;
         }
         for (int t = 0; t < it.tiles; ++t, ++tile) {
           ok &= kv16_wait(&bars[Bars8::s_ready + (tile & 1)], (tile >> 1) & 1, abort_flag);
           tc::fence_after_sync();
-          uint32_t sr[G::cols];
-          tmem_load<G::cols>(tmem_base + G::s_col + (tile & 1) * G::cols + lane_addr, sr);
-          tc::tmem_ld_wait<G::cols>(sr);
+          uint32_t sr[G::q_digits][RW];
+#pragma unroll
+          for (int g = 0; g < G::q_digits; ++g) tmem_load<RW>(tmem_base + G::s_col + (tile & 1) * G::cols + g * RP + row_base + lane_addr, sr[g]);
           const float* const scale = reinterpret_cast<const float*>(smem + G::scales + (tile % kScaleTiles) * 64);
-          const float k_scale = scale[tid / kRun], v_scale = scale[8 + tid / kRun];
+          const float k_scale = scale[key / kRun], v_scale = scale[8 + key / kRun];
           float most = 0.f;
 #pragma unroll
           for (int i = 0; i < 8; ++i) most = fmaxf(most, fabsf(scale[8 + i]));
-          const int pos = it.key0 + t * kTile + tid;
-          float s[RP];
+          tc::tmem_ld_wait();
 #pragma unroll
-          for (int n = 0; n < RP; ++n) {
-            float x = fmaf(__uint_as_float(sr[RP + n]), 0.0625f, __uint_as_float(sr[n]));
-            if constexpr (G::q_digits == 3) x = fmaf(__uint_as_float(sr[2 * RP + n]), 0.00390625f, x);
-            s[n] = x * k_scale * factor[n];
+          for (int g = 0; g < G::q_digits; ++g) tc::tmem_landed<RW>(sr[g]);
+          const int key0 = it.key0 + t * kTile, pos = key0 + key;
+          float s[RW], x[RW], top = -INFINITY;   // a key's scores but for the rows' factors; above ref
+#pragma unroll
+          for (int n = 0; n < RW; ++n) {
+            float sum = fmaf(__uint_as_float(sr[1][n]), 0.0625f, __uint_as_float(sr[0][n]));
+            if constexpr (G::q_digits == 3) sum = fmaf(__uint_as_float(sr[G::q_digits - 1][n]), 0.00390625f, sum);
+            s[n] = sum * k_scale;
           }
-          const int key0 = it.key0 + t * kTile;
           if (pos < it.lo || pos >= it.hi) {
 #pragma unroll
-            for (int n = 0; n < RP; ++n) s[n] = -INFINITY;
+            for (int n = 0; n < RW; ++n) s[n] = -INFINITY;
           } else if (key0 < mask_lo || key0 + kTile > mask_hi) {
 #pragma unroll
-            for (int n = 0; n < RP; ++n) {
+            for (int n = 0; n < RW; ++n) {
               const int own = row_at[n];
               if ((p.causal && pos > own) || pos < kv8_low(p, own)) s[n] = -INFINITY;
             }
           }
-          float x[RP];
-          bool outgrown = false;
 #pragma unroll
-          for (int n = 0; n < RP; ++n) {
-            x[n] = s[n] - ref[n];
-            outgrown |= n < it.rows && !(x[n] <= kGainY + kSlackY);   // (also where ref is not set yet)
+          for (int n = 0; n < RW; ++n) {
+            x[n] = fmaf(s[n], factor[n], -ref[n]);
+            top = fmaxf(top, x[n]);
           }
+          const bool outgrown = top > kGainY + kSlackY;   // (also where a ref is not set yet)
           const int e = min(126, max(-126, (int)((__float_as_uint(most) + 0x7fffffu) >> 23) - 127));   // 2^e >= most
           const bool larger = e > unit_e;   // (the same in all threads)
-          if (softmax_any(outgrown || larger)) {
+          if (group_any(wg, outgrown || larger)) {
 #pragma unroll
-            for (int n = 0; n < RP; ++n) {
-              const float m = redux_max(s[n]);
-              if (lane == 0) wmax[warp * RP + n] = m;
+            for (int n = 0; n < RW; ++n) {
+              const float m = redux_max(s[n] * factor[n]);
+              if (lane == 0) wmax[(warp & 3) * RW + n] = m;
             }
-            softmax_sync();
+            group_sync();
             const int unit_to = max(unit_e, e);
             const float shrink = kv16_exp2((float)(unit_e - unit_to));
             unit_e = unit_to;
-            float alpha[RP];
+            float alpha[RW];
             bool moved = shrink != 1.f;
 #pragma unroll
-            for (int n = 0; n < RP; ++n) {
-              const float m = fmaxf(fmaxf(wmax[n], wmax[RP + n]), fmaxf(wmax[2 * RP + n], wmax[3 * RP + n])) - kGainY;
+            for (int n = 0; n < RW; ++n) {
+              const float m = fmaxf(fmaxf(wmax[n], wmax[RW + n]), fmaxf(wmax[2 * RW + n], wmax[3 * RW + n])) - kGainY;
               const float to = fmaxf(ref[n], m);
-              alpha[n] = to == -INFINITY ? 1.f : kv16_exp2(ref[n] - to);
+              alpha[n] = kv16_exp2(ref[n] - to);
               moved |= alpha[n] != 1.f;
               ref[n] = to;
               l[n] *= alpha[n];
-              x[n] = s[n] - (to == -INFINITY ? 0.f : to);
+              x[n] = fmaf(s[n], factor[n], -to);
             }
-            if (t > 0 && moved) {   // (the same in all threads)
+            if (t > 0 && moved) {   // (the same in all of the group's threads)
               ok &= kv16_wait(&bars[Bars8::pv_done], (tile - 1) & 1, abort_flag);
               tc::fence_after_sync();
 #pragma unroll
               for (int d = 0; d < kDigitsY * G::parts; ++d) {
-                uint32_t o[RP];
-                const uint32_t addr = tmem_base + G::o_col + (d / kDigitsY) * G::pcols + (d % kDigitsY) * RP + lane_addr;
-                tmem_load<RP>(addr, o);
-                tc::tmem_ld_wait<RP>(o);
+                uint32_t o[RW];
+                const uint32_t addr = tmem_base + G::o_col + (d / kDigitsY) * G::pcols + (d % kDigitsY) * RP + row_base + lane_addr;
+                tmem_load<RW>(addr, o);
+                tc::tmem_ld_wait<RW>(o);
 #pragma unroll
-                for (int n = 0; n < RP; ++n) o[n] = __float_as_uint(__uint_as_float(o[n]) * (alpha[n] * shrink));
-                tmem_store<RP>(addr, o);
+                for (int n = 0; n < RW; ++n) o[n] = __float_as_uint(__uint_as_float(o[n]) * (alpha[n] * shrink));
+                tmem_store<RW>(addr, o);
               }
               tc::tmem_st_wait();
             }
-            softmax_sync();  // (the maxima have been read)
+            group_sync();  // (the maxima have been read)
           }
           const float y_scale = v_scale * power_of_two(-unit_e);
-          uint32_t y[RP / 2][kDigitsY];   // digits of two rows each
+          uint32_t y[kDigitsY][RW / 4];   // digits of four rows each
 #pragma unroll
-          for (int n = 0; n < RP; n += 2) {
+          for (int n = 0; n < RW; n += 2) {
             const float a = kv16_exp2(x[n]), b = kv16_exp2(x[n + 1]);
             l[n] += a;
             l[n + 1] += b;
-            digits2<kDigitsY>(a * y_scale, b * y_scale, y[n / 2]);
+            uint32_t d[kDigitsY];
+            weight_digits2(a * y_scale, b * y_scale, d);
+#pragma unroll
+            for (int g = 0; g < kDigitsY; ++g) y[g][n / 4] = n % 4 == 0 ? d[g] : y[g][n / 4] | d[g] << 16;
           }
           if (tile > 0) ok &= kv16_wait(&bars[Bars8::pv_done], (tile - 1) & 1, abort_flag);  // (P of the last tile has been read)
-          // column d RP + n: digit d of row n; 16 columns are 16 bytes of the key's
+          // column g RP + n: digit g of row n; 16 columns are 16 bytes of the key's
 #pragma unroll
-          for (int j = 0; j < G::pcols / 16; ++j) {
-            uint32_t w[4];
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-              const int c = j * 16 + i * 4, d = c / RP, n = c % RP;
-              w[i] = d < kDigitsY ? y[n / 2][d < kDigitsY ? d : 0] | y[n / 2 + 1][d < kDigitsY ? d : 0] << 16 : 0u;
-            }
-            *reinterpret_cast<uint4*>(p_img + j * (kTile * 16)) = make_uint4(w[0], w[1], w[2], w[3]);
+          for (int g = 0; g < kDigitsY; ++g) {
+            const int c = g * RP + row_base;
+            uint8_t* const to = p_img + (c >> 4) * (kTile * 16) + (c & 15);
+            if constexpr (RW == 8) *reinterpret_cast<uint2*>(to) = make_uint2(y[g][0], y[g][1]);
+            else *reinterpret_cast<uint4*>(to) = make_uint4(y[g][0], y[g][1], y[g][2], y[g][3]);
           }
           tc::fence_async_smem();
           tc::fence_before_sync();
@@ -524,21 +564,21 @@ __global__ void __launch_bounds__(kThreads, (Geo8<HD, RP, kHalf>::ctas)) kv8_sho
         }
         // ---- the piece's rows ----
 #pragma unroll
-        for (int n = 0; n < RP; ++n) {
-          if (n < it.rows) {
+        for (int n = 0; n < RW; ++n) {
+          if (n < rows) {
 #pragma unroll
             for (int o = 16; o > 0; o >>= 1) l[n] += __shfl_xor_sync(0xffffffffu, l[n], o);
           }
         }
         if (lane == 0) {
 #pragma unroll
-          for (int n = 0; n < RP; ++n) wsum[warp * RP + n] = l[n];
+          for (int n = 0; n < RW; ++n) wsum[(warp & 3) * RW + n] = l[n];
         }
-        softmax_sync();
-        if (tid == 0) mbar_arrive(&bars[Bars8::q_empty + (item & 1)]);   // (all have read the factors)
+        group_sync();
+        if (key == 0) mbar_arrive(&bars[Bars8::q_empty + (item & 1)]);   // (all of the group have read the factors)
         ++item;
 #pragma unroll
-        for (int n = 0; n < RP; ++n) l[n] = (wsum[n] + wsum[RP + n]) + (wsum[2 * RP + n] + wsum[3 * RP + n]);
+        for (int n = 0; n < RW; ++n) l[n] = (wsum[n] + wsum[RW + n]) + (wsum[2 * RW + n] + wsum[3 * RW + n]);
         ok &= kv16_wait(&bars[Bars8::pv_done], (tile - 1) & 1, abort_flag);
         tc::fence_after_sync();
         const bool whole = it.begins && it.ends;
@@ -546,62 +586,65 @@ __global__ void __launch_bounds__(kThreads, (Geo8<HD, RP, kHalf>::ctas)) kv8_sho
         const float unit_value = power_of_two(unit_e);
 #pragma unroll
         for (int part = 0; part < G::parts; ++part) {
-          uint32_t o[G::pcols];
-          tmem_load<G::pcols>(tmem_base + G::o_col + part * G::pcols + lane_addr, o);
-          tc::tmem_ld_wait<G::pcols>(o);
-          const int d = part * 128 + tid;
+          uint32_t o[kDigitsY][RW];
+#pragma unroll
+          for (int g = 0; g < kDigitsY; ++g) tmem_load<RW>(tmem_base + G::o_col + part * G::pcols + g * RP + row_base + lane_addr, o[g]);
+          tc::tmem_ld_wait();
+#pragma unroll
+          for (int g = 0; g < kDigitsY; ++g) tc::tmem_landed<RW>(o[g]);
+          const int d = part * 128 + key;
           if (d < HD) {
 #pragma unroll
-            for (int n = 0; n < RP; ++n) {
-              if (n < it.rows) {
-                const float v = fmaf(fmaf(__uint_as_float(o[2 * RP + n]), 0.0625f, __uint_as_float(o[RP + n])), 0.0625f, __uint_as_float(o[n])) * unit_value;
+            for (int n = 0; n < RW; ++n) {
+              if (n < rows) {
+                const float v = fmaf(fmaf(__uint_as_float(o[2][n]), 0.0625f, __uint_as_float(o[1][n])), 0.0625f, __uint_as_float(o[0][n])) * unit_value;
                 if (whole) {
                   int token, head;
-                  row_of(p, it.first_token, kvh, it.row0 + n, &token, &head);
+                  row_of(p, it.first_token, kvh, it.row0 + row_base + n, &token, &head);
                   store_out_elem(p.out + (int64_t)token * p.out_stride_token + (int64_t)head * p.out_stride_head, d, kHalf ? PTH_ATTN_F16 : PTH_ATTN_BF16,
                                  l[n] == 0.f ? 0.f : __fdividef(v, l[n]));
                 } else {
-                  slot[n * HD + d] = v;
+                  slot[(row_base + n) * HD + d] = v;
                 }
               }
             }
           }
         }
         tc::fence_before_sync();
-        if (tid == 0) {
+        if (key == 0) {
 #pragma unroll
-          for (int n = 0; n < RP; ++n) {
-            if (n < it.rows) {
+          for (int n = 0; n < RW; ++n) {
+            if (n < rows) {
               if (whole) {
                 int token, head;
-                row_of(p, it.first_token, kvh, it.row0 + n, &token, &head);
+                row_of(p, it.first_token, kvh, it.row0 + row_base + n, &token, &head);
                 if (p.lse != nullptr)
-                  p.lse[(int64_t)token * p.num_q_heads + head] = l[n] == 0.f ? -INFINITY : ((ref[n] == -INFINITY ? 0.f : ref[n]) + log2f(l[n])) * kLn2;
+                  p.lse[(int64_t)token * p.num_q_heads + head] = l[n] == 0.f ? -INFINITY : (ref[n] + log2f(l[n])) * kLn2;
               } else {
-                slot[RP * HD + n] = ref[n];
-                slot[RP * HD + RP + n] = l[n];
+                slot[RP * HD + row_base + n] = ref[n];
+                slot[RP * HD + RP + row_base + n] = l[n];
               }
             }
           }
         }
         if (!whole) {
-          const int g0 = it.first_cta, g1 = it.last_cta;   // (groups)
-          softmax_sync();
+          const int g0 = it.first_cta, g1 = it.last_cta;   // (groups of CTAs)
+          all_sync();
           int* const counter = reinterpret_cast<int*>(p.workspace) + g0 * heads + hslot;
           if (tid == 0) {
             *arrival = arrive_at(counter);
             if (*arrival == g1 - g0) *counter = 0;   // (for the next call)
           }
-          softmax_sync();
-          if (*arrival == g1 - g0) merge_pieces<HD, RP, kHalf>(p, it, kvh, g0, g1 - g0 + 1, heads, hslot);
+          all_sync();
+          if (*arrival == g1 - g0) merge_pieces<HD, RP, kHalf, 4 * G::groups>(p, it, kvh, g0, g1 - g0 + 1, heads, hslot);
         }
-        softmax_sync();  // (the sums and the arrival have been read)
+        all_sync();  // (the sums and the arrival have been read)
       }
     }
   }
   tc::fence_before_sync();
   __syncthreads();
-  if (warp == kMmaWarp) {
+  if (warp == G::mma_warp) {
     if (*abort_flag) {   // (copies have landed, MMAs may be in flight)
       if (elect_one()) {
         tc::mma_commit(&bars[Bars8::drained]);
@@ -634,7 +677,7 @@ cudaError_t launch_one(const Kv8Params& p, cudaStream_t stream) {
   }
   const int sms = sm_count();
   if (sms <= 0) return cudaErrorInvalidDevice;
-  return pdl_launch(kv8_short_kernel<HD, RP, kHalf>, dim3((unsigned)(sms * G::ctas)), dim3(kThreads), G::total, stream, p);
+  return pdl_launch(kv8_short_kernel<HD, RP, kHalf>, dim3((unsigned)(sms * G::ctas)), dim3(G::threads), G::total, stream, p);
 }
 template <int HD, int RP>
 cudaError_t launch_type(const Kv8Params& p, cudaStream_t stream) {
