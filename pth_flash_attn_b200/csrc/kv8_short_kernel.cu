@@ -27,6 +27,7 @@
 #include "kv8.cuh"
 
 #include "kv16_short.cuh"
+#include "kv8_boxes.cuh"
 #include "pdl.cuh"
 
 namespace pthb200 {
@@ -62,7 +63,12 @@ struct Geo8 {
   // Softmax warpgroups, which share the rows out among themselves; thread t of each is key t of a tile, then dim t of the output.
   static constexpr int groups = RP == 8 ? 1 : 2;
   static constexpr int rows = RP / groups;           // of a group
-  static constexpr int load_warp = 4 * groups, mma_warp = load_warp + 4, schedule_warp = mma_warp + 1, threads = (schedule_warp + 1) * 32;
+  // One warp asks for boxes; rows of 64 bytes come faster by 16-byte copies of four (64 x 8,192 keys, 32 heads of 8, us: 123 / 142 by
+  // boxes; at 128 dims 176 / 174 with 8 rows, 142 / 126 with 16, at 256 dims 92 / 93 and 104 / 105).
+  static constexpr int load_warps = HD == 64 ? 4 : 1;
+  static constexpr int load_warp = 4 * groups, mma_warp = load_warp + load_warps, schedule_warp = mma_warp + 1;
+  static constexpr int others = (load_warps + 2 + 3) / 4 * 4;    // whole warpgroups beside the softmax, whose last warps have nothing to do
+  static constexpr int threads = (load_warp + others) * 32;
   static constexpr int cols = (q_digits * RP + 15) / 16 * 16;     // N of QK
   static constexpr int pcols = (kDigitsY * RP + 15) / 16 * 16;    // N of PV
   static constexpr int qimage = cols * HD;           // column block c of 16 dims at c (cols 16), column n at n 16
@@ -74,10 +80,12 @@ struct Geo8 {
   static constexpr int fit = ctas == 2 ? units2 : (232448 - fixed - 1024) / unit;
   static constexpr int units = fit < most ? fit : most;
   static_assert(units >= 3, "K and V of a tile, and the next K");
-  // Registers that the copies hand to the softmax from what a thread starts with (launch_one asks).
-  static constexpr int start_regs = RP == 8 ? 96 : ctas == 2 ? 72 : 128;
-  static constexpr int copy_regs = RP != 8 && ctas == 2 ? 40 : 64, softmax_regs = RP == 8 ? 112 : ctas == 2 ? 88 : 160;
-  static_assert(4 * groups * softmax_regs + 4 * copy_regs <= (4 * groups + 4) * start_regs, "a split that the launch holds");
+  // Registers that the other warps hand to the softmax from what a thread starts with (launch_one asks).
+  static constexpr int start_regs = HD == 64 ? (RP == 8 ? 80 : ctas == 2 ? 64 : 128) : RP == 8 ? 128 : ctas == 2 ? 80 : 168;
+  static constexpr int other_regs = HD == 64 ? (RP == 8 ? 64 : ctas == 2 ? 48 : 80) : RP == 8 ? 128 : ctas == 2 ? 64 : 104;
+  static constexpr int softmax_regs = HD == 64 ? (RP == 8 ? 112 : ctas == 2 ? 80 : 176) : RP == 8 ? 128 : ctas == 2 ? 88 : 200;
+  static constexpr bool moves = softmax_regs != start_regs;
+  static_assert(4 * groups * softmax_regs + others * other_regs <= (4 * groups + others) * start_regs, "a split that the launch holds");
   static constexpr int s_col = 0, o_col = 2 * cols;  // TMEM columns: S twice, O of every part
   static constexpr int tmem_need = 2 * cols + parts * pcols;
   static constexpr int tmem = tmem_need <= 64 ? 64 : tmem_need <= 128 ? 128 : tmem_need <= 256 ? 256 : 512;
@@ -148,6 +156,7 @@ __device__ __forceinline__ void weight_digits2(float a, float b, uint32_t (&d)[k
   }
 }
 
+// ---- copies by four warps, 16 bytes at a time ----
 // The 32 keys of a warp, from `base_key` of a tile on: rows of `kDims` bytes from off (the lane's key's) into a unit.
 template <int kDims>
 __device__ __forceinline__ void copy_keys8(uint32_t unit, int base_key, const uint8_t* src, long long off) {
@@ -161,11 +170,6 @@ __device__ __forceinline__ void copy_keys8(uint32_t unit, int base_key, const ui
     copy16(dst + row * kDims + (swizzled_chunk<kDims>(row, chunk) << 4), o >= 0 ? src + o + chunk * 16 : src, o >= 0);
   }
 }
-// Asynchronous copy of four bytes, or of none: then the destination is zeroed.
-__device__ __forceinline__ void copy4(uint32_t dst, const void* src, bool live) {
-  asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(dst), "l"(src), "r"(live ? 4 : 0) : "memory");
-}
-
 // The scales of a warp's two runs of 16 keys: of the first key of each that is visible (they share them).
 __device__ __forceinline__ void copy_scales(const Kv8Params& p, uint32_t to, int base_key, int kvh, int blk, int slot) {
   const int lane = threadIdx.x & 31;
@@ -176,6 +180,61 @@ __device__ __forceinline__ void copy_scales(const Kv8Params& p, uint32_t to, int
     const int64_t at = (int64_t)b * p.scale_stride_block + (int64_t)((uint32_t)s / (uint32_t)p.scale_tokens) * p.scale_stride_group + (int64_t)kvh * p.scale_stride_head;
     const float* const base = (lane & 15) == 0 ? p.k_scale : p.v_scale;
     copy4(to + (lane & 15) * 32 + (base_key / kRun + (lane >> 4)) * 4, live != 0 ? base + at : base, live != 0);
+  }
+}
+
+// ---- copies by one warp, in boxes ----
+// Where the runs of 16 keys of a tile lie, one per lane of the first eight.
+struct TileRuns {
+  int key0, lo, hi, kvh;
+  int blk, slot;       // the lane's run: block (-1: none that is seen) and first slot
+};
+__device__ __forceinline__ void tile_runs(const Kv8Params& p, const Piece& it, int t, TileRuns* r) {
+  const int lane = threadIdx.x & 31;
+  r->key0 = it.key0 + t * kTile;
+  r->lo = it.lo;
+  r->hi = it.hi;
+  r->kvh = it.kvh;
+  r->blk = -1;
+  const int pos = r->key0 + lane * kRun;
+  if (lane < kTile / kRun && pos < r->hi && pos + kRun > r->lo) {
+    const int page = p.block_shift >= 0 ? pos >> p.block_shift : (int)((uint32_t)pos / (uint32_t)p.block_size);
+    r->slot = pos - page * p.block_size;
+    r->blk = __ldg(p.block_table + (int64_t)it.r * p.block_table_row_stride + page);
+  }
+}
+// One unit of the tile's keys or values: boxes that the lanes of `boxes` ask for, and 16-byte copies of the runs `copied`, which zero
+// what is not seen.  All lanes; the unit's barrier counts their 32 copies' ends and one arrival with the boxes' bytes.
+template <int kDims>
+__device__ __forceinline__ void load_unit(const Kv8Params& p, const TileRuns& r, const CUtensorMap& map, const uint8_t* src, int part, uint32_t unit, uint64_t* full,
+                                          uint32_t boxes, uint32_t copied) {
+  constexpr int kChunks = kDims / 16, kRows = 32 / kChunks;   // 16-byte chunks of a row, rows at a time
+  const int lane = threadIdx.x & 31, chunk = lane % kChunks, sub = lane / kChunks;
+  if (lane == 0) mbar_arrive_expect_tx(full, __popc(boxes) * p.box_slots * kDims);
+  __syncwarp();
+  if (boxes >> lane & 1) tma_load_4d(unit + lane * kRun * kDims, &map, part * 128, r.kvh, r.slot, r.blk, full);
+#pragma unroll 1
+  for (; copied != 0; copied &= copied - 1) {
+    const int run = __ffs(copied) - 1, blk = __shfl_sync(0xffffffffu, r.blk, run), slot = __shfl_sync(0xffffffffu, r.slot, run);
+    const uint8_t* from = src + (int64_t)blk * p.stride_block + (int64_t)(slot + sub) * p.stride_slot + (int64_t)r.kvh * p.stride_head + part * 128 + chunk * 16;
+    const int row0 = run * kRun + sub;
+#pragma unroll
+    for (int i = 0; i < kRun / kRows; ++i) {
+      const int row = row0 + i * kRows, pos = r.key0 + row;
+      const bool live = blk >= 0 && pos >= r.lo && pos < r.hi;
+      copy16(unit + row * kDims + (swizzled_chunk<kDims>(row, chunk) << 4), live ? from : src, live);
+      from += kRows * p.stride_slot;
+    }
+  }
+  copies_arrive(full);
+}
+// The scales of a tile's runs: lanes 0 to 7 the keys', 8 to 15 the values'.
+__device__ __forceinline__ void load_scales(const Kv8Params& p, const TileRuns& r, uint32_t to) {
+  const int lane = threadIdx.x & 31, blk = __shfl_sync(0xffffffffu, r.blk, lane & 7), slot = __shfl_sync(0xffffffffu, r.slot, lane & 7);
+  if (lane < 16) {
+    const int64_t at = (int64_t)blk * p.scale_stride_block + (int64_t)((uint32_t)slot / (uint32_t)p.scale_tokens) * p.scale_stride_group + (int64_t)r.kvh * p.scale_stride_head;
+    const float* const base = lane < 8 ? p.k_scale : p.v_scale;
+    copy4(to + lane * 4, blk >= 0 ? base + at : base, blk >= 0);
   }
 }
 
@@ -235,7 +294,7 @@ __device__ __forceinline__ void stage_queries(const Kv8Params& p, const Piece& i
 }
 
 template <int HD, int RP, bool kHalf>
-__global__ void __launch_bounds__((Geo8<HD, RP, kHalf>::threads), (Geo8<HD, RP, kHalf>::ctas)) kv8_short_kernel(const __grid_constant__ Kv8Params p) {
+__global__ void __launch_bounds__((Geo8<HD, RP, kHalf>::threads), (Geo8<HD, RP, kHalf>::ctas)) kv8_short_kernel(const __grid_constant__ Kv8Params p, const __grid_constant__ CUtensorMap k_map, const __grid_constant__ CUtensorMap v_map) {
   using G = Geo8<HD, RP, kHalf>;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* const smem = smem_raw + ((1024u - (tc::smem_u32(smem_raw) & 1023u)) & 1023u);
@@ -248,10 +307,12 @@ __global__ void __launch_bounds__((Geo8<HD, RP, kHalf>::threads), (Geo8<HD, RP, 
   int* const stop = arrival + 1;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
 
+  if (warp == G::load_warp && lane < 2 && p.box_slots > 0)
+    asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(lane == 0 ? &k_map : &v_map)) : "memory");
   if (warp == G::mma_warp) {
     if (lane == 0) {
       for (int i = 0; i < G::units; ++i) {
-        tc::mbar_init(&full[i], 128);
+        tc::mbar_init(&full[i], G::load_warps == 4 ? 128 : 33);   // (copies_arrive, load_unit)
         tc::mbar_init(&empty[i], 1);
       }
       for (int i = 0; i < 2; ++i) {
@@ -262,7 +323,7 @@ __global__ void __launch_bounds__((Geo8<HD, RP, kHalf>::threads), (Geo8<HD, RP, 
       tc::mbar_init(&bars[Bars8::p_ready], kSoftmaxThreads * G::groups);
       tc::mbar_init(&bars[Bars8::pv_done], 1);
       tc::mbar_init(&bars[Bars8::drained], 1);
-      PieceQueue(nullptr, &bars[Bars8::queue], stop).init(G::threads / 32 - 1);
+      PieceQueue(nullptr, &bars[Bars8::queue], stop).init(4 * G::groups + G::load_warps + 1);
       *abort_flag = 0;
       tc::mbar_init_fence();
     }
@@ -279,9 +340,11 @@ __global__ void __launch_bounds__((Geo8<HD, RP, kHalf>::threads), (Geo8<HD, RP, 
   PieceQueue queue(reinterpret_cast<Piece*>(smem + G::pieces), &bars[Bars8::queue], stop);
   float* const qfactor = reinterpret_cast<float*>(smem + G::qfactor);
   bool ok = true;
+  uint32_t asked = 0;   // units that the loading warp has asked for
 
   if (warp == G::schedule_warp) {
     // =========================== schedule and queries ============================
+    if constexpr (G::moves) asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(G::other_regs));
     Piece it;
     uint32_t item = 0;
     bool going = true;
@@ -303,55 +366,114 @@ __global__ void __launch_bounds__((Geo8<HD, RP, kHalf>::threads), (Geo8<HD, RP, 
     }
   } else if (warp >= G::load_warp && warp < G::mma_warp) {
     // =========================== copies ==========================================
-    // A warp owns 32 keys of every tile: lane l knows where key l of them lies.
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(G::copy_regs));
-    const int base_key = (warp - G::load_warp) * 32;
-    const uint32_t ring = tc::smem_u32(smem), scales = tc::smem_u32(smem + G::scales);
-    uint32_t unit = 0, tile = 0;
-    auto next_unit = [&]() -> uint32_t {
-      const uint32_t s = unit % G::units;
-      if (unit >= G::units) ok &= kv16_wait(&empty[s], ((unit / G::units) - 1) & 1, abort_flag);
-      ++unit;
-      return s;
-    };
-    {
-      KeyLookup keys(p, queue, abort_flag, base_key + lane);
-      bool have = keys.fetch(), have_v = false;
-      long long off_v = 0;
-      int64_t head_v = 0;
-      while (have || have_v) {
+    if constexpr (G::moves) asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(G::other_regs));
+    if constexpr (G::load_warps == 4) {
+      // A warp owns 32 keys of every tile: lane l knows where key l of them lies.
+      const int base_key = (warp - G::load_warp) * 32;
+      const uint32_t ring = tc::smem_u32(smem), scales = tc::smem_u32(smem + G::scales);
+      uint32_t unit = 0, tile = 0;
+      auto next_unit = [&]() -> uint32_t {
+        const uint32_t s = unit % G::units;
+        if (unit >= G::units) ok &= kv16_wait(&empty[s], ((unit / G::units) - 1) & 1, abort_flag);
+        ++unit;
+        return s;
+      };
+      {
+        KeyLookup keys(p, queue, abort_flag, base_key + lane);
+        bool have = keys.fetch(), have_v = false;
+        long long off_v = 0;
+        int64_t head_v = 0;
+        while (have || have_v) {
+          const bool now = have;
+          long long off = 0;
+          int64_t head_k = 0;
+          if (now) {
+            off = keys.offset();
+            const int kvh = keys.it.kvh, blk = keys.blk, slot = keys.slot;
+            head_k = (int64_t)kvh * p.stride_head;
+            have = keys.fetch();
+#pragma unroll
+            for (int part = 0; part < G::parts; ++part) {
+              const uint32_t s = next_unit();
+              if (part == 0) copy_scales(p, scales + (tile++ % kScaleTiles) * 64, base_key, kvh, blk, slot);
+              copy_keys8<G::dims>(ring + s * G::unit, base_key, p.k + head_k + part * 128, off);
+              copies_arrive(&full[s]);
+            }
+          }
+          if (have_v) {
+#pragma unroll
+            for (int part = 0; part < G::parts; ++part) {
+              const uint32_t s = next_unit();
+              copy_keys8<G::dims>(ring + s * G::unit, base_key, p.v + head_v + part * 128, off_v);
+              copies_arrive(&full[s]);
+            }
+          }
+          off_v = off;
+          head_v = head_k;
+          have_v = now;
+        }
+      }
+    } else {
+      // (Behind a wait that gave up nothing more is asked for: a unit that is not free may be waiting for its boxes.)
+      const uint32_t ring = tc::smem_u32(smem), scales = tc::smem_u32(smem + G::scales);
+      uint32_t tile = 0;
+      Piece it;
+      int left = 0, t = 0;
+      TileRuns next;
+      next.slot = 0;
+      auto fetch = [&]() -> bool {
+        if (left == 0) {
+          if (!queue.get(&it, abort_flag)) return false;
+          left = it.tiles;
+          t = 0;
+        }
+        tile_runs(p, it, t++, &next);
+        --left;
+        return true;
+      };
+      // K of a tile is asked for ahead of V of the one before.
+      auto units = [&](const TileRuns& r, const CUtensorMap& map, const uint8_t* src, uint32_t boxes, uint32_t copied, bool with_scales) {
+#pragma unroll
+        for (int part = 0; part < G::parts; ++part, ++asked) {
+          const uint32_t s = asked % G::units;
+          if (asked >= G::units) ok &= kv16_wait(&empty[s], ((asked / G::units) - 1) & 1, abort_flag);
+          ok = __all_sync(0xffffffffu, ok);
+          if (!ok) return;
+          // (the scales go where the unit that is free now says that they have been read)
+          if (part == 0 && with_scales) load_scales(p, r, scales + (tile % kScaleTiles) * 64);
+          load_unit<G::dims>(p, r, map, src, part, ring + s * G::unit, &full[s], boxes, copied);
+        }
+      };
+      bool have = fetch(), have_v = false;
+      TileRuns last;
+      uint32_t last_boxes = 0, last_copied = 0;
+      while ((have || have_v) && ok) {
         const bool now = have;
-        long long off = 0;
-        int64_t head_k = 0;
+        TileRuns here = next;
+        uint32_t boxes = 0, copied = 0;
         if (now) {
-          off = keys.offset();
-          const int kvh = keys.it.kvh, blk = keys.blk, slot = keys.slot;
-          head_k = (int64_t)kvh * p.stride_head;
-          have = keys.fetch();
-#pragma unroll
-          for (int part = 0; part < G::parts; ++part) {
-            const uint32_t s = next_unit();
-            if (part == 0) copy_scales(p, scales + (tile++ % kScaleTiles) * 64, base_key, kvh, blk, slot);
-            copy_keys8<G::dims>(ring + s * G::unit, base_key, p.k + head_k + part * 128, off);
-            copies_arrive(&full[s]);
-          }
+          have = fetch();   // (the look-up of the next tile is on its way while this one's cells are asked for)
+          const int pos = here.key0 + lane * kRun;
+          if ((uint32_t)here.blk >= (uint32_t)p.num_blocks) here.blk = -1;
+          const uint32_t seen = __ballot_sync(0xffffffffu, lane < kTile / kRun && pos < here.hi && pos + kRun > here.lo);
+          const uint32_t whole = __ballot_sync(0xffffffffu, here.blk >= 0 && pos >= here.lo && pos + kRun <= here.hi);
+          boxes = p.box_slots == 32 ? whole & whole >> 1 & 0x55u : p.box_slots == 16 ? whole : 0u;
+          copied = 0xffu & ~(p.box_slots == 32 ? boxes | boxes << 1 : boxes);
+          // (scores of keys that nobody sees are replaced, whatever they are: those need no zeros)
+          units(here, k_map, p.k, boxes, copied & seen, true);
+          ++tile;
         }
-        if (have_v) {
-#pragma unroll
-          for (int part = 0; part < G::parts; ++part) {
-            const uint32_t s = next_unit();
-            copy_keys8<G::dims>(ring + s * G::unit, base_key, p.v + head_v + part * 128, off_v);
-            copies_arrive(&full[s]);
-          }
-        }
-        off_v = off;
-        head_v = head_k;
+        if (have_v && ok) units(last, v_map, p.v, last_boxes, last_copied, false);
+        last = here;
+        last_boxes = boxes;
+        last_copied = copied;
         have_v = now;
       }
     }
     copies_wait_all();
   } else if (warp == G::mma_warp) {
     // =========================== MMAs ============================================
+    if constexpr (G::moves) asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(G::other_regs));
     // QK of a tile is issued ahead of PV of the one before, in the order in which the units arrive.
     constexpr uint32_t qk_desc = instr_desc_e4m3(128, G::cols, 0, 0);
     constexpr uint32_t pv_desc = instr_desc_e4m3(128, G::pcols, 1, 1);
@@ -360,7 +482,7 @@ __global__ void __launch_bounds__((Geo8<HD, RP, kHalf>::threads), (Geo8<HD, RP, 
     auto arrived = [&]() -> uint32_t {
       const uint32_t s = unit % G::units;
       ok &= kv16_wait(&full[s], (unit / G::units) & 1, abort_flag);
-      tc::fence_async_smem();   // (the copies wrote through the generic proxy)
+      tc::fence_async_smem();   // (copies wrote through the generic proxy)
       ++unit;
       return s;
     };
@@ -377,7 +499,7 @@ __global__ void __launch_bounds__((Geo8<HD, RP, kHalf>::threads), (Geo8<HD, RP, 
             const uint64_t b = tc::smem_desc(q_s + (item & 1) * G::qimage + (part * (G::dims / 16) + kk * 2) * (G::cols * 16), G::cols * 16, 128);
             mma_e4m3(tmem_base + G::s_col + (tile & 1) * G::cols, a, b, qk_desc, part > 0 || kk > 0);
           }
-          tc::mma_commit(&empty[s]);
+          if (ok) tc::mma_commit(&empty[s]);   // (a unit that has not landed is not given back)
           if (part == G::parts - 1) {
             tc::mma_commit(&bars[Bars8::s_ready + (tile & 1)]);
             mbar_arrive(&bars[Bars8::s_ready + (tile & 1)]);
@@ -404,7 +526,7 @@ __global__ void __launch_bounds__((Geo8<HD, RP, kHalf>::threads), (Geo8<HD, RP, 
             const uint64_t b = tc::smem_desc(p_s + kk * 512, 128, kTile * 16);
             mma_e4m3(tmem_base + G::o_col + part * G::pcols, a, b, pv_desc, !first_of_item || kk > 0);
           }
-          tc::mma_commit(&empty[s]);
+          if (ok) tc::mma_commit(&empty[s]);
           if (part == G::parts - 1) tc::mma_commit(&bars[Bars8::pv_done]);
         }
         __syncwarp();
@@ -422,9 +544,9 @@ __global__ void __launch_bounds__((Geo8<HD, RP, kHalf>::threads), (Geo8<HD, RP, 
       }
     }
     if (pending) pv(pending_first);
-  } else {
+  } else if (warp < G::load_warp) {
     // =========================== softmax =========================================
-    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(G::softmax_regs));
+    if constexpr (G::moves) asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(G::softmax_regs));
     constexpr int RW = G::rows;
     const int wg = warp >> 2, key = tid & 127, row_base = wg * RW;
     const uint32_t lane_addr = (uint32_t)((warp & 3) * 32) << 16;
@@ -641,25 +763,30 @@ __global__ void __launch_bounds__((Geo8<HD, RP, kHalf>::threads), (Geo8<HD, RP, 
         all_sync();  // (the sums and the arrival have been read)
       }
     }
+  } else {
+    if constexpr (G::moves) asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(G::other_regs));
   }
   tc::fence_before_sync();
   __syncthreads();
-  if (warp == G::mma_warp) {
-    if (*abort_flag) {   // (copies have landed, MMAs may be in flight)
-      if (elect_one()) {
-        tc::mma_commit(&bars[Bars8::drained]);
-        kv16_drain(&bars[Bars8::drained], 0);
-        atomicOr(&g_kv8_short_status, 32u);
-      }
-      __syncwarp();
+  if (*abort_flag) {   // (the same in all threads) what is in flight comes to its end first: MMAs, and boxes
+    if (warp == G::mma_warp && elect_one()) {
+      tc::mma_commit(&bars[Bars8::drained]);
+      kv16_drain(&bars[Bars8::drained], 0);
+      atomicOr(&g_kv8_short_status, 32u);
     }
+    if (warp == G::load_warp) {   // (boxes are one warp's)
+      for (uint32_t u = asked > G::units ? asked - G::units : 0; u < asked; ++u) kv16_drain(&full[u % G::units], (u / G::units) & 1);
+    }
+    __syncthreads();
+  }
+  if (warp == G::mma_warp) {
     tc::tmem_dealloc(tmem_base, G::tmem);
   }
   (void)ok;
 }
 
 template <int HD, int RP, bool kHalf>
-cudaError_t launch_one(const Kv8Params& p, cudaStream_t stream) {
+cudaError_t launch_one(const Kv8Params& p, const CUtensorMap& k_map, const CUtensorMap& v_map, cudaStream_t stream) {
   using G = Geo8<HD, RP, kHalf>;
   static_assert(G::total <= 232448, "shared memory of one CTA");
   static_assert(G::ctas == 1 || G::total <= 115712, "shared memory of two CTAs");
@@ -670,25 +797,25 @@ cudaError_t launch_one(const Kv8Params& p, cudaStream_t stream) {
   if (dev < 0 || dev >= 64 || !configured[dev]) {
     cudaFuncAttributes attr;
     err = cudaFuncGetAttributes(&attr, kv8_short_kernel<HD, RP, kHalf>);
-    if (err == cudaSuccess && attr.numRegs < G::start_regs) err = cudaErrorInvalidConfiguration;   // (setmaxnreg would wait without end)
+    if (err == cudaSuccess && G::moves && attr.numRegs < G::start_regs) err = cudaErrorInvalidConfiguration;   // (setmaxnreg would wait without end)
     if (err == cudaSuccess) err = cudaFuncSetAttribute(kv8_short_kernel<HD, RP, kHalf>, cudaFuncAttributeMaxDynamicSharedMemorySize, G::total);
     if (err != cudaSuccess) return err;
     if (dev >= 0 && dev < 64) configured[dev] = true;
   }
   const int sms = sm_count();
   if (sms <= 0) return cudaErrorInvalidDevice;
-  return pdl_launch(kv8_short_kernel<HD, RP, kHalf>, dim3((unsigned)(sms * G::ctas)), dim3(G::threads), G::total, stream, p);
+  return pdl_launch(kv8_short_kernel<HD, RP, kHalf>, dim3((unsigned)(sms * G::ctas)), dim3(G::threads), G::total, stream, p, k_map, v_map);
 }
 template <int HD, int RP>
-cudaError_t launch_type(const Kv8Params& p, cudaStream_t stream) {
-  return p.dtype == PTH_ATTN_F16 ? launch_one<HD, RP, true>(p, stream) : launch_one<HD, RP, false>(p, stream);
+cudaError_t launch_type(const Kv8Params& p, const CUtensorMap& k_map, const CUtensorMap& v_map, cudaStream_t stream) {
+  return p.dtype == PTH_ATTN_F16 ? launch_one<HD, RP, true>(p, k_map, v_map, stream) : launch_one<HD, RP, false>(p, k_map, v_map, stream);
 }
 template <int HD>
-cudaError_t launch_rows(const Kv8Params& p, cudaStream_t stream) {
+cudaError_t launch_rows(const Kv8Params& p, const CUtensorMap& k_map, const CUtensorMap& v_map, cudaStream_t stream) {
   const int64_t rows = (int64_t)p.max_query_len * p.group;
-  if (rows <= 8) return launch_type<HD, 8>(p, stream);
-  if (rows <= 16) return launch_type<HD, 16>(p, stream);
-  return launch_type<HD, 32>(p, stream);
+  if (rows <= 8) return launch_type<HD, 8>(p, k_map, v_map, stream);
+  if (rows <= 16) return launch_type<HD, 16>(p, k_map, v_map, stream);
+  return launch_type<HD, 32>(p, k_map, v_map, stream);
 }
 
 }  // namespace
@@ -699,13 +826,18 @@ int64_t kv8_short_workspace_bytes(int head_size, int num_sms) {
 }
 
 cudaError_t launch_kv8_short(const Kv8Params& p, cudaStream_t stream) {
+  // Boxes of 32 slots where pages are whole numbers of them (a piece's tiles begin at multiples of 32 keys), else of 16.
+  Kv8Params q = p;
+  q.box_slots = p.head_size == 64 ? 0 : p.block_size % 32 == 0 ? 32 : 16;
+  CUtensorMap k_map{}, v_map{};
+  if (q.box_slots > 0 && (!cell_box_map(q, p.k, q.box_slots, &k_map) || !cell_box_map(q, p.v, q.box_slots, &v_map))) q.box_slots = 0;
   switch (p.head_size) {
     case 64:
-      return launch_rows<64>(p, stream);
+      return launch_rows<64>(q, k_map, v_map, stream);
     case 128:
-      return launch_rows<128>(p, stream);
+      return launch_rows<128>(q, k_map, v_map, stream);
     default:
-      return launch_rows<256>(p, stream);
+      return launch_rows<256>(q, k_map, v_map, stream);
   }
 }
 

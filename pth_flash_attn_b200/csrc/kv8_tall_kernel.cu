@@ -26,7 +26,7 @@
 // CTA.  The pieces of a row tile that a cut divides are merged by the CTA that arrives last.
 #include "kv8.cuh"
 
-#include "page_copy.cuh"
+#include "kv8_boxes.cuh"
 #include "pdl.cuh"
 #include "umma_rows.cuh"
 
@@ -228,16 +228,6 @@ __device__ __forceinline__ void mma_e4m3_words(uint32_t d_tmem, uint32_t alo, ui
       "}\n" ::"r"(d_tmem),
       "r"(alo), "r"(ahi), "r"(blo), "r"(bhi), "r"(idesc), "n"(kAccumulate ? 1 : 0)
       : "memory");
-}
-// Tiled TMA load of one box of a rank-4 tensor map into shared memory.
-__device__ __forceinline__ void tma_load_4d(uint32_t dst, const CUtensorMap* map, int x, int y, int z, int w, uint64_t* bar) {
-  asm volatile(
-      "cp.async.bulk.tensor.4d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5}], [%6];" ::"r"(dst),
-      "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(z), "r"(w), "r"(tc::smem_u32(bar))
-      : "memory");
-}
-__device__ __forceinline__ void copy4(uint32_t dst, const void* src, bool live) {
-  asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(dst), "l"(src), "r"(live ? 4 : 0) : "memory");
 }
 // Swizzled operand descriptor of raw rows: 128 bytes, or 64 bytes in the 64-byte swizzle.
 template <int HD>
@@ -827,18 +817,6 @@ __global__ void __launch_bounds__((Tall8<HD, kHalf>::threads), (Tall8<HD, kHalf>
   if (warp == G::mma_warp) tc::tmem_dealloc(tmem_base, G::tmem);
 }
 
-// Tensor map over one of the caches, [dims][heads][slots][blocks], a box being up to 128 dims of 16 slots of one head, swizzled by its
-// rows.  False: the driver refuses the view.  (Encoded for every call: a microsecond of the host.)
-bool cell_box_map(const Kv8Params& p, const uint8_t* base, CUtensorMap* map) {
-  const EncodeTiledFn fn = encode_tiled_fn();
-  const cuuint64_t dims[4] = {(cuuint64_t)p.head_size, (cuuint64_t)p.num_kv_heads, (cuuint64_t)p.block_size, (cuuint64_t)p.num_blocks};
-  const cuuint64_t strides[3] = {(cuuint64_t)p.stride_head, (cuuint64_t)p.stride_slot, (cuuint64_t)p.stride_block};
-  const cuuint32_t box[4] = {(cuuint32_t)(p.head_size < 128 ? 64 : 128), 1, 16, 1}, elem[4] = {1, 1, 1, 1};
-  return fn != nullptr && fn(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 4, const_cast<uint8_t*>(base), dims, strides, box, elem, CU_TENSOR_MAP_INTERLEAVE_NONE,
-                             p.head_size < 128 ? CU_TENSOR_MAP_SWIZZLE_64B : CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
-                             CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
-}
-
 template <int HD, bool kHalf>
 cudaError_t launch_one(const Kv8Params& p, const CUtensorMap& k_map, const CUtensorMap& v_map, cudaStream_t stream) {
   using G = Tall8<HD, kHalf>;
@@ -876,7 +854,7 @@ int64_t kv8_tall_workspace_bytes(int head_size, int num_sms) {
 
 cudaError_t launch_kv8_tall(const Kv8Params& p, cudaStream_t stream, bool* taken) {
   CUtensorMap k_map{}, v_map{};
-  *taken = cell_box_map(p, p.k, &k_map) && cell_box_map(p, p.v, &v_map);
+  *taken = cell_box_map(p, p.k, 16, &k_map) && cell_box_map(p, p.v, 16, &v_map);
   if (!*taken) return cudaSuccess;
   switch (p.head_size) {
     case 64:
