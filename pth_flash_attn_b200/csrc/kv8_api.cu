@@ -206,7 +206,7 @@ int32_t pthb200_kv8_read(const PthB200Kv8ReadArgs* a, void* stream) {
   if (a->num_rows == 0 || a->num_reqs == 0 || a->max_rows == 0) return PTH_ATTN_OK;
   if (int32_t rc = check_rows(a->key, a->key_stride_token, a->key_stride_head, 16, "key")) return rc;
   if (int32_t rc = check_rows(a->value, a->value_stride_token, a->value_stride_head, 16, "value")) return rc;
-  if (int32_t rc = check_cache(a, 8)) return rc;
+  if (int32_t rc = check_cache(a, 16)) return rc;
   KV8_REQUIRE(a->first != nullptr && a->row_start_loc != nullptr, "first and row_start_loc must not be NULL");
   return launched(launch_kv8_reader(*a, static_cast<cudaStream_t>(stream)), "reader");
 }
@@ -227,7 +227,7 @@ int32_t pthb200_rotary(const PthB200RotaryArgs* a, void* stream) {
   KV8_REQUIRE(a->head_size >= 1 && a->head_size <= 1024, "head_size must be in [1, 1024]");
   KV8_REQUIRE(a->num_frequencies >= 1 && a->num_frequencies <= a->head_size / 2, "num_frequencies must be in [1, head_size / 2]");
   KV8_REQUIRE(a->num_tokens >= 0 && a->num_q_heads >= 0 && a->num_k_heads >= 0, "num_tokens, num_q_heads and num_k_heads must be >= 0");
-  KV8_REQUIRE((int64_t)(a->num_q_heads + (int64_t)a->num_k_heads) * a->head_size <= INT32_MAX, "a token's heads must have fewer than 2^31 dimensions");
+  KV8_REQUIRE(((int64_t)a->num_q_heads + a->num_k_heads) * a->head_size < (1 << 28), "a token's heads must have fewer than 2^28 dimensions");
   KV8_REQUIRE(std::isfinite(a->scale), "scale must be finite");
   if (a->num_tokens == 0 || (a->num_q_heads == 0 && a->num_k_heads == 0)) return PTH_ATTN_OK;
   const int64_t elem = size_of(a->dtype);

@@ -19,7 +19,6 @@ namespace pthb200 {
 namespace {
 
 constexpr int kWarps = 8;
-constexpr int kRowsKept = 4;   // pieces of 16 source bytes (32 in fp32) that a lane keeps
 
 struct Write8Params {
   const uint8_t* src[2];
@@ -35,61 +34,75 @@ struct Write8Params {
   int32_t num_blocks, block_size, scale_tokens, num_kv_heads, num_reqs, num_tokens, num_pages, max_query_len, src_dtype;
 };
 
-// Eight elements of a source row in 32 bits.  kWide: rows lie on 16-byte boundaries.
-template <int kDtype, bool kWide>
-__device__ __forceinline__ void load8(const uint8_t* row, int e0, float (&x)[8]) {
-  if constexpr (kDtype == PTH_ATTN_F32) {
+// Eight elements of a source row, as they are.  kWide: rows lie on 16-byte boundaries.
+template <int kDtype>
+struct Eight {
+  uint32_t w[kDtype == PTH_ATTN_F32 ? 8 : 4];
+  template <bool kWide>
+  __device__ __forceinline__ void load(const uint8_t* row, int e0) {
+    constexpr int kWords = kDtype == PTH_ATTN_F32 ? 8 : 4;
     if constexpr (kWide) {
-      const float4 a = __ldg(reinterpret_cast<const float4*>(row) + e0 / 4), b = __ldg(reinterpret_cast<const float4*>(row) + e0 / 4 + 1);
-      x[0] = a.x, x[1] = a.y, x[2] = a.z, x[3] = a.w, x[4] = b.x, x[5] = b.y, x[6] = b.z, x[7] = b.w;
-    } else {
 #pragma unroll
-      for (int i = 0; i < 8; ++i) x[i] = __ldg(reinterpret_cast<const float*>(row) + e0 + i);
-    }
-  } else {
-    uint32_t w[4];
-    if constexpr (kWide) {
-      const uint4 v = __ldg(reinterpret_cast<const uint4*>(row) + e0 / 8);
-      w[0] = v.x, w[1] = v.y, w[2] = v.z, w[3] = v.w;
+      for (int i = 0; i < kWords; i += 4) {
+        const uint4 v = __ldg(reinterpret_cast<const uint4*>(row) + (e0 * kWords / 8 + i) / 4);
+        w[i] = v.x, w[i + 1] = v.y, w[i + 2] = v.z, w[i + 3] = v.w;
+      }
+    } else if constexpr (kDtype == PTH_ATTN_F32) {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) w[i] = __ldg(reinterpret_cast<const uint32_t*>(row) + e0 + i);
     } else {
       const uint16_t* const h = reinterpret_cast<const uint16_t*>(row) + e0;
 #pragma unroll
       for (int i = 0; i < 4; ++i) w[i] = (uint32_t)__ldg(h + 2 * i) | (uint32_t)__ldg(h + 2 * i + 1) << 16;
     }
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      if constexpr (kDtype == PTH_ATTN_F16) {
-        const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w[i]));
-        x[2 * i] = f.x;
-        x[2 * i + 1] = f.y;
-      } else {
-        x[2 * i] = __uint_as_float(w[i] << 16);
-        x[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
-      }
-    }
   }
-}
-__device__ __forceinline__ float finite_max(const float (&x)[8]) {
-  float m = 0.f;
+  __device__ __forceinline__ void clear() {
 #pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    const float a = fabsf(x[i]);
-    m = a < INFINITY ? fmaxf(m, a) : m;
+    for (int i = 0; i < (int)(sizeof(w) / 4); ++i) w[i] = 0u;
+  }
+  __device__ __forceinline__ float get(int i) const {
+    if constexpr (kDtype == PTH_ATTN_F32) return __uint_as_float(w[i]);
+    else if constexpr (kDtype == PTH_ATTN_F16) return __half2float(__ushort_as_half((unsigned short)(w[i / 2] >> 16 * (i & 1))));
+    else return __uint_as_float(i & 1 ? w[i / 2] & 0xffff0000u : w[i / 2] << 16);
+  }
+};
+// The largest finite magnitude of some rows' pieces.
+template <int kDtype, int kCount>
+__device__ __forceinline__ float finite_max(const Eight<kDtype> (&x)[kCount]) {
+  float m = 0.f;
+  if constexpr (kDtype != PTH_ATTN_F32) {   // magnitudes are ordered as 16-bit integers, of which infinities and NaN are the largest
+    constexpr uint32_t kInf = kDtype == PTH_ATTN_F16 ? 0x7c00u : 0x7f80u;
+    uint32_t top = 0;
+#pragma unroll
+    for (int i = 0; i < kCount; ++i) {
+      top = __vimax3_u16x2(top, x[i].w[0] & 0x7fff7fffu, x[i].w[1] & 0x7fff7fffu);
+      top = __vimax3_u16x2(top, x[i].w[2] & 0x7fff7fffu, x[i].w[3] & 0x7fff7fffu);
+    }
+    const uint32_t one = max(top & 0xffffu, top >> 16);
+    if (one < kInf) return kDtype == PTH_ATTN_F16 ? __half2float(__ushort_as_half((unsigned short)one)) : __uint_as_float(one << 16);
+  }
+#pragma unroll
+  for (int i = 0; i < kCount; ++i) {
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
+      const float a = fabsf(x[i].get(k));
+      m = a < INFINITY ? fmaxf(m, a) : m;
+    }
   }
   return m;
 }
 // The smallest power of two, 2^-126 to 2^120, with most <= 448 times it.
 __device__ __forceinline__ float needed_scale(float most) { return power_of_two(min(120, max(-126, e4m3_exponent(most)))); }
-// Eight numbers as cells, x / scale: exactly scaled where the scale is a power of two.
-__device__ __forceinline__ uint2 cells8(const float (&x)[8], float scale) {
+// Eight numbers as cells, x / scale: exactly scaled where the scale is a power of two (up: its reciprocal; 0: it is none).
+template <int kDtype>
+__device__ __forceinline__ uint2 cells8(const Eight<kDtype>& x, float scale, float up) {
   float y[8];
-  if ((__float_as_uint(scale) & 0x7fffffu) == 0) {
-    const float up = power_of_two(127 - (int)(__float_as_uint(scale) >> 23));
+  if (up != 0.f) {
 #pragma unroll
-    for (int i = 0; i < 8; ++i) y[i] = x[i] * up;
+    for (int i = 0; i < 8; ++i) y[i] = x.get(i) * up;
   } else {
 #pragma unroll
-    for (int i = 0; i < 8; ++i) y[i] = __fdiv_rn(x[i], scale);
+    for (int i = 0; i < 8; ++i) y[i] = __fdiv_rn(x.get(i), scale);
   }
   return make_uint2(e4m3x2(y[0], y[1]) | e4m3x2(y[2], y[3]) << 16, e4m3x2(y[4], y[5]) | e4m3x2(y[6], y[7]) << 16);
 }
@@ -102,42 +115,42 @@ __device__ __forceinline__ uint32_t rescaled(uint32_t w, float ratio) {
 struct Block {
   int row0, rows;      // first new row of the source, their number
   int begin;           // first new position in the block of tokens
-  int block, group;    // of the cache
+  int block, group;    // of the cache; the block may be none of it
 };
 
 // Block number x of the launch, found by a warp (the same in all lanes); false: there is none.
 __device__ __forceinline__ bool find_block(const Write8Params& p, int x, Block* out) {
   const int g = p.scale_tokens, lane = threadIdx.x & 31;
-  auto base = [&](int r) -> long long {
-    return p.max_query_len == 1 ? r : (long long)(min(max(0, __ldg(p.query_start_loc + r)), p.num_tokens) / g) + 2ll * r;
-  };
-  int r = x;
-  if (p.max_query_len > 1) {   // the last request whose numbers begin at or in front of x, 32 at a time
-    int lo = 0, hi = p.num_reqs;
+  const bool single = p.max_query_len == 1;
+  auto start_of = [&](int r) -> int { return min(max(0, __ldg(p.query_start_loc + r)), p.num_tokens); };
+  auto number_of = [&](int r, int start) -> long long { return single ? r : (long long)(start / g) + 2ll * r; };
+  // the last request whose numbers begin at or in front of x: among 32, whose offsets and lengths a lane each loads
+  int lo = single ? x : 0, hi = single ? x + 1 : p.num_reqs;
+  if (lo >= p.num_reqs) return false;
 #pragma unroll 1
-    while (hi - lo > 1) {
-      const int step = (hi - lo + 31) / 32, at = lo + lane * step;
-      const uint32_t before = __ballot_sync(0xffffffffu, at < hi && base(at) <= x);
-      if (before == 0) return false;   // (start offsets that go backwards)
-      const int last = 31 - __clz(before);
-      hi = min(hi, lo + (last + 1) * step);
-      lo += last * step;
-    }
-    r = lo;
+  while (hi - lo > 32) {
+    const int step = (hi - lo + 31) / 32, at = lo + lane * step;
+    const uint32_t before = __ballot_sync(0xffffffffu, at < hi && number_of(at, start_of(at)) <= x);
+    if (before == 0) return false;   // (start offsets that go backwards)
+    const int last = 31 - __clz(before);
+    hi = min(hi, lo + (last + 1) * step);
+    lo += last * step;
   }
-  if (r >= p.num_reqs) return false;
-  const int first = max(0, __ldg(p.query_start_loc + r)), end = min(max(0, __ldg(p.query_start_loc + r + 1)), p.num_tokens);
-  const int all = max(0, end - first), tokens = min(all, p.max_query_len), pos0 = max(0, __ldg(p.seq_lens + r)) - all;
+  const int mine = min(lo + lane, hi - 1), begin = start_of(mine), stop = start_of(mine + 1), length = max(0, __ldg(p.seq_lens + mine));
+  const uint32_t before = __ballot_sync(0xffffffffu, lo + lane < hi && number_of(mine, begin) <= x);
+  if (before == 0) return false;
+  const int from_lane = 31 - __clz(before), r = lo + from_lane;
+  const int first = __shfl_sync(0xffffffffu, begin, from_lane), end = __shfl_sync(0xffffffffu, stop, from_lane), seq = __shfl_sync(0xffffffffu, length, from_lane);
+  const int all = max(0, end - first), tokens = min(all, p.max_query_len), pos0 = seq - all;
   const int skip = max(0, -pos0);   // tokens at negative positions
   if (tokens <= skip) return false;
-  const long long nth = x - base(r);
+  const long long nth = x - number_of(r, first);
   const long long start = ((long long)(pos0 + skip) / g + nth) * g;
   const long long from = max(start, (long long)pos0 + skip), to = min(start + g, (long long)pos0 + tokens);
   if (nth < 0 || to <= from) return false;
   const long long page = from / p.block_size;
   if (page >= p.num_pages) return false;
-  out->block = __ldg(p.block_table + (int64_t)r * p.block_table_row_stride + page);
-  if ((uint32_t)out->block >= (uint32_t)p.num_blocks) return false;
+  out->block = __ldg(p.block_table + (int64_t)r * p.block_table_row_stride + page);   // (not looked at here: the rows' loads go out beside it)
   out->group = (int)(start - page * p.block_size) / g;
   out->begin = (int)(from - start);
   out->rows = (int)(to - from);
@@ -145,9 +158,11 @@ __device__ __forceinline__ bool find_block(const Write8Params& p, int x, Block* 
   return true;
 }
 
+// kKept: pieces of eight elements that a lane keeps, as many as 16 rows of a warp.
 template <int HD, int kDtype, bool kWide, bool kCta>
-__global__ void __launch_bounds__(kWarps * 32) kv8_writer_kernel(const __grid_constant__ Write8Params p) {
+__global__ void __launch_bounds__(kWarps * 32, kDtype != PTH_ATTN_F32 && HD < 256 && !kCta ? 4 : 1) kv8_writer_kernel(const __grid_constant__ Write8Params p) {
   constexpr int kLanes = HD / 8, kAtOnce = 32 / kLanes;      // lanes of a row, rows of a warp at a time
+  constexpr int kKept = kDtype == PTH_ATTN_F32 || HD == 256 ? 8 : 16 / kAtOnce;
   __shared__ float most_of[kWarps];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int chunk = lane % kLanes, sub = lane / kLanes;
@@ -160,25 +175,25 @@ __global__ void __launch_bounds__(kWarps * 32) kv8_writer_kernel(const __grid_co
   if (!find_block(p, x, &b)) return;
   const uint8_t* const src = p.src[v] + (int64_t)b.row0 * p.src_stride_token[v] + (int64_t)head * p.src_stride_head[v];
   const int64_t stride = p.src_stride_token[v];
+  constexpr int kStep = (kCta ? kWarps : 1) * kAtOnce;       // rows of a round
+  const int mine = (kCta ? warp * kAtOnce : 0) + sub;
+  float most = 0.f;
+  Eight<kDtype> kept[kKept];
+#pragma unroll 1
+  for (int n0 = 0; n0 < b.rows; n0 += kKept * kStep) {
+    const uint8_t* at = src + (n0 + mine) * stride;
+#pragma unroll
+    for (int i = 0; i < kKept; ++i, at += kStep * stride) {
+      kept[i].clear();
+      if (n0 + i * kStep + mine < b.rows) kept[i].template load<kWide>(at, chunk * 8);
+    }
+    most = fmaxf(most, finite_max(kept));
+  }
+  if ((uint32_t)b.block >= (uint32_t)p.num_blocks) return;   // (the same in all threads that share the block)
   uint8_t* const cells = p.cache[v] + (int64_t)b.block * p.stride_block[v] + (int64_t)(b.group * p.scale_tokens) * p.stride_slot[v] + (int64_t)head * p.stride_head[v] + chunk * 8;
   float* const scale_at = p.scale[v] + (int64_t)b.block * p.scale_stride_block[v] + (int64_t)b.group * p.scale_stride_group[v] + (int64_t)head * p.scale_stride_head[v];
   float was = b.begin > 0 ? *scale_at : 0.f;
   if (!(was > 0.f && was < INFINITY)) was = 0.f;
-  constexpr int kStep = (kCta ? kWarps : 1) * kAtOnce;       // rows of a round
-  const int mine = (kCta ? warp * kAtOnce : 0) + sub;
-  float most = 0.f, kept[kRowsKept][8];
-#pragma unroll 1
-  for (int n0 = 0; n0 < b.rows; n0 += kRowsKept * kStep) {
-#pragma unroll
-    for (int i = 0; i < kRowsKept; ++i) {
-      const int n = n0 + i * kStep + mine;
-#pragma unroll
-      for (int k = 0; k < 8; ++k) kept[i][k] = 0.f;
-      if (n < b.rows) load8<kDtype, kWide>(src + n * stride, chunk * 8, kept[i]);
-    }
-#pragma unroll
-    for (int i = 0; i < kRowsKept; ++i) most = fmaxf(most, finite_max(kept[i]));
-  }
   most = redux_max(most);
   if constexpr (kCta) {
     if (lane == 0) most_of[warp] = most;
@@ -197,19 +212,19 @@ __global__ void __launch_bounds__(kWarps * 32) kv8_writer_kernel(const __grid_co
       *at = make_uint2(rescaled(w.x, ratio), rescaled(w.y, ratio));
     }
   }
-  const bool once = b.rows <= kRowsKept * kStep;   // (the rows are in registers still)
+  const float up = (__float_as_uint(scale) & 0x7fffffu) == 0 ? power_of_two(127 - (int)(__float_as_uint(scale) >> 23)) : 0.f;
+  const bool once = b.rows <= kKept * kStep;   // (the rows are in registers still)
 #pragma unroll 1
-  for (int n0 = 0; n0 < b.rows; n0 += kRowsKept * kStep) {
+  for (int n0 = 0; n0 < b.rows; n0 += kKept * kStep) {
+    if (!once) {
 #pragma unroll
-    for (int i = 0; i < kRowsKept; ++i) {
-      const int n = n0 + i * kStep + mine;
-      if (!once && n < b.rows) load8<kDtype, kWide>(src + n * stride, chunk * 8, kept[i]);
+      for (int i = 0; i < kKept; ++i)
+        if (n0 + i * kStep + mine < b.rows) kept[i].template load<kWide>(src + (n0 + i * kStep + mine) * stride, chunk * 8);
     }
+    uint8_t* to = cells + (int64_t)(b.begin + n0 + mine) * p.stride_slot[v];
 #pragma unroll
-    for (int i = 0; i < kRowsKept; ++i) {
-      const int n = n0 + i * kStep + mine;
-      if (n < b.rows) *reinterpret_cast<uint2*>(cells + (int64_t)(b.begin + n) * p.stride_slot[v]) = cells8(kept[i], scale);
-    }
+    for (int i = 0; i < kKept; ++i, to += kStep * p.stride_slot[v])
+      if (n0 + i * kStep + mine < b.rows) *reinterpret_cast<uint2*>(to) = cells8(kept[i], scale, up);
   }
   if constexpr (kCta) __syncthreads();   // (all have read the old scale)
   if (lane == 0 && (!kCta || warp == 0) && scale != was) *scale_at = scale;
@@ -219,7 +234,6 @@ template <int HD, int kDtype>
 cudaError_t launch_for(const Write8Params& p, bool wide, cudaStream_t stream) {
   const int64_t numbers = p.max_query_len == 1 ? p.num_reqs : (int64_t)(p.num_tokens / p.scale_tokens) + 2ll * p.num_reqs;
   const int64_t units = numbers * 2 * p.num_kv_heads;
-  // a warp reads a block of 32 rows in two to eight rounds
   const bool cta = p.scale_tokens > 32 && p.max_query_len > 1;
   const int64_t ctas = cta ? units : (units + kWarps - 1) / kWarps;
   if (ctas > 0x7fffffff) return cudaErrorInvalidConfiguration;

@@ -2,11 +2,11 @@
 // k are read and written once.
 //
 // The angle is a product in 64 bits, taken to [-pi, pi] there (a position of 10^6 has 20 bits in front of the point, which 32 bits
-// would take from the angle), and its sine and cosine have 32 bits.  A CTA works them out once for a token and all its heads, in
+// would take from the angle), and its sine and cosine have 32 bits.  A CTA works them out once for a few tokens and all their heads, in
 // shared memory.
 //
-// A thread turns kVec pairs of a head: vectors of 16 bytes where the rows' places allow it, else pair by pair.  Both of a pair are
-// read before either is written, so a tensor may be turned in place.
+// A thread turns kVec pairs of a head: vectors of 16 bytes where the rows' places allow it, kBatch of them in flight, else pair by pair.
+// Both of a pair are read before either is written, so a tensor may be turned in place.
 #include "kv8.cuh"
 
 #include "pdl.cuh"
@@ -14,7 +14,7 @@
 namespace pthb200 {
 namespace {
 
-constexpr int kThreads = 256;
+constexpr int kThreads = 256, kBatch = 1;
 
 struct RotaryParams {
   const uint8_t* src[2];
@@ -61,6 +61,12 @@ struct Vec {
       }
     }
   }
+  // Turns the pair (this i, y j) by t.
+  __device__ __forceinline__ void turn(int i, Vec& y, int j, float2 t) {
+    const float u = x[i], v = y.x[j];
+    x[i] = u * t.x - v * t.y;
+    y.x[j] = u * t.y + v * t.x;
+  }
   __device__ __forceinline__ void store(uint8_t* at) const {
     uint32_t w[4];
 #pragma unroll
@@ -84,72 +90,115 @@ __device__ __forceinline__ float2 turn_of(const RotaryParams& p, long long posit
   return make_float2(c * p.scale, (p.inverse ? -s : s) * p.scale);
 }
 
+// Where piece x of a CTA's tokens lies: of a head's pairs, then of the dimensions that are copied.
 template <int kDtype, bool kInterleaved, bool kVector>
-__global__ void __launch_bounds__(kThreads) rotary_kernel(const __grid_constant__ RotaryParams p) {
-  extern __shared__ float2 turns[];   // [half]
-  constexpr int kVec = Vec<kDtype>::n, kSize = kDtype == PTH_ATTN_F32 ? 4 : 2;
-  const int token = (int)blockIdx.x, heads = p.heads[0] + p.heads[1], half = p.half;
-  pdl_wait();
-  const long long position = __ldg(reinterpret_cast<const long long*>(p.positions) + token);
-  for (int i = threadIdx.x; i < half; i += kThreads) turns[i] = turn_of(p, position, i);
-  __syncthreads();
-  // pieces of a head: of its pairs, then of the dimensions that are copied
-  const int turning = kVector ? 2 * half / (2 * kVec) : half, copied = kVector ? (p.head_size - 2 * half) / kVec : p.head_size - 2 * half;
-  const int per = turning + copied;
-  for (int x = threadIdx.x; x < heads * per; x += kThreads) {
-    const int h = x / per, i = x - h * per, k = h >= p.heads[0] ? 1 : 0, head = h - (k ? p.heads[0] : 0);
-    const uint8_t* const src = p.src[k] + (int64_t)token * p.src_stride_token[k] + (int64_t)head * p.src_stride_head[k];
-    uint8_t* const dst = p.dst[k] + (int64_t)token * p.dst_stride_token[k] + (int64_t)head * p.dst_stride_head[k];
+struct Place {
+  const uint8_t* src;
+  uint8_t* dst;
+  int i, turning;      // piece of the head; pieces that turn
+  int token;           // of the CTA
+  __device__ __forceinline__ Place(const RotaryParams& p, int token0, uint32_t x) {
+    constexpr int kVec = Vec<kDtype>::n;
+    turning = kVector ? p.half / kVec : p.half;
+    const uint32_t per = kVector ? (p.head_size - p.half) / kVec : p.head_size - p.half, heads = p.heads[0] + p.heads[1];
+    const uint32_t row = x / per;
+    i = (int)(x - row * per);
+    token = (int)(row / heads);
+    const int h = (int)(row - token * heads), k = h >= p.heads[0] ? 1 : 0, head = h - (k ? p.heads[0] : 0);
+    src = p.src[k] + (int64_t)(token0 + token) * p.src_stride_token[k] + (int64_t)head * p.src_stride_head[k];
+    dst = p.dst[k] + (int64_t)(token0 + token) * p.dst_stride_token[k] + (int64_t)head * p.dst_stride_head[k];
+  }
+  // byte offsets of a vector piece's two halves (of a copied one: the same twice)
+  __device__ __forceinline__ int2 halves(const RotaryParams& p) const {
+    constexpr int kVec = Vec<kDtype>::n, kSize = 16 / kVec;
     if (i >= turning) {
-      if constexpr (kVector) {
-        const int at = (2 * half + (i - turning) * kVec) * kSize;
-        *reinterpret_cast<uint4*>(dst + at) = *reinterpret_cast<const uint4*>(src + at);
-      } else {
-        put<kDtype>(dst, 2 * half + i - turning, get<kDtype>(src, 2 * half + i - turning));
-      }
-    } else if constexpr (kVector) {
-      // kVec pairs: 16 bytes of either half, or 32 bytes of pairs side by side
-      const int a0 = (kInterleaved ? 2 * i * kVec : i * kVec) * kSize, b0 = kInterleaved ? a0 + 16 : a0 + half * kSize;
-      Vec<kDtype> a, b;
-      a.load(src + a0);
-      b.load(src + b0);
-      if constexpr (kInterleaved) {
+      const int at = (2 * p.half + (i - turning) * kVec) * kSize;
+      return make_int2(at, at);
+    }
+    const int a = (kInterleaved ? 2 * i * kVec : i * kVec) * kSize;
+    return make_int2(a, kInterleaved ? a + 16 : a + p.half * kSize);
+  }
+};
+
+template <int kDtype, bool kInterleaved, bool kVector>
+__global__ void __launch_bounds__(kThreads) rotary_kernel(const __grid_constant__ RotaryParams p, int per_cta) {
+  extern __shared__ float2 turns[];   // [tokens of the CTA][half]
+  constexpr int kVec = Vec<kDtype>::n;
+  using At = Place<kDtype, kInterleaved, kVector>;
+  const int token0 = (int)blockIdx.x * per_cta, tokens = min(per_cta, p.num_tokens - token0), half = p.half;
+  const uint32_t pieces = (uint32_t)tokens * (uint32_t)((p.heads[0] + p.heads[1]) * (kVector ? (p.head_size - half) / kVec : p.head_size - half));
+  pdl_wait();
+  for (int i = threadIdx.x; i < tokens * half; i += kThreads) {
+    const int t = i / half, pair = i - t * half;
+    // (vectors: the e-th pairs of all pieces side by side, so that lanes read from banks of their own)
+    turns[kVector ? t * half + pair % kVec * (half / kVec) + pair / kVec : i] = turn_of(p, __ldg(reinterpret_cast<const long long*>(p.positions) + token0 + t), pair);
+  }
+  __syncthreads();
+  if constexpr (kVector) {
+    const int step = half / kVec;
+#pragma unroll 1
+    for (uint32_t x0 = threadIdx.x; x0 < pieces; x0 += kBatch * kThreads) {
+      Vec<kDtype> a[kBatch], b[kBatch];
+      const float2* t[kBatch];
+      uint8_t* to_a[kBatch];
+      uint8_t* to_b[kBatch];   // nullptr: a copied piece
 #pragma unroll
-        for (int e = 0; e < kVec / 2; ++e) {
-          const float2 t = turns[i * kVec + e], u = turns[i * kVec + kVec / 2 + e];
-          const float ax = a.x[2 * e], ay = a.x[2 * e + 1], bx = b.x[2 * e], by = b.x[2 * e + 1];
-          a.x[2 * e] = ax * t.x - ay * t.y;
-          a.x[2 * e + 1] = ax * t.y + ay * t.x;
-          b.x[2 * e] = bx * u.x - by * u.y;
-          b.x[2 * e + 1] = bx * u.y + by * u.x;
-        }
-      } else {
-#pragma unroll
-        for (int e = 0; e < kVec; ++e) {
-          const float2 t = turns[i * kVec + e];
-          const float ax = a.x[e], bx = b.x[e];
-          a.x[e] = ax * t.x - bx * t.y;
-          b.x[e] = ax * t.y + bx * t.x;
-        }
+      for (int k = 0; k < kBatch; ++k) {
+        const uint32_t x = x0 + k * kThreads;
+        to_a[k] = nullptr;
+        if (x >= pieces) continue;
+        const At at(p, token0, x);
+        const int2 to = at.halves(p);
+        a[k].load(at.src + to.x);
+        b[k].load(at.src + to.y);
+        t[k] = turns + at.token * half + at.i;
+        to_a[k] = at.dst + to.x;
+        to_b[k] = at.i < at.turning ? at.dst + to.y : nullptr;
       }
-      a.store(dst + a0);
-      b.store(dst + b0);
-    } else {
-      const int ia = kInterleaved ? 2 * i : i, ib = kInterleaved ? 2 * i + 1 : i + half;
-      const float2 t = turns[i];
-      const float a = get<kDtype>(src, ia), b = get<kDtype>(src, ib);
-      put<kDtype>(dst, ia, a * t.x - b * t.y);
-      put<kDtype>(dst, ib, a * t.y + b * t.x);
+#pragma unroll
+      for (int k = 0; k < kBatch; ++k) {
+        if (to_a[k] == nullptr) continue;
+        if (to_b[k] != nullptr) {
+          if constexpr (kInterleaved) {
+#pragma unroll
+            for (int e = 0; e < kVec / 2; ++e) {
+              a[k].turn(2 * e, a[k], 2 * e + 1, t[k][e * step]);
+              b[k].turn(2 * e, b[k], 2 * e + 1, t[k][(kVec / 2 + e) * step]);
+            }
+          } else {
+#pragma unroll
+            for (int e = 0; e < kVec; ++e) a[k].turn(e, b[k], e, t[k][e * step]);
+          }
+          b[k].store(to_b[k]);
+        }
+        a[k].store(to_a[k]);
+      }
+    }
+  } else {
+#pragma unroll 1
+    for (uint32_t x = threadIdx.x; x < pieces; x += kThreads) {
+      const At at(p, token0, x);
+      if (at.i >= at.turning) {
+        put<kDtype>(at.dst, half + at.i, get<kDtype>(at.src, half + at.i));   // (dimension 2 half + i - half)
+        continue;
+      }
+      const int ia = kInterleaved ? 2 * at.i : at.i, ib = kInterleaved ? 2 * at.i + 1 : at.i + half;
+      const float2 t = turns[at.token * half + at.i];
+      const float x0 = get<kDtype>(at.src, ia), y0 = get<kDtype>(at.src, ib);
+      put<kDtype>(at.dst, ia, x0 * t.x - y0 * t.y);
+      put<kDtype>(at.dst, ib, x0 * t.y + y0 * t.x);
     }
   }
 }
 
 template <int kDtype>
 cudaError_t launch_for(const RotaryParams& p, bool interleaved, bool vector, cudaStream_t stream) {
-  const dim3 grid((unsigned)p.num_tokens);
-  const size_t smem = (size_t)p.half * sizeof(float2);
-  if (interleaved) return pdl_launch(vector ? rotary_kernel<kDtype, true, true> : rotary_kernel<kDtype, true, false>, grid, kThreads, smem, stream, p);
-  return pdl_launch(vector ? rotary_kernel<kDtype, false, true> : rotary_kernel<kDtype, false, false>, grid, kThreads, smem, stream, p);
+  // tokens of a CTA: one where there are too few to give every SM several CTAs of four
+  const int per_cta = p.num_tokens >= 4 * 148 * 4 ? 4 : 1;
+  const dim3 grid((unsigned)((p.num_tokens + per_cta - 1) / per_cta));
+  const size_t smem = (size_t)per_cta * p.half * sizeof(float2);
+  if (interleaved) return pdl_launch(vector ? rotary_kernel<kDtype, true, true> : rotary_kernel<kDtype, true, false>, grid, kThreads, smem, stream, p, per_cta);
+  return pdl_launch(vector ? rotary_kernel<kDtype, false, true> : rotary_kernel<kDtype, false, false>, grid, kThreads, smem, stream, p, per_cta);
 }
 
 }  // namespace

@@ -272,7 +272,7 @@ def test_c_abi_read_refusals(field, value, message):
     ("abi_version", 1, "abi_version"), ("dtype", 9, "dtype"), ("head_size", 0, "head_size"), ("head_size", 1025, "head_size"),
     ("num_frequencies", 0, "num_frequencies"), ("num_frequencies", 33, "num_frequencies"), ("num_k_heads", -1, "num_k_heads"), ("q", None, "q is NULL"),
     ("k_out", _BASE + 1, "k_out must be 2-byte aligned"), ("positions", _BASE + 4, "positions"), ("frequencies", None, "frequencies"),
-    ("scale", float("nan"), "scale must be finite"), ("num_q_heads", 1 << 30, "fewer than 2^31")])
+    ("scale", float("nan"), "scale must be finite"), ("num_q_heads", 1 << 30, "fewer than 2^28")])
 def test_c_abi_rotary_refusals(field, value, message):
     lib, a = capi.load_library(), _rotary_struct()
     setattr(a, field, value)
