@@ -60,6 +60,20 @@ __device__ __forceinline__ void mma_e4m3(uint32_t d_tmem, uint64_t a_desc, uint6
       : "memory");
 }
 
+// NaN cells of a word: the top bit of their bytes; they become zero.
+__device__ __forceinline__ uint32_t take_nan(uint32_t& w) {
+  const uint32_t nan = (w & 0x7f7f7f7fu) + 0x01010101u & 0x80808080u;
+  w &= ~((nan >> 7) * 0xffu);
+  return nan;
+}
+// The block and slot of a key of a request; -1: there is none.
+__device__ __forceinline__ int block_of(const Kv16Params& p, int r, int pos, int* slot) {
+  const int page = pos / p.block_size;
+  *slot = pos - page * p.block_size;
+  const int blk = __ldg(p.block_table + (int64_t)r * p.block_table_row_stride + page);
+  return (uint32_t)blk < (uint32_t)p.num_blocks ? blk : -1;
+}
+
 }  // namespace
 
 // (Not in the unnamed namespace: the schedule's templates find these by their argument's namespace.)

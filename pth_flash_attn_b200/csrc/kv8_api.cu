@@ -142,8 +142,14 @@ int32_t build(const PthB200Kv8Args* a, bool decode, Kv8Params* p) {
   return PTH_ATTN_OK;
 }
 
-// Rows (query tokens x G) from which a launch of more than one token goes to the kernel with the rows on the MMA's M dimension.
-constexpr int64_t kTallRows = 33;
+// Rows (query tokens x G) from which a launch of more than one token goes to the kernel with the rows on the MMA's M
+// dimension.  Keys on M against rows on M, us, four heads of a KV head:
+//   rows   D 128: 8 x 500  8 x 4,000  64 x 500  64 x 4,000 keys   D 64: 64 x 500  64 x 4,000   D 256: 64 x 500  64 x 4,000
+//     16         19 / 22      30 / 50      42 / 63     107 / 255           42 / 39     105 / 136        64 / 99     188 / 343
+//     32         35 / 22      43 / 50      81 / 62     184 / 256           78 / 39     184 / 137       110 / 99     268 / 345
+//     48         31 / 22      56 / 50     142 / 65     327 / 256
+// Single tokens of wide groups stay with the keys on M, which divides few requests better.
+int64_t tall_rows(int head_size) { return head_size == 64 ? 17 : 33; }
 
 int64_t workspace_bytes(int head_size, int num_sms) {
   return std::max(kv8_short_workspace_bytes(head_size, num_sms), kv8_tall_workspace_bytes(head_size, num_sms));
@@ -159,7 +165,7 @@ int32_t attention(const PthB200Kv8Args* a, bool decode, void* stream) {
     return set_error(PTH_ATTN_ECUDA, "cannot query the current device");
   const int64_t need = workspace_bytes(a->head_size, sms);
   KV8_REQUIRE(a->workspace_bytes >= need, "workspace has " + std::to_string(a->workspace_bytes) + " bytes, " + std::to_string(need) + " are needed");
-  if ((int64_t)p.max_query_len * p.group >= kTallRows && p.max_query_len > 1) {
+  if ((int64_t)p.max_query_len * p.group >= tall_rows(a->head_size) && p.max_query_len > 1) {
     bool taken = false;
     const int32_t rc = launched(launch_kv8_tall(p, static_cast<cudaStream_t>(stream), &taken), "attention");
     if (rc != PTH_ATTN_OK || taken) return rc;

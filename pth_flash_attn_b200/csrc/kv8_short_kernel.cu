@@ -101,8 +101,8 @@ struct Geo8 {
   static constexpr int pieces = scales + kScaleTiles * 64;   // PieceQueue's entries
   static constexpr int bars = pieces + kQueue * 64;
   static constexpr int n_bars = 2 * units + 2 + 2 + 2 + 1 + 1 + 2 * kQueue + 1;
-  static constexpr int misc = bars + n_bars * 8;     // ints: abort flag, TMEM address, arrival, stop; scratch of find_run
-  static constexpr int total = misc + 160 + 1024;
+  static constexpr int misc = bars + n_bars * 8;     // ints: abort flag, TMEM address, arrival, stop; scratch of find_run; nan_item
+  static constexpr int total = misc + 176 + 1024;
   static_assert(kQueue * 64 + n_bars * 8 + 160 <= 1024, "fixed part");
 };
 
@@ -293,6 +293,51 @@ __device__ __forceinline__ void stage_queries(const Kv8Params& p, const Piece& i
   }
 }
 
+// Rows of several tokens: keys that some of them see and others do not, [.., lo) and [hi, ..).
+struct Masks {
+  int lo, hi;
+  __device__ __forceinline__ Masks(const Kv8Params& p, const Piece& it) : lo(0), hi(INT_MAX) {
+    if (p.query_start_loc == nullptr) return;
+    if (p.causal) hi = it.pos0 + it.row0 / p.group + 1;
+    lo = kv8_low(p, it.pos0 + (it.row0 + it.rows - 1) / p.group);
+  }
+  __device__ __forceinline__ bool divide(int key0) const { return key0 < lo || key0 + kTile > hi; }
+};
+// A value that is NaN under a hidden key: its weight is zero, but zero times NaN is NaN.  So where the rows of a piece do not all see a
+// tile's keys, NaN among its values becomes zero in front of the MMA, and what the rows see of it is put in at the piece's end.  Both
+// are rare, so slow.
+template <int kDims>
+__device__ __forceinline__ bool clear_nan(uint8_t* unit) {   // one warp; whether there was any
+  uint32_t any = 0;
+#pragma unroll 1
+  for (int i = threadIdx.x & 31; i < kTile * kDims / 16; i += 32) {
+    uint4 v = reinterpret_cast<const uint4*>(unit)[i];
+    const uint32_t nan = take_nan(v.x) | take_nan(v.y) | take_nan(v.z) | take_nan(v.w);
+    if (nan != 0) reinterpret_cast<uint4*>(unit)[i] = v;
+    any |= nan;
+  }
+  return __any_sync(0xffffffffu, any != 0);
+}
+// The rows, of `rows` from row0 of the piece on, that see a key whose value is NaN at dimension d, of the tiles that were cleared.
+__device__ __forceinline__ uint32_t nan_rows(const Kv8Params& p, const Piece& it, int row0, int rows, int d) {
+  const Masks masks(p, it);
+  uint32_t seen = 0;
+#pragma unroll 1
+  for (int pos = max(it.lo, it.key0); pos < it.hi; ++pos) {
+    if (!masks.divide(it.key0 + (pos - it.key0) / kTile * kTile)) continue;
+    int slot;
+    const int blk = block_of(p, it.r, pos, &slot);
+    if (blk < 0) continue;
+    const uint8_t c = p.v[(int64_t)blk * p.stride_block + (int64_t)slot * p.stride_slot + (int64_t)it.kvh * p.stride_head + d];
+    if ((c & 0x7f) != 0x7f) continue;
+    for (int n = 0; n < rows; ++n) {
+      const int own = it.pos0 + (it.row0 + row0 + n) / p.group;
+      if ((!p.causal || pos <= own) && pos >= kv8_low(p, own)) seen |= 1u << n;
+    }
+  }
+  return seen;
+}
+
 template <int HD, int RP, bool kHalf>
 __global__ void __launch_bounds__((Geo8<HD, RP, kHalf>::threads), (Geo8<HD, RP, kHalf>::ctas)) kv8_short_kernel(const __grid_constant__ Kv8Params p, const __grid_constant__ CUtensorMap k_map, const __grid_constant__ CUtensorMap v_map) {
   using G = Geo8<HD, RP, kHalf>;
@@ -305,6 +350,7 @@ __global__ void __launch_bounds__((Geo8<HD, RP, kHalf>::threads), (Geo8<HD, RP, 
   uint32_t* const tslot = reinterpret_cast<uint32_t*>(smem + G::misc + 4);
   int* const arrival = reinterpret_cast<int*>(smem + G::misc + 8);
   int* const stop = arrival + 1;
+  volatile uint32_t* const nan_item = reinterpret_cast<volatile uint32_t*>(smem + G::misc + 160);   // 1 + the last item whose values had NaN taken out
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
 
   if (warp == G::load_warp && lane < 2 && p.box_slots > 0)
@@ -325,6 +371,7 @@ __global__ void __launch_bounds__((Geo8<HD, RP, kHalf>::threads), (Geo8<HD, RP, 
       tc::mbar_init(&bars[Bars8::drained], 1);
       PieceQueue(nullptr, &bars[Bars8::queue], stop).init(4 * G::groups + G::load_warps + 1);
       *abort_flag = 0;
+      *nan_item = 0;
       tc::mbar_init_fence();
     }
     __syncwarp();
@@ -512,11 +559,16 @@ __global__ void __launch_bounds__((Geo8<HD, RP, kHalf>::threads), (Geo8<HD, RP, 
       if (last_of_item) ++item;
     };
     uint32_t pv_tile = 0;
-    auto pv = [&](bool first_of_item) {
+    auto pv = [&](bool first_of_item, bool divided, uint32_t its_item) {
       ok &= kv16_wait(&bars[Bars8::p_ready], pv_tile & 1, abort_flag);
 #pragma unroll
       for (int part = 0; part < G::parts; ++part) {
         const uint32_t s = arrived();
+        if (divided && clear_nan<G::dims>(smem + s * G::unit)) {
+          if (lane == 0) *nan_item = its_item + 1;
+          tc::fence_async_smem();
+          __syncwarp();
+        }
         if (elect_one()) {
           tc::fence_after_sync();
 #pragma unroll
@@ -534,16 +586,21 @@ __global__ void __launch_bounds__((Geo8<HD, RP, kHalf>::threads), (Geo8<HD, RP, 
       ++pv_tile;
     };
     Piece it;
-    bool pending = false, pending_first = false;
+    bool pending = false, pending_first = false, pending_divided = false;
+    uint32_t pending_item = 0;
     while (queue.get(&it, abort_flag)) {
+      const Masks masks(p, it);
       for (int t = 0; t < it.tiles; ++t) {
+        const uint32_t here = item;
         qk(t == 0, t == it.tiles - 1);
-        if (pending) pv(pending_first);
+        if (pending) pv(pending_first, pending_divided, pending_item);
         pending = true;
         pending_first = t == 0;
+        pending_divided = masks.divide(it.key0 + t * kTile);
+        pending_item = here;
       }
     }
-    if (pending) pv(pending_first);
+    if (pending) pv(pending_first, pending_divided, pending_item);
   } else if (warp < G::load_warp) {
     // =========================== softmax =========================================
     if constexpr (G::moves) asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(G::softmax_regs));
@@ -565,11 +622,8 @@ __global__ void __launch_bounds__((Geo8<HD, RP, kHalf>::threads), (Geo8<HD, RP, 
         const int kvh = it.kvh, rows = it.rows - row_base;   // of the group: RW or fewer, or none
         ok &= kv16_wait(&bars[Bars8::q_full + (item & 1)], (item >> 1) & 1, abort_flag);
         const float* const factor = qfactor + (item & 1) * RP + row_base;
-        // rows of several tokens: keys that some of them see and others do not, [.., mask_lo) and [mask_hi, ..)
-        int mask_lo = 0, mask_hi = INT_MAX;
+        const Masks masks(p, it);
         if (p.query_start_loc != nullptr) {
-          if (p.causal) mask_hi = it.pos0 + it.row0 / p.group + 1;
-          mask_lo = kv8_low(p, it.pos0 + (it.row0 + it.rows - 1) / p.group);
           if (key < RW) row_at[key] = it.pos0 + (it.row0 + min(row_base + key, it.rows - 1)) / p.group;
           group_sync();
         }
@@ -605,7 +659,7 @@ __global__ void __launch_bounds__((Geo8<HD, RP, kHalf>::threads), (Geo8<HD, RP, 
           if (pos < it.lo || pos >= it.hi) {
 #pragma unroll
             for (int n = 0; n < RW; ++n) s[n] = -INFINITY;
-          } else if (key0 < mask_lo || key0 + kTile > mask_hi) {
+          } else if (masks.divide(key0)) {
 #pragma unroll
             for (int n = 0; n < RW; ++n) {
               const int own = row_at[n];
@@ -706,6 +760,7 @@ __global__ void __launch_bounds__((Geo8<HD, RP, kHalf>::threads), (Geo8<HD, RP, 
         const bool whole = it.begins && it.ends;
         float* const slot = partial_slot<HD, RP>(p, (int)blockIdx.x, it.begins);
         const float unit_value = power_of_two(unit_e);
+        const bool had_nan = *nan_item == item;   // (the item has been counted already)
 #pragma unroll
         for (int part = 0; part < G::parts; ++part) {
           uint32_t o[kDigitsY][RW];
@@ -716,6 +771,11 @@ __global__ void __launch_bounds__((Geo8<HD, RP, kHalf>::threads), (Geo8<HD, RP, 
           for (int g = 0; g < kDigitsY; ++g) tc::tmem_landed<RW>(o[g]);
           const int d = part * 128 + key;
           if (d < HD) {
+            if (had_nan) {
+              const uint32_t nan = nan_rows(p, it, row_base, min(rows, RW), d);
+#pragma unroll
+              for (int n = 0; n < RW; ++n) o[0][n] = nan >> n & 1 ? 0x7fffffffu : o[0][n];
+            }
 #pragma unroll
             for (int n = 0; n < RW; ++n) {
               if (n < rows) {

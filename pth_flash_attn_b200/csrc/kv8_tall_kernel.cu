@@ -241,9 +241,9 @@ __device__ __forceinline__ uint2 widen4(uint32_t w, __half2 factor) {
   const __half2 x = __hmul2(*reinterpret_cast<const __half2*>(&a), factor), y = __hmul2(*reinterpret_cast<const __half2*>(&b), factor);
   return make_uint2(*reinterpret_cast<const uint32_t*>(&x), *reinterpret_cast<const uint32_t*>(&y));
 }
+__device__ __forceinline__ float largest(float4 s) { return max3(fmaxf(s.x, s.y), s.z, s.w); }
 // Exponent e of the power of two that is a step's unit: 2^e >= its largest scale.
-__device__ __forceinline__ int unit_exponent(float4 s) {
-  const float most = fmaxf(fmaxf(fabsf(s.x), fabsf(s.y)), fmaxf(fabsf(s.z), fabsf(s.w)));
+__device__ __forceinline__ int unit_exponent(float most) {
   return min(126, max(-126, (int)((__float_as_uint(most) + 0x7fffffu) >> 23) - 127));
 }
 
@@ -270,7 +270,16 @@ __device__ __forceinline__ float exponentials8(const uint32_t (&r)[64], const fl
   return sum_pairs(sum);
 }
 
-// The digits of a query row, by its thread: returns u x softmax scale x log2(e), NaN for a row that is not finite.
+__device__ __forceinline__ int64_t scale_at(const Kv8Params& p, int kvh, int blk, int slot) {
+  return (int64_t)blk * p.scale_stride_block + (int64_t)((uint32_t)slot / (uint32_t)p.scale_tokens) * p.scale_stride_group + (int64_t)kvh * p.scale_stride_head;
+}
+template <bool kHalf>
+__device__ __forceinline__ float load_elem16(const uint8_t* row, int d) {
+  if constexpr (kHalf) return __half2float(reinterpret_cast<const __half*>(row)[d]);
+  else return __bfloat162float(reinterpret_cast<const __nv_bfloat16*>(row)[d]);
+}
+
+// The digits of a query row, by its thread: returns u x softmax scale x log2(e), below zero for a row that is not finite.
 template <int HD, bool kHalf>
 __device__ __forceinline__ float stage_row(const Kv8Params& p, const uint8_t* row, uint8_t* image) {
   using G = Tall8<HD, kHalf>;
@@ -313,7 +322,36 @@ __device__ __forceinline__ float stage_row(const Kv8Params& p, const uint8_t* ro
 #pragma unroll
     for (int g = 0; g < G::q_digits; ++g) *reinterpret_cast<uint4*>(image + g * G::q_digit + c * 2048) = make_uint4(d[g][0], d[g][1], d[g][2], d[g][3]);
   }
-  return finite ? power_of_two(e) * p.scale_log2 : NAN;
+  return finite ? power_of_two(e) * p.scale_log2 : -1.f;
+}
+
+// A value that is NaN under a key that a row does not see makes the row's sum NaN all the same: its weight is zero, but zero times NaN
+// is NaN.  So a row that finds NaN among its sums adds 32 of them up again, key by key, over the piece's keys [lo, hi) that it sees.
+// (Looking for NaN as V is widened cost every launch: twelve prompts 276 us instead of 237.  A function of its own, which the hot
+// code does not run through; only softmax threads call it, who have more registers than the launch gave.)
+template <int HD, bool kHalf>
+__device__ __noinline__ void sum_again(const Kv8Params& p, const Piece& it, const uint8_t* q_row, int lo, int hi, float ref, int d0, uint32_t* sums) {
+  for (int d = 0; d < 32; ++d) sums[d] = 0u;
+#pragma unroll 1
+  for (int pos = lo; pos < hi; ++pos) {
+    int slot;
+    const int blk = block_of(p, it.r, pos, &slot);
+    if (blk < 0) continue;   // (a value of zero)
+    const int64_t at = (int64_t)blk * p.stride_block + (int64_t)slot * p.stride_slot + (int64_t)it.kvh * p.stride_head, scale = scale_at(p, it.kvh, blk, slot);
+    float s = 0.f;
+#pragma unroll 1
+    for (int d = 0; d < HD; d += 2) {
+      const float2 k = float2_of_e4m3x2(*reinterpret_cast<const uint16_t*>(p.k + at + d));
+      s = fmaf(load_elem16<kHalf>(q_row, d), k.x, s);
+      s = fmaf(load_elem16<kHalf>(q_row, d + 1), k.y, s);
+    }
+    const float w = ex2f(s * p.k_scale[scale] * p.scale_log2 - ref) * p.v_scale[scale];
+    for (int d = 0; d < 32; d += 2) {
+      const float2 v = float2_of_e4m3x2(*reinterpret_cast<const uint16_t*>(p.v + at + d0 + d));
+      sums[d] = __float_as_uint(fmaf(w, v.x, __uint_as_float(sums[d])));
+      sums[d + 1] = __float_as_uint(fmaf(w, v.y, __uint_as_float(sums[d + 1])));
+    }
+  }
 }
 
 template <int HD, bool kHalf>
@@ -333,7 +371,7 @@ __global__ void __launch_bounds__((Tall8<HD, kHalf>::threads), (Tall8<HD, kHalf>
   if (warp == G::mma_warp) {
     if (lane == 0) {
       for (int i = 0; i < G::k_units; ++i) {
-        tc::mbar_init(&bars[G::k_full + i], 4);         // one arrival per run of 16 keys
+        tc::mbar_init(&bars[G::k_full + i], 12);        // one arrival per run of 16 keys, and one per scale
         tc::mbar_init(&bars[G::k_empty + i], G::rts);   // one commit per row tile
       }
       for (int i = 0; i < G::v_units; ++i) {
@@ -349,7 +387,7 @@ __global__ void __launch_bounds__((Tall8<HD, kHalf>::threads), (Tall8<HD, kHalf>
         tc::mbar_init(&bars[G::drained + i], 1);
       }
       for (int i = 0; i < 2 * G::rts; ++i) {
-        tc::mbar_init(&bars[G::s_ready + i], 1);
+        tc::mbar_init(&bars[G::s_ready + i], 2);        // the MMAs are complete; who issued them has seen the step's scales land
         tc::mbar_init(&bars[G::p_ready + i], 128);
         tc::mbar_init(&bars[G::pv_done + i], 1);
       }
@@ -422,19 +460,18 @@ __global__ void __launch_bounds__((Tall8<HD, kHalf>::threads), (Tall8<HD, kHalf>
           ok = false;
           break;
         }
+        // (the unit of V that was free for the last step says that the scales of kScaleSteps steps ago have been read)
+        if (lane < 8) {
+          const float* const base = lane < 4 ? p.k_scale : p.v_scale;
+          copy4(scales + su * 32 + lane * 4, blk >= 0 ? base + scale_at(p, it.kvh, blk, slot) : base, blk >= 0);
+          copies_arrive(&bars[G::k_full + ku]);
+          copies_arrive(&bars[G::scales_full + su]);
+        }
         if (lane < 4) ask(k_map, k_ring + ku * G::raw, &bars[G::k_full + ku]);
         __syncwarp();
         if (asked >= G::v_units) ok = kv16_wait(&bars[G::v_empty + vu], ((asked / G::v_units) - 1) & 1, abort_flag);
         ok = __all_sync(0xffffffffu, ok);
-        // (the unit of V that is free now says that the scales of kScaleSteps steps ago have been read)
-        if (lane >= 4 && lane < 8) {
-          if (ok) ask(v_map, v_ring + vu * G::raw, &bars[G::v_full + vu]);
-        }
-        if (ok && lane < 8) {
-          const int64_t at = (int64_t)max(blk, 0) * p.scale_stride_block + (int64_t)((uint32_t)slot / (uint32_t)p.scale_tokens) * p.scale_stride_group + (int64_t)it.kvh * p.scale_stride_head;
-          copy4(scales + su * 32 + lane * 4, (lane < 4 ? p.k_scale : p.v_scale) + (blk >= 0 ? at : 0), blk >= 0);
-          copies_arrive(&bars[G::scales_full + su]);
-        }
+        if (ok && lane >= 4 && lane < 8) ask(v_map, v_ring + vu * G::raw, &bars[G::v_full + vu]);
         __syncwarp();
       }
     }
@@ -458,7 +495,7 @@ __global__ void __launch_bounds__((Tall8<HD, kHalf>::threads), (Tall8<HD, kHalf>
         const uint32_t vu = step % G::v_units, wu = step % G::w_units, su = step % kScaleSteps;
         ok &= kv16_wait(&bars[G::scales_full + su], (step / kScaleSteps) & 1, abort_flag);
         const float4 vs = *reinterpret_cast<const float4*>(smem + G::scales + su * 32 + 16);
-        unit_e = max(unit_e, unit_exponent(vs));
+        unit_e = max(unit_e, unit_exponent(largest(vs)));
         const float down = power_of_two(-unit_e);
         ok &= kv16_wait(&bars[G::v_full + vu], (step / G::v_units) & 1, abort_flag);
         if (step >= G::w_units) ok &= kv16_wait(&bars[G::w_empty + wu], ((step / G::w_units) - 1) & 1, abort_flag);
@@ -533,6 +570,7 @@ __global__ void __launch_bounds__((Tall8<HD, kHalf>::threads), (Tall8<HD, kHalf>
       }
       tc::mma_commit(&bars[G::k_empty + k_slot]);
       tc::mma_commit(&bars[G::s_ready + 2 * rt + b]);
+      mbar_arrive(&bars[G::s_ready + 2 * rt + b]);
       next_k();
       ++s_qk;
     };
@@ -615,6 +653,7 @@ __global__ void __launch_bounds__((Tall8<HD, kHalf>::threads), (Tall8<HD, kHalf>
         const int row_lo = kv8_low(p, own), row_hi = p.causal ? min(own + 1, it.hi) : it.hi;
         float ref = -INFINITY, l = 0.f;
         int unit_e = -126;
+        const bool not_finite = q_factor < 0.f;
 #pragma unroll 1
         for (int t = 0; t < n_steps; ++t, ++count, ++step) {
           const uint32_t b = 2 * rt + (count & 1), use = count >> 1, su = step % kScaleSteps;
@@ -624,16 +663,14 @@ __global__ void __launch_bounds__((Tall8<HD, kHalf>::threads), (Tall8<HD, kHalf>
             mbar_arrive(&bars[G::p_ready + b]);
             continue;
           }
-          ok &= kv16_wait(&bars[G::scales_full + su], (step / kScaleSteps) & 1, abort_flag);
           tc::fence_after_sync();
           uint32_t r[64];
           tc::tmem_ld32(s_tmem, r);
           tc::tmem_ld32(s_tmem + 32, r + 32);
           const float4 ks = *reinterpret_cast<const float4*>(smem + G::scales + su * 32);
-          const int e = unit_exponent(*reinterpret_cast<const float4*>(smem + G::scales + su * 32 + 16));
-          float factor[4] = {ks.x * q_factor, ks.y * q_factor, ks.z * q_factor, ks.w * q_factor};
-#pragma unroll
-          for (int i = 0; i < 4; ++i) factor[i] = factor[i] < 1e-37f ? 1e-37f : factor[i];   // (a hidden score is -inf under a scale of zero too)
+          const float most = largest(*reinterpret_cast<const float4*>(smem + G::scales + su * 32 + 16));
+          // (never zero: a hidden score is -inf under a scale of zero too)
+          const float factor[4] = {fmaxf(ks.x * q_factor, 1e-37f), fmaxf(ks.y * q_factor, 1e-37f), fmaxf(ks.z * q_factor, 1e-37f), fmaxf(ks.w * q_factor, 1e-37f)};
           tc::tmem_ld_wait<64>(r);
           const int key0 = it.key0 + t * kKeys;
           if (key0 < row_lo || key0 + kKeys > row_hi) {
@@ -655,19 +692,20 @@ __global__ void __launch_bounds__((Tall8<HD, kHalf>::threads), (Tall8<HD, kHalf>
           };
           if (t == 0) {
             ref = maximum();
-            unit_e = e;
+            unit_e = unit_exponent(most);
           }
           uint32_t pk[32];
           float total = exponentials8(r, factor, ref == -INFINITY ? 0.f : -ref, pk);
           const bool outgrown = !(total <= kMostSum) || ref == -INFINITY;
-          const bool larger = e > unit_e;   // (the same in all threads)
+          const bool larger = most > power_of_two(unit_e) && unit_e < 126;   // (the same in all threads)
           if (__any_sync(0xffffffffu, outgrown) || larger) {
+            const int e = max(unit_e, unit_exponent(most));
             const float to = outgrown ? fmaxf(ref, maximum()) : ref;
             const float alpha = to == -INFINITY ? 1.f : ex2f(ref - to);
             ref = to;
             l *= alpha;
             if (t > 0) {   // (PV of what P holds already is complete first)
-              const float both = larger ? alpha * ex2f((float)(unit_e - e)) : alpha;
+              const float both = alpha * ex2f((float)(unit_e - e));
               ok &= kv16_wait(&bars[G::pv_done + (b ^ 1)], ((count - 1) >> 1) & 1, abort_flag);
               tc::fence_after_sync();
 #pragma unroll 1
@@ -681,7 +719,7 @@ __global__ void __launch_bounds__((Tall8<HD, kHalf>::threads), (Tall8<HD, kHalf>
               }
               tc::tmem_st_wait();
             }
-            unit_e = max(unit_e, e);
+            unit_e = e;
             total = exponentials8(r, factor, ref == -INFINITY ? 0.f : -ref, pk);
           }
           l += total;
@@ -693,6 +731,7 @@ __global__ void __launch_bounds__((Tall8<HD, kHalf>::threads), (Tall8<HD, kHalf>
         // ---- the piece's rows ----
         ok &= kv16_wait(&bars[G::pv_done + 2 * rt + ((count - 1) & 1)], ((count - 1) >> 1) & 1, abort_flag);
         tc::fence_after_sync();
+        if (not_finite) l = NAN;
         const bool whole = it.begins && it.ends, live = row < it.rows;
         uint8_t* const out = p.out + (int64_t)token * p.out_stride_token + (int64_t)head * p.out_stride_head;
         float* const lse = p.lse != nullptr ? p.lse + (int64_t)token * p.num_q_heads + head : nullptr;
@@ -718,6 +757,17 @@ __global__ void __launch_bounds__((Tall8<HD, kHalf>::threads), (Tall8<HD, kHalf>
             uint32_t r[32];
             tc::tmem_ld32(o_tmem + c * 32, r);
             tc::tmem_ld_wait<32>(r);
+            float any = 0.f;
+#pragma unroll
+            for (int n = 0; n < 32; ++n) any = fmaf(__uint_as_float(r[n]), 0.f, any);
+            if (__builtin_expect(any != any && l == l, 0)) {   // NaN, which may be of a key that the row does not see
+              uint32_t sums[32];
+              sum_again<HD, kHalf>(p, it, p.q + (int64_t)token * p.q_stride_token + (int64_t)head * p.q_stride_head, max(row_lo, it.key0),
+                                   min(min(row_hi, it.hi), it.key0 + it.tiles * kTile), ref == -INFINITY ? 0.f : ref, c * 32, sums);
+#pragma unroll
+              for (int n = 0; n < 32; ++n) r[n] = __float_as_uint(__uint_as_float(sums[n]) * power_of_two(-unit_e));
+            }
+            __syncwarp();
             if (whole) {
               float o[32];
 #pragma unroll

@@ -34,21 +34,30 @@ def _gathered(cells, scales, table, at):
     return torch.where(known[:, None, None], c, 0.0), torch.where(known[:, None], s, 0.0)
 
 
-def reference(q, k_cache, v_cache, k_scale, v_scale, table, kv_lens, starts, scale, window=0, causal=True):
+def _powers_of_two(scale):
+    seen = scale[scale.isfinite()]
+    return bool((torch.frexp(seen)[0] == 0.5).all())
+
+
+def reference(q, k_cache, v_cache, k_scale, v_scale, table, kv_lens, starts, scale, window=0, causal=True, tall=False):
     """``out``, ``lse`` in 64 bits, and per element the bound on a kernel's error, from these roundings (e = 2^-24):
 
     * the result's own, u |out|;
-    * queries as sums of e4m3 digits: of 2^-21 of a row's largest (bf16, two digits: exact above 2^-14 of it) or 2^-25 (fp16, three),
-      times sum |k| in a score;
+    * queries as sums of e4m3 digits, whose smallest step is 2^-9.  Few rows: digits scaled by 16 each, the row's largest in [128, 256): off
+      by 2^-10 / 16 with two (bf16), by 2^-10 / 256 with three (fp16), 2^-21 and 2^-25 of the row's largest.  Many rows (``tall``): digits of one
+      unit, the largest in (224, 448]: off by 2^-10, 2^-17 of it.  Times sum |k| in a score;
     * scores: D + 8 32-bit roundings of the sum, and 8 of the score and its distance from the row's bound;
-    * weights p scale_V as three digits: 2^-12 of one, and 2^-24 of the largest weight times the largest scale where they are small;
+    * weights: fp16, 2^-11 of one.  Few rows: of p scale_V, in digits, off by 2^-18 where they are small, of a row's largest between 2^6 and
+      2^8, times the largest scale to the next power of two.  Many rows: of p, off by 2^-25 where they are small, of a largest of 2^7 or
+      more; and scale_V c_V in fp16, 2^-11 each of the scale and the product where the scale is no power of two;
     * the sums over n keys, n + 8 roundings, and 2^-21 for the exponentials and the quotient.
     """
     dev = q.device
     T, Hq, D = q.shape
     Hkv, page = k_cache.shape[2], k_cache.shape[1]
     G, u, e = Hq // Hkv, ROUNDING[q.dtype], 2.0 ** -24
-    digit = 2.0 ** -21 if q.dtype == torch.bfloat16 else 2.0 ** -25
+    digit = 2.0 ** -17 if tall else 2.0 ** -21 if q.dtype == torch.bfloat16 else 2.0 ** -25
+    weight = 2.0 ** -11 + (0.0 if not tall or _powers_of_two(v_scale) else 2.0 ** -10)
     out = torch.zeros((T, Hq, D), dtype=torch.float64, device=dev)
     lse = torch.full((T, Hq), -math.inf, dtype=torch.float64, device=dev)
     out_tol, lse_tol = torch.zeros_like(out), torch.zeros_like(lse)
@@ -78,12 +87,12 @@ def reference(q, k_cache, v_cache, k_scale, v_scale, table, kv_lens, starts, sca
         p = torch.softmax(s, -1).masked_fill(empty[:, None, None, None], 0.0)
         o = torch.einsum("thgj,jhd->thgd", p, v)
         spread = torch.einsum("thgj,jhd->thgd", p, v.abs())
-        # weights far below the largest: 2^-24 of it, times twice the largest scale (the unit is the next power of two)
+        # weights far below the largest: 2^-24 of it (2^-18 / 2^6), times twice the largest scale (the unit is the next power of two)
         small = 2.0 ** -24 * p.amax(-1)[..., None] * 2 * vs.masked_fill(~used[:, None], 0.0).amax(0)[None, :, None, None] \
             * torch.einsum("tj,jhd->thd", seen.double(), vc.abs())[:, :, None]
         sums = (n + 8) * e + 2.0 ** -21
         out[t0:t1] = o.reshape(t1 - t0, Hq, D)
-        out_tol[t0:t1] = (u * o.abs() + (2.0 ** -12 + 2 * score_err[..., None] + 2 * sums) * spread + small).reshape(t1 - t0, Hq, D)
+        out_tol[t0:t1] = (u * o.abs() + (weight + 2 * score_err[..., None] + 2 * sums) * spread + small).reshape(t1 - t0, Hq, D)
         logs = torch.logsumexp(s, -1)
         lse[t0:t1] = logs.reshape(t1 - t0, Hq)
         lse_tol[t0:t1] = (score_err + sums + 4 * e * (logs.abs() + 1)).masked_fill(empty[:, None, None], 0.0).reshape(t1 - t0, Hq)

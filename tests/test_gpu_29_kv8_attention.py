@@ -66,8 +66,12 @@ class Batch:
     def check(self, window=0, causal=True, what=""):
         torch.cuda.synchronize()
         assert capi.load_library().device_status() == 0
-        check(self.out, self.lse, reference(self.q, self.k, self.v, self.ks, self.vs, self.table, self.kv_lens, self.starts, self.D ** -0.5,
-                                            window, causal), what)
+        check(self.out, self.lse, self.reference(window, causal), what)
+
+    def reference(self, window=0, causal=True):
+        rows = self.longest_q * (self.q.shape[1] // self.k.shape[2])
+        tall = self.longest_q > 1 and rows >= (17 if self.D == 64 else 33)   # (the rule of kv8_api.cu)
+        return reference(self.q, self.k, self.v, self.ks, self.vs, self.table, self.kv_lens, self.starts, self.D ** -0.5, window, causal, tall)
 
 
 EDGES = [0, 1, 15, 16, 17, 127, 128, 129, 255, 300, 0, 1000]
@@ -182,6 +186,66 @@ def test_prompts(Hq, Hkv, D, causal, window):
     Batch(kv, q, Hq, Hkv, D, seed=D).attend(window, causal).check(window, causal)
 
 
+@pytest.mark.parametrize("dtype", [BF16, F16])
+@pytest.mark.parametrize("Hq,Hkv,D,page,group,layout", [(32, 8, 128, 64, 16, "NHD"), (8, 1, 128, 16, 16, "HND"), (16, 16, 64, 48, 48, "NHD"),
+                                                        (6, 1, 256, 816, 48, "HND"), (5, 5, 128, 80, 80, "NHD")])
+def test_long_prompts(Hq, Hkv, D, page, group, layout, dtype):
+    """Row tiles that several CTAs share, ragged, over pages of every kind."""
+    Batch([2300, 700, 64, 1], [500, 700, 1, 1], Hq, Hkv, D, dtype, page=page, group=group, layout=layout, seed=page, pad=16 if page == 48 else 0).attend().check()
+
+
+@pytest.mark.parametrize("foreign", [False, True])
+@pytest.mark.parametrize("D", [64, 128, 256])
+def test_prompts_over_scales_that_differ(D, foreign):
+    Batch([1000, 300], [200, 300], 8, 2, D, scales=(-14, 1), foreign=foreign, seed=7, scale_up=2.0 ** -3).attend().check()
+
+
+@pytest.mark.parametrize("size", [-100, -30, 30, 90])
+def test_prompts_over_scales_of_any_size(size):
+    b = Batch([300, 129], [100, 129], 8, 2, 128, scales=(-7, -6), seed=4)
+    b.vs.mul_(2.0 ** size)
+    b.attend().check()
+
+
+def test_prompts_of_rows_of_their_own_size():
+    b = Batch([500, 64], [100, 64], 8, 2, 128, seed=2)
+    b.q[10, 1] *= 2.0 ** -20
+    b.q[11, 2] *= 2.0 ** 8
+    b.q[12, 3] = 0.0
+    b.attend().check()
+
+
+def test_prompts_with_a_later_maximum():
+    n, D = 2000, 128
+    b = Batch([n], [120], 4, 1, D, seed=3, scales=(-7, -6))
+    at = torch.arange(n, device="cuda")
+    k = torch.zeros((n, 1, D), device="cuda")
+    k[..., 0] = (at.float() / n * 440)[:, None]
+    b.k[b.table[0].cuda().long()[at // 32], at % 32] = k.to(E4M3)
+    b.q.zero_()
+    b.q[..., 0] = 200.0
+    b.attend().check()
+
+
+def test_prompts_over_bad_blocks_and_past_the_table():
+    b = Batch([400, 300, 256], [100, 300, 200], 8, 2, 128, seed=6)
+    b.table[0, 1], b.table[1, 2], b.table[2, 7] = -1, 1 << 20, 77777
+    b.bt = b.table.cuda()
+    # tokens whose own positions are past the row of the table: they see what there is
+    b.kv_lens[2] = b.table.shape[1] * 32 + 50
+    b.lens[2] = b.kv_lens[2]
+    b.table[2, 8:], b.bt[2, 8:] = -1, -1
+    b.attend().check()
+
+
+def test_more_tokens_than_keys():
+    """Lengths below the number of tokens: the first of them are at negative positions and see nothing."""
+    b = Batch([40, 3, 0], [60, 5, 4], 8, 2, 128, seed=1)
+    b.attend().check()
+    Batch([40, 3, 0], [4, 4, 4], 8, 2, 128, seed=1).attend().check()
+    Batch([2, 1, 0], [4, 4, 4], 8, 2, 128, seed=1).attend().check()
+
+
 def test_one_token_through_both_calls():
     """A single token's call and a call of one token each give the same."""
     b = Batch(EDGES, [1] * len(EDGES), 8, 2, 128, seed=1)
@@ -269,3 +333,54 @@ def test_offsets_past_32_bits():
     b.k = b.v = cells
     b.ks = b.vs = scale
     b.decode().check()
+
+
+def _sees(b, r, i, key, window, causal):
+    """Whether token i of request r sees a key."""
+    own = b.kv_lens[r] - (b.starts[r + 1] - b.starts[r]) + i
+    return (not causal or key <= own) and (not window or key > own - window) and key < b.kv_lens[r]
+
+
+@pytest.mark.parametrize("Hq,Hkv,D", [(8, 2, 128), (8, 8, 64), (12, 2, 256), (16, 2, 128)])
+@pytest.mark.parametrize("kv,q", [([300, 4, 140], [4, 3, 2]), ([700, 300, 90], [260, 300, 33])])
+@pytest.mark.parametrize("causal,window", [(True, 0), (True, 70), (False, 50)])
+def test_nan_under_keys_that_some_tokens_do_not_see(Hq, Hkv, D, kv, q, causal, window):
+    """NaN among the keys and values of a request's own tokens: it reaches the tokens that see it, in a value only its dimension,
+    and no other.  (Values: their weight of zero times NaN would be NaN.)"""
+    b = Batch(kv, q, Hq, Hkv, D, seed=D, spare=0)
+    clean = b.reference(window, causal)
+    want_out, want_lse = (x.clone() for x in clean[:2])
+    gen = torch.Generator().manual_seed(1)
+    G = Hq // Hkv
+    for r, (n, t) in enumerate(zip(kv, q)):
+        for key in {n - 1, n - t // 2 - 1, max(0, n - t - 3), max(0, n - window), int(torch.randint(n, (1,), generator=gen))}:
+            h, d = int(torch.randint(Hkv, (1,), generator=gen)), int(torch.randint(D, (1,), generator=gen))
+            block, slot = int(b.table[r, key // b.page]), key % b.page
+            b.v[block, slot, h, d] = math.nan
+            for i in range(t):
+                if _sees(b, r, i, key, window, causal):
+                    want_out[b.starts[r] + i, h * G:(h + 1) * G, d] = math.nan
+        key, h = n - 1 - t // 3, int(torch.randint(Hkv, (1,), generator=gen))
+        b.k[int(b.table[r, key // b.page]), key % b.page, h, 3] = math.nan
+        for i in range(t):
+            if _sees(b, r, i, key, window, causal):
+                want_out[b.starts[r] + i, h * G:(h + 1) * G] = math.nan
+                want_lse[b.starts[r] + i, h * G:(h + 1) * G] = math.nan
+    b.attend(window, causal)
+    torch.cuda.synchronize()
+    assert capi.load_library().device_status() == 0
+    assert torch.equal(b.out.isnan(), want_out.isnan()) and torch.equal(b.lse.isnan(), want_lse.isnan())
+    ok = ~want_out.isnan()
+    assert bool(((b.out.double() - clean[0]).abs() <= clean[2])[ok].all())
+
+
+def test_nan_among_the_keys_that_all_tokens_see():
+    """NaN far from the tokens' own keys, where nothing is masked; and for a single token."""
+    for q in ([1, 1], [4, 4], [200, 1]):
+        b = Batch([900, 500], q, 8, 2, 128, seed=3)
+        block, slot = int(b.table[0, 100 // b.page]), 100 % b.page
+        b.v[block, slot, 1, 7] = math.nan
+        b.attend() if max(q) > 1 else b.decode()
+        nan = torch.zeros_like(b.out, dtype=torch.bool)
+        nan[:q[0], 4:8, 7] = True
+        assert torch.equal(b.out.isnan(), nan)
