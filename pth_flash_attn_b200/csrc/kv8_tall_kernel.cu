@@ -283,29 +283,31 @@ __device__ __forceinline__ float load_elem16(const uint8_t* row, int d) {
 template <int HD, bool kHalf>
 __device__ __forceinline__ float stage_row(const Kv8Params& p, const uint8_t* row, uint8_t* image) {
   using G = Tall8<HD, kHalf>;
-  uint4 w[HD / 8];
-#pragma unroll
-  for (int c = 0; c < HD / 8; ++c) w[c] = __ldg(reinterpret_cast<const uint4*>(row) + c);
+  const uint4* const in = reinterpret_cast<const uint4*>(row);
   uint32_t m = 0;   // largest magnitudes, as 16-bit integers
 #pragma unroll
   for (int c = 0; c < HD / 8; ++c) {
-    m = __vimax3_u16x2(m, w[c].x & 0x7fff7fffu, w[c].y & 0x7fff7fffu);
-    m = __vimax3_u16x2(m, w[c].z & 0x7fff7fffu, w[c].w & 0x7fff7fffu);
+    const uint4 w = __ldg(in + c);
+    m = __vimax3_u16x2(m, w.x & 0x7fff7fffu, w.y & 0x7fff7fffu);
+    m = __vimax3_u16x2(m, w.z & 0x7fff7fffu, w.w & 0x7fff7fffu);
   }
   const uint32_t top16 = max(m & 0xffffu, m >> 16);
   const bool finite = top16 < (kHalf ? 0x7c00u : 0x7f80u);
   const float top = kHalf ? __half2float(__ushort_as_half((unsigned short)top16)) : __uint_as_float(top16 << 16);
   const int e = min(119, max(-119, e4m3_exponent(top)));
   const float up = power_of_two(-e);
-#pragma unroll
+  // (Rolled at 64 dims, from the first level cache: what runs once a piece costs by its instructions, which come from beyond theirs.  Twelve
+  // prompts of 37 to 2,500 tokens, rolled and not, us: 243 / 250 at 64 dims, 446 / 405 at 128.)
+#pragma unroll(HD == 64 ? 1 : HD / 16)
   for (int c = 0; c < HD / 16; ++c) {
-    const uint32_t in[8] = {w[2 * c].x, w[2 * c].y, w[2 * c].z, w[2 * c].w, w[2 * c + 1].x, w[2 * c + 1].y, w[2 * c + 1].z, w[2 * c + 1].w};
+    const uint4 w0 = __ldg(in + 2 * c), w1 = __ldg(in + 2 * c + 1);
+    const uint32_t pairs[8] = {w0.x, w0.y, w0.z, w0.w, w1.x, w1.y, w1.z, w1.w};
     uint32_t d[G::q_digits][4];
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
       float2 f;
-      if constexpr (kHalf) f = __half22float2(*reinterpret_cast<const __half2*>(&in[i]));
-      else f = make_float2(__uint_as_float(in[i] << 16), __uint_as_float(in[i] & 0xffff0000u));
+      if constexpr (kHalf) f = __half22float2(*reinterpret_cast<const __half2*>(&pairs[i]));
+      else f = make_float2(__uint_as_float(pairs[i] << 16), __uint_as_float(pairs[i] & 0xffff0000u));
       f.x *= up;
       f.y *= up;
 #pragma unroll
@@ -674,12 +676,27 @@ __global__ void __launch_bounds__((Tall8<HD, kHalf>::threads), (Tall8<HD, kHalf>
           tc::tmem_ld_wait<64>(r);
           const int key0 = it.key0 + t * kKeys;
           if (key0 < row_lo || key0 + kKeys > row_hi) {
-            const int lo = row_lo - key0, hi = row_hi - key0;
+            // bit n: key n is seen
+            const int lo = min(max(row_lo - key0, 0), 64), hi = min(max(row_hi - key0, 0), 64);
+            const uint64_t from = lo < 64 ? ~0ull << lo : 0ull, upto = hi < 64 ? (1ull << hi) - 1 : ~0ull, seen = from & upto;
 #pragma unroll
             for (int n = 0; n < 64; ++n)
-              if (n < lo || n >= hi) r[n] = 0xff800000u;  // -inf
+              r[n] = (uint32_t)(n < 32 ? seen : seen >> 32) >> (n & 31) & 1u ? r[n] : 0xff800000u;  // -inf
           }
-          auto maximum = [&] {
+          uint32_t pk[32];
+          float total;
+          // (One copy of the code for a step's first look and its second: the instruction caches are small.)
+          bool move = t == 0;
+#pragma unroll 1
+          for (bool again = false;; again = true) {
+            bool outgrown = true;
+            if (!move) {
+              total = exponentials8(r, factor, ref == -INFINITY ? 0.f : -ref, pk);
+              if (again) break;
+              outgrown = !(total <= kMostSum) || ref == -INFINITY;
+              if (!__any_sync(0xffffffffu, outgrown) && !(most > power_of_two(unit_e) && unit_e < 126)) break;
+            }
+            move = false;
             float mx[4];
 #pragma unroll
             for (int g = 0; g < 4; ++g) {
@@ -688,24 +705,14 @@ __global__ void __launch_bounds__((Tall8<HD, kHalf>::threads), (Tall8<HD, kHalf>
               for (int n = 0; n < 16; n += 2) mx[g] = max3(mx[g], __uint_as_float(r[16 * g + n]), __uint_as_float(r[16 * g + n + 1]));
               mx[g] *= factor[g];
             }
-            return max3(fmaxf(mx[0], mx[1]), mx[2], mx[3]) - kGainP;
-          };
-          if (t == 0) {
-            ref = maximum();
-            unit_e = unit_exponent(most);
-          }
-          uint32_t pk[32];
-          float total = exponentials8(r, factor, ref == -INFINITY ? 0.f : -ref, pk);
-          const bool outgrown = !(total <= kMostSum) || ref == -INFINITY;
-          const bool larger = most > power_of_two(unit_e) && unit_e < 126;   // (the same in all threads)
-          if (__any_sync(0xffffffffu, outgrown) || larger) {
+            const float to = outgrown ? fmaxf(ref, max3(fmaxf(mx[0], mx[1]), mx[2], mx[3]) - kGainP) : ref;
             const int e = max(unit_e, unit_exponent(most));
-            const float to = outgrown ? fmaxf(ref, maximum()) : ref;
             const float alpha = to == -INFINITY ? 1.f : ex2f(ref - to);
+            const float both = alpha * ex2f((float)(unit_e - e));
             ref = to;
             l *= alpha;
+            unit_e = e;
             if (t > 0) {   // (PV of what P holds already is complete first)
-              const float both = alpha * ex2f((float)(unit_e - e));
               ok &= kv16_wait(&bars[G::pv_done + (b ^ 1)], ((count - 1) >> 1) & 1, abort_flag);
               tc::fence_after_sync();
 #pragma unroll 1
@@ -719,8 +726,6 @@ __global__ void __launch_bounds__((Tall8<HD, kHalf>::threads), (Tall8<HD, kHalf>
               }
               tc::tmem_st_wait();
             }
-            unit_e = e;
-            total = exponentials8(r, factor, ref == -INFINITY ? 0.f : -ref, pk);
           }
           l += total;
           tc::tmem_st32(s_tmem, pk);
