@@ -29,6 +29,11 @@ __device__ __forceinline__ uint32_t e4m3x2(float a, float b) {
   asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(r) : "f"(b), "f"(a));
   return r;
 }
+__device__ __forceinline__ uint32_t e4m3x2_of_f16x2(__half2 h) {
+  uint16_t r;
+  asm("cvt.rn.satfinite.e4m3x2.f16x2 %0, %1;" : "=h"(r) : "r"(*reinterpret_cast<const uint32_t*>(&h)));
+  return r;
+}
 // Two e4m3 numbers (of the low half of w) as fp16, which holds them all.
 __device__ __forceinline__ uint32_t f16x2_of_e4m3x2(uint32_t w) {
   uint32_t r;

@@ -145,11 +145,9 @@ __device__ __forceinline__ void weight_digits2(float a, float b, uint32_t (&d)[k
   __half2 h = __floats2half2_rn(a, b);
 #pragma unroll
   for (int i = 0; i < kDigitsY; ++i) {
-    uint16_t r;
-    asm("cvt.rn.satfinite.e4m3x2.f16x2 %0, %1;" : "=h"(r) : "r"(*reinterpret_cast<const uint32_t*>(&h)));
-    d[i] = r;
+    d[i] = e4m3x2_of_f16x2(h);
     if (i + 1 < kDigitsY) {
-      const uint32_t f = f16x2_of_e4m3x2(r);
+      const uint32_t f = f16x2_of_e4m3x2(d[i]);
       const __half2 sixteen = __float2half2_rn(16.f);
       h = __hfma2(*reinterpret_cast<const __half2*>(&f), __float2half2_rn(-16.f), __hmul2(h, sixteen));   // (exact)
     }

@@ -308,16 +308,14 @@ __device__ __forceinline__ float stage_row(const Kv8Params& p, const uint8_t* ro
       float2 f;
       if constexpr (kHalf) f = __half22float2(*reinterpret_cast<const __half2*>(&pairs[i]));
       else f = make_float2(__uint_as_float(pairs[i] << 16), __uint_as_float(pairs[i] & 0xffff0000u));
-      f.x *= up;
-      f.y *= up;
+      __half2 h = __floats2half2_rn(f.x * up, f.y * up);   // (exactly, down to 2^-24, which is far below a digit's last step)
 #pragma unroll
       for (int g = 0; g < G::q_digits; ++g) {
-        const uint32_t b = e4m3x2(f.x, f.y);
+        const uint32_t b = e4m3x2_of_f16x2(h);
         if (i & 1) d[g][i / 2] |= b << 16; else d[g][i / 2] = b;
         if (g + 1 < G::q_digits) {
-          const float2 done = float2_of_e4m3x2(b);
-          f.x -= done.x;
-          f.y -= done.y;
+          const uint32_t done = f16x2_of_e4m3x2(b);
+          h = __hsub2(h, *reinterpret_cast<const __half2*>(&done));
         }
       }
     }
@@ -755,16 +753,17 @@ __global__ void __launch_bounds__((Tall8<HD, kHalf>::threads), (Tall8<HD, kHalf>
           }
         };
         if (!padding) {
-          const float unit = power_of_two(unit_e), inv = l == 0.f ? 0.f : 1.f / l;
+          const float unit = power_of_two(unit_e), factor = whole ? (l == 0.f ? 0.f : unit / l) : unit;
           float* const slot = tall8_slot<HD, kHalf>(p, (int)blockIdx.x, it.begins) + row;
 #pragma unroll 1
           for (int c = 0; c < HD / 32; ++c) {
             uint32_t r[32];
             tc::tmem_ld32(o_tmem + c * 32, r);
             tc::tmem_ld_wait<32>(r);
-            float any = 0.f;
+            f32x2 all[2] = {0ull, 0ull};
 #pragma unroll
-            for (int n = 0; n < 32; ++n) any = fmaf(__uint_as_float(r[n]), 0.f, any);
+            for (int n = 0; n < 32; n += 2) all[n / 2 & 1] = add2(all[n / 2 & 1], pair(__uint_as_float(r[n]), __uint_as_float(r[n + 1])));
+            const float any = sum_pairs(all);
             if (__builtin_expect(any != any && l == l, 0)) {   // NaN, which may be of a key that the row does not see
               uint32_t sums[32];
               sum_again<HD, kHalf>(p, it, p.q + (int64_t)token * p.q_stride_token + (int64_t)head * p.q_stride_head, max(row_lo, it.key0),
@@ -773,17 +772,17 @@ __global__ void __launch_bounds__((Tall8<HD, kHalf>::threads), (Tall8<HD, kHalf>
               for (int n = 0; n < 32; ++n) r[n] = __float_as_uint(__uint_as_float(sums[n]) * power_of_two(-unit_e));
             }
             __syncwarp();
-            if (whole) {
-              float o[32];
+            float o[32];
 #pragma unroll
-              for (int n = 0; n < 32; ++n) o[n] = __uint_as_float(r[n]) * inv * unit;
+            for (int n = 0; n < 32; ++n) o[n] = __uint_as_float(r[n]) * factor;
+            if (whole) {
               if (live) {
                 write16(o, c * 32);
                 write16(o + 16, c * 32 + 16);
               }
             } else {
 #pragma unroll
-              for (int n = 0; n < 32; ++n) slot[(c * 32 + n) * RP] = __uint_as_float(r[n]) * unit;
+              for (int n = 0; n < 32; ++n) slot[(c * 32 + n) * RP] = o[n];
             }
           }
           if (whole) {
