@@ -45,13 +45,19 @@ __device__ __forceinline__ Place place_of(const Read8Params& p, int row0, int ro
     lo += last * step;
   }
   if (lane >= rows) return Place{-2, 0};
-  int r = lo, start = __ldg(p.row_start_loc + r), end = __ldg(p.row_start_loc + r + 1);
+  // (steps that grow, then halves: requests without rows may lie between)
+  int r = lo, above = lo + 1;
 #pragma unroll 1
-  while (row >= end && r + 1 < p.num_reqs) {
-    ++r;
-    start = end;
-    end = __ldg(p.row_start_loc + r + 1);
+  for (int step = 1; above < p.num_reqs && __ldg(p.row_start_loc + above) <= row; step *= 2) {
+    r = above;
+    above = step < p.num_reqs - above ? above + step : p.num_reqs;
   }
+#pragma unroll 1
+  while (above - r > 1) {
+    const int middle = r + (above - r) / 2;
+    if (__ldg(p.row_start_loc + middle) <= row) r = middle; else above = middle;
+  }
+  const int start = __ldg(p.row_start_loc + r), end = __ldg(p.row_start_loc + r + 1);
   if (row < start || row >= end || (long long)row - start >= p.max_rows) return Place{-2, 0};
   const long long pos = (long long)__ldg(p.first + r) + ((long long)row - start);
   if (pos < 0 || pos / p.block_size >= p.num_pages) return Place{-1, 0};

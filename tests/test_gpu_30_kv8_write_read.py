@@ -196,3 +196,25 @@ def test_round_trip_error():
     for got, x in zip(out, (w.key, w.value)):
         most = x.float().abs().amax()
         assert bool(((got.float() - x.float()).abs() <= 2.0 ** -4 * x.float().abs() + 2.0 ** -10 * most / 224).all())
+
+
+def test_reads_with_many_requests_without_rows_between():
+    """Requests of no rows, thousands of them between two that have some."""
+    gen = torch.Generator(device="cuda").manual_seed(6)
+    page, Hkv, D, R = 32, 2, 64, 9000
+    cache = make_cache(40, page, 16, Hkv, D)
+    for cells, scale in ((cache[0], cache[2]), (cache[1], cache[3])):
+        cells.copy_((torch.randn(cells.shape, generator=gen, device="cuda") * 100).clamp(-448, 448))
+        scale.copy_(torch.exp2(torch.randint(-12, -5, scale.shape, generator=gen, device="cuda").float()))
+    rows = [0] * R
+    for r, n in ((3, 5), (4, 1), (17, 40), (4099, 2), (8000, 1), (8001, 33), (8999, 7)):
+        rows[r] = n
+    starts = [0]
+    for n in rows:
+        starts.append(starts[-1] + n)
+    table = torch.randint(0, 40, (R, 2), generator=torch.Generator().manual_seed(7), dtype=torch.int32)
+    first = [r % 11 for r in range(R)]
+    out = [torch.full((starts[-1], Hkv, D), 7.0, dtype=BF16, device="cuda") for _ in range(2)]
+    want = [read_reference(c, s, table, first, starts, 40, o) for c, s, o in ((cache[0], cache[2], out[0]), (cache[1], cache[3], out[1]))]
+    ops.kv8_read(*out, *cache, table.cuda(), _i32(first), _i32(starts), 40)
+    assert torch.equal(out[0], want[0]) and torch.equal(out[1], want[1])
