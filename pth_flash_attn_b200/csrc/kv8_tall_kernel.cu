@@ -241,7 +241,13 @@ __device__ __forceinline__ uint2 widen4(uint32_t w, __half2 factor) {
   const __half2 x = __hmul2(*reinterpret_cast<const __half2*>(&a), factor), y = __hmul2(*reinterpret_cast<const __half2*>(&b), factor);
   return make_uint2(*reinterpret_cast<const uint32_t*>(&x), *reinterpret_cast<const uint32_t*>(&y));
 }
-__device__ __forceinline__ float largest(float4 s) { return max3(fmaxf(s.x, s.y), s.z, s.w); }
+__device__ __forceinline__ float largest(float4 s) { return max3(fmaxf(fabsf(s.x), fabsf(s.y)), fabsf(s.z), fabsf(s.w)); }
+// A run's factor of its scores: never zero, since a hidden score is -inf under a scale of zero too; NaN stays NaN.
+__device__ __forceinline__ float score_factor(float scale, float q_factor) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(scale * q_factor), "f"(1e-37f));
+  return r;
+}
 // Exponent e of the power of two that is a step's unit: 2^e >= its largest scale.
 __device__ __forceinline__ int unit_exponent(float most) {
   return min(126, max(-126, (int)((__float_as_uint(most) + 0x7fffffu) >> 23) - 127));
@@ -669,8 +675,7 @@ __global__ void __launch_bounds__((Tall8<HD, kHalf>::threads), (Tall8<HD, kHalf>
           tc::tmem_ld32(s_tmem + 32, r + 32);
           const float4 ks = *reinterpret_cast<const float4*>(smem + G::scales + su * 32);
           const float most = largest(*reinterpret_cast<const float4*>(smem + G::scales + su * 32 + 16));
-          // (never zero: a hidden score is -inf under a scale of zero too)
-          const float factor[4] = {fmaxf(ks.x * q_factor, 1e-37f), fmaxf(ks.y * q_factor, 1e-37f), fmaxf(ks.z * q_factor, 1e-37f), fmaxf(ks.w * q_factor, 1e-37f)};
+          float factor[4] = {score_factor(ks.x, q_factor), score_factor(ks.y, q_factor), score_factor(ks.z, q_factor), score_factor(ks.w, q_factor)};
           tc::tmem_ld_wait<64>(r);
           const int key0 = it.key0 + t * kKeys;
           if (key0 < row_lo || key0 + kKeys > row_hi) {
@@ -680,6 +685,8 @@ __global__ void __launch_bounds__((Tall8<HD, kHalf>::threads), (Tall8<HD, kHalf>
 #pragma unroll
             for (int n = 0; n < 64; ++n)
               r[n] = (uint32_t)(n < 32 ? seen : seen >> 32) >> (n & 31) & 1u ? r[n] : 0xff800000u;  // -inf
+#pragma unroll
+            for (int g = 0; g < 4; ++g) factor[g] = (uint32_t)(seen >> 16 * g) & 0xffffu ? factor[g] : 1.f;   // (a scale that the row does not see)
           }
           uint32_t pk[32];
           float total;

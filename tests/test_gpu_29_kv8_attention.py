@@ -384,3 +384,38 @@ def test_nan_among_the_keys_that_all_tokens_see():
         nan = torch.zeros_like(b.out, dtype=torch.bool)
         nan[:q[0], 4:8, 7] = True
         assert torch.equal(b.out.isnan(), nan)
+
+
+@pytest.mark.parametrize("q_lens", [[1, 1], [4, 3], [200, 130]])
+def test_scales_that_are_broadcast(q_lens):
+    """One scale for a whole cache: strides of zero."""
+    b = Batch([300, 140], q_lens, 8, 2, 128, seed=8)
+    b.ks, b.vs = (torch.full((1, 1, 1), s, device="cuda").expand(b.ks.shape) for s in (2.0 ** -7, 0.013))
+    b.attend().check()
+
+
+@pytest.mark.parametrize("D", [64, 128, 256])
+def test_a_scale_that_is_no_number_reaches_the_rows_that_see_it(D):
+    """Prompts over keys, and values, of which a block's scale is NaN: NaN where a row sees the block, the others as they are."""
+    for which in ("ks", "vs"):
+        b = Batch([200, 90], [200, 60], 16, 2, D, seed=D)
+        page, slot = divmod(100, b.page)
+        scales = getattr(b, which)
+        was = scales.clone()
+        scales[int(b.table[0][page]), slot // 16] = math.nan
+        b.attend()
+        torch.cuda.synchronize()
+        assert capi.load_library().device_status() == 0
+        first = 100 // 16 * 16
+        assert bool(b.out[first:200].isnan().all()) and bool(b.out[:first].isfinite().all()) and bool(b.out[200:].isfinite().all())
+        setattr(b, which, was)
+        want = b.reference()
+        keep = torch.cat([torch.arange(first), torch.arange(200, 260)]).cuda()
+        check(b.out[keep], b.lse[keep], tuple(x[keep] for x in want))
+
+
+def test_scales_of_minus_zero():
+    """Values of a scale of -0 are zeros, and take nothing from the blocks behind them."""
+    b = Batch([400, 90], [300, 60], 16, 2, 128, seed=2)
+    b.vs[b.table[0].cuda().long()[:4]] = -0.0
+    b.attend().check()
