@@ -503,7 +503,7 @@ int32_t pthb200_kv8_read(const PthB200Kv8ReadArgs* args, void* stream);
  *                       not computed.
  * A token that sees no key gets out = 0 and a log-sum-exp of -inf.  lse (optional) is the natural logarithm, dense
  * [num_tokens, num_q_heads].  Keys past the row of the block table do not exist, and a block outside [0, num_blocks) stands for
- * keys and values of zero.  Scales are positive finite numbers.  Statistics and sums have 32 bits; out is rounded once.
+ * keys and values of zero.  Scales are positive finite numbers.  out must not overlap the inputs.  Statistics and sums have 32 bits; out is rounded once.
  *
  * workspace: pthb200_kv8_workspace_bytes of it, 256-byte aligned, zeroed ONCE before its first use; a call leaves it ready for the
  * next one.  Calls that may overlap need workspaces of their own.  (Zero it again after pthb200_device_status has reported a

@@ -49,6 +49,7 @@ template <class Args>
 int32_t check_shape(const Args* a) {
   KV8_REQUIRE(is_head_size(a->head_size), "head_size must be 64, 128 or 256");
   KV8_REQUIRE(a->num_kv_heads >= 1 && a->block_size >= 1 && a->num_blocks >= 1, "num_kv_heads, block_size and num_blocks must be >= 1");
+  KV8_REQUIRE(a->num_kv_heads <= 65536, "num_kv_heads must be <= 65536");
   KV8_REQUIRE(a->scale_tokens >= 16 && a->scale_tokens % 16 == 0 && a->block_size % a->scale_tokens == 0,
               "scale_tokens must be a multiple of 16 that divides block_size");
   KV8_REQUIRE(a->num_reqs >= 0 && a->num_pages >= 0 && a->block_table_row_stride >= 0, "num_reqs, num_pages and block_table_row_stride must be >= 0");

@@ -236,7 +236,7 @@ cudaError_t launch_for(const Write8Params& p, bool wide, cudaStream_t stream) {
   const int64_t units = numbers * 2 * p.num_kv_heads;
   const bool cta = p.scale_tokens > 32 && p.max_query_len > 1;
   const int64_t ctas = cta ? units : (units + kWarps - 1) / kWarps;
-  if (ctas > 0x7fffffff) return cudaErrorInvalidConfiguration;
+  if (numbers > 0x7fffffff || ctas > 0x7fffffff) return cudaErrorInvalidConfiguration;
   const dim3 grid((unsigned)ctas), block(kWarps * 32);
   if (cta) return pdl_launch(wide ? kv8_writer_kernel<HD, kDtype, true, true> : kv8_writer_kernel<HD, kDtype, false, true>, grid, block, 0, stream, p);
   return pdl_launch(wide ? kv8_writer_kernel<HD, kDtype, true, false> : kv8_writer_kernel<HD, kDtype, false, false>, grid, block, 0, stream, p);

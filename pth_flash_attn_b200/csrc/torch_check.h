@@ -58,6 +58,11 @@ struct Check {
     STD_TORCH_CHECK(t.numel() == 0 || t.stride(t.dim() - 1) == 1, op, name, " must have stride 1 in its last dimension, got ",
                     t.stride(t.dim() - 1));
   }
+  // of a tensor that the op writes: every element has a place of its own, as far as strides of zero go
+  void written(const Tensor& t, const char* name) const {
+    for (int64_t d = 0; d < t.dim(); ++d)
+      STD_TORCH_CHECK(t.size(d) <= 1 || t.stride(d) != 0 || t.numel() == 0, op, name, " is written and must not have stride 0, as in dimension ", d);
+  }
   void device(const Tensor& t, const Tensor& as, const char* name, const char* of) const {
     // (a CPU tensor's index is -1)
     STD_TORCH_CHECK(t.get_device_index() == as.get_device_index(), op, name, " must be on the same device as ", of);

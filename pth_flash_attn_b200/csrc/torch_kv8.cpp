@@ -106,6 +106,10 @@ void kv8_write(const Tensor& key, const Tensor& value, Tensor& k_cache, Tensor& 
   check_rows(c, key, value, k_cache);
   check_table(c, block_table, seq_lens, "seq_lens");
   check_starts(c, query_start_loc, seq_lens.size(0), max_query_len, key.size(0), "query_start_loc", "max_query_len");
+  c.written(k_cache, "k_cache");
+  c.written(v_cache, "v_cache");
+  c.written(k_scale, "k_scale");
+  c.written(v_scale, "v_scale");
   check_devices(c, {{&value, "value"}, {&k_cache, "k_cache"}, {&v_cache, "v_cache"}, {&k_scale, "k_scale"}, {&v_scale, "v_scale"},
                     {&block_table, "block_table"}, {&seq_lens, "seq_lens"}, {&query_start_loc, "query_start_loc"}}, key, "key");
   int32_t device = 0;
@@ -130,6 +134,8 @@ void kv8_read(Tensor& key, Tensor& value, const Tensor& k_cache, const Tensor& v
   check_rows(c, key, value, k_cache);
   check_table(c, block_table, first, "first");
   check_starts(c, row_start_loc, first.size(0), max_rows, key.size(0), "row_start_loc", "max_rows");
+  c.written(key, "key");
+  c.written(value, "value");
   check_devices(c, {{&value, "value"}, {&k_cache, "k_cache"}, {&v_cache, "v_cache"}, {&k_scale, "k_scale"}, {&v_scale, "v_scale"},
                     {&block_table, "block_table"}, {&first, "first"}, {&row_start_loc, "row_start_loc"}}, key, "key");
   int32_t device = 0;
@@ -163,6 +169,7 @@ PthB200Kv8Args attention_args(const Check& c, Tensor& out, Tensor& lse, const Te
   c.size(out, 1, Hq, "out", "Hq");
   c.size(out, 2, D, "out", "D");
   c.inner(out, "out");
+  c.written(out, "out");
   STD_TORCH_CHECK(Hq >= 1 && Hq % Hkv == 0, c.op, "Hq = ", Hq, " must be a positive multiple of Hkv = ", Hkv);
   STD_TORCH_CHECK(Hq / Hkv <= 64, c.op, "G = Hq/Hkv = ", Hq / Hkv, " exceeds the supported maximum 64");
   c.dtype(lse, ScalarType::Float, "lse");
@@ -254,6 +261,7 @@ void rotary(Tensor& q_out, Tensor& k_out, const Tensor& q, const Tensor& k, cons
     c.size(*out[i], 1, in[i]->size(1), names[i], i == 0 ? "q.size(1)" : "k.size(1)");
     c.size(*out[i], 2, D, names[i], "D");
     c.inner(*out[i], names[i]);
+    c.written(*out[i], names[i]);
     if (in[i]->numel() != 0 && in[i]->data_ptr() == out[i]->data_ptr())
       STD_TORCH_CHECK(in[i]->stride(0) == out[i]->stride(0) && in[i]->stride(1) == out[i]->stride(1), c.op, names[i], " in the place of ", in_names[i],
                       " must have its strides");

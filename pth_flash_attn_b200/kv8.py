@@ -56,6 +56,12 @@ class _Check(_Check16):
     def name(dtype: torch.dtype) -> str:
         return _MORE_NAMES.get(dtype) or _Check16.name(dtype)
 
+    def written(self, **tensors) -> None:
+        for name, t in tensors.items():
+            for d in range(t.dim()):
+                if t.size(d) > 1 and t.stride(d) == 0 and t.numel() != 0:
+                    self.fail(name, " is written and must not have stride 0, as in dimension ", d)
+
     def caches8(self, k_cache, v_cache, k_scale, v_scale) -> None:
         self.rank(k_cache, 4, "k_cache")
         self.rank(v_cache, 4, "v_cache")
@@ -123,6 +129,7 @@ def _kv8_write_fake(key, value, k_cache, v_cache, k_scale, v_scale, block_table,
     c.rows(key, value, k_cache)
     c.table(block_table, seq_lens, "seq_lens")
     c.starts(query_start_loc, seq_lens.size(0), max_query_len, key.size(0), "query_start_loc", "max_query_len")
+    c.written(k_cache=k_cache, v_cache=v_cache, k_scale=k_scale, v_scale=v_scale)
     c.devices(key, "key", value=value, k_cache=k_cache, v_cache=v_cache, k_scale=k_scale, v_scale=v_scale, block_table=block_table,
               seq_lens=seq_lens, query_start_loc=query_start_loc)
 
@@ -133,6 +140,7 @@ def _kv8_read_fake(key, value, k_cache, v_cache, k_scale, v_scale, block_table, 
     c.rows(key, value, k_cache)
     c.table(block_table, first, "first")
     c.starts(row_start_loc, first.size(0), max_rows, key.size(0), "row_start_loc", "max_rows")
+    c.written(key=key, value=value)
     c.devices(key, "key", value=value, k_cache=k_cache, v_cache=v_cache, k_scale=k_scale, v_scale=v_scale, block_table=block_table,
               first=first, row_start_loc=row_start_loc)
 
@@ -151,6 +159,7 @@ def _check_attention(c, out, lse, q, k_cache, v_cache, k_scale, v_scale, block_t
     c.size(out, 1, Hq, "out", "Hq")
     c.size(out, 2, D, "out", "D")
     c.inner(out, "out")
+    c.written(out=out)
     if Hq < 1 or Hq % Hkv != 0:
         c.fail("Hq = ", Hq, " must be a positive multiple of Hkv = ", Hkv)
     if Hq // Hkv > 64:
@@ -207,6 +216,7 @@ def _rotary_fake(q_out, k_out, q, k, positions, frequencies, scale=1.0, interlea
         c.size(y, 1, x.size(1), f"{name}_out", f"{name}.size(1)")
         c.size(y, 2, D, f"{name}_out", "D")
         c.inner(y, f"{name}_out")
+        c.written(**{f"{name}_out": y})
     c.vector(positions, torch.int64, "positions")
     c.size(positions, 0, T, "positions", "T")
     c.rank(frequencies, 1, "frequencies")
@@ -320,7 +330,8 @@ def kv8_decode_attention(out, lse, q, k_cache, v_cache, k_scale, v_scale, block_
     """Attention of one new token of each request over its cache.
 
     ``q``, ``out`` ``[R, Hq, D]`` bf16 or fp16; ``lse`` fp32 ``[R, Hq]`` (natural logarithm) may be empty.  ``window > 0`` limits a
-    token to the newest ``window`` keys.  ``workspace`` (uint8, at least :func:`workspace_bytes`) is zeroed once by its owner, and
+    token to the newest ``window`` keys.  Scales are positive finite numbers, and may be broadcast; ``out`` must not overlap the
+    inputs.  ``workspace`` (uint8, at least :func:`workspace_bytes`) is zeroed once by its owner, and
     left ready for the next call; calls that may overlap need one each.
     """
     _op("kv8_decode_attention")(out, lse, q, k_cache, v_cache, k_scale, v_scale, block_table, seq_lens, softmax_scale, workspace, window)
@@ -333,7 +344,8 @@ def kv8_attention(out, lse, q, k_cache, v_cache, k_scale, v_scale, block_table, 
 
     A token at position ``p`` sees the keys ``max(0, p - window + 1) .. p`` (all up to ``p`` with a window of 0; up to the request's end
     without ``causal``).  ``q``, ``out`` ``[T, Hq, D]``; ``max_query_len`` bounds the tokens of a request; ``lse`` and ``workspace`` as in
-    :func:`kv8_decode_attention`.
+    :func:`kv8_decode_attention`.  ``max_query_len`` also chooses the kernel, for all of the call's requests: tokens of prompts and single
+    ones are served best by a call each.
     """
     _op("kv8_attention")(out, lse, q, k_cache, v_cache, k_scale, v_scale, block_table, seq_lens, query_start_loc, max_query_len,
                          softmax_scale, workspace, window, causal)

@@ -103,6 +103,11 @@ BAD = [(op, *bad) for op in _ARGS if op != "rotary" for bad in _CACHE_BAD] + [
     ("rotary", "frequencies", _t(0, F64), r"frequencies.size\(0\) must be in \[1, D / 2 = 32\], got 0"),
     ("rotary", "frequencies", _t(32, BF16), "frequencies must be float64 or float32, got bfloat16"),
     ("rotary", "scale", lambda d: float("inf"), "scale must be finite, got inf"),
+    ("rotary", "k_out", lambda d: torch.zeros((3, 1, 64), dtype=BF16, device=d).expand(3, 2, 64), "k_out is written and must not have stride 0, as in dimension 1"),
+    ("kv8_write", "k_cache", lambda d: torch.zeros((1, 32, 2, 64), dtype=F8, device=d).expand(4, 32, 2, 64), "k_cache is written and must not have stride 0"),
+    ("kv8_write", "v_scale", lambda d: torch.zeros((4, 2, 1), device=d).expand(4, 2, 2), "v_scale is written and must not have stride 0, as in dimension 2"),
+    ("kv8_read", "value", lambda d: torch.zeros((1, 2, 64), device=d).expand(3, 2, 64), "value is written and must not have stride 0, as in dimension 0"),
+    ("kv8_decode_attention", "out", lambda d: torch.zeros((3, 1, 64), dtype=BF16, device=d).expand(3, 8, 64), "out is written and must not have stride 0"),
 ]
 
 
@@ -205,7 +210,7 @@ def _rotary_struct():
 
 _SHAPE_BAD = [
     ("abi_version", 1, "abi_version"), ("struct_bytes", 8, "struct_bytes"), ("head_size", 96, "head_size must be"), ("block_size", 0, "block_size"),
-    ("num_blocks", 0, "num_blocks"), ("num_kv_heads", 0, "num_kv_heads"), ("scale_tokens", 24, "scale_tokens must be a multiple of 16"),
+    ("num_blocks", 0, "num_blocks"), ("num_kv_heads", 0, "num_kv_heads"), ("num_kv_heads", 1 << 17, "num_kv_heads must be <= 65536"), ("scale_tokens", 24, "scale_tokens must be a multiple of 16"),
     ("scale_tokens", 48, "that divides block_size"), ("scale_tokens", 0, "scale_tokens"), ("num_pages", -1, "num_pages"), ("num_reqs", -1, "num_reqs"),
     ("block_table", None, "block_table is NULL")]
 
