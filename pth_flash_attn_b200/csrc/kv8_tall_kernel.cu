@@ -65,7 +65,7 @@ struct Tall8 {
   static constexpr int threads = (mma_warp + rts) * 32;
   // Registers that a thread starts with (launch_one asks), which setmaxnreg moves from the widening warps to the softmax.
   static constexpr int start_regs = HD == 256 ? 168 : HD == 128 ? 128 : 96;
-  static constexpr int widen_regs = HD == 256 ? 104 : 64, softmax_regs = HD == 256 ? 232 : HD == 128 ? 160 : 128;
+  static constexpr int widen_regs = HD == 256 ? 104 : HD == 128 ? 80 : 56, softmax_regs = HD == 256 ? 232 : HD == 128 ? 152 : 136;
   static_assert(softmax_warps * softmax_regs + kWidenWarps * widen_regs <= (softmax_warps + kWidenWarps) * start_regs, "a split that the launch holds");
   static constexpr int s_col = 0, o_col = 2 * rts * kKeys;   // TMEM columns: S(rt, b) at (2 rt + b) 64, O(rt) at o_col + rt HD
   static constexpr int tmem = HD == 64 ? 256 : 512;
@@ -259,19 +259,26 @@ __device__ __forceinline__ float* tall8_slot(const Kv8Params& p, int cta, bool b
   return reinterpret_cast<float*>(p.workspace + kCounterBytes) + (int64_t)(2 * cta + (begins ? 1 : 0)) * (Tall8<HD, kHalf>::rows * (HD + 2));
 }
 
-// P of 64 scores as pairs of fp16 numbers, 2^(score factor + minus_ref), a factor for every 16 of them; returns the sum of the
-// unrounded ones.
-__device__ __forceinline__ float exponentials8(const uint32_t (&r)[64], const float (&factor)[4], float minus_ref, uint32_t (&pk)[32]) {
+// P of 64 scores, 2^(score factor + minus_ref), a factor for every 16 of them, to TMEM as pairs of fp16 numbers; returns the sum of the
+// unrounded ones.  (Kept in registers until the step is settled, P and the scores were more than 64 dims' warps have: what spilled went
+// round in the first level cache, which shared memory leaves small.)
+__device__ __forceinline__ float exponentials8(const uint32_t (&r)[64], const float (&factor)[4], float minus_ref, uint32_t p_tmem) {
   const f32x2 ref2 = pair(minus_ref, minus_ref);
   f32x2 sum[2] = {0ull, 0ull};
 #pragma unroll
-  for (int n = 0; n < 32; ++n) {
-    float x, y;
-    unpair(fma2(pair(__uint_as_float(r[2 * n]), __uint_as_float(r[2 * n + 1])), pair(factor[n / 8], factor[n / 8]), ref2), x, y);
-    x = ex2f(x);
-    y = ex2f(y);
-    sum[n & 1] = add2(sum[n & 1], pair(x, y));
-    pk[n] = pack_f16(x, y);
+  for (int part = 0; part < 2; ++part) {
+    uint32_t pk[16];
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+      const int n = part * 16 + i;
+      float x, y;
+      unpair(fma2(pair(__uint_as_float(r[2 * n]), __uint_as_float(r[2 * n + 1])), pair(factor[n / 8], factor[n / 8]), ref2), x, y);
+      x = ex2f(x);
+      y = ex2f(y);
+      sum[n & 1] = add2(sum[n & 1], pair(x, y));
+      pk[i] = pack_f16(x, y);
+    }
+    tc::tmem_st16(p_tmem + part * 16, pk);
   }
   return sum_pairs(sum);
 }
@@ -688,7 +695,6 @@ __global__ void __launch_bounds__((Tall8<HD, kHalf>::threads), (Tall8<HD, kHalf>
 #pragma unroll
             for (int g = 0; g < 4; ++g) factor[g] = (uint32_t)(seen >> 16 * g) & 0xffffu ? factor[g] : 1.f;   // (a scale that the row does not see)
           }
-          uint32_t pk[32];
           float total;
           // (One copy of the code for a step's first look and its second: the instruction caches are small.)
           bool move = t == 0;
@@ -696,7 +702,7 @@ __global__ void __launch_bounds__((Tall8<HD, kHalf>::threads), (Tall8<HD, kHalf>
           for (bool again = false;; again = true) {
             bool outgrown = true;
             if (!move) {
-              total = exponentials8(r, factor, ref == -INFINITY ? 0.f : -ref, pk);
+              total = exponentials8(r, factor, ref == -INFINITY ? 0.f : -ref, s_tmem);
               if (again) break;
               outgrown = !(total <= kMostSum) || ref == -INFINITY;
               if (!__any_sync(0xffffffffu, outgrown) && !(most > power_of_two(unit_e) && unit_e < 126)) break;
@@ -733,7 +739,6 @@ __global__ void __launch_bounds__((Tall8<HD, kHalf>::threads), (Tall8<HD, kHalf>
             }
           }
           l += total;
-          tc::tmem_st32(s_tmem, pk);
           tc::tmem_st_wait();
           tc::fence_before_sync();
           mbar_arrive(&bars[G::p_ready + b]);
