@@ -75,6 +75,13 @@ struct PieceQueue {
     ++i;
     return true;
   }
+  // The entry that get takes next, if it is there already.
+  __device__ __forceinline__ bool peek(Piece* x) const {
+    const uint32_t k = i % kQueue;
+    if (!__all_sync(0xffffffffu, tc::mbar_test_wait(&full[k], (i / kQueue) & 1))) return false;
+    *x = entry[k];
+    return x->tiles > 0;
+  }
   __device__ __forceinline__ bool get(Piece* x, volatile int* abort_flag) {
     const uint32_t k = i % kQueue;
     if (!tc::mbar_test_wait(&full[k], (i / kQueue) & 1)) {

@@ -56,7 +56,7 @@ struct Tall8 {
   static constexpr int wide = kKeys * HD * 2;        // W of a step: slabs of 64 dims, 64 rows of 128 bytes, swizzled
   static constexpr int q_digit = 128 * HD;           // column block c of 16 dims at c 2,048, row r at r 16
   static constexpr int q_tile = q_digits * q_digit;
-  static constexpr int k_units = HD == 64 ? 6 : HD == 128 ? (kHalf ? 4 : 6) : (kHalf ? 2 : 3);
+  static constexpr int k_units = HD == 64 ? 4 : HD == 128 ? (kHalf ? 4 : 6) : (kHalf ? 2 : 3);
   static constexpr int v_units = HD == 64 ? 4 : HD == 128 ? (kHalf ? 3 : 4) : 2;
   static constexpr int w_units = HD == 64 ? 4 : HD == 128 ? 3 : 2;
   static_assert(v_units + w_units + 1 < kScaleSteps, "scales outlive their readers");
@@ -74,7 +74,8 @@ struct Tall8 {
   static constexpr int v = k_units * raw;
   static constexpr int w = v + v_units * raw;
   static constexpr int q = w + w_units * wide;
-  static constexpr int scales = q + rts * q_tile;    // float [kScaleSteps][2][4]: of the keys' runs of 16, of the values'
+  static constexpr int raw_q = q + rts * q_tile;     // query rows as they are (others: in the place of their digits)
+  static constexpr int scales = raw_q + (HD == 64 ? 128 * HD * 2 : 0);   // float [kScaleSteps][2][4]: of the keys' runs of 16, of the values'
   static constexpr int bars = scales + kScaleSteps * 32;
   static constexpr int k_full = 0, k_empty = k_full + k_units, v_full = k_empty + k_units, v_empty = v_full + v_units, w_full = v_empty + v_units,
                        w_empty = w_full + w_units, q_full = w_empty + w_units, s_ready = q_full + rts, p_ready = s_ready + 2 * rts,
@@ -292,28 +293,48 @@ __device__ __forceinline__ float load_elem16(const uint8_t* row, int d) {
   else return __bfloat162float(reinterpret_cast<const __nv_bfloat16*>(row)[d]);
 }
 
-// The digits of a query row, by its thread: returns u x softmax scale x log2(e), below zero for a row that is not finite.
-template <int HD, bool kHalf>
-__device__ __forceinline__ float stage_row(const Kv8Params& p, const uint8_t* row, uint8_t* image) {
+// Asks for a warp's 32 query rows of a piece, as they are: row n at raw + n 2 HD, its 16-byte pieces swizzled by n.
+template <int HD>
+__device__ __forceinline__ void copy_rows(const Kv8Params& p, const Piece& it, int row0, uint32_t raw) {
+  constexpr int kChunks = HD / 8, kRows = 32 / kChunks;   // pieces of a row, rows at a time
+  const int lane = threadIdx.x & 31, chunk = lane % kChunks, sub = lane / kChunks;
+  if (it.rows <= row0) return;
+  int token, head;
+  row_of(p, it.first_token, it.kvh, it.row0 + min(row0 + lane, it.rows - 1), &token, &head);
+  const long long off = (long long)token * p.q_stride_token + (long long)head * p.q_stride_head;
+#pragma unroll 4
+  for (int i = 0; i < 32 / kRows; ++i) {
+    const int row = i * kRows + sub;
+    copy16(raw + row * (2 * HD) + ((chunk ^ (row & 7)) << 4), p.q + __shfl_sync(0xffffffffu, off, row) + chunk * 16, true);
+  }
+}
+// The digits of a query row, by its thread, to `image`; wait(): all of the row tile have read their rows.  Returns u x softmax scale x log2(e),
+// below zero for a row that is not finite.
+template <int HD, bool kHalf, class Wait>
+__device__ __forceinline__ float stage_row(const Kv8Params& p, const uint8_t* raw, int row, uint8_t* image, Wait wait) {
   using G = Tall8<HD, kHalf>;
-  const uint4* const in = reinterpret_cast<const uint4*>(row);
+  constexpr bool kKept = HD != 64;   // all of the row in registers: its place is the image's
+  auto chunk = [&](int c) { return *reinterpret_cast<const uint4*>(raw + ((c ^ (row & 7)) << 4)); };
+  uint4 kept[kKept ? HD / 8 : 1];
   uint32_t m = 0;   // largest magnitudes, as 16-bit integers
 #pragma unroll
   for (int c = 0; c < HD / 8; ++c) {
-    const uint4 w = __ldg(in + c);
+    const uint4 w = chunk(c);
+    if constexpr (kKept) kept[c] = w;
     m = __vimax3_u16x2(m, w.x & 0x7fff7fffu, w.y & 0x7fff7fffu);
     m = __vimax3_u16x2(m, w.z & 0x7fff7fffu, w.w & 0x7fff7fffu);
   }
+  if constexpr (kKept) wait();
   const uint32_t top16 = max(m & 0xffffu, m >> 16);
   const bool finite = top16 < (kHalf ? 0x7c00u : 0x7f80u);
   const float top = kHalf ? __half2float(__ushort_as_half((unsigned short)top16)) : __uint_as_float(top16 << 16);
   const int e = min(119, max(-119, e4m3_exponent(top)));
   const float up = power_of_two(-e);
-  // (Rolled at 64 dims, from the first level cache: what runs once a piece costs by its instructions, which come from beyond theirs.  Twelve
-  // prompts of 37 to 2,500 tokens, rolled and not, us: 243 / 250 at 64 dims, 446 / 405 at 128.)
+  // (Rolled at 64 dims: what runs once a piece costs by its instructions, which come from beyond the first caches.  Twelve
+  // prompts of 37 to 2,500 tokens, rolled and not, us: 174 / 182 at 64 dims, 402 / 357 at 128.)
 #pragma unroll(HD == 64 ? 1 : HD / 16)
   for (int c = 0; c < HD / 16; ++c) {
-    const uint4 w0 = __ldg(in + 2 * c), w1 = __ldg(in + 2 * c + 1);
+    const uint4 w0 = kKept ? kept[kKept ? 2 * c : 0] : chunk(2 * c), w1 = kKept ? kept[kKept ? 2 * c + 1 : 0] : chunk(2 * c + 1);
     const uint32_t pairs[8] = {w0.x, w0.y, w0.z, w0.w, w1.x, w1.y, w1.z, w1.w};
     uint32_t d[G::q_digits][4];
 #pragma unroll
@@ -344,7 +365,7 @@ __device__ __forceinline__ float stage_row(const Kv8Params& p, const uint8_t* ro
 // code does not run through; only softmax threads call it, who have more registers than the launch gave.)
 template <int HD, bool kHalf>
 __device__ __noinline__ void sum_again(const Kv8Params& p, const Piece& it, const uint8_t* q_row, int lo, int hi, float ref, int d0, uint32_t* sums) {
-  for (int d = 0; d < 32; ++d) sums[d] = 0u;
+  for (int d = 0; d < 16; ++d) sums[d] = 0u;
 #pragma unroll 1
   for (int pos = lo; pos < hi; ++pos) {
     int slot;
@@ -359,7 +380,7 @@ __device__ __noinline__ void sum_again(const Kv8Params& p, const Piece& it, cons
       s = fmaf(load_elem16<kHalf>(q_row, d + 1), k.y, s);
     }
     const float w = ex2f(s * p.k_scale[scale] * p.scale_log2 - ref) * p.v_scale[scale];
-    for (int d = 0; d < 32; d += 2) {
+    for (int d = 0; d < 16; d += 2) {
       const float2 v = float2_of_e4m3x2(*reinterpret_cast<const uint16_t*>(p.v + at + d0 + d));
       sums[d] = __float_as_uint(fmaf(w, v.x, __uint_as_float(sums[d])));
       sums[d + 1] = __float_as_uint(fmaf(w, v.y, __uint_as_float(sums[d + 1])));
@@ -641,6 +662,9 @@ __global__ void __launch_bounds__((Tall8<HD, kHalf>::threads), (Tall8<HD, kHalf>
     uint32_t count = 0;    // live steps so far
     uint32_t step = 0;     // steps so far (of all pieces)
     auto rt_sync = [&] { named_barrier(1 + rt, 128); };
+    uint8_t* const raw_q = smem + (HD == 64 ? G::raw_q : G::q + rt * G::q_tile);
+    const uint32_t raw_rows = tc::smem_u32(raw_q) + (row & 96) * (2 * HD);   // of the warp
+    bool copied = false;   // the piece's query rows are on their way
     zero_requests<HD, RP, 128 * G::rts>(p);
     {
       Piece it;
@@ -648,6 +672,7 @@ __global__ void __launch_bounds__((Tall8<HD, kHalf>::threads), (Tall8<HD, kHalf>
         const int n_steps = steps8(it);
         if (it.rows <= rt * 128) {
           step += n_steps;
+          copied = false;
           continue;
         }
         const int kvh = it.kvh;
@@ -657,10 +682,15 @@ __global__ void __launch_bounds__((Tall8<HD, kHalf>::threads), (Tall8<HD, kHalf>
         // (QK has read the last piece's digits: its last S has been waited for)
         float q_factor = 0.f;
         if (!padding) {
-          q_factor = stage_row<HD, kHalf>(p, p.q + (int64_t)token * p.q_stride_token + (int64_t)head * p.q_stride_head,
-                                          smem + G::q + rt * G::q_tile + (row & 127) * 16);
+          if (!copied) copy_rows<HD>(p, it, row & ~31, raw_rows);
+          copies_wait_all();
+          __syncwarp();
+          q_factor = stage_row<HD, kHalf>(p, raw_q + (row & 127) * (2 * HD), row, smem + G::q + rt * G::q_tile + (row & 127) * 16, rt_sync);
           tc::fence_async_smem();
+        } else if constexpr (HD != 64) {
+          rt_sync();
         }
+        copied = false;
         mbar_arrive(&bars[G::q_full + rt]);
         const int own = it.pos0 + token - it.first_token;
         const int row_lo = kv8_low(p, own), row_hi = p.causal ? min(own + 1, it.hi) : it.hi;
@@ -743,6 +773,12 @@ __global__ void __launch_bounds__((Tall8<HD, kHalf>::threads), (Tall8<HD, kHalf>
           tc::fence_before_sync();
           mbar_arrive(&bars[G::p_ready + b]);
         }
+        // (QK has read the digits: the next piece's rows can come in the meantime)
+        Piece next;
+        if (queue.peek(&next)) {
+          copy_rows<HD>(p, next, row & ~31, raw_rows);
+          copied = true;
+        }
         // ---- the piece's rows ----
         ok &= kv16_wait(&bars[G::pv_done + 2 * rt + ((count - 1) & 1)], ((count - 1) >> 1) & 1, abort_flag);
         tc::fence_after_sync();
@@ -768,33 +804,32 @@ __global__ void __launch_bounds__((Tall8<HD, kHalf>::threads), (Tall8<HD, kHalf>
           const float unit = power_of_two(unit_e), factor = whole ? (l == 0.f ? 0.f : unit / l) : unit;
           float* const slot = tall8_slot<HD, kHalf>(p, (int)blockIdx.x, it.begins) + row;
 #pragma unroll 1
-          for (int c = 0; c < HD / 32; ++c) {
-            uint32_t r[32];
-            tc::tmem_ld32(o_tmem + c * 32, r);
-            tc::tmem_ld_wait<32>(r);
+          for (int c = 0; c < HD / 16; ++c) {
+            uint32_t r[16];
+            tc::tmem_ld16(o_tmem + c * 16, r);
+            tc::tmem_ld_wait<16>(r);
             f32x2 all[2] = {0ull, 0ull};
 #pragma unroll
-            for (int n = 0; n < 32; n += 2) all[n / 2 & 1] = add2(all[n / 2 & 1], pair(__uint_as_float(r[n]), __uint_as_float(r[n + 1])));
+            for (int n = 0; n < 16; n += 2) all[n / 2 & 1] = add2(all[n / 2 & 1], pair(__uint_as_float(r[n]), __uint_as_float(r[n + 1])));
             const float any = sum_pairs(all);
             if (__builtin_expect(any != any && l == l, 0)) {   // NaN, which may be of a key that the row does not see
-              uint32_t sums[32];
+              uint32_t sums[16];
               sum_again<HD, kHalf>(p, it, p.q + (int64_t)token * p.q_stride_token + (int64_t)head * p.q_stride_head, max(row_lo, it.key0),
-                                   min(min(row_hi, it.hi), it.key0 + it.tiles * kTile), ref == -INFINITY ? 0.f : ref, c * 32, sums);
+                                   min(min(row_hi, it.hi), it.key0 + it.tiles * kTile), ref == -INFINITY ? 0.f : ref, c * 16, sums);
 #pragma unroll
-              for (int n = 0; n < 32; ++n) r[n] = __float_as_uint(__uint_as_float(sums[n]) * power_of_two(-unit_e));
+              for (int n = 0; n < 16; ++n) r[n] = __float_as_uint(__uint_as_float(sums[n]) * power_of_two(-unit_e));
             }
             __syncwarp();
-            float o[32];
+            float o[16];
 #pragma unroll
-            for (int n = 0; n < 32; ++n) o[n] = __uint_as_float(r[n]) * factor;
+            for (int n = 0; n < 16; ++n) o[n] = __uint_as_float(r[n]) * factor;
             if (whole) {
               if (live) {
-                write16(o, c * 32);
-                write16(o + 16, c * 32 + 16);
+                write16(o, c * 16);
               }
             } else {
 #pragma unroll
-              for (int n = 0; n < 32; ++n) slot[(c * 32 + n) * RP] = o[n];
+              for (int n = 0; n < 16; ++n) slot[(c * 16 + n) * RP] = o[n];
             }
           }
           if (whole) {
@@ -862,6 +897,7 @@ __global__ void __launch_bounds__((Tall8<HD, kHalf>::threads), (Tall8<HD, kHalf>
           rt_sync();   // (the arrival has been read)
         }
       }
+      copies_wait_all();
     }
   }
   tc::fence_before_sync();
