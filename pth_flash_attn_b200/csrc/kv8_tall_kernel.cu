@@ -18,8 +18,15 @@
 // a row's first 64 keys.  Later ones need no maximum: the sum of 64 P says whether one of them has outgrown ref too far
 // (kMostSum); then ref moves to their maximum, O and l are rescaled and the 64 are computed again.
 //
-// Warps: softmax (four per row tile), which also make the digits of a piece's queries; four that widen V; one that works out the
-// pieces and asks for their cells, by TMA boxes of 16 slots (a page holds a whole number of them), and for the scales; an MMA warp per row tile.
+// Warps: softmax (four per row tile), which also ask for a piece's queries, while the last one's rows go out, and make their digits; four
+// that widen V; one that works out the pieces and asks for their cells, by TMA boxes of 16 slots (a page holds a whole number of them), and for
+// the scales; an MMA warp per row tile.
+//
+// What bounds it.  A step's softmax, 1,300 to 1,500 clocks of 64 exponentials and their conversions a row, beside 300 to 500 of waiting for S; power
+// (the 1,000 W limit) in long calls; a piece's own 8,000 to 10,000 clocks (queries, first S, rows, merge) in short ones.  Measured (bf16 unless
+// said, calls behind one another): four chunks of 2,048 tokens over 8,192 keys before them, 32 heads of 8, 128 dims: 1,260 to 1,340 us, 0.56 to
+// 0.59 of the bf16 rate of a library product.  Twelve prompts of 37 to 2,500 tokens: 16 heads of 16, 64 dims, fp16, 174 us; 32 heads of 8, 128 dims,
+// 329 us.  256 dims, the same chunks: 3,400 us, one row tile per SM.
 //
 // Schedule: the rows of a request and KV head in row tiles, a first one together with a last one, so that under a causal mask
 // these units are about equally long; all units form one sequence in KV tiles of 128 keys, which is cut into equal runs, one per
@@ -56,6 +63,7 @@ struct Tall8 {
   static constexpr int wide = kKeys * HD * 2;        // W of a step: slabs of 64 dims, 64 rows of 128 bytes, swizzled
   static constexpr int q_digit = 128 * HD;           // column block c of 16 dims at c 2,048, row r at r 16
   static constexpr int q_tile = q_digits * q_digit;
+  // (K of 64 dims with two, three, four and six units: the twelve prompts 178, 178, 174, 178 us)
   static constexpr int k_units = HD == 64 ? 4 : HD == 128 ? (kHalf ? 4 : 6) : (kHalf ? 2 : 3);
   static constexpr int v_units = HD == 64 ? 4 : HD == 128 ? (kHalf ? 3 : 4) : 2;
   static constexpr int w_units = HD == 64 ? 4 : HD == 128 ? 3 : 2;
@@ -63,7 +71,9 @@ struct Tall8 {
   static constexpr int softmax_warps = 4 * rts;
   static constexpr int widen_warp = softmax_warps, load_warp = widen_warp + kWidenWarps, mma_warp = load_warp + 1;
   static constexpr int threads = (mma_warp + rts) * 32;
-  // Registers that a thread starts with (launch_one asks), which setmaxnreg moves from the widening warps to the softmax.
+  // Registers that a thread starts with (launch_one asks), which setmaxnreg moves from the widening warps to the softmax: as many as leave
+  // both without spills.  (Widening and softmax with 64 and 128, 56 and 136, 32 and 160 at 64 dims: 177, 174, 178 us for the twelve prompts, 166, 155,
+  // 155 for 512 of 64 tokens; with 64 and 160, 96 and 144, 80 and 152 at 128 dims: 369, 370, 358.)
   static constexpr int start_regs = HD == 256 ? 168 : HD == 128 ? 128 : 96;
   static constexpr int widen_regs = HD == 256 ? 104 : HD == 128 ? 80 : 56, softmax_regs = HD == 256 ? 232 : HD == 128 ? 152 : 136;
   static_assert(softmax_warps * softmax_regs + kWidenWarps * widen_regs <= (softmax_warps + kWidenWarps) * start_regs, "a split that the launch holds");
