@@ -65,9 +65,10 @@ struct Tall8 {
   static constexpr int q_tile = q_digits * q_digit;
   // (K of 64 dims with two, three, four and six units: the twelve prompts 178, 178, 174, 178 us)
   static constexpr int k_units = HD == 64 ? 4 : HD == 128 ? (kHalf ? 4 : 6) : (kHalf ? 2 : 3);
+  static constexpr int at_once = HD == 256 ? 1 : 2;   // steps that the loading warp asks for together (256 dims have no room for more)
   static constexpr int v_units = HD == 64 ? 4 : HD == 128 ? (kHalf ? 3 : 4) : 2;
   static constexpr int w_units = HD == 64 ? 4 : HD == 128 ? 3 : 2;
-  static_assert(v_units + w_units + 1 < kScaleSteps, "scales outlive their readers");
+  static_assert(v_units + w_units + at_once < kScaleSteps, "scales outlive their readers");
   static constexpr int softmax_warps = 4 * rts;
   static constexpr int widen_warp = softmax_warps, load_warp = widen_warp + kWidenWarps, mma_warp = load_warp + 1;
   static constexpr int threads = (mma_warp + rts) * 32;
@@ -452,13 +453,14 @@ __global__ void __launch_bounds__((Tall8<HD, kHalf>::threads), (Tall8<HD, kHalf>
   const uint32_t tmem_base = *tslot;
   PieceQueue queue(reinterpret_cast<Piece*>(smem + G::pieces), &bars[G::queue], stop);
   bool ok = true;
-  uint32_t asked = 0;   // steps whose cells this CTA has asked for (loading warp)
+  uint32_t asked_k = 0, asked_v = 0;   // steps whose keys, and values, this CTA has asked for (loading warp)
 
   if (warp == G::load_warp) {
     // =========================== schedule and copies =============================
-    // The warp hands a piece to the others, then asks for its cells: lanes 0 to 3 for a run of 16 keys of a step each, lanes 4 to 7
-    // for their values.  (Behind a wait that gave up nothing more is asked for: a unit that is not free may be waiting for its boxes.)
-    const int run = lane & 3;
+    // The warp hands a piece to the others, then asks for its cells, kAtOnce steps at a time: a lane for a run of 16 keys, or of their values,
+    // and its scale.  (Behind a wait that gave up nothing more is asked for: a unit that is not free may be waiting for its boxes.)
+    constexpr int kRuns = G::at_once * (kKeys / 16);
+    const int run = lane % kRuns, kind = lane / kRuns, mine = run / 4;   // kind 0: keys, 1: values; the lane's step of those
     const uint32_t k_ring = tc::smem_u32(smem), v_ring = k_ring + G::v, scales = k_ring + G::scales;
     TallWalk8<RP> walk = plan;
     Piece it;
@@ -477,47 +479,54 @@ __global__ void __launch_bounds__((Tall8<HD, kHalf>::threads), (Tall8<HD, kHalf>
         return (uint32_t)blk < (uint32_t)p.num_blocks ? blk : -1;
       };
       int slot = 0, next_slot = 0, next_blk = look_up(0, &next_slot);
+      auto free_units = [&](int first, int units, uint32_t asked_for, int here) {
+        for (int i = 0; i < here; ++i) {
+          const uint32_t u = asked_for + i;
+          if (u >= (uint32_t)units) ok &= kv16_wait(&bars[first + u % units], ((u / units) - 1) & 1, abort_flag);
+        }
+        ok = __all_sync(0xffffffffu, ok);
+        return ok;
+      };
 #pragma unroll 1
-      for (int j = 0; j < n && ok; ++j, ++asked) {
-        const int blk = next_blk;
+      for (int j = 0; j < n; j += G::at_once) {
+        const int blk = next_blk, here = min(G::at_once, n - j);
         slot = next_slot;
-        if (j + 1 < n) next_blk = look_up(j + 1, &next_slot);
+        if (j + G::at_once < n) next_blk = look_up(j + G::at_once, &next_slot);
         auto ask = [&](const CUtensorMap& map, uint32_t to, uint64_t* full) {   // the lane's run
+          to += (run & 3) * 16 * G::dims;
           if (blk >= 0) {
             mbar_arrive_expect_tx(full, 16 * HD);
 #pragma unroll
-            for (int part = 0; part < G::parts; ++part)
-              tma_load_4d(to + part * (kKeys * 128) + run * 16 * G::dims, &map, part * 128, it.kvh, slot, blk, full);
+            for (int part = 0; part < G::parts; ++part) tma_load_4d(to + part * (kKeys * 128), &map, part * 128, it.kvh, slot, blk, full);
           } else {
             if (blk == -1) {   // keys and values of zero
 #pragma unroll 1
               for (int i = 0; i < HD; ++i)   // 16 rows of HD bytes, 16 at a time
-                asm volatile("st.shared.v4.u32 [%0], {%1, %1, %1, %1};" ::"r"(to + i * 16 / (16 * G::dims) * (kKeys * 128) + run * 16 * G::dims + i * 16 % (16 * G::dims)), "r"(0) : "memory");
+                asm volatile("st.shared.v4.u32 [%0], {%1, %1, %1, %1};" ::"r"(to + i * 16 / (16 * G::dims) * (kKeys * 128) + i * 16 % (16 * G::dims)), "r"(0) : "memory");
               tc::fence_async_smem();
             }
             mbar_arrive(full);
           }
         };
-        const uint32_t ku = asked % G::k_units, vu = asked % G::v_units, su = asked % kScaleSteps;
-        if (asked >= G::k_units) ok = kv16_wait(&bars[G::k_empty + ku], ((asked / G::k_units) - 1) & 1, abort_flag);
-        if (!__all_sync(0xffffffffu, ok)) {
-          ok = false;
-          break;
-        }
+        const bool live = kind < 2 && mine < here;
+        const uint32_t step = asked_v + mine, ku = step % G::k_units, vu = step % G::v_units, su = step % kScaleSteps;
+        if (!free_units(G::k_empty, G::k_units, asked_k, here)) break;
         // (the unit of V that was free for the last step says that the scales of kScaleSteps steps ago have been read)
-        if (lane < 8) {
-          const float* const base = lane < 4 ? p.k_scale : p.v_scale;
-          copy4(scales + su * 32 + lane * 4, blk >= 0 ? base + scale_at(p, it.kvh, blk, slot) : base, blk >= 0);
+        if (live) {
+          const float* const base = kind == 0 ? p.k_scale : p.v_scale;
+          copy4(scales + su * 32 + kind * 16 + (run & 3) * 4, blk >= 0 ? base + scale_at(p, it.kvh, blk, slot) : base, blk >= 0);
           copies_arrive(&bars[G::k_full + ku]);
           copies_arrive(&bars[G::scales_full + su]);
+          if (kind == 0) ask(k_map, k_ring + ku * G::raw, &bars[G::k_full + ku]);
         }
-        if (lane < 4) ask(k_map, k_ring + ku * G::raw, &bars[G::k_full + ku]);
+        asked_k += here;
         __syncwarp();
-        if (asked >= G::v_units) ok = kv16_wait(&bars[G::v_empty + vu], ((asked / G::v_units) - 1) & 1, abort_flag);
-        ok = __all_sync(0xffffffffu, ok);
-        if (ok && lane >= 4 && lane < 8) ask(v_map, v_ring + vu * G::raw, &bars[G::v_full + vu]);
+        if (!free_units(G::v_empty, G::v_units, asked_v, here)) break;
+        if (live && kind == 1) ask(v_map, v_ring + vu * G::raw, &bars[G::v_full + vu]);
+        asked_v += here;
         __syncwarp();
       }
+      if (!ok) break;
     }
     if (going) {
       it.tiles = 0;
@@ -919,9 +928,8 @@ __global__ void __launch_bounds__((Tall8<HD, kHalf>::threads), (Tall8<HD, kHalf>
       kv16_drain(drained, 0);
     }
     if (warp == G::load_warp) {
-      // (of the last step K alone may have been asked for)
-      for (uint32_t u = asked + 1 > G::k_units ? asked + 1 - G::k_units : 0; u < asked; ++u) kv16_drain(&bars[G::k_full + u % G::k_units], (u / G::k_units) & 1);
-      for (uint32_t u = asked > G::v_units ? asked - G::v_units : 0; u < asked; ++u) kv16_drain(&bars[G::v_full + u % G::v_units], (u / G::v_units) & 1);
+      for (uint32_t u = asked_k > G::k_units ? asked_k - G::k_units : 0; u < asked_k; ++u) kv16_drain(&bars[G::k_full + u % G::k_units], (u / G::k_units) & 1);
+      for (uint32_t u = asked_v > G::v_units ? asked_v - G::v_units : 0; u < asked_v; ++u) kv16_drain(&bars[G::v_full + u % G::v_units], (u / G::v_units) & 1);
     }
     if (tid == 0) atomicOr(&g_kv8_tall_status, 64u);
     __syncthreads();
