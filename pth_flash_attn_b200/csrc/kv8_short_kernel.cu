@@ -79,12 +79,17 @@ struct Geo8 {
   static constexpr int pcols = (kDigitsY * RP + 15) / 16 * 16;    // N of PV
   static constexpr int qimage = cols * HD;           // column block c of 16 dims at c (cols 16), column n at n 16
   static constexpr int pimage = pcols * kTile;       // block of 16 columns at 2,048 each, key t at t 16
-  static constexpr int fixed = 2 * qimage + pimage + 9 * RP * 4 + 2 * RP * 4 + kScaleTiles * 64 + 1024;
+  // Images of Y: two where a tile's PV takes long, so that the next softmax need not wait for it (8 rows, 256 dims, 61 requests of 4,096 to
+  // 12,288 keys: 90.3 us instead of 93.5; 128 dims, one token of 64 requests, the same; 16 rows, four of 32 requests, 125.3 us, with one 124.5).
+  static constexpr int p_images = HD == 256 && RP == 8 ? 2 : 1;
+  static constexpr int fixed = 2 * qimage + p_images * pimage + 9 * RP * 4 + 2 * RP * 4 + kScaleTiles * 64 + 1024;
   static constexpr int units2 = (115712 - fixed - 1024) / unit;
   static constexpr int ctas = units2 >= 3 && RP <= 16 ? 2 : 1;
   static constexpr int most = 2 * (kScaleTiles - 3);   // (see kScaleTiles)
   static constexpr int fit = ctas == 2 ? units2 : (232448 - fixed - 1024) / unit;
-  static constexpr int units = fit < most ? fit : most;
+  // (Four with 16 rows, whose registers spill: what spills goes round in the first level cache, which shared memory leaves small.  Four and as many
+  // as fit, us: four tokens of 32 requests 124.5 / 126.3, 16 heads each of 64 requests 60.8 / 63.0, at 256 dims 103.3 / 109.2, at 64 dims 106.7 / 109.)
+  static constexpr int units = RP == 16 && fit > 4 ? 4 : fit < most ? fit : most;
   static_assert(units >= 3, "K and V of a tile, and the next K");
   // Registers that the other warps hand to the softmax from what a thread starts with (launch_one asks).
   static constexpr int start_regs = HD == 64 ? (RP == 8 ? 80 : ctas == 2 ? 64 : 128) : RP == 8 ? 128 : ctas == 2 ? 80 : 168;
@@ -99,21 +104,21 @@ struct Geo8 {
   // shared memory, behind the first 1,024-byte boundary
   static constexpr int q = units * unit;
   static constexpr int p = q + 2 * qimage;
-  static constexpr int wmax = p + pimage;            // float [groups][4 warps][rows]
+  static constexpr int wmax = p + p_images * pimage;    // float [groups][4 warps][rows]
   static constexpr int wsum = wmax + 4 * RP * 4;     // float [groups][4 warps][rows]
   static constexpr int at = wsum + 4 * RP * 4;       // int [RP]: positions of the piece's rows
   static constexpr int qfactor = at + RP * 4;    // float [2][RP]: a row's u x softmax scale x log2(e)
   static constexpr int scales = qfactor + 2 * RP * 4;   // [kScaleTiles][2][8]: of the keys, of the values
   static constexpr int pieces = scales + kScaleTiles * 64;   // PieceQueue's entries
   static constexpr int bars = pieces + kQueue * 64;
-  static constexpr int n_bars = 2 * units + 2 + 2 + 2 + 1 + 1 + 2 * kQueue + 1;
+  static constexpr int n_bars = 2 * units + 2 + 2 + 2 + 2 * 2 + 2 * kQueue + 1;
   static constexpr int misc = bars + n_bars * 8;     // ints: abort flag, TMEM address, arrival, stop; scratch of find_run; nan_item
   static constexpr int total = misc + 176 + 1024;
   static_assert(kQueue * 64 + n_bars * 8 + 160 <= 1024, "fixed part");
 };
 
 struct Bars8 {  // offsets behind [units] full, [units] empty
-  static constexpr int q_full = 0, q_empty = 2, s_ready = 4, p_ready = 6, pv_done = 7, queue = 8, drained = queue + 2 * kQueue;
+  static constexpr int q_full = 0, q_empty = 2, s_ready = 4, p_ready = 6, pv_done = 8, queue = 10, drained = queue + 2 * kQueue;
 };
 
 // Barrier of a softmax warpgroup that tells whether any of its threads has seen `x`.
@@ -370,8 +375,10 @@ __global__ void __launch_bounds__((Geo8<HD, RP, kHalf>::threads), (Geo8<HD, RP, 
         tc::mbar_init(&bars[Bars8::q_empty + i], 1 + G::groups);   // the last QK has read the digits, the softmax the factors
         tc::mbar_init(&bars[Bars8::s_ready + i], 2);   // the MMAs are complete; this warp has seen the tile's scales land
       }
-      tc::mbar_init(&bars[Bars8::p_ready], kSoftmaxThreads * G::groups);
-      tc::mbar_init(&bars[Bars8::pv_done], 1);
+      for (int i = 0; i < 2; ++i) {
+        tc::mbar_init(&bars[Bars8::p_ready + i], kSoftmaxThreads * G::groups);
+        tc::mbar_init(&bars[Bars8::pv_done + i], 1);
+      }
       tc::mbar_init(&bars[Bars8::drained], 1);
       PieceQueue(nullptr, &bars[Bars8::queue], stop).init(4 * G::groups + G::load_warps + 1);
       *abort_flag = 0;
@@ -564,7 +571,7 @@ __global__ void __launch_bounds__((Geo8<HD, RP, kHalf>::threads), (Geo8<HD, RP, 
     };
     uint32_t pv_tile = 0;
     auto pv = [&](bool first_of_item, bool divided, uint32_t its_item) {
-      ok &= kv16_wait(&bars[Bars8::p_ready], pv_tile & 1, abort_flag);
+      ok &= kv16_wait(&bars[Bars8::p_ready + pv_tile % G::p_images], (pv_tile / G::p_images) & 1, abort_flag);
 #pragma unroll
       for (int part = 0; part < G::parts; ++part) {
         const uint32_t s = arrived();
@@ -579,11 +586,11 @@ __global__ void __launch_bounds__((Geo8<HD, RP, kHalf>::threads), (Geo8<HD, RP, 
           for (int kk = 0; kk < kTile / 32; ++kk) {
             // (64 dims: the instruction's other 64 rows are the same bytes again, which nothing reads)
             const uint64_t a = unit_desc<G::dims>(ring + s * G::unit + kk * 32 * G::dims, 0);
-            const uint64_t b = tc::smem_desc(p_s + kk * 512, 128, kTile * 16);
+            const uint64_t b = tc::smem_desc(p_s + pv_tile % G::p_images * G::pimage + kk * 512, 128, kTile * 16);
             mma_e4m3(tmem_base + G::o_col + part * G::pcols, a, b, pv_desc, !first_of_item || kk > 0);
           }
           if (ok) tc::mma_commit(&empty[s]);
-          if (part == G::parts - 1) tc::mma_commit(&bars[Bars8::pv_done]);
+          if (part == G::parts - 1) tc::mma_commit(&bars[Bars8::pv_done + pv_tile % G::p_images]);
         }
         __syncwarp();
       }
@@ -701,7 +708,7 @@ __global__ void __launch_bounds__((Geo8<HD, RP, kHalf>::threads), (Geo8<HD, RP, 
               x[n] = fmaf(s[n], factor[n], -to);
             }
             if (t > 0 && moved) {   // (the same in all of the group's threads)
-              ok &= kv16_wait(&bars[Bars8::pv_done], (tile - 1) & 1, abort_flag);
+              ok &= kv16_wait(&bars[Bars8::pv_done + (tile - 1) % G::p_images], ((tile - 1) / G::p_images) & 1, abort_flag);
               tc::fence_after_sync();
 #pragma unroll
               for (int d = 0; d < kDigitsY * G::parts; ++d) {
@@ -729,18 +736,18 @@ __global__ void __launch_bounds__((Geo8<HD, RP, kHalf>::threads), (Geo8<HD, RP, 
 #pragma unroll
             for (int g = 0; g < kDigitsY; ++g) y[g][n / 4] = n % 4 == 0 ? d[g] : y[g][n / 4] | d[g] << 16;
           }
-          if (tile > 0) ok &= kv16_wait(&bars[Bars8::pv_done], (tile - 1) & 1, abort_flag);  // (P of the last tile has been read)
+          if (tile >= G::p_images) ok &= kv16_wait(&bars[Bars8::pv_done + tile % G::p_images], (tile / G::p_images - 1) & 1, abort_flag);   // (the image has been read)
           // column g RP + n: digit g of row n; 16 columns are 16 bytes of the key's
 #pragma unroll
           for (int g = 0; g < kDigitsY; ++g) {
             const int c = g * RP + row_base;
-            uint8_t* const to = p_img + (c >> 4) * (kTile * 16) + (c & 15);
+            uint8_t* const to = p_img + tile % G::p_images * G::pimage + (c >> 4) * (kTile * 16) + (c & 15);
             if constexpr (RW == 8) *reinterpret_cast<uint2*>(to) = make_uint2(y[g][0], y[g][1]);
             else *reinterpret_cast<uint4*>(to) = make_uint4(y[g][0], y[g][1], y[g][2], y[g][3]);
           }
           tc::fence_async_smem();
           tc::fence_before_sync();
-          mbar_arrive(&bars[Bars8::p_ready]);
+          mbar_arrive(&bars[Bars8::p_ready + tile % G::p_images]);
         }
         // ---- the piece's rows ----
 #pragma unroll
@@ -759,7 +766,7 @@ __global__ void __launch_bounds__((Geo8<HD, RP, kHalf>::threads), (Geo8<HD, RP, 
         ++item;
 #pragma unroll
         for (int n = 0; n < RW; ++n) l[n] = (wsum[n] + wsum[RW + n]) + (wsum[2 * RW + n] + wsum[3 * RW + n]);
-        ok &= kv16_wait(&bars[Bars8::pv_done], (tile - 1) & 1, abort_flag);
+        ok &= kv16_wait(&bars[Bars8::pv_done + (tile - 1) % G::p_images], ((tile - 1) / G::p_images) & 1, abort_flag);
         tc::fence_after_sync();
         const bool whole = it.begins && it.ends;
         float* const slot = partial_slot<HD, RP>(p, (int)blockIdx.x, it.begins);
