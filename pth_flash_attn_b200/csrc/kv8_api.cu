@@ -146,9 +146,10 @@ int32_t build(const PthB200Kv8Args* a, bool decode, Kv8Params* p) {
 // Rows (query tokens x G) from which a launch of more than one token goes to the kernel with the rows on the MMA's M
 // dimension.  Keys on M against rows on M, us, four heads of a KV head:
 //   rows   D 128: 8 x 500  8 x 4,000  64 x 500  64 x 4,000 keys   D 64: 64 x 500  64 x 4,000   D 256: 64 x 500  64 x 4,000
-//     16         19 / 22      30 / 50      42 / 63     107 / 255           42 / 39     105 / 136        64 / 99     188 / 343
-//     32         35 / 22      43 / 50      81 / 62     184 / 256           78 / 39     184 / 137       110 / 99     268 / 345
-//     48         31 / 22      56 / 50     142 / 65     327 / 256
+//     16         20 / 23      32 / 48      43 / 64     109 / 237           42 / 36     106 / 126        67 / 101    188 / 353
+//     24         33 / 23      42 / 48      80 / 64     181 / 237                                       114 / 102    271 / 354
+//     32         37 / 23      45 / 48      85 / 62     190 / 237           78 / 36     184 / 126       122 / 103    289 / 358
+//     48         31 / 22      56 / 48     142 / 65     327 / 237
 // Single tokens of wide groups stay with the keys on M, which divides few requests better.
 int64_t tall_rows(int head_size) { return head_size == 64 ? 17 : 33; }
 

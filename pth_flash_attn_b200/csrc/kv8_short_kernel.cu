@@ -20,13 +20,13 @@
 //
 // What bounds it: the cache's bytes, 2 D per key and KV head.  The tile's parts (128 keys x 128 dims of K, of V) are units of one
 // ring of shared memory, K of the next tile ahead of V of this one (the other way round, the four tokens below took 136 us
-// instead of 126).  One warp fills it with TMA boxes of 16 or 32 slots; runs of 16 keys that are not wholly visible, and all of them at 64 dims,
+// instead of 126 then).  One warp fills it with TMA boxes of 16 or 32 slots; runs of 16 keys that are not wholly visible, and all of them at 64 dims,
 // come by 16-byte copies, zero where a key is not visible, so what lies there in memory, NaN included, is never read.
 // Scales come with them, one per 16 keys.  The warp that works out the pieces makes the digits of their queries.
 //
 // Measured (32 heads of 8, 128 dims, bf16, calls behind one another): one token of 64 requests x 8,192 keys, 1.08 GB, 172 us, 0.96 of the
-// copy bandwidth; four tokens of 32 requests of 2,000 to 16,384 keys, 0.65 GB, 126 us, 0.79: 16 rows' softmax, two groups of warps
-// with a barrier for each tile's vote, takes as long as their bytes.  12 heads of 2, 256 dims, 0.53 GB: 92 us, 0.87.  Eight requests of up to 4,095 keys
+// copy bandwidth; four tokens of 32 requests of 2,000 to 16,384 keys, 0.65 GB, 125 us, 0.80: 16 rows' softmax, two groups of warps
+// with a barrier for each tile's vote, takes as long as their bytes.  12 heads of 2, 256 dims, 0.53 GB: 90 us, 0.90.  Eight requests of up to 4,095 keys
 // 19 us, of which 10 are one tile's way through launch, look-ups, queries, products and rows, and 2 to 5 the merge.
 //
 // Schedule and merge: kv16_short.cuh.

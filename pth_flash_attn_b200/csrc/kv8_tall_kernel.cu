@@ -24,9 +24,9 @@
 //
 // What bounds it.  A step's softmax, 1,300 to 1,500 clocks of 64 exponentials and their conversions a row, beside 300 to 500 of waiting for S; power
 // (the 1,000 W limit) in long calls; a piece's own 8,000 to 10,000 clocks (queries, first S, rows, merge) in short ones.  Measured (bf16 unless
-// said, calls behind one another): four chunks of 2,048 tokens over 8,192 keys before them, 32 heads of 8, 128 dims: 1,260 to 1,340 us, 0.56 to
-// 0.59 of the bf16 rate of a library product.  Twelve prompts of 37 to 2,500 tokens: 16 heads of 16, 64 dims, fp16, 174 us; 32 heads of 8, 128 dims,
-// 329 us.  256 dims, the same chunks: 3,400 us, one row tile per SM.
+// said, calls behind one another): four chunks of 2,048 tokens over 8,192 keys before them, 32 heads of 8, 128 dims: 1,150 to 1,245 us, 0.60 to
+// 0.65 of the bf16 rate of a library product (fp16 1,370; 16 heads of 16, 64 dims, 553).  Twelve prompts of 37 to 2,500 tokens: 16 heads of 16, 64 dims, fp16, 171 us; 32 heads of 8, 128 dims,
+// 326 us.  256 dims, the same chunks: 3,400 us, one row tile per SM.
 //
 // Schedule: the rows of a request and KV head in row tiles, a first one together with a last one, so that under a causal mask
 // these units are about equally long; all units form one sequence in KV tiles of 128 keys, which is cut into equal runs, one per
@@ -63,9 +63,10 @@ struct Tall8 {
   static constexpr int wide = kKeys * HD * 2;        // W of a step: slabs of 64 dims, 64 rows of 128 bytes, swizzled
   static constexpr int q_digit = 128 * HD;           // column block c of 16 dims at c 2,048, row r at r 16
   static constexpr int q_tile = q_digits * q_digit;
-  // (K of 64 dims with two, three, four and six units: the twelve prompts 178, 178, 174, 178 us)
   static constexpr int k_units = HD == 64 ? 4 : HD == 128 ? (kHalf ? 4 : 6) : (kHalf ? 2 : 3);
-  static constexpr int at_once = HD == 256 ? 1 : 2;   // steps that the loading warp asks for together (256 dims have no room for more)
+  // Steps that the loading warp asks for together: with one its own instructions took as long as a step, and the MMAs waited for keys (the chunks 617
+  // instead of 553 us at 64 dims, 1,297 instead of 1,196 at 128; 256 dims have no room for two).
+  static constexpr int at_once = HD == 256 ? 1 : 2;
   static constexpr int v_units = HD == 64 ? 4 : HD == 128 ? (kHalf ? 3 : 4) : 2;
   static constexpr int w_units = HD == 64 ? 4 : HD == 128 ? 3 : 2;
   static_assert(v_units + w_units + at_once < kScaleSteps, "scales outlive their readers");
