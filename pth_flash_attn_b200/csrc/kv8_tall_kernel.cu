@@ -25,8 +25,8 @@
 // What bounds it.  A step's softmax, 1,300 to 1,500 clocks of 64 exponentials and their conversions a row, beside 300 to 500 of waiting for S; power
 // (the 1,000 W limit) in long calls; a piece's own 8,000 to 10,000 clocks (queries, first S, rows, merge) in short ones.  Measured (bf16 unless
 // said, calls behind one another): four chunks of 2,048 tokens over 8,192 keys before them, 32 heads of 8, 128 dims: 1,150 to 1,245 us, 0.60 to
-// 0.65 of the bf16 rate of a library product (fp16 1,370; 16 heads of 16, 64 dims, 553).  Twelve prompts of 37 to 2,500 tokens: 16 heads of 16, 64 dims, fp16, 171 us; 32 heads of 8, 128 dims,
-// 326 us.  256 dims, the same chunks: 3,400 us, one row tile per SM.
+// 0.65 of the bf16 rate of a library product (fp16 1,370; 16 heads of 16, 64 dims, 553).  Twelve prompts of 37 to 2,500 tokens: 16 heads of 16, 64 dims, fp16, 166 us; 32 heads of 8, 128 dims,
+// 316 us.  256 dims, the same chunks: 3,400 us, one row tile per SM.
 //
 // Schedule: the rows of a request and KV head in row tiles, a first one together with a last one, so that under a causal mask
 // these units are about equally long; all units form one sequence in KV tiles of 128 keys, which is cut into equal runs, one per
@@ -48,8 +48,9 @@ constexpr float kMostSum = 0x1p15f;    // of 64 P
 constexpr int kKeys = 64;              // of a step
 constexpr int kScaleSteps = 16;        // steps whose scales are kept: more than the rings hold of V, raw and wide, and one
 constexpr int kWidenWarps = 4;
-// KV tiles that a row tile counts besides its own: its queries, its first maximum and its rows' way out.
-constexpr int kItemTiles = 2;
+// KV tiles that a row tile counts besides its own: its queries, its first maximum and its rows' way out.  (With 1, 2, 3, 4 and 6, the twelve
+// prompts above: 183, 172, 166, 166, 169 us at 64 dims, 358, 325, 316, 315, 323 at 128.)
+constexpr int kItemTiles = 3;
 
 template <int HD, bool kHalf>
 struct Tall8 {

@@ -1,5 +1,5 @@
 """The schedule of the 8-bit cache's kernel for prompts, as the kernel computes it (``kv8_tall_kernel.cu``: row_tile8, units8, TallWalk8)."""
-TILE, ITEM_TILES = 128, 2
+TILE, ITEM_TILES = 128, 3
 
 
 class Request:
