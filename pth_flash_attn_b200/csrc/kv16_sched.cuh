@@ -34,7 +34,7 @@ struct Piece {
   int first_cta, last_cta;    // that have its pieces (in the counting of the kernel's schedule)
   int sparse;                 // CTAs between them may have none
   int pos0;                   // position of the request's first query token (8-bit cache)
-  int unused;
+  int edges;                  // its steps at either end that some rows do not see whole (kv8_tall_kernel.cu)
 };
 static_assert(sizeof(Piece) == 64, "queue entry");
 

@@ -65,9 +65,11 @@ __device__ __forceinline__ void mma_e4m3(uint32_t d_tmem, uint64_t a_desc, uint6
       : "memory");
 }
 
-// NaN cells of a word: the top bit of their bytes; they become zero.
+// NaN cells of a word: the top bit of their bytes.
+__device__ __forceinline__ uint32_t nan_cells(uint32_t w) { return (w & 0x7f7f7f7fu) + 0x01010101u & 0x80808080u; }
+// The same; they become zero.
 __device__ __forceinline__ uint32_t take_nan(uint32_t& w) {
-  const uint32_t nan = (w & 0x7f7f7f7fu) + 0x01010101u & 0x80808080u;
+  const uint32_t nan = nan_cells(w);
   w &= ~((nan >> 7) * 0xffu);
   return nan;
 }

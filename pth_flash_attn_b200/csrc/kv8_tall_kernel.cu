@@ -95,7 +95,14 @@ struct Tall8 {
                        pv_done = p_ready + 2 * rts, scales_full = pv_done + 2 * rts, queue = scales_full + kScaleSteps, drained = queue + 2 * kQueue,
                        n_bars = drained + rts;
   static constexpr int pieces = bars + n_bars * 8;   // PieceQueue's entries
-  static constexpr int misc = pieces + kQueue * 64;  // ints: abort flag, TMEM address, arrivals [2], stop; scratch of find_run
+  // Steps of a piece that some of its rows do not see whole (edges8), at most: in front of the last row's window 4 (of 128 rows) or 6
+  // (256), from the first row's own key on 3 or 5.
+  static constexpr int nan_steps = rows == 128 ? 8 : 12;
+  static constexpr int nan_words = 1 + 2 * nan_steps;
+  // Pieces whose notes are kept: these are cleared in front of a piece's entry into the queue, when all warps have begun the piece kQueue + 1 before.
+  static constexpr int nan_pieces = kQueue + 2;
+  static constexpr int nan = pieces + kQueue * 64;   // uint32_t [nan_pieces][nan_words]: whether there is any; 64 keys of each such step
+  static constexpr int misc = nan + (nan_pieces * nan_words + 1) / 2 * 8;   // ints: abort flag, TMEM address, arrivals [2], stop; scratch of find_run
   static constexpr int total = misc + 32 + (threads / 32 + 2) * 8 + 1024;
   static_assert(total <= (ctas == 2 ? 115712 : 232448), "shared memory");
 };
@@ -227,6 +234,9 @@ __device__ __forceinline__ TallWalk8<RP> find_run8(const Kv8Params& p, long long
 // Steps of a piece: its keys from key0 on, as far as its row tile sees them; one at least.
 __device__ __forceinline__ int steps8(const Piece& it) { return max(1, (min(it.tiles * kTile, it.hi - it.key0) + kKeys - 1) / kKeys); }
 
+// Behind any of a CTA's waits may stand a row tile whose rows are on their way out, merged or not: all have the bound of whole pieces.
+__device__ __forceinline__ bool piece_wait(uint64_t* bar, uint32_t parity, volatile int* abort_flag) { return kv16_wait<kPieceTimes>(bar, parity, abort_flag); }
+
 // ---- operands ----
 
 template <bool kAccumulate>
@@ -300,11 +310,6 @@ __device__ __forceinline__ float exponentials8(const uint32_t (&r)[64], const fl
 __device__ __forceinline__ int64_t scale_at(const Kv8Params& p, int kvh, int blk, int slot) {
   return (int64_t)blk * p.scale_stride_block + (int64_t)((uint32_t)slot / (uint32_t)p.scale_tokens) * p.scale_stride_group + (int64_t)kvh * p.scale_stride_head;
 }
-template <bool kHalf>
-__device__ __forceinline__ float load_elem16(const uint8_t* row, int d) {
-  if constexpr (kHalf) return __half2float(reinterpret_cast<const __half*>(row)[d]);
-  else return __bfloat162float(reinterpret_cast<const __nv_bfloat16*>(row)[d]);
-}
 
 // Asks for a warp's 32 query rows of a piece, as they are: row n at raw + n 2 HD, its 16-byte pieces swizzled by n.
 template <int HD>
@@ -372,31 +377,48 @@ __device__ __forceinline__ float stage_row(const Kv8Params& p, const uint8_t* ra
   return finite ? power_of_two(e) * p.scale_log2 : -1.f;
 }
 
-// A value that is NaN under a key that a row does not see makes the row's sum NaN all the same: its weight is zero, but zero times NaN
-// is NaN.  So a row that finds NaN among its sums adds 32 of them up again, key by key, over the piece's keys [lo, hi) that it sees.
-// (Looking for NaN as V is widened cost every launch: twelve prompts 276 us instead of 237.  A function of its own, which the hot
-// code does not run through; only softmax threads call it, who have more registers than the launch gave.)
-template <int HD, bool kHalf>
-__device__ __noinline__ void sum_again(const Kv8Params& p, const Piece& it, const uint8_t* q_row, int lo, int hi, float ref, int d0, uint32_t* sums) {
-  for (int d = 0; d < 16; ++d) sums[d] = 0u;
+// A value that is NaN under a key that a row does not see would make the row's sum NaN all the same: its weight is zero, but zero times NaN
+// is NaN.  So in the steps that some of a piece's rows do not see whole, the widening warps make NaN zero and note the key; at
+// the piece's end a row puts NaN where one of those that it sees has it.  Such steps are few, at a piece's ends, so the others' cells
+// are not looked at (of all, prompts of 37 to 2,500 tokens took 276 us instead of 237), and what is put in costs by the keys noted.
+//
+// Piece::edges: steps at its beginning, in front of what the last row sees, + 16 times those at its end, behind what the first row sees.
+__device__ __forceinline__ int edges8(const Kv8Params& p, const Piece& it) {
+  const int steps = steps8(it), lo = kv8_low(p, it.pos0 + (it.row0 + it.rows - 1) / p.group);
+  const int hi = p.causal ? max(0, it.pos0 + it.row0 / p.group + 1) : INT_MAX;
+  const int below = min(steps, (max(0, lo - it.key0) + kKeys - 1) / kKeys), from = min(steps, max(below, max(0, hi - it.key0) / kKeys));
+  return below | (steps - from) << 4;
+}
+struct Edges8 {
+  int below, from, notes;   // steps [0, below) and [from, ..), their number
+  __device__ __forceinline__ Edges8(const Piece& it, int steps) : below(it.edges & 15), from(steps - (it.edges >> 4)), notes(below + (it.edges >> 4)) {}
+  __device__ __forceinline__ bool has(int step) const { return step < below || step >= from; }
+  __device__ __forceinline__ int note_of(int step) const { return step < below ? step : below + step - from; }
+  __device__ __forceinline__ int step_of(int note) const { return note < below ? note : from + note - below; }
+};
+// The columns of a row that are NaN by a key that was noted and that the row sees, [lo, hi): 16 to a word.  (A function of its own, which the
+// hot code does not run through; only softmax threads call it, who have more registers than the launch gave.)
+template <int HD>
+__device__ __noinline__ void nan_columns(const Kv8Params& p, const Piece& it, const uint32_t* noted, int lo, int hi, uint32_t* columns) {
+  const Edges8 edges(it, steps8(it));
+  for (int c = 0; c < HD / 16; ++c) columns[c] = 0u;
 #pragma unroll 1
-  for (int pos = lo; pos < hi; ++pos) {
-    int slot;
-    const int blk = block_of(p, it.r, pos, &slot);
-    if (blk < 0) continue;   // (a value of zero)
-    const int64_t at = (int64_t)blk * p.stride_block + (int64_t)slot * p.stride_slot + (int64_t)it.kvh * p.stride_head, scale = scale_at(p, it.kvh, blk, slot);
-    float s = 0.f;
+  for (int i = 0; i < 2 * edges.notes; ++i) {
 #pragma unroll 1
-    for (int d = 0; d < HD; d += 2) {
-      const float2 k = float2_of_e4m3x2(*reinterpret_cast<const uint16_t*>(p.k + at + d));
-      s = fmaf(load_elem16<kHalf>(q_row, d), k.x, s);
-      s = fmaf(load_elem16<kHalf>(q_row, d + 1), k.y, s);
-    }
-    const float w = ex2f(s * p.k_scale[scale] * p.scale_log2 - ref) * p.v_scale[scale];
-    for (int d = 0; d < 16; d += 2) {
-      const float2 v = float2_of_e4m3x2(*reinterpret_cast<const uint16_t*>(p.v + at + d0 + d));
-      sums[d] = __float_as_uint(fmaf(w, v.x, __uint_as_float(sums[d])));
-      sums[d + 1] = __float_as_uint(fmaf(w, v.y, __uint_as_float(sums[d + 1])));
+    for (uint32_t keys = noted[1 + i]; keys != 0; keys &= keys - 1) {
+      const int pos = it.key0 + edges.step_of(i / 2) * kKeys + (i & 1) * 32 + __ffs(keys) - 1;
+      if (pos < lo || pos >= hi) continue;
+      int slot;
+      const int blk = block_of(p, it.r, pos, &slot);
+      if (blk < 0) continue;
+      const float scale = p.v_scale[scale_at(p, it.kvh, blk, slot)];
+      const uint4* const v = reinterpret_cast<const uint4*>(p.v + (int64_t)blk * p.stride_block + (int64_t)slot * p.stride_slot + (int64_t)it.kvh * p.stride_head);
+      auto four = [](uint32_t w) { return (nan_cells(w) >> 7) * 0x01020408u >> 24 & 15u; };   // (bytes' top bits side by side)
+#pragma unroll 4
+      for (int c = 0; c < HD / 16; ++c) {
+        const uint4 w = v[c];
+        columns[c] |= scale != scale ? 0xffffu : four(w.x) | four(w.y) << 4 | four(w.z) << 8 | four(w.w) << 12;
+      }
     }
   }
 }
@@ -468,6 +490,8 @@ __global__ void __launch_bounds__((Tall8<HD, kHalf>::threads), (Tall8<HD, kHalf>
     Piece it;
     bool going = true;
     while (going && walk.next(p, &it)) {
+      it.edges = edges8(p, it);
+      if (lane < G::nan_words) reinterpret_cast<uint32_t*>(smem + G::nan)[queue.i % G::nan_pieces * G::nan_words + lane] = 0u;
       going = queue.put(it, abort_flag);
       if (!going) break;
       const int n = steps8(it);
@@ -484,7 +508,7 @@ __global__ void __launch_bounds__((Tall8<HD, kHalf>::threads), (Tall8<HD, kHalf>
       auto free_units = [&](int first, int units, uint32_t asked_for, int here) {
         for (int i = 0; i < here; ++i) {
           const uint32_t u = asked_for + i;
-          if (u >= (uint32_t)units) ok &= kv16_wait(&bars[first + u % units], ((u / units) - 1) & 1, abort_flag);
+          if (u >= (uint32_t)units) ok &= piece_wait(&bars[first + u % units], ((u / units) - 1) & 1, abort_flag);
         }
         ok = __all_sync(0xffffffffu, ok);
         return ok;
@@ -540,30 +564,57 @@ __global__ void __launch_bounds__((Tall8<HD, kHalf>::threads), (Tall8<HD, kHalf>
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(G::widen_regs));
     constexpr int kCols = G::dims / 16, kPer = G::parts * kKeys * kCols / 128;   // 16-byte pieces of a thread
     const int thread = tid - G::widen_warp * 32;
-    uint32_t step = 0;
+    uint32_t step = 0, piece = 0;
     Piece it;
     while (queue.get(&it, abort_flag)) {
       const int n = steps8(it);
+      const Edges8 edges(it, n);
+      uint32_t* const noted = reinterpret_cast<uint32_t*>(smem + G::nan) + piece++ % G::nan_pieces * G::nan_words;
       int unit_e = -126;
 #pragma unroll 1
       for (int j = 0; j < n; ++j, ++step) {
         const uint32_t vu = step % G::v_units, wu = step % G::w_units, su = step % kScaleSteps;
-        ok &= kv16_wait(&bars[G::scales_full + su], (step / kScaleSteps) & 1, abort_flag);
-        const float4 vs = *reinterpret_cast<const float4*>(smem + G::scales + su * 32 + 16);
+        ok &= piece_wait(&bars[G::scales_full + su], (step / kScaleSteps) & 1, abort_flag);
+        float4 vs = *reinterpret_cast<const float4*>(smem + G::scales + su * 32 + 16);
         unit_e = max(unit_e, unit_exponent(largest(vs)));
         const float down = power_of_two(-unit_e);
-        ok &= kv16_wait(&bars[G::v_full + vu], (step / G::v_units) & 1, abort_flag);
-        if (step >= G::w_units) ok &= kv16_wait(&bars[G::w_empty + wu], ((step / G::w_units) - 1) & 1, abort_flag);
+        ok &= piece_wait(&bars[G::v_full + vu], (step / G::v_units) & 1, abort_flag);
+        if (step >= G::w_units) ok &= piece_wait(&bars[G::w_empty + wu], ((step / G::w_units) - 1) & 1, abort_flag);
         const uint8_t* const raw = smem + G::v + vu * G::raw;
         uint8_t* const wide = smem + G::w + wu * G::wide;
         const int key0 = it.key0 + j * kKeys;
+        uint4 cells[kPer];
+#pragma unroll
+        for (int i = 0; i < kPer; ++i) {
+          const int x = i * 128 + thread, part = x / (kKeys * kCols), key = x / kCols % kKeys, c = x % kCols;
+          cells[i] = *reinterpret_cast<const uint4*>(raw + part * (kKeys * 128) + key * G::dims + ((HD == 64 ? c ^ ((key >> 1) & 3) : c ^ (key & 7)) << 4));
+          if (key0 + key < it.lo || key0 + key >= it.hi) cells[i] = make_uint4(0u, 0u, 0u, 0u);
+        }
+        if (edges.has(j)) {
+          uint32_t nan = 0;
+#pragma unroll
+          for (int i = 0; i < kPer; ++i) nan |= nan_cells(cells[i].x) | nan_cells(cells[i].y) | nan_cells(cells[i].z) | nan_cells(cells[i].w);
+          const float scales_sum = (vs.x + vs.y) + (vs.z + vs.w);   // (NaN where one of them is)
+          if (__builtin_expect(nan != 0 || scales_sum != scales_sum, 0)) {
+#pragma unroll
+            for (int i = 0; i < kPer; ++i) {
+              const int key = (i * 128 + thread) / kCols % kKeys;
+              const float s = key < 16 ? vs.x : key < 32 ? vs.y : key < 48 ? vs.z : vs.w;
+              const uint32_t found = take_nan(cells[i].x) | take_nan(cells[i].y) | take_nan(cells[i].z) | take_nan(cells[i].w);
+              if (found != 0 || (s != s && key0 + key >= it.lo && key0 + key < it.hi)) {
+                atomicOr(noted + 1 + 2 * edges.note_of(j) + (key >> 5), 1u << (key & 31));
+                *noted = 1u;
+              }
+            }
+            vs = make_float4(vs.x == vs.x ? vs.x : 0.f, vs.y == vs.y ? vs.y : 0.f, vs.z == vs.z ? vs.z : 0.f, vs.w == vs.w ? vs.w : 0.f);
+          }
+        }
 #pragma unroll
         for (int i = 0; i < kPer; ++i) {
           const int x = i * 128 + thread, part = x / (kKeys * kCols), key = x / kCols % kKeys, c = x % kCols;
           const float s = key < 16 ? vs.x : key < 32 ? vs.y : key < 48 ? vs.z : vs.w;
           const __half2 factor = __float2half2_rn(s * down);
-          uint4 v = *reinterpret_cast<const uint4*>(raw + part * (kKeys * 128) + key * G::dims + ((HD == 64 ? c ^ ((key >> 1) & 3) : c ^ (key & 7)) << 4));
-          if (key0 + key < it.lo || key0 + key >= it.hi) v = make_uint4(0u, 0u, 0u, 0u);
+          const uint4 v = cells[i];
           const uint2 a = widen4(v.x, factor), b = widen4(v.y, factor), d = widen4(v.z, factor), e = widen4(v.w, factor);
           // dims 16 c .. of slab c / 4: two pieces of 8, in an order that leaves lanes of two slabs on different banks
           uint8_t* const to = wide + (part * 2 + (c >> 2)) * (kKeys * 128) + key * 128;
@@ -605,9 +656,9 @@ __global__ void __launch_bounds__((Tall8<HD, kHalf>::threads), (Tall8<HD, kHalf>
     uint32_t s_qk = 0, s_pv = 0, pieces = 0;   // steps so far, pieces with live rows
     auto qk = [&](bool first) {
       const uint32_t b = s_qk & 1;
-      if (first) ok &= kv16_wait(&bars[G::q_full + rt], (pieces - 1) & 1, abort_flag);
-      ok &= kv16_wait(&bars[G::k_full + k_slot], k_phase, abort_flag);
-      if (s_qk > 1) ok &= kv16_wait(&bars[G::pv_done + 2 * rt + b], ((s_qk >> 1) - 1) & 1, abort_flag);   // (P of the step before last has been read)
+      if (first) ok &= piece_wait(&bars[G::q_full + rt], (pieces - 1) & 1, abort_flag);
+      ok &= piece_wait(&bars[G::k_full + k_slot], k_phase, abort_flag);
+      if (s_qk > 1) ok &= piece_wait(&bars[G::pv_done + 2 * rt + b], ((s_qk >> 1) - 1) & 1, abort_flag);   // (P of the step before last has been read)
       if (!ok) return;
       tc::fence_after_sync();
 #pragma unroll
@@ -631,8 +682,8 @@ __global__ void __launch_bounds__((Tall8<HD, kHalf>::threads), (Tall8<HD, kHalf>
     };
     auto pv = [&](bool first) {
       const uint32_t b = s_pv & 1;
-      ok &= kv16_wait(&bars[G::w_full + w_slot], w_phase, abort_flag);
-      ok &= kv16_wait(&bars[G::p_ready + 2 * rt + b], (s_pv >> 1) & 1, abort_flag);
+      ok &= piece_wait(&bars[G::w_full + w_slot], w_phase, abort_flag);
+      ok &= piece_wait(&bars[G::p_ready + 2 * rt + b], (s_pv >> 1) & 1, abort_flag);
       if (!ok) return;
       tc::fence_after_sync();
 #pragma unroll
@@ -655,8 +706,8 @@ __global__ void __launch_bounds__((Tall8<HD, kHalf>::threads), (Tall8<HD, kHalf>
       if (it.rows <= rt * 128) {   // no rows: free the units as if they had been read
 #pragma unroll 1
         for (int j = 0; j < n; ++j) {
-          ok &= kv16_wait(&bars[G::k_full + k_slot], k_phase, abort_flag);
-          ok &= kv16_wait(&bars[G::w_full + w_slot], w_phase, abort_flag);
+          ok &= piece_wait(&bars[G::k_full + k_slot], k_phase, abort_flag);
+          ok &= piece_wait(&bars[G::w_full + w_slot], w_phase, abort_flag);
           if (!ok) break;
           mbar_arrive(&bars[G::k_empty + k_slot]);
           mbar_arrive(&bars[G::w_empty + w_slot]);
@@ -685,12 +736,14 @@ __global__ void __launch_bounds__((Tall8<HD, kHalf>::threads), (Tall8<HD, kHalf>
     auto rt_sync = [&] { named_barrier(1 + rt, 128); };
     uint8_t* const raw_q = smem + (HD == 64 ? G::raw_q : G::q + rt * G::q_tile);
     const uint32_t raw_rows = tc::smem_u32(raw_q) + (row & 96) * (2 * HD);   // of the warp
+    uint32_t piece = 0;    // pieces so far
     bool copied = false;   // the piece's query rows are on their way
     zero_requests<HD, RP, 128 * G::rts>(p);
     {
       Piece it;
       while (queue.get(&it, abort_flag)) {
         const int n_steps = steps8(it);
+        const uint32_t* const noted = reinterpret_cast<const uint32_t*>(smem + G::nan) + piece++ % G::nan_pieces * G::nan_words;
         if (it.rows <= rt * 128) {
           step += n_steps;
           copied = false;
@@ -722,7 +775,7 @@ __global__ void __launch_bounds__((Tall8<HD, kHalf>::threads), (Tall8<HD, kHalf>
         for (int t = 0; t < n_steps; ++t, ++count, ++step) {
           const uint32_t b = 2 * rt + (count & 1), use = count >> 1, su = step % kScaleSteps;
           const uint32_t s_tmem = tmem_base + G::s_col + b * kKeys + lane_addr;
-          ok &= kv16_wait(&bars[G::s_ready + b], use & 1, abort_flag);
+          ok &= piece_wait(&bars[G::s_ready + b], use & 1, abort_flag);
           if (padding) {   // (the order of the waits is kept, nothing is computed)
             mbar_arrive(&bars[G::p_ready + b]);
             continue;
@@ -775,7 +828,7 @@ __global__ void __launch_bounds__((Tall8<HD, kHalf>::threads), (Tall8<HD, kHalf>
             l *= alpha;
             unit_e = e;
             if (t > 0) {   // (PV of what P holds already is complete first)
-              ok &= kv16_wait(&bars[G::pv_done + (b ^ 1)], ((count - 1) >> 1) & 1, abort_flag);
+              ok &= piece_wait(&bars[G::pv_done + (b ^ 1)], ((count - 1) >> 1) & 1, abort_flag);
               tc::fence_after_sync();
 #pragma unroll 1
               for (int d = 0; d < HD / 16; ++d) {
@@ -801,7 +854,7 @@ __global__ void __launch_bounds__((Tall8<HD, kHalf>::threads), (Tall8<HD, kHalf>
           copied = true;
         }
         // ---- the piece's rows ----
-        ok &= kv16_wait(&bars[G::pv_done + 2 * rt + ((count - 1) & 1)], ((count - 1) >> 1) & 1, abort_flag);
+        ok &= piece_wait(&bars[G::pv_done + 2 * rt + ((count - 1) & 1)], ((count - 1) >> 1) & 1, abort_flag);
         tc::fence_after_sync();
         if (not_finite) l = NAN;
         const bool whole = it.begins && it.ends, live = row < it.rows;
@@ -824,23 +877,18 @@ __global__ void __launch_bounds__((Tall8<HD, kHalf>::threads), (Tall8<HD, kHalf>
         if (!padding) {
           const float unit = power_of_two(unit_e), factor = whole ? (l == 0.f ? 0.f : unit / l) : unit;
           float* const slot = tall8_slot<HD, kHalf>(p, (int)blockIdx.x, it.begins) + row;
+          const bool nan = it.edges != 0 && *noted != 0u;   // (the same in all threads)
+          uint32_t columns[HD / 16];
+          if (nan) nan_columns<HD>(p, it, noted, row_lo, row_hi, columns);
 #pragma unroll 1
           for (int c = 0; c < HD / 16; ++c) {
             uint32_t r[16];
             tc::tmem_ld16(o_tmem + c * 16, r);
             tc::tmem_ld_wait<16>(r);
-            f32x2 all[2] = {0ull, 0ull};
+            if (nan) {
 #pragma unroll
-            for (int n = 0; n < 16; n += 2) all[n / 2 & 1] = add2(all[n / 2 & 1], pair(__uint_as_float(r[n]), __uint_as_float(r[n + 1])));
-            const float any = sum_pairs(all);
-            if (__builtin_expect(any != any && l == l, 0)) {   // NaN, which may be of a key that the row does not see
-              uint32_t sums[16];
-              sum_again<HD, kHalf>(p, it, p.q + (int64_t)token * p.q_stride_token + (int64_t)head * p.q_stride_head, max(row_lo, it.key0),
-                                   min(min(row_hi, it.hi), it.key0 + it.tiles * kTile), ref == -INFINITY ? 0.f : ref, c * 16, sums);
-#pragma unroll
-              for (int n = 0; n < 16; ++n) r[n] = __float_as_uint(__uint_as_float(sums[n]) * power_of_two(-unit_e));
+              for (int n = 0; n < 16; ++n) r[n] = columns[c] >> n & 1u ? 0x7fffffffu : r[n];
             }
-            __syncwarp();
             float o[16];
 #pragma unroll
             for (int n = 0; n < 16; ++n) o[n] = __uint_as_float(r[n]) * factor;
