@@ -287,9 +287,10 @@ __device__ __forceinline__ void stage_queries(const Kv8Params& p, const Piece& i
       for (int i = 0; i < 8; ++i) top = fmaxf(top, fabsf(x[i]));
 #pragma unroll
       for (int o = kLanes / 2; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-      // u = 2^e: the row's largest into [128, 256); of a row with an infinity or NaN any u will do, of an empty one too
+      // u = 2^e: the row's largest into [128, 256); an empty row takes any.  A row with an infinity is NaN as a whole (not its factor: keys that it does
+      // not see have scores of -inf, and those stay)
       const int e = min(120, max(-119, (int)(__float_as_uint(top) >> 23) - 127 - 7));
-      const float up = power_of_two(-e);
+      const float up = isinf(top) ? NAN : power_of_two(-e);
       uint32_t d[4][G::q_digits];
 #pragma unroll
       for (int i = 0; i < 4; ++i) digits2<G::q_digits>(x[2 * i] * up, x[2 * i + 1] * up, d[i]);
@@ -297,7 +298,7 @@ __device__ __forceinline__ void stage_queries(const Kv8Params& p, const Piece& i
 #pragma unroll
       for (int g = 0; g < G::q_digits; ++g)
         *reinterpret_cast<uint2*>(to + g * (RP * 16)) = make_uint2(d[0][g] | d[1][g] << 16, d[2][g] | d[3][g] << 16);
-      if (chunk == 0) factor[n] = isinf(top) ? NAN : fmaxf(power_of_two(e) * p.scale_log2, 1e-37f);   // (never zero: hidden scores are -inf)
+      if (chunk == 0) factor[n] = fmaxf(power_of_two(e) * p.scale_log2, 1e-37f);   // (never zero: hidden scores are -inf)
     }
   }
 }

@@ -856,7 +856,7 @@ __global__ void __launch_bounds__((Tall8<HD, kHalf>::threads), (Tall8<HD, kHalf>
         // ---- the piece's rows ----
         ok &= piece_wait(&bars[G::pv_done + 2 * rt + ((count - 1) & 1)], ((count - 1) >> 1) & 1, abort_flag);
         tc::fence_after_sync();
-        if (not_finite) l = NAN;
+        if (not_finite && max(row_lo, it.key0) < min(row_hi, it.key0 + it.tiles * kTile)) l = NAN;   // (a row that sees no key is zero)
         const bool whole = it.begins && it.ends, live = row < it.rows;
         uint8_t* const out = p.out + (int64_t)token * p.out_stride_token + (int64_t)head * p.out_stride_head;
         float* const lse = p.lse != nullptr ? p.lse + (int64_t)token * p.num_q_heads + head : nullptr;
