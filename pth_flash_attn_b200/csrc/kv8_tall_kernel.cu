@@ -2,7 +2,7 @@
 //
 // Orientation: query rows on the MMA's M dimension, a thread per row in the softmax:
 //   S[row, key] = sum_d Q[row, d] c_K[key, d]    A = digits of Q, B = c_K as it lies in the cache (kind::f8f6f4), accumulator in TMEM
-//   O[row, d]  += sum_key P[row, key] W[key, d]  A = P in TMEM over S, B = W = c_V scale_V / U in fp16 (kind::f16)
+//   O[row, d]  += sum_key Y[row, key] c_V[key, d]  A = Y = P scale_V / U in TMEM over S, B = c_V in fp16 (kind::f16)
 // An SM holds two row tiles of 128 rows: of one CTA at 128 dims, where every tile of keys then serves twice, of two CTAs at 64 dims; at
 // 256 dims O alone takes half of TMEM: one row tile.  A step is 64 keys; S has two buffers, so that a step's QK and the last
 // one's PV run beside its softmax.
@@ -10,9 +10,11 @@
 // Q is a sum of e4m3 digits (two for bf16, three for fp16), all in one accumulator: x = u (d0 + d1 + d2), u a power of two per row that
 // puts the row's largest into (224, 448].  A digit is the rounding of what is left, so bf16 numbers are exact down to 2^-10 of their row's
 // largest and off by 2^-17 of it at most below.  Two MMAs over 8-bit operands take as long as one over 16-bit ones.
-// V passes through registers once per tile: a cell times scale_V / U is fp16, exactly where the scales are powers of two within 2^15
-// of the largest (U, the largest scale_V so far in the piece, to the next power of two: O is rescaled where a tile brings a larger
-// one); what is below 2^-25 of it is zero.  So P needs no digits: one 16-bit number, with 32-bit sums.
+// V passes through registers once per tile: fp16 holds every e4m3 number.  Its scale goes into the weights, in 32 bits, ahead of their one rounding to
+// fp16: U is the largest scale that the row has seen so far in the piece (O is rescaled where a step brings a larger one), so weights are at most
+// P, and keys that a row does not see change nothing for it, whatever their scale.  (With c_V scale_V / U as operand B and a U for all rows, a scale that is
+// no power of two was rounded to 11 bits itself, the same way for all its keys, and a scale 2^25 times the others', under keys that a row did not see,
+// left nothing of those that it did.)  So Y needs no digits: one 16-bit number, with 32-bit sums.
 //
 // Softmax in one pass: ref is a running bound of a row's scores (log2 units), P = 2^(s - ref), l = sum P, ref kGain below the maximum of
 // a row's first 64 keys.  Later ones need no maximum: the sum of 64 P says whether one of them has outgrown ref too far
@@ -46,7 +48,6 @@ namespace {
 constexpr float kGainP = 7.f;          // log2 of P of a row's largest score when its reference is set
 constexpr float kMostSum = 0x1p15f;    // of 64 P
 constexpr int kKeys = 64;              // of a step
-constexpr int kScaleSteps = 16;        // steps whose scales are kept: more than the rings hold of V, raw and wide, and one
 constexpr int kWidenWarps = 4;
 // KV tiles that a row tile counts besides its own: its queries, its first maximum and its rows' way out.  (With 1, 2, 3, 4 and 6, the twelve
 // prompts above: 183, 172, 166, 166, 169 us at 64 dims, 358, 325, 316, 315, 323 at 128.)
@@ -70,7 +71,9 @@ struct Tall8 {
   static constexpr int at_once = HD == 256 ? 1 : 2;
   static constexpr int v_units = HD == 64 ? 4 : HD == 128 ? (kHalf ? 3 : 4) : 2;
   static constexpr int w_units = HD == 64 ? 4 : HD == 128 ? 3 : 2;
-  static_assert(v_units + w_units + at_once < kScaleSteps, "scales outlive their readers");
+  // Steps whose scales are kept.  A unit of K that is free again says that QK of its step is complete, which waited for P of two steps before.
+  static constexpr int scale_steps = HD == 256 ? 8 : 16;
+  static_assert(k_units + at_once + 1 < scale_steps, "scales outlive their readers");
   static constexpr int softmax_warps = 4 * rts;
   static constexpr int widen_warp = softmax_warps, load_warp = widen_warp + kWidenWarps, mma_warp = load_warp + 1;
   static constexpr int threads = (mma_warp + rts) * 32;
@@ -89,10 +92,10 @@ struct Tall8 {
   static constexpr int q = w + w_units * wide;
   static constexpr int raw_q = q + rts * q_tile;     // query rows as they are (others: in the place of their digits)
   static constexpr int scales = raw_q + (HD == 64 ? 128 * HD * 2 : 0);   // float [kScaleSteps][2][4]: of the keys' runs of 16, of the values'
-  static constexpr int bars = scales + kScaleSteps * 32;
+  static constexpr int bars = scales + scale_steps * 32;
   static constexpr int k_full = 0, k_empty = k_full + k_units, v_full = k_empty + k_units, v_empty = v_full + v_units, w_full = v_empty + v_units,
                        w_empty = w_full + w_units, q_full = w_empty + w_units, s_ready = q_full + rts, p_ready = s_ready + 2 * rts,
-                       pv_done = p_ready + 2 * rts, scales_full = pv_done + 2 * rts, queue = scales_full + kScaleSteps, drained = queue + 2 * kQueue,
+                       pv_done = p_ready + 2 * rts, queue = pv_done + 2 * rts, drained = queue + 2 * kQueue,
                        n_bars = drained + rts;
   static constexpr int pieces = bars + n_bars * 8;   // PieceQueue's entries
   // Steps of a piece that some of its rows do not see whole (edges8), at most: in front of the last row's window 4 (of 128 rows) or 6
@@ -259,34 +262,29 @@ __device__ __forceinline__ uint64_t raw_desc(uint32_t saddr) {
   if constexpr (HD == 64) return tc::smem_desc(saddr, 16, 512) | (uint64_t)4 << 61;
   return swizzled_desc(saddr, 16, 1024);
 }
-// Four cells as fp16 times a factor; the keys' own NaN stays.
-__device__ __forceinline__ uint2 widen4(uint32_t w, __half2 factor) {
-  const uint32_t a = f16x2_of_e4m3x2(w & 0xffffu), b = f16x2_of_e4m3x2(w >> 16);
-  const __half2 x = __hmul2(*reinterpret_cast<const __half2*>(&a), factor), y = __hmul2(*reinterpret_cast<const __half2*>(&b), factor);
-  return make_uint2(*reinterpret_cast<const uint32_t*>(&x), *reinterpret_cast<const uint32_t*>(&y));
+// Four cells as fp16, which holds them all; NaN stays.
+__device__ __forceinline__ uint2 widen4(uint32_t w) { return make_uint2(f16x2_of_e4m3x2(w & 0xffffu), f16x2_of_e4m3x2(w >> 16)); }
+__device__ __forceinline__ f32x2 mul2(f32x2 a, f32x2 b) {
+  f32x2 r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
 }
-__device__ __forceinline__ float largest(float4 s) { return max3(fmaxf(fabsf(s.x), fabsf(s.y)), fabsf(s.z), fabsf(s.w)); }
 // A run's factor of its scores: never zero, since a hidden score is -inf under a scale of zero too; NaN stays NaN.
 __device__ __forceinline__ float score_factor(float scale, float q_factor) {
   float r;
   asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(scale * q_factor), "f"(1e-37f));
   return r;
 }
-// Exponent e of the power of two that is a step's unit: 2^e >= its largest scale.
-__device__ __forceinline__ int unit_exponent(float most) {
-  return min(126, max(-126, (int)((__float_as_uint(most) + 0x7fffffu) >> 23) - 127));
-}
-
 template <int HD, bool kHalf>
 __device__ __forceinline__ float* tall8_slot(const Kv8Params& p, int cta, bool begins) {
   // [HD][rows] O, [rows] ref, [rows] l
   return reinterpret_cast<float*>(p.workspace + kCounterBytes) + (int64_t)(2 * cta + (begins ? 1 : 0)) * (Tall8<HD, kHalf>::rows * (HD + 2));
 }
 
-// P of 64 scores, 2^(score factor + minus_ref), a factor for every 16 of them, to TMEM as pairs of fp16 numbers; returns the sum of the
-// unrounded ones.  (Kept in registers until the step is settled, P and the scores were more than 64 dims' warps have: what spilled went
+// P of 64 scores, 2^(score factor + minus_ref), a factor for every 16 of them, times a weight for every 16 of them, to TMEM as pairs of fp16 numbers; returns
+// the sum of P.  (Kept in registers until the step is settled, these and the scores were more than 64 dims' warps have: what spilled went
 // round in the first level cache, which shared memory leaves small.)
-__device__ __forceinline__ float exponentials8(const uint32_t (&r)[64], const float (&factor)[4], float minus_ref, uint32_t p_tmem) {
+__device__ __forceinline__ float exponentials8(const uint32_t (&r)[64], const float (&factor)[4], float minus_ref, const float (&weight)[4], uint32_t p_tmem) {
   const f32x2 ref2 = pair(minus_ref, minus_ref);
   f32x2 sum[2] = {0ull, 0ull};
 #pragma unroll
@@ -300,6 +298,7 @@ __device__ __forceinline__ float exponentials8(const uint32_t (&r)[64], const fl
       x = ex2f(x);
       y = ex2f(y);
       sum[n & 1] = add2(sum[n & 1], pair(x, y));
+      unpair(mul2(pair(x, y), pair(weight[n / 8], weight[n / 8])), x, y);
       pk[i] = pack_f16(x, y);
     }
     tc::tmem_st16(p_tmem + part * 16, pk);
@@ -384,8 +383,8 @@ __device__ __forceinline__ float stage_row(const Kv8Params& p, const uint8_t* ra
 //
 // Piece::edges: steps at its beginning, in front of what the last row sees, + 16 times those at its end, behind what the first row sees.
 __device__ __forceinline__ int edges8(const Kv8Params& p, const Piece& it) {
-  const int steps = steps8(it), lo = kv8_low(p, it.pos0 + (it.row0 + it.rows - 1) / p.group);
-  const int hi = p.causal ? max(0, it.pos0 + it.row0 / p.group + 1) : INT_MAX;
+  const int steps = steps8(it), hi = p.causal ? max(0, it.pos0 + it.row0 / p.group + 1) : INT_MAX;
+  const int lo = p.window > 0 ? kv8_low(p, it.pos0 + (it.row0 + it.rows - 1) / p.group) : 0;
   const int below = min(steps, (max(0, lo - it.key0) + kKeys - 1) / kKeys), from = min(steps, max(below, max(0, hi - it.key0) / kKeys));
   return below | (steps - from) << 4;
 }
@@ -411,13 +410,12 @@ __device__ __noinline__ void nan_columns(const Kv8Params& p, const Piece& it, co
       int slot;
       const int blk = block_of(p, it.r, pos, &slot);
       if (blk < 0) continue;
-      const float scale = p.v_scale[scale_at(p, it.kvh, blk, slot)];
       const uint4* const v = reinterpret_cast<const uint4*>(p.v + (int64_t)blk * p.stride_block + (int64_t)slot * p.stride_slot + (int64_t)it.kvh * p.stride_head);
       auto four = [](uint32_t w) { return (nan_cells(w) >> 7) * 0x01020408u >> 24 & 15u; };   // (bytes' top bits side by side)
 #pragma unroll 4
       for (int c = 0; c < HD / 16; ++c) {
         const uint4 w = v[c];
-        columns[c] |= scale != scale ? 0xffffu : four(w.x) | four(w.y) << 4 | four(w.z) << 8 | four(w.w) << 12;
+        columns[c] |= four(w.x) | four(w.y) << 4 | four(w.z) << 8 | four(w.w) << 12;
       }
     }
   }
@@ -460,7 +458,6 @@ __global__ void __launch_bounds__((Tall8<HD, kHalf>::threads), (Tall8<HD, kHalf>
         tc::mbar_init(&bars[G::p_ready + i], 128);
         tc::mbar_init(&bars[G::pv_done + i], 1);
       }
-      for (int i = 0; i < kScaleSteps; ++i) tc::mbar_init(&bars[G::scales_full + i], 8);
       PieceQueue(nullptr, &bars[G::queue], stop).init(G::threads / 32 - 1);
       *abort_flag = 0;
       tc::mbar_init_fence();
@@ -535,14 +532,12 @@ __global__ void __launch_bounds__((Tall8<HD, kHalf>::threads), (Tall8<HD, kHalf>
           }
         };
         const bool live = kind < 2 && mine < here;
-        const uint32_t step = asked_v + mine, ku = step % G::k_units, vu = step % G::v_units, su = step % kScaleSteps;
+        const uint32_t step = asked_v + mine, ku = step % G::k_units, vu = step % G::v_units, su = step % G::scale_steps;
         if (!free_units(G::k_empty, G::k_units, asked_k, here)) break;
-        // (the unit of V that was free for the last step says that the scales of kScaleSteps steps ago have been read)
         if (live) {
           const float* const base = kind == 0 ? p.k_scale : p.v_scale;
           copy4(scales + su * 32 + kind * 16 + (run & 3) * 4, blk >= 0 ? base + scale_at(p, it.kvh, blk, slot) : base, blk >= 0);
           copies_arrive(&bars[G::k_full + ku]);
-          copies_arrive(&bars[G::scales_full + su]);
           if (kind == 0) ask(k_map, k_ring + ku * G::raw, &bars[G::k_full + ku]);
         }
         asked_k += here;
@@ -570,58 +565,50 @@ __global__ void __launch_bounds__((Tall8<HD, kHalf>::threads), (Tall8<HD, kHalf>
       const int n = steps8(it);
       const Edges8 edges(it, n);
       uint32_t* const noted = reinterpret_cast<uint32_t*>(smem + G::nan) + piece++ % G::nan_pieces * G::nan_words;
-      int unit_e = -126;
 #pragma unroll 1
       for (int j = 0; j < n; ++j, ++step) {
-        const uint32_t vu = step % G::v_units, wu = step % G::w_units, su = step % kScaleSteps;
-        ok &= piece_wait(&bars[G::scales_full + su], (step / kScaleSteps) & 1, abort_flag);
-        float4 vs = *reinterpret_cast<const float4*>(smem + G::scales + su * 32 + 16);
-        unit_e = max(unit_e, unit_exponent(largest(vs)));
-        const float down = power_of_two(-unit_e);
+        const uint32_t vu = step % G::v_units, wu = step % G::w_units;
         ok &= piece_wait(&bars[G::v_full + vu], (step / G::v_units) & 1, abort_flag);
         if (step >= G::w_units) ok &= piece_wait(&bars[G::w_empty + wu], ((step / G::w_units) - 1) & 1, abort_flag);
         const uint8_t* const raw = smem + G::v + vu * G::raw;
         uint8_t* const wide = smem + G::w + wu * G::wide;
         const int key0 = it.key0 + j * kKeys;
-        uint4 cells[kPer];
+        constexpr int kBatch = kPer < 4 ? kPer : 2;
 #pragma unroll
-        for (int i = 0; i < kPer; ++i) {
-          const int x = i * 128 + thread, part = x / (kKeys * kCols), key = x / kCols % kKeys, c = x % kCols;
+        for (int i0 = 0; i0 < kPer; i0 += kBatch) {
+        uint4 cells[kBatch];
+#pragma unroll
+        for (int i = 0; i < kBatch; ++i) {
+          const int x = (i0 + i) * 128 + thread, part = x / (kKeys * kCols), key = x / kCols % kKeys, c = x % kCols;
           cells[i] = *reinterpret_cast<const uint4*>(raw + part * (kKeys * 128) + key * G::dims + ((HD == 64 ? c ^ ((key >> 1) & 3) : c ^ (key & 7)) << 4));
           if (key0 + key < it.lo || key0 + key >= it.hi) cells[i] = make_uint4(0u, 0u, 0u, 0u);
         }
         if (edges.has(j)) {
           uint32_t nan = 0;
 #pragma unroll
-          for (int i = 0; i < kPer; ++i) nan |= nan_cells(cells[i].x) | nan_cells(cells[i].y) | nan_cells(cells[i].z) | nan_cells(cells[i].w);
-          const float scales_sum = (vs.x + vs.y) + (vs.z + vs.w);   // (NaN where one of them is)
-          if (__builtin_expect(nan != 0 || scales_sum != scales_sum, 0)) {
+          for (int i = 0; i < kBatch; ++i) nan |= nan_cells(cells[i].x) | nan_cells(cells[i].y) | nan_cells(cells[i].z) | nan_cells(cells[i].w);
+          if (__builtin_expect(nan != 0, 0)) {
 #pragma unroll
-            for (int i = 0; i < kPer; ++i) {
-              const int key = (i * 128 + thread) / kCols % kKeys;
-              const float s = key < 16 ? vs.x : key < 32 ? vs.y : key < 48 ? vs.z : vs.w;
-              const uint32_t found = take_nan(cells[i].x) | take_nan(cells[i].y) | take_nan(cells[i].z) | take_nan(cells[i].w);
-              if (found != 0 || (s != s && key0 + key >= it.lo && key0 + key < it.hi)) {
-                atomicOr(noted + 1 + 2 * edges.note_of(j) + (key >> 5), 1u << (key & 31));
-                *noted = 1u;
-              }
+            for (int i = 0; i < kBatch; ++i) {
+              const int key = ((i0 + i) * 128 + thread) / kCols % kKeys;
+              if ((take_nan(cells[i].x) | take_nan(cells[i].y) | take_nan(cells[i].z) | take_nan(cells[i].w)) == 0) continue;
+              atomicOr(noted + 1 + 2 * edges.note_of(j) + (key >> 5), 1u << (key & 31));
+              *noted = 1u;
             }
-            vs = make_float4(vs.x == vs.x ? vs.x : 0.f, vs.y == vs.y ? vs.y : 0.f, vs.z == vs.z ? vs.z : 0.f, vs.w == vs.w ? vs.w : 0.f);
           }
         }
 #pragma unroll
-        for (int i = 0; i < kPer; ++i) {
-          const int x = i * 128 + thread, part = x / (kKeys * kCols), key = x / kCols % kKeys, c = x % kCols;
-          const float s = key < 16 ? vs.x : key < 32 ? vs.y : key < 48 ? vs.z : vs.w;
-          const __half2 factor = __float2half2_rn(s * down);
+        for (int i = 0; i < kBatch; ++i) {
+          const int x = (i0 + i) * 128 + thread, part = x / (kKeys * kCols), key = x / kCols % kKeys, c = x % kCols;
           const uint4 v = cells[i];
-          const uint2 a = widen4(v.x, factor), b = widen4(v.y, factor), d = widen4(v.z, factor), e = widen4(v.w, factor);
+          const uint2 a = widen4(v.x), b = widen4(v.y), d = widen4(v.z), e = widen4(v.w);
           // dims 16 c .. of slab c / 4: two pieces of 8, in an order that leaves lanes of two slabs on different banks
           uint8_t* const to = wide + (part * 2 + (c >> 2)) * (kKeys * 128) + key * 128;
           const int first = (c >> 2) & 1;
           const uint4 lo = make_uint4(a.x, a.y, b.x, b.y), hi = make_uint4(d.x, d.y, e.x, e.y);
           *reinterpret_cast<uint4*>(to + (((2 * (c & 3) + first) ^ (key & 7)) << 4)) = first ? hi : lo;
           *reinterpret_cast<uint4*>(to + (((2 * (c & 3) + (first ^ 1)) ^ (key & 7)) << 4)) = first ? lo : hi;
+        }
         }
         tc::fence_async_smem();   // (W to the tensor core; the raw rows' reads in front of the boxes that come there next)
         __syncwarp();
@@ -769,11 +756,11 @@ __global__ void __launch_bounds__((Tall8<HD, kHalf>::threads), (Tall8<HD, kHalf>
         const int own = it.pos0 + token - it.first_token;
         const int row_lo = kv8_low(p, own), row_hi = p.causal ? min(own + 1, it.hi) : it.hi;
         float ref = -INFINITY, l = 0.f;
-        int unit_e = -126;
+        float unit = 0x1p-126f, inverse = 0x1p126f;   // U: the largest scale of values that the row has seen
         const bool not_finite = q_factor < 0.f;
 #pragma unroll 1
         for (int t = 0; t < n_steps; ++t, ++count, ++step) {
-          const uint32_t b = 2 * rt + (count & 1), use = count >> 1, su = step % kScaleSteps;
+          const uint32_t b = 2 * rt + (count & 1), use = count >> 1, su = step % G::scale_steps;
           const uint32_t s_tmem = tmem_base + G::s_col + b * kKeys + lane_addr;
           ok &= piece_wait(&bars[G::s_ready + b], use & 1, abort_flag);
           if (padding) {   // (the order of the waits is kept, nothing is computed)
@@ -785,7 +772,8 @@ __global__ void __launch_bounds__((Tall8<HD, kHalf>::threads), (Tall8<HD, kHalf>
           tc::tmem_ld32(s_tmem, r);
           tc::tmem_ld32(s_tmem + 32, r + 32);
           const float4 ks = *reinterpret_cast<const float4*>(smem + G::scales + su * 32);
-          const float most = largest(*reinterpret_cast<const float4*>(smem + G::scales + su * 32 + 16));
+          const float4 vs = *reinterpret_cast<const float4*>(smem + G::scales + su * 32 + 16);
+          float value_scale[4] = {vs.x, vs.y, vs.z, vs.w};
           float factor[4] = {score_factor(ks.x, q_factor), score_factor(ks.y, q_factor), score_factor(ks.z, q_factor), score_factor(ks.w, q_factor)};
           tc::tmem_ld_wait<64>(r);
           const int key0 = it.key0 + t * kKeys;
@@ -797,8 +785,12 @@ __global__ void __launch_bounds__((Tall8<HD, kHalf>::threads), (Tall8<HD, kHalf>
             for (int n = 0; n < 64; ++n)
               r[n] = (uint32_t)(n < 32 ? seen : seen >> 32) >> (n & 31) & 1u ? r[n] : 0xff800000u;  // -inf
 #pragma unroll
-            for (int g = 0; g < 4; ++g) factor[g] = (uint32_t)(seen >> 16 * g) & 0xffffu ? factor[g] : 1.f;   // (a scale that the row does not see)
+            for (int g = 0; g < 4; ++g) {   // (scales that the row does not see)
+              factor[g] = (uint32_t)(seen >> 16 * g) & 0xffffu ? factor[g] : 1.f;
+              value_scale[g] = (uint32_t)(seen >> 16 * g) & 0xffffu ? value_scale[g] : 0.f;
+            }
           }
+          const float top_scale = max3(fmaxf(value_scale[0], value_scale[1]), value_scale[2], value_scale[3]);
           float total;
           // (One copy of the code for a step's first look and its second: the instruction caches are small.)
           bool move = t == 0;
@@ -806,10 +798,11 @@ __global__ void __launch_bounds__((Tall8<HD, kHalf>::threads), (Tall8<HD, kHalf>
           for (bool again = false;; again = true) {
             bool outgrown = true;
             if (!move) {
-              total = exponentials8(r, factor, ref == -INFINITY ? 0.f : -ref, s_tmem);
+              const float weight[4] = {value_scale[0] * inverse, value_scale[1] * inverse, value_scale[2] * inverse, value_scale[3] * inverse};
+              total = exponentials8(r, factor, ref == -INFINITY ? 0.f : -ref, weight, s_tmem);
               if (again) break;
               outgrown = !(total <= kMostSum) || ref == -INFINITY;
-              if (!__any_sync(0xffffffffu, outgrown) && !(most > power_of_two(unit_e) && unit_e < 126)) break;
+              if (!__any_sync(0xffffffffu, outgrown || top_scale > unit)) break;
             }
             move = false;
             float mx[4];
@@ -821,12 +814,13 @@ __global__ void __launch_bounds__((Tall8<HD, kHalf>::threads), (Tall8<HD, kHalf>
               mx[g] *= factor[g];
             }
             const float to = outgrown ? fmaxf(ref, max3(fmaxf(mx[0], mx[1]), mx[2], mx[3]) - kGainP) : ref;
-            const int e = max(unit_e, unit_exponent(most));
+            const float to_unit = fmaxf(unit, top_scale);
             const float alpha = to == -INFINITY ? 1.f : ex2f(ref - to);
-            const float both = alpha * ex2f((float)(unit_e - e));
+            asm("rcp.approx.f32 %0, %1;" : "=f"(inverse) : "f"(to_unit));
+            const float both = alpha * (unit * inverse);
             ref = to;
             l *= alpha;
-            unit_e = e;
+            unit = to_unit;
             if (t > 0) {   // (PV of what P holds already is complete first)
               ok &= piece_wait(&bars[G::pv_done + (b ^ 1)], ((count - 1) >> 1) & 1, abort_flag);
               tc::fence_after_sync();
@@ -875,7 +869,7 @@ __global__ void __launch_bounds__((Tall8<HD, kHalf>::threads), (Tall8<HD, kHalf>
           }
         };
         if (!padding) {
-          const float unit = power_of_two(unit_e), factor = whole ? (l == 0.f ? 0.f : unit / l) : unit;
+          const float factor = whole ? (l == 0.f ? 0.f : unit / l) : unit;
           float* const slot = tall8_slot<HD, kHalf>(p, (int)blockIdx.x, it.begins) + row;
           const bool nan = it.edges != 0 && *noted != 0u;   // (the same in all threads)
           uint32_t columns[HD / 16];
