@@ -12,11 +12,12 @@
 // 2^-(14 + 4 n) of it below.  bf16 queries take two (they are exact), fp16 queries three.  Y is rounded to fp16, which three digits
 // hold: 2^-11 of a weight is an eighth of the rounding of a bf16 output, and a key of 2^-24 of its row's largest weight still
 // counts, over 131,072 keys.  At eight rows and 16 or 32 columns they cost the tensor core nothing that shows.
-//   u is a power of two per row for Q (its largest into [128, 256)).  For Y it is U, the largest scale_V so far in the piece, to the
-// next power of two: the accumulators are rescaled where a tile brings a larger one.  scale_K multiplies a key's scores.
+//   u is a power of two per row for Q (its largest into [128, 256)).  U is the power of two above the largest scale_V of a piece's first tile.
+// scale_K multiplies a key's scores.
 //
-// Softmax in one pass: ref is a running bound of a row's scores (log2 units), P = 2^(s - ref), l = sum P.  ref is a row's
-// maximum less kGain when it is set, and moves (with l and O rescaled) only when a score outgrows it by kSlack: P is at most 2^8.
+// Softmax in one pass: P = 2^(s - ref), l = sum P, and ref (log2 units) is a running bound of a row's s + log2(scale_V / U), over the keys that the row sees: it is
+// their maximum less kGainY when it is set, and moves (with l and O rescaled) only when one outgrows it by kSlackY.  So Y is at most 2^8,
+// whatever the scales, and a row's weights have their bits whatever the scales of keys that it does not see.
 //
 // What bounds it: the cache's bytes, 2 D per key and KV head.  The tile's parts (128 keys x 128 dims of K, of V) are units of one
 // ring of shared memory, K of the next tile ahead of V of this one (the other way round, the four tokens below took 136 us
@@ -301,6 +302,20 @@ __device__ __forceinline__ void stage_queries(const Kv8Params& p, const Piece& i
       if (chunk == 0) factor[n] = fmaxf(power_of_two(e) * p.scale_log2, 1e-37f);   // (never zero: hidden scores are -inf)
     }
   }
+}
+
+// The exponent of the power of two at or above the largest of a tile's eight scales.  Scales of 2^-126, which are those of values that are all zero, do
+// not count; where there is no other, the exponent is one that scales of ordinary values are near.
+__device__ __forceinline__ int unit_exponent(const float* scales) {
+  float most = 0.f;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) most = fmaxf(most, scales[i]);
+  return most > 0x1p-126f ? min(126, (int)((__float_as_uint(most) + 0x7fffffu) >> 23) - 127) : -7;
+}
+__device__ __forceinline__ float log2_approx(float x) {
+  float y;
+  asm("lg2.approx.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
 }
 
 // Rows of several tokens: keys that some of them see and others do not, [.., lo) and [hi, ..).
@@ -640,7 +655,7 @@ __global__ void __launch_bounds__((Geo8<HD, RP, kHalf>::threads), (Geo8<HD, RP, 
           group_sync();
         }
         float ref[RW], l[RW];
-        int unit_e = -126;   // U = 2^unit_e
+        int unit_e = 0;   // U = 2^unit_e
 #pragma unroll
         for (int n = 0; n < RW; ++n) {
           ref[n] = kUnset;
@@ -654,9 +669,9 @@ __global__ void __launch_bounds__((Geo8<HD, RP, kHalf>::threads), (Geo8<HD, RP, 
           for (int g = 0; g < G::q_digits; ++g) tmem_load<RW>(tmem_base + G::s_col + (tile & 1) * G::cols + g * RP + row_base + lane_addr, sr[g]);
           const float* const scale = reinterpret_cast<const float*>(smem + G::scales + (tile % kScaleTiles) * 64);
           const float k_scale = scale[key / kRun], v_scale = scale[8 + key / kRun];
-          float most = 0.f;
-#pragma unroll
-          for (int i = 0; i < 8; ++i) most = fmaxf(most, fabsf(scale[8 + i]));
+          if (t == 0) unit_e = unit_exponent(scale + 8);
+          // (a scale far below U, or zero: its keys' P are 2^90 at most)
+          const float value_lg = fmaxf(log2_approx(v_scale) - (float)unit_e, -90.f);
           tc::tmem_ld_wait();
 #pragma unroll
           for (int g = 0; g < G::q_digits; ++g) tc::tmem_landed<RW>(sr[g]);
@@ -683,21 +698,16 @@ __global__ void __launch_bounds__((Geo8<HD, RP, kHalf>::threads), (Geo8<HD, RP, 
             x[n] = fmaf(s[n], factor[n], -ref[n]);
             top = fmaxf(top, x[n]);
           }
-          const bool outgrown = top > kGainY + kSlackY;   // (also where a ref is not set yet)
-          const int e = min(126, max(-126, (int)((__float_as_uint(most) + 0x7fffffu) >> 23) - 127));   // 2^e >= most
-          const bool larger = e > unit_e;   // (the same in all threads)
-          if (group_any(wg, outgrown || larger)) {
+          const bool outgrown = top + value_lg > kGainY + kSlackY;   // (also where a ref is not set yet)
+          if (group_any(wg, outgrown)) {
 #pragma unroll
             for (int n = 0; n < RW; ++n) {
-              const float m = redux_max(s[n] * factor[n]);
+              const float m = redux_max(fmaf(s[n], factor[n], value_lg));
               if (lane == 0) wmax[(warp & 3) * RW + n] = m;
             }
             group_sync();
-            const int unit_to = max(unit_e, e);
-            const float shrink = kv16_exp2((float)(unit_e - unit_to));
-            unit_e = unit_to;
             float alpha[RW];
-            bool moved = shrink != 1.f;
+            bool moved = false;
 #pragma unroll
             for (int n = 0; n < RW; ++n) {
               const float m = fmaxf(fmaxf(wmax[n], wmax[RW + n]), fmaxf(wmax[2 * RW + n], wmax[3 * RW + n])) - kGainY;
@@ -718,7 +728,7 @@ __global__ void __launch_bounds__((Geo8<HD, RP, kHalf>::threads), (Geo8<HD, RP, 
                 tmem_load<RW>(addr, o);
                 tc::tmem_ld_wait<RW>(o);
 #pragma unroll
-                for (int n = 0; n < RW; ++n) o[n] = __float_as_uint(__uint_as_float(o[n]) * (alpha[n] * shrink));
+                for (int n = 0; n < RW; ++n) o[n] = __float_as_uint(__uint_as_float(o[n]) * alpha[n]);
                 tmem_store<RW>(addr, o);
               }
               tc::tmem_st_wait();

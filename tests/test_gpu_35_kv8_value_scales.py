@@ -54,3 +54,55 @@ def test_prompts_with_a_larger_scale_under_keys_that_some_tokens_do_not_see(Hq, 
     if dtype == BF16 or up <= 2.0 ** 16:   # (fp16 has no larger results)
         want = b.reference()
         check(b.out[seen], b.lse[seen], tuple(x[seen] for x in want))
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16])
+@pytest.mark.parametrize("Hq,Hkv,D,q", [(8, 2, 128, 4), (8, 2, 128, 2), (8, 2, 128, 8), (8, 8, 64, 4), (12, 2, 256, 4)])
+@pytest.mark.parametrize("up", [2.0 ** 10, 2.0 ** 16, 2.0 ** 30, 2.0 ** 60])
+def test_few_tokens_with_a_larger_scale_under_keys_that_some_do_not_see(Hq, Hkv, D, q, dtype, up):
+    """A block that begins with the last token but one: those in front of it are as exact as without it."""
+    kv = [1026, 258, 5010, 18, 130]
+    b = Batch(kv, [q] * len(kv), Hq, Hkv, D, dtype, seed=D + q)
+    clean = b.reference()
+    seen = torch.zeros(b.out.shape[0], dtype=torch.bool, device="cuda")
+    for r, n in enumerate(kv):
+        first = n - 2
+        b.vs[int(b.table[r, first // b.page]), first % b.page // 16] *= up * (1.0 if dtype == BF16 else 2.0 ** -6)
+        seen[b.starts[r + 1] - 2:b.starts[r + 1]] = True
+    b.attend()
+    torch.cuda.synchronize()
+    assert capi.load_library().device_status() == 0
+    check(b.out[~seen], b.lse[~seen], tuple(x[~seen] for x in clean))
+    if dtype == BF16 or up <= 2.0 ** 16:
+        want = b.reference()
+        check(b.out[seen], b.lse[seen], tuple(x[seen] for x in want))
+
+
+@pytest.mark.parametrize("first", [0.0, 2.0 ** -126, 2.0 ** -60, 2.0 ** 60])
+def test_scales_of_the_first_keys_far_from_the_others(first):
+    """A whole tile of values of no size, or of a size of their own, in front of the others."""
+    for q in (1, 4, 100):
+        b = Batch([1000, 140, 300], [q] * 3, 8, 2, 128, seed=5)
+        for r in range(3):
+            blocks = b.bt[r, :4].long()   # (128 keys)
+            b.vs[blocks] = first
+            if first <= 2.0 ** -126:
+                b.v[blocks] = 0.0
+        (b.decode() if q == 1 else b.attend()).check()
+
+
+@pytest.mark.parametrize("q", [1, 4])
+def test_a_row_whose_weight_lies_under_small_scales(q):
+    """Scales of 2^-24 of the others', under the keys that have nearly all of the weight: bits of their own."""
+    b = Batch([900], [q], 8, 2, 128, seed=6, scales=(-7, -6))
+    at = torch.arange(600, 616, device="cuda")
+    where = b.bt[0].long()[at // b.page], at % b.page
+    b.q[...] = b.q.abs()
+    b.k[where] = torch.full((16, 2, 128), 448.0, device="cuda").to(E4M3)   # scores far above the others'
+    b.vs[b.bt[0, 600 // b.page].long(), 600 % b.page // 16] *= 2.0 ** -24
+    want = b.reference()
+    (b.decode() if q == 1 else b.attend())
+    torch.cuda.synchronize()
+    # what the other keys weigh is less than 2^-60 of it, so nothing but 16 weights of 2^-11 each and the result is rounded
+    spread = torch.einsum("jhd->hd", b.v[where].double().abs()).repeat_interleave(4, 0) * 2.0 ** -31 / 16
+    assert bool(((b.out.double() - want[0]).abs() <= 2.0 ** -8 * want[0].abs() + 2.0 ** -10 * 16 * spread).all())
