@@ -6,9 +6,11 @@
 // quotients and the re-rounding exact up to the one rounding.
 //
 // Blocks up to 32 tokens are a warp's work: its rows of 16 bytes a lane stay in registers between the maximum and the rounding.
-// Larger ones are a CTA's, which reads the rows again (from L2) for the rounding.  Bytes bound it: T Hkv D (source + 1) x 2.
-// 4 x 2,048 bf16 tokens of 8 heads, 128 dims: 13.4 us one call behind another, 7.7 of them bytes at the copy bandwidth; the others are the
-// launch and a unit's dependent look-ups (offsets, block table, scale).  64 tokens: 3.4 us on the device, less than the host takes.
+// Larger ones are a CTA's, which reads the rows again (from L2) for the rounding; but where a request has one token at most, a warp's too, whose CTA rounds
+// more than 32 older rows again for it (with a CTA for each, 64 requests that have nothing to round again took 10.8 us instead of 3.7; with the
+// warp alone, 815 older rows of 128 dims 94 us instead of 20, of 256 dims 166 instead of 35).  Bytes bound it: T Hkv D (source + 1) x 2.
+// 4 x 2,048 bf16 tokens of 8 heads, 128 dims: 11.3 to 13.1 us one call behind another, 7.7 of them bytes at the copy bandwidth; the others are the
+// launch and a unit's dependent look-ups (offsets, block table, scale).  64 tokens: 3.2 us on the device, less than the host takes.
 //
 // Units find their block without a list: request r's blocks are numbered from start_r / g + 2 r on, which leaves room for the two
 // more blocks than q / g that its tokens may touch (r itself where a request has one token at most).  Numbers that no block has
@@ -21,6 +23,7 @@ namespace pthb200 {
 namespace {
 
 constexpr int kWarps = 8;
+constexpr int kMostOlder = 32;   // older rows that a warp rounds again by itself
 
 struct Write8Params {
   const uint8_t* src[2];
@@ -160,19 +163,40 @@ __device__ __forceinline__ bool find_block(const Write8Params& p, int x, Block* 
   return true;
 }
 
+// Rounds `rows` older rows again, of which these threads take every step-th from `first` on, kOlder of them in flight.
+template <int kOlder>
+__device__ __forceinline__ void round_again(uint8_t* cells, int64_t stride, int rows, int first, int step, float ratio) {
+#pragma unroll 1
+  for (int n0 = first; n0 < rows; n0 += kOlder * step) {
+    uint2 w[kOlder];
+#pragma unroll
+    for (int i = 0; i < kOlder; ++i)
+      if (n0 + i * step < rows) w[i] = *reinterpret_cast<const uint2*>(cells + (int64_t)(n0 + i * step) * stride);
+#pragma unroll
+    for (int i = 0; i < kOlder; ++i)
+      if (n0 + i * step < rows) *reinterpret_cast<uint2*>(cells + (int64_t)(n0 + i * step) * stride) = make_uint2(rescaled(w[i].x, ratio), rescaled(w[i].y, ratio));
+  }
+}
+// Older rows that are left to the whole CTA.
+struct Older {
+  uint8_t* cells;
+  int64_t stride;
+  int rows;
+  float ratio;
+};
+
+// A unit of work, by a warp or a CTA.  A warp leaves more than kMostOlder older rows to its CTA.
 // kKept: pieces of eight elements that a lane keeps, as many as 16 rows of a warp.
 template <int HD, int kDtype, bool kWide, bool kCta>
-__global__ void __launch_bounds__(kWarps * 32, kDtype != PTH_ATTN_F32 && HD < 256 && !kCta ? 4 : 1) kv8_writer_kernel(const __grid_constant__ Write8Params p) {
+__device__ __forceinline__ void write_unit(const Write8Params& p, float* most_of, Older* older) {
   constexpr int kLanes = HD / 8, kAtOnce = 32 / kLanes;      // lanes of a row, rows of a warp at a time
   constexpr int kKept = kDtype == PTH_ATTN_F32 || HD == 256 ? 8 : 16 / kAtOnce;
-  __shared__ float most_of[kWarps];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int chunk = lane % kLanes, sub = lane / kLanes;
   // units: (block number, head, K or V), the last fastest
   const int per = 2 * p.num_kv_heads;
   const int64_t unit = kCta ? (int64_t)blockIdx.x : (int64_t)blockIdx.x * kWarps + warp;
   const int x = (int)(unit / per), rest = (int)(unit - (int64_t)x * per), head = rest >> 1, v = rest & 1;
-  pdl_wait();
   Block b;
   if (!find_block(p, x, &b)) return;
   const uint8_t* const src = p.src[v] + (int64_t)b.row0 * p.src_stride_token[v] + (int64_t)head * p.src_stride_head[v];
@@ -207,12 +231,8 @@ __global__ void __launch_bounds__(kWarps * 32, kDtype != PTH_ATTN_F32 && HD < 25
   // the cells in front of the new ones
   if (b.begin > 0 && scale > was) {
     const float ratio = was / scale;
-#pragma unroll 1
-    for (int n = mine; n < b.begin; n += kStep) {
-      uint2* const at = reinterpret_cast<uint2*>(cells + (int64_t)n * p.stride_slot[v]);
-      const uint2 w = *at;
-      *at = make_uint2(rescaled(w.x, ratio), rescaled(w.y, ratio));
-    }
+    if (kCta || b.begin <= kMostOlder) round_again<4>(cells, p.stride_slot[v], b.begin, mine, kStep, ratio);
+    else if (lane == 0) *older = Older{cells, p.stride_slot[v], b.begin, ratio};
   }
   const float up = (__float_as_uint(scale) & 0x7fffffu) == 0 ? power_of_two(127 - (int)(__float_as_uint(scale) >> 23)) : 0.f;
   const bool once = b.rows <= kKept * kStep;   // (the rows are in registers still)
@@ -232,11 +252,30 @@ __global__ void __launch_bounds__(kWarps * 32, kDtype != PTH_ATTN_F32 && HD < 25
   if (lane == 0 && (!kCta || warp == 0) && scale != was) *scale_at = scale;
 }
 
+template <int HD, int kDtype, bool kWide, bool kCta>
+__global__ void __launch_bounds__(kWarps * 32, kDtype != PTH_ATTN_F32 && HD < 256 && !kCta ? 4 : 1) kv8_writer_kernel(const __grid_constant__ Write8Params p) {
+  __shared__ float most_of[kWarps];
+  __shared__ Older older[kWarps];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  if (lane == 0) older[warp].rows = 0;
+  __syncwarp();
+  pdl_wait();
+  write_unit<HD, kDtype, kWide, kCta>(p, most_of, &older[warp]);
+  if constexpr (!kCta) {
+    if (p.scale_tokens <= kMostOlder) return;
+    __syncthreads();
+    constexpr int kLanes = HD / 8, kAtOnce = 32 / kLanes;
+#pragma unroll 1
+    for (int w = 0; w < kWarps; ++w)   // (cells: from the first lane's on)
+      if (older[w].rows > 0) round_again<8>(older[w].cells + lane % kLanes * 8, older[w].stride, older[w].rows, warp * kAtOnce + lane / kLanes, kWarps * kAtOnce, older[w].ratio);
+  }
+}
+
 template <int HD, int kDtype>
 cudaError_t launch_for(const Write8Params& p, bool wide, cudaStream_t stream) {
   const int64_t numbers = p.max_query_len == 1 ? p.num_reqs : (int64_t)(p.num_tokens / p.scale_tokens) + 2ll * p.num_reqs;
   const int64_t units = numbers * 2 * p.num_kv_heads;
-  const bool cta = p.scale_tokens > 32 && p.max_query_len > 1;
+  const bool cta = p.scale_tokens > kMostOlder && p.max_query_len > 1;
   const int64_t ctas = cta ? units : (units + kWarps - 1) / kWarps;
   if (numbers > 0x7fffffff || ctas > 0x7fffffff) return cudaErrorInvalidConfiguration;
   const dim3 grid((unsigned)ctas), block(kWarps * 32);
