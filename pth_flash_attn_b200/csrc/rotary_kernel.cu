@@ -2,8 +2,8 @@
 // k are read and written once.
 //
 // The angle is a product in 64 bits, taken to [-pi, pi] there (a position of 10^6 has 20 bits in front of the point, which 32 bits
-// would take from the angle), and its sine and cosine have 32 bits.  A CTA works them out once for a few tokens and all their heads, in
-// shared memory.
+// would take from the angle), and its sine and cosine have 32 bits, near their zeros too: they are those of the angle's rounding to 32 bits, corrected by what
+// that left.  A CTA works them out once for a few tokens and all their heads, in shared memory.
 //
 // A thread turns kVec pairs of a head: vectors of 16 bytes where the rows' places allow it, kBatch of them in flight, else pair by pair.
 // Both of a pair are read before either is written, so a tensor may be turned in place.  8,192 tokens of 32 + 8 heads, 128 dims, bf16, 0.17 GB:
@@ -85,9 +85,11 @@ __device__ __forceinline__ float2 turn_of(const RotaryParams& p, long long posit
   const double a = (double)position * f;
   // less the nearest multiple of 2 pi (in two parts: the quotient has up to 31 bits)
   const double turns = rint(a * 0.15915494309189533577);
-  const float r = (float)fma(-turns, 2.4492935982947064e-16, fma(-turns, 6.28318530717958623, a));
-  float s, c;
-  sincosf(r, &s, &c);
+  const double r = fma(-turns, 2.4492935982947064e-16, fma(-turns, 6.28318530717958623, a));
+  const float near = (float)r, rest = (float)(r - (double)near);
+  float sn, cn;
+  sincosf(near, &sn, &cn);
+  const float s = fmaf(rest, cn, sn), c = fmaf(-rest, sn, cn);
   return make_float2(c * p.scale, (p.inverse ? -s : s) * p.scale);
 }
 
