@@ -6,6 +6,7 @@
 // the copy bandwidth.
 #include "kv8.cuh"
 
+#include "page_copy.cuh"
 #include "pdl.cuh"
 
 namespace pthb200 {
@@ -139,7 +140,7 @@ __global__ void __launch_bounds__(kThreads) kv8_reader_kernel(const __grid_const
 template <int HD, int kDtype>
 cudaError_t launch_for(const Read8Params& p, cudaStream_t stream) {
   // rows of a CTA: four where there are too few to give every SM several CTAs of sixteen
-  const int rows = p.num_rows >= 16 * 148 * 4 ? 16 : 4;
+  const int rows = p.num_rows >= 16 * sm_count() * 4 ? 16 : 4;
   const dim3 grid((unsigned)((p.num_rows + rows - 1) / rows));
   return pdl_launch(rows == 16 ? kv8_reader_kernel<HD, kDtype, 16> : kv8_reader_kernel<HD, kDtype, 4>, grid, kThreads, 0, stream, p);
 }

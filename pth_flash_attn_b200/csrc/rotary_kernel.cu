@@ -5,17 +5,18 @@
 // would take from the angle), and its sine and cosine have 32 bits, near their zeros too: they are those of the angle's rounding to 32 bits, corrected by what
 // that left.  A CTA works them out once for a few tokens and all their heads, in shared memory.
 //
-// A thread turns kVec pairs of a head: vectors of 16 bytes where the rows' places allow it, kBatch of them in flight, else pair by pair.
+// A thread turns the pairs of two vectors of 16 bytes at a time where the rows' places allow it, else pair by pair.
 // Both of a pair are read before either is written, so a tensor may be turned in place.  8,192 tokens of 32 + 8 heads, 128 dims, bf16, 0.17 GB:
-// 33 us, 0.78 of the copy bandwidth.
+// 33 to 36 us, 0.72 to 0.78 of the copy bandwidth.
 #include "kv8.cuh"
 
+#include "page_copy.cuh"
 #include "pdl.cuh"
 
 namespace pthb200 {
 namespace {
 
-constexpr int kThreads = 256, kBatch = 1;
+constexpr int kThreads = 256;
 
 struct RotaryParams {
   const uint8_t* src[2];
@@ -140,42 +141,27 @@ __global__ void __launch_bounds__(kThreads) rotary_kernel(const __grid_constant_
   if constexpr (kVector) {
     const int step = half / kVec;
 #pragma unroll 1
-    for (uint32_t x0 = threadIdx.x; x0 < pieces; x0 += kBatch * kThreads) {
-      Vec<kDtype> a[kBatch], b[kBatch];
-      const float2* t[kBatch];
-      uint8_t* to_a[kBatch];
-      uint8_t* to_b[kBatch];   // nullptr: a copied piece
+    for (uint32_t x = threadIdx.x; x < pieces; x += kThreads) {
+      const At at(p, token0, x);
+      const int2 to = at.halves(p);
+      Vec<kDtype> a, b;
+      a.load(at.src + to.x);
+      b.load(at.src + to.y);   // (a copied piece twice)
+      if (at.i < at.turning) {
+        const float2* const t = turns + at.token * half + at.i;
+        if constexpr (kInterleaved) {
 #pragma unroll
-      for (int k = 0; k < kBatch; ++k) {
-        const uint32_t x = x0 + k * kThreads;
-        to_a[k] = nullptr;
-        if (x >= pieces) continue;
-        const At at(p, token0, x);
-        const int2 to = at.halves(p);
-        a[k].load(at.src + to.x);
-        b[k].load(at.src + to.y);
-        t[k] = turns + at.token * half + at.i;
-        to_a[k] = at.dst + to.x;
-        to_b[k] = at.i < at.turning ? at.dst + to.y : nullptr;
-      }
-#pragma unroll
-      for (int k = 0; k < kBatch; ++k) {
-        if (to_a[k] == nullptr) continue;
-        if (to_b[k] != nullptr) {
-          if constexpr (kInterleaved) {
-#pragma unroll
-            for (int e = 0; e < kVec / 2; ++e) {
-              a[k].turn(2 * e, a[k], 2 * e + 1, t[k][e * step]);
-              b[k].turn(2 * e, b[k], 2 * e + 1, t[k][(kVec / 2 + e) * step]);
-            }
-          } else {
-#pragma unroll
-            for (int e = 0; e < kVec; ++e) a[k].turn(e, b[k], e, t[k][e * step]);
+          for (int e = 0; e < kVec / 2; ++e) {
+            a.turn(2 * e, a, 2 * e + 1, t[e * step]);
+            b.turn(2 * e, b, 2 * e + 1, t[(kVec / 2 + e) * step]);
           }
-          b[k].store(to_b[k]);
+        } else {
+#pragma unroll
+          for (int e = 0; e < kVec; ++e) a.turn(e, b, e, t[e * step]);
         }
-        a[k].store(to_a[k]);
+        b.store(at.dst + to.y);
       }
+      a.store(at.dst + to.x);
     }
   } else {
 #pragma unroll 1
@@ -197,7 +183,7 @@ __global__ void __launch_bounds__(kThreads) rotary_kernel(const __grid_constant_
 template <int kDtype>
 cudaError_t launch_for(const RotaryParams& p, bool interleaved, bool vector, cudaStream_t stream) {
   // tokens of a CTA: one where there are too few to give every SM several CTAs of four
-  const int per_cta = p.num_tokens >= 4 * 148 * 4 ? 4 : 1;
+  const int per_cta = p.num_tokens >= 4 * sm_count() * 4 ? 4 : 1;
   const dim3 grid((unsigned)((p.num_tokens + per_cta - 1) / per_cta));
   const size_t smem = (size_t)per_cta * p.half * sizeof(float2);
   if (interleaved) return pdl_launch(vector ? rotary_kernel<kDtype, true, true> : rotary_kernel<kDtype, true, false>, grid, kThreads, smem, stream, p, per_cta);
