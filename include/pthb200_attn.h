@@ -548,6 +548,11 @@ int32_t pthb200_kv8_args_bytes(void);
 int64_t pthb200_kv8_workspace_bytes(int32_t head_size, int32_t num_sms);
 int32_t pthb200_kv8_decode(const PthB200Kv8Args* args, void* stream);
 int32_t pthb200_kv8_attend(const PthB200Kv8Args* args, void* stream);
+/* Test only: the call of that form (decode: query_start_loc is NULL), in which a warp of CTA 0 stops short, so that the CTA's waits
+ * run out (a few seconds at most), it leaves and pthb200_device_status says so: role 1 the scheduling warp after `after` pieces,
+ * 2 a copying warp after as many units or steps, 3 an MMA warp after as many steps.  128 dims, bf16, at most 8 rows or more than 32.
+ * The results are void; zero the workspace behind it. */
+int32_t pthb200_test_kv8_held(const PthB200Kv8Args* args, int32_t role, int32_t after, void* stream);
 /* Validates as the calls above do, without launching (decode: query_start_loc is NULL). */
 int32_t pthb200_kv8_check(const PthB200Kv8Args* args);
 

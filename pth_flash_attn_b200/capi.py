@@ -383,6 +383,7 @@ EXPORTED_SYMBOLS = (
     "pthb200_kv8_decode",
     "pthb200_kv8_attend",
     "pthb200_kv8_check",
+    "pthb200_test_kv8_held",
     "pthb200_rotary_args_bytes",
     "pthb200_rotary",
     "pthb200_tile_tokens",
@@ -465,6 +466,8 @@ class B200Lib:
         lib.pthb200_test_kv16_held.argtypes = [ctypes.POINTER(PthB200Kv16Args), ctypes.c_int32, ctypes.c_int32, ctypes.c_void_p]
         lib.pthb200_kv16_check.restype = ctypes.c_int32
         lib.pthb200_kv16_check.argtypes = [ctypes.POINTER(PthB200Kv16Args)]
+        lib.pthb200_test_kv8_held.restype = ctypes.c_int32
+        lib.pthb200_test_kv8_held.argtypes = [ctypes.POINTER(PthB200Kv8Args), ctypes.c_int32, ctypes.c_int32, ctypes.c_void_p]
         lib.pthb200_kv8_check.restype = ctypes.c_int32
         lib.pthb200_kv8_check.argtypes = [ctypes.POINTER(PthB200Kv8Args)]
         for fn in (lib.pthb200_test_schedule, lib.pthb200_test_range_schedule):
@@ -576,6 +579,10 @@ class B200Lib:
     def kv8_attend(self, args: PthB200Kv8Args, *, stream: int = 0) -> int:
         """Attention of every request's new tokens over the 8-bit cache."""
         return int(self.lib.pthb200_kv8_attend(ctypes.byref(args), stream or None))
+
+    def test_kv8_held(self, args: PthB200Kv8Args, role: int, after: int, *, stream: int = 0) -> int:
+        """Test only: a call one of whose warps stops short."""
+        return int(self.lib.pthb200_test_kv8_held(ctypes.byref(args), role, after, stream or None))
 
     def kv8_check(self, args: PthB200Kv8Args) -> int:
         """The checks of the two calls above, without a launch."""

@@ -123,9 +123,11 @@ __device__ __forceinline__ void place_piece(Piece* out, const ReqShape8& s) { ou
 // kv8_short_kernel.cu
 int64_t kv8_short_workspace_bytes(int head_size, int num_sms);
 cudaError_t launch_kv8_short(const Kv8Params& p, cudaStream_t stream);
+cudaError_t launch_kv8_short_held(const Kv8Params& p, cudaStream_t stream);   // 128 dims, bf16, at most 8 rows
 // kv8_tall_kernel.cu.  *taken: whether the cache's view can be read by TMA boxes; if not, nothing has been launched.
 int64_t kv8_tall_workspace_bytes(int head_size, int num_sms);
 cudaError_t launch_kv8_tall(const Kv8Params& p, cudaStream_t stream, bool* taken);
+cudaError_t launch_kv8_tall_held(const Kv8Params& p, cudaStream_t stream);    // 128 dims, bf16
 // kv8_writer_kernel.cu, kv8_reader_kernel.cu, rotary_kernel.cu
 cudaError_t launch_kv8_writer(const PthB200Kv8WriteArgs& a, cudaStream_t stream);
 cudaError_t launch_kv8_reader(const PthB200Kv8ReadArgs& a, cudaStream_t stream);

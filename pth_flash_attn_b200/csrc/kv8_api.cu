@@ -157,7 +157,7 @@ int64_t workspace_bytes(int head_size, int num_sms) {
   return std::max(kv8_short_workspace_bytes(head_size, num_sms), kv8_tall_workspace_bytes(head_size, num_sms));
 }
 
-int32_t attention(const PthB200Kv8Args* a, bool decode, void* stream) {
+int32_t attention(const PthB200Kv8Args* a, bool decode, void* stream, Kv16Held held = kHeldNone, int32_t held_after = 0) {
   clear_error();
   Kv8Params p;
   if (int32_t rc = build(a, decode, &p)) return rc;
@@ -167,7 +167,15 @@ int32_t attention(const PthB200Kv8Args* a, bool decode, void* stream) {
     return set_error(PTH_ATTN_ECUDA, "cannot query the current device");
   const int64_t need = workspace_bytes(a->head_size, sms);
   KV8_REQUIRE(a->workspace_bytes >= need, "workspace has " + std::to_string(a->workspace_bytes) + " bytes, " + std::to_string(need) + " are needed");
-  if ((int64_t)p.max_query_len * p.group >= tall_rows(a->head_size) && p.max_query_len > 1) {
+  const bool tall = (int64_t)p.max_query_len * p.group >= tall_rows(a->head_size) && p.max_query_len > 1;
+  if (held != kHeldNone) {
+    KV8_REQUIRE(a->head_size == 128 && a->dtype == PTH_ATTN_BF16 && (tall || (int64_t)p.max_query_len * p.group <= 8),
+                "the test's instances take 128 dims, bf16, and at most 8 rows or more than 32");
+    p.held_role = held;
+    p.held_after = held_after;
+    return launched((tall ? launch_kv8_tall_held : launch_kv8_short_held)(p, static_cast<cudaStream_t>(stream)), "attention");
+  }
+  if (tall) {
     bool taken = false;
     const int32_t rc = launched(launch_kv8_tall(p, static_cast<cudaStream_t>(stream), &taken), "attention");
     if (rc != PTH_ATTN_OK || taken) return rc;
@@ -226,6 +234,13 @@ int32_t pthb200_kv8_check(const PthB200Kv8Args* a) {
 }
 int32_t pthb200_kv8_decode(const PthB200Kv8Args* a, void* stream) { return pthb200::attention(a, true, stream); }
 int32_t pthb200_kv8_attend(const PthB200Kv8Args* a, void* stream) { return pthb200::attention(a, false, stream); }
+int32_t pthb200_test_kv8_held(const PthB200Kv8Args* a, int32_t role, int32_t after, void* stream) {
+  using namespace pthb200;
+  clear_error();
+  KV8_REQUIRE(a != nullptr, "args is NULL");
+  KV8_REQUIRE(role >= kHeldSchedule && role <= kHeldMma && after >= 0, "role must be in [1, 3], after >= 0");
+  return attention(a, a->query_start_loc == nullptr, stream, static_cast<Kv16Held>(role), after);
+}
 
 int32_t pthb200_rotary(const PthB200RotaryArgs* a, void* stream) {
   using namespace pthb200;

@@ -363,7 +363,7 @@ __device__ __forceinline__ uint32_t nan_rows(const Kv8Params& p, const Piece& it
   return seen;
 }
 
-template <int HD, int RP, bool kHalf>
+template <int HD, int RP, bool kHalf, bool kHeld>
 __global__ void __launch_bounds__((Geo8<HD, RP, kHalf>::threads), (Geo8<HD, RP, kHalf>::ctas)) kv8_short_kernel(const __grid_constant__ Kv8Params p, const __grid_constant__ CUtensorMap k_map, const __grid_constant__ CUtensorMap v_map) {
   using G = Geo8<HD, RP, kHalf>;
   extern __shared__ uint8_t smem_raw[];
@@ -423,6 +423,7 @@ __global__ void __launch_bounds__((Geo8<HD, RP, kHalf>::threads), (Geo8<HD, RP, 
     uint32_t item = 0;
     bool going = true;
     while (going && walk.next(p, &it)) {
+      if (kv16_held<kHeld>(p, kHeldSchedule, queue.i)) kv16_wait(&bars[Bars8::drained], 0, abort_flag);   // (that nothing arrives on here)
       going = queue.put(it, abort_flag);
       if (!going) break;
       // (behind a wait that gave up the digits may still be read: nothing is written, and the next put ends the queue)
@@ -522,6 +523,7 @@ __global__ void __launch_bounds__((Geo8<HD, RP, kHalf>::threads), (Geo8<HD, RP, 
       TileRuns last;
       uint32_t last_boxes = 0, last_copied = 0;
       while ((have || have_v) && ok) {
+        if (kv16_held<kHeld>(p, kHeldCopies, asked)) break;
         const bool now = have;
         TileRuns here = next;
         uint32_t boxes = 0, copied = 0;
@@ -618,6 +620,7 @@ __global__ void __launch_bounds__((Geo8<HD, RP, kHalf>::threads), (Geo8<HD, RP, 
     while (queue.get(&it, abort_flag)) {
       const Masks masks(p, it);
       for (int t = 0; t < it.tiles; ++t) {
+        if (kv16_held<kHeld>(p, kHeldMma, tile)) break;
         const uint32_t here = item;
         qk(t == 0, t == it.tiles - 1);
         if (pending) pv(pending_first, pending_divided, pending_item);
@@ -867,7 +870,7 @@ __global__ void __launch_bounds__((Geo8<HD, RP, kHalf>::threads), (Geo8<HD, RP, 
   (void)ok;
 }
 
-template <int HD, int RP, bool kHalf>
+template <int HD, int RP, bool kHalf, bool kHeld = false>
 cudaError_t launch_one(const Kv8Params& p, const CUtensorMap& k_map, const CUtensorMap& v_map, cudaStream_t stream) {
   using G = Geo8<HD, RP, kHalf>;
   static_assert(G::total <= 232448, "shared memory of one CTA");
@@ -878,15 +881,15 @@ cudaError_t launch_one(const Kv8Params& p, const CUtensorMap& k_map, const CUten
   if (err != cudaSuccess) return err;
   if (dev < 0 || dev >= 64 || !configured[dev]) {
     cudaFuncAttributes attr;
-    err = cudaFuncGetAttributes(&attr, kv8_short_kernel<HD, RP, kHalf>);
+    err = cudaFuncGetAttributes(&attr, kv8_short_kernel<HD, RP, kHalf, kHeld>);
     if (err == cudaSuccess && G::moves && attr.numRegs < G::start_regs) err = cudaErrorInvalidConfiguration;   // (setmaxnreg would wait without end)
-    if (err == cudaSuccess) err = cudaFuncSetAttribute(kv8_short_kernel<HD, RP, kHalf>, cudaFuncAttributeMaxDynamicSharedMemorySize, G::total);
+    if (err == cudaSuccess) err = cudaFuncSetAttribute(kv8_short_kernel<HD, RP, kHalf, kHeld>, cudaFuncAttributeMaxDynamicSharedMemorySize, G::total);
     if (err != cudaSuccess) return err;
     if (dev >= 0 && dev < 64) configured[dev] = true;
   }
   const int sms = sm_count();
   if (sms <= 0) return cudaErrorInvalidDevice;
-  return pdl_launch(kv8_short_kernel<HD, RP, kHalf>, dim3((unsigned)(sms * G::ctas)), dim3(G::threads), G::total, stream, p, k_map, v_map);
+  return pdl_launch(kv8_short_kernel<HD, RP, kHalf, kHeld>, dim3((unsigned)(sms * G::ctas)), dim3(G::threads), G::total, stream, p, k_map, v_map);
 }
 template <int HD, int RP>
 cudaError_t launch_type(const Kv8Params& p, const CUtensorMap& k_map, const CUtensorMap& v_map, cudaStream_t stream) {
@@ -907,12 +910,24 @@ int64_t kv8_short_workspace_bytes(int head_size, int num_sms) {
   return kCounterBytes + (int64_t)num_sms * 2 * 2 * 16 * (head_size + 2) * 4;
 }
 
-cudaError_t launch_kv8_short(const Kv8Params& p, cudaStream_t stream) {
-  // Boxes of 32 slots where pages are whole numbers of them (a piece's tiles begin at multiples of 32 keys), else of 16.
+namespace {
+// Boxes of 32 slots where pages are whole numbers of them (a piece's tiles begin at multiples of 32 keys), else of 16.
+void make_maps(Kv8Params& q, CUtensorMap* k_map, CUtensorMap* v_map) {
+  q.box_slots = q.head_size == 64 ? 0 : q.block_size % 32 == 0 ? 32 : 16;
+  if (q.box_slots > 0 && (!cell_box_map(q, q.k, q.box_slots, k_map) || !cell_box_map(q, q.v, q.box_slots, v_map))) q.box_slots = 0;
+}
+}  // namespace
+
+cudaError_t launch_kv8_short_held(const Kv8Params& p, cudaStream_t stream) {
   Kv8Params q = p;
-  q.box_slots = p.head_size == 64 ? 0 : p.block_size % 32 == 0 ? 32 : 16;
   CUtensorMap k_map{}, v_map{};
-  if (q.box_slots > 0 && (!cell_box_map(q, p.k, q.box_slots, &k_map) || !cell_box_map(q, p.v, q.box_slots, &v_map))) q.box_slots = 0;
+  make_maps(q, &k_map, &v_map);
+  return launch_one<128, 8, false, true>(q, k_map, v_map, stream);
+}
+cudaError_t launch_kv8_short(const Kv8Params& p, cudaStream_t stream) {
+  Kv8Params q = p;
+  CUtensorMap k_map{}, v_map{};
+  make_maps(q, &k_map, &v_map);
   switch (p.head_size) {
     case 64:
       return launch_rows<64>(q, k_map, v_map, stream);

@@ -237,8 +237,12 @@ __device__ __forceinline__ TallWalk8<RP> find_run8(const Kv8Params& p, long long
 // Steps of a piece: its keys from key0 on, as far as its row tile sees them; one at least.
 __device__ __forceinline__ int steps8(const Piece& it) { return max(1, (min(it.tiles * kTile, it.hi - it.key0) + kKeys - 1) / kKeys); }
 
-// Behind any of a CTA's waits may stand a row tile whose rows are on their way out, merged or not: all have the bound of whole pieces.
-__device__ __forceinline__ bool piece_wait(uint64_t* bar, uint32_t parity, volatile int* abort_flag) { return kv16_wait<kPieceTimes>(bar, parity, abort_flag); }
+// Behind any of a CTA's waits may stand a row tile whose rows are on their way out, merged or not: all have the bound of whole pieces (but
+// in the test's instances, which wait for it to pass).
+template <bool kHeld>
+__device__ __forceinline__ bool piece_wait(uint64_t* bar, uint32_t parity, volatile int* abort_flag) {
+  return kv16_wait<kHeld ? 1u : kPieceTimes>(bar, parity, abort_flag);
+}
 
 // ---- operands ----
 
@@ -421,7 +425,7 @@ __device__ __noinline__ void nan_columns(const Kv8Params& p, const Piece& it, co
   }
 }
 
-template <int HD, bool kHalf>
+template <int HD, bool kHalf, bool kHeld>
 __global__ void __launch_bounds__((Tall8<HD, kHalf>::threads), (Tall8<HD, kHalf>::ctas)) kv8_tall_kernel(const __grid_constant__ Kv8Params p, const __grid_constant__ CUtensorMap k_map,
                                                                         const __grid_constant__ CUtensorMap v_map) {
   using G = Tall8<HD, kHalf>;
@@ -488,6 +492,7 @@ __global__ void __launch_bounds__((Tall8<HD, kHalf>::threads), (Tall8<HD, kHalf>
     bool going = true;
     while (going && walk.next(p, &it)) {
       it.edges = edges8(p, it);
+      if (kv16_held<kHeld>(p, kHeldSchedule, queue.i)) piece_wait<kHeld>(&bars[G::drained], 0, abort_flag);   // (that nothing arrives on here)
       if (lane < G::nan_words) reinterpret_cast<uint32_t*>(smem + G::nan)[queue.i % G::nan_pieces * G::nan_words + lane] = 0u;
       going = queue.put(it, abort_flag);
       if (!going) break;
@@ -505,7 +510,7 @@ __global__ void __launch_bounds__((Tall8<HD, kHalf>::threads), (Tall8<HD, kHalf>
       auto free_units = [&](int first, int units, uint32_t asked_for, int here) {
         for (int i = 0; i < here; ++i) {
           const uint32_t u = asked_for + i;
-          if (u >= (uint32_t)units) ok &= piece_wait(&bars[first + u % units], ((u / units) - 1) & 1, abort_flag);
+          if (u >= (uint32_t)units) ok &= piece_wait<kHeld>(&bars[first + u % units], ((u / units) - 1) & 1, abort_flag);
         }
         ok = __all_sync(0xffffffffu, ok);
         return ok;
@@ -533,6 +538,7 @@ __global__ void __launch_bounds__((Tall8<HD, kHalf>::threads), (Tall8<HD, kHalf>
         };
         const bool live = kind < 2 && mine < here;
         const uint32_t step = asked_v + mine, ku = step % G::k_units, vu = step % G::v_units, su = step % G::scale_steps;
+        if (kv16_held<kHeld>(p, kHeldCopies, asked_k)) ok = false;
         if (!free_units(G::k_empty, G::k_units, asked_k, here)) break;
         if (live) {
           const float* const base = kind == 0 ? p.k_scale : p.v_scale;
@@ -568,8 +574,8 @@ __global__ void __launch_bounds__((Tall8<HD, kHalf>::threads), (Tall8<HD, kHalf>
 #pragma unroll 1
       for (int j = 0; j < n; ++j, ++step) {
         const uint32_t vu = step % G::v_units, wu = step % G::w_units;
-        ok &= piece_wait(&bars[G::v_full + vu], (step / G::v_units) & 1, abort_flag);
-        if (step >= G::w_units) ok &= piece_wait(&bars[G::w_empty + wu], ((step / G::w_units) - 1) & 1, abort_flag);
+        ok &= piece_wait<kHeld>(&bars[G::v_full + vu], (step / G::v_units) & 1, abort_flag);
+        if (step >= G::w_units) ok &= piece_wait<kHeld>(&bars[G::w_empty + wu], ((step / G::w_units) - 1) & 1, abort_flag);
         const uint8_t* const raw = smem + G::v + vu * G::raw;
         uint8_t* const wide = smem + G::w + wu * G::wide;
         const int key0 = it.key0 + j * kKeys;
@@ -643,9 +649,9 @@ __global__ void __launch_bounds__((Tall8<HD, kHalf>::threads), (Tall8<HD, kHalf>
     uint32_t s_qk = 0, s_pv = 0, pieces = 0;   // steps so far, pieces with live rows
     auto qk = [&](bool first) {
       const uint32_t b = s_qk & 1;
-      if (first) ok &= piece_wait(&bars[G::q_full + rt], (pieces - 1) & 1, abort_flag);
-      ok &= piece_wait(&bars[G::k_full + k_slot], k_phase, abort_flag);
-      if (s_qk > 1) ok &= piece_wait(&bars[G::pv_done + 2 * rt + b], ((s_qk >> 1) - 1) & 1, abort_flag);   // (P of the step before last has been read)
+      if (first) ok &= piece_wait<kHeld>(&bars[G::q_full + rt], (pieces - 1) & 1, abort_flag);
+      ok &= piece_wait<kHeld>(&bars[G::k_full + k_slot], k_phase, abort_flag);
+      if (s_qk > 1) ok &= piece_wait<kHeld>(&bars[G::pv_done + 2 * rt + b], ((s_qk >> 1) - 1) & 1, abort_flag);   // (P of the step before last has been read)
       if (!ok) return;
       tc::fence_after_sync();
 #pragma unroll
@@ -669,8 +675,8 @@ __global__ void __launch_bounds__((Tall8<HD, kHalf>::threads), (Tall8<HD, kHalf>
     };
     auto pv = [&](bool first) {
       const uint32_t b = s_pv & 1;
-      ok &= piece_wait(&bars[G::w_full + w_slot], w_phase, abort_flag);
-      ok &= piece_wait(&bars[G::p_ready + 2 * rt + b], (s_pv >> 1) & 1, abort_flag);
+      ok &= piece_wait<kHeld>(&bars[G::w_full + w_slot], w_phase, abort_flag);
+      ok &= piece_wait<kHeld>(&bars[G::p_ready + 2 * rt + b], (s_pv >> 1) & 1, abort_flag);
       if (!ok) return;
       tc::fence_after_sync();
 #pragma unroll
@@ -688,13 +694,14 @@ __global__ void __launch_bounds__((Tall8<HD, kHalf>::threads), (Tall8<HD, kHalf>
     Piece it;
     const bool leader = elect_one();   // (one lane takes all steps of a piece: the others would only have to be waited for)
     while (queue.get(&it, abort_flag)) {
+      if (kv16_held<kHeld>(p, kHeldMma, s_qk)) ok = false;
       if (!leader || !ok) continue;
       const int n = steps8(it);
       if (it.rows <= rt * 128) {   // no rows: free the units as if they had been read
 #pragma unroll 1
         for (int j = 0; j < n; ++j) {
-          ok &= piece_wait(&bars[G::k_full + k_slot], k_phase, abort_flag);
-          ok &= piece_wait(&bars[G::w_full + w_slot], w_phase, abort_flag);
+          ok &= piece_wait<kHeld>(&bars[G::k_full + k_slot], k_phase, abort_flag);
+          ok &= piece_wait<kHeld>(&bars[G::w_full + w_slot], w_phase, abort_flag);
           if (!ok) break;
           mbar_arrive(&bars[G::k_empty + k_slot]);
           mbar_arrive(&bars[G::w_empty + w_slot]);
@@ -762,7 +769,7 @@ __global__ void __launch_bounds__((Tall8<HD, kHalf>::threads), (Tall8<HD, kHalf>
         for (int t = 0; t < n_steps; ++t, ++count, ++step) {
           const uint32_t b = 2 * rt + (count & 1), use = count >> 1, su = step % G::scale_steps;
           const uint32_t s_tmem = tmem_base + G::s_col + b * kKeys + lane_addr;
-          ok &= piece_wait(&bars[G::s_ready + b], use & 1, abort_flag);
+          ok &= piece_wait<kHeld>(&bars[G::s_ready + b], use & 1, abort_flag);
           if (padding) {   // (the order of the waits is kept, nothing is computed)
             mbar_arrive(&bars[G::p_ready + b]);
             continue;
@@ -822,7 +829,7 @@ __global__ void __launch_bounds__((Tall8<HD, kHalf>::threads), (Tall8<HD, kHalf>
             l *= alpha;
             unit = to_unit;
             if (t > 0) {   // (PV of what P holds already is complete first)
-              ok &= piece_wait(&bars[G::pv_done + (b ^ 1)], ((count - 1) >> 1) & 1, abort_flag);
+              ok &= piece_wait<kHeld>(&bars[G::pv_done + (b ^ 1)], ((count - 1) >> 1) & 1, abort_flag);
               tc::fence_after_sync();
 #pragma unroll 1
               for (int d = 0; d < HD / 16; ++d) {
@@ -848,7 +855,7 @@ __global__ void __launch_bounds__((Tall8<HD, kHalf>::threads), (Tall8<HD, kHalf>
           copied = true;
         }
         // ---- the piece's rows ----
-        ok &= piece_wait(&bars[G::pv_done + 2 * rt + ((count - 1) & 1)], ((count - 1) >> 1) & 1, abort_flag);
+        ok &= piece_wait<kHeld>(&bars[G::pv_done + 2 * rt + ((count - 1) & 1)], ((count - 1) >> 1) & 1, abort_flag);
         tc::fence_after_sync();
         if (not_finite && max(row_lo, it.key0) < min(row_hi, it.key0 + it.tiles * kTile)) l = NAN;   // (a row that sees no key is zero)
         const bool whole = it.begins && it.ends, live = row < it.rows;
@@ -981,7 +988,7 @@ __global__ void __launch_bounds__((Tall8<HD, kHalf>::threads), (Tall8<HD, kHalf>
   if (warp == G::mma_warp) tc::tmem_dealloc(tmem_base, G::tmem);
 }
 
-template <int HD, bool kHalf>
+template <int HD, bool kHalf, bool kHeld = false>
 cudaError_t launch_one(const Kv8Params& p, const CUtensorMap& k_map, const CUtensorMap& v_map, cudaStream_t stream) {
   using G = Tall8<HD, kHalf>;
   static bool configured[64] = {};
@@ -990,9 +997,9 @@ cudaError_t launch_one(const Kv8Params& p, const CUtensorMap& k_map, const CUten
   if (err != cudaSuccess) return err;
   if (dev < 0 || dev >= 64 || !configured[dev]) {
     cudaFuncAttributes attr;
-    err = cudaFuncGetAttributes(&attr, kv8_tall_kernel<HD, kHalf>);
+    err = cudaFuncGetAttributes(&attr, kv8_tall_kernel<HD, kHalf, kHeld>);
     if (err == cudaSuccess && attr.numRegs < G::start_regs) err = cudaErrorInvalidConfiguration;   // (setmaxnreg would wait without end)
-    if (err == cudaSuccess) err = cudaFuncSetAttribute(kv8_tall_kernel<HD, kHalf>, cudaFuncAttributeMaxDynamicSharedMemorySize, G::total);
+    if (err == cudaSuccess) err = cudaFuncSetAttribute(kv8_tall_kernel<HD, kHalf, kHeld>, cudaFuncAttributeMaxDynamicSharedMemorySize, G::total);
     if (err != cudaSuccess) return err;
     if (dev >= 0 && dev < 64) configured[dev] = true;
   }
@@ -1001,7 +1008,7 @@ cudaError_t launch_one(const Kv8Params& p, const CUtensorMap& k_map, const CUten
   if (sms <= 0 || sms * G::ctas * G::rts * 4 > kCounterBytes) return cudaErrorInvalidDevice;
   Kv8Params q = p;
   q.out_wide = reinterpret_cast<uintptr_t>(p.out) % 32 == 0 && p.out_stride_token % 32 == 0 && p.out_stride_head % 32 == 0;
-  return pdl_launch(kv8_tall_kernel<HD, kHalf>, dim3((unsigned)(sms * G::ctas)), dim3(G::threads), G::total, stream, q, k_map, v_map);
+  return pdl_launch(kv8_tall_kernel<HD, kHalf, kHeld>, dim3((unsigned)(sms * G::ctas)), dim3(G::threads), G::total, stream, q, k_map, v_map);
 }
 template <int HD>
 cudaError_t launch_type(const Kv8Params& p, const CUtensorMap& k_map, const CUtensorMap& v_map, cudaStream_t stream) {
@@ -1016,6 +1023,11 @@ int64_t kv8_tall_workspace_bytes(int head_size, int num_sms) {
   return kCounterBytes + (int64_t)num_sms * 2 * rows * (head_size + 2) * 4;
 }
 
+cudaError_t launch_kv8_tall_held(const Kv8Params& p, cudaStream_t stream) {
+  CUtensorMap k_map{}, v_map{};
+  if (!cell_box_map(p, p.k, 16, &k_map) || !cell_box_map(p, p.v, 16, &v_map)) return cudaErrorInvalidValue;
+  return launch_one<128, false, true>(p, k_map, v_map, stream);
+}
 cudaError_t launch_kv8_tall(const Kv8Params& p, cudaStream_t stream, bool* taken) {
   CUtensorMap k_map{}, v_map{};
   *taken = cell_box_map(p, p.k, 16, &k_map) && cell_box_map(p, p.v, 16, &v_map);
