@@ -25,9 +25,9 @@
 // come by 16-byte copies, zero where a key is not visible, so what lies there in memory, NaN included, is never read.
 // Scales come with them, one per 16 keys.  The warp that works out the pieces makes the digits of their queries.
 //
-// Measured (32 heads of 8, 128 dims, bf16, calls behind one another): one token of 64 requests x 8,192 keys, 1.08 GB, 172 us, 0.96 of the
-// copy bandwidth; four tokens of 32 requests of 2,000 to 16,384 keys, 0.65 GB, 125 us, 0.80: 16 rows' softmax, two groups of warps
-// with a barrier for each tile's vote, takes as long as their bytes.  12 heads of 2, 256 dims, 0.53 GB: 90 us, 0.90.  Eight requests of up to 4,095 keys
+// Measured (32 heads of 8, 128 dims, bf16, calls behind one another): one token of 64 requests x 8,192 keys, 1.08 GB, 169 to 175 us, 0.94 to 0.97 of the
+// copy bandwidth; four tokens of 32 requests of 2,000 to 16,384 keys, 0.65 GB, 127 us with part of the cells in L2, 136 among other work, 0.73: 16 rows'
+// softmax, two groups of warps with a barrier for each tile's vote, takes longer than their bytes.  12 heads of 2, 256 dims, 0.53 GB: 90 us, 0.90.  Eight requests of up to 4,095 keys
 // 19 us, of which 10 are one tile's way through launch, look-ups, queries, products and rows, and 2 to 5 the merge.
 //
 // Schedule and merge: kv16_short.cuh.

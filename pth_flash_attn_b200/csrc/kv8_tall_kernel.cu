@@ -14,7 +14,8 @@
 // fp16: U is the largest scale that the row has seen so far in the piece (O is rescaled where a step brings a larger one), so weights are at most
 // P, and keys that a row does not see change nothing for it, whatever their scale.  (With c_V scale_V / U as operand B and a U for all rows, a scale that is
 // no power of two was rounded to 11 bits itself, the same way for all its keys, and a scale 2^25 times the others', under keys that a row did not see,
-// left nothing of those that it did.)  So Y needs no digits: one 16-bit number, with 32-bit sums.
+// left nothing of those that it did.)  So Y needs no digits: one 16-bit number, with 32-bit sums; its rounding by 2^-11 is an eighth of that
+// of a bf16 result (fp16 results are off by 2.6e-4 of their norm, by 2.0e-4 with weights of 32 bits).
 //
 // Softmax in one pass: ref is a running bound of a row's scores (log2 units), P = 2^(s - ref), l = sum P, ref kGain below the maximum of
 // a row's first 64 keys.  Later ones need no maximum: the sum of 64 P says whether one of them has outgrown ref too far
@@ -26,9 +27,9 @@
 //
 // What bounds it.  A step's softmax, 1,300 to 1,500 clocks of 64 exponentials and their conversions a row, beside 300 to 500 of waiting for S; power
 // (the 1,000 W limit) in long calls; a piece's own 8,000 to 10,000 clocks (queries, first S, rows, merge) in short ones.  Measured (bf16 unless
-// said, calls behind one another): four chunks of 2,048 tokens over 8,192 keys before them, 32 heads of 8, 128 dims: 1,150 to 1,245 us, 0.60 to
-// 0.65 of the bf16 rate of a library product (fp16 1,370; 16 heads of 16, 64 dims, 553).  Twelve prompts of 37 to 2,500 tokens: 16 heads of 16, 64 dims, fp16, 166 us; 32 heads of 8, 128 dims,
-// 316 us.  256 dims, the same chunks: 3,400 us, one row tile per SM.
+// said, calls behind one another): four chunks of 2,048 tokens over 8,192 keys before them, 32 heads of 8, 128 dims: 1,100 to 1,240 us (1,285 among other
+// work), 0.58 to 0.68 of the bf16 rate of a library product (fp16 1,380; 16 heads of 16, 64 dims, 590 to 650).  Twelve prompts of 37 to 2,500 tokens: 16 heads of 16, 64 dims,
+// fp16, 164 us; 32 heads of 8, 128 dims, 316 to 336 us.  256 dims, the same chunks: 3,210 to 3,300 us, one row tile per SM.
 //
 // Schedule: the rows of a request and KV head in row tiles, a first one together with a last one, so that under a causal mask
 // these units are about equally long; all units form one sequence in KV tiles of 128 keys, which is cut into equal runs, one per
@@ -126,7 +127,8 @@ __device__ __forceinline__ RowTile8 row_tile8(const Kv8Params& p, const ReqShape
   return t;
 }
 // Lengths in the sequence, in KV tiles: of a first and a last row tile together, of the one in the middle of an odd number, and of
-// all of a KV head.  (A pair may be some tiles longer or shorter than those this goes by: a row tile's last piece takes what is left.)
+// all of a KV head.  (Pairs may be longer or shorter than those this goes by: a row tile's last piece takes what is left.  Under a causal mask by some tiles; under a
+// window by up to its own length: the longest run of 8,192 fresh tokens with a window of 4,096 is 1.36 of the mean one.)
 struct Units8 {
   int pairs, pair, middle;
   long long head;
