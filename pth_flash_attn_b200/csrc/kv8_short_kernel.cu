@@ -113,7 +113,7 @@ struct Geo8 {
   static constexpr int pieces = scales + kScaleTiles * 64;   // PieceQueue's entries
   static constexpr int bars = pieces + kQueue * 64;
   static constexpr int n_bars = 2 * units + 2 + 2 + 2 + 2 * 2 + 2 * kQueue + 1;
-  static constexpr int misc = bars + n_bars * 8;     // ints: abort flag, TMEM address, arrival, stop; scratch of find_run; nan_item
+  static constexpr int misc = bars + n_bars * 8;     // ints: abort flag, TMEM address, arrival, stop; scratch of find_run, then NanNotes
   static constexpr int total = misc + 176 + 1024;
   static_assert(kQueue * 64 + n_bars * 8 + 160 <= 1024, "fixed part");
 };
@@ -318,46 +318,84 @@ __device__ __forceinline__ float log2_approx(float x) {
   return y;
 }
 
-// Rows of several tokens: keys that some of them see and others do not, [.., lo) and [hi, ..).
+// Rows of several tokens: keys that some of them see and others do not, [.., lo) and [hi, ..); keys that any of them sees, [first, last).
 struct Masks {
-  int lo, hi;
-  __device__ __forceinline__ Masks(const Kv8Params& p, const Piece& it) : lo(0), hi(INT_MAX) {
+  int lo, hi, first, last;
+  __device__ __forceinline__ Masks(const Kv8Params& p, const Piece& it) : lo(0), hi(INT_MAX), first(0), last(INT_MAX) {
     if (p.query_start_loc == nullptr) return;
-    if (p.causal) hi = it.pos0 + it.row0 / p.group + 1;
-    lo = kv8_low(p, it.pos0 + (it.row0 + it.rows - 1) / p.group);
+    const int top = it.pos0 + it.row0 / p.group, bottom = it.pos0 + (it.row0 + it.rows - 1) / p.group;   // positions of the first and last row
+    if (p.causal) {
+      hi = top + 1;
+      last = bottom + 1;
+    }
+    lo = kv8_low(p, bottom);
+    first = kv8_low(p, top);
   }
   __device__ __forceinline__ bool divide(int key0) const { return key0 < lo || key0 + kTile > hi; }
+  __device__ __forceinline__ bool see(int key0) const { return key0 < last && key0 + kTile > first; }
 };
 // A value that is NaN under a hidden key: its weight is zero, but zero times NaN is NaN.  So where the rows of a piece do not all see a
-// tile's keys, NaN among its values becomes zero in front of the MMA, and what the rows see of it is put in at the piece's end.  Both
-// are rare, so slow.
-template <int kDims>
-__device__ __forceinline__ bool clear_nan(uint8_t* unit) {   // one warp; whether there was any
-  uint32_t any = 0;
-#pragma unroll 1
-  for (int i = threadIdx.x & 31; i < kTile * kDims / 16; i += 32) {
-    uint4 v = reinterpret_cast<const uint4*>(unit)[i];
-    const uint32_t nan = take_nan(v.x) | take_nan(v.y) | take_nan(v.z) | take_nan(v.w);
-    if (nan != 0) reinterpret_cast<uint4*>(unit)[i] = v;
-    any |= nan;
+// tile's keys, NaN among its values becomes zero in front of the MMA, and where some of them do, its keys are noted: what the rows see of them is put in at the
+// piece's end.  The rows are of 32 tokens at most, so such tiles are four at most: key0 is in 158 places about the windows' edges, and in as many about
+// the rows' own keys.
+constexpr int kNanTiles = 4;
+struct NanNotes {
+  uint32_t item;           // 1 + the item that they are of
+  uint32_t any;
+  int tiles, key0[kNanTiles];
+  uint32_t keys[kNanTiles][4];
+};
+static_assert(sizeof(NanNotes) <= 144, "find_run's scratch");
+__device__ __forceinline__ void note_tile(NanNotes* notes, uint32_t item, int key0) {   // one thread
+  if (notes->item != item) {
+    notes->item = item;
+    notes->any = 0;
+    notes->tiles = 0;
   }
-  return __any_sync(0xffffffffu, any != 0);
+  const int i = min(notes->tiles, kNanTiles - 1);
+  notes->key0[i] = key0;
+  for (int w = 0; w < 4; ++w) notes->keys[i][w] = 0;
+  notes->tiles = i + 1;
 }
-// The rows, of `rows` from row0 of the piece on, that see a key whose value is NaN at dimension d, of the tiles that were cleared.
-__device__ __forceinline__ uint32_t nan_rows(const Kv8Params& p, const Piece& it, int row0, int rows, int d) {
-  const Masks masks(p, it);
+template <int kDims>
+__device__ __forceinline__ void clear_nan(uint8_t* unit, NanNotes* notes) {   // one warp; notes: of the tile noted last, nullptr: none are taken
+  uint4* const cells = reinterpret_cast<uint4*>(unit);
+#pragma unroll 1
+  for (int i0 = threadIdx.x & 31; i0 < kTile * kDims / 16; i0 += 128) {
+    uint32_t nan = 0;
+#pragma unroll
+    for (int i = i0; i < i0 + 128; i += 32) nan |= nan_cells(cells[i].x) | nan_cells(cells[i].y) | nan_cells(cells[i].z) | nan_cells(cells[i].w);
+    if (nan == 0) continue;
+#pragma unroll 1
+    for (int i = i0; i < i0 + 128; i += 32) {
+      uint4 v = cells[i];
+      if ((take_nan(v.x) | take_nan(v.y) | take_nan(v.z) | take_nan(v.w)) == 0) continue;
+      cells[i] = v;
+      if (notes == nullptr) continue;
+      const int key = i / (kDims / 16);
+      atomicOr(&notes->keys[notes->tiles - 1][key >> 5], 1u << (key & 31));
+      notes->any = 1;
+    }
+  }
+}
+// The rows, of `rows` from row0 of the piece on, that see a key whose value is NaN at dimension d.
+__device__ __forceinline__ uint32_t nan_rows(const Kv8Params& p, const Piece& it, const NanNotes* notes, int row0, int rows, int d) {
   uint32_t seen = 0;
 #pragma unroll 1
-  for (int pos = max(it.lo, it.key0); pos < it.hi; ++pos) {
-    if (!masks.divide(it.key0 + (pos - it.key0) / kTile * kTile)) continue;
-    int slot;
-    const int blk = block_of(p, it.r, pos, &slot);
-    if (blk < 0) continue;
-    const uint8_t c = p.v[(int64_t)blk * p.stride_block + (int64_t)slot * p.stride_slot + (int64_t)it.kvh * p.stride_head + d];
-    if ((c & 0x7f) != 0x7f) continue;
-    for (int n = 0; n < rows; ++n) {
-      const int own = it.pos0 + (it.row0 + row0 + n) / p.group;
-      if ((!p.causal || pos <= own) && pos >= kv8_low(p, own)) seen |= 1u << n;
+  for (int i = 0; i < 4 * notes->tiles; ++i) {
+#pragma unroll 1
+    for (uint32_t keys = notes->keys[i >> 2][i & 3]; keys != 0; keys &= keys - 1) {
+      const int pos = notes->key0[i >> 2] + (i & 3) * 32 + __ffs(keys) - 1;
+      if (pos < it.lo || pos >= it.hi) continue;
+      int slot;
+      const int blk = block_of(p, it.r, pos, &slot);
+      if (blk < 0) continue;
+      const uint8_t c = p.v[(int64_t)blk * p.stride_block + (int64_t)slot * p.stride_slot + (int64_t)it.kvh * p.stride_head + d];
+      if ((c & 0x7f) != 0x7f) continue;
+      for (int n = 0; n < rows; ++n) {
+        const int own = it.pos0 + (it.row0 + row0 + n) / p.group;
+        if ((!p.causal || pos <= own) && pos >= kv8_low(p, own)) seen |= 1u << n;
+      }
     }
   }
   return seen;
@@ -375,7 +413,7 @@ __global__ void __launch_bounds__((Geo8<HD, RP, kHalf>::threads), (Geo8<HD, RP, 
   uint32_t* const tslot = reinterpret_cast<uint32_t*>(smem + G::misc + 4);
   int* const arrival = reinterpret_cast<int*>(smem + G::misc + 8);
   int* const stop = arrival + 1;
-  volatile uint32_t* const nan_item = reinterpret_cast<volatile uint32_t*>(smem + G::misc + 160);   // 1 + the last item whose values had NaN taken out
+  NanNotes* const notes = reinterpret_cast<NanNotes*>(smem + G::misc + 16);   // (where find_run's scratch was)
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
 
   if (warp == G::load_warp && lane < 2 && p.box_slots > 0)
@@ -398,7 +436,6 @@ __global__ void __launch_bounds__((Geo8<HD, RP, kHalf>::threads), (Geo8<HD, RP, 
       tc::mbar_init(&bars[Bars8::drained], 1);
       PieceQueue(nullptr, &bars[Bars8::queue], stop).init(4 * G::groups + G::load_warps + 1);
       *abort_flag = 0;
-      *nan_item = 0;
       tc::mbar_init_fence();
     }
     __syncwarp();
@@ -411,6 +448,7 @@ __global__ void __launch_bounds__((Geo8<HD, RP, kHalf>::threads), (Geo8<HD, RP, 
   __syncthreads();
   tc::fence_after_sync();
   const uint32_t tmem_base = *tslot;
+  if (warp == G::mma_warp && lane == 0) notes->item = 0;   // (read behind PV's barriers)
   PieceQueue queue(reinterpret_cast<Piece*>(smem + G::pieces), &bars[Bars8::queue], stop);
   float* const qfactor = reinterpret_cast<float*>(smem + G::qfactor);
   bool ok = true;
@@ -588,13 +626,15 @@ __global__ void __launch_bounds__((Geo8<HD, RP, kHalf>::threads), (Geo8<HD, RP, 
       if (last_of_item) ++item;
     };
     uint32_t pv_tile = 0;
-    auto pv = [&](bool first_of_item, bool divided, uint32_t its_item) {
+    auto pv = [&](bool first_of_item, bool divided, bool seen, uint32_t its_item, int key0) {
       ok &= kv16_wait(&bars[Bars8::p_ready + pv_tile % G::p_images], (pv_tile / G::p_images) & 1, abort_flag);
 #pragma unroll
       for (int part = 0; part < G::parts; ++part) {
         const uint32_t s = arrived();
-        if (divided && clear_nan<G::dims>(smem + s * G::unit)) {
-          if (lane == 0) *nan_item = its_item + 1;
+        if (divided) {
+          if (part == 0 && lane == 0 && seen) note_tile(notes, its_item + 1, key0);
+          __syncwarp();
+          clear_nan<G::dims>(smem + s * G::unit, seen ? notes : nullptr);
           tc::fence_async_smem();
           __syncwarp();
         }
@@ -615,22 +655,25 @@ __global__ void __launch_bounds__((Geo8<HD, RP, kHalf>::threads), (Geo8<HD, RP, 
       ++pv_tile;
     };
     Piece it;
-    bool pending = false, pending_first = false, pending_divided = false;
+    bool pending = false, pending_first = false, pending_divided = false, pending_seen = false;
     uint32_t pending_item = 0;
+    int pending_key0 = 0;
     while (queue.get(&it, abort_flag)) {
       const Masks masks(p, it);
       for (int t = 0; t < it.tiles; ++t) {
         if (kv16_held<kHeld>(p, kHeldMma, tile)) break;
         const uint32_t here = item;
         qk(t == 0, t == it.tiles - 1);
-        if (pending) pv(pending_first, pending_divided, pending_item);
+        if (pending) pv(pending_first, pending_divided, pending_seen, pending_item, pending_key0);
         pending = true;
         pending_first = t == 0;
-        pending_divided = masks.divide(it.key0 + t * kTile);
+        pending_key0 = it.key0 + t * kTile;
+        pending_divided = masks.divide(pending_key0);
+        pending_seen = masks.see(pending_key0);
         pending_item = here;
       }
     }
-    if (pending) pv(pending_first, pending_divided, pending_item);
+    if (pending) pv(pending_first, pending_divided, pending_seen, pending_item, pending_key0);
   } else if (warp < G::load_warp) {
     // =========================== softmax =========================================
     if constexpr (G::moves) asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(G::softmax_regs));
@@ -785,7 +828,7 @@ __global__ void __launch_bounds__((Geo8<HD, RP, kHalf>::threads), (Geo8<HD, RP, 
         const bool whole = it.begins && it.ends;
         float* const slot = partial_slot<HD, RP>(p, (int)blockIdx.x, it.begins);
         const float unit_value = power_of_two(unit_e);
-        const bool had_nan = *nan_item == item;   // (the item has been counted already)
+        const bool had_nan = notes->item == item && notes->any != 0;   // (the item has been counted already)
 #pragma unroll
         for (int part = 0; part < G::parts; ++part) {
           uint32_t o[kDigitsY][RW];
@@ -797,7 +840,7 @@ __global__ void __launch_bounds__((Geo8<HD, RP, kHalf>::threads), (Geo8<HD, RP, 
           const int d = part * 128 + key;
           if (d < HD) {
             if (had_nan) {
-              const uint32_t nan = nan_rows(p, it, row_base, min(rows, RW), d);
+              const uint32_t nan = nan_rows(p, it, notes, row_base, min(rows, RW), d);
 #pragma unroll
               for (int n = 0; n < RW; ++n) o[0][n] = nan >> n & 1 ? 0x7fffffffu : o[0][n];
             }

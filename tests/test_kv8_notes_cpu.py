@@ -30,3 +30,19 @@ def test_steps_that_are_not_whole(seed):
             key = key0 + step * STEP
             for pos in range(first, last + 1):
                 assert key >= s.low(pos) and (not causal or key + STEP <= pos + 1)
+
+
+@pytest.mark.parametrize("seed", range(50))
+def test_tiles_of_few_rows_that_are_not_whole(seed):
+    """The kernel of few rows (``kv8_short_kernel.cu``: Masks): tiles that some of a piece's rows see and some do not see whole, four at most."""
+    rng = random.Random(seed)
+    for _ in range(200):
+        tokens, top = rng.randint(1, 32), rng.choice((-20, 0, 5, rng.randint(0, 3000)))
+        window, causal = rng.choice((0, 1, 31, 100, 128, 1000)), rng.random() < 0.8
+        low = lambda pos: max(0, max(pos, -1) - window + 1) if window else 0
+        bottom = top + tokens - 1
+        lo, first = low(bottom), low(top)
+        hi, last = (top + 1, bottom + 1) if causal else (1 << 31, 1 << 31)
+        key0 = rng.randrange(0, 2000, 32)   # of the piece: a grain of 32 keys
+        tiles = [k for k in range(key0, 5000, TILE) if (k < lo or k + TILE > hi) and k < last and k + TILE > first]
+        assert len(tiles) <= 4
