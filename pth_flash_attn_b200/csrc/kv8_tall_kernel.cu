@@ -496,6 +496,7 @@ __global__ void __launch_bounds__((Tall8<HD, kHalf>::threads), (Tall8<HD, kHalf>
       it.edges = edges8(p, it);
       if (kv16_held<kHeld>(p, kHeldSchedule, queue.i)) piece_wait<kHeld>(&bars[G::drained], 0, abort_flag);   // (that nothing arrives on here)
       if (lane < G::nan_words) reinterpret_cast<uint32_t*>(smem + G::nan)[queue.i % G::nan_pieces * G::nan_words + lane] = 0u;
+      __syncwarp();   // (ahead of the entry that one lane makes known)
       going = queue.put(it, abort_flag);
       if (!going) break;
       const int n = steps8(it);
